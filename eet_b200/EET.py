@@ -163,6 +163,9 @@ _STATUS_TEXT = {
     4: "tensor-parallel exchange: a peer's partial sums never arrived",
     5: "decode attention: the step ran past the end of the KV cache",
 }
+_STATUS_TEXT_PAGED = {   # of eet_b200.paged
+    6: "paged cache: a page number outside the cache, or a position behind the end of its row of the page table",
+}
 
 
 def check_device_status(tp=None):
@@ -179,7 +182,8 @@ def check_device_status(tp=None):
     _pool.rezero()
     if tp is not None and getattr(tp, "_peer", None) is not None:
         tp._peer.clear_local()
-    raise EETError(f"device status {status}: {_STATUS_TEXT.get(status, 'unknown code')}; scratch buffers were re-zeroed")
+    text = _STATUS_TEXT.get(status) or _STATUS_TEXT_PAGED.get(status, "unknown code")
+    raise EETError(f"device status {status}: {text}; scratch buffers were re-zeroed")
 
 
 # ---------------------------------------------------------------------------------------------------

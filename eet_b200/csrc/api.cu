@@ -4,6 +4,7 @@
 #include "../../include/eet_b200.h"
 
 #include <cstring>
+#include <initializer_list>
 #include <string>
 
 #include "common.cuh"
@@ -54,6 +55,7 @@ static inline bool aligned16(const void* p)
 #include "attention_tc.cu"
 #include "glue.cu"
 #include "noalloc.cu"
+#include "paged.cu"
 #include "quantize.cu"
 
 using namespace eet;
@@ -582,6 +584,150 @@ int eet_gather_rows(const void* table, const int64_t* ids, void* out, int rows, 
     EET_CHECK(rows >= 0 && n > 0 && rows_in_table > 0 && (rows == 0 || (table && ids && out)), "eet_gather_rows: bad arguments");
     EET_CHECK(aligned16(table) && aligned16(out), "eet_gather_rows: pointers must be 16-byte aligned");
     return launch_gather_rows((const __half*)table, ids, (__half*)out, rows, n, rows_in_table, (cudaStream_t)stream);
+}
+
+// ---- serving from a paged cache -----------------------------------------------------------------------------------------
+
+static bool multiples_of_8(std::initializer_list<int64_t> strides)
+{
+    for (int64_t s : strides) {
+        if (s % 8 != 0) return false;
+    }
+    return true;
+}
+
+static bool all_aligned16(std::initializer_list<const void*> pointers)
+{
+    for (const void* p : pointers) {
+        if (!aligned16(p)) return false;
+    }
+    return true;
+}
+
+// Sizes and the table of a call on a paged cache.
+static int check_paged(const char* who, int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                       int64_t num_pages, int64_t page_size, int64_t max_pages, int64_t pages_stride)
+{
+    EET_CHECK(tokens >= 0 && tokens <= INT32_MAX && seqs >= 0 && seqs <= INT32_MAX, "%s: bad number of tokens or sequences", who);
+    EET_CHECK(heads >= 0 && kv_heads > 0 && heads <= 65535 && kv_heads <= 65535, "%s: bad number of heads", who);
+    EET_CHECK(head_dim == 64 || head_dim == 128, "%s: head size %lld, only 64 and 128 are supported", who, (long long)head_dim);
+    EET_CHECK(page_size >= 16 && page_size <= 256 && (page_size & (page_size - 1)) == 0,
+              "%s: page size %lld, only 16, 32, 64, 128 and 256 are supported", who, (long long)page_size);
+    EET_CHECK(num_pages >= 0 && num_pages <= INT32_MAX, "%s: bad number of pages", who);
+    EET_CHECK(max_pages >= 0 && max_pages <= INT32_MAX / page_size, "%s: sequences are limited to 2^31 - 1 positions", who);
+    EET_CHECK(pages_stride >= max_pages || seqs <= 1, "%s: rows of the page table overlap", who);
+    return 0;
+}
+
+static int page_shift(int64_t page_size)
+{
+    int s = 0;
+    while (((int64_t)1 << s) < page_size) ++s;
+    return s;
+}
+
+int eet_rotary(const eet_rotary_args* p, void* stream)
+{
+    EET_CHECK(p != nullptr, "eet_rotary: args is NULL");
+    EET_CHECK(p->tokens >= 0 && p->tokens <= INT32_MAX, "eet_rotary: bad number of tokens");
+    EET_CHECK(p->heads >= 0 && p->kv_heads >= 0 && p->heads <= 65535 && p->kv_heads <= 65535, "eet_rotary: bad number of heads");
+    EET_CHECK(p->head_dim > 0 && p->head_dim <= 256 && p->head_dim % 16 == 0, "eet_rotary: head size %lld must be a multiple of 16 up to 256",
+              (long long)p->head_dim);
+    EET_CHECK(p->rotary_dim > 0 && p->rotary_dim <= p->head_dim && p->rotary_dim % 16 == 0,
+              "eet_rotary: rotary_dim %lld must be a multiple of 16 within the head size", (long long)p->rotary_dim);
+    if (p->tokens == 0 || p->heads + p->kv_heads == 0) return 0;
+    EET_CHECK(p->positions && p->freqs && (p->heads == 0 || (p->q && p->q_out)) && (p->kv_heads == 0 || (p->k && p->k_out)),
+              "eet_rotary: NULL argument");
+    EET_CHECK(all_aligned16({p->q, p->k, p->q_out, p->k_out}), "eet_rotary: pointers must be 16-byte aligned");
+    EET_CHECK(multiples_of_8({p->q_tok, p->q_head, p->k_tok, p->k_head, p->qo_tok, p->qo_head, p->ko_tok, p->ko_head}),
+              "eet_rotary: strides must be multiples of 8 elements");
+    RotaryArgs a = {};
+    a.q = p->q, a.k = p->k, a.q_out = p->q_out, a.k_out = p->k_out;
+    a.positions = p->positions, a.freqs = p->freqs;
+    a.tokens = (int)p->tokens, a.heads = (int)p->heads, a.kv_heads = (int)p->kv_heads, a.head_dim = (int)p->head_dim;
+    a.rotary_dim = (int)p->rotary_dim, a.interleaved = p->interleaved != 0, a.bf16 = p->bf16 != 0;
+    a.q_tok = p->q_tok, a.q_head = p->q_head, a.k_tok = p->k_tok, a.k_head = p->k_head;
+    a.qo_tok = p->qo_tok, a.qo_head = p->qo_head, a.ko_tok = p->ko_tok, a.ko_head = p->ko_head;
+    a.magnitude = (float)p->magnitude;
+    return launch_rotary(a, false, (cudaStream_t)stream);
+}
+
+int eet_paged_store(const eet_paged_store_args* p, void* stream)
+{
+    EET_CHECK(p != nullptr, "eet_paged_store: args is NULL");
+    if (int rc = check_paged("eet_paged_store", p->tokens, p->seqs, p->heads, p->kv_heads, p->head_dim, p->num_pages, p->page_size,
+                             p->max_pages, p->pages_stride)) return rc;
+    EET_CHECK(p->rotary_dim >= 0 && p->rotary_dim <= p->head_dim && p->rotary_dim % 16 == 0,
+              "eet_paged_store: rotary_dim %lld must be a multiple of 16 within the head size", (long long)p->rotary_dim);
+    if (p->tokens == 0 || p->seqs == 0) return 0;
+    EET_CHECK(p->k && p->v && p->k_cache && p->v_cache && p->pages && p->starts && p->lens && (p->heads == 0 || (p->q && p->q_out)) &&
+                  (p->rotary_dim == 0 || p->freqs),
+              "eet_paged_store: NULL argument");
+    EET_CHECK(all_aligned16({p->q, p->k, p->v, p->q_out, p->k_cache, p->v_cache}), "eet_paged_store: pointers must be 16-byte aligned");
+    EET_CHECK(multiples_of_8({p->q_tok, p->q_head, p->k_tok, p->k_head, p->v_tok, p->v_head, p->qo_tok, p->qo_head, p->kc_page, p->kc_head,
+                              p->kc_slot, p->vc_page, p->vc_head, p->vc_slot}),
+              "eet_paged_store: strides must be multiples of 8 elements");
+    RotaryArgs a = {};
+    a.q = p->q, a.k = p->k, a.v = p->v, a.q_out = p->q_out, a.k_cache = p->k_cache, a.v_cache = p->v_cache;
+    a.pages = p->pages, a.starts = p->starts, a.lens = p->lens, a.positions = p->positions, a.freqs = p->freqs;
+    a.tokens = (int)p->tokens, a.seqs = (int)p->seqs, a.heads = (int)p->heads, a.kv_heads = (int)p->kv_heads;
+    a.head_dim = (int)p->head_dim, a.rotary_dim = (int)p->rotary_dim, a.interleaved = p->interleaved != 0, a.bf16 = p->bf16 != 0;
+    a.num_pages = (int)p->num_pages, a.page_shift = page_shift(p->page_size), a.max_pages = (int)p->max_pages;
+    a.pages_stride = p->pages_stride;
+    a.q_tok = p->q_tok, a.q_head = p->q_head, a.k_tok = p->k_tok, a.k_head = p->k_head, a.v_tok = p->v_tok, a.v_head = p->v_head;
+    a.qo_tok = p->qo_tok, a.qo_head = p->qo_head;
+    a.kc_page = p->kc_page, a.kc_head = p->kc_head, a.kc_slot = p->kc_slot;
+    a.vc_page = p->vc_page, a.vc_head = p->vc_head, a.vc_slot = p->vc_slot;
+    a.magnitude = (float)p->magnitude;
+    return launch_rotary(a, true, (cudaStream_t)stream);
+}
+
+static int paged_mha_args(const eet_paged_mha_args* p, PagedMhaArgs& a)
+{
+    EET_CHECK(p != nullptr, "eet_paged_mha: args is NULL");
+    if (int rc = check_paged("eet_paged_mha", p->tokens, p->seqs, p->heads, p->kv_heads, p->head_dim, p->num_pages, p->page_size,
+                             p->max_pages, p->pages_stride)) return rc;
+    EET_CHECK(p->heads > 0 && p->heads % p->kv_heads == 0 && p->heads / p->kv_heads <= 128,
+              "eet_paged_mha: %lld heads must be 1 to 128 times the %lld kv heads", (long long)p->heads, (long long)p->kv_heads);
+    EET_CHECK(p->window >= 0, "eet_paged_mha: window must not be negative");
+    EET_CHECK(multiples_of_8({p->q_tok, p->q_head, p->o_tok, p->o_head, p->kc_page, p->kc_head, p->kc_slot, p->vc_page, p->vc_head, p->vc_slot}),
+              "eet_paged_mha: strides must be multiples of 8 elements");
+    a.q = p->q, a.k_cache = p->k_cache, a.v_cache = p->v_cache, a.out = p->out;
+    a.pages = p->pages, a.starts = p->starts, a.lens = p->lens, a.first_key = p->first_key, a.slopes = p->alibi_slopes;
+    a.tokens = (int)p->tokens, a.seqs = (int)p->seqs, a.heads = (int)p->heads, a.kv_heads = (int)p->kv_heads;
+    a.head_dim = (int)p->head_dim, a.bf16 = p->bf16 != 0;
+    a.num_pages = (int)p->num_pages, a.page_shift = page_shift(p->page_size), a.max_pages = (int)p->max_pages;
+    a.pages_stride = p->pages_stride;
+    a.q_tok = p->q_tok, a.q_head = p->q_head, a.o_tok = p->o_tok, a.o_head = p->o_head;
+    a.kc_page = p->kc_page, a.kc_head = p->kc_head, a.kc_slot = p->kc_slot;
+    a.vc_page = p->vc_page, a.vc_head = p->vc_head, a.vc_slot = p->vc_slot;
+    a.window = p->window;
+    const auto clamp = [](int64_t v, int64_t top) { return (int)(v < 1 || v > top ? top : v); };
+    a.max_tokens = clamp(p->max_tokens, p->tokens);
+    a.max_len = clamp(p->max_len, p->max_pages * p->page_size);
+    a.scale = (float)p->scale;
+    return 0;
+}
+
+size_t eet_paged_mha_workspace_bytes(const eet_paged_mha_args* args)
+{
+    PagedMhaArgs a = {};
+    if (paged_mha_args(args, a) || a.tokens == 0 || a.seqs == 0) return 0;
+    return paged_mha_workspace_bytes(a);
+}
+
+int eet_paged_mha(const eet_paged_mha_args* p, void* stream)
+{
+    PagedMhaArgs a = {};
+    if (int rc = paged_mha_args(p, a)) return rc;
+    if (a.tokens == 0 || a.seqs == 0) return 0;
+    EET_CHECK(p->q && p->k_cache && p->v_cache && p->out && p->pages && p->starts && p->lens, "eet_paged_mha: NULL argument");
+    EET_CHECK(all_aligned16({p->q, p->k_cache, p->v_cache, p->out, p->ws}), "eet_paged_mha: pointers must be 16-byte aligned");
+    a.ws = p->ws;
+    a.ws_bytes = p->ws_bytes > 0 ? (size_t)p->ws_bytes : 0;
+    EET_CHECK(a.ws_bytes >= paged_mha_workspace_bytes(a) && (a.ws != nullptr || paged_mha_workspace_bytes(a) == 0),
+              "eet_paged_mha: workspace too small");
+    return launch_paged_mha(a, (cudaStream_t)stream);
 }
 
 }  // extern "C"

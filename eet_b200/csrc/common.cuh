@@ -2,6 +2,7 @@
 // mbarrier / bulk-copy (TMA engine) wrappers with bounded waits, and the int8 -> fp16 register
 // conversion used by both GEMM kernels.
 #pragma once
+#include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -42,6 +43,7 @@ void set_error(const char* fmt, ...);
 //   3  decode attention: a pipeline wait ran out
 //   4  tensor-parallel exchange: a peer's partial sums never arrived in this rank's inbox
 //   5  decode attention: the device-resident step was outside [1, cache length]; nothing was appended
+//   6  paged cache: a page number outside the cache, or a position behind the end of its sequence's row of the table
 // After a non-zero status the contents of every fp32 scratch buffer the failed kernel used are undefined.
 // (The library is built as one translation unit, so these definitions are seen exactly once.)
 #ifdef __CUDACC__

@@ -146,4 +146,38 @@ bool prefill_mha_tc_supported(int S, int D);
 int launch_prefill_mha_tc(const __half* q, const __half* kcache, const __half* vcache, __half* ctx, int B, int S, int H,
                           int T_max, const int64_t* pad_len, const __half* alibi, int alibi_stride, cudaStream_t stream);
 
+// paged.cu (serving from a paged cache)
+struct RotaryArgs {
+    const void *q, *k, *v;
+    void *q_out, *k_out, *k_cache, *v_cache;     // k_out without, the caches with the append
+    const int *pages, *starts, *lens;
+    const int64_t* positions;
+    const double* freqs;
+    int tokens, seqs, heads, kv_heads, head_dim, rotary_dim, interleaved, bf16;
+    int num_pages, page_shift, max_pages;
+    long long pages_stride;
+    long long q_tok, q_head, k_tok, k_head, v_tok, v_head, qo_tok, qo_head, ko_tok, ko_head;
+    long long kc_page, kc_head, kc_slot, vc_page, vc_head, vc_slot;
+    float magnitude;
+};
+int launch_rotary(const RotaryArgs& a, bool store, cudaStream_t stream);
+struct PagedMhaArgs {
+    const void *q, *k_cache, *v_cache;
+    void* out;
+    const int *pages, *starts, *lens, *first_key;
+    const float* slopes;
+    int tokens, seqs, heads, kv_heads, head_dim, bf16;
+    int num_pages, page_shift, max_pages;
+    long long pages_stride;
+    long long q_tok, q_head, o_tok, o_head;
+    long long kc_page, kc_head, kc_slot, vc_page, vc_head, vc_slot;
+    long long window;
+    int max_tokens, max_len;
+    float scale;
+    void* ws;
+    size_t ws_bytes;
+};
+size_t paged_mha_workspace_bytes(const PagedMhaArgs& a);
+int launch_paged_mha(const PagedMhaArgs& a, cudaStream_t stream);
+
 }  // namespace eet

@@ -1,0 +1,233 @@
+// Rotary positions and the append of new keys and values to a paged cache.
+//
+// One CTA takes a token (or, when the tokens are few, a share of its heads).  The angles of a token are the same for all of its
+// heads: they are computed once, into shared memory.  An angle is position * freqs[i] in 64 bits, reduced to a part of one turn
+// there and only then rounded to 32 bits: at position 10^6 a 32-bit product would be off by 0.06 radians.  sincospif of the
+// rest is good to 2 ulp.
+//
+// Bound: HBM for prompts, launch latency for decode steps.
+#include "common.cuh"
+#include "kernels.h"
+
+namespace eet {
+
+namespace {
+
+constexpr int kRotThreads = 128;
+constexpr int kRotMaxPairs = 128;   // head sizes up to 256
+
+template<typename T>
+struct Pair2;
+template<>
+struct Pair2<__half> {
+    using type = __half2;
+    static __device__ __forceinline__ float2 up(__half2 v) { return __half22float2(v); }
+    static __device__ __forceinline__ __half2 down(float a, float b) { return __floats2half2_rn(a, b); }
+};
+template<>
+struct Pair2<__nv_bfloat16> {
+    using type = __nv_bfloat162;
+    static __device__ __forceinline__ float2 up(__nv_bfloat162 v) { return __bfloat1622float2(v); }
+    static __device__ __forceinline__ __nv_bfloat162 down(float a, float b) { return __floats2bfloat162_rn(a, b); }
+};
+
+// kStore: the keys go to their pages and the values with them, the position follows from the lengths unless it is given.
+// An item is 16 dims of a head: with the half layout dims 8c .. 8c+7 and the partners half the rotated part further, with the
+// interleaved layout and in the part that is not rotated dims 16c .. 16c+15.
+template<typename T, bool kStore>
+__global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryArgs a)
+{
+    using P2 = Pair2<T>;
+    using V2 = typename P2::type;
+    __shared__ __align__(16) float2 cs[kRotMaxPairs];
+    const int token = blockIdx.x;
+    const int tid = threadIdx.x;
+    const int pairs = a.rotary_dim >> 1;
+    long long pos = 0;
+    T* kdst = nullptr;
+    T* vdst = nullptr;
+    if (kStore) {
+        // the sequence of the token: how many of them end at or before it
+        int seq = 0;
+        for (int i = 0; i < a.seqs; i += kRotThreads) {
+            seq += __syncthreads_count(i + tid < a.seqs && a.starts[i + tid + 1] <= token);
+        }
+        if (seq >= a.seqs || a.starts[seq] > token) return;   // a row that belongs to no sequence
+        pos = (long long)a.lens[seq] - a.starts[seq + 1] + token;
+        if (pos >= 0) {
+            const long long column = pos >> a.page_shift;
+            const int page = column < a.max_pages ? a.pages[seq * a.pages_stride + column] : -1;
+            if (page >= 0 && page < a.num_pages) {
+                const long long slot = pos & ((1 << a.page_shift) - 1);
+                kdst = (T*)a.k_cache + page * a.kc_page + slot * a.kc_slot;
+                vdst = (T*)a.v_cache + page * a.vc_page + slot * a.vc_slot;
+            }
+            else if (tid == 0) {
+                g_device_status = 6;
+            }
+        }
+    }
+    if (a.positions != nullptr) pos = a.positions[token];
+    for (int i = tid; i < pairs; i += kRotThreads) {
+        const double turns = (double)pos * (a.freqs[i] * 0.15915494309189533577);   // 1 / (2 pi)
+        float s, c;
+        sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
+        cs[i] = make_float2(c * a.magnitude, s * a.magnitude);
+    }
+    __syncthreads();
+
+    const int per_row = a.head_dim >> 4;
+    const int rows = a.heads + a.kv_heads + (kStore ? a.kv_heads : 0);
+    const int step = (int)gridDim.y * (kRotThreads / per_row);
+    const int c = tid % per_row;
+    if (tid >= kRotThreads / per_row * per_row) return;
+    const bool turned = c < (a.rotary_dim >> 4);
+    const int d0 = (turned && !a.interleaved) ? 8 * c : 16 * c;
+    const int d1 = (turned && !a.interleaved) ? 8 * c + pairs : 16 * c + 8;
+    for (int row = (int)blockIdx.y * (kRotThreads / per_row) + tid / per_row; row < rows; row += step) {
+        const T* src;
+        T* dst;
+        bool rot = turned;
+        if (row < a.heads) {
+            src = (const T*)a.q + (size_t)token * a.q_tok + (size_t)row * a.q_head;
+            dst = (T*)a.q_out + (size_t)token * a.qo_tok + (size_t)row * a.qo_head;
+        }
+        else if (row < a.heads + a.kv_heads) {
+            const int h = row - a.heads;
+            src = (const T*)a.k + (size_t)token * a.k_tok + (size_t)h * a.k_head;
+            dst = kStore ? kdst : (T*)a.k_out + (size_t)token * a.ko_tok;
+            if (dst != nullptr) dst += (size_t)h * (kStore ? a.kc_head : a.ko_head);
+        }
+        else {
+            const int h = row - a.heads - a.kv_heads;
+            src = (const T*)a.v + (size_t)token * a.v_tok + (size_t)h * a.v_head;
+            dst = vdst;
+            if (dst != nullptr) dst += (size_t)h * a.vc_head;
+            rot = false;
+        }
+        if (dst == nullptr) continue;
+        uint4 x = *reinterpret_cast<const uint4*>(src + d0), y = *reinterpret_cast<const uint4*>(src + d1);
+        if (rot) {
+            V2* xh = reinterpret_cast<V2*>(&x);
+            V2* yh = reinterpret_cast<V2*>(&y);
+            if (a.interleaved) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 t0 = cs[8 * c + e], t1 = cs[8 * c + 4 + e];
+                    const float2 u = P2::up(xh[e]), w = P2::up(yh[e]);
+                    xh[e] = P2::down(u.x * t0.x - u.y * t0.y, u.y * t0.x + u.x * t0.y);
+                    yh[e] = P2::down(w.x * t1.x - w.y * t1.y, w.y * t1.x + w.x * t1.y);
+                }
+            }
+            else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 t0 = cs[8 * c + 2 * e], t1 = cs[8 * c + 2 * e + 1];
+                    const float2 u = P2::up(xh[e]), w = P2::up(yh[e]);
+                    xh[e] = P2::down(u.x * t0.x - w.x * t0.y, u.y * t1.x - w.y * t1.y);
+                    yh[e] = P2::down(w.x * t0.x + u.x * t0.y, w.y * t1.x + u.y * t1.y);
+                }
+            }
+        }
+        *reinterpret_cast<uint4*>(dst + d0) = x;
+        *reinterpret_cast<uint4*>(dst + d1) = y;
+    }
+}
+
+// Attention over the pages, one warp a (token, head): a lane holds D / 32 dims of the query and of the sum.
+template<typename T, int D>
+__global__ void __launch_bounds__(128) paged_mha_kernel(const PagedMhaArgs a)
+{
+    constexpr int E = D / 32;
+    const int lane = threadIdx.x & 31;
+    const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (item >= (long long)a.tokens * a.heads) return;
+    const int token = (int)(item / a.heads), head = (int)(item % a.heads);
+    int seq = 0;
+    for (int i = 0; i < a.seqs; i += 32) {
+        seq += __popc(__ballot_sync(0xffffffffu, i + lane < a.seqs && a.starts[i + lane + 1] <= token));
+    }
+    if (seq >= a.seqs || a.starts[seq] > token) return;
+    const long long pos = (long long)a.lens[seq] - a.starts[seq + 1] + token;
+    long long first = a.first_key != nullptr ? a.first_key[seq] : 0;
+    if (first < 0) first = 0;
+    if (a.window > 0 && pos - a.window + 1 > first) first = pos - a.window + 1;
+    const int kvh = head / (a.heads / a.kv_heads);
+    float q[E], acc[E];
+    for (int e = 0; e < E; ++e) {
+        q[e] = (float)((const T*)a.q)[(size_t)token * a.q_tok + (size_t)head * a.q_head + lane + 32 * e];
+        acc[e] = 0.f;
+    }
+    const float slope = a.slopes != nullptr ? a.slopes[head] : 0.f;
+    float m = -INFINITY, l = 0.f;
+    for (long long j = first; j <= pos; ++j) {
+        const long long column = j >> a.page_shift;
+        const int page = column < a.max_pages ? a.pages[seq * a.pages_stride + column] : -1;
+        if (page < 0 || page >= a.num_pages) {
+            if (lane == 0) g_device_status = 6;
+            continue;
+        }
+        const long long slot = j & ((1 << a.page_shift) - 1);
+        const T* kr = (const T*)a.k_cache + page * a.kc_page + kvh * a.kc_head + slot * a.kc_slot;
+        const T* vr = (const T*)a.v_cache + page * a.vc_page + kvh * a.vc_head + slot * a.vc_slot;
+        float s = 0.f;
+        for (int e = 0; e < E; ++e) s += q[e] * (float)kr[lane + 32 * e];
+        s = warp_sum(s) * a.scale + slope * (float)(j - pos);
+        const float m_new = fmaxf(m, s);
+        const float corr = expf(m - m_new), p = expf(s - m_new);
+        l = l * corr + p;
+        for (int e = 0; e < E; ++e) acc[e] = acc[e] * corr + p * (float)vr[lane + 32 * e];
+        m = m_new;
+    }
+    for (int e = 0; e < E; ++e) {
+        ((T*)a.out)[(size_t)token * a.o_tok + (size_t)head * a.o_head + lane + 32 * e] = (T)(l > 0.f ? acc[e] / l : 0.f);
+    }
+}
+
+}  // namespace
+
+template<typename T, bool kStore>
+static int launch_rotary_t(const RotaryArgs& a, cudaStream_t stream)
+{
+    // few tokens: their heads are shared out, so that some 600 CTAs exist
+    const int rows_at_once = kRotThreads / (a.head_dim / 16);
+    const int rows = a.heads + a.kv_heads + (kStore ? a.kv_heads : 0);
+    int shares = (rows + rows_at_once - 1) / rows_at_once;
+    const int wanted = (4 * sm_count() + a.tokens - 1) / a.tokens;
+    if (shares > wanted) shares = wanted;
+    if (shares < 1) shares = 1;
+    rotary_kernel<T, kStore><<<dim3((unsigned)a.tokens, (unsigned)shares), kRotThreads, 0, stream>>>(a);
+    EET_LAUNCH_CHECK();
+    return 0;
+}
+
+int launch_rotary(const RotaryArgs& a, bool store, cudaStream_t stream)
+{
+    if (a.tokens == 0 || (store && a.seqs == 0)) return 0;
+    if (a.bf16) return store ? launch_rotary_t<__nv_bfloat16, true>(a, stream) : launch_rotary_t<__nv_bfloat16, false>(a, stream);
+    return store ? launch_rotary_t<__half, true>(a, stream) : launch_rotary_t<__half, false>(a, stream);
+}
+
+size_t paged_mha_workspace_bytes(const PagedMhaArgs&)
+{
+    return 0;
+}
+
+int launch_paged_mha(const PagedMhaArgs& a, cudaStream_t stream)
+{
+    if (a.tokens == 0 || a.seqs == 0) return 0;
+    const long long blocks = ((long long)a.tokens * a.heads + 3) / 4;
+    EET_CHECK(blocks <= 0x7fffffffLL, "paged attention: %d tokens of %d heads are too many", a.tokens, a.heads);
+    if (a.head_dim == 128) {
+        if (a.bf16) paged_mha_kernel<__nv_bfloat16, 128><<<(unsigned)blocks, 128, 0, stream>>>(a);
+        else paged_mha_kernel<__half, 128><<<(unsigned)blocks, 128, 0, stream>>>(a);
+    }
+    else {
+        if (a.bf16) paged_mha_kernel<__nv_bfloat16, 64><<<(unsigned)blocks, 128, 0, stream>>>(a);
+        else paged_mha_kernel<__half, 64><<<(unsigned)blocks, 128, 0, stream>>>(a);
+    }
+    EET_LAUNCH_CHECK();
+    return 0;
+}
+
+}  // namespace eet

@@ -1,0 +1,258 @@
+"""Serving from a paged cache: rotary positions, the append of new keys and values to pages, and the attention of new tokens -
+one a sequence, or a chunk of a prompt behind its history - over the pages.
+
+A cache is two tensors k_cache, v_cache [pages, kv_heads, page_size, head_dim], fp16 or bf16, allocated by the caller (views
+with other strides will do as long as rows of head_dim are contiguous).  Sequence b holds ``lens[b]`` positions; position p
+of it is slot ``p % page_size`` of page ``pages[b, p // page_size]``.  The new tokens of all sequences are rows behind one
+another: those of sequence b are rows ``starts[b]`` to ``starts[b + 1]``, and they are the last positions of their sequence.
+A step of a model with chunks and single tokens side by side is therefore, in each layer,
+
+    q = paged_store(k, v, k_cache, v_cache, pages, starts, lens, q=q, freqs=freqs)
+    ctx = paged_mha(q, k_cache, v_cache, pages, starts, lens)
+
+with ``pages`` int32 [sequences, columns], ``starts`` int32 [sequences + 1] and ``lens`` int32 [sequences] on the GPU.  They
+are read there, so a captured CUDA graph of these calls serves whatever they hold when it is replayed.  Entries of ``pages``
+behind a sequence's last position are not read.  A page number outside the cache is not followed: the call completes and
+``EET.check_device_status()`` reports it.
+
+The reference serves one contiguous cache an op, all sequences at the same step (csrc/op/llama_mmha.cpp:94-112).
+"""
+import math
+import struct
+
+import torch
+
+from ._lib import check, lib
+from .EET import _on, _ptr, _stream
+
+__all__ = ["rotary_frequencies", "apply_rotary", "paged_store", "paged_mha"]
+
+_DTYPES = (torch.float16, torch.bfloat16)
+_PAGE_SIZES = (16, 32, 64, 128, 256)
+_pack_rotary = struct.Struct("6P15qd").pack
+_pack_store = struct.Struct("11P26qd").pack
+_pack_mha = struct.Struct("9P23qdPq").pack
+
+
+def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, device="cuda:0"):
+    """(freqs, magnitude): radians a position of each pair of a head's rotated part, float64 [rotary_dim / 2], and the factor
+    on the rotated values (1.0 but for "yarn").
+
+    Pair i turns by base ** (-2 i / rotary_dim) a position.  ``scaling`` stretches that for contexts longer than a model was
+    trained on, a dict with "type", "factor" and
+      "linear"  every frequency / factor
+      "ntk"     base * factor ** (rotary_dim / (rotary_dim - 2)) instead of base
+      "bands"   "original" (the trained length L), "low" and "high": pairs that turn more than `high` times in L stay, those that turn
+                less than `low` times are divided by factor, between them a blend that is linear in the number of turns
+      "yarn"    "original", optional "fast" (32) and "slow" (1): the same idea with a blend that is linear in the pair's index,
+                from the index that turns `fast` times in L (rounded down) to the one that turns `slow` times (rounded up), and a
+                magnitude of 0.1 ln(factor) + 1, or "magnitude" (Peng et al., 2023)"""
+    if rotary_dim <= 0 or rotary_dim % 16:
+        raise RuntimeError(f"rotary_frequencies: rotary_dim {rotary_dim} must be a multiple of 16")
+    half, magnitude = rotary_dim // 2, 1.0
+    scaling = dict(scaling) if scaling else {"type": "none", "factor": 1.0}
+    kind, factor = scaling.pop("type"), float(scaling.pop("factor"))
+    if not base > 1.0 or not factor > 0.0:
+        raise RuntimeError("rotary_frequencies: base must be above 1 and factor above 0")
+    if kind == "ntk":
+        base = base * factor ** (rotary_dim / (rotary_dim - 2))
+    freqs = [base ** (-2.0 * i / rotary_dim) for i in range(half)]
+    if kind == "linear":
+        freqs = [f / factor for f in freqs]
+    elif kind == "bands":
+        length, low, high = (float(scaling.pop(k)) for k in ("original", "low", "high"))
+        if not high > low:
+            raise RuntimeError("rotary_frequencies: high must be above low")
+        stay = [min(1.0, max(0.0, (f * length / (2 * math.pi) - low) / (high - low))) for f in freqs]
+        freqs = [s * f + (1.0 - s) * f / factor for s, f in zip(stay, freqs)]
+    elif kind == "yarn":
+        length = float(scaling.pop("original"))
+        fast, slow = float(scaling.pop("fast", 32.0)), float(scaling.pop("slow", 1.0))
+        magnitude = float(scaling.pop("magnitude", 0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0))
+        index = [rotary_dim * math.log(length / (turns * 2 * math.pi)) / (2 * math.log(base)) for turns in (fast, slow)]
+        low, high = max(0, math.floor(index[0])), min(rotary_dim - 1, math.ceil(index[1]))
+        part = [min(1.0, max(0.0, (i - low) / max(high - low, 0.001))) for i in range(half)]
+        freqs = [s * f / factor + (1.0 - s) * f for s, f in zip(part, freqs)]
+    elif kind not in ("none", "ntk"):
+        raise RuntimeError(f"rotary_frequencies: unknown scaling type {kind!r}")
+    if scaling:
+        raise RuntimeError(f"rotary_frequencies: {sorted(scaling)} mean nothing to scaling type {kind!r}")
+    return torch.tensor(freqs, dtype=torch.float64, device=device), magnitude
+
+
+def _heads(who, name, t, like, heads=None, head_dim=None):
+    """The token and head strides of a [tokens, heads, head_dim] tensor that stands beside `like`."""
+    shape = t.shape
+    if len(shape) != 3 or t.dtype != like.dtype or t.device != like.device:
+        raise RuntimeError(f"{who}: {name} must be a CUDA {like.dtype} tensor [tokens, heads, head_dim] on {like.device}, got "
+                           f"{tuple(shape)} {t.dtype} on {t.device}")
+    if shape[0] != like.shape[0] or shape[2] != (head_dim or like.shape[2]) or (heads is not None and shape[1] != heads):
+        raise RuntimeError(f"{who}: {name} has shape {tuple(shape)} beside {tuple(like.shape)}")
+    strides = t.stride()
+    if strides[2] != 1:
+        raise RuntimeError(f"{who}: the last dimension of {name} must be contiguous")
+    return strides[0], strides[1]
+
+
+def _first(who, name, t):
+    if t.dim() != 3 or t.dtype not in _DTYPES or not t.is_cuda:
+        raise RuntimeError(f"{who}: {name} must be a CUDA fp16 or bf16 tensor [tokens, heads, head_dim], got {tuple(t.shape)} {t.dtype} "
+                           f"on {t.device}")
+
+
+def _index(who, name, t, dtype, numel, device):
+    if t.dtype != dtype or t.device != device or t.dim() != 1 or t.numel() != numel or (numel > 1 and t.stride(0) != 1):
+        raise RuntimeError(f"{who}: {name} must be a contiguous {dtype} tensor [{numel}] on {device}, got {tuple(t.shape)} {t.dtype} on "
+                           f"{t.device}")
+    return t.data_ptr()
+
+
+def _cache(who, k_cache, v_cache, like):
+    """(pages, kv_heads, page_size, head_dim) and the strides of a cache."""
+    shape = k_cache.shape
+    if len(shape) != 4 or v_cache.shape != shape:
+        raise RuntimeError(f"{who}: k_cache and v_cache must both be [pages, kv_heads, page_size, head_dim], got {tuple(shape)} and "
+                           f"{tuple(v_cache.shape)}")
+    dtype, device = like.dtype, like.device
+    if k_cache.dtype != dtype or v_cache.dtype != dtype or k_cache.device != device or v_cache.device != device:
+        raise RuntimeError(f"{who}: the caches must be {dtype} on {device}, as the other tensors are")
+    ks, vs = k_cache.stride(), v_cache.stride()
+    if ks[3] != 1 or vs[3] != 1:
+        raise RuntimeError(f"{who}: the last dimension of the caches must be contiguous")
+    if shape[2] not in _PAGE_SIZES:
+        raise RuntimeError(f"{who}: page size {shape[2]}, only 16, 32, 64, 128 and 256 are supported")
+    return shape, ks[:3] + vs[:3]
+
+
+def _table(who, pages, starts, lens, device):
+    """(sequences, columns, row stride) of the page table."""
+    if pages.dim() != 2 or pages.dtype != torch.int32 or pages.device != device or (pages.shape[1] > 1 and pages.stride(1) != 1):
+        raise RuntimeError(f"{who}: pages must be an int32 tensor [sequences, columns] with contiguous rows on {device}, got "
+                           f"{tuple(pages.shape)} {pages.dtype} on {pages.device}")
+    seqs, columns = pages.shape
+    _index(who, "starts", starts, torch.int32, seqs + 1, device)
+    _index(who, "lens", lens, torch.int32, seqs, device)
+    return seqs, columns, pages.stride(0) if seqs > 1 else columns
+
+
+def apply_rotary(q, k, positions, freqs, interleaved=False, magnitude=1.0, q_out=None, k_out=None):
+    """Rotary positions of q [tokens, heads, head_dim] and k [tokens, kv_heads, head_dim] (either may be None): returns
+    (q_out, k_out), new tensors unless given; q_out=q works in place.
+
+    positions int64 [tokens]; freqs from rotary_frequencies, float64 [rotary_dim / 2], any rotary_dim up to head_dim that is a
+    multiple of 16 - the rest of a head is copied.  Pair i is dims (i, i + rotary_dim / 2), with `interleaved` (2 i, 2 i + 1).
+    Token and head strides are free (a view of a fused projection will do) but multiples of 8."""
+    who = "apply_rotary"
+    like = q if q is not None else k
+    if like is None:
+        raise RuntimeError("apply_rotary: neither q nor k is given")
+    _first(who, "k" if q is None else "q", like)
+    tokens, _, head_dim = like.shape
+    device = like.device
+    heads = kv_heads = 0
+    strides = [0] * 8
+    if q is not None:
+        heads = q.shape[1]
+        q_out = torch.empty((tokens, heads, head_dim), dtype=q.dtype, device=device) if q_out is None else q_out
+        strides[0:2], strides[4:6] = _heads(who, "q", q, like), _heads(who, "q_out", q_out, like, heads)
+    if k is not None:
+        strides[2:4] = _heads(who, "k", k, like)
+        kv_heads = k.shape[1]
+        k_out = torch.empty((tokens, kv_heads, head_dim), dtype=k.dtype, device=device) if k_out is None else k_out
+        strides[6:8] = _heads(who, "k_out", k_out, like, kv_heads)
+    where = _index(who, "positions", positions, torch.int64, tokens, device)
+    rotary_dim = 2 * freqs.numel()
+    turns = _index(who, "freqs", freqs, torch.float64, rotary_dim // 2, device)
+    args = _pack_rotary(_ptr(q) or 0, _ptr(k) or 0, _ptr(q_out) or 0 if heads else 0, _ptr(k_out) or 0 if kv_heads else 0, where, turns,
+                        tokens, heads, kv_heads, head_dim, rotary_dim, bool(interleaved), like.dtype == torch.bfloat16, *strides,
+                        magnitude)
+    with _on(device):
+        check(lib.eet_rotary(args, _stream()))
+    return q_out if heads else q_out, k_out
+
+
+def paged_store(k, v, k_cache, v_cache, pages, starts, lens, q=None, freqs=None, interleaved=False, magnitude=1.0, positions=None,
+                q_out=None):
+    """Appends k and v [tokens, kv_heads, head_dim] of new tokens to their pages, k rotated when freqs is given, and returns q
+    [tokens, heads, head_dim] rotated the same way (in q_out; a new tensor unless given, q_out=q works in place; None without q).
+
+    The positions of the rotation are those in the sequence, or positions int64 [tokens].  Rows of k, v and q that belong to no
+    sequence are not touched.  Two sequences must not append to the same slot (one that they share must lie before both's new
+    tokens)."""
+    who = "paged_store"
+    _first(who, "k", k)
+    tokens, kv_heads, head_dim = k.shape
+    device = k.device
+    k_str, v_str = _heads(who, "k", k, k), _heads(who, "v", v, k, kv_heads)
+    shape, cache_strides = _cache(who, k_cache, v_cache, k)
+    if shape[1] != kv_heads or shape[3] != head_dim:
+        raise RuntimeError(f"paged_store: caches of {shape[1]} heads of {shape[3]} beside {kv_heads} heads of {head_dim}")
+    seqs, columns, pages_stride = _table(who, pages, starts, lens, device)
+    heads, q_str, qo_str = 0, (0, 0), (0, 0)
+    if q is not None:
+        q_str = _heads(who, "q", q, k)
+        heads = q.shape[1]
+        if q_out is None:
+            q_out = torch.empty((tokens, heads, head_dim), dtype=q.dtype, device=device)
+        qo_str = _heads(who, "q_out", q_out, k, heads)
+    elif q_out is not None:
+        raise RuntimeError("paged_store: q_out without q")
+    rotary_dim = turns = where = 0
+    if freqs is not None:
+        rotary_dim = 2 * freqs.numel()
+        turns = _index(who, "freqs", freqs, torch.float64, rotary_dim // 2, device)
+    if positions is not None:
+        where = _index(who, "positions", positions, torch.int64, tokens, device)
+    args = _pack_store(_ptr(q) or 0, _ptr(k) or 0, _ptr(v) or 0, _ptr(q_out) or 0, _ptr(k_cache) or 0, _ptr(v_cache) or 0,
+                       pages.data_ptr(), starts.data_ptr(), lens.data_ptr(), where, turns, tokens, seqs, heads, kv_heads, head_dim,
+                       rotary_dim, bool(interleaved), k.dtype == torch.bfloat16, shape[0], shape[2], columns, pages_stride, *q_str, *k_str,
+                       *v_str, *qo_str, *cache_strides, magnitude)
+    with _on(device):
+        check(lib.eet_paged_store(args, _stream()))
+    return q_out
+
+
+def paged_mha(q, k_cache, v_cache, pages, starts, lens, max_tokens=None, max_len=None, scale=None, window=0, first_key=None,
+              alibi_slopes=None, out=None):
+    """Attention of new tokens q [tokens, heads, head_dim] over the pages, which hold the new tokens' own keys and values already
+    (paged_store).  Returns out, the shape of q.
+
+    A token at position p of sequence b sees positions max(0, first_key[b], p - window + 1) .. p; one that sees none gets zeros.
+    heads is a multiple of kv_heads: that many query heads in a row share a kv head.
+      max_tokens, max_len   the most new tokens and the most positions that a sequence has, as far as the caller knows (a captured
+                            call: the most there may be).  They choose how the work is cut up, not what is computed.
+      scale                 of the scores, 1 / sqrt(head_dim) by default
+      window                0: no window
+      first_key             int32 [sequences]: positions before it are padding
+      alibi_slopes          float32 [heads]: slope * (key position - p) is added to the scores
+    Rows of out that belong to no sequence are left as they are, uninitialised where this call allocated out.
+    K and V of every position that a token of the same tile sees must be finite."""
+    who = "paged_mha"
+    _first(who, "q", q)
+    tokens, heads, head_dim = q.shape
+    device = q.device
+    q_str = _heads(who, "q", q, q)
+    shape, cache_strides = _cache(who, k_cache, v_cache, q)
+    if shape[3] != head_dim:
+        raise RuntimeError(f"paged_mha: caches of head size {shape[3]} beside a q of {head_dim}")
+    seqs, columns, pages_stride = _table(who, pages, starts, lens, device)
+    if out is None:
+        out = torch.empty((tokens, heads, head_dim), dtype=q.dtype, device=device)
+    o_str = _heads(who, "out", out, q, heads)
+    first = _index(who, "first_key", first_key, torch.int32, seqs, device) if first_key is not None else 0
+    slopes = _index(who, "alibi_slopes", alibi_slopes, torch.float32, heads, device) if alibi_slopes is not None else 0
+    if max_tokens is None:
+        max_tokens = 1 if tokens == seqs else tokens
+    if scale is None:
+        scale = 1.0 / math.sqrt(head_dim)
+    fields = [_ptr(q) or 0, _ptr(k_cache) or 0, _ptr(v_cache) or 0, _ptr(out) or 0, pages.data_ptr(), starts.data_ptr(), lens.data_ptr(),
+              first, slopes, tokens, seqs, heads, shape[1], head_dim, q.dtype == torch.bfloat16, shape[0], shape[2], columns, pages_stride,
+              *q_str, *o_str, *cache_strides, window, max_tokens, max_len or 0, scale]
+    with _on(device):
+        args = _pack_mha(*fields, 0, 0)
+        ws_bytes = lib.eet_paged_mha_workspace_bytes(args)
+        if ws_bytes:
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
+            args = _pack_mha(*fields, ws.data_ptr(), ws_bytes)
+        check(lib.eet_paged_mha(args, _stream()))
+    return out

@@ -33,6 +33,7 @@ const char* eet_last_error(void);
  *   3  decode attention: a pipeline wait ran out
  *   4  tensor-parallel exchange: a peer's partial sums never arrived
  *   5  decode attention: the device-resident step was outside [1, T_max]; nothing was appended to the cache
+ *   6  paged cache: a page number outside the cache, or a position behind the end of its sequence's row of the table
  * After a non-zero status the fp32 scratch buffers of the failed call hold undefined values: zero them (and, for
  * the tensor-parallel exchange, the inboxes and epoch counters of every rank) before the next call.
  * Synchronises the device.  The reference reports asynchronous failures the same way, at its next
@@ -327,6 +328,89 @@ int eet_lm_head_argmax(float* sums, const void* scale, int M, int n_local, int64
  * [0, rows_in_table) reads row 0): the token-embedding lookup, torch.nn.Embedding in the reference
  * (python/eet/transformers/modeling_llama.py:281-283). */
 int eet_gather_rows(const void* table, const int64_t* ids, void* out, int rows, int n, int64_t rows_in_table, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Serving from a paged cache
+ *
+ * A cache is k and v of [pages][kv_heads][page_size][head_dim] values, fp16 or bf16, any strides with contiguous rows of
+ * head_dim.  Sequence b holds lens[b] positions; position p of it is slot p % page_size of page pages[b][p / page_size].
+ * The new tokens of all sequences are rows behind one another, those of sequence b the rows [starts[b], starts[b + 1]), and
+ * they are the last positions of their sequence: row starts[b] + i is position lens[b] - (starts[b + 1] - starts[b]) + i.
+ * Rows that belong to no sequence and positions below zero are left alone (paged_mha: zeros for positions below zero).
+ * starts, lens and pages are read on the device, so that a captured graph serves other lengths when it is replayed; a page
+ * outside the cache is not touched and recorded as status 6 (paged_mha: its keys count as zeros).
+ * The reference has contiguous caches [batch][head][time][dim] with all sequences at the same step (csrc/op/llama_mmha.cpp:
+ * 94-112); these calls have no counterpart there.
+ *
+ * The arguments are structures of 8-byte fields; strides are in elements, token / head / page / slot as named.  Pointers must be
+ * 16-byte aligned and strides multiples of 8 elements, except of the index arrays and of pages_stride.
+ * ---------------------------------------------------------------------------------------------- */
+typedef struct {
+    const void *q, *k;         /* [tokens][heads][head_dim], [tokens][kv_heads][head_dim]; either may be NULL with its heads 0 */
+    void *q_out, *k_out;       /* the same shapes; each may be its input */
+    const int64_t* positions;  /* [tokens] */
+    const double* freqs;       /* [rotary_dim / 2], radians a position */
+    int64_t tokens, heads, kv_heads, head_dim;   /* head_dim a multiple of 16 up to 256 */
+    int64_t rotary_dim;        /* dims [0, rotary_dim) of a head are rotated, a multiple of 16; the others are copied */
+    int64_t interleaved;       /* pairs (2i, 2i + 1); else (i, i + rotary_dim / 2) */
+    int64_t bf16;              /* else fp16 */
+    int64_t q_tok, q_head, k_tok, k_head, qo_tok, qo_head, ko_tok, ko_head;
+    double magnitude;          /* factor on the rotated values */
+} eet_rotary_args;
+
+/* Rotary positions: pair (a, b) of a head becomes magnitude * (a cos t - b sin t, b cos t + a sin t), t = positions[token] *
+ * freqs[i] in 64 bits, the rest in fp32 with one rounding.
+ * Stands beside: the rotary half of fused_QKV_bias_rotary_kernel (csrc/core/self_add_bias.cu:369-403), which knows the half
+ * layout over the whole head, positions 0, 1, ... and fp32 angles. */
+int eet_rotary(const eet_rotary_args* args, void* stream);
+
+typedef struct {
+    const void *q, *k, *v;     /* [tokens][heads or kv_heads][head_dim]; q may be NULL with heads = 0 */
+    void* q_out;               /* receives the rotated q; may be q */
+    void *k_cache, *v_cache;
+    const int32_t *pages, *starts, *lens;   /* [seqs][max_pages] pages_stride apart, [seqs + 1], [seqs] */
+    const int64_t* positions;  /* [tokens] for the rotation, or NULL: the position in the sequence */
+    const double* freqs;       /* NULL with rotary_dim = 0: nothing is rotated */
+    int64_t tokens, seqs, heads, kv_heads, head_dim, rotary_dim, interleaved, bf16;   /* head_dim 64 or 128 */
+    int64_t num_pages, page_size, max_pages, pages_stride;                            /* page_size 16, 32, 64, 128 or 256 */
+    int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head, qo_tok, qo_head;
+    int64_t kc_page, kc_head, kc_slot, vc_page, vc_head, vc_slot;
+    double magnitude;
+} eet_paged_store_args;
+
+/* Appends the new tokens' k (rotated) and v to their pages and rotates q, in one launch.
+ * Stands beside: eet_qkv_split_store, which does this for contiguous caches and prompts from position 0. */
+int eet_paged_store(const eet_paged_store_args* args, void* stream);
+
+typedef struct {
+    const void *q, *k_cache, *v_cache;      /* q [tokens][heads][head_dim] */
+    void* out;                              /* [tokens][heads][head_dim] */
+    const int32_t *pages, *starts, *lens;   /* as above */
+    const int32_t* first_key;               /* [seqs]: the first position that counts, or NULL */
+    const float* alibi_slopes;              /* [heads] or NULL */
+    int64_t tokens, seqs, heads, kv_heads, head_dim, bf16;   /* heads a multiple of kv_heads; head_dim 64 or 128 */
+    int64_t num_pages, page_size, max_pages, pages_stride;   /* page_size 16, 32, 64, 128 or 256 */
+    int64_t q_tok, q_head, o_tok, o_head;
+    int64_t kc_page, kc_head, kc_slot, vc_page, vc_head, vc_slot;
+    int64_t window;                         /* a token sees its own and the window - 1 positions before; 0: all */
+    int64_t max_tokens, max_len;            /* the most new tokens and positions of one sequence: what the launch is planned
+                                               for, not a limit */
+    double scale;
+    void* ws;                               /* scratch, eet_paged_mha_workspace_bytes; need not be zero */
+    int64_t ws_bytes;
+} eet_paged_mha_args;
+
+/* Scratch needed by eet_paged_mha; ws and ws_bytes of args are not read.  Calls that share scratch must not overlap on the GPU. */
+size_t eet_paged_mha_workspace_bytes(const eet_paged_mha_args* args);
+
+/*
+ * Attention of the new tokens over the pages (their own keys are there already): row i of sequence b, at position p, is
+ * out = sum_j softmax_j(scale q.k_j + slope[head] (j - p)) v_j over positions j in [max(first_key[b], p - window + 1, 0), p],
+ * zeros where there is none.  heads / kv_heads query heads share a kv head.  Scores, softmax and sums in fp32; the
+ * probabilities enter the product with v in the type of the cache.
+ * Stands beside: eet_prefill_mha and eet_decode_mha (csrc/op/llama_mmha.cpp:354-426, csrc/core/attention_dispatch.cu:140-324).
+ */
+int eet_paged_mha(const eet_paged_mha_args* args, void* stream);
 
 #ifdef __cplusplus
 }

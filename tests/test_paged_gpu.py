@@ -1,0 +1,479 @@
+"""Serving from a paged cache against a plain restatement in 64 bits (paged_util), through the Python calls."""
+import itertools
+import math
+
+import pytest
+import torch
+
+from paged_util import HALF_STEP, Batch, attend64, rotate64, rotate_tolerance
+
+pytestmark = pytest.mark.gpu
+
+FP16, BF16 = torch.float16, torch.bfloat16
+
+
+def _paged():
+    from eet_b200 import paged
+    return paged
+
+
+def _status():
+    from eet_b200 import _lib
+    return _lib.device_status()
+
+
+def _within(got, ref, tol, what=""):
+    off = (got.double().cpu() - ref).abs() - tol
+    assert not torch.isnan(off).any(), what
+    assert (off <= 0).all(), f"{what} {off.max().item():.3g} beyond the tolerance at {int(off.argmax())}"
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# rotary positions
+# ---------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("tokens,heads,kv_heads,head_dim,rotary_dim", [
+    (1, 1, 1, 128, 128), (3, 5, 2, 128, 64), (7, 32, 8, 64, 64), (130, 40, 40, 128, 32), (5, 2, 1, 256, 256), (2, 3, 1, 96, 48),
+    (9, 4, 4, 16, 16), (1000, 8, 2, 128, 96)])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", [FP16, BF16])
+def test_rotary(tokens, heads, kv_heads, head_dim, rotary_dim, interleaved, dtype):
+    gen = torch.Generator().manual_seed(tokens)
+    q, k = (torch.randn(tokens, h, head_dim, generator=gen).to(dtype) for h in (heads, kv_heads))
+    positions = torch.randint(0, 1 << 20, (tokens,), generator=gen)
+    freqs, magnitude = _paged().rotary_frequencies(rotary_dim, scaling={"type": "yarn", "factor": 4.0, "original": 4096}, device="cpu")
+    got = _paged().apply_rotary(q.cuda(), k.cuda(), positions.cuda(), freqs.cuda(), interleaved=interleaved, magnitude=magnitude)
+    for x, y in zip((q, k), got):
+        ref = rotate64(x, positions, freqs, interleaved, magnitude)
+        tol = HALF_STEP[dtype] * ref.abs() + rotate_tolerance(x, freqs, interleaved, dtype, magnitude) + 2.0 ** -25
+        _within(y, ref, tol)
+        assert torch.equal(y[..., rotary_dim:].cpu(), x[..., rotary_dim:])
+
+
+def test_rotary_in_place_on_views_of_a_projection():
+    gen = torch.Generator().manual_seed(5)
+    qkv = torch.randn(33, (6 + 2 + 2) * 128, generator=gen).half().cuda()
+    before = qkv.clone()
+    q, k = qkv[:, :768].view(33, 6, 128), qkv[:, 768:1024].view(33, 2, 128)
+    positions = torch.arange(100, 133).cuda()
+    freqs, _ = _paged().rotary_frequencies(128)
+    fresh = _paged().apply_rotary(q, k, positions, freqs)
+    out = _paged().apply_rotary(q, k, positions, freqs, q_out=q, k_out=k)
+    assert out[0] is q and out[1] is k
+    assert torch.equal(q, fresh[0]) and torch.equal(k, fresh[1])
+    assert torch.equal(qkv[:, 1024:], before[:, 1024:])
+
+
+def test_rotary_of_one_of_the_two_and_of_nothing():
+    gen = torch.Generator().manual_seed(6)
+    x = torch.randn(4, 3, 64, generator=gen).half().cuda()
+    positions = torch.tensor([0, 1, -5, 2 ** 30]).cuda()
+    freqs, _ = _paged().rotary_frequencies(64)
+    a, none = _paged().apply_rotary(x, None, positions, freqs)
+    assert none is None
+    none, b = _paged().apply_rotary(None, x, positions, freqs)
+    assert none is None and torch.equal(a, b)
+    ref = rotate64(x.cpu(), positions.cpu(), freqs.cpu(), False)
+    _within(a, ref, 2.0 ** -11 * ref.abs() + rotate_tolerance(x.cpu(), freqs.cpu(), False, FP16) + 2.0 ** -25)
+    empty = _paged().apply_rotary(x[:0], x[:0], positions[:0], freqs)
+    assert empty[0].shape == (0, 3, 64)
+
+
+def test_rotary_refuses():
+    paged = _paged()
+    x = torch.zeros(4, 3, 64, dtype=FP16, device="cuda")
+    positions = torch.zeros(4, dtype=torch.int64, device="cuda")
+    freqs, _ = paged.rotary_frequencies(64)
+    for bad in (dict(positions=positions.int()), dict(positions=positions[:3]), dict(positions=positions.cpu()), dict(freqs=freqs.float()),
+                dict(k=x.bfloat16()), dict(k=x[:3]), dict(q_out=x[:, :2]), dict(k=x.transpose(1, 2)), dict(k_out=x.float()),
+                dict(freqs=torch.zeros(40, dtype=torch.float64, device="cuda")),
+                dict(q=torch.zeros(4, 3, 65, dtype=FP16, device="cuda")[..., :64]),
+                dict(q=torch.zeros(800, dtype=FP16, device="cuda")[1:769].view(4, 3, 64))):
+        args = dict(q=x, k=x, positions=positions, freqs=freqs)
+        args.update(bad)
+        with pytest.raises(RuntimeError):
+            paged.apply_rotary(args.pop("q"), args.pop("k"), args.pop("positions"), args.pop("freqs"), **args)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# append
+# ---------------------------------------------------------------------------------------------------------------------
+def _gpu(batch):
+    return [t.cuda() for t in (batch.k_cache, batch.v_cache, batch.pages, batch.starts, batch.lens)]
+
+
+@pytest.mark.parametrize("new,lens,page", [
+    ([1], [1], 16), ([1, 1, 1], [5, 16, 17], 16), ([3, 0, 20, 1], [3, 40, 33, 64], 32), ([130], [257], 64), ([0, 0], [3, 0], 16),
+    ([5, 2], [300, 2], 256), ([1] * 300, [1 + i % 50 for i in range(300)], 16)])
+@pytest.mark.parametrize("dtype,head_dim,interleaved,rotary_dim", [(FP16, 128, False, 128), (BF16, 64, True, 32), (FP16, 64, False, 0)])
+def test_store(new, lens, page, dtype, head_dim, interleaved, rotary_dim):
+    batch = Batch(new, lens, 6, 2, head_dim, page, dtype, behind=2)
+    kc, vc, pages, starts, n = _gpu(batch)
+    freqs = _paged().rotary_frequencies(rotary_dim, device="cpu")[0] if rotary_dim else None
+    out = torch.full_like(batch.q, 7.0).cuda()
+    got = _paged().paged_store(batch.k.cuda(), batch.v.cuda(), kc, vc, pages, starts, n, q=batch.q.cuda(), interleaved=interleaved,
+                               freqs=None if freqs is None else freqs.cuda(), q_out=out)
+    assert got is out
+    total, positions = sum(new), batch.positions()
+    if rotary_dim:
+        q64, k64 = (rotate64(x[:total], positions, freqs, interleaved) for x in (batch.q, batch.k))
+        tols = [HALF_STEP[dtype] * y.abs() + rotate_tolerance(x[:total], freqs, interleaved, dtype) + 2.0 ** -25
+                for x, y in ((batch.q, q64), (batch.k, k64))]
+    else:
+        q64, k64 = batch.q[:total].double(), batch.k[:total].double()
+        tols = [torch.zeros_like(q64), torch.zeros_like(k64)]
+    _within(out[:total], q64, tols[0])
+    assert (out[total:] == 7.0).all(), "rows behind the last sequence"
+    # every slot of the new tokens holds its row, every other slot what it held
+    kc, vc = kc.cpu(), vc.cpu()
+    at = 0
+    for b, t in enumerate(new):
+        p = torch.arange(lens[b] - t, lens[b])
+        page_of, slot = batch.pages[b].long()[p // page], p % page
+        _within(kc[page_of, :, slot], k64[at:at + t], tols[1][at:at + t])
+        assert torch.equal(vc[page_of, :, slot], batch.v[at:at + t])
+        kc[page_of, :, slot] = batch.k_cache[page_of, :, slot]
+        vc[page_of, :, slot] = batch.v_cache[page_of, :, slot]
+        at += t
+    assert torch.equal(kc, batch.k_cache) and torch.equal(vc, batch.v_cache)
+    assert _status() == 0
+
+
+def test_store_with_positions_of_its_own_and_caches_in_another_order():
+    """The cache as [pages][page][heads][dim] with k and v in one tensor, positions from the caller, q in place."""
+    batch = Batch([4, 2], [20, 18], 4, 2)
+    both = torch.zeros(batch.k_cache.shape[0], 2, 16, 2, 128, dtype=FP16, device="cuda")
+    kc, vc = both[:, 0].transpose(1, 2), both[:, 1].transpose(1, 2)
+    positions = torch.tensor([3, 1, 4, 1, 5, 9])
+    freqs, _ = _paged().rotary_frequencies(128)
+    q = batch.q.cuda()
+    assert _paged().paged_store(batch.k.cuda(), batch.v.cuda(), kc, vc, batch.pages.cuda(), batch.starts.cuda(), batch.lens.cuda(), q=q,
+                                freqs=freqs, positions=positions.cuda(), q_out=q) is q
+    want, _ = _paged().apply_rotary(batch.q.cuda(), None, positions.cuda(), freqs)
+    assert torch.equal(q, want)
+    want, _ = _paged().apply_rotary(batch.k.cuda(), None, positions.cuda(), freqs)
+    stored = torch.cat([batch.history(kc.cpu(), b)[n - t:] for b, (t, n) in enumerate(zip([4, 2], [20, 18]))])
+    assert torch.equal(stored, want.cpu())
+    assert int((both != 0).any(-1).sum()) == 2 * 6 * 2
+
+
+def test_store_does_not_follow_bad_pages_or_positions():
+    batch = Batch([2, 2, 3, 2], [17, 33, 1, 40], 4, 2)      # the third has two tokens in front of its first position
+    batch.pages[0, 1] = batch.k_cache.shape[0]              # the page behind the last
+    batch.pages[1, 2] = -1
+    kc, vc, pages, starts, lens = _gpu(batch)
+    lens[3] = 1 << 20                                       # positions behind its row of the table
+    q = _paged().paged_store(batch.k.cuda(), batch.v.cuda(), kc, vc, pages, starts, lens, q=batch.q.cuda())
+    assert _status() == 6
+    assert torch.equal(q.cpu(), batch.q)
+    changed = (kc.cpu() != batch.k_cache).any(-1).any(1).nonzero().tolist()
+    assert changed == sorted([[int(batch.pages[0, 0]), 15], [int(batch.pages[1, 1]), 15], [int(batch.pages[2, 0]), 0]])
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------------------------------------------------
+def _mha(batch, out=None, **kw):
+    kc, vc, pages, starts, lens = _gpu(batch)
+    kw = {k: v.cuda() if torch.is_tensor(v) else v for k, v in kw.items()}
+    return _paged().paged_mha(batch.q.cuda(), kc, vc, pages, starts, lens, out=out, **kw)
+
+
+def _check(batch, hints=True, **kw):
+    batch.poison()
+    out = torch.full_like(batch.q, 7.0).cuda()
+    if hints:
+        kw = dict(kw, max_tokens=max(batch.new), max_len=max(batch.lens_list))
+    got = _mha(batch, out, **kw)
+    assert got is out and _status() == 0
+    for k in ("max_tokens", "max_len"):
+        kw.pop(k, None)
+    ref, tol = attend64(batch, **kw)
+    n = sum(batch.new)
+    _within(out[:n], ref, tol)
+    assert (out[n:] == 7.0).all(), "rows behind the last sequence"
+    return out
+
+
+LENGTHS = [
+    ([1], [1]), ([1], [129]), ([1, 1, 1], [16, 127, 300]), ([1, 0, 1], [64, 5, 1000]), ([5, 3, 1, 2], [5, 70, 128, 131]),
+    ([17], [17]), ([40, 1], [640, 33]), ([130, 1, 129], [130, 900, 700]), ([300], [333]),
+]
+HEADS = [(1, 1), (4, 4), (8, 2), (5, 1), (12, 2), (16, 1), (28, 4), (32, 1)]
+
+
+@pytest.mark.parametrize("new,lens", LENGTHS)
+@pytest.mark.parametrize("heads,kv_heads", HEADS)
+def test_mha(new, lens, heads, kv_heads):
+    n = len(new) * 10 + heads
+    dtype, head_dim, page = (FP16, BF16)[n % 2], (128, 64, 128)[n % 3], (16, 32, 64, 128, 256)[n % 5]
+    _check(Batch(new, lens, heads, kv_heads, head_dim, page, dtype, seed=n, behind=1))
+
+
+@pytest.mark.parametrize("page,head_dim,dtype", list(itertools.product((16, 32, 64, 128, 256), (64, 128), (FP16, BF16))))
+@pytest.mark.parametrize("new", [[1, 1], [4, 3], [200, 70]])
+def test_mha_pages_types_and_head_sizes(page, head_dim, dtype, new):
+    _check(Batch(new, [405, 258], 8, 4, head_dim, page, dtype, seed=page))
+
+
+@pytest.mark.parametrize("window", [1, 2, 63, 64, 65, 128, 200, 100000])
+@pytest.mark.parametrize("new", [[1, 1, 1], [3, 1, 2], [150, 1, 33]])
+def test_mha_window(window, new):
+    _check(Batch(new, [150, 700, 333], 4, 2, seed=window), window=window)
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1, 1], [3, 1, 2, 4], [150, 1, 33, 140]])
+def test_mha_left_padding_and_rows_that_see_nothing(new):
+    first = torch.tensor([100, 0, 333, 500], dtype=torch.int32)    # the third sees its last position only if that is 332: nothing
+    batch = Batch(new, [150, 700, 333, 501], 4, 2)
+    out = _check(batch, first_key=first)
+    at = sum(new[:2])
+    assert (out[at:at + new[2]] == 0).all()
+    _check(Batch(new, [150, 700, 333, 501], 4, 2, seed=9), first_key=first, window=70)
+
+
+@pytest.mark.parametrize("new", [[5, 2], [1, 1], [40, 30], [200, 3]])
+def test_mha_tokens_in_front_of_the_first_position(new):
+    """A sequence shorter than its new tokens: the first ones stand at positions below zero, see nothing and get zeros."""
+    lens = [3 if new[0] > 3 else 0, 2]
+    batch = Batch(new, lens, 4, 2)
+    out = torch.full_like(batch.q, 7.0).cuda()
+    _mha(batch, out)
+    ref, tol = attend64(batch)
+    _within(out, ref, tol)
+    assert (out[:new[0] - lens[0]] == 0).all()
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(4, 4), (40, 8)])
+@pytest.mark.parametrize("new", [[1, 1], [6, 2], [140, 1]])
+def test_mha_alibi(heads, kv_heads, new):
+    from eet_b200.EET import alibi_slopes
+    slopes = torch.tensor(alibi_slopes(heads), dtype=torch.float32)
+    _check(Batch(new, [141, 900], heads, kv_heads), alibi_slopes=slopes)
+    _check(Batch(new, [141, 900], heads, kv_heads, dtype=BF16), alibi_slopes=slopes, window=100,
+           first_key=torch.tensor([30, 0], dtype=torch.int32))
+
+
+@pytest.mark.parametrize("new", [[1], [200]])
+def test_mha_scale_and_large_scores(new):
+    _check(Batch(new, [500], 4, 2, q_scale=30.0))
+    _check(Batch(new, [500], 4, 2), scale=0.0)
+    _check(Batch(new, [500], 4, 2), scale=-0.2)
+
+
+@pytest.mark.parametrize("new", [[1, 1], [6, 1], [140, 20]])
+def test_mha_without_hints_and_with_wrong_ones(new):
+    """The hints choose how the work is cut up; what is computed does not depend on them."""
+    _check(Batch(new, [400, 333], 8, 2), hints=False)
+    _check(Batch(new, [400, 333], 8, 2), hints=False, max_tokens=1, max_len=1)
+    _check(Batch(new, [400, 333], 8, 2), hints=False, max_tokens=10 ** 6, max_len=10 ** 9)
+
+
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan, 65504.0])
+@pytest.mark.parametrize("new", [[1, 1], [7, 1], [100, 150]])
+def test_mha_of_slots_behind_the_end_and_before_the_window(value, new):
+    batch = Batch(new, [333, 190], 4, 2)
+    batch.poison(value)
+    # what lies before the window of the first new token, too
+    for b, (t, n) in enumerate(zip(new, batch.lens_list)):
+        p = torch.arange(max(0, n - t - 20 + 1))
+        for cache in (batch.k_cache, batch.v_cache):
+            cache[batch.pages[b].long()[p // 16], :, p % 16] = value
+    got = _mha(batch, window=20)
+    for b, (t, n) in enumerate(zip(new, batch.lens_list)):
+        p = torch.arange(max(0, n - t - 20 + 1))
+        for cache in (batch.k_cache, batch.v_cache):
+            cache[batch.pages[b].long()[p // 16], :, p % 16] = 0.0
+    ref, tol = attend64(batch, window=20)
+    _within(got, ref, tol)
+
+
+def test_mha_strides():
+    """q and out as parts of wider rows, the caches as [pages][page][heads][dim] in one tensor, rows of the table far apart."""
+    for new in ([1, 1], [5, 2], [150, 3]):
+        batch = Batch(new, [222, 300], 6, 2)
+        n = sum(new)
+        wide = torch.zeros(n, 10, 128, dtype=FP16, device="cuda")
+        wide[:, 2:8] = batch.q.cuda()
+        both = torch.stack((batch.k_cache, batch.v_cache), 1).transpose(2, 3).contiguous().cuda()     # [pages][2][page][heads][dim]
+        table = torch.full((2, 50), -1, dtype=torch.int32, device="cuda")
+        table[:, :batch.pages.shape[1]] = batch.pages.cuda()
+        out = torch.full((n, 8, 256), 7.0, dtype=FP16, device="cuda")
+        _paged().paged_mha(wide[:, 2:8], both[:, 0].transpose(1, 2), both[:, 1].transpose(1, 2), table[:, :batch.pages.shape[1]],
+                           batch.starts.cuda(), batch.lens.cuda(), out=out[:, 1:7, 128:])
+        ref, tol = attend64(batch)
+        _within(out[:, 1:7, 128:], ref, tol)
+        assert (out[..., :128] == 7.0).all() and (out[:, 0] == 7.0).all() and (out[:, 7] == 7.0).all()
+    assert _status() == 0
+
+
+def test_mha_shared_pages():
+    """Two sequences with a common beginning, held once; the same sequence twice in a batch."""
+    for new in ([1, 1, 1], [2, 3, 2], [60, 70, 60]):
+        batch = Batch(new, [160, 200, 160], 8, 2)
+        batch.pages[1, :5] = batch.pages[0, :5]
+        batch.pages[2] = batch.pages[0]
+        _check(batch)
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [5, 1, 6], [140, 1, 60]])
+def test_mha_does_not_follow_bad_pages(new):
+    """The other sequences are served, the status names the fault."""
+    batch = Batch(new, [160, 333, 160], 8, 2)
+    ref, tol = attend64(batch)
+    batch.pages[1, 3] = batch.k_cache.shape[0] + 5
+    batch.pages[1, 4] = -7
+    got = _mha(batch)
+    assert _status() == 6
+    a, b = new[0], new[0] + new[1]
+    _within(got[:a], ref[:a], tol[:a])
+    _within(got[b:], ref[b:], tol[b:])
+
+
+def test_mha_of_nothing():
+    batch = Batch([0, 0], [5, 0], 4, 2)
+    assert _mha(batch).shape == (0, 4, 128)
+    none = Batch([1], [4], 4, 2)
+    empty = torch.zeros(0, 3, dtype=torch.int32, device="cuda")
+    out = torch.full_like(none.q, 7.0).cuda()
+    _paged().paged_mha(none.q.cuda(), none.k_cache.cuda(), none.v_cache.cuda(), empty, torch.zeros(1, dtype=torch.int32, device="cuda"),
+                       torch.zeros(0, dtype=torch.int32, device="cuda"), out=out)
+    assert (out == 7.0).all()
+
+
+def test_mha_many_sequences():
+    lens = [1 + (37 * i) % 400 for i in range(700)]
+    _check(Batch([1] * 700, lens, 4, 1))
+    _check(Batch([min(n, 1 + i % 3) for i, n in enumerate(lens)], lens, 20, 1, head_dim=64))
+
+
+def test_mha_long():
+    """Split over many CTAs: a long history, for one token and for a few."""
+    _check(Batch([1, 1], [20000, 300], 8, 1))
+    _check(Batch([1], [9000], 32, 1, dtype=BF16))
+    _check(Batch([30], [9000], 8, 1))
+
+
+def test_mha_twice_is_the_same():
+    for new in ([1, 1], [3, 1], [130, 9]):
+        batch = Batch(new, [3000, 333], 8, 2)
+        assert torch.equal(_mha(batch), _mha(batch))
+
+
+def test_mha_refuses():
+    paged = _paged()
+    batch = Batch([1, 2], [20, 30], 4, 2)
+    q = batch.q.cuda()
+    kc, vc, pages, starts, lens = _gpu(batch)
+    names = ("q", "k_cache", "v_cache", "pages", "starts", "lens")
+    for bad in (dict(q=q.float()), dict(q=q[0]), dict(q=q.bfloat16()), dict(k_cache=kc[0]), dict(v_cache=vc[:1]), dict(v_cache=vc.bfloat16()),
+                dict(pages=pages.long()), dict(pages=pages.cpu()), dict(pages=pages[:1]), dict(starts=starts[:2]), dict(starts=starts.long()),
+                dict(lens=lens[:1]), dict(lens=lens.cpu()), dict(out=q[:, :2]), dict(out=q.float()), dict(first_key=lens.long()),
+                dict(first_key=lens[:1]), dict(alibi_slopes=torch.ones(3, device="cuda")), dict(alibi_slopes=torch.ones(4)),
+                dict(window=-1), dict(q=torch.zeros(3, 3, 128, dtype=FP16, device="cuda")),
+                dict(q=torch.zeros(3, 4, 64, dtype=FP16, device="cuda")), dict(k_cache=kc[:, :, :8], v_cache=vc[:, :, :8]),
+                dict(q=torch.zeros(3 * 512 + 8, dtype=FP16, device="cuda")[1:1537].view(3, 4, 128)),
+                dict(q=torch.zeros(3, 4, 129, dtype=FP16, device="cuda")[..., :128])):
+        args = dict(zip(names, (q, kc, vc, pages, starts, lens)))
+        args.update(bad)
+        with pytest.raises(RuntimeError):
+            paged.paged_mha(*[args.pop(n) for n in names], **args)
+
+
+def test_mha_captured_and_replayed_with_other_lengths():
+    batch = Batch([1, 1, 2], [100, 300, 200], 8, 2)
+    later = Batch([1, 1, 2], [140, 3, 310], 8, 2, seed=4)
+    width, total = 20, max(batch.k_cache.shape[0], later.k_cache.shape[0])
+    q = batch.q.cuda()
+    kc, vc = (torch.zeros(total, 2, 16, 128, dtype=FP16, device="cuda") for _ in range(2))
+    pages, starts, lens = (torch.zeros(3, width, dtype=torch.int32, device="cuda"), batch.starts.cuda(),
+                           torch.zeros(3, dtype=torch.int32, device="cuda"))
+
+    def fill(b):
+        q.copy_(b.q)
+        kc[:b.k_cache.shape[0]].copy_(b.k_cache)
+        vc[:b.v_cache.shape[0]].copy_(b.v_cache)
+        pages.fill_(-1)
+        pages[:, :b.pages.shape[1]].copy_(b.pages)
+        starts.copy_(b.starts)
+        lens.copy_(b.lens)
+
+    fill(batch)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        _paged().paged_mha(q, kc, vc, pages, starts, lens, max_tokens=2)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = _paged().paged_mha(q, kc, vc, pages, starts, lens, max_tokens=2)
+    for b in (batch, later, batch):
+        fill(b)
+        graph.replay()
+        ref, tol = attend64(b)
+        _within(out, ref, tol)
+
+
+def test_two_captured_graphs_and_two_streams_do_not_share_scratch():
+    batches = [Batch([1, 3], [3000, 500], 8, 2, seed=s) for s in (1, 2)]
+    refs = [attend64(b) for b in batches]
+    inputs = [(b.q.cuda(), *_gpu(b)) for b in batches]
+    streams = [torch.cuda.Stream() for _ in batches]
+    graphs, outs = [], []
+    for args, s in zip(inputs, streams):
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            _paged().paged_mha(*args)
+        s.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            outs.append(_paged().paged_mha(*args))
+        graphs.append(g)
+    for _ in range(20):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for out, (ref, tol) in zip(outs, refs):
+        _within(out, ref, tol)
+    eager = []
+    for _ in range(10):
+        for args, s in zip(inputs, streams):
+            with torch.cuda.stream(s):
+                eager.append(_paged().paged_mha(*args))
+    torch.cuda.synchronize()
+    for i, out in enumerate(eager):
+        _within(out, *refs[i % 2])
+
+
+def test_store_and_attention_of_a_prompt_in_chunks_and_then_token_by_token():
+    """As they are used: the sequence grows by chunks of 50, 1, 128 and single tokens; each step's context is that of the whole
+    sequence so far."""
+    H, K, D, page = 8, 2, 128, 32
+    gen = torch.Generator().manual_seed(0)
+    total = [183, 90]
+    qkv = [torch.randn(n, H + 2 * K, D, generator=gen).half() for n in total]
+    kc, vc = (torch.full((12, K, page, D), math.nan, dtype=FP16, device="cuda") for _ in range(2))
+    pages = torch.tensor([[3, 9, 0, 5, 11, 1], [2, 10, 4, -1, -1, -1]], dtype=torch.int32)
+    freqs, _ = _paged().rotary_frequencies(D)
+    done = [0, 0]
+    for step in ([50, 0], [1, 30], [128, 1], [1, 57], [1, 1], [1, 1], [1, 0]):
+        new = [qkv[b][done[b]:done[b] + n] for b, n in enumerate(step)]
+        done = [a + n for a, n in zip(done, step)]
+        rows = torch.cat(new).cuda()
+        starts = torch.tensor([0, step[0], sum(step)], dtype=torch.int32).cuda()
+        lens = torch.tensor(done, dtype=torch.int32).cuda()
+        q = _paged().paged_store(rows[:, H:H + K], rows[:, H + K:], kc, vc, pages.cuda(), starts, lens, q=rows[:, :H], freqs=freqs)
+        ctx = _paged().paged_mha(q, kc, vc, pages.cuda(), starts, lens, max_tokens=max(step))
+        # the same from what the cache holds now
+        view = Batch.__new__(Batch)
+        view.new, view.lens_list, view.page, view.dtype = step, done, page, FP16
+        view.k_cache, view.v_cache, view.pages, view.q = kc.cpu(), vc.cpu(), pages, q.cpu()
+        ref, tol = attend64(view)
+        _within(ctx, ref, tol, f"step {step}")
+    # and the cache holds every rotated key
+    for b in range(2):
+        want = rotate64(qkv[b][:done[b], H:H + K], torch.arange(done[b]), freqs.cpu(), False)
+        got = kc.cpu()[pages[b].long()[torch.arange(done[b]) // page], :, torch.arange(done[b]) % page]
+        x = qkv[b][:done[b], H:H + K]
+        _within(got, want, 2.0 ** -11 * want.abs() + rotate_tolerance(x, freqs.cpu(), False, FP16) + 2.0 ** -25)
+    assert _status() == 0
