@@ -55,6 +55,7 @@ static inline bool aligned16(const void* p)
 #include "attention_tc.cu"
 #include "glue.cu"
 #include "noalloc.cu"
+#include "paged_tc.cu"
 #include "paged.cu"
 #include "quantize.cu"
 

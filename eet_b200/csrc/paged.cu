@@ -134,56 +134,6 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryArgs a)
     }
 }
 
-// Attention over the pages, one warp a (token, head): a lane holds D / 32 dims of the query and of the sum.
-template<typename T, int D>
-__global__ void __launch_bounds__(128) paged_mha_kernel(const PagedMhaArgs a)
-{
-    constexpr int E = D / 32;
-    const int lane = threadIdx.x & 31;
-    const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (item >= (long long)a.tokens * a.heads) return;
-    const int token = (int)(item / a.heads), head = (int)(item % a.heads);
-    int seq = 0;
-    for (int i = 0; i < a.seqs; i += 32) {
-        seq += __popc(__ballot_sync(0xffffffffu, i + lane < a.seqs && a.starts[i + lane + 1] <= token));
-    }
-    if (seq >= a.seqs || a.starts[seq] > token) return;
-    const long long pos = (long long)a.lens[seq] - a.starts[seq + 1] + token;
-    long long first = a.first_key != nullptr ? a.first_key[seq] : 0;
-    if (first < 0) first = 0;
-    if (a.window > 0 && pos - a.window + 1 > first) first = pos - a.window + 1;
-    const int kvh = head / (a.heads / a.kv_heads);
-    float q[E], acc[E];
-    for (int e = 0; e < E; ++e) {
-        q[e] = (float)((const T*)a.q)[(size_t)token * a.q_tok + (size_t)head * a.q_head + lane + 32 * e];
-        acc[e] = 0.f;
-    }
-    const float slope = a.slopes != nullptr ? a.slopes[head] : 0.f;
-    float m = -INFINITY, l = 0.f;
-    for (long long j = first; j <= pos; ++j) {
-        const long long column = j >> a.page_shift;
-        const int page = column < a.max_pages ? a.pages[seq * a.pages_stride + column] : -1;
-        if (page < 0 || page >= a.num_pages) {
-            if (lane == 0) g_device_status = 6;
-            continue;
-        }
-        const long long slot = j & ((1 << a.page_shift) - 1);
-        const T* kr = (const T*)a.k_cache + page * a.kc_page + kvh * a.kc_head + slot * a.kc_slot;
-        const T* vr = (const T*)a.v_cache + page * a.vc_page + kvh * a.vc_head + slot * a.vc_slot;
-        float s = 0.f;
-        for (int e = 0; e < E; ++e) s += q[e] * (float)kr[lane + 32 * e];
-        s = warp_sum(s) * a.scale + slope * (float)(j - pos);
-        const float m_new = fmaxf(m, s);
-        const float corr = expf(m - m_new), p = expf(s - m_new);
-        l = l * corr + p;
-        for (int e = 0; e < E; ++e) acc[e] = acc[e] * corr + p * (float)vr[lane + 32 * e];
-        m = m_new;
-    }
-    for (int e = 0; e < E; ++e) {
-        ((T*)a.out)[(size_t)token * a.o_tok + (size_t)head * a.o_head + lane + 32 * e] = (T)(l > 0.f ? acc[e] / l : 0.f);
-    }
-}
-
 }  // namespace
 
 template<typename T, bool kStore>
@@ -208,26 +158,14 @@ int launch_rotary(const RotaryArgs& a, bool store, cudaStream_t stream)
     return store ? launch_rotary_t<__half, true>(a, stream) : launch_rotary_t<__half, false>(a, stream);
 }
 
-size_t paged_mha_workspace_bytes(const PagedMhaArgs&)
+size_t paged_mha_workspace_bytes(const PagedMhaArgs& a)
 {
-    return 0;
+    return paged_mha_tc_workspace_bytes(a);
 }
 
 int launch_paged_mha(const PagedMhaArgs& a, cudaStream_t stream)
 {
-    if (a.tokens == 0 || a.seqs == 0) return 0;
-    const long long blocks = ((long long)a.tokens * a.heads + 3) / 4;
-    EET_CHECK(blocks <= 0x7fffffffLL, "paged attention: %d tokens of %d heads are too many", a.tokens, a.heads);
-    if (a.head_dim == 128) {
-        if (a.bf16) paged_mha_kernel<__nv_bfloat16, 128><<<(unsigned)blocks, 128, 0, stream>>>(a);
-        else paged_mha_kernel<__half, 128><<<(unsigned)blocks, 128, 0, stream>>>(a);
-    }
-    else {
-        if (a.bf16) paged_mha_kernel<__nv_bfloat16, 64><<<(unsigned)blocks, 128, 0, stream>>>(a);
-        else paged_mha_kernel<__half, 64><<<(unsigned)blocks, 128, 0, stream>>>(a);
-    }
-    EET_LAUNCH_CHECK();
-    return 0;
+    return launch_paged_mha_tc(a, stream);
 }
 
 }  // namespace eet

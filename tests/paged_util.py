@@ -98,7 +98,7 @@ def attend64(batch, scale=None, window=0, first_key=None, alibi_slopes=None):
         if first_key is not None:
             seen &= j >= first_key[b]
         s = scale * q @ k.transpose(1, 2)
-        size = scale * q.abs() @ k.abs().transpose(1, 2) if length else s
+        size = abs(scale) * q.abs() @ k.abs().transpose(1, 2) if length else s
         if alibi_slopes is not None:
             bias = alibi_slopes.double()[:, None, None] * (j - p)
             s, size = s + bias, size + bias.abs()
