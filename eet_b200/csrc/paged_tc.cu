@@ -611,7 +611,7 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             int low = valid ? p.s.first : 0, high = valid ? min(pos, cap - 1) : 0x7fffffff;
             if (valid && a.window > 0) low = (int)max((long long)low, (long long)pos - a.window + 1);
             float slope = 0.f;
-            if (kBias) slope = valid && a.slopes != nullptr ? a.slopes[head] : 0.f;
+            if (kBias && valid && a.slopes != nullptr) slope = a.slopes[head];
             float m_run = kPgNone, m_ref = kPgNone, l_run = 0.f;
             for (int j = turns.first; j < turns.end && ok; j += turns.stride) {
                 const int key0 = (p.block0 + j) * kPgKeys;
@@ -621,31 +621,49 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 }
                 ++used;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                uint32_t v[kPgKeys];
+                // scores of keys c0 .. c0 + 31 of the block: bias, masks
+                const bool masked = !__all_sync(0xffffffffu, low <= key0 && high >= key0 + kPgKeys - 1);
+                auto finish = [&](uint32_t* v, int c0) {
+                    if (kBias) {
+                        const float base = slope * (float)(key0 + c0 - pos);
 #pragma unroll
-                for (int c = 0; c < kPgKeys; c += 32) tmem_ld32_async(t_s + c, v + c);
-                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-                for (int c = 0; c < kPgKeys; ++c) asm volatile("" : "+r"(v[c]));
-                if (kBias) {
-                    const float base = slope * (float)(key0 - pos);
-#pragma unroll
-                    for (int c = 0; c < kPgKeys; ++c) {
-                        v[c] = __float_as_uint(fmaf(__uint_as_float(v[c]), a.scale, fmaf(slope, (float)c, base)));
+                        for (int c = 0; c < 32; ++c) {
+                            v[c] = __float_as_uint(fmaf(__uint_as_float(v[c]), a.scale, fmaf(slope, (float)c, base)));
+                        }
                     }
-                }
-                if (!__all_sync(0xffffffffu, low <= key0 && high >= key0 + kPgKeys - 1)) {
-                    const int c0 = low - key0, c1 = high - key0;
+                    if (masked) {
+                        const int from = low - key0 - c0, to = high - key0 - c0;
 #pragma unroll
-                    for (int c = 0; c < kPgKeys; ++c) {
-                        if (c < c0 || c > c1) v[c] = 0xff800000u;   // -inf
+                        for (int c = 0; c < 32; ++c) {
+                            if (c < from || c > to) v[c] = 0xff800000u;   // -inf
+                        }
                     }
-                }
+                };
                 float mx[4] = {kPgNone, kPgNone, kPgNone, kPgNone};
+                auto maxima = [&](const uint32_t* v) {
 #pragma unroll
-                for (int c = 0; c < kPgKeys; c += 2) {
-                    mx[(c >> 1) & 3] = max3(mx[(c >> 1) & 3], __uint_as_float(v[c]), __uint_as_float(v[c + 1]));
-                }
+                    for (int c = 0; c < 32; c += 2) {
+                        mx[(c >> 1) & 3] = max3(mx[(c >> 1) & 3], __uint_as_float(v[c]), __uint_as_float(v[c + 1]));
+                    }
+                };
+                // The upper half of the row for its maximum, then the lower half, which stays; the upper one is read again for
+                // its exponentials (all 128 at once did not fit the registers).  The probabilities go over the scores of keys
+                // 0 .. 63, so the lower half comes first.
+                uint32_t v[64];
+                tmem_ld32_async(t_s + 64, v);
+                tmem_ld32_async(t_s + 96, v + 32);
+                tmem_ld_wait(v);
+                finish(v, 64);
+                finish(v + 32, 96);
+                maxima(v);
+                maxima(v + 32);
+                tmem_ld32_async(t_s, v);
+                tmem_ld32_async(t_s + 32, v + 32);
+                tmem_ld_wait(v);
+                finish(v, 0);
+                finish(v + 32, 32);
+                maxima(v);
+                maxima(v + 32);
                 m_run = fmaxf(m_run, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
                 float corr = 1.0f;
                 const bool first = j == turns.first;
@@ -656,18 +674,27 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 }
                 const uint64_t scale2 = pair2(to_log2, to_log2), off2 = pair2(-m_ref * to_log2, -m_ref * to_log2);
                 uint64_t psum[2] = {0ull, 0ull};
+                auto exponents = [&](const uint32_t* v, uint32_t* pk) {
 #pragma unroll
-                for (int c0 = 0; c0 < kPgKeys; c0 += 64) {
-                    uint32_t pk[32];
-#pragma unroll
-                    for (int c = 0; c < 32; ++c) {
-                        const float2 e = split2(fma2(pair2(__uint_as_float(v[c0 + 2 * c]), __uint_as_float(v[c0 + 2 * c + 1])), scale2, off2));
+                    for (int c = 0; c < 16; ++c) {
+                        const float2 e = split2(fma2(pair2(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1])), scale2, off2));
                         const float p0 = ex2_approx(e.x), p1 = ex2_approx(e.y);
                         psum[c & 1] = add2(psum[c & 1], pair2(p0, p1));
                         pk[c] = PgType<T>::pack(p0, p1);
                     }
-                    tmem_st32_async(t_s + c0 / 2, pk);
-                }
+                };
+                uint32_t pk[32];
+                exponents(v, pk);
+                exponents(v + 32, pk + 16);
+                tmem_ld32_async(t_s + 64, v);
+                tmem_ld32_async(t_s + 96, v + 32);
+                tmem_st32_async(t_s, pk);
+                tmem_ld_wait(v);
+                finish(v, 64);
+                finish(v + 32, 96);
+                exponents(v, pk);
+                exponents(v + 32, pk + 16);
+                tmem_st32_async(t_s + 32, pk);
                 const float2 ps = split2(add2(psum[0], psum[1]));
                 l_run = l_run * corr + (ps.x + ps.y);
                 // O under the new reference.  The P.V of the block before has completed: s_full was committed behind it.
