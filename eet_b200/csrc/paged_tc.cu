@@ -312,7 +312,8 @@ struct PgSmem {
     uint64_t q_full, q_empty;
     uint64_t full[kPgStages], empty[kPgStages];
     uint64_t s_full[2];      // Q.K^T of a block has completed, and the P.V before it
-    uint64_t p_ready[2];     // the probabilities are there, O is rescaled (four warps)
+    uint64_t p_half[2];      // the probabilities of the block's first 64 keys are there, O is rescaled (four warps)
+    uint64_t p_ready[2];     // those of the others, too
     uint64_t o_full[2];      // the last P.V of a piece has completed
     uint64_t o_free[2];      // O has been read (four warps)
     uint64_t b_ready;        // split: b's maximum and sum are in b_max, b_sum, its O is complete (four warps)
@@ -321,6 +322,16 @@ struct PgSmem {
     float b_max[kPgRows], b_sum[kPgRows];
     PgFound found;
 };
+
+__device__ __forceinline__ void tmem_st16_async(uint32_t taddr, const uint32_t (&v)[16])
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};\n" ::"r"(
+            taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+        "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
 
 __device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar)
 {
@@ -386,6 +397,7 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         }
         for (int x = 0; x < 2; ++x) {
             mbar_init(&sm.s_full[x], 1);
+            mbar_init(&sm.p_half[x], 4);
             mbar_init(&sm.p_ready[x], 4);
             mbar_init(&sm.o_full[x], 1);
             mbar_init(&sm.o_free[x], 4);
@@ -536,15 +548,19 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 auto issue_pv = [&](int x, int j) -> bool {
                     const bool first = j == turns[x].first;
                     if (first && outs[x] > 0 && !tc_wait(&sm.o_free[x], (uint32_t)((outs[x] - 1) & 1), &sm.abort)) return false;
-                    if (!landed(v_entry(j)) || !tc_wait(&sm.p_ready[x], (uint32_t)(used[x] & 1), &sm.abort)) return false;
-                    ++used[x];
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    if (!landed(v_entry(j))) return false;
                     const uint64_t vd = v_desc + (uint64_t)((v_entry(j) % kPgStages) * (kTile >> 4));
 #pragma unroll
-                    for (int kk = 0; kk < kPgKeys / 16; ++kk) {
-                        umma_f16_ts(tmem + 256 + x * 128, tmem + x * kPgKeys + kk * 8, vd + (uint64_t)(kk * (2048 >> 4)), idesc_pv,
-                                    !first || kk != 0);
+                    for (int half = 0; half < 2; ++half) {
+                        if (!tc_wait(half ? &sm.p_ready[x] : &sm.p_half[x], (uint32_t)(used[x] & 1), &sm.abort)) return false;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+                        for (int kk = half * 4; kk < half * 4 + 4; ++kk) {
+                            umma_f16_ts(tmem + 256 + x * 128, tmem + x * kPgKeys + kk * 8, vd + (uint64_t)(kk * (2048 >> 4)), idesc_pv,
+                                        !first || kk != 0);
+                        }
                     }
+                    ++used[x];
                     return true;
                 };
                 // The last Q.K^T of the piece lets go of Q, whoever issues it; a K or V stage is free behind its last user.
@@ -672,43 +688,17 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     corr = ex2_approx((m_ref - m_run) * to_log2);
                     m_ref = m_run;
                 }
-                const uint64_t scale2 = pair2(to_log2, to_log2), off2 = pair2(-m_ref * to_log2, -m_ref * to_log2);
-                uint64_t psum[2] = {0ull, 0ull};
-                auto exponents = [&](const uint32_t* v, uint32_t* pk) {
-#pragma unroll
-                    for (int c = 0; c < 16; ++c) {
-                        const float2 e = split2(fma2(pair2(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1])), scale2, off2));
-                        const float p0 = ex2_approx(e.x), p1 = ex2_approx(e.y);
-                        psum[c & 1] = add2(psum[c & 1], pair2(p0, p1));
-                        pk[c] = PgType<T>::pack(p0, p1);
-                    }
-                };
-                uint32_t pk[32];
-                exponents(v, pk);
-                exponents(v + 32, pk + 16);
-                tmem_ld32_async(t_s + 64, v);
-                tmem_ld32_async(t_s + 96, v + 32);
-                tmem_st32_async(t_s, pk);
-                tmem_ld_wait(v);
-                finish(v, 64);
-                finish(v + 32, 96);
-                exponents(v, pk);
-                exponents(v + 32, pk + 16);
-                tmem_st32_async(t_s + 32, pk);
-                const float2 ps = split2(add2(psum[0], psum[1]));
-                l_run = l_run * corr + (ps.x + ps.y);
                 // O under the new reference.  The P.V of the block before has completed: s_full was committed behind it.
                 if (!first && __any_sync(0xffffffffu, moves)) {
 #pragma unroll 1
-                    for (int c0 = 0; c0 < D; c0 += 32) {
-                        uint32_t o[32];
-                        tmem_ld32(t_o + (uint32_t)c0, o);
+                    for (int c0 = 0; c0 < D; c0 += 16) {
+                        uint32_t o[16];
+                        tmem_ld16(t_o + (uint32_t)c0, o);
 #pragma unroll
-                        for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * corr);
-                        tmem_st32_async(t_o + (uint32_t)c0, o);
+                        for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * corr);
+                        tmem_st16_async(t_o + (uint32_t)c0, o);
                     }
                 }
-                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 if (key0 < span.lo || key0 + kPgKeys > span.hi) {
                     // rows of V that nobody sees
                     const int entry = entry0 + pg_v_entry(j, p.blocks), stage = entry % kPgStages;
@@ -726,9 +716,39 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
+                const uint64_t scale2 = pair2(to_log2, to_log2), off2 = pair2(-m_ref * to_log2, -m_ref * to_log2);
+                uint64_t psum[2] = {0ull, 0ull};
+                auto exponents = [&](const uint32_t* v, uint32_t* pk) {
+#pragma unroll
+                    for (int c = 0; c < 16; ++c) {
+                        const float2 e = split2(fma2(pair2(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1])), scale2, off2));
+                        const float p0 = ex2_approx(e.x), p1 = ex2_approx(e.y);
+                        psum[c & 1] = add2(psum[c & 1], pair2(p0, p1));
+                        pk[c] = PgType<T>::pack(p0, p1);
+                    }
+                };
+                uint32_t pk[32];
+                exponents(v, pk);
+                exponents(v + 32, pk + 16);
+                tmem_ld32_async(t_s + 64, v);
+                tmem_ld32_async(t_s + 96, v + 32);
+                tmem_st32_async(t_s, pk);
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.p_half[x]);
+                tmem_ld_wait(v);
+                finish(v, 64);
+                finish(v + 32, 96);
+                exponents(v, pk);
+                exponents(v + 32, pk + 16);
+                tmem_st32_async(t_s + 32, pk);
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sm.p_ready[x]);
+                const float2 ps = split2(add2(psum[0], psum[1]));
+                l_run = l_run * corr + (ps.x + ps.y);
             }
             entry0 += 2 * p.blocks;
             if (!ok) break;
