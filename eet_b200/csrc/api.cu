@@ -56,6 +56,7 @@ static inline bool aligned16(const void* p)
 #include "glue.cu"
 #include "noalloc.cu"
 #include "paged_tc.cu"
+#include "paged_rows.cu"
 #include "paged.cu"
 #include "quantize.cu"
 

@@ -180,8 +180,4 @@ struct PagedMhaArgs {
 size_t paged_mha_workspace_bytes(const PagedMhaArgs& a);
 int launch_paged_mha(const PagedMhaArgs& a, cudaStream_t stream);
 
-// paged_tc.cu (tcgen05)
-size_t paged_mha_tc_workspace_bytes(const PagedMhaArgs& a);
-int launch_paged_mha_tc(const PagedMhaArgs& a, cudaStream_t stream);
-
 }  // namespace eet

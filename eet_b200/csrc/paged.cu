@@ -158,14 +158,79 @@ int launch_rotary(const RotaryArgs& a, bool store, cudaStream_t stream)
     return store ? launch_rotary_t<__half, true>(a, stream) : launch_rotary_t<__half, false>(a, stream);
 }
 
+// Which kernels serve a call.  Sequences of at most `few` new tokens are for the kernel of few rows (paged_rows.cu), the others
+// for that of 128-row tiles (paged_tc.cu); each takes any number of tokens where it is alone.
+struct PagedPlan {
+    int nr;              // rows of the first kernel: 16, 32, 64, or 0
+    int few;
+    bool tiles;          // whether the second one runs
+    bool whole[2];       // their tiles are not cut (no scratch, no second launch)
+    size_t bytes[2];     // scratch
+};
+
+static PagedPlan paged_plan(const PagedMhaArgs& a)
+{
+    PagedPlan p = {};
+    const int group = a.heads / a.kv_heads;
+    auto rows_for = [&](long long tokens) {
+        const long long rows = tokens * group;
+        return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 0;
+    };
+    p.nr = rows_for(a.max_tokens);
+    p.few = 0x7fffffff;
+    if (p.nr == 0) {
+        p.tiles = true;
+        // beside the longest: few tokens each?
+        const long long others = a.seqs - 1, rest = a.tokens - a.max_tokens;
+        if (others > 0) p.nr = rows_for((rest + others - 1) / others);
+        p.few = p.nr / group;
+    }
+    p.whole[0] = p.whole[1] = a.max_len <= kPgKeys;
+    if (p.nr > 0 && !p.whole[0]) p.bytes[0] = pg_scratch_bytes(sm_count(), p.nr, a.head_dim);
+    if (p.tiles && !p.whole[1]) p.bytes[1] = pg_scratch_bytes(sm_count(), 2 * kPgRows, a.head_dim);
+    return p;
+}
+
 size_t paged_mha_workspace_bytes(const PagedMhaArgs& a)
 {
-    return paged_mha_tc_workspace_bytes(a);
+    const PagedPlan p = paged_plan(a);
+    return p.bytes[0] + p.bytes[1];
+}
+
+template<typename T, int D>
+static int launch_paged_mha_t(const PagedMhaArgs& a, const PagedPlan& p, cudaStream_t stream)
+{
+    void* ws[2] = {a.ws, (char*)a.ws + p.bytes[0]};
+    int rc = 0;
+    if (p.nr == 16) rc = pg_launch_rows<T, D, 16>(a, ws[0], p.few, p.whole[0], stream);
+    if (p.nr == 32) rc = pg_launch_rows<T, D, 32>(a, ws[0], p.few, p.whole[0], stream);
+    if (p.nr == 64) rc = pg_launch_rows<T, D, 64>(a, ws[0], p.few, p.whole[0], stream);
+    if (rc) return rc;
+    if (p.tiles) {
+        const int least = p.nr > 0 ? p.few + 1 : 1;
+        // (the kernel without a bias takes the maximum of the scores before the scale, which a negative one would turn round)
+        rc = a.slopes != nullptr || !(a.scale > 0.f) ? pg_launch_tc<T, D, true>(a, ws[1], least, p.whole[1], stream)
+                                                     : pg_launch_tc<T, D, false>(a, ws[1], least, p.whole[1], stream);
+        if (rc) return rc;
+    }
+    PgScratch s[2] = {};
+    int n = 0;
+    if (p.bytes[0]) s[n++] = {ws[0], p.nr, 0};
+    if (p.bytes[1]) s[n++] = {ws[1], 2 * kPgRows, 1};
+    if (n > 0) {
+        const int y = p.bytes[1] ? 8 : p.nr * D / 4 / 256;
+        EET_CUDA(launch_pdl(paged_mha_join_kernel<T, D>, dim3(sm_count(), y < 1 ? 1 : y, n), dim3(256), 0, stream, a, s[0], s[1]));
+    }
+    return 0;
 }
 
 int launch_paged_mha(const PagedMhaArgs& a, cudaStream_t stream)
 {
-    return launch_paged_mha_tc(a, stream);
+    const PagedPlan p = paged_plan(a);
+    if (a.bf16) {
+        return a.head_dim == 128 ? launch_paged_mha_t<__nv_bfloat16, 128>(a, p, stream) : launch_paged_mha_t<__nv_bfloat16, 64>(a, p, stream);
+    }
+    return a.head_dim == 128 ? launch_paged_mha_t<__half, 128>(a, p, stream) : launch_paged_mha_t<__half, 64>(a, p, stream);
 }
 
 }  // namespace eet

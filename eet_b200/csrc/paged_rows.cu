@@ -1,0 +1,475 @@
+// Attention of few new tokens over a paged cache (decode steps, guessed tokens): up to 64 rows a kv head, a row being a (token,
+// query head) pair that shares it.
+//
+// Bound: HBM, the keys and values of every sequence once.  So that everything else fits behind that, the products are turned
+// round - keys and dims are the 128 rows of the tensor core's tile, the few query rows its columns:
+//   S^T [128 keys][NR] = K.Q^T       both K-major from shared memory
+//   O^T [dims][NR] += V^T.P^T        V as an MN-major A operand straight from its [key][dim] tile, P K-major from shared memory
+// (queries as the 128 rows, as in paged_tc.cu, spend an exponential on every one of 128 x 128 scores of which 1 to 64 rows count:
+// 64 sequences of 200 to 8000 tokens, 32 / 8 heads: 140 us, of which the transfer needs 81).
+//
+// One CTA per SM, its share of the work as paged_share.cuh says:
+//   warps 0-3  softmax: a thread per key = TMEM lane.  The powers are taken under a reference per row that all threads share; it
+//              moves only when a score has outgrown it by 2^8 (one vote of the 128 threads a block tells), so that no maximum
+//              crosses the threads in the usual block.  Sums stay with the threads until the end.
+//   warp 4     producer: Q, then K and V blocks of 128 keys through a ring of 32 KiB stages
+//   warp 5     one thread issues the products; scores and probabilities have two buffers, so that S of the next block is there when
+//              the softmax of this one ends
+// Keys that no row sees may be anything, even NaN: masked by selection, their rows of V set to zero before the product.
+#include "paged_share.cuh"
+
+namespace eet {
+
+namespace {
+
+constexpr int kPwThreads = 192;
+constexpr float kPwNone = -1e20f;   // reference of a row that has seen nothing
+
+template<int D, int NR>
+struct PwShape {
+    static constexpr int kHalves = D / 64;
+    static constexpr int kTile = kHalves * kPgKeys * 128;                    // a K or V block
+    static constexpr int kStages = D == 64 ? 8 : NR == 64 ? 5 : 6;
+    static constexpr int kQ = kHalves * NR * 128;                            // rows of Q; two of them
+    static constexpr int kP = 2 * NR * 128;                                  // probabilities [2 x 64 keys][NR]; two of them
+    static constexpr int kSmem = kStages * kTile + 2 * kQ + 2 * kP;
+    static constexpr uint32_t kTmemCols = NR == 16 ? 64 : 4 * NR;            // two S, one O
+};
+
+template<int NR>
+struct PwSmem {
+    uint64_t q_full[2], q_empty[2];
+    uint64_t full[8], empty[8];
+    uint64_t s_full[2];      // S^T of a block has been computed
+    uint64_t p_ready[2];     // its probabilities are there (four warps)
+    uint64_t pv_done[2];     // its V^T.P^T has completed
+    uint64_t o_free;         // O of a piece has been read (four warps)
+    uint32_t tmem_base;
+    volatile int abort;
+    int low[NR], high[NR];   // keys that a row sees
+    float slope[NR], ref[NR];
+    int pos[NR];
+    float warp_part[4][NR];
+    PgFound found;
+};
+
+// Barrier of the four softmax warps: whether any thread says so.
+__device__ __forceinline__ bool pw_any(bool p)
+{
+    uint32_t r;
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "bar.red.or.pred q, 1, 128, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t"
+        "}\n"
+        : "=r"(r)
+        : "r"((uint32_t)p)
+        : "memory");
+    return r != 0;
+}
+
+template<int NR>
+__device__ __forceinline__ void pw_tmem_ld(uint32_t taddr, float (&v)[NR])
+{
+    if constexpr (NR == 16) {
+        uint32_t u[16];
+        tmem_ld16(taddr, u);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(u[i]);
+    }
+    else {
+#pragma unroll
+        for (int c = 0; c < NR; c += 32) {
+            uint32_t u[32];
+            tmem_ld32(taddr + c, u);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[c + i] = __uint_as_float(u[i]);
+        }
+    }
+}
+
+template<typename T, int D, int NR>
+__global__ void __launch_bounds__(kPwThreads, 1)
+paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                      const __grid_constant__ CUtensorMap map_v, const __grid_constant__ PagedMhaArgs a, void* ws, int most, int whole)
+{
+    using Shape = PwShape<D, NR>;
+    constexpr int kHalves = Shape::kHalves, kTile = Shape::kTile, kStages = Shape::kStages, kHalf = kPgKeys * 128;
+    extern __shared__ __align__(1024) uint8_t pw_dyn[];
+    __shared__ PwSmem<NR> sm;
+    if (smem_u32(pw_dyn) & 1023) {   // the swizzle goes by addresses; the alignment above is there, so this does not happen
+        g_device_status = 2;
+        return;
+    }
+    uint8_t* ring = pw_dyn;
+    uint8_t* q_rows = ring + kStages * kTile;
+    uint8_t* p_rows = q_rows + 2 * Shape::kQ;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int group = a.heads / a.kv_heads;
+    const int tile_tokens = NR / group;
+    const PgTiling tiling = {tile_tokens, 1, most};
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sm.q_full[i], 1);
+            mbar_init(&sm.q_empty[i], 1);
+            mbar_init(&sm.s_full[i], 1);
+            mbar_init(&sm.p_ready[i], 4);
+            mbar_init(&sm.pv_done[i], 1);
+        }
+        for (int i = 0; i < kStages; ++i) {
+            mbar_init(&sm.full[i], 1);
+            mbar_init(&sm.empty[i], 1);
+        }
+        mbar_init(&sm.o_free, 4);
+        sm.abort = 0;
+        mbar_fence_init();
+    }
+    if (warp == 5) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)),
+                     "r"(Shape::kTmemCols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    pdl_launch_dependents();
+    pdl_wait();
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    PgShare share;
+    const bool work = pg_find_share(a, tiling, (int)blockIdx.x, (int)gridDim.x, whole != 0, sm.found, share);
+    const uint32_t tmem = sm.tmem_base;
+    const uint32_t tmem_o = tmem + 2 * NR;
+    if (!whole && threadIdx.x == 0) pg_write_header(a, tiling, ws, (int)blockIdx.x, work, share, sm.found);
+    PgPiece p;
+
+    if (!work) {
+    }
+    else if (warp == 4) {
+        // ------------------------------------------------------------------ producer
+        const long long cap = (long long)a.max_pages << a.page_shift;
+        int stage = 0, issued = 0, pieces = 0;
+        uint32_t phase = 1;                                       // of `empty`: the first round finds the stages free
+        bool ok = true;
+        while (ok && share.next(a, tiling, p)) {
+            if (p.blocks == 0) continue;
+            const PgSpan span = pg_span(a, p.s, p.tile * tile_tokens, (p.tile + 1) * tile_tokens);
+            const PgLoader<D> loader = {a, a.pages + p.seq * a.pages_stride, p.head, span};
+            int page = loader.page(p.block0 * kPgKeys), before = 0;
+            const int qb = pieces & 1;
+            if (pieces > 1 && !tc_wait_warp(&sm.q_empty[qb], (uint32_t)((pieces / 2 - 1) & 1), &sm.abort)) break;
+            ++pieces;
+            if (lane == 0) mbar_arrive_expect_tx(&sm.q_full[qb], (uint32_t)(tile_tokens * group * 128 * kHalves));
+            __syncwarp();
+            if (lane < kHalves) {
+                tma_load_3d(q_rows + qb * Shape::kQ + lane * NR * 128, &map_q, 64 * lane, p.head * group, p.s.row0 + p.tile * tile_tokens,
+                            &sm.q_full[qb]);
+            }
+            if (p.s.p0 + p.s.tokens > cap && lane == 0) g_device_status = 6;
+            auto put = [&](const CUtensorMap* map, int j, int page) -> bool {
+                if (!tc_wait_warp(&sm.empty[stage], phase, &sm.abort)) return false;
+                loader.load(map, (p.block0 + j) * kPgKeys, page, ring + stage * kTile, &sm.full[stage]);
+                ++issued;
+                if (++stage == kStages) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+                return true;
+            };
+            for (int j = 0; j <= p.blocks && ok; ++j) {
+                const int next = j + 1 < p.blocks ? loader.page((p.block0 + j + 1) * kPgKeys) : 0;
+                if (j < p.blocks) ok = put(&map_k, j, page);
+                if (j > 0 && ok) ok = put(&map_v, j - 1, before);
+                before = page;
+                page = next;
+            }
+        }
+        if (sm.abort) {
+            // nothing of this CTA may still be on its way when it ends
+            for (int e = max(0, issued - kStages); e < issued; ++e) {
+                mbar_wait_bounded(&sm.full[e % kStages], (uint32_t)((e / kStages) & 1));
+            }
+            for (int i = max(0, pieces - 2); i < pieces; ++i) mbar_wait_bounded(&sm.q_full[i & 1], (uint32_t)((i / 2) & 1));
+        }
+    }
+    else if (warp == 5) {
+        // ------------------------------------------------------------------ MMA issuer
+        if (elect_one()) {
+            constexpr uint32_t idesc_qk = umma_idesc_f16(kPgKeys, NR) | PgType<T>::idesc;
+            constexpr uint32_t idesc_pv = umma_idesc_f16(128, NR) | PgType<T>::idesc | (1u << 15);   // A (V^T) MN-major
+            const uint64_t q_desc = umma_desc_sw128(smem_u32(q_rows));
+            const uint64_t p_desc = umma_desc_sw128(smem_u32(p_rows));
+            const uint64_t k_desc = umma_desc_sw128(smem_u32(ring));
+            // (heads of 64: the tile's upper 64 rows read the same dims once more, nobody reads their sums)
+            const uint64_t v_desc = umma_desc_mn_sw128(smem_u32(ring), D == 128 ? (uint32_t)kHalf : 0u);
+            int pieces = 0;
+            int stage = 0;                  // loads are used in the order they are made
+            uint32_t phase = 0;
+            int qk = 0, pv = 0;             // blocks whose products have been issued
+            bool ok = true;
+            auto next_stage = [&]() {
+                umma_commit(&sm.empty[stage]);
+                if (++stage == kStages) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+            };
+            while (ok && share.next(a, tiling, p)) {
+                if (p.blocks == 0) continue;
+                const int n = p.blocks, qb = pieces & 1;
+                ok = tc_wait(&sm.q_full[qb], (uint32_t)((pieces / 2) & 1), &sm.abort);
+                if (!ok) break;
+                auto issue_qk = [&](int j) -> bool {
+                    if (!tc_wait(&sm.full[stage], phase, &sm.abort)) return false;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint64_t kd = k_desc + (uint64_t)(stage * (kTile >> 4)), qd = q_desc + (uint64_t)(qb * (Shape::kQ >> 4));
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; ++kk) {
+                        umma_f16(tmem + (uint32_t)((qk & 1) * NR), kd + (uint64_t)((kk >> 2) * (kHalf >> 4) + (kk & 3) * 2),
+                                 qd + (uint64_t)((kk >> 2) * (NR * 128 >> 4) + (kk & 3) * 2), idesc_qk, kk != 0);
+                    }
+                    umma_commit(&sm.s_full[qk & 1]);
+                    next_stage();
+                    if (j == n - 1) umma_commit(&sm.q_empty[qb]);
+                    ++qk;
+                    return true;
+                };
+                // S of block j + 2 goes where that of block j was, which has been read when its probabilities are there
+                ok = issue_qk(0) && (n == 1 || issue_qk(1));
+                if (ok && pieces > 0) ok = tc_wait(&sm.o_free, (uint32_t)((pieces - 1) & 1), &sm.abort);
+                for (int j = 0; j < n && ok; ++j) {
+                    ok = tc_wait(&sm.full[stage], phase, &sm.abort) && tc_wait(&sm.p_ready[pv & 1], (uint32_t)((pv >> 1) & 1), &sm.abort);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint64_t vd = v_desc + (uint64_t)(stage * (kTile >> 4)), pd = p_desc + (uint64_t)((pv & 1) * (Shape::kP >> 4));
+#pragma unroll
+                    for (int kk = 0; kk < kPgKeys / 16; ++kk) {
+                        umma_f16(tmem_o, vd + (uint64_t)(kk * (2048 >> 4)), pd + (uint64_t)((kk >> 2) * (NR * 128 >> 4) + (kk & 3) * 2),
+                                 idesc_pv, j != 0 || kk != 0);
+                    }
+                    umma_commit(&sm.pv_done[pv & 1]);
+                    next_stage();
+                    ++pv;
+                    if (j + 2 < n) ok = issue_qk(j + 2);
+                }
+                ++pieces;
+            }
+        }
+    }
+    else {
+        // ------------------------------------------------------------------ softmax, epilogue
+        const int r = warp * 32 + lane;                       // key of the block, and dim of O
+        const uint32_t t_lane = (uint32_t)(warp * 32) << 16;
+        const float log2e = 1.4426950408889634f;
+        const float to_log2 = a.scale * log2e;
+        const int cap = (int)min((long long)a.max_pages << a.page_shift, 0x7fffffffLL);
+        int stage = 0;                                        // of the loads, as the issuer counts them
+        uint32_t phase = 0;
+        int block = 0;                                        // blocks done
+        bool ok = true;
+        while (share.next(a, tiling, p)) {
+            const int token0 = p.tile * tile_tokens;
+            const int rows = min(tile_tokens, p.s.tokens - token0) * group;
+            const PgSpan span = pg_span(a, p.s, token0, token0 + tile_tokens);
+            // (everybody has left the piece before: its last barrier stands behind the last use of these)
+            if (r < NR) {
+                const int pos = p.s.p0 + token0 + r / group;
+                sm.pos[r] = pos;
+                sm.low[r] = a.window > 0 ? (int)max((long long)p.s.first, (long long)pos - a.window + 1) : p.s.first;
+                sm.high[r] = r < rows ? min(pos, cap - 1) : -1;
+                sm.slope[r] = a.slopes != nullptr && r < rows ? a.slopes[p.head * group + r % group] * log2e : 0.f;
+                sm.ref[r] = kPwNone;
+            }
+            pw_any(false);
+            // blocks all of whose keys every row sees
+            const int all_low = sm.low[rows - 1], all_high = sm.high[0];
+            float l[NR];
+#pragma unroll
+            for (int n = 0; n < NR; ++n) l[n] = 0.f;
+            for (int j = 0; j < p.blocks; ++j, ++block) {
+                const int key0 = (p.block0 + j) * kPgKeys, key = key0 + r;
+                const int buf = block & 1;
+                ok = tc_wait_warp(&sm.s_full[buf], (uint32_t)((block >> 1) & 1), &sm.abort);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                float t[NR];
+                pw_tmem_ld<NR>(tmem + t_lane + (uint32_t)(buf * NR), t);
+                if (a.slopes != nullptr) {
+#pragma unroll
+                    for (int n = 0; n < NR; ++n) t[n] = fmaf(t[n], to_log2, sm.slope[n] * (float)(key - sm.pos[n]));
+                }
+                else {
+#pragma unroll
+                    for (int n = 0; n < NR; ++n) t[n] *= to_log2;
+                }
+                if (all_low <= key0 && all_high >= key0 + kPgKeys - 1) {
+#pragma unroll
+                    for (int n = 0; n < NR; ++n) t[n] = n < rows ? t[n] : -INFINITY;
+                }
+                else {
+#pragma unroll
+                    for (int n = 0; n < NR; ++n) t[n] = key >= sm.low[n] && key <= sm.high[n] ? t[n] : -INFINITY;
+                }
+                bool over = j == 0;
+#pragma unroll
+                for (int n = 0; n < NR; ++n) over |= t[n] - sm.ref[n] > 8.0f;
+                // the buffer that the probabilities go to has been read by the product of two blocks before
+                if (block > 1) ok = tc_wait_warp(&sm.pv_done[buf], (uint32_t)(((block >> 1) - 1) & 1), &sm.abort) && ok;
+                const int v_entry = pg_v_entry(j, p.blocks);   // of the piece's loads
+                int v_stage = stage + v_entry;
+                uint32_t v_phase = phase;
+                while (v_stage >= kStages) {
+                    v_stage -= kStages;
+                    v_phase ^= 1;
+                }
+                const bool ragged = key0 < span.lo || key0 + kPgKeys > span.hi;
+                if (ragged) {
+                    // rows of V that nobody sees
+                    ok = tc_wait_warp(&sm.full[v_stage], v_phase, &sm.abort) && ok;
+                    if (key < span.lo || key >= span.hi) {
+                        uint4* dst = reinterpret_cast<uint4*>(ring + v_stage * kTile + r * 128);
+#pragma unroll
+                        for (int h = 0; h < kHalves; ++h) {
+#pragma unroll
+                            for (int c = 0; c < 8; ++c) dst[h * (kHalf / 16) + c] = make_uint4(0u, 0u, 0u, 0u);
+                        }
+                    }
+                }
+                if (pw_any(over || !ok)) {
+                    // Some row's reference moves (or a wait has run out: all leave together).
+                    if (j > 0) ok = tc_wait_warp(&sm.pv_done[buf ^ 1], (uint32_t)(((block - 1) >> 1) & 1), &sm.abort) && ok;
+#pragma unroll
+                    for (int n = 0; n < NR; ++n) {
+                        const float m = warp_max(t[n]);
+                        if (lane == 0) sm.warp_part[warp][n] = m;
+                    }
+                    if (pw_any(!ok)) {
+                        ok = false;
+                        break;
+                    }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    float corr[NR];
+#pragma unroll
+                    for (int n = 0; n < NR; ++n) {
+                        const float m = fmaxf(fmaxf(sm.warp_part[0][n], sm.warp_part[1][n]), fmaxf(sm.warp_part[2][n], sm.warp_part[3][n]));
+                        corr[n] = m - sm.ref[n] > 8.0f ? ex2_approx(sm.ref[n] - m) : 1.0f;
+                        l[n] *= corr[n];
+                    }
+                    if (j > 0) {
+                        float o[NR];
+                        pw_tmem_ld<NR>(tmem_o + t_lane, o);
+#pragma unroll
+                        for (int c = 0; c < NR; c += 16) {
+                            uint32_t u[16];
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(o[c + i] * corr[c + i]);
+                            tmem_st16_async(tmem_o + t_lane + (uint32_t)c, u);
+                        }
+                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    }
+                    pw_any(false);   // the references have been read
+                    if (r < NR) {
+                        const float m = fmaxf(fmaxf(sm.warp_part[0][r], sm.warp_part[1][r]), fmaxf(sm.warp_part[2][r], sm.warp_part[3][r]));
+                        if (m - sm.ref[r] > 8.0f) sm.ref[r] = m;
+                    }
+                    pw_any(false);
+                }
+                // probabilities: row n of P holds 64 keys in 128 bytes, 16-byte pieces swizzled by n
+                uint8_t* dst = p_rows + buf * Shape::kP + (r >> 6) * (NR * 128) + (r & 7) * 2;
+                const int piece = (r & 63) >> 3;
+#pragma unroll
+                for (int n = 0; n < NR; ++n) {
+                    const float e = ex2_approx(t[n] - sm.ref[n]);
+                    l[n] += e;
+                    *reinterpret_cast<T*>(dst + n * 128 + ((piece ^ (n & 7)) << 4)) = (T)e;
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.p_ready[buf]);
+            }
+            if (!ok) break;
+            stage += 2 * p.blocks;
+            phase ^= (uint32_t)((stage / kStages) & 1);
+            stage %= kStages;
+
+            // ---- epilogue
+#pragma unroll
+            for (int n = 0; n < NR; ++n) {
+                const float sum = warp_sum(l[n]);
+                if (lane == 0) sm.warp_part[warp][n] = sum;
+            }
+            if (p.blocks > 0) ok = tc_wait_warp(&sm.pv_done[(block - 1) & 1], (uint32_t)(((block - 1) >> 1) & 1), &sm.abort);
+            if (pw_any(!ok)) {
+                ok = false;
+                break;
+            }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const bool complete = p.starts && p.ends;
+            const PgPartial part = pg_partial(ws, (int)gridDim.x, (int)blockIdx.x, p.starts ? 1 : 0, NR, D);
+            if (!complete && r < NR) {
+                part.max2[r] = sm.ref[r];
+                part.sum[r] = sm.warp_part[0][r] + sm.warp_part[1][r] + sm.warp_part[2][r] + sm.warp_part[3][r];
+            }
+            float o[NR];
+            if (p.blocks > 0) {
+                pw_tmem_ld<NR>(tmem_o + t_lane, o);
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.o_free);
+            }
+            if (r < D) {
+                T* dst = (T*)a.out + (size_t)(p.s.row0 + token0) * a.o_tok + (size_t)(p.head * group) * a.o_head + r;
+                int g = 0;
+#pragma unroll
+                for (int n = 0; n < NR; ++n) {
+                    if (n < rows) {
+                        if (complete) {
+                            const float sum = sm.warp_part[0][n] + sm.warp_part[1][n] + sm.warp_part[2][n] + sm.warp_part[3][n];
+                            *dst = (T)(p.blocks > 0 && sum > 0.f ? o[n] / sum : 0.f);
+                            dst += a.o_head;
+                            if (++g == group) {
+                                g = 0;
+                                dst += a.o_tok - group * a.o_head;
+                            }
+                        }
+                        else if (p.blocks > 0) {
+                            reinterpret_cast<float*>(part.o)[n * D + r] = o[n];
+                        }
+                    }
+                }
+            }
+            pw_any(false);   // the sums have been read
+        }
+    }
+
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 5) {
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Shape::kTmemCols) : "memory");
+    }
+}
+
+template<typename T, int D, int NR>
+int pg_launch_rows(const PagedMhaArgs& a, void* ws, int most, int whole, cudaStream_t stream)
+{
+    CUtensorMap map_q, map_k, map_v;
+    if (int rc = pg_encode_maps<T, D>(a, NR / (a.heads / a.kv_heads), &map_q, &map_k, &map_v)) return rc;
+    auto kern = paged_mha_rows_kernel<T, D, NR>;
+    static bool attr_set[64] = {};
+    int dev = 0;
+    EET_CUDA(cudaGetDevice(&dev));
+    dev &= 63;
+    constexpr int kSmem = PwShape<D, NR>::kSmem;
+    if (!attr_set[dev]) {
+        EET_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+        attr_set[dev] = true;
+    }
+    EET_CUDA(launch_pdl(kern, dim3(sm_count()), dim3(kPwThreads), kSmem, stream, map_q, map_k, map_v, a, ws, most, whole));
+    return 0;
+}
+
+}  // namespace
+
+}  // namespace eet

@@ -1,0 +1,457 @@
+// What the kernels of the paged attention share: how the work is cut up, and how partial results are kept and added up.
+//
+// The work is all blocks of 128 keys of all tiles of all (sequence, kv head)s, laid out behind one another; every CTA gets an
+// equal, contiguous share of it, cut anywhere.  Each finds its share from starts and lens (pg_find_share), so that lengths live
+// on the device and a captured call serves others.  A tile that is cut leaves partial sums (O, maximum, sum) in the scratch, and
+// a second launch adds them up in a fixed order: the same bits every time.
+#pragma once
+#include <cuda.h>
+
+#include "common.cuh"
+#include "kernels.h"
+
+namespace eet {
+
+namespace {
+
+constexpr int kPgRows = 128;            // rows of a tile (paged_tc.cu)
+constexpr int kPgKeys = 128;            // keys of a block
+
+template<typename T>
+struct PgType;
+template<>
+struct PgType<__half> {
+    static constexpr uint32_t idesc = 0;
+    static constexpr CUtensorMapDataType tma = CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    static __device__ __forceinline__ uint32_t pack(float a, float b)
+    {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+};
+template<>
+struct PgType<__nv_bfloat16> {
+    static constexpr uint32_t idesc = (1u << 7) | (1u << 10);
+    static constexpr CUtensorMapDataType tma = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    static __device__ __forceinline__ uint32_t pack(float a, float b)
+    {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+};
+
+// ------------------------------------------------------------------------------------------------ the shares of the work
+
+struct PgSeq {
+    int row0, tokens;   // rows of q
+    int p0;             // position of the first of them
+    int first;          // first position that counts
+};
+
+// What a kernel works on: sequences with `least` to `most` new tokens, `tokens` of them to a tile (both tiles of a pair counted).
+struct PgTiling {
+    int tokens, least, most;
+    __device__ __forceinline__ int tiles(const PgSeq& s) const { return (s.tokens + tokens - 1) / tokens; }
+};
+
+__device__ __forceinline__ PgSeq pg_seq(const PagedMhaArgs& a, const PgTiling& g, int b)
+{
+    PgSeq s;
+    s.row0 = a.starts[b];
+    const int end = min(a.starts[b + 1], a.tokens);
+    s.tokens = s.row0 >= 0 ? max(0, end - s.row0) : 0;
+    s.p0 = a.lens[b] - s.tokens;
+    if (s.tokens < g.least || s.tokens > g.most) s.tokens = 0;
+    s.first = a.first_key != nullptr ? max(0, a.first_key[b]) : 0;
+    return s;
+}
+
+// The key blocks of tile t: keys [lo, hi) are seen by some row of it.
+struct PgSpan {
+    int lo, hi;
+    __device__ __forceinline__ int first_block() const { return lo / kPgKeys; }
+    __device__ __forceinline__ int blocks() const { return hi > lo ? (hi + kPgKeys - 1) / kPgKeys - lo / kPgKeys : 0; }
+};
+
+__device__ __forceinline__ PgSpan pg_span(const PagedMhaArgs& a, const PgSeq& s, int token0, int token1)
+{
+    PgSpan r;
+    const long long cap = (long long)a.max_pages << a.page_shift;
+    r.hi = (int)min((long long)s.p0 + min(token1, s.tokens), cap);
+    r.lo = s.first;
+    if (a.window > 0) r.lo = (int)max((long long)r.lo, (long long)s.p0 + token0 - a.window + 1);
+    return r;
+}
+
+struct PgPiece {
+    PgSeq s;
+    int seq, head, tile;
+    int block0, blocks;   // key blocks of it to be worked on; 0: its rows see nothing
+    bool starts, ends;    // whether those are its first, its last
+};
+
+// Walks the share of a CTA tile by tile.  All threads of a warp hold the same.
+struct PgShare {
+    long long left;       // blocks of the share still to come (a tile that sees nothing counts as one)
+    int seq, head, tile, at;
+    PgSeq s;
+    bool whole;           // tiles are not cut: the share has those that begin in it
+
+    __device__ __forceinline__ void step(const PagedMhaArgs& a, const PgTiling& g)
+    {
+        at = 0;
+        if (++tile < g.tiles(s)) return;
+        tile = 0;
+        if (++head < a.kv_heads) return;
+        head = 0;
+        do {
+            if (++seq >= a.seqs) {
+                left = 0;
+                return;
+            }
+            s = pg_seq(a, g, seq);
+        } while (s.tokens == 0);
+    }
+    __device__ __forceinline__ bool next(const PagedMhaArgs& a, const PgTiling& g, PgPiece& p)
+    {
+        while (left > 0) {
+            const PgSpan span = pg_span(a, s, tile * g.tokens, (tile + 1) * g.tokens);
+            const int n = span.blocks(), cost = max(1, n);
+            if (whole && at > 0) {   // it began in the share before
+                left -= cost - at;
+                step(a, g);
+                continue;
+            }
+            const int take = whole ? cost : (int)min(left, (long long)(cost - at));
+            p.s = s;
+            p.seq = seq;
+            p.head = head;
+            p.tile = tile;
+            p.block0 = span.first_block() + at;
+            p.blocks = n == 0 ? 0 : take;
+            p.starts = at == 0;
+            p.ends = at + take == cost;
+            left -= take;
+            at += take;
+            if (p.ends) step(a, g);
+            return true;
+        }
+        return false;
+    }
+};
+
+__device__ __forceinline__ long long pg_warp_scan(long long v)
+{
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long u = __shfl_up_sync(0xffffffffu, v, o);
+        if ((int)(threadIdx.x & 31) >= o) v += u;
+    }
+    return v;
+}
+
+// Blocks of all tiles of a kv head of the sequences that the lanes of a warp hold.  One with many tiles is added up by the warp.
+__device__ __forceinline__ long long pg_seq_blocks(const PagedMhaArgs& a, const PgTiling& g, const PgSeq& mine)
+{
+    const int tiles = g.tiles(mine);
+    long long sum = 0;
+    if (tiles <= 4) {
+        for (int t = 0; t < tiles; ++t) sum += max(1, pg_span(a, mine, t * g.tokens, (t + 1) * g.tokens).blocks());
+    }
+    uint32_t many = __ballot_sync(0xffffffffu, tiles > 4);
+    while (many) {
+        const int src = __ffs(many) - 1;
+        many &= many - 1;
+        PgSeq s;
+        s.row0 = 0;
+        s.tokens = __shfl_sync(0xffffffffu, mine.tokens, src);
+        s.p0 = __shfl_sync(0xffffffffu, mine.p0, src);
+        s.first = __shfl_sync(0xffffffffu, mine.first, src);
+        const int n = g.tiles(s);
+        long long part = 0;
+        for (int t = threadIdx.x & 31; t < n; t += 32) part += max(1, pg_span(a, s, t * g.tokens, (t + 1) * g.tokens).blocks());
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+        if ((int)(threadIdx.x & 31) == src) sum = part;
+    }
+    return sum;
+}
+
+struct PgFound {
+    long long warp_sum[12];
+    long long begin, end, total;
+    long long rest;        // of the share's begin, within its sequence
+    int seq, head, tile, at;
+    int ctas;              // that have a share
+};
+
+// The share of CTA `cta` of `ctas`, by all threads of the block.  Ends with a block-wide barrier; false: it has none.
+__device__ bool pg_find_share(const PagedMhaArgs& a, const PgTiling& g, int cta, int ctas, bool whole, PgFound& f, PgShare& share)
+{
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5;
+    long long total = 0;
+    for (int pass = 0; pass < 2; ++pass) {
+        long long before = 0;   // of the sequences of earlier rounds
+        for (int base = 0; base < a.seqs; base += (int)blockDim.x) {
+            PgSeq s = {0, 0, 0, 0};
+            if (base + tid < a.seqs) s = pg_seq(a, g, base + tid);
+            const long long cost = a.kv_heads * pg_seq_blocks(a, g, s);
+            const long long upto = pg_warp_scan(cost);
+            if (lane == 31) f.warp_sum[warp] = upto;
+            __syncthreads();
+            long long offset = before;
+            long long round = 0;
+            for (int w = 0; w < warps; ++w) {
+                if (w < warp) offset += f.warp_sum[w];
+                round += f.warp_sum[w];
+            }
+            before += round;
+            const bool last = base + (int)blockDim.x >= a.seqs;
+            if (pass == 0 && last) total = before;
+            // with one round the first pass knows all there is to know
+            if (pass == 1 || (last && base == 0)) {
+                const long long n = min((long long)ctas, total);
+                const long long begin = n > 0 && cta < n ? total * cta / n : total;
+                const long long start = offset + upto - cost;
+                if (start <= begin && begin < start + cost) {
+                    f.begin = begin;
+                    f.seq = base + tid;
+                    f.rest = begin - start;
+                }
+                if (pass == 0) pass = 1;
+            }
+            __syncthreads();
+        }
+    }
+    const long long n = min((long long)ctas, total);
+    if (cta >= n) return false;
+    const int seq = f.seq;
+    const PgSeq s = pg_seq(a, g, seq);
+    if (warp == 0) {
+        // the head and the tile within the sequence
+        const int tiles = g.tiles(s);
+        long long part = 0;
+        for (int t = lane; t < tiles; t += 32) part += max(1, pg_span(a, s, t * g.tokens, (t + 1) * g.tokens).blocks());
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+        const int head = (int)(f.rest / part);
+        long long rest = f.rest - head * part;
+        for (int t0 = 0; t0 < tiles; t0 += 32) {
+            const int t = t0 + lane;
+            const long long cost = t < tiles ? max(1, pg_span(a, s, t * g.tokens, (t + 1) * g.tokens).blocks()) : 0;
+            const long long upto = pg_warp_scan(cost);
+            if (upto - cost <= rest && rest < upto) {
+                f.head = head;
+                f.tile = t;
+                f.at = (int)(rest - (upto - cost));
+            }
+            const long long all = __shfl_sync(0xffffffffu, upto, 31);
+            if (rest < all) break;
+            rest -= all;
+        }
+    }
+    __syncthreads();
+    share.left = total * (cta + 1) / n - f.begin;
+    share.seq = seq;
+    share.head = f.head;
+    share.tile = f.tile;
+    share.at = f.at;
+    share.s = s;
+    share.whole = whole;
+    f.total = total;   // (the same from every thread)
+    f.ctas = (int)n;
+    return true;
+}
+
+// ------------------------------------------------------------------------------------------------ scratch
+// Per CTA a header of the piece that it begins with, and two partial results: of that piece where it continues a tile (0), and
+// of the piece that it ends with where that begins a tile and does not end it (1).  A partial result of R rows: the maximum (as a
+// power of two) and the sum of each, and O as float4 [R][D / 4], or for the 256 rows of a pair of tiles as [D / 4][R].
+struct PgHeader {
+    int kind;              // 0: nothing to add up; 1: the piece ends a tile that began in CTA `from`; 2: it neither begins nor ends one
+    int from;
+    int head;              // kv head
+    int row0, tokens;      // of q: of the tile
+    int pad[3];
+};
+
+__host__ __device__ constexpr size_t pg_partial_bytes(int rows, int head_dim)
+{
+    return (size_t)rows * (2 + head_dim) * sizeof(float);
+}
+
+__host__ __device__ constexpr size_t pg_scratch_bytes(int ctas, int rows, int head_dim)
+{
+    return ctas * (sizeof(PgHeader) + 2 * pg_partial_bytes(rows, head_dim));
+}
+
+struct PgPartial {
+    float *max2, *sum;
+    float4* o;
+};
+
+__device__ __forceinline__ PgPartial pg_partial(void* ws, int ctas, int cta, int which, int rows, int head_dim)
+{
+    float* at = reinterpret_cast<float*>((char*)ws + ctas * sizeof(PgHeader) + (2 * (size_t)cta + which) * pg_partial_bytes(rows, head_dim));
+    return {at, at + rows, reinterpret_cast<float4*>(at + 2 * rows)};
+}
+
+// The header of the CTA's share, written by one thread.
+__device__ __forceinline__ void pg_write_header(const PagedMhaArgs& a, const PgTiling& g, void* ws, int cta, bool work, const PgShare& share,
+                                                const PgFound& found)
+{
+    PgHeader h = {};
+    if (work && share.at > 0) {
+        const PgSpan span = pg_span(a, share.s, share.tile * g.tokens, (share.tile + 1) * g.tokens);
+        const long long begin = found.begin - share.at;   // of the tile
+        h.kind = share.at + share.left >= max(1, span.blocks()) ? 1 : 2;
+        h.from = (int)(((begin + 1) * found.ctas - 1) / found.total);
+        h.head = share.head;
+        h.row0 = share.s.row0 + share.tile * g.tokens;
+        h.tokens = min(g.tokens, share.s.tokens - share.tile * g.tokens);
+    }
+    reinterpret_cast<PgHeader*>(ws)[cta] = h;
+}
+
+struct PgScratch {
+    void* ws;
+    int rows;              // of a partial result; 0: none
+    int by_dim;            // O is [D / 4][rows], and a tile of 128 rows holds whole tokens only
+};
+
+// Adds up the partial results of the tiles that end in CTA blockIdx.x of one of the kernels (blockIdx.z), four dims of a row a
+// thread and turn.
+template<typename T, int D>
+__global__ void __launch_bounds__(256) paged_mha_join_kernel(const __grid_constant__ PagedMhaArgs a, PgScratch s0, PgScratch s1)
+{
+    pdl_wait();
+    const PgScratch s = blockIdx.z ? s1 : s0;
+    const PgHeader h = reinterpret_cast<const PgHeader*>(s.ws)[blockIdx.x];
+    if (h.kind != 1) return;
+    const int cta = blockIdx.x, ctas = gridDim.x;
+    const int group = a.heads / a.kv_heads;
+    const int rows = h.tokens * group;
+    const int per_tile = s.by_dim ? kPgRows / group * group : s.rows;   // rows of a tile in use
+    for (int i = (int)(blockIdx.y * blockDim.x + threadIdx.x); i < rows * (D / 4); i += (int)(gridDim.y * blockDim.x)) {
+        const int row = s.by_dim ? i % rows : i / (D / 4), d4 = s.by_dim ? i / rows : i % (D / 4);
+        const int at = s.by_dim ? row / per_tile * kPgRows + row % per_tile : row;
+        const size_t o_at = s.by_dim ? (size_t)d4 * s.rows + at : (size_t)at * (D / 4) + d4;
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll 4
+        for (int c = h.from; c <= cta; ++c) {
+            const PgPartial p = pg_partial(s.ws, ctas, c, c == h.from ? 1 : 0, s.rows, D);
+            const float l = p.sum[at], m = p.max2[at];
+            if (l > 0.f) top = fmaxf(top, m);
+        }
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int c = h.from; c <= cta; ++c) {
+            const PgPartial p = pg_partial(s.ws, ctas, c, c == h.from ? 1 : 0, s.rows, D);
+            const float l = p.sum[at], m = p.max2[at];
+            const float4 o = p.o[o_at];
+            if (l > 0.f) {   // (a piece that sees nothing has left no O)
+                const float w = ex2_approx(m - top);
+                sum += l * w;
+                acc.x += o.x * w;
+                acc.y += o.y * w;
+                acc.z += o.z * w;
+                acc.w += o.w * w;
+            }
+        }
+        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+        uint2 w;
+        w.x = PgType<T>::pack(acc.x * inv, acc.y * inv);
+        w.y = PgType<T>::pack(acc.z * inv, acc.w * inv);
+        T* dst = (T*)a.out + (size_t)(h.row0 + row / group) * a.o_tok + (size_t)(h.head * group + row % group) * a.o_head + 4 * d4;
+        *reinterpret_cast<uint2*>(dst) = w;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ keys and values
+
+__device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+            smem_u32(smem_dst)),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// The blocks of a piece on their way into the ring, by a whole warp: a lane per page and 64 dims.  Pages that hold none of the keys
+// that the tile sees are not asked for.
+template<int D>
+struct PgLoader {
+    static constexpr int kHalves = D / 64;
+    const PagedMhaArgs& a;
+    const int* row;      // the sequence's row of the page table
+    int head;
+    PgSpan span;
+
+    __device__ __forceinline__ int lane_key() const { return (int)(threadIdx.x & 31) / kHalves * min(1 << a.page_shift, kPgKeys); }
+    __device__ __forceinline__ bool mine(int key0) const
+    {
+        const int at = lane_key();
+        return at < kPgKeys && key0 + at < span.hi && key0 + at + min(1 << a.page_shift, kPgKeys) > span.lo;
+    }
+    // the page of this lane's keys of the block at key0
+    __device__ __forceinline__ int page(int key0) const { return mine(key0) ? row[(key0 + lane_key()) >> a.page_shift] : 0; }
+    __device__ __forceinline__ void load(const CUtensorMap* map, int key0, int page, uint8_t* stage, uint64_t* full) const
+    {
+        const int lane = threadIdx.x & 31, rows = min(1 << a.page_shift, kPgKeys), at = lane_key(), h = lane % kHalves;
+        const bool m = mine(key0);
+        const int count = __popc(__ballot_sync(0xffffffffu, m));
+        if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)(count * rows * 128));
+        __syncwarp();
+        if (m) {
+            if (page < 0 || page >= a.num_pages) {
+                g_device_status = 6;
+                page = a.num_pages;   // behind the last: reads as zeros
+            }
+            tma_load_4d(stage + h * (kPgKeys * 128) + at * 128, map, 64 * h, (key0 + at) & ((1 << a.page_shift) - 1), head, page, full);
+        }
+    }
+};
+
+// Where K and V of block j of a piece of n blocks stand in its order of loads: K0 K1 V0 K2 V1 ... K(n-1) V(n-2) V(n-1).
+__device__ __forceinline__ int pg_k_entry(int j) { return j == 0 ? 0 : 2 * j - 1; }
+__device__ __forceinline__ int pg_v_entry(int j, int n) { return j + 1 < n ? 2 * j + 2 : 2 * n - 1; }
+
+// [..][rows][values] of 16-bit values as boxes of 64 values (128 bytes, swizzled); dims and strides from the innermost.
+int pg_encode(CUtensorMap* map, CUtensorMapDataType type, const void* base, int rank, const long long* dims, const long long* strides,
+              const int* box)
+{
+    EncodeTiledFn encode = encode_tiled_fn();
+    EET_CHECK(encode != nullptr, "paged attention: cuTensorMapEncodeTiled is not available from the driver");
+    cuuint64_t d[4], st[3];
+    cuuint32_t bx[4], elem[4] = {1, 1, 1, 1};
+    for (int i = 0; i < rank; ++i) {
+        d[i] = (cuuint64_t)dims[i];
+        bx[i] = (cuuint32_t)box[i];
+        if (i > 0) st[i - 1] = (cuuint64_t)strides[i] * 2;
+    }
+    const CUresult rc = encode(map, type, (cuuint32_t)rank, const_cast<void*>(base), d, st, bx, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    EET_CHECK(rc == CUDA_SUCCESS, "paged attention: cuTensorMapEncodeTiled failed with code %d (strides too large or negative)", (int)rc);
+    return 0;
+}
+
+// Q as [token][head][dim] with boxes of `tokens` x the heads of a group, K and V as [page][head][slot][dim] with boxes of a page
+// (of 128 slots of a larger one).
+template<typename T, int D>
+int pg_encode_maps(const PagedMhaArgs& a, int tokens, CUtensorMap* q, CUtensorMap* k, CUtensorMap* v)
+{
+    const long long q_dims[3] = {D, a.heads, a.tokens}, q_str[3] = {1, a.q_head, a.q_tok};
+    const int q_box[3] = {64, a.heads / a.kv_heads, tokens};
+    if (int rc = pg_encode(q, PgType<T>::tma, a.q, 3, q_dims, q_str, q_box)) return rc;
+    const int page = 1 << a.page_shift;
+    const long long dims[4] = {D, page, a.kv_heads, a.num_pages};
+    const int box[4] = {64, page < kPgKeys ? page : kPgKeys, 1, 1};
+    const long long ks[4] = {1, a.kc_slot, a.kc_head, a.kc_page}, vs[4] = {1, a.vc_slot, a.vc_head, a.vc_page};
+    if (int rc = pg_encode(k, PgType<T>::tma, a.k_cache, 4, dims, ks, box)) return rc;
+    return pg_encode(v, PgType<T>::tma, a.v_cache, 4, dims, vs, box);
+}
+
+}  // namespace
+
+}  // namespace eet

@@ -8,9 +8,7 @@
 //   paired   a and b are neighbouring tiles of a long chunk and use the same key blocks
 //   split    there is only one tile (few new tokens): a takes its even key blocks, b its odd ones, merged at the end
 //
-// The work is all key blocks of all tiles of all (sequence, kv head)s, laid out behind one another; every CTA gets an equal,
-// contiguous share of it, cut anywhere.  Each finds its share from starts and lens (find_share), so lengths live on the device.
-// A tile that is cut leaves partial sums (O, maximum, sum) in the scratch and a second launch adds them up in a fixed order.
+// The work is cut up as paged_share.cuh says.
 //
 //   warps 0-3, 4-7  softmax of tile a / b: one thread per row = TMEM lane
 //   warp 8          producer: Q, then K and V blocks through a ring of five 32 KiB stages (order K0 K1 V0 K2 V1 ...), a lane
@@ -18,293 +16,16 @@
 //   warp 9          one thread issues S = Q.K^T and O += P.V (P from tensor memory, V as MN-major operand)
 // Keys outside of what any row of the pair sees may be anything, even NaN (slots behind the end of a sequence): their scores are
 // masked by selection and their rows of V are set to zero in shared memory before the product reads them.
-#include <cuda.h>
-
-#include "common.cuh"
-#include "kernels.h"
+#include "paged_share.cuh"
 
 namespace eet {
 
 namespace {
 
-constexpr int kPgRows = 128;            // rows of a tile
-constexpr int kPgKeys = 128;            // keys of a block
 constexpr int kPgThreads = 320;
 constexpr int kPgStages = 5;
 constexpr uint32_t kPgTmemCols = 512;   // S of a, S of b (their probabilities over them), O of a, O of b: 128 each
 constexpr float kPgNone = -1e20f;       // running maximum of a row that has seen nothing
-
-template<typename T>
-struct PgType;
-template<>
-struct PgType<__half> {
-    static constexpr uint32_t idesc = 0;
-    static constexpr CUtensorMapDataType tma = CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    static __device__ __forceinline__ uint32_t pack(float a, float b)
-    {
-        const __half2 h = __floats2half2_rn(a, b);
-        return *reinterpret_cast<const uint32_t*>(&h);
-    }
-};
-template<>
-struct PgType<__nv_bfloat16> {
-    static constexpr uint32_t idesc = (1u << 7) | (1u << 10);
-    static constexpr CUtensorMapDataType tma = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-    static __device__ __forceinline__ uint32_t pack(float a, float b)
-    {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-        return *reinterpret_cast<const uint32_t*>(&h);
-    }
-};
-
-// ------------------------------------------------------------------------------------------------ the shares of the work
-
-struct PgSeq {
-    int row0, tokens;   // rows of q
-    int p0;             // position of the first of them
-    int first;          // first position that counts
-};
-
-__device__ __forceinline__ PgSeq pg_seq(const PagedMhaArgs& a, int b)
-{
-    PgSeq s;
-    s.row0 = a.starts[b];
-    const int end = min(a.starts[b + 1], a.tokens);
-    s.tokens = s.row0 >= 0 ? max(0, end - s.row0) : 0;
-    s.p0 = a.lens[b] - s.tokens;
-    s.first = a.first_key != nullptr ? max(0, a.first_key[b]) : 0;
-    return s;
-}
-
-// The key blocks of tile t: keys [lo, hi) are seen by some row of it.
-struct PgSpan {
-    int lo, hi;
-    __device__ __forceinline__ int first_block() const { return lo / kPgKeys; }
-    __device__ __forceinline__ int blocks() const { return hi > lo ? (hi + kPgKeys - 1) / kPgKeys - lo / kPgKeys : 0; }
-};
-
-__device__ __forceinline__ PgSpan pg_span(const PagedMhaArgs& a, const PgSeq& s, int token0, int token1)
-{
-    PgSpan r;
-    const long long cap = (long long)a.max_pages << a.page_shift;
-    r.hi = (int)min((long long)s.p0 + min(token1, s.tokens), cap);
-    r.lo = s.first;
-    if (a.window > 0) r.lo = (int)max((long long)r.lo, (long long)s.p0 + token0 - a.window + 1);
-    return r;
-}
-
-struct PgPiece {
-    PgSeq s;
-    int seq, head, tile;
-    int block0, blocks;   // key blocks of it to be worked on; 0: its rows see nothing
-    bool starts, ends;    // whether those are its first, its last
-};
-
-// Walks the share of a CTA tile by tile.  All threads of a warp hold the same.
-struct PgShare {
-    long long left;       // blocks of the share still to come (a tile that sees nothing counts as one)
-    int seq, head, tile, at;
-    PgSeq s;
-    bool whole;           // tiles are not cut: the share has those that begin in it
-
-    __device__ __forceinline__ int tiles(int pair_tokens) const { return (s.tokens + pair_tokens - 1) / pair_tokens; }
-    __device__ __forceinline__ void step(const PagedMhaArgs& a, int pair_tokens)
-    {
-        at = 0;
-        if (++tile < tiles(pair_tokens)) return;
-        tile = 0;
-        if (++head < a.kv_heads) return;
-        head = 0;
-        do {
-            if (++seq >= a.seqs) {
-                left = 0;
-                return;
-            }
-            s = pg_seq(a, seq);
-        } while (s.tokens == 0);
-    }
-    __device__ __forceinline__ bool next(const PagedMhaArgs& a, int pair_tokens, PgPiece& p)
-    {
-        while (left > 0) {
-            const PgSpan span = pg_span(a, s, tile * pair_tokens, (tile + 1) * pair_tokens);
-            const int n = span.blocks(), cost = max(1, n);
-            if (whole && at > 0) {   // it began in the share before
-                left -= cost - at;
-                step(a, pair_tokens);
-                continue;
-            }
-            const int take = whole ? cost : (int)min(left, (long long)(cost - at));
-            p.s = s;
-            p.seq = seq;
-            p.head = head;
-            p.tile = tile;
-            p.block0 = span.first_block() + at;
-            p.blocks = n == 0 ? 0 : take;
-            p.starts = at == 0;
-            p.ends = at + take == cost;
-            left -= take;
-            at += take;
-            if (p.ends) step(a, pair_tokens);
-            return true;
-        }
-        return false;
-    }
-};
-
-__device__ __forceinline__ long long pg_warp_scan(long long v)
-{
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long u = __shfl_up_sync(0xffffffffu, v, o);
-        if ((int)(threadIdx.x & 31) >= o) v += u;
-    }
-    return v;
-}
-
-// Blocks of all tiles of a kv head of the sequences that the lanes of a warp hold.  One with many tiles is added up by the warp.
-__device__ __forceinline__ long long pg_seq_blocks(const PagedMhaArgs& a, const PgSeq& mine, int pair_tokens)
-{
-    const int tiles = (mine.tokens + pair_tokens - 1) / pair_tokens;
-    long long sum = 0;
-    if (tiles <= 4) {
-        for (int t = 0; t < tiles; ++t) sum += max(1, pg_span(a, mine, t * pair_tokens, (t + 1) * pair_tokens).blocks());
-    }
-    uint32_t many = __ballot_sync(0xffffffffu, tiles > 4);
-    while (many) {
-        const int src = __ffs(many) - 1;
-        many &= many - 1;
-        PgSeq s;
-        s.row0 = 0;
-        s.tokens = __shfl_sync(0xffffffffu, mine.tokens, src);
-        s.p0 = __shfl_sync(0xffffffffu, mine.p0, src);
-        s.first = __shfl_sync(0xffffffffu, mine.first, src);
-        const int n = (s.tokens + pair_tokens - 1) / pair_tokens;
-        long long part = 0;
-        for (int t = threadIdx.x & 31; t < n; t += 32) part += max(1, pg_span(a, s, t * pair_tokens, (t + 1) * pair_tokens).blocks());
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-        if ((int)(threadIdx.x & 31) == src) sum = part;
-    }
-    return sum;
-}
-
-struct PgFound {
-    long long warp_sum[32];
-    long long begin, end, total;
-    long long rest;        // of the share's begin, within its sequence
-    int seq, head, tile, at;
-    int ctas;              // that have a share
-};
-
-// The share of CTA `cta` of `ctas`, by all threads of the block.  Ends with a block-wide barrier; false: it has none.
-__device__ bool pg_find_share(const PagedMhaArgs& a, int pair_tokens, int cta, int ctas, bool whole, PgFound& f, PgShare& share)
-{
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5;
-    long long total = 0;
-    for (int pass = 0; pass < 2; ++pass) {
-        long long before = 0;   // of the sequences of earlier rounds
-        for (int base = 0; base < a.seqs; base += (int)blockDim.x) {
-            PgSeq s = {0, 0, 0, 0};
-            if (base + tid < a.seqs) s = pg_seq(a, base + tid);
-            const long long cost = a.kv_heads * pg_seq_blocks(a, s, pair_tokens);
-            const long long upto = pg_warp_scan(cost);
-            if (lane == 31) f.warp_sum[warp] = upto;
-            __syncthreads();
-            long long offset = before;
-            long long round = 0;
-            for (int w = 0; w < warps; ++w) {
-                if (w < warp) offset += f.warp_sum[w];
-                round += f.warp_sum[w];
-            }
-            before += round;
-            const bool last = base + (int)blockDim.x >= a.seqs;
-            if (pass == 0 && last) total = before;
-            // with one round the first pass knows all there is to know
-            if (pass == 1 || (last && base == 0)) {
-                const long long n = min((long long)ctas, total);
-                const long long begin = n > 0 && cta < n ? total * cta / n : total;
-                const long long start = offset + upto - cost;
-                if (start <= begin && begin < start + cost) {
-                    f.begin = begin;
-                    f.seq = base + tid;
-                    f.rest = begin - start;
-                }
-                if (pass == 0) pass = 1;
-            }
-            __syncthreads();
-        }
-    }
-    const long long n = min((long long)ctas, total);
-    if (cta >= n) return false;
-    const int seq = f.seq;
-    const PgSeq s = pg_seq(a, seq);
-    if (warp == 0) {
-        // the head and the tile within the sequence
-        const int tiles = (s.tokens + pair_tokens - 1) / pair_tokens;
-        long long part = 0;
-        for (int t = lane; t < tiles; t += 32) part += max(1, pg_span(a, s, t * pair_tokens, (t + 1) * pair_tokens).blocks());
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-        const int head = (int)(f.rest / part);
-        long long rest = f.rest - head * part;
-        for (int t0 = 0; t0 < tiles; t0 += 32) {
-            const int t = t0 + lane;
-            const long long cost = t < tiles ? max(1, pg_span(a, s, t * pair_tokens, (t + 1) * pair_tokens).blocks()) : 0;
-            const long long upto = pg_warp_scan(cost);
-            if (upto - cost <= rest && rest < upto) {
-                f.head = head;
-                f.tile = t;
-                f.at = (int)(rest - (upto - cost));
-            }
-            const long long all = __shfl_sync(0xffffffffu, upto, 31);
-            if (rest < all) break;
-            rest -= all;
-        }
-    }
-    __syncthreads();
-    share.left = total * (cta + 1) / n - f.begin;
-    share.seq = seq;
-    share.head = f.head;
-    share.tile = f.tile;
-    share.at = f.at;
-    share.s = s;
-    share.whole = whole;
-    f.total = total;   // (the same from every thread)
-    f.ctas = (int)n;
-    return true;
-}
-
-// ------------------------------------------------------------------------------------------------ scratch
-// Per CTA a header of the piece that it begins with, and two partial results: of that piece where it continues a tile (0), and
-// of the piece that it ends with where that begins a tile and does not end it (1).  A partial result: per tile a / b the maximum
-// (as a power of two) and the sum of its 128 rows, and O as [dim / 4][row][4].
-struct PgHeader {
-    int kind;         // 0: nothing to add up; 1: the piece ends a tile that began in CTA `from`; 2: it neither begins nor ends one
-    int seq, head, tile, from;
-    int pad[3];
-};
-
-template<int D>
-struct PgPartial {
-    float max2[2][kPgRows], sum[2][kPgRows];
-    float4 o[2][D / 4][kPgRows];
-};
-
-__host__ __device__ constexpr size_t pg_partial_bytes(int head_dim)
-{
-    return (size_t)2 * kPgRows * (2 + head_dim) * sizeof(float);
-}
-
-size_t pg_scratch_bytes(int ctas, int head_dim)
-{
-    return ctas * (sizeof(PgHeader) + 2 * pg_partial_bytes(head_dim));
-}
-
-template<int D>
-__device__ __forceinline__ PgPartial<D>* pg_partial(void* ws, int ctas, int cta, int which)
-{
-    return reinterpret_cast<PgPartial<D>*>((char*)ws + ctas * sizeof(PgHeader)) + (2 * (size_t)cta + which);
-}
 
 // ------------------------------------------------------------------------------------------------ the kernel
 
@@ -331,21 +52,6 @@ __device__ __forceinline__ void tmem_st16_async(uint32_t taddr, const uint32_t (
         "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
         "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
         : "memory");
-}
-
-__device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar)
-{
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
-            smem_u32(smem_dst)),
-        "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
-        : "memory");
-}
-
-// Entry of the ring, counted from the piece's first, that holds V of its block j of n (K of block j > 0: 2 j - 1).
-__device__ __forceinline__ int pg_v_entry(int j, int n)
-{
-    return j + 1 < n ? 2 * j + 2 : 2 * n - 1;
 }
 
 // The blocks of a piece that tile x (0: a, 1: b) works on: first, first + stride, ... below end (block numbers of the piece).
@@ -375,7 +81,7 @@ __device__ __forceinline__ PgTurns pg_turns(const PagedMhaArgs& a, const PgPiece
 template<typename T, int D, bool kBias>
 __global__ void __launch_bounds__(kPgThreads, 1)
 paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                    const __grid_constant__ CUtensorMap map_v, const __grid_constant__ PagedMhaArgs a, int whole)
+                    const __grid_constant__ CUtensorMap map_v, const __grid_constant__ PagedMhaArgs a, void* ws, int least, int whole)
 {
     constexpr int kHalves = D / 64;
     constexpr int kHalf = kPgRows * 128;         // bytes of [128 rows][64 values], swizzled
@@ -387,6 +93,7 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int group = a.heads / a.kv_heads;
     const int tile_tokens = kPgRows / group, pair_tokens = 2 * tile_tokens;
+    const PgTiling tiling = {pair_tokens, least, 0x7fffffff};
 
     if (threadIdx.x == 0) {
         mbar_init(&sm.q_full, 1);
@@ -418,36 +125,20 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     PgShare share;
-    const bool work = pg_find_share(a, pair_tokens, (int)blockIdx.x, (int)gridDim.x, whole != 0, sm.found, share);
+    const bool work = pg_find_share(a, tiling, (int)blockIdx.x, (int)gridDim.x, whole != 0, sm.found, share);
     const uint32_t tmem = sm.tmem_base;
-    PgHeader* header = reinterpret_cast<PgHeader*>(a.ws) + blockIdx.x;
-    if (!whole && threadIdx.x == 0) {
-        PgHeader h = {};
-        if (work && share.at > 0) {
-            const PgSpan span = pg_span(a, share.s, share.tile * pair_tokens, (share.tile + 1) * pair_tokens);
-            const long long begin = sm.found.begin - share.at;   // of the tile
-            h.kind = share.at + share.left >= max(1, span.blocks()) ? 1 : 2;
-            h.seq = share.seq;
-            h.head = share.head;
-            h.tile = share.tile;
-            h.from = (int)(((begin + 1) * sm.found.ctas - 1) / sm.found.total);
-        }
-        *header = h;
-    }
+    if (!whole && threadIdx.x == 0) pg_write_header(a, tiling, ws, (int)blockIdx.x, work, share, sm.found);
     PgPiece p;
 
     if (!work) {
     }
     else if (warp == 8) {
         // ------------------------------------------------------------------ producer
-        const int page_rows = min(1 << a.page_shift, kPgKeys);
-        const int boxes = kPgKeys / page_rows * kHalves;          // 1 to 16: a lane each
-        const uint32_t box_bytes = (uint32_t)(page_rows * 128);
         const long long cap = (long long)a.max_pages << a.page_shift;
         int stage = 0, issued = 0, pieces = 0;
         uint32_t phase = 1;                                       // of `empty`: the first round finds the stages free
         bool ok = true;
-        while (ok && share.next(a, pair_tokens, p)) {
+        while (ok && share.next(a, tiling, p)) {
             if (p.blocks == 0) continue;
             const PgSpan span = pg_span(a, p.s, p.tile * pair_tokens, (p.tile + 1) * pair_tokens);
             if (pieces > 0 && !tc_wait_warp(&sm.q_empty, (uint32_t)((pieces - 1) & 1), &sm.abort)) break;
@@ -463,37 +154,24 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                             &sm.q_full);
             }
             if (p.s.p0 + p.s.tokens > cap && lane == 0) g_device_status = 6;
-            const int* row = a.pages + p.seq * a.pages_stride;
-            for (int e = 0; e < 2 * p.blocks; ++e) {
-                // K0 K1 V0 K2 V1 ... V(n-1)
-                const bool is_k = e == 0 || ((e & 1) && e != 2 * p.blocks - 1);
-                const int j = is_k ? (e + 1) / 2 : (e == 2 * p.blocks - 1 ? p.blocks - 1 : e / 2 - 1);
-                const int key0 = (p.block0 + j) * kPgKeys + lane / kHalves * page_rows;
-                const bool mine = lane < boxes && key0 < span.hi && key0 + page_rows > span.lo;   // no page without a need for it
-                int page = 0;
-                if (mine) {
-                    page = row[key0 >> a.page_shift];
-                    if (page < 0 || page >= a.num_pages) {
-                        g_device_status = 6;
-                        page = a.num_pages;   // behind the last: reads as zeros
-                    }
-                }
-                const int count = __popc(__ballot_sync(0xffffffffu, mine));
-                if (!tc_wait_warp(&sm.empty[stage], phase, &sm.abort)) {
-                    ok = false;
-                    break;
-                }
-                if (lane == 0) mbar_arrive_expect_tx(&sm.full[stage], count * box_bytes);
-                __syncwarp();
-                if (mine) {
-                    tma_load_4d(ring + stage * kTile + (lane % kHalves) * kHalf + lane / kHalves * page_rows * 128, is_k ? &map_k : &map_v,
-                                64 * (lane % kHalves), key0 & ((1 << a.page_shift) - 1), p.head, page, &sm.full[stage]);
-                }
+            const PgLoader<D> loader = {a, a.pages + p.seq * a.pages_stride, p.head, span};
+            auto put = [&](const CUtensorMap* map, int j, int page) -> bool {
+                if (!tc_wait_warp(&sm.empty[stage], phase, &sm.abort)) return false;
+                loader.load(map, (p.block0 + j) * kPgKeys, page, ring + stage * kTile, &sm.full[stage]);
                 ++issued;
                 if (++stage == kPgStages) {
                     stage = 0;
                     phase ^= 1;
                 }
+                return true;
+            };
+            int page = loader.page(p.block0 * kPgKeys), before = 0;
+            for (int j = 0; j <= p.blocks && ok; ++j) {
+                const int next = j + 1 < p.blocks ? loader.page((p.block0 + j + 1) * kPgKeys) : 0;
+                if (j < p.blocks) ok = put(&map_k, j, page);
+                if (j > 0 && ok) ok = put(&map_v, j - 1, before);
+                before = page;
+                page = next;
             }
         }
         if (sm.abort) {
@@ -521,7 +199,7 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 // (entries are waited for in any order within the ring's length)
                 return tc_wait(&sm.full[entry % kPgStages], (uint32_t)((entry / kPgStages) & 1), &sm.abort);
             };
-            while (ok && share.next(a, pair_tokens, p)) {
+            while (ok && share.next(a, tiling, p)) {
                 if (p.blocks == 0) continue;
                 const bool split = p.s.tokens - p.tile * pair_tokens <= tile_tokens;
                 const PgTurns turns[2] = {pg_turns(a, p, tile_tokens, 0), pg_turns(a, p, tile_tokens, 1)};
@@ -529,7 +207,7 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 ok = tc_wait(&sm.q_full, (uint32_t)(pieces & 1), &sm.abort);
                 ++pieces;
                 if (!ok) break;
-                auto k_entry = [&](int j) { return entry0 + (j == 0 ? 0 : 2 * j - 1); };
+                auto k_entry = [&](int j) { return entry0 + pg_k_entry(j); };
                 auto v_entry = [&](int j) { return entry0 + pg_v_entry(j, n); };
                 auto active = [&](int x, int j) { return j >= turns[x].first && j < turns[x].end; };
                 auto issue_qk = [&](int x, int j) -> bool {
@@ -614,7 +292,7 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         const int cap = (int)min((long long)a.max_pages << a.page_shift, 0x7fffffffLL);
         int entry0 = 0, used = 0, outs = 0, merges = 0;
         bool ok = true;
-        while (ok && share.next(a, pair_tokens, p)) {
+        while (ok && share.next(a, tiling, p)) {
             const int token0 = p.tile * pair_tokens;
             const bool split = p.s.tokens - token0 <= tile_tokens;
             const int token = token0 + (split ? 0 : x * tile_tokens) + tok;      // of the sequence
@@ -789,15 +467,15 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 l_run = l_run * scale_a + sm.b_sum[r] * scale_b;
             }
             const bool complete = p.starts && p.ends;
-            PgPartial<D>* part = pg_partial<D>(a.ws, (int)gridDim.x, (int)blockIdx.x, p.starts ? 1 : 0);
+            const PgPartial part = pg_partial(ws, (int)gridDim.x, (int)blockIdx.x, p.starts ? 1 : 0, 2 * kPgRows, D);
             if (complete) {
                 const float inv = l_run > 0.f ? 1.0f / l_run : 0.f;
                 scale_a *= inv;
                 scale_b *= inv;
             }
             else {
-                part->max2[x][r] = max2;
-                part->sum[x][r] = l_run;
+                part.max2[x * kPgRows + r] = max2;
+                part.sum[x * kPgRows + r] = l_run;
             }
             T* dst = (T*)a.out + (size_t)(p.s.row0 + token) * a.o_tok + (size_t)head * a.o_head;
             if (!mine && complete && valid) {
@@ -821,8 +499,8 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     if (!complete) {
 #pragma unroll
                         for (int c = 0; c < 32; c += 4) {
-                            part->o[x][(c0 + c) / 4][r] = make_float4(__uint_as_float(o[c]), __uint_as_float(o[c + 1]),
-                                                                      __uint_as_float(o[c + 2]), __uint_as_float(o[c + 3]));
+                            part.o[(c0 + c) / 4 * 2 * kPgRows + x * kPgRows + r] = make_float4(
+                                __uint_as_float(o[c]), __uint_as_float(o[c + 1]), __uint_as_float(o[c + 2]), __uint_as_float(o[c + 3]));
                         }
                     }
                     else if (valid) {
@@ -855,95 +533,12 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     }
 }
 
-// Adds up the partial results of the tile that ends in CTA blockIdx.x of the kernel above: 32 dims (blockIdx.y) of tile a or b
-// (blockIdx.z), a row a thread.
-template<typename T, int D>
-__global__ void __launch_bounds__(kPgRows) paged_mha_join_kernel(const __grid_constant__ PagedMhaArgs a)
-{
-    pdl_wait();
-    const PgHeader h = reinterpret_cast<const PgHeader*>(a.ws)[blockIdx.x];
-    if (h.kind != 1) return;
-    const int x = blockIdx.z, r = threadIdx.x, cta = blockIdx.x, ctas = gridDim.x;
-    const int group = a.heads / a.kv_heads, tile_tokens = kPgRows / group;
-    const PgSeq s = pg_seq(a, h.seq);
-    const int token0 = 2 * h.tile * tile_tokens;
-    if (x == 1 && s.tokens - token0 <= tile_tokens) return;
-    const int tok = r / group, token = token0 + x * tile_tokens + tok;
-    if (tok >= tile_tokens || token >= s.tokens) return;
-    float top = -INFINITY, sum = 0.f;
-    for (int c = h.from; c <= cta; ++c) {
-        const PgPartial<D>* p = pg_partial<D>(a.ws, ctas, c, c == h.from ? 1 : 0);
-        if (p->sum[x][r] > 0.f) top = fmaxf(top, p->max2[x][r]);
-    }
-    float4 acc[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int c = h.from; c <= cta; ++c) {
-        const PgPartial<D>* p = pg_partial<D>(a.ws, ctas, c, c == h.from ? 1 : 0);
-        const float l = p->sum[x][r];
-        if (!(l > 0.f)) continue;
-        const float w = ex2_approx(p->max2[x][r] - top);
-        sum += l * w;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float4 o = p->o[x][blockIdx.y * 8 + i][r];
-            acc[i].x += o.x * w;
-            acc[i].y += o.y * w;
-            acc[i].z += o.z * w;
-            acc[i].w += o.w * w;
-        }
-    }
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
-    T* dst = (T*)a.out + (size_t)(s.row0 + token) * a.o_tok + (size_t)(h.head * group + r - tok * group) * a.o_head + 32 * blockIdx.y;
-#pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-        uint4 w;
-        w.x = PgType<T>::pack(acc[i].x * inv, acc[i].y * inv);
-        w.y = PgType<T>::pack(acc[i].z * inv, acc[i].w * inv);
-        w.z = PgType<T>::pack(acc[i + 1].x * inv, acc[i + 1].y * inv);
-        w.w = PgType<T>::pack(acc[i + 1].z * inv, acc[i + 1].w * inv);
-        *reinterpret_cast<uint4*>(dst + 4 * i) = w;
-    }
-}
-
-// [..][rows][values] of 16-bit values as boxes of 64 values (128 bytes, swizzled); dims and strides from the innermost.
-int pg_encode(CUtensorMap* map, CUtensorMapDataType type, const void* base, int rank, const long long* dims, const long long* strides,
-              const int* box)
-{
-    EncodeTiledFn encode = encode_tiled_fn();
-    EET_CHECK(encode != nullptr, "paged attention: cuTensorMapEncodeTiled is not available from the driver");
-    cuuint64_t d[4], st[3];
-    cuuint32_t bx[4], elem[4] = {1, 1, 1, 1};
-    for (int i = 0; i < rank; ++i) {
-        d[i] = (cuuint64_t)dims[i];
-        bx[i] = (cuuint32_t)box[i];
-        if (i > 0) st[i - 1] = (cuuint64_t)strides[i] * 2;
-    }
-    const CUresult rc = encode(map, type, (cuuint32_t)rank, const_cast<void*>(base), d, st, bx, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    EET_CHECK(rc == CUDA_SUCCESS, "paged attention: cuTensorMapEncodeTiled failed with code %d (strides too large or negative)", (int)rc);
-    return 0;
-}
-
 template<typename T, int D, bool kBias>
-int pg_launch(const PagedMhaArgs& a, cudaStream_t stream)
+int pg_launch_tc(const PagedMhaArgs& a, void* ws, int least, int whole, cudaStream_t stream)
 {
     constexpr int kSmem = (2 + kPgStages) * (D / 64) * kPgRows * 128 + 1024;
-    const int group = a.heads / a.kv_heads;
     CUtensorMap map_q, map_k, map_v;
-    {
-        const long long dims[3] = {D, a.heads, a.tokens}, strides[3] = {1, a.q_head, a.q_tok};
-        const int box[3] = {64, group, kPgRows / group};
-        if (int rc = pg_encode(&map_q, PgType<T>::tma, a.q, 3, dims, strides, box)) return rc;
-    }
-    {
-        const long long dims[4] = {D, 1ll << a.page_shift, a.kv_heads, a.num_pages};
-        const int page_rows = (1 << a.page_shift) < kPgKeys ? (1 << a.page_shift) : kPgKeys;
-        const int box[4] = {64, page_rows, 1, 1};
-        const long long ks[4] = {1, a.kc_slot, a.kc_head, a.kc_page}, vs[4] = {1, a.vc_slot, a.vc_head, a.vc_page};
-        if (int rc = pg_encode(&map_k, PgType<T>::tma, a.k_cache, 4, dims, ks, box)) return rc;
-        if (int rc = pg_encode(&map_v, PgType<T>::tma, a.v_cache, 4, dims, vs, box)) return rc;
-    }
+    if (int rc = pg_encode_maps<T, D>(a, kPgRows / (a.heads / a.kv_heads), &map_q, &map_k, &map_v)) return rc;
     auto kern = paged_mha_tc_kernel<T, D, kBias>;
     static bool attr_set[64] = {};
     int dev = 0;
@@ -953,30 +548,10 @@ int pg_launch(const PagedMhaArgs& a, cudaStream_t stream)
         EET_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
         attr_set[dev] = true;
     }
-    // sequences of one block have nothing to cut
-    const int whole = a.max_len <= kPgKeys;
-    const int ctas = sm_count();
-    EET_CUDA(launch_pdl(kern, dim3(ctas), dim3(kPgThreads), kSmem, stream, map_q, map_k, map_v, a, whole));
-    if (!whole) EET_CUDA(launch_pdl(paged_mha_join_kernel<T, D>, dim3(ctas, D / 32, 2), dim3(kPgRows), 0, stream, a));
+    EET_CUDA(launch_pdl(kern, dim3(sm_count()), dim3(kPgThreads), kSmem, stream, map_q, map_k, map_v, a, ws, least, whole));
     return 0;
 }
 
 }  // namespace
-
-size_t paged_mha_tc_workspace_bytes(const PagedMhaArgs& a)
-{
-    return pg_scratch_bytes(sm_count(), a.head_dim);
-}
-
-int launch_paged_mha_tc(const PagedMhaArgs& a, cudaStream_t stream)
-{
-    const bool bias = a.slopes != nullptr || !(a.scale > 0.f);
-    if (a.bf16) {
-        if (a.head_dim == 128) return bias ? pg_launch<__nv_bfloat16, 128, true>(a, stream) : pg_launch<__nv_bfloat16, 128, false>(a, stream);
-        return bias ? pg_launch<__nv_bfloat16, 64, true>(a, stream) : pg_launch<__nv_bfloat16, 64, false>(a, stream);
-    }
-    if (a.head_dim == 128) return bias ? pg_launch<__half, 128, true>(a, stream) : pg_launch<__half, 128, false>(a, stream);
-    return bias ? pg_launch<__half, 64, true>(a, stream) : pg_launch<__half, 64, false>(a, stream);
-}
 
 }  // namespace eet
