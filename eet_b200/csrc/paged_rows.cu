@@ -29,7 +29,7 @@ template<int D, int NR>
 struct PwShape {
     static constexpr int kHalves = D / 64;
     static constexpr int kTile = kHalves * kPgKeys * 128;                    // a K or V block
-    static constexpr int kStages = D == 64 ? 8 : NR == 64 ? 5 : 6;
+    static constexpr int kStages = D == 64 ? 8 : 5;
     static constexpr int kQ = kHalves * NR * 128;                            // rows of Q; two of them
     static constexpr int kP = 2 * NR * 128;                                  // probabilities [2 x 64 keys][NR]; two of them
     static constexpr int kSmem = kStages * kTile + 2 * kQ + 2 * kP;
@@ -47,9 +47,11 @@ struct PwSmem {
     uint32_t tmem_base;
     volatile int abort;
     int low[NR], high[NR];   // keys that a row sees
-    float slope[NR], ref[NR];
-    int pos[NR];
-    float warp_part[4][NR];
+    float slope[NR];         // of the bias, to the power of two
+    int pos[NR];             // its position
+    long long out_at[NR];    // where its result goes
+    float ref[NR];           // the reference of its powers, as a power of two
+    float corr[NR];          // what a moved reference takes from the sums so far; at the end 1 / sum
     PgFound found;
 };
 
@@ -68,6 +70,13 @@ __device__ __forceinline__ bool pw_any(bool p)
         : "r"((uint32_t)p)
         : "memory");
     return r != 0;
+}
+
+__device__ __forceinline__ void tmem_st8_async(uint32_t taddr, const uint32_t (&v)[8])
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"r"(taddr), "r"(v[0]), "r"(v[1]),
+                 "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
 }
 
 template<int NR>
@@ -265,6 +274,7 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         const float log2e = 1.4426950408889634f;
         const float to_log2 = a.scale * log2e;
         const int cap = (int)min((long long)a.max_pages << a.page_shift, 0x7fffffffLL);
+        float* cross = reinterpret_cast<float*>(p_rows);      // [NR][128], for what crosses the threads while no product reads P
         int stage = 0;                                        // of the loads, as the issuer counts them
         uint32_t phase = 0;
         int block = 0;                                        // blocks done
@@ -280,6 +290,7 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 sm.low[r] = a.window > 0 ? (int)max((long long)p.s.first, (long long)pos - a.window + 1) : p.s.first;
                 sm.high[r] = r < rows ? min(pos, cap - 1) : -1;
                 sm.slope[r] = a.slopes != nullptr && r < rows ? a.slopes[p.head * group + r % group] * log2e : 0.f;
+                sm.out_at[r] = (long long)(p.s.row0 + token0 + r / group) * a.o_tok + (long long)(p.head * group + r % group) * a.o_head;
                 sm.ref[r] = kPwNone;
             }
             pw_any(false);
@@ -339,41 +350,39 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 if (pw_any(over || !ok)) {
                     // Some row's reference moves (or a wait has run out: all leave together).
                     if (j > 0) ok = tc_wait_warp(&sm.pv_done[buf ^ 1], (uint32_t)(((block - 1) >> 1) & 1), &sm.abort) && ok;
+                    // (no product reads the probabilities now: their place holds the scores for a moment, row by row)
 #pragma unroll
-                    for (int n = 0; n < NR; ++n) {
-                        const float m = warp_max(t[n]);
-                        if (lane == 0) sm.warp_part[warp][n] = m;
-                    }
+                    for (int n = 0; n < NR; ++n) cross[n * kPgKeys + r] = t[n];
                     if (pw_any(!ok)) {
                         ok = false;
                         break;
                     }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    float corr[NR];
-#pragma unroll
-                    for (int n = 0; n < NR; ++n) {
-                        const float m = fmaxf(fmaxf(sm.warp_part[0][n], sm.warp_part[1][n]), fmaxf(sm.warp_part[2][n], sm.warp_part[3][n]));
-                        corr[n] = m - sm.ref[n] > 8.0f ? ex2_approx(sm.ref[n] - m) : 1.0f;
-                        l[n] *= corr[n];
+#pragma unroll 1
+                    for (int n = warp; n < NR; n += 4) {
+                        const float4 v = reinterpret_cast<const float4*>(cross + n * kPgKeys)[lane];
+                        const float m = warp_max(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
+                        const float old = sm.ref[n];
+                        __syncwarp();
+                        if (lane == 0) {
+                            sm.corr[n] = m - old > 8.0f ? ex2_approx(old - m) : 1.0f;
+                            sm.ref[n] = m - old > 8.0f ? m : old;
+                        }
                     }
+                    pw_any(false);
+#pragma unroll
+                    for (int n = 0; n < NR; ++n) l[n] *= sm.corr[n];
                     if (j > 0) {
-                        float o[NR];
-                        pw_tmem_ld<NR>(tmem_o + t_lane, o);
+#pragma unroll 1
+                        for (int c = 0; c < NR; c += 8) {
+                            uint32_t o[8];
+                            tmem_ld8(tmem_o + t_lane + (uint32_t)c, o);
 #pragma unroll
-                        for (int c = 0; c < NR; c += 16) {
-                            uint32_t u[16];
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(o[c + i] * corr[c + i]);
-                            tmem_st16_async(tmem_o + t_lane + (uint32_t)c, u);
+                            for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * sm.corr[c + i]);
+                            tmem_st8_async(tmem_o + t_lane + (uint32_t)c, o);
                         }
                         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                     }
-                    pw_any(false);   // the references have been read
-                    if (r < NR) {
-                        const float m = fmaxf(fmaxf(sm.warp_part[0][r], sm.warp_part[1][r]), fmaxf(sm.warp_part[2][r], sm.warp_part[3][r]));
-                        if (m - sm.ref[r] > 8.0f) sm.ref[r] = m;
-                    }
-                    pw_any(false);
                 }
                 // probabilities: row n of P holds 64 keys in 128 bytes, 16-byte pieces swizzled by n
                 uint8_t* dst = p_rows + buf * Shape::kP + (r >> 6) * (NR * 128) + (r & 7) * 2;
@@ -394,13 +403,10 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             phase ^= (uint32_t)((stage / kStages) & 1);
             stage %= kStages;
 
-            // ---- epilogue
-#pragma unroll
-            for (int n = 0; n < NR; ++n) {
-                const float sum = warp_sum(l[n]);
-                if (lane == 0) sm.warp_part[warp][n] = sum;
-            }
+            // ---- epilogue: the sums of the threads, then O, a dim a thread
             if (p.blocks > 0) ok = tc_wait_warp(&sm.pv_done[(block - 1) & 1], (uint32_t)(((block - 1) >> 1) & 1), &sm.abort);
+#pragma unroll
+            for (int n = 0; n < NR; ++n) cross[n * kPgKeys + r] = l[n];
             if (pw_any(!ok)) {
                 ok = false;
                 break;
@@ -408,39 +414,40 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const bool complete = p.starts && p.ends;
             const PgPartial part = pg_partial(ws, (int)gridDim.x, (int)blockIdx.x, p.starts ? 1 : 0, NR, D);
-            if (!complete && r < NR) {
-                part.max2[r] = sm.ref[r];
-                part.sum[r] = sm.warp_part[0][r] + sm.warp_part[1][r] + sm.warp_part[2][r] + sm.warp_part[3][r];
+#pragma unroll 1
+            for (int n = warp; n < rows; n += 4) {
+                const float4 v = reinterpret_cast<const float4*>(cross + n * kPgKeys)[lane];
+                const float sum = warp_sum((v.x + v.y) + (v.z + v.w));
+                if (lane == 0) {
+                    sm.corr[n] = sum > 0.f ? 1.0f / sum : 0.f;
+                    if (!complete) {
+                        part.max2[n] = sm.ref[n];
+                        part.sum[n] = sum;
+                    }
+                }
             }
-            float o[NR];
-            if (p.blocks > 0) {
-                pw_tmem_ld<NR>(tmem_o + t_lane, o);
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sm.o_free);
-            }
-            if (r < D) {
-                T* dst = (T*)a.out + (size_t)(p.s.row0 + token0) * a.o_tok + (size_t)(p.head * group) * a.o_head + r;
-                int g = 0;
+            pw_any(false);
+#pragma unroll 1
+            for (int c = 0; c < rows; c += 8) {
+                uint32_t o[8] = {};
+                if (p.blocks > 0) tmem_ld8(tmem_o + t_lane + (uint32_t)c, o);
+                if (r < D) {
 #pragma unroll
-                for (int n = 0; n < NR; ++n) {
-                    if (n < rows) {
-                        if (complete) {
-                            const float sum = sm.warp_part[0][n] + sm.warp_part[1][n] + sm.warp_part[2][n] + sm.warp_part[3][n];
-                            *dst = (T)(p.blocks > 0 && sum > 0.f ? o[n] / sum : 0.f);
-                            dst += a.o_head;
-                            if (++g == group) {
-                                g = 0;
-                                dst += a.o_tok - group * a.o_head;
-                            }
-                        }
-                        else if (p.blocks > 0) {
-                            reinterpret_cast<float*>(part.o)[n * D + r] = o[n];
+                    for (int i = 0; i < 8; ++i) {
+                        if (c + i < rows) {
+                            const float v = __uint_as_float(o[i]), inv = sm.corr[c + i];
+                            if (!complete) reinterpret_cast<float*>(part.o)[(c + i) * D + r] = v;
+                            else ((T*)a.out)[sm.out_at[c + i] + r] = (T)(inv > 0.f ? v * inv : 0.f);
                         }
                     }
                 }
             }
-            pw_any(false);   // the sums have been read
+            if (p.blocks > 0) {
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.o_free);
+            }
+            pw_any(false);   // the row's values have been read
         }
     }
 

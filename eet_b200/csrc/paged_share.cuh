@@ -177,89 +177,110 @@ __device__ __forceinline__ long long pg_seq_blocks(const PagedMhaArgs& a, const 
     return sum;
 }
 
+// Kernels this short spend much of their time on what runs once - the first fetch of every instruction among it - so what follows
+// is kept small: no 64-bit divisions, one pass over the sequences where the block has a thread for each.
 struct PgFound {
     long long warp_sum[12];
-    long long begin, end, total;
-    long long rest;        // of the share's begin, within its sequence
+    long long total;       // blocks in all
+    long long begin;       // of the share
+    long long rest;        // from the sequence's first block of a head to it
+    PgSeq s;
     int seq, head, tile, at;
-    int ctas;              // that have a share
+};
+
+// CTA c's share of `total` blocks begins at q c + min(c, r), with total = q ctas + r.
+struct PgCut {
+    long long q;
+    int r;
+    __device__ __forceinline__ PgCut(long long total, int ctas)
+    {
+        q = total >> 32 ? total / ctas : (long long)((uint32_t)total / (uint32_t)ctas);
+        r = (int)(total - q * ctas);
+    }
+    __device__ __forceinline__ long long begin(int cta) const { return q * cta + min(cta, r); }
+    // the CTA whose share holds block x
+    __device__ __forceinline__ int of(long long x) const
+    {
+        const long long large = (q + 1) * r;
+        const long long y = x < large ? x : x - large, d = x < large ? q + 1 : q;
+        return (x < large ? 0 : r) + (int)(y >> 32 ? y / d : (long long)((uint32_t)y / (uint32_t)d));
+    }
 };
 
 // The share of CTA `cta` of `ctas`, by all threads of the block.  Ends with a block-wide barrier; false: it has none.
-__device__ bool pg_find_share(const PagedMhaArgs& a, const PgTiling& g, int cta, int ctas, bool whole, PgFound& f, PgShare& share)
+__device__ __forceinline__ bool pg_find_share(const PagedMhaArgs& a, const PgTiling& g, int cta, int ctas, bool whole, PgFound& f,
+                                              PgShare& share)
 {
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5, threads = blockDim.x;
+    const bool once = a.seqs <= threads;
     long long total = 0;
-    for (int pass = 0; pass < 2; ++pass) {
-        long long before = 0;   // of the sequences of earlier rounds
-        for (int base = 0; base < a.seqs; base += (int)blockDim.x) {
+    for (int pass = once; pass < 2; ++pass) {   // the first pass adds up, the second (or only) one looks for the share's begin
+        long long before = 0;                   // of the sequences of earlier rounds
+        for (int base = 0; base < a.seqs; base += threads) {
             PgSeq s = {0, 0, 0, 0};
             if (base + tid < a.seqs) s = pg_seq(a, g, base + tid);
-            const long long cost = a.kv_heads * pg_seq_blocks(a, g, s);
+            const long long per_head = pg_seq_blocks(a, g, s), cost = a.kv_heads * per_head;
             const long long upto = pg_warp_scan(cost);
             if (lane == 31) f.warp_sum[warp] = upto;
             __syncthreads();
-            long long offset = before;
-            long long round = 0;
+            long long end = before + upto;
             for (int w = 0; w < warps; ++w) {
-                if (w < warp) offset += f.warp_sum[w];
-                round += f.warp_sum[w];
+                if (w < warp) end += f.warp_sum[w];
+                before += f.warp_sum[w];
             }
-            before += round;
-            const bool last = base + (int)blockDim.x >= a.seqs;
-            if (pass == 0 && last) total = before;
-            // with one round the first pass knows all there is to know
-            if (pass == 1 || (last && base == 0)) {
-                const long long n = min((long long)ctas, total);
-                const long long begin = n > 0 && cta < n ? total * cta / n : total;
-                const long long start = offset + upto - cost;
-                if (start <= begin && begin < start + cost) {
+            if (once) total = before;
+            if (pass == 1) {
+                const long long begin = PgCut(total, ctas).begin(cta);
+                if (end - cost <= begin && begin < end) {
+                    long long rest = begin - (end - cost);
+                    int head = 0;
+                    if (rest >= per_head) {
+                        head = rest >> 32 ? (int)(rest / per_head) : (int)((uint32_t)rest / (uint32_t)per_head);
+                        rest -= head * per_head;
+                    }
                     f.begin = begin;
                     f.seq = base + tid;
-                    f.rest = begin - start;
+                    f.s = s;
+                    f.head = head;
+                    f.tile = 0;
+                    f.at = (int)rest;
+                    f.rest = rest;
                 }
-                if (pass == 0) pass = 1;
             }
             __syncthreads();
         }
+        total = before;
     }
-    const long long n = min((long long)ctas, total);
-    if (cta >= n) return false;
-    const int seq = f.seq;
-    const PgSeq s = pg_seq(a, g, seq);
-    if (warp == 0) {
-        // the head and the tile within the sequence
-        const int tiles = g.tiles(s);
-        long long part = 0;
-        for (int t = lane; t < tiles; t += 32) part += max(1, pg_span(a, s, t * g.tokens, (t + 1) * g.tokens).blocks());
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-        const int head = (int)(f.rest / part);
-        long long rest = f.rest - head * part;
-        for (int t0 = 0; t0 < tiles; t0 += 32) {
-            const int t = t0 + lane;
-            const long long cost = t < tiles ? max(1, pg_span(a, s, t * g.tokens, (t + 1) * g.tokens).blocks()) : 0;
-            const long long upto = pg_warp_scan(cost);
-            if (upto - cost <= rest && rest < upto) {
-                f.head = head;
-                f.tile = t;
-                f.at = (int)(rest - (upto - cost));
+    const PgCut cut(total, ctas);
+    share.left = cut.begin(cta + 1) - cut.begin(cta);
+    if (share.left == 0) return false;
+    share.s = f.s;
+    if (g.tiles(share.s) > 1) {
+        if (warp == 0) {
+            // the tile within the sequence
+            long long rest = f.rest;
+            const int tiles = g.tiles(share.s);
+            for (int t0 = 0; t0 < tiles; t0 += 32) {
+                const int t = t0 + lane;
+                const long long cost = t < tiles ? max(1, pg_span(a, share.s, t * g.tokens, (t + 1) * g.tokens).blocks()) : 0;
+                const long long upto = pg_warp_scan(cost);
+                if (upto - cost <= rest && rest < upto) {
+                    f.tile = t;
+                    f.at = (int)(rest - (upto - cost));
+                }
+                const long long all = __shfl_sync(0xffffffffu, upto, 31);
+                if (rest < all) break;
+                rest -= all;
             }
-            const long long all = __shfl_sync(0xffffffffu, upto, 31);
-            if (rest < all) break;
-            rest -= all;
         }
+        __syncthreads();
     }
-    __syncthreads();
-    share.left = total * (cta + 1) / n - f.begin;
-    share.seq = seq;
+    share.seq = f.seq;
     share.head = f.head;
     share.tile = f.tile;
     share.at = f.at;
-    share.s = s;
     share.whole = whole;
     f.total = total;   // (the same from every thread)
-    f.ctas = (int)n;
     return true;
 }
 
@@ -305,7 +326,7 @@ __device__ __forceinline__ void pg_write_header(const PagedMhaArgs& a, const PgT
         const PgSpan span = pg_span(a, share.s, share.tile * g.tokens, (share.tile + 1) * g.tokens);
         const long long begin = found.begin - share.at;   // of the tile
         h.kind = share.at + share.left >= max(1, span.blocks()) ? 1 : 2;
-        h.from = (int)(((begin + 1) * found.ctas - 1) / found.total);
+        h.from = PgCut(found.total, (int)gridDim.x).of(begin);
         h.head = share.head;
         h.row0 = share.s.row0 + share.tile * g.tokens;
         h.tokens = min(g.tokens, share.s.tokens - share.tile * g.tokens);
