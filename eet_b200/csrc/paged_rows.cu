@@ -9,11 +9,12 @@
 // 64 sequences of 200 to 8000 tokens, 32 / 8 heads: 140 us, of which the transfer needs 81).
 //
 // One CTA per SM, its share of the work as paged_share.cuh says:
-//   warps 0-3  softmax: a thread per key = TMEM lane.  The powers are taken under a reference per row that all threads share; it
+//   warps 0-3, 4-7  softmax, two groups that take the pieces of the share in turn, so that the beginning of one runs beside the end
+//              of the one before (2.7 us a piece when there was one group): a thread per key = TMEM lane.  The powers are taken under a reference per row that all threads share; it
 //              moves only when a score has outgrown it by 2^8 (one vote of the 128 threads a block tells), so that no maximum
 //              crosses the threads in the usual block.  Sums stay with the threads until the end.
-//   warp 4     producer: Q, then K and V blocks of 128 keys through a ring of 32 KiB stages
-//   warp 5     one thread issues the products; scores and probabilities have two buffers, so that S of the next block is there when
+//   warp 8     producer: Q, then K and V blocks of 128 keys through a ring of 32 KiB stages
+//   warp 9     one thread issues the products; scores and probabilities have two buffers, so that S of the next block is there when
 //              the softmax of this one ends
 // Keys that no row sees may be anything, even NaN: masked by selection, their rows of V set to zero before the product.
 #include "paged_share.cuh"
@@ -22,52 +23,59 @@ namespace eet {
 
 namespace {
 
-constexpr int kPwThreads = 192;
+constexpr int kPwThreads = 320;
+constexpr int kPwExtra = 2;         // a piece's beginning and end cost as much as two blocks
 constexpr float kPwNone = -1e20f;   // reference of a row that has seen nothing
 
 template<int D, int NR>
 struct PwShape {
     static constexpr int kHalves = D / 64;
     static constexpr int kTile = kHalves * kPgKeys * 128;                    // a K or V block
-    static constexpr int kStages = D == 64 ? 8 : 5;
+    static constexpr int kStages = D == 64 ? (NR == 64 ? 6 : 8) : NR == 64 ? 3 : NR == 32 ? 5 : 6;
     static constexpr int kQ = kHalves * NR * 128;                            // rows of Q; two of them
-    static constexpr int kP = 2 * NR * 128;                                  // probabilities [2 x 64 keys][NR]; two of them
-    static constexpr int kSmem = kStages * kTile + 2 * kQ + 2 * kP;
-    static constexpr uint32_t kTmemCols = NR == 16 ? 64 : 4 * NR;            // two S, one O
+    static constexpr int kP = 2 * NR * 128;                                  // probabilities [2 x 64 keys][NR]; two of them a group
+    static constexpr int kSmem = kStages * kTile + 2 * kQ + 4 * kP;
+    static constexpr uint32_t kTmemCols = NR == 16 ? 128 : 8 * NR;           // two S, one O of either group
 };
 
+// What the four warps of a softmax group know of their piece, by row.
 template<int NR>
-struct PwSmem {
-    uint64_t q_full[2], q_empty[2];
-    uint64_t full[8], empty[8];
-    uint64_t s_full[2];      // S^T of a block has been computed
-    uint64_t p_ready[2];     // its probabilities are there (four warps)
-    uint64_t pv_done[2];     // its V^T.P^T has completed
-    uint64_t o_free;         // O of a piece has been read (four warps)
-    uint32_t tmem_base;
-    volatile int abort;
+struct PwRows {
     int low[NR], high[NR];   // keys that a row sees
     float slope[NR];         // of the bias, to the power of two
     int pos[NR];             // its position
     long long out_at[NR];    // where its result goes
     float ref[NR];           // the reference of its powers, as a power of two
     float corr[NR];          // what a moved reference takes from the sums so far; at the end 1 / sum
+};
+
+template<int NR>
+struct PwSmem {
+    uint64_t q_full[2], q_empty[2];
+    uint64_t full[8], empty[8];
+    uint64_t s_full[2][2];      // [group][buffer]: S^T of a block has been computed
+    uint64_t p_ready[2][2];     // its probabilities are there (four warps)
+    uint64_t pv_done[2][2];     // its V^T.P^T has completed
+    uint64_t o_free[2];         // O of a piece has been read (four warps)
+    uint32_t tmem_base;
+    volatile int abort;
+    PwRows<NR> rows[2];
     PgFound found;
 };
 
-// Barrier of the four softmax warps: whether any thread says so.
-__device__ __forceinline__ bool pw_any(bool p)
+// Barrier of the four warps of a softmax group: whether any thread says so.
+__device__ __forceinline__ bool pw_any(int group, bool p)
 {
     uint32_t r;
     asm volatile(
         "{\n\t"
         ".reg .pred p, q;\n\t"
         "setp.ne.u32 p, %1, 0;\n\t"
-        "bar.red.or.pred q, 1, 128, p;\n\t"
+        "bar.red.or.pred q, %2, 128, p;\n\t"
         "selp.u32 %0, 1, 0, q;\n\t"
         "}\n"
         : "=r"(r)
-        : "r"((uint32_t)p)
+        : "r"((uint32_t)p), "r"(1 + group)
         : "memory");
     return r != 0;
 }
@@ -118,25 +126,27 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int group = a.heads / a.kv_heads;
     const int tile_tokens = NR / group;
-    const PgTiling tiling = {tile_tokens, 1, most};
+    const PgTiling tiling = {tile_tokens, 1, most, kPwExtra};
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sm.q_full[i], 1);
             mbar_init(&sm.q_empty[i], 1);
-            mbar_init(&sm.s_full[i], 1);
-            mbar_init(&sm.p_ready[i], 4);
-            mbar_init(&sm.pv_done[i], 1);
+            for (int buf = 0; buf < 2; ++buf) {
+                mbar_init(&sm.s_full[i][buf], 1);
+                mbar_init(&sm.p_ready[i][buf], 4);
+                mbar_init(&sm.pv_done[i][buf], 1);
+            }
+            mbar_init(&sm.o_free[i], 4);
         }
         for (int i = 0; i < kStages; ++i) {
             mbar_init(&sm.full[i], 1);
             mbar_init(&sm.empty[i], 1);
         }
-        mbar_init(&sm.o_free, 4);
         sm.abort = 0;
         mbar_fence_init();
     }
-    if (warp == 5) {
+    if (warp == 9) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)),
                      "r"(Shape::kTmemCols)
                      : "memory");
@@ -150,13 +160,12 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     PgShare share;
     const bool work = pg_find_share(a, tiling, (int)blockIdx.x, (int)gridDim.x, whole != 0, sm.found, share);
     const uint32_t tmem = sm.tmem_base;
-    const uint32_t tmem_o = tmem + 2 * NR;
     if (!whole && threadIdx.x == 0) pg_write_header(a, tiling, ws, (int)blockIdx.x, work, share, sm.found);
     PgPiece p;
 
     if (!work) {
     }
-    else if (warp == 4) {
+    else if (warp == 8) {
         // ------------------------------------------------------------------ producer
         const long long cap = (long long)a.max_pages << a.page_shift;
         int stage = 0, issued = 0, pieces = 0;
@@ -203,7 +212,7 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             for (int i = max(0, pieces - 2); i < pieces; ++i) mbar_wait_bounded(&sm.q_full[i & 1], (uint32_t)((i / 2) & 1));
         }
     }
-    else if (warp == 5) {
+    else if (warp == 9) {
         // ------------------------------------------------------------------ MMA issuer
         if (elect_one()) {
             constexpr uint32_t idesc_qk = umma_idesc_f16(kPgKeys, NR) | PgType<T>::idesc;
@@ -216,7 +225,7 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             int pieces = 0;
             int stage = 0;                  // loads are used in the order they are made
             uint32_t phase = 0;
-            int qk = 0, pv = 0;             // blocks whose products have been issued
+            int qk[2] = {0, 0};             // blocks of either group whose products have been issued
             bool ok = true;
             auto next_stage = [&]() {
                 umma_commit(&sm.empty[stage]);
@@ -230,85 +239,104 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 const int n = p.blocks, qb = pieces & 1;
                 ok = tc_wait(&sm.q_full[qb], (uint32_t)((pieces / 2) & 1), &sm.abort);
                 if (!ok) break;
+                const uint32_t tmem_s = tmem + (uint32_t)(qb * 3 * NR), tmem_o = tmem_s + 2 * NR;
+                int done_qk = qb ? qk[1] : qk[0], done_pv = done_qk;
                 auto issue_qk = [&](int j) -> bool {
                     if (!tc_wait(&sm.full[stage], phase, &sm.abort)) return false;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint64_t kd = k_desc + (uint64_t)(stage * (kTile >> 4)), qd = q_desc + (uint64_t)(qb * (Shape::kQ >> 4));
 #pragma unroll
                     for (int kk = 0; kk < D / 16; ++kk) {
-                        umma_f16(tmem + (uint32_t)((qk & 1) * NR), kd + (uint64_t)((kk >> 2) * (kHalf >> 4) + (kk & 3) * 2),
+                        umma_f16(tmem_s + (uint32_t)((done_qk & 1) * NR), kd + (uint64_t)((kk >> 2) * (kHalf >> 4) + (kk & 3) * 2),
                                  qd + (uint64_t)((kk >> 2) * (NR * 128 >> 4) + (kk & 3) * 2), idesc_qk, kk != 0);
                     }
-                    umma_commit(&sm.s_full[qk & 1]);
+                    umma_commit(&sm.s_full[qb][done_qk & 1]);
                     next_stage();
                     if (j == n - 1) umma_commit(&sm.q_empty[qb]);
-                    ++qk;
+                    ++done_qk;
                     return true;
                 };
                 // S of block j + 2 goes where that of block j was, which has been read when its probabilities are there
                 ok = issue_qk(0) && (n == 1 || issue_qk(1));
-                if (ok && pieces > 0) ok = tc_wait(&sm.o_free, (uint32_t)((pieces - 1) & 1), &sm.abort);
+                if (ok && pieces > 1) ok = tc_wait(&sm.o_free[qb], (uint32_t)((pieces / 2 - 1) & 1), &sm.abort);
                 for (int j = 0; j < n && ok; ++j) {
-                    ok = tc_wait(&sm.full[stage], phase, &sm.abort) && tc_wait(&sm.p_ready[pv & 1], (uint32_t)((pv >> 1) & 1), &sm.abort);
+                    ok = tc_wait(&sm.full[stage], phase, &sm.abort) &&
+                         tc_wait(&sm.p_ready[qb][done_pv & 1], (uint32_t)((done_pv >> 1) & 1), &sm.abort);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint64_t vd = v_desc + (uint64_t)(stage * (kTile >> 4)), pd = p_desc + (uint64_t)((pv & 1) * (Shape::kP >> 4));
+                    const uint64_t vd = v_desc + (uint64_t)(stage * (kTile >> 4)),
+                                   pd = p_desc + (uint64_t)((2 * qb + (done_pv & 1)) * (Shape::kP >> 4));
 #pragma unroll
                     for (int kk = 0; kk < kPgKeys / 16; ++kk) {
                         umma_f16(tmem_o, vd + (uint64_t)(kk * (2048 >> 4)), pd + (uint64_t)((kk >> 2) * (NR * 128 >> 4) + (kk & 3) * 2),
                                  idesc_pv, j != 0 || kk != 0);
                     }
-                    umma_commit(&sm.pv_done[pv & 1]);
+                    umma_commit(&sm.pv_done[qb][done_pv & 1]);
                     next_stage();
-                    ++pv;
+                    ++done_pv;
                     if (j + 2 < n) ok = issue_qk(j + 2);
                 }
+                if (qb) qk[1] = done_qk;
+                else qk[0] = done_qk;
                 ++pieces;
             }
         }
     }
     else {
         // ------------------------------------------------------------------ softmax, epilogue
-        const int r = warp * 32 + lane;                       // key of the block, and dim of O
-        const uint32_t t_lane = (uint32_t)(warp * 32) << 16;
+        const int x = warp >> 2;                              // pieces go to the two groups in turn
+        const int r = (warp & 3) * 32 + lane;                 // key of the block, and dim of O
+        const uint32_t t_lane = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t tmem_s = tmem + t_lane + (uint32_t)(x * 3 * NR), tmem_o = tmem_s + 2 * NR;
         const float log2e = 1.4426950408889634f;
         const float to_log2 = a.scale * log2e;
         const int cap = (int)min((long long)a.max_pages << a.page_shift, 0x7fffffffLL);
-        float* cross = reinterpret_cast<float*>(p_rows);      // [NR][128], for what crosses the threads while no product reads P
+        PwRows<NR>& row = sm.rows[x];
+        uint8_t* p_mine = p_rows + x * 2 * Shape::kP;
+        float* cross = reinterpret_cast<float*>(p_mine);      // [NR][128], for what crosses the threads while no product reads P
         int stage = 0;                                        // of the loads, as the issuer counts them
         uint32_t phase = 0;
         int block = 0;                                        // blocks done
+        int pieces = 0;
         bool ok = true;
         while (share.next(a, tiling, p)) {
+            const bool mine = p.blocks > 0 ? (pieces & 1) == x : x == 0;
+            pieces += p.blocks > 0;
+            if (!mine) {
+                stage += 2 * p.blocks;
+                phase ^= (uint32_t)((stage / kStages) & 1);
+                stage %= kStages;
+                continue;
+            }
             const int token0 = p.tile * tile_tokens;
             const int rows = min(tile_tokens, p.s.tokens - token0) * group;
             const PgSpan span = pg_span(a, p.s, token0, token0 + tile_tokens);
             // (everybody has left the piece before: its last barrier stands behind the last use of these)
             if (r < NR) {
                 const int pos = p.s.p0 + token0 + r / group;
-                sm.pos[r] = pos;
-                sm.low[r] = a.window > 0 ? (int)max((long long)p.s.first, (long long)pos - a.window + 1) : p.s.first;
-                sm.high[r] = r < rows ? min(pos, cap - 1) : -1;
-                sm.slope[r] = a.slopes != nullptr && r < rows ? a.slopes[p.head * group + r % group] * log2e : 0.f;
-                sm.out_at[r] = (long long)(p.s.row0 + token0 + r / group) * a.o_tok + (long long)(p.head * group + r % group) * a.o_head;
-                sm.ref[r] = kPwNone;
+                row.pos[r] = pos;
+                row.low[r] = a.window > 0 ? (int)max((long long)p.s.first, (long long)pos - a.window + 1) : p.s.first;
+                row.high[r] = r < rows ? min(pos, cap - 1) : -1;
+                row.slope[r] = a.slopes != nullptr && r < rows ? a.slopes[p.head * group + r % group] * log2e : 0.f;
+                row.out_at[r] = (long long)(p.s.row0 + token0 + r / group) * a.o_tok + (long long)(p.head * group + r % group) * a.o_head;
+                row.ref[r] = kPwNone;
             }
-            pw_any(false);
+            pw_any(x, false);
             // blocks all of whose keys every row sees
-            const int all_low = sm.low[rows - 1], all_high = sm.high[0];
+            const int all_low = row.low[rows - 1], all_high = row.high[0];
             float l[NR];
 #pragma unroll
             for (int n = 0; n < NR; ++n) l[n] = 0.f;
             for (int j = 0; j < p.blocks; ++j, ++block) {
                 const int key0 = (p.block0 + j) * kPgKeys, key = key0 + r;
                 const int buf = block & 1;
-                ok = tc_wait_warp(&sm.s_full[buf], (uint32_t)((block >> 1) & 1), &sm.abort);
+                ok = tc_wait_warp(&sm.s_full[x][buf], (uint32_t)((block >> 1) & 1), &sm.abort);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 float t[NR];
-                pw_tmem_ld<NR>(tmem + t_lane + (uint32_t)(buf * NR), t);
+                pw_tmem_ld<NR>(tmem_s + (uint32_t)(buf * NR), t);
                 if (a.slopes != nullptr) {
 #pragma unroll
-                    for (int n = 0; n < NR; ++n) t[n] = fmaf(t[n], to_log2, sm.slope[n] * (float)(key - sm.pos[n]));
+                    for (int n = 0; n < NR; ++n) t[n] = fmaf(t[n], to_log2, row.slope[n] * (float)(key - row.pos[n]));
                 }
                 else {
 #pragma unroll
@@ -320,13 +348,13 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 }
                 else {
 #pragma unroll
-                    for (int n = 0; n < NR; ++n) t[n] = key >= sm.low[n] && key <= sm.high[n] ? t[n] : -INFINITY;
+                    for (int n = 0; n < NR; ++n) t[n] = key >= row.low[n] && key <= row.high[n] ? t[n] : -INFINITY;
                 }
                 bool over = j == 0;
 #pragma unroll
-                for (int n = 0; n < NR; ++n) over |= t[n] - sm.ref[n] > 8.0f;
+                for (int n = 0; n < NR; ++n) over |= t[n] - row.ref[n] > 8.0f;
                 // the buffer that the probabilities go to has been read by the product of two blocks before
-                if (block > 1) ok = tc_wait_warp(&sm.pv_done[buf], (uint32_t)(((block >> 1) - 1) & 1), &sm.abort) && ok;
+                if (block > 1) ok = tc_wait_warp(&sm.pv_done[x][buf], (uint32_t)(((block >> 1) - 1) & 1), &sm.abort) && ok;
                 const int v_entry = pg_v_entry(j, p.blocks);   // of the piece's loads
                 int v_stage = stage + v_entry;
                 uint32_t v_phase = phase;
@@ -347,56 +375,56 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                         }
                     }
                 }
-                if (pw_any(over || !ok)) {
+                if (pw_any(x, over || !ok)) {
                     // Some row's reference moves (or a wait has run out: all leave together).
-                    if (j > 0) ok = tc_wait_warp(&sm.pv_done[buf ^ 1], (uint32_t)(((block - 1) >> 1) & 1), &sm.abort) && ok;
+                    if (j > 0) ok = tc_wait_warp(&sm.pv_done[x][buf ^ 1], (uint32_t)(((block - 1) >> 1) & 1), &sm.abort) && ok;
                     // (no product reads the probabilities now: their place holds the scores for a moment, row by row)
 #pragma unroll
                     for (int n = 0; n < NR; ++n) cross[n * kPgKeys + r] = t[n];
-                    if (pw_any(!ok)) {
+                    if (pw_any(x, !ok)) {
                         ok = false;
                         break;
                     }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
-                    for (int n = warp; n < NR; n += 4) {
+                    for (int n = warp & 3; n < NR; n += 4) {
                         const float4 v = reinterpret_cast<const float4*>(cross + n * kPgKeys)[lane];
                         const float m = warp_max(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
-                        const float old = sm.ref[n];
+                        const float old = row.ref[n];
                         __syncwarp();
                         if (lane == 0) {
-                            sm.corr[n] = m - old > 8.0f ? ex2_approx(old - m) : 1.0f;
-                            sm.ref[n] = m - old > 8.0f ? m : old;
+                            row.corr[n] = m - old > 8.0f ? ex2_approx(old - m) : 1.0f;
+                            row.ref[n] = m - old > 8.0f ? m : old;
                         }
                     }
-                    pw_any(false);
+                    pw_any(x, false);
 #pragma unroll
-                    for (int n = 0; n < NR; ++n) l[n] *= sm.corr[n];
+                    for (int n = 0; n < NR; ++n) l[n] *= row.corr[n];
                     if (j > 0) {
 #pragma unroll 1
                         for (int c = 0; c < NR; c += 8) {
                             uint32_t o[8];
-                            tmem_ld8(tmem_o + t_lane + (uint32_t)c, o);
+                            tmem_ld8(tmem_o + (uint32_t)c, o);
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * sm.corr[c + i]);
-                            tmem_st8_async(tmem_o + t_lane + (uint32_t)c, o);
+                            for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * row.corr[c + i]);
+                            tmem_st8_async(tmem_o + (uint32_t)c, o);
                         }
                         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                     }
                 }
                 // probabilities: row n of P holds 64 keys in 128 bytes, 16-byte pieces swizzled by n
-                uint8_t* dst = p_rows + buf * Shape::kP + (r >> 6) * (NR * 128) + (r & 7) * 2;
+                uint8_t* dst = p_mine + buf * Shape::kP + (r >> 6) * (NR * 128) + (r & 7) * 2;
                 const int piece = (r & 63) >> 3;
 #pragma unroll
                 for (int n = 0; n < NR; ++n) {
-                    const float e = ex2_approx(t[n] - sm.ref[n]);
+                    const float e = ex2_approx(t[n] - row.ref[n]);
                     l[n] += e;
                     *reinterpret_cast<T*>(dst + n * 128 + ((piece ^ (n & 7)) << 4)) = (T)e;
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&sm.p_ready[buf]);
+                if (lane == 0) mbar_arrive(&sm.p_ready[x][buf]);
             }
             if (!ok) break;
             stage += 2 * p.blocks;
@@ -404,10 +432,10 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             stage %= kStages;
 
             // ---- epilogue: the sums of the threads, then O, a dim a thread
-            if (p.blocks > 0) ok = tc_wait_warp(&sm.pv_done[(block - 1) & 1], (uint32_t)(((block - 1) >> 1) & 1), &sm.abort);
+            if (p.blocks > 0) ok = tc_wait_warp(&sm.pv_done[x][(block - 1) & 1], (uint32_t)(((block - 1) >> 1) & 1), &sm.abort);
 #pragma unroll
             for (int n = 0; n < NR; ++n) cross[n * kPgKeys + r] = l[n];
-            if (pw_any(!ok)) {
+            if (pw_any(x, !ok)) {
                 ok = false;
                 break;
             }
@@ -415,29 +443,29 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             const bool complete = p.starts && p.ends;
             const PgPartial part = pg_partial(ws, (int)gridDim.x, (int)blockIdx.x, p.starts ? 1 : 0, NR, D);
 #pragma unroll 1
-            for (int n = warp; n < rows; n += 4) {
+            for (int n = warp & 3; n < rows; n += 4) {
                 const float4 v = reinterpret_cast<const float4*>(cross + n * kPgKeys)[lane];
                 const float sum = warp_sum((v.x + v.y) + (v.z + v.w));
                 if (lane == 0) {
-                    sm.corr[n] = sum > 0.f ? 1.0f / sum : 0.f;
+                    row.corr[n] = sum > 0.f ? 1.0f / sum : 0.f;
                     if (!complete) {
-                        part.max2[n] = sm.ref[n];
+                        part.max2[n] = row.ref[n];
                         part.sum[n] = sum;
                     }
                 }
             }
-            pw_any(false);
+            pw_any(x, false);
 #pragma unroll 1
             for (int c = 0; c < rows; c += 8) {
                 uint32_t o[8] = {};
-                if (p.blocks > 0) tmem_ld8(tmem_o + t_lane + (uint32_t)c, o);
+                if (p.blocks > 0) tmem_ld8(tmem_o + (uint32_t)c, o);
                 if (r < D) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         if (c + i < rows) {
-                            const float v = __uint_as_float(o[i]), inv = sm.corr[c + i];
+                            const float v = __uint_as_float(o[i]), inv = row.corr[c + i];
                             if (!complete) reinterpret_cast<float*>(part.o)[(c + i) * D + r] = v;
-                            else ((T*)a.out)[sm.out_at[c + i] + r] = (T)(inv > 0.f ? v * inv : 0.f);
+                            else ((T*)a.out)[row.out_at[c + i] + r] = (T)(inv > 0.f ? v * inv : 0.f);
                         }
                     }
                 }
@@ -445,15 +473,15 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             if (p.blocks > 0) {
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&sm.o_free);
+                if (lane == 0) mbar_arrive(&sm.o_free[x]);
             }
-            pw_any(false);   // the row's values have been read
+            pw_any(x, false);   // the row's values have been read
         }
     }
 
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (warp == 5) {
+    if (warp == 9) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Shape::kTmemCols) : "memory");
     }
 }

@@ -49,8 +49,10 @@ struct PgSeq {
 };
 
 // What a kernel works on: sequences with `least` to `most` new tokens, `tokens` of them to a tile (both tiles of a pair counted).
+// A tile counts as `extra` blocks more than it has: what its beginning and end cost.  These stand before its first block; a share
+// that ends within them leaves the tile to the next.
 struct PgTiling {
-    int tokens, least, most;
+    int tokens, least, most, extra;
     __device__ __forceinline__ int tiles(const PgSeq& s) const { return (s.tokens + tokens - 1) / tokens; }
 };
 
@@ -87,12 +89,12 @@ struct PgPiece {
     PgSeq s;
     int seq, head, tile;
     int block0, blocks;   // key blocks of it to be worked on; 0: its rows see nothing
-    bool starts, ends;    // whether those are its first, its last
+    bool starts, ends;    // whether those begin with its first, end with its last
 };
 
 // Walks the share of a CTA tile by tile.  All threads of a warp hold the same.
 struct PgShare {
-    long long left;       // blocks of the share still to come (a tile that sees nothing counts as one)
+    long long left;       // of the share still to come, in blocks
     int seq, head, tile, at;
     PgSeq s;
     bool whole;           // tiles are not cut: the share has those that begin in it
@@ -116,25 +118,26 @@ struct PgShare {
     {
         while (left > 0) {
             const PgSpan span = pg_span(a, s, tile * g.tokens, (tile + 1) * g.tokens);
-            const int n = span.blocks(), cost = max(1, n);
+            const int n = span.blocks(), cost = n + g.extra;
             if (whole && at > 0) {   // it began in the share before
                 left -= cost - at;
                 step(a, g);
                 continue;
             }
             const int take = whole ? cost : (int)min(left, (long long)(cost - at));
+            const int from = max(0, at - g.extra), to = max(0, at + take - g.extra);
             p.s = s;
             p.seq = seq;
             p.head = head;
             p.tile = tile;
-            p.block0 = span.first_block() + at;
-            p.blocks = n == 0 ? 0 : take;
-            p.starts = at == 0;
+            p.block0 = span.first_block() + from;
+            p.blocks = to - from;
+            p.starts = from == 0;
             p.ends = at + take == cost;
             left -= take;
             at += take;
             if (p.ends) step(a, g);
-            return true;
+            if (p.blocks > 0 || n == 0 && p.ends) return true;
         }
         return false;
     }
@@ -156,7 +159,7 @@ __device__ __forceinline__ long long pg_seq_blocks(const PagedMhaArgs& a, const 
     const int tiles = g.tiles(mine);
     long long sum = 0;
     if (tiles <= 4) {
-        for (int t = 0; t < tiles; ++t) sum += max(1, pg_span(a, mine, t * g.tokens, (t + 1) * g.tokens).blocks());
+        for (int t = 0; t < tiles; ++t) sum += pg_span(a, mine, t * g.tokens, (t + 1) * g.tokens).blocks() + g.extra;
     }
     uint32_t many = __ballot_sync(0xffffffffu, tiles > 4);
     while (many) {
@@ -169,7 +172,7 @@ __device__ __forceinline__ long long pg_seq_blocks(const PagedMhaArgs& a, const 
         s.first = __shfl_sync(0xffffffffu, mine.first, src);
         const int n = g.tiles(s);
         long long part = 0;
-        for (int t = threadIdx.x & 31; t < n; t += 32) part += max(1, pg_span(a, s, t * g.tokens, (t + 1) * g.tokens).blocks());
+        for (int t = threadIdx.x & 31; t < n; t += 32) part += pg_span(a, s, t * g.tokens, (t + 1) * g.tokens).blocks() + g.extra;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
         if ((int)(threadIdx.x & 31) == src) sum = part;
@@ -262,7 +265,7 @@ __device__ __forceinline__ bool pg_find_share(const PagedMhaArgs& a, const PgTil
             const int tiles = g.tiles(share.s);
             for (int t0 = 0; t0 < tiles; t0 += 32) {
                 const int t = t0 + lane;
-                const long long cost = t < tiles ? max(1, pg_span(a, share.s, t * g.tokens, (t + 1) * g.tokens).blocks()) : 0;
+                const long long cost = t < tiles ? pg_span(a, share.s, t * g.tokens, (t + 1) * g.tokens).blocks() + g.extra : 0;
                 const long long upto = pg_warp_scan(cost);
                 if (upto - cost <= rest && rest < upto) {
                     f.tile = t;
@@ -322,11 +325,10 @@ __device__ __forceinline__ void pg_write_header(const PagedMhaArgs& a, const PgT
                                                 const PgFound& found)
 {
     PgHeader h = {};
-    if (work && share.at > 0) {
+    if (work && share.at > g.extra) {
         const PgSpan span = pg_span(a, share.s, share.tile * g.tokens, (share.tile + 1) * g.tokens);
-        const long long begin = found.begin - share.at;   // of the tile
-        h.kind = share.at + share.left >= max(1, span.blocks()) ? 1 : 2;
-        h.from = PgCut(found.total, (int)gridDim.x).of(begin);
+        h.kind = share.at + share.left >= span.blocks() + g.extra ? 1 : 2;
+        h.from = PgCut(found.total, (int)gridDim.x).of(found.begin - share.at + g.extra);   // where its first block is
         h.head = share.head;
         h.row0 = share.s.row0 + share.tile * g.tokens;
         h.tokens = min(g.tokens, share.s.tokens - share.tile * g.tokens);

@@ -24,6 +24,7 @@ namespace {
 
 constexpr int kPgThreads = 320;
 constexpr int kPgStages = 5;
+constexpr int kPgExtra = 2;
 constexpr uint32_t kPgTmemCols = 512;   // S of a, S of b (their probabilities over them), O of a, O of b: 128 each
 constexpr float kPgNone = -1e20f;       // running maximum of a row that has seen nothing
 
@@ -93,7 +94,7 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int group = a.heads / a.kv_heads;
     const int tile_tokens = kPgRows / group, pair_tokens = 2 * tile_tokens;
-    const PgTiling tiling = {pair_tokens, least, 0x7fffffff};
+    const PgTiling tiling = {pair_tokens, least, 0x7fffffff, kPgExtra};
 
     if (threadIdx.x == 0) {
         mbar_init(&sm.q_full, 1);
