@@ -185,7 +185,15 @@ static PagedPlan paged_plan(const PagedMhaArgs& a)
         if (others > 0) p.nr = rows_for((rest + others - 1) / others);
         p.few = p.nr / group;
     }
-    p.whole[0] = p.whole[1] = a.max_len <= kPgKeys;
+    // Cutting tiles evens out the shares and costs a second launch, some 4 us or the time of five blocks: not where whole tiles
+    // make the longest share no more than that longer (taking sequences to be half as long as the longest).
+    auto whole = [&](long long tokens) {
+        const long long sms = sm_count(), blocks = (a.max_len + kPgKeys - 1) / kPgKeys;
+        const long long tiles = (a.seqs + (a.max_tokens > tokens ? a.tokens / tokens : 0)) * a.kv_heads;
+        return blocks - (tiles < sms ? blocks * tiles / (2 * sms) : 0) <= 5;
+    };
+    if (p.nr > 0) p.whole[0] = whole(p.nr / group);
+    if (p.tiles) p.whole[1] = whole(2 * (kPgRows / group));
     if (p.nr > 0 && !p.whole[0]) p.bytes[0] = pg_scratch_bytes(sm_count(), p.nr, a.head_dim);
     if (p.tiles && !p.whole[1]) p.bytes[1] = pg_scratch_bytes(sm_count(), 2 * kPgRows, a.head_dim);
     return p;
@@ -218,8 +226,8 @@ static int launch_paged_mha_t(const PagedMhaArgs& a, const PagedPlan& p, cudaStr
     if (p.bytes[0]) s[n++] = {ws[0], p.nr, 0};
     if (p.bytes[1]) s[n++] = {ws[1], 2 * kPgRows, 1};
     if (n > 0) {
-        const int y = p.bytes[1] ? 8 : p.nr * D / 4 / 256;
-        EET_CUDA(launch_pdl(paged_mha_join_kernel<T, D>, dim3(sm_count(), y < 1 ? 1 : y, n), dim3(256), 0, stream, a, s[0], s[1]));
+        const int y = ((p.bytes[1] ? 2 * kPgRows : p.nr) * D / 16 + 255) / 256;   // 16 dims a thread
+        EET_CUDA(launch_pdl(paged_mha_join_kernel<T, D>, dim3(sm_count(), y, n), dim3(256), 0, stream, a, s[0], s[1]));
     }
     return 0;
 }

@@ -160,10 +160,10 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     PgShare share;
     const bool work = pg_find_share(a, tiling, (int)blockIdx.x, (int)gridDim.x, whole != 0, sm.found, share);
     const uint32_t tmem = sm.tmem_base;
-    if (!whole && threadIdx.x == 0) pg_write_header(a, tiling, ws, (int)blockIdx.x, work, share, sm.found);
     PgPiece p;
 
     if (!work) {
+        if (!whole && threadIdx.x == 0) pg_write_header(a, tiling, ws, (int)blockIdx.x, false, share, sm.found);
     }
     else if (warp == 8) {
         // ------------------------------------------------------------------ producer
@@ -171,11 +171,12 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         int stage = 0, issued = 0, pieces = 0;
         uint32_t phase = 1;                                       // of `empty`: the first round finds the stages free
         bool ok = true;
+        const PgShare all = share;
         while (ok && share.next(a, tiling, p)) {
             if (p.blocks == 0) continue;
             const PgSpan span = pg_span(a, p.s, p.tile * tile_tokens, (p.tile + 1) * tile_tokens);
             const PgLoader<D> loader = {a, a.pages + p.seq * a.pages_stride, p.head, span};
-            int page = loader.page(p.block0 * kPgKeys), before = 0;
+            int page = loader.page(p.top * kPgKeys), before = 0;
             const int qb = pieces & 1;
             if (pieces > 1 && !tc_wait_warp(&sm.q_empty[qb], (uint32_t)((pieces / 2 - 1) & 1), &sm.abort)) break;
             ++pieces;
@@ -188,7 +189,7 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             if (p.s.p0 + p.s.tokens > cap && lane == 0) g_device_status = 6;
             auto put = [&](const CUtensorMap* map, int j, int page) -> bool {
                 if (!tc_wait_warp(&sm.empty[stage], phase, &sm.abort)) return false;
-                loader.load(map, (p.block0 + j) * kPgKeys, page, ring + stage * kTile, &sm.full[stage]);
+                loader.load(map, (p.top - j) * kPgKeys, page, ring + stage * kTile, &sm.full[stage]);
                 ++issued;
                 if (++stage == kStages) {
                     stage = 0;
@@ -197,13 +198,14 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 return true;
             };
             for (int j = 0; j <= p.blocks && ok; ++j) {
-                const int next = j + 1 < p.blocks ? loader.page((p.block0 + j + 1) * kPgKeys) : 0;
+                const int next = j + 1 < p.blocks ? loader.page((p.top - j - 1) * kPgKeys) : 0;
                 if (j < p.blocks) ok = put(&map_k, j, page);
                 if (j > 0 && ok) ok = put(&map_v, j - 1, before);
                 before = page;
                 page = next;
             }
         }
+        if (!whole && lane == 0) pg_write_header(a, tiling, ws, (int)blockIdx.x, true, all, sm.found);
         if (sm.abort) {
             // nothing of this CTA may still be on its way when it ends
             for (int e = max(0, issued - kStages); e < issued; ++e) {
@@ -298,7 +300,7 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         uint32_t phase = 0;
         int block = 0;                                        // blocks done
         int pieces = 0;
-        bool ok = true;
+        bool ok = true, failed = false;                       // this thread's waits; what the group has agreed on: all leave together
         while (share.next(a, tiling, p)) {
             const bool mine = p.blocks > 0 ? (pieces & 1) == x : x == 0;
             pieces += p.blocks > 0;
@@ -328,9 +330,9 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
 #pragma unroll
             for (int n = 0; n < NR; ++n) l[n] = 0.f;
             for (int j = 0; j < p.blocks; ++j, ++block) {
-                const int key0 = (p.block0 + j) * kPgKeys, key = key0 + r;
+                const int key0 = (p.top - j) * kPgKeys, key = key0 + r;
                 const int buf = block & 1;
-                ok = tc_wait_warp(&sm.s_full[x][buf], (uint32_t)((block >> 1) & 1), &sm.abort);
+                ok = tc_wait_warp(&sm.s_full[x][buf], (uint32_t)((block >> 1) & 1), &sm.abort) && ok;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 float t[NR];
                 pw_tmem_ld<NR>(tmem_s + (uint32_t)(buf * NR), t);
@@ -355,36 +357,14 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 for (int n = 0; n < NR; ++n) over |= t[n] - row.ref[n] > 8.0f;
                 // the buffer that the probabilities go to has been read by the product of two blocks before
                 if (block > 1) ok = tc_wait_warp(&sm.pv_done[x][buf], (uint32_t)(((block >> 1) - 1) & 1), &sm.abort) && ok;
-                const int v_entry = pg_v_entry(j, p.blocks);   // of the piece's loads
-                int v_stage = stage + v_entry;
-                uint32_t v_phase = phase;
-                while (v_stage >= kStages) {
-                    v_stage -= kStages;
-                    v_phase ^= 1;
-                }
-                const bool ragged = key0 < span.lo || key0 + kPgKeys > span.hi;
-                if (ragged) {
-                    // rows of V that nobody sees
-                    ok = tc_wait_warp(&sm.full[v_stage], v_phase, &sm.abort) && ok;
-                    if (key < span.lo || key >= span.hi) {
-                        uint4* dst = reinterpret_cast<uint4*>(ring + v_stage * kTile + r * 128);
-#pragma unroll
-                        for (int h = 0; h < kHalves; ++h) {
-#pragma unroll
-                            for (int c = 0; c < 8; ++c) dst[h * (kHalf / 16) + c] = make_uint4(0u, 0u, 0u, 0u);
-                        }
-                    }
-                }
                 if (pw_any(x, over || !ok)) {
                     // Some row's reference moves (or a wait has run out: all leave together).
                     if (j > 0) ok = tc_wait_warp(&sm.pv_done[x][buf ^ 1], (uint32_t)(((block - 1) >> 1) & 1), &sm.abort) && ok;
                     // (no product reads the probabilities now: their place holds the scores for a moment, row by row)
 #pragma unroll
                     for (int n = 0; n < NR; ++n) cross[n * kPgKeys + r] = t[n];
-                    if (pw_any(x, !ok)) {
-                        ok = false;
-                        break;
-                    }
+                    failed = pw_any(x, !ok);
+                    if (failed) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
                     for (int n = warp & 3; n < NR; n += 4) {
@@ -421,24 +401,39 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                     l[n] += e;
                     *reinterpret_cast<T*>(dst + n * 128 + ((piece ^ (n & 7)) << 4)) = (T)e;
                 }
+                if (key0 < span.lo || key0 + kPgKeys > span.hi) {
+                    // rows of V that nobody sees (late: V lands behind K, and this is the first block of most pieces)
+                    int v_stage = stage + pg_v_entry(j, p.blocks);
+                    uint32_t v_phase = phase;
+                    while (v_stage >= kStages) {
+                        v_stage -= kStages;
+                        v_phase ^= 1;
+                    }
+                    ok = tc_wait_warp(&sm.full[v_stage], v_phase, &sm.abort) && ok;   // (told at the next barrier)
+                    if (key < span.lo || key >= span.hi) {
+                        uint4* zero = reinterpret_cast<uint4*>(ring + v_stage * kTile + r * 128);
+#pragma unroll
+                        for (int h = 0; h < kHalves; ++h) {
+#pragma unroll
+                            for (int c = 0; c < 8; ++c) zero[h * (kHalf / 16) + c] = make_uint4(0u, 0u, 0u, 0u);
+                        }
+                    }
+                }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sm.p_ready[x][buf]);
             }
-            if (!ok) break;
+            if (failed) break;
             stage += 2 * p.blocks;
             phase ^= (uint32_t)((stage / kStages) & 1);
             stage %= kStages;
 
             // ---- epilogue: the sums of the threads, then O, a dim a thread
-            if (p.blocks > 0) ok = tc_wait_warp(&sm.pv_done[x][(block - 1) & 1], (uint32_t)(((block - 1) >> 1) & 1), &sm.abort);
+            if (p.blocks > 0) ok = tc_wait_warp(&sm.pv_done[x][(block - 1) & 1], (uint32_t)(((block - 1) >> 1) & 1), &sm.abort) && ok;
 #pragma unroll
             for (int n = 0; n < NR; ++n) cross[n * kPgKeys + r] = l[n];
-            if (pw_any(x, !ok)) {
-                ok = false;
-                break;
-            }
+            if (pw_any(x, !ok)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const bool complete = p.starts && p.ends;
             const PgPartial part = pg_partial(ws, (int)gridDim.x, (int)blockIdx.x, p.starts ? 1 : 0, NR, D);

@@ -85,10 +85,12 @@ __device__ __forceinline__ PgSpan pg_span(const PagedMhaArgs& a, const PgSeq& s,
     return r;
 }
 
+// (The newest keys first: with ALiBi, and mostly without, the largest scores are there, and the reference of the powers stays
+// where the first block puts it.  Oldest first it moved with every block of a head with a steep slope.)
 struct PgPiece {
     PgSeq s;
     int seq, head, tile;
-    int block0, blocks;   // key blocks of it to be worked on; 0: its rows see nothing
+    int top, blocks;      // key blocks top, top - 1, .. of it to be worked on; 0: its rows see nothing
     bool starts, ends;    // whether those begin with its first, end with its last
 };
 
@@ -130,7 +132,7 @@ struct PgShare {
             p.seq = seq;
             p.head = head;
             p.tile = tile;
-            p.block0 = span.first_block() + from;
+            p.top = span.first_block() + to - 1;
             p.blocks = to - from;
             p.starts = from == 0;
             p.ends = at + take == cost;
@@ -320,9 +322,9 @@ __device__ __forceinline__ PgPartial pg_partial(void* ws, int ctas, int cta, int
     return {at, at + rows, reinterpret_cast<float4*>(at + 2 * rows)};
 }
 
-// The header of the CTA's share, written by one thread.
+// The header of a CTA's share (as pg_find_share left it), written by one thread that has time for the divisions.
 __device__ __forceinline__ void pg_write_header(const PagedMhaArgs& a, const PgTiling& g, void* ws, int cta, bool work, const PgShare& share,
-                                                const PgFound& found)
+                                             const PgFound& found)
 {
     PgHeader h = {};
     if (work && share.at > g.extra) {
@@ -342,7 +344,7 @@ struct PgScratch {
     int by_dim;            // O is [D / 4][rows], and a tile of 128 rows holds whole tokens only
 };
 
-// Adds up the partial results of the tiles that end in CTA blockIdx.x of one of the kernels (blockIdx.z), four dims of a row a
+// Adds up the partial results of the tiles that end in CTA blockIdx.x of one of the kernels (blockIdx.z), 16 dims of a row a
 // thread and turn.
 template<typename T, int D>
 __global__ void __launch_bounds__(256) paged_mha_join_kernel(const __grid_constant__ PagedMhaArgs a, PgScratch s0, PgScratch s1)
@@ -355,38 +357,51 @@ __global__ void __launch_bounds__(256) paged_mha_join_kernel(const __grid_consta
     const int group = a.heads / a.kv_heads;
     const int rows = h.tokens * group;
     const int per_tile = s.by_dim ? kPgRows / group * group : s.rows;   // rows of a tile in use
-    for (int i = (int)(blockIdx.y * blockDim.x + threadIdx.x); i < rows * (D / 4); i += (int)(gridDim.y * blockDim.x)) {
-        const int row = s.by_dim ? i % rows : i / (D / 4), d4 = s.by_dim ? i / rows : i % (D / 4);
+    for (int i = (int)(blockIdx.y * blockDim.x + threadIdx.x); i < rows * (D / 16); i += (int)(gridDim.y * blockDim.x)) {
+        const int row = s.by_dim ? i % rows : i / (D / 16), d16 = s.by_dim ? i / rows : i % (D / 16);
         const int at = s.by_dim ? row / per_tile * kPgRows + row % per_tile : row;
-        const size_t o_at = s.by_dim ? (size_t)d4 * s.rows + at : (size_t)at * (D / 4) + d4;
+        const size_t o_at = s.by_dim ? (size_t)(4 * d16) * s.rows + at : (size_t)at * (D / 4) + 4 * d16;
+        const int o_step = s.by_dim ? s.rows : 1;
         float top = -INFINITY, sum = 0.f;
-#pragma unroll 4
+#pragma unroll 8
         for (int c = h.from; c <= cta; ++c) {
             const PgPartial p = pg_partial(s.ws, ctas, c, c == h.from ? 1 : 0, s.rows, D);
             const float l = p.sum[at], m = p.max2[at];
             if (l > 0.f) top = fmaxf(top, m);
         }
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        float4 acc[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
         for (int c = h.from; c <= cta; ++c) {
             const PgPartial p = pg_partial(s.ws, ctas, c, c == h.from ? 1 : 0, s.rows, D);
             const float l = p.sum[at], m = p.max2[at];
-            const float4 o = p.o[o_at];
+            float4 o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = p.o[o_at + e * o_step];
             if (l > 0.f) {   // (a piece that sees nothing has left no O)
                 const float w = ex2_approx(m - top);
                 sum += l * w;
-                acc.x += o.x * w;
-                acc.y += o.y * w;
-                acc.z += o.z * w;
-                acc.w += o.w * w;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    acc[e].x += o[e].x * w;
+                    acc[e].y += o[e].y * w;
+                    acc[e].z += o[e].z * w;
+                    acc[e].w += o[e].w * w;
+                }
             }
         }
         const float inv = sum > 0.f ? 1.f / sum : 0.f;
-        uint2 w;
-        w.x = PgType<T>::pack(acc.x * inv, acc.y * inv);
-        w.y = PgType<T>::pack(acc.z * inv, acc.w * inv);
-        T* dst = (T*)a.out + (size_t)(h.row0 + row / group) * a.o_tok + (size_t)(h.head * group + row % group) * a.o_head + 4 * d4;
-        *reinterpret_cast<uint2*>(dst) = w;
+        T* dst = (T*)a.out + (size_t)(h.row0 + row / group) * a.o_tok + (size_t)(h.head * group + row % group) * a.o_head + 16 * d16;
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+            uint4 w;
+            w.x = PgType<T>::pack(acc[e].x * inv, acc[e].y * inv);
+            w.y = PgType<T>::pack(acc[e].z * inv, acc[e].w * inv);
+            w.z = PgType<T>::pack(acc[e + 1].x * inv, acc[e + 1].y * inv);
+            w.w = PgType<T>::pack(acc[e + 1].z * inv, acc[e + 1].w * inv);
+            *reinterpret_cast<uint4*>(dst + 4 * e) = w;
+        }
     }
 }
 

@@ -24,7 +24,7 @@ namespace {
 
 constexpr int kPgThreads = 320;
 constexpr int kPgStages = 5;
-constexpr int kPgExtra = 2;
+constexpr int kPgExtra = 3;             // a tile's beginning and end cost as much as three blocks
 constexpr uint32_t kPgTmemCols = 512;   // S of a, S of b (their probabilities over them), O of a, O of b: 128 each
 constexpr float kPgNone = -1e20f;       // running maximum of a row that has seen nothing
 
@@ -42,6 +42,9 @@ struct PgSmem {
     uint32_t tmem_base;
     volatile int abort;
     float b_max[kPgRows], b_sum[kPgRows];
+    // what a softmax warp needs between its pieces, out of its registers while it works on one
+    PgShare share[8];
+    PgPiece piece[8];
     PgFound found;
 };
 
@@ -73,8 +76,8 @@ __device__ __forceinline__ PgTurns pg_turns(const PagedMhaArgs& a, const PgPiece
     }
     const PgSpan span = pg_span(a, p.s, token0 + x * tile_tokens, token0 + (x + 1) * tile_tokens);
     const int n = span.blocks();
-    r.first = max(0, span.first_block() - p.block0);
-    r.end = n > 0 ? min(p.blocks, span.first_block() + n - p.block0) : 0;
+    r.first = max(0, p.top - (span.first_block() + n - 1));
+    r.end = n > 0 ? min(p.blocks, p.top - span.first_block() + 1) : 0;
     r.stride = 1;
     return r;
 }
@@ -89,7 +92,11 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     constexpr int kTile = kHalves * kHalf;       // a Q tile, a K or a V block
     extern __shared__ __align__(1024) uint8_t pg_dyn[];
     __shared__ PgSmem sm;
-    uint8_t* q_tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pg_dyn) + 1023) & ~(uintptr_t)1023);
+    if (smem_u32(pg_dyn) & 1023) {   // the swizzle goes by addresses; the alignment above is there, so this does not happen
+        g_device_status = 2;
+        return;
+    }
+    uint8_t* q_tiles = pg_dyn;
     uint8_t* ring = q_tiles + 2 * kTile;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int group = a.heads / a.kv_heads;
@@ -128,10 +135,10 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     PgShare share;
     const bool work = pg_find_share(a, tiling, (int)blockIdx.x, (int)gridDim.x, whole != 0, sm.found, share);
     const uint32_t tmem = sm.tmem_base;
-    if (!whole && threadIdx.x == 0) pg_write_header(a, tiling, ws, (int)blockIdx.x, work, share, sm.found);
     PgPiece p;
 
     if (!work) {
+        if (!whole && threadIdx.x == 0) pg_write_header(a, tiling, ws, (int)blockIdx.x, false, share, sm.found);
     }
     else if (warp == 8) {
         // ------------------------------------------------------------------ producer
@@ -139,6 +146,7 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         int stage = 0, issued = 0, pieces = 0;
         uint32_t phase = 1;                                       // of `empty`: the first round finds the stages free
         bool ok = true;
+        const PgShare all = share;
         while (ok && share.next(a, tiling, p)) {
             if (p.blocks == 0) continue;
             const PgSpan span = pg_span(a, p.s, p.tile * pair_tokens, (p.tile + 1) * pair_tokens);
@@ -158,7 +166,7 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             const PgLoader<D> loader = {a, a.pages + p.seq * a.pages_stride, p.head, span};
             auto put = [&](const CUtensorMap* map, int j, int page) -> bool {
                 if (!tc_wait_warp(&sm.empty[stage], phase, &sm.abort)) return false;
-                loader.load(map, (p.block0 + j) * kPgKeys, page, ring + stage * kTile, &sm.full[stage]);
+                loader.load(map, (p.top - j) * kPgKeys, page, ring + stage * kTile, &sm.full[stage]);
                 ++issued;
                 if (++stage == kPgStages) {
                     stage = 0;
@@ -166,15 +174,16 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 }
                 return true;
             };
-            int page = loader.page(p.block0 * kPgKeys), before = 0;
+            int page = loader.page(p.top * kPgKeys), before = 0;
             for (int j = 0; j <= p.blocks && ok; ++j) {
-                const int next = j + 1 < p.blocks ? loader.page((p.block0 + j + 1) * kPgKeys) : 0;
+                const int next = j + 1 < p.blocks ? loader.page((p.top - j - 1) * kPgKeys) : 0;
                 if (j < p.blocks) ok = put(&map_k, j, page);
                 if (j > 0 && ok) ok = put(&map_v, j - 1, before);
                 before = page;
                 page = next;
             }
         }
+        if (!whole && lane == 0) pg_write_header(a, tiling, ws, (int)blockIdx.x, true, all, sm.found);
         if (sm.abort) {
             // nothing of this CTA may still be on its way when it ends
             for (int e = max(0, issued - kPgStages); e < issued; ++e) {
@@ -293,23 +302,41 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         const int cap = (int)min((long long)a.max_pages << a.page_shift, 0x7fffffffLL);
         int entry0 = 0, used = 0, outs = 0, merges = 0;
         bool ok = true;
-        while (ok && share.next(a, tiling, p)) {
-            const int token0 = p.tile * pair_tokens;
-            const bool split = p.s.tokens - token0 <= tile_tokens;
-            const int token = token0 + (split ? 0 : x * tile_tokens) + tok;      // of the sequence
-            const bool valid = tok < tile_tokens && token < p.s.tokens;
-            const int head = p.head * group + g;
-            const int pos = p.s.p0 + token;
-            const PgTurns turns = pg_turns(a, p, tile_tokens, x);
-            const PgSpan span = pg_span(a, p.s, token0, token0 + pair_tokens);
-            // the keys that this row sees; a row that stands for no token takes whatever comes
-            int low = valid ? p.s.first : 0, high = valid ? min(pos, cap - 1) : 0x7fffffff;
-            if (valid && a.window > 0) low = (int)max((long long)low, (long long)pos - a.window + 1);
+        if (lane == 0) sm.share[warp] = share;
+        __syncwarp();
+        while (ok) {
+            PgTurns turns;
+            PgSpan span;
+            int top, blocks, low, high, pos;
             float slope = 0.f;
-            if (kBias && valid && a.slopes != nullptr) slope = a.slopes[head];
+            {
+                PgShare walk = sm.share[warp];
+                if (!walk.next(a, tiling, p)) break;
+                __syncwarp();
+                if (lane == 0) {
+                    sm.share[warp] = walk;
+                    sm.piece[warp] = p;
+                }
+                __syncwarp();
+                const int token0 = p.tile * pair_tokens;
+                const bool split = p.s.tokens - token0 <= tile_tokens;
+                const int token = token0 + (split ? 0 : x * tile_tokens) + tok;      // of the sequence
+                const bool valid = tok < tile_tokens && token < p.s.tokens;
+                pos = p.s.p0 + token;
+                top = p.top;
+                blocks = p.blocks;
+                turns = pg_turns(a, p, tile_tokens, x);
+                span = pg_span(a, p.s, token0, token0 + pair_tokens);
+                // the keys that this row sees; a row that stands for no token takes whatever comes
+                low = valid ? p.s.first : 0;
+                high = valid ? min(pos, cap - 1) : 0x7ffffffe;
+                if (valid && a.window > 0) low = (int)max((long long)low, (long long)pos - a.window + 1);
+                if (kBias && valid && a.slopes != nullptr) slope = a.slopes[p.head * group + g];
+            }
+            const uint64_t rise[2] = {pair2(0.f, slope), pair2(2.f * slope, 3.f * slope)};   // of the bias over four keys
             float m_run = kPgNone, m_ref = kPgNone, l_run = 0.f;
             for (int j = turns.first; j < turns.end && ok; j += turns.stride) {
-                const int key0 = (p.block0 + j) * kPgKeys;
+                const int key0 = (top - j) * kPgKeys;
                 if (!tc_wait_warp(&sm.s_full[x], (uint32_t)(used & 1), &sm.abort)) {
                     ok = false;
                     break;
@@ -320,17 +347,25 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 const bool masked = !__all_sync(0xffffffffu, low <= key0 && high >= key0 + kPgKeys - 1);
                 auto finish = [&](uint32_t* v, int c0) {
                     if (kBias) {
-                        const float base = slope * (float)(key0 + c0 - pos);
 #pragma unroll
-                        for (int c = 0; c < 32; ++c) {
-                            v[c] = __float_as_uint(fmaf(__uint_as_float(v[c]), a.scale, fmaf(slope, (float)c, base)));
+                        for (int c = 0; c < 32; c += 4) {
+                            const float base = slope * (float)(key0 + c0 + c - pos);
+                            const uint64_t base2 = pair2(base, base);
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const float2 t = split2(fma2(pair2(__uint_as_float(v[c + 2 * e]), __uint_as_float(v[c + 2 * e + 1])),
+                                                             pair2(a.scale, a.scale), add2(base2, rise[e])));
+                                v[c + 2 * e] = __float_as_uint(t.x);
+                                v[c + 2 * e + 1] = __float_as_uint(t.y);
+                            }
                         }
                     }
                     if (masked) {
-                        const int from = low - key0 - c0, to = high - key0 - c0;
+                        const int from = min(max(low - key0 - c0, 0), 32), to = min(max(high + 1 - key0 - c0, 0), 32);
+                        const uint32_t seen = (to < 32 ? (1u << to) - 1 : 0xffffffffu) & ~(from < 32 ? (1u << from) - 1 : 0xffffffffu);
 #pragma unroll
                         for (int c = 0; c < 32; ++c) {
-                            if (c < from || c > to) v[c] = 0xff800000u;   // -inf
+                            if (!(seen & (1u << c))) v[c] = 0xff800000u;   // -inf
                         }
                     }
                 };
@@ -378,23 +413,6 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                         tmem_st16_async(t_o + (uint32_t)c0, o);
                     }
                 }
-                if (key0 < span.lo || key0 + kPgKeys > span.hi) {
-                    // rows of V that nobody sees
-                    const int entry = entry0 + pg_v_entry(j, p.blocks), stage = entry % kPgStages;
-                    if (!tc_wait_warp(&sm.full[stage], (uint32_t)((entry / kPgStages) & 1), &sm.abort)) {
-                        ok = false;
-                        break;
-                    }
-                    if (key0 + r < span.lo || key0 + r >= span.hi) {
-                        uint4* dst = reinterpret_cast<uint4*>(ring + stage * kTile + r * 128);
-#pragma unroll
-                        for (int h = 0; h < kHalves; ++h) {
-#pragma unroll
-                            for (int c = 0; c < 8; ++c) dst[h * (kHalf / 16) + c] = make_uint4(0u, 0u, 0u, 0u);
-                        }
-                    }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                }
                 const uint64_t scale2 = pair2(to_log2, to_log2), off2 = pair2(-m_ref * to_log2, -m_ref * to_log2);
                 uint64_t psum[2] = {0ull, 0ull};
                 auto exponents = [&](const uint32_t* v, uint32_t* pk) {
@@ -412,6 +430,23 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 tmem_ld32_async(t_s + 64, v);
                 tmem_ld32_async(t_s + 96, v + 32);
                 tmem_st32_async(t_s, pk);
+                if (key0 < span.lo || key0 + kPgKeys > span.hi) {
+                    // rows of V that nobody sees
+                    const int entry = entry0 + pg_v_entry(j, blocks), stage = entry % kPgStages;
+                    if (!tc_wait_warp(&sm.full[stage], (uint32_t)((entry / kPgStages) & 1), &sm.abort)) {
+                        ok = false;
+                        break;
+                    }
+                    if (key0 + r < span.lo || key0 + r >= span.hi) {
+                        uint4* dst = reinterpret_cast<uint4*>(ring + stage * kTile + r * 128);
+#pragma unroll
+                        for (int h = 0; h < kHalves; ++h) {
+#pragma unroll
+                            for (int c = 0; c < 8; ++c) dst[h * (kHalf / 16) + c] = make_uint4(0u, 0u, 0u, 0u);
+                        }
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                }
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
@@ -429,8 +464,14 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 const float2 ps = split2(add2(psum[0], psum[1]));
                 l_run = l_run * corr + (ps.x + ps.y);
             }
-            entry0 += 2 * p.blocks;
+            entry0 += 2 * blocks;
             if (!ok) break;
+            p = sm.piece[warp];
+            const int token0 = p.tile * pair_tokens;
+            const bool split = p.s.tokens - token0 <= tile_tokens;
+            const int token = token0 + (split ? 0 : x * tile_tokens) + tok;
+            const bool valid = tok < tile_tokens && token < p.s.tokens;
+            const int head = p.head * group + g;
             const bool mine = turns.any();
             if (mine) {
                 if (!tc_wait_warp(&sm.o_full[x], (uint32_t)(outs & 1), &sm.abort)) {
@@ -537,7 +578,7 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 template<typename T, int D, bool kBias>
 int pg_launch_tc(const PagedMhaArgs& a, void* ws, int least, int whole, cudaStream_t stream)
 {
-    constexpr int kSmem = (2 + kPgStages) * (D / 64) * kPgRows * 128 + 1024;
+    constexpr int kSmem = (2 + kPgStages) * (D / 64) * kPgRows * 128;
     CUtensorMap map_q, map_k, map_v;
     if (int rc = pg_encode_maps<T, D>(a, kPgRows / (a.heads / a.kv_heads), &map_q, &map_k, &map_v)) return rc;
     auto kern = paged_mha_tc_kernel<T, D, kBias>;

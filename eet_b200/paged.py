@@ -23,7 +23,7 @@ import struct
 import torch
 
 from ._lib import check, lib
-from .EET import _on, _ptr, _stream
+from .EET import _on, _stream
 
 __all__ = ["rotary_frequencies", "apply_rotary", "paged_store", "paged_mha"]
 
@@ -31,7 +31,9 @@ _DTYPES = (torch.float16, torch.bfloat16)
 _PAGE_SIZES = (16, 32, 64, 128, 256)
 _pack_rotary = struct.Struct("6P15qd").pack
 _pack_store = struct.Struct("11P26qd").pack
-_pack_mha = struct.Struct("9P23qdPq").pack
+_pack_mha = struct.Struct("9P23qd").pack
+_pack_scratch = struct.Struct("Pq").pack
+_NO_SCRATCH = _pack_scratch(0, 0)
 
 
 def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, device="cuda:0"):
@@ -80,42 +82,42 @@ def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, device="cuda:0"):
     return torch.tensor(freqs, dtype=torch.float64, device=device), magnitude
 
 
-def _heads(who, name, t, like, heads=None, head_dim=None):
-    """The token and head strides of a [tokens, heads, head_dim] tensor that stands beside `like`."""
-    shape = t.shape
-    if len(shape) != 3 or t.dtype != like.dtype or t.device != like.device:
-        raise RuntimeError(f"{who}: {name} must be a CUDA {like.dtype} tensor [tokens, heads, head_dim] on {like.device}, got "
-                           f"{tuple(shape)} {t.dtype} on {t.device}")
-    if shape[0] != like.shape[0] or shape[2] != (head_dim or like.shape[2]) or (heads is not None and shape[1] != heads):
-        raise RuntimeError(f"{who}: {name} has shape {tuple(shape)} beside {tuple(like.shape)}")
-    strides = t.stride()
-    if strides[2] != 1:
-        raise RuntimeError(f"{who}: the last dimension of {name} must be contiguous")
-    return strides[0], strides[1]
-
-
+# The checks below run once per tensor and call; a decode step's calls last about as long on the host as on the GPU, so each
+# reads as few attributes as it can (a device is compared as its index, -1 for the CPU's).
 def _first(who, name, t):
-    if t.dim() != 3 or t.dtype not in _DTYPES or not t.is_cuda:
-        raise RuntimeError(f"{who}: {name} must be a CUDA fp16 or bf16 tensor [tokens, heads, head_dim], got {tuple(t.shape)} {t.dtype} "
+    """(tokens, heads, head_dim) of the tensor that the others are held against."""
+    shape = t.shape
+    if len(shape) != 3 or t.dtype not in _DTYPES or t.get_device() < 0:
+        raise RuntimeError(f"{who}: {name} must be a CUDA fp16 or bf16 tensor [tokens, heads, head_dim], got {tuple(shape)} {t.dtype} "
                            f"on {t.device}")
+    return shape
 
 
-def _index(who, name, t, dtype, numel, device):
-    if t.dtype != dtype or t.device != device or t.dim() != 1 or t.numel() != numel or (numel > 1 and t.stride(0) != 1):
-        raise RuntimeError(f"{who}: {name} must be a contiguous {dtype} tensor [{numel}] on {device}, got {tuple(t.shape)} {t.dtype} on "
+def _heads(who, name, t, shape, dtype, index):
+    """Token and head strides of a tensor that must have this shape."""
+    strides = t.stride()
+    if t.shape != shape or t.dtype != dtype or t.get_device() != index or strides[2] != 1:
+        raise RuntimeError(f"{who}: {name} must be a {dtype} tensor of shape {tuple(shape)} with a contiguous last dimension on cuda:{index}, "
+                           f"got {tuple(t.shape)} {t.dtype} with strides {strides} on {t.device}")
+    return strides[:2]
+
+
+def _array(who, name, t, dtype, numel, index):
+    """The address of a contiguous vector on the device."""
+    if t.dtype != dtype or t.get_device() != index or t.shape != (numel,) or not t.is_contiguous():
+        raise RuntimeError(f"{who}: {name} must be a contiguous {dtype} tensor [{numel}] on cuda:{index}, got {tuple(t.shape)} {t.dtype} on "
                            f"{t.device}")
     return t.data_ptr()
 
 
-def _cache(who, k_cache, v_cache, like):
+def _cache(who, k_cache, v_cache, dtype, index):
     """(pages, kv_heads, page_size, head_dim) and the strides of a cache."""
     shape = k_cache.shape
     if len(shape) != 4 or v_cache.shape != shape:
         raise RuntimeError(f"{who}: k_cache and v_cache must both be [pages, kv_heads, page_size, head_dim], got {tuple(shape)} and "
                            f"{tuple(v_cache.shape)}")
-    dtype, device = like.dtype, like.device
-    if k_cache.dtype != dtype or v_cache.dtype != dtype or k_cache.device != device or v_cache.device != device:
-        raise RuntimeError(f"{who}: the caches must be {dtype} on {device}, as the other tensors are")
+    if k_cache.dtype != dtype or v_cache.dtype != dtype or k_cache.get_device() != index or v_cache.get_device() != index:
+        raise RuntimeError(f"{who}: the caches must be {dtype} on cuda:{index}, as the other tensors are")
     ks, vs = k_cache.stride(), v_cache.stride()
     if ks[3] != 1 or vs[3] != 1:
         raise RuntimeError(f"{who}: the last dimension of the caches must be contiguous")
@@ -124,15 +126,16 @@ def _cache(who, k_cache, v_cache, like):
     return shape, ks[:3] + vs[:3]
 
 
-def _table(who, pages, starts, lens, device):
-    """(sequences, columns, row stride) of the page table."""
-    if pages.dim() != 2 or pages.dtype != torch.int32 or pages.device != device or (pages.shape[1] > 1 and pages.stride(1) != 1):
-        raise RuntimeError(f"{who}: pages must be an int32 tensor [sequences, columns] with contiguous rows on {device}, got "
-                           f"{tuple(pages.shape)} {pages.dtype} on {pages.device}")
-    seqs, columns = pages.shape
-    _index(who, "starts", starts, torch.int32, seqs + 1, device)
-    _index(who, "lens", lens, torch.int32, seqs, device)
-    return seqs, columns, pages.stride(0) if seqs > 1 else columns
+def _table(who, pages, starts, lens, index):
+    """(sequences, columns, row stride) of the page table, the addresses of it, starts and lens."""
+    shape = pages.shape
+    if len(shape) != 2 or pages.dtype != torch.int32 or pages.get_device() != index or (shape[1] > 1 and pages.stride(1) != 1):
+        raise RuntimeError(f"{who}: pages must be an int32 tensor [sequences, columns] with contiguous rows on cuda:{index}, got "
+                           f"{tuple(shape)} {pages.dtype} on {pages.device}")
+    seqs, columns = shape
+    addresses = (pages.data_ptr(), _array(who, "starts", starts, torch.int32, seqs + 1, index),
+                 _array(who, "lens", lens, torch.int32, seqs, index))
+    return seqs, columns, pages.stride(0) if seqs > 1 else columns, addresses
 
 
 def apply_rotary(q, k, positions, freqs, interleaved=False, magnitude=1.0, q_out=None, k_out=None):
@@ -143,32 +146,36 @@ def apply_rotary(q, k, positions, freqs, interleaved=False, magnitude=1.0, q_out
     multiple of 16 - the rest of a head is copied.  Pair i is dims (i, i + rotary_dim / 2), with `interleaved` (2 i, 2 i + 1).
     Token and head strides are free (a view of a fused projection will do) but multiples of 8."""
     who = "apply_rotary"
-    like = q if q is not None else k
+    like = k if q is None else q
     if like is None:
         raise RuntimeError("apply_rotary: neither q nor k is given")
-    _first(who, "k" if q is None else "q", like)
-    tokens, _, head_dim = like.shape
-    device = like.device
-    heads = kv_heads = 0
-    strides = [0] * 8
-    if q is not None:
-        heads = q.shape[1]
-        q_out = torch.empty((tokens, heads, head_dim), dtype=q.dtype, device=device) if q_out is None else q_out
-        strides[0:2], strides[4:6] = _heads(who, "q", q, like), _heads(who, "q_out", q_out, like, heads)
+    tokens, heads, head_dim = _first(who, "k" if q is None else "q", like)
+    dtype, device, index = like.dtype, like.device, like.get_device()
+    kv_heads = 0
+    q_str = qo_str = k_str = ko_str = (0, 0)
+    q_at = qo_at = k_at = ko_at = 0
+    if q is None:
+        heads = 0
+    else:
+        if q_out is None:
+            q_out = torch.empty(tokens, heads, head_dim, dtype=dtype, device=device)
+        q_str, qo_str = _heads(who, "q", q, q.shape, dtype, index), _heads(who, "q_out", q_out, q.shape, dtype, index)
+        q_at, qo_at = q.data_ptr(), q_out.data_ptr()
     if k is not None:
-        strides[2:4] = _heads(who, "k", k, like)
-        kv_heads = k.shape[1]
-        k_out = torch.empty((tokens, kv_heads, head_dim), dtype=k.dtype, device=device) if k_out is None else k_out
-        strides[6:8] = _heads(who, "k_out", k_out, like, kv_heads)
-    where = _index(who, "positions", positions, torch.int64, tokens, device)
-    rotary_dim = 2 * freqs.numel()
-    turns = _index(who, "freqs", freqs, torch.float64, rotary_dim // 2, device)
-    args = _pack_rotary(_ptr(q) or 0, _ptr(k) or 0, _ptr(q_out) or 0 if heads else 0, _ptr(k_out) or 0 if kv_heads else 0, where, turns,
-                        tokens, heads, kv_heads, head_dim, rotary_dim, bool(interleaved), like.dtype == torch.bfloat16, *strides,
-                        magnitude)
+        shape = k.shape
+        kv_heads = shape[1] if len(shape) == 3 else 0
+        k_str = _heads(who, "k", k, (tokens, kv_heads, head_dim), dtype, index)
+        if k_out is None:
+            k_out = torch.empty(tokens, kv_heads, head_dim, dtype=dtype, device=device)
+        ko_str = _heads(who, "k_out", k_out, shape, dtype, index)
+        k_at, ko_at = k.data_ptr(), k_out.data_ptr()
+    half = freqs.numel()
+    args = _pack_rotary(q_at, k_at, qo_at, ko_at, _array(who, "positions", positions, torch.int64, tokens, index),
+                        _array(who, "freqs", freqs, torch.float64, half, index), tokens, heads, kv_heads, head_dim, 2 * half,
+                        bool(interleaved), dtype == torch.bfloat16, *q_str, *k_str, *qo_str, *ko_str, magnitude)
     with _on(device):
         check(lib.eet_rotary(args, _stream()))
-    return q_out if heads else q_out, k_out
+    return q_out, k_out
 
 
 def paged_store(k, v, k_cache, v_cache, pages, starts, lens, q=None, freqs=None, interleaved=False, magnitude=1.0, positions=None,
@@ -180,33 +187,33 @@ def paged_store(k, v, k_cache, v_cache, pages, starts, lens, q=None, freqs=None,
     sequence are not touched.  Two sequences must not append to the same slot (one that they share must lie before both's new
     tokens)."""
     who = "paged_store"
-    _first(who, "k", k)
-    tokens, kv_heads, head_dim = k.shape
-    device = k.device
-    k_str, v_str = _heads(who, "k", k, k), _heads(who, "v", v, k, kv_heads)
-    shape, cache_strides = _cache(who, k_cache, v_cache, k)
-    if shape[1] != kv_heads or shape[3] != head_dim:
-        raise RuntimeError(f"paged_store: caches of {shape[1]} heads of {shape[3]} beside {kv_heads} heads of {head_dim}")
-    seqs, columns, pages_stride = _table(who, pages, starts, lens, device)
-    heads, q_str, qo_str = 0, (0, 0), (0, 0)
+    shape = tokens, kv_heads, head_dim = _first(who, "k", k)
+    dtype, device, index = k.dtype, k.device, k.get_device()
+    k_str, v_str = _heads(who, "k", k, shape, dtype, index), _heads(who, "v", v, shape, dtype, index)
+    cache_shape, cache_strides = _cache(who, k_cache, v_cache, dtype, index)
+    if cache_shape[1] != kv_heads or cache_shape[3] != head_dim:
+        raise RuntimeError(f"paged_store: caches of {cache_shape[1]} heads of {cache_shape[3]} beside {kv_heads} heads of {head_dim}")
+    seqs, columns, pages_stride, table = _table(who, pages, starts, lens, index)
+    heads, q_str, qo_str, q_at, qo_at = 0, (0, 0), (0, 0), 0, 0
     if q is not None:
-        q_str = _heads(who, "q", q, k)
-        heads = q.shape[1]
+        q_shape = q.shape
+        heads = q_shape[1] if len(q_shape) == 3 else 0
+        q_str = _heads(who, "q", q, (tokens, heads, head_dim), dtype, index)
         if q_out is None:
-            q_out = torch.empty((tokens, heads, head_dim), dtype=q.dtype, device=device)
-        qo_str = _heads(who, "q_out", q_out, k, heads)
+            q_out = torch.empty(tokens, heads, head_dim, dtype=dtype, device=device)
+        qo_str = _heads(who, "q_out", q_out, q_shape, dtype, index)
+        q_at, qo_at = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         raise RuntimeError("paged_store: q_out without q")
-    rotary_dim = turns = where = 0
+    half = turns = where = 0
     if freqs is not None:
-        rotary_dim = 2 * freqs.numel()
-        turns = _index(who, "freqs", freqs, torch.float64, rotary_dim // 2, device)
+        half = freqs.numel()
+        turns = _array(who, "freqs", freqs, torch.float64, half, index)
     if positions is not None:
-        where = _index(who, "positions", positions, torch.int64, tokens, device)
-    args = _pack_store(_ptr(q) or 0, _ptr(k) or 0, _ptr(v) or 0, _ptr(q_out) or 0, _ptr(k_cache) or 0, _ptr(v_cache) or 0,
-                       pages.data_ptr(), starts.data_ptr(), lens.data_ptr(), where, turns, tokens, seqs, heads, kv_heads, head_dim,
-                       rotary_dim, bool(interleaved), k.dtype == torch.bfloat16, shape[0], shape[2], columns, pages_stride, *q_str, *k_str,
-                       *v_str, *qo_str, *cache_strides, magnitude)
+        where = _array(who, "positions", positions, torch.int64, tokens, index)
+    args = _pack_store(q_at, k.data_ptr(), v.data_ptr(), qo_at, k_cache.data_ptr(), v_cache.data_ptr(), *table, where, turns, tokens, seqs,
+                       heads, kv_heads, head_dim, 2 * half, bool(interleaved), dtype == torch.bfloat16, cache_shape[0], cache_shape[2],
+                       columns, pages_stride, *q_str, *k_str, *v_str, *qo_str, *cache_strides, magnitude)
     with _on(device):
         check(lib.eet_paged_store(args, _stream()))
     return q_out
@@ -228,31 +235,29 @@ def paged_mha(q, k_cache, v_cache, pages, starts, lens, max_tokens=None, max_len
     Rows of out that belong to no sequence are left as they are, uninitialised where this call allocated out.
     K and V of every position that a token of the same tile sees must be finite."""
     who = "paged_mha"
-    _first(who, "q", q)
-    tokens, heads, head_dim = q.shape
-    device = q.device
-    q_str = _heads(who, "q", q, q)
-    shape, cache_strides = _cache(who, k_cache, v_cache, q)
-    if shape[3] != head_dim:
-        raise RuntimeError(f"paged_mha: caches of head size {shape[3]} beside a q of {head_dim}")
-    seqs, columns, pages_stride = _table(who, pages, starts, lens, device)
+    shape = tokens, heads, head_dim = _first(who, "q", q)
+    dtype, device, index = q.dtype, q.device, q.get_device()
+    q_str = _heads(who, "q", q, shape, dtype, index)
+    cache_shape, cache_strides = _cache(who, k_cache, v_cache, dtype, index)
+    if cache_shape[3] != head_dim:
+        raise RuntimeError(f"paged_mha: caches of head size {cache_shape[3]} beside a q of {head_dim}")
+    seqs, columns, pages_stride, table = _table(who, pages, starts, lens, index)
     if out is None:
-        out = torch.empty((tokens, heads, head_dim), dtype=q.dtype, device=device)
-    o_str = _heads(who, "out", out, q, heads)
-    first = _index(who, "first_key", first_key, torch.int32, seqs, device) if first_key is not None else 0
-    slopes = _index(who, "alibi_slopes", alibi_slopes, torch.float32, heads, device) if alibi_slopes is not None else 0
+        out = torch.empty(tokens, heads, head_dim, dtype=dtype, device=device)
+    o_str = _heads(who, "out", out, shape, dtype, index)
+    first = 0 if first_key is None else _array(who, "first_key", first_key, torch.int32, seqs, index)
+    slopes = 0 if alibi_slopes is None else _array(who, "alibi_slopes", alibi_slopes, torch.float32, heads, index)
     if max_tokens is None:
         max_tokens = 1 if tokens == seqs else tokens
-    if scale is None:
-        scale = 1.0 / math.sqrt(head_dim)
-    fields = [_ptr(q) or 0, _ptr(k_cache) or 0, _ptr(v_cache) or 0, _ptr(out) or 0, pages.data_ptr(), starts.data_ptr(), lens.data_ptr(),
-              first, slopes, tokens, seqs, heads, shape[1], head_dim, q.dtype == torch.bfloat16, shape[0], shape[2], columns, pages_stride,
-              *q_str, *o_str, *cache_strides, window, max_tokens, max_len or 0, scale]
+    args = _pack_mha(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), *table, first, slopes, tokens, seqs, heads,
+                     cache_shape[1], head_dim, dtype == torch.bfloat16, cache_shape[0], cache_shape[2], columns, pages_stride, *q_str,
+                     *o_str, *cache_strides, window, max_tokens, max_len or 0, 1.0 / math.sqrt(head_dim) if scale is None else scale)
     with _on(device):
-        args = _pack_mha(*fields, 0, 0)
-        ws_bytes = lib.eet_paged_mha_workspace_bytes(args)
+        ws_bytes = lib.eet_paged_mha_workspace_bytes(args + _NO_SCRATCH)
         if ws_bytes:
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
-            args = _pack_mha(*fields, ws.data_ptr(), ws_bytes)
+            args += _pack_scratch(ws.data_ptr(), ws_bytes)
+        else:
+            args += _NO_SCRATCH
         check(lib.eet_paged_mha(args, _stream()))
     return out

@@ -93,7 +93,8 @@ def _mha(**kw):
              o_tok=1024, o_head=128, kc_page=4096, kc_head=2048, kc_slot=128, vc_page=4096, vc_head=2048, vc_slot=128, window=0,
              max_tokens=2, max_len=64, scale=0.1, ws=0, ws_bytes=0)
     f.update(kw)
-    return paged._pack_mha(*f.values())
+    *fields, ws, ws_bytes = f.values()
+    return paged._pack_mha(*fields) + paged._pack_scratch(ws, ws_bytes)
 
 
 @pytest.mark.parametrize("change,message", [
