@@ -185,15 +185,18 @@ static PagedPlan paged_plan(const PagedMhaArgs& a)
         if (others > 0) p.nr = rows_for((rest + others - 1) / others);
         p.few = p.nr / group;
     }
-    // Cutting tiles evens out the shares and costs a second launch, some 4 us or the time of five blocks: not where whole tiles
-    // make the longest share no more than that longer (taking sequences to be half as long as the longest).
-    auto whole = [&](long long tokens) {
-        const long long sms = sm_count(), blocks = (a.max_len + kPgKeys - 1) / kPgKeys;
+    // Cutting tiles evens out the shares and costs a second launch: 4 us behind the first kernel, 7 behind the second, whose blocks
+    // take 0.8 us and 1.4 (heads of 64) or 1.9 us.  Not where whole tiles make the longest share no more than that longer, taking
+    // tiles to be three quarters as long as the longest on average.
+    auto whole = [&](long long tokens, int most) {
+        const long long sms = sm_count();
+        const long long keys = a.window > 0 && a.window + tokens < a.max_len ? a.window + tokens : a.max_len;
+        const long long blocks = keys / kPgKeys + 1;
         const long long tiles = (a.seqs + (a.max_tokens > tokens ? a.tokens / tokens : 0)) * a.kv_heads;
-        return blocks - (tiles < sms ? blocks * tiles / (2 * sms) : 0) <= 5;
+        return blocks - (tiles < sms ? 3 * blocks * tiles / (4 * sms) : 0) <= most;
     };
-    if (p.nr > 0) p.whole[0] = whole(p.nr / group);
-    if (p.tiles) p.whole[1] = whole(2 * (kPgRows / group));
+    if (p.nr > 0) p.whole[0] = whole(p.nr / group, 5);
+    if (p.tiles) p.whole[1] = whole(2 * (kPgRows / group), 4);
     if (p.nr > 0 && !p.whole[0]) p.bytes[0] = pg_scratch_bytes(sm_count(), p.nr, a.head_dim);
     if (p.tiles && !p.whole[1]) p.bytes[1] = pg_scratch_bytes(sm_count(), 2 * kPgRows, a.head_dim);
     return p;

@@ -366,13 +366,17 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                     failed = pw_any(x, !ok);
                     if (failed) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    // (eight lanes a row: four rows of a warp at once)
 #pragma unroll 1
-                    for (int n = warp & 3; n < NR; n += 4) {
-                        const float4 v = reinterpret_cast<const float4*>(cross + n * kPgKeys)[lane];
-                        const float m = warp_max(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
-                        const float old = row.ref[n];
-                        __syncwarp();
-                        if (lane == 0) {
+                    for (int n = (warp & 3) * 4 + (lane >> 3); n < NR; n += 16) {
+                        const float4* v = reinterpret_cast<const float4*>(cross + n * kPgKeys) + (lane & 7);
+                        float m = -INFINITY;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) m = fmaxf(m, fmaxf(fmaxf(v[8 * i].x, v[8 * i].y), fmaxf(v[8 * i].z, v[8 * i].w)));
+#pragma unroll
+                        for (int o = 4; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                        if ((lane & 7) == 0) {
+                            const float old = row.ref[n];
                             row.corr[n] = m - old > 8.0f ? ex2_approx(old - m) : 1.0f;
                             row.ref[n] = m - old > 8.0f ? m : old;
                         }
@@ -438,10 +442,14 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             const bool complete = p.starts && p.ends;
             const PgPartial part = pg_partial(ws, (int)gridDim.x, (int)blockIdx.x, p.starts ? 1 : 0, NR, D);
 #pragma unroll 1
-            for (int n = warp & 3; n < rows; n += 4) {
-                const float4 v = reinterpret_cast<const float4*>(cross + n * kPgKeys)[lane];
-                const float sum = warp_sum((v.x + v.y) + (v.z + v.w));
-                if (lane == 0) {
+            for (int n = (warp & 3) * 4 + (lane >> 3); n < NR; n += 16) {
+                const float4* v = reinterpret_cast<const float4*>(cross + n * kPgKeys) + (lane & 7);
+                float sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum += (v[8 * i].x + v[8 * i].y) + (v[8 * i].z + v[8 * i].w);
+#pragma unroll
+                for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                if ((lane & 7) == 0) {
                     row.corr[n] = sum > 0.f ? 1.0f / sum : 0.f;
                     if (!complete) {
                         part.max2[n] = row.ref[n];

@@ -344,12 +344,13 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 ++used;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 // scores of keys c0 .. c0 + 31 of the block: bias, masks
+                float base0 = kBias ? slope * (float)(key0 - pos) : 0.f;
                 const bool masked = !__all_sync(0xffffffffu, low <= key0 && high >= key0 + kPgKeys - 1);
                 auto finish = [&](uint32_t* v, int c0) {
                     if (kBias) {
 #pragma unroll
                         for (int c = 0; c < 32; c += 4) {
-                            const float base = slope * (float)(key0 + c0 + c - pos);
+                            const float base = fmaf(slope, (float)(c0 + c), base0);
                             const uint64_t base2 = pair2(base, base);
 #pragma unroll
                             for (int e = 0; e < 2; ++e) {
@@ -424,12 +425,13 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                         pk[c] = PgType<T>::pack(p0, p1);
                     }
                 };
-                uint32_t pk[32];
+                uint32_t pk[16];
                 exponents(v, pk);
-                exponents(v + 32, pk + 16);
+                tmem_st16_async(t_s, pk);
+                exponents(v + 32, pk);
+                tmem_st16_async(t_s + 16, pk);
                 tmem_ld32_async(t_s + 64, v);
                 tmem_ld32_async(t_s + 96, v + 32);
-                tmem_st32_async(t_s, pk);
                 if (key0 < span.lo || key0 + kPgKeys > span.hi) {
                     // rows of V that nobody sees
                     const int entry = entry0 + pg_v_entry(j, blocks), stage = entry % kPgStages;
@@ -452,11 +454,13 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sm.p_half[x]);
                 tmem_ld_wait(v);
+                if (kBias) asm volatile("" : "+f"(base0), "+f"(slope));   // (or the bias would be kept from the first time, in 64 registers)
                 finish(v, 64);
                 finish(v + 32, 96);
                 exponents(v, pk);
-                exponents(v + 32, pk + 16);
-                tmem_st32_async(t_s + 32, pk);
+                tmem_st16_async(t_s + 32, pk);
+                exponents(v + 32, pk);
+                tmem_st16_async(t_s + 48, pk);
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();

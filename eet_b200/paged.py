@@ -23,7 +23,7 @@ import struct
 import torch
 
 from ._lib import check, lib
-from .EET import _on, _stream
+from .EET import _current_device, _raw_stream
 
 __all__ = ["rotary_frequencies", "apply_rotary", "paged_store", "paged_mha"]
 
@@ -102,6 +102,30 @@ def _heads(who, name, t, shape, dtype, index):
     return strides[:2]
 
 
+def _output(who, name, t, shape, dtype, device, index):
+    """The tensor for a result, and its token and head strides."""
+    if t is not None:
+        return t, _heads(who, name, t, shape, dtype, index)
+    tokens, heads, head_dim = shape
+    return torch.empty(tokens, heads, head_dim, dtype=dtype, device=device), (heads * head_dim, head_dim)
+
+
+def _call(function, args, index):
+    """One entry point on the current stream of the tensors' device."""
+    if index == _current_device():
+        check(function(args, _raw_stream(index)))
+    else:
+        with torch.cuda.device(index):
+            check(function(args, _raw_stream(index)))
+
+
+def _workspace_bytes(args, index):
+    if index == _current_device():
+        return lib.eet_paged_mha_workspace_bytes(args + _NO_SCRATCH)
+    with torch.cuda.device(index):
+        return lib.eet_paged_mha_workspace_bytes(args + _NO_SCRATCH)
+
+
 def _array(who, name, t, dtype, numel, index):
     """The address of a contiguous vector on the device."""
     if t.dtype != dtype or t.get_device() != index or t.shape != (numel,) or not t.is_contiguous():
@@ -157,24 +181,20 @@ def apply_rotary(q, k, positions, freqs, interleaved=False, magnitude=1.0, q_out
     if q is None:
         heads = 0
     else:
-        if q_out is None:
-            q_out = torch.empty(tokens, heads, head_dim, dtype=dtype, device=device)
-        q_str, qo_str = _heads(who, "q", q, q.shape, dtype, index), _heads(who, "q_out", q_out, q.shape, dtype, index)
+        q_str = _heads(who, "q", q, q.shape, dtype, index)
+        q_out, qo_str = _output(who, "q_out", q_out, (tokens, heads, head_dim), dtype, device, index)
         q_at, qo_at = q.data_ptr(), q_out.data_ptr()
     if k is not None:
         shape = k.shape
         kv_heads = shape[1] if len(shape) == 3 else 0
         k_str = _heads(who, "k", k, (tokens, kv_heads, head_dim), dtype, index)
-        if k_out is None:
-            k_out = torch.empty(tokens, kv_heads, head_dim, dtype=dtype, device=device)
-        ko_str = _heads(who, "k_out", k_out, shape, dtype, index)
+        k_out, ko_str = _output(who, "k_out", k_out, (tokens, kv_heads, head_dim), dtype, device, index)
         k_at, ko_at = k.data_ptr(), k_out.data_ptr()
     half = freqs.numel()
     args = _pack_rotary(q_at, k_at, qo_at, ko_at, _array(who, "positions", positions, torch.int64, tokens, index),
                         _array(who, "freqs", freqs, torch.float64, half, index), tokens, heads, kv_heads, head_dim, 2 * half,
                         bool(interleaved), dtype == torch.bfloat16, *q_str, *k_str, *qo_str, *ko_str, magnitude)
-    with _on(device):
-        check(lib.eet_rotary(args, _stream()))
+    _call(lib.eet_rotary, args, index)
     return q_out, k_out
 
 
@@ -199,9 +219,7 @@ def paged_store(k, v, k_cache, v_cache, pages, starts, lens, q=None, freqs=None,
         q_shape = q.shape
         heads = q_shape[1] if len(q_shape) == 3 else 0
         q_str = _heads(who, "q", q, (tokens, heads, head_dim), dtype, index)
-        if q_out is None:
-            q_out = torch.empty(tokens, heads, head_dim, dtype=dtype, device=device)
-        qo_str = _heads(who, "q_out", q_out, q_shape, dtype, index)
+        q_out, qo_str = _output(who, "q_out", q_out, (tokens, heads, head_dim), dtype, device, index)
         q_at, qo_at = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         raise RuntimeError("paged_store: q_out without q")
@@ -214,8 +232,7 @@ def paged_store(k, v, k_cache, v_cache, pages, starts, lens, q=None, freqs=None,
     args = _pack_store(q_at, k.data_ptr(), v.data_ptr(), qo_at, k_cache.data_ptr(), v_cache.data_ptr(), *table, where, turns, tokens, seqs,
                        heads, kv_heads, head_dim, 2 * half, bool(interleaved), dtype == torch.bfloat16, cache_shape[0], cache_shape[2],
                        columns, pages_stride, *q_str, *k_str, *v_str, *qo_str, *cache_strides, magnitude)
-    with _on(device):
-        check(lib.eet_paged_store(args, _stream()))
+    _call(lib.eet_paged_store, args, index)
     return q_out
 
 
@@ -242,9 +259,7 @@ def paged_mha(q, k_cache, v_cache, pages, starts, lens, max_tokens=None, max_len
     if cache_shape[3] != head_dim:
         raise RuntimeError(f"paged_mha: caches of head size {cache_shape[3]} beside a q of {head_dim}")
     seqs, columns, pages_stride, table = _table(who, pages, starts, lens, index)
-    if out is None:
-        out = torch.empty(tokens, heads, head_dim, dtype=dtype, device=device)
-    o_str = _heads(who, "out", out, shape, dtype, index)
+    out, o_str = _output(who, "out", out, shape, dtype, device, index)
     first = 0 if first_key is None else _array(who, "first_key", first_key, torch.int32, seqs, index)
     slopes = 0 if alibi_slopes is None else _array(who, "alibi_slopes", alibi_slopes, torch.float32, heads, index)
     if max_tokens is None:
@@ -252,12 +267,12 @@ def paged_mha(q, k_cache, v_cache, pages, starts, lens, max_tokens=None, max_len
     args = _pack_mha(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), *table, first, slopes, tokens, seqs, heads,
                      cache_shape[1], head_dim, dtype == torch.bfloat16, cache_shape[0], cache_shape[2], columns, pages_stride, *q_str,
                      *o_str, *cache_strides, window, max_tokens, max_len or 0, 1.0 / math.sqrt(head_dim) if scale is None else scale)
-    with _on(device):
-        ws_bytes = lib.eet_paged_mha_workspace_bytes(args + _NO_SCRATCH)
-        if ws_bytes:
-            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
-            args += _pack_scratch(ws.data_ptr(), ws_bytes)
-        else:
-            args += _NO_SCRATCH
-        check(lib.eet_paged_mha(args, _stream()))
+    # (how the call is planned, and with it the scratch, goes by sizes and by the device's number of SMs)
+    ws_bytes = _workspace_bytes(args, index)
+    if ws_bytes:
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
+        args += _pack_scratch(ws.data_ptr(), ws_bytes)
+    else:
+        args += _NO_SCRATCH
+    _call(lib.eet_paged_mha, args, index)
     return out
