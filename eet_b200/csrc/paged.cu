@@ -158,12 +158,13 @@ int launch_rotary(const RotaryArgs& a, bool store, cudaStream_t stream)
     return store ? launch_rotary_t<__half, true>(a, stream) : launch_rotary_t<__half, false>(a, stream);
 }
 
-// Which kernels serve a call.  Sequences of at most `few` new tokens are for the kernel of few rows (paged_rows.cu), the others
-// for that of 128-row tiles (paged_tc.cu); each takes any number of tokens where it is alone.
+// Which kernels serve a call.  Sequences whose new tokens make at most 16 rows with the heads that share a kv head are for the kernel
+// of few rows (paged_rows.cu), the others for that of 128-row tiles (paged_tc.cu); each takes any number of tokens where it is alone.
+// Measured with 16 sequences of 1000 to 3000 positions, 32 / 8 heads: 20 rows (5 tokens) 39 us on the first kernel with 32 columns, 40 on the
+// second; 48 rows 95 with 64 columns and 47; 4 rows (64 sequences) 93 and 140.
 struct PagedPlan {
-    int nr;              // rows of the first kernel: 16, 32, 64, or 0
-    int few;
-    bool tiles;          // whether the second one runs
+    bool rows, tiles;    // which of them run
+    int few;             // sequences of up to so many tokens go to the first
     bool whole[2];       // their tiles are not cut (no scratch, no second launch)
     size_t bytes[2];     // scratch
 };
@@ -172,18 +173,15 @@ static PagedPlan paged_plan(const PagedMhaArgs& a)
 {
     PagedPlan p = {};
     const int group = a.heads / a.kv_heads;
-    auto rows_for = [&](long long tokens) {
-        const long long rows = tokens * group;
-        return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 0;
-    };
-    p.nr = rows_for(a.max_tokens);
+    auto is_few = [&](long long tokens) { return tokens * group <= kPwRows; };
+    p.rows = is_few(a.max_tokens);
+    p.tiles = !p.rows;
     p.few = 0x7fffffff;
-    if (p.nr == 0) {
-        p.tiles = true;
+    if (p.tiles) {
         // beside the longest: few tokens each?
         const long long others = a.seqs - 1, rest = a.tokens - a.max_tokens;
-        if (others > 0) p.nr = rows_for((rest + others - 1) / others);
-        p.few = p.nr / group;
+        p.rows = others > 0 && is_few((rest + others - 1) / others);
+        p.few = p.rows ? kPwRows / group : 0;
     }
     // Cutting tiles evens out the shares and costs a second launch: 4 us behind the first kernel, 7 behind the second, whose blocks
     // take 0.8 us and 1.4 (heads of 64) or 1.9 us.  Not where whole tiles make the longest share no more than that longer, taking
@@ -195,9 +193,9 @@ static PagedPlan paged_plan(const PagedMhaArgs& a)
         const long long tiles = (a.seqs + (a.max_tokens > tokens ? a.tokens / tokens : 0)) * a.kv_heads;
         return blocks - (tiles < sms ? 3 * blocks * tiles / (4 * sms) : 0) <= most;
     };
-    if (p.nr > 0) p.whole[0] = whole(p.nr / group, 5);
+    if (p.rows) p.whole[0] = whole(kPwRows / group, 5);
     if (p.tiles) p.whole[1] = whole(2 * (kPgRows / group), 4);
-    if (p.nr > 0 && !p.whole[0]) p.bytes[0] = pg_scratch_bytes(sm_count(), p.nr, a.head_dim);
+    if (p.rows && !p.whole[0]) p.bytes[0] = pg_scratch_bytes(sm_count(), kPwRows, a.head_dim);
     if (p.tiles && !p.whole[1]) p.bytes[1] = pg_scratch_bytes(sm_count(), 2 * kPgRows, a.head_dim);
     return p;
 }
@@ -213,12 +211,10 @@ static int launch_paged_mha_t(const PagedMhaArgs& a, const PagedPlan& p, cudaStr
 {
     void* ws[2] = {a.ws, (char*)a.ws + p.bytes[0]};
     int rc = 0;
-    if (p.nr == 16) rc = pg_launch_rows<T, D, 16>(a, ws[0], p.few, p.whole[0], stream);
-    if (p.nr == 32) rc = pg_launch_rows<T, D, 32>(a, ws[0], p.few, p.whole[0], stream);
-    if (p.nr == 64) rc = pg_launch_rows<T, D, 64>(a, ws[0], p.few, p.whole[0], stream);
+    if (p.rows) rc = pg_launch_rows<T, D>(a, ws[0], p.few, p.whole[0], stream);
     if (rc) return rc;
     if (p.tiles) {
-        const int least = p.nr > 0 ? p.few + 1 : 1;
+        const int least = p.few + 1;
         // (the kernel without a bias takes the maximum of the scores before the scale, which a negative one would turn round)
         rc = a.slopes != nullptr || !(a.scale > 0.f) ? pg_launch_tc<T, D, true>(a, ws[1], least, p.whole[1], stream)
                                                      : pg_launch_tc<T, D, false>(a, ws[1], least, p.whole[1], stream);
@@ -226,10 +222,10 @@ static int launch_paged_mha_t(const PagedMhaArgs& a, const PagedPlan& p, cudaStr
     }
     PgScratch s[2] = {};
     int n = 0;
-    if (p.bytes[0]) s[n++] = {ws[0], p.nr, 0};
+    if (p.bytes[0]) s[n++] = {ws[0], kPwRows, 0};
     if (p.bytes[1]) s[n++] = {ws[1], 2 * kPgRows, 1};
     if (n > 0) {
-        const int y = ((p.bytes[1] ? 2 * kPgRows : p.nr) * D / 16 + 255) / 256;   // 16 dims a thread
+        const int y = ((p.bytes[1] ? 2 * kPgRows : kPwRows) * D / 16 + 255) / 256;   // 16 dims a thread
         EET_CUDA(launch_pdl(paged_mha_join_kernel<T, D>, dim3(sm_count(), y, n), dim3(256), 0, stream, a, s[0], s[1]));
     }
     return 0;

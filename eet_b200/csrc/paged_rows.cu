@@ -1,11 +1,11 @@
-// Attention of few new tokens over a paged cache (decode steps, guessed tokens): up to 64 rows a kv head, a row being a (token,
+// Attention of few new tokens over a paged cache (decode steps, guessed tokens): up to 16 rows a kv head, a row being a (token,
 // query head) pair that shares it.
 //
 // Bound: HBM, the keys and values of every sequence once.  So that everything else fits behind that, the products are turned
 // round - keys and dims are the 128 rows of the tensor core's tile, the few query rows its columns:
-//   S^T [128 keys][NR] = K.Q^T       both K-major from shared memory
-//   O^T [dims][NR] += V^T.P^T        V as an MN-major A operand straight from its [key][dim] tile, P K-major from shared memory
-// (queries as the 128 rows, as in paged_tc.cu, spend an exponential on every one of 128 x 128 scores of which 1 to 64 rows count:
+//   S^T [128 keys][16] = K.Q^T       both K-major from shared memory
+//   O^T [dims][16] += V^T.P^T        V as an MN-major A operand straight from its [key][dim] tile, P K-major from shared memory
+// (queries as the 128 rows, as in paged_tc.cu, spend an exponential on every one of 128 x 128 scores of which 1 to 16 rows count:
 // 64 sequences of 200 to 8000 tokens, 32 / 8 heads: 140 us, of which the transfer needs 81).
 //
 // One CTA per SM, its share of the work as paged_share.cuh says:
@@ -23,33 +23,32 @@ namespace eet {
 
 namespace {
 
+constexpr int kPwRows = 16;          // rows of a tile: the fewest columns that a product with 128 rows has
 constexpr int kPwThreads = 320;
 constexpr int kPwExtra = 2;         // a piece's beginning and end cost as much as two blocks
 constexpr float kPwNone = -1e20f;   // reference of a row that has seen nothing
 
-template<int D, int NR>
+template<int D>
 struct PwShape {
     static constexpr int kHalves = D / 64;
     static constexpr int kTile = kHalves * kPgKeys * 128;                    // a K or V block
-    static constexpr int kStages = D == 64 ? (NR == 64 ? 6 : 8) : NR == 64 ? 3 : NR == 32 ? 5 : 6;
-    static constexpr int kQ = kHalves * NR * 128;                            // rows of Q; two of them
-    static constexpr int kP = 2 * NR * 128;                                  // probabilities [2 x 64 keys][NR]; two of them a group
+    static constexpr int kStages = D == 64 ? 8 : 6;
+    static constexpr int kQ = kHalves * kPwRows * 128;                            // rows of Q; two of them
+    static constexpr int kP = 2 * kPwRows * 128;                                  // probabilities [2 x 64 keys][kPwRows]; two of them a group
     static constexpr int kSmem = kStages * kTile + 2 * kQ + 4 * kP;
-    static constexpr uint32_t kTmemCols = NR == 16 ? 128 : 8 * NR;           // two S, one O of either group
+    static constexpr uint32_t kTmemCols = 128;                               // two S, one O of either group: 96
 };
 
 // What the four warps of a softmax group know of their piece, by row.
-template<int NR>
 struct PwRows {
-    int low[NR], high[NR];   // keys that a row sees
-    float slope[NR];         // of the bias, to the power of two
-    int pos[NR];             // its position
-    long long out_at[NR];    // where its result goes
-    float ref[NR];           // the reference of its powers, as a power of two
-    float corr[NR];          // what a moved reference takes from the sums so far; at the end 1 / sum
+    int low[kPwRows], high[kPwRows];   // keys that a row sees
+    float slope[kPwRows];         // of the bias, to the power of two
+    int pos[kPwRows];             // its position
+    long long out_at[kPwRows];    // where its result goes
+    float ref[kPwRows];           // the reference of its powers, as a power of two
+    float corr[kPwRows];          // what a moved reference takes from the sums so far; at the end 1 / sum
 };
 
-template<int NR>
 struct PwSmem {
     uint64_t q_full[2], q_empty[2];
     uint64_t full[8], empty[8];
@@ -59,7 +58,7 @@ struct PwSmem {
     uint64_t o_free[2];         // O of a piece has been read (four warps)
     uint32_t tmem_base;
     volatile int abort;
-    PwRows<NR> rows[2];
+    PwRows rows[2];
     PgFound found;
 };
 
@@ -87,35 +86,15 @@ __device__ __forceinline__ void tmem_st8_async(uint32_t taddr, const uint32_t (&
                  : "memory");
 }
 
-template<int NR>
-__device__ __forceinline__ void pw_tmem_ld(uint32_t taddr, float (&v)[NR])
-{
-    if constexpr (NR == 16) {
-        uint32_t u[16];
-        tmem_ld16(taddr, u);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(u[i]);
-    }
-    else {
-#pragma unroll
-        for (int c = 0; c < NR; c += 32) {
-            uint32_t u[32];
-            tmem_ld32(taddr + c, u);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[c + i] = __uint_as_float(u[i]);
-        }
-    }
-}
-
-template<typename T, int D, int NR>
+template<typename T, int D>
 __global__ void __launch_bounds__(kPwThreads, 1)
 paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                       const __grid_constant__ CUtensorMap map_v, const __grid_constant__ PagedMhaArgs a, void* ws, int most, int whole)
 {
-    using Shape = PwShape<D, NR>;
+    using Shape = PwShape<D>;
     constexpr int kHalves = Shape::kHalves, kTile = Shape::kTile, kStages = Shape::kStages, kHalf = kPgKeys * 128;
     extern __shared__ __align__(1024) uint8_t pw_dyn[];
-    __shared__ PwSmem<NR> sm;
+    __shared__ PwSmem sm;
     if (smem_u32(pw_dyn) & 1023) {   // the swizzle goes by addresses; the alignment above is there, so this does not happen
         g_device_status = 2;
         return;
@@ -125,7 +104,7 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     uint8_t* p_rows = q_rows + 2 * Shape::kQ;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int group = a.heads / a.kv_heads;
-    const int tile_tokens = NR / group;
+    const int tile_tokens = kPwRows / group;
     const PgTiling tiling = {tile_tokens, 1, most, kPwExtra};
 
     if (threadIdx.x == 0) {
@@ -183,7 +162,7 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             if (lane == 0) mbar_arrive_expect_tx(&sm.q_full[qb], (uint32_t)(tile_tokens * group * 128 * kHalves));
             __syncwarp();
             if (lane < kHalves) {
-                tma_load_3d(q_rows + qb * Shape::kQ + lane * NR * 128, &map_q, 64 * lane, p.head * group, p.s.row0 + p.tile * tile_tokens,
+                tma_load_3d(q_rows + qb * Shape::kQ + lane * kPwRows * 128, &map_q, 64 * lane, p.head * group, p.s.row0 + p.tile * tile_tokens,
                             &sm.q_full[qb]);
             }
             if (p.s.p0 + p.s.tokens > cap && lane == 0) g_device_status = 6;
@@ -217,8 +196,8 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     else if (warp == 9) {
         // ------------------------------------------------------------------ MMA issuer
         if (elect_one()) {
-            constexpr uint32_t idesc_qk = umma_idesc_f16(kPgKeys, NR) | PgType<T>::idesc;
-            constexpr uint32_t idesc_pv = umma_idesc_f16(128, NR) | PgType<T>::idesc | (1u << 15);   // A (V^T) MN-major
+            constexpr uint32_t idesc_qk = umma_idesc_f16(kPgKeys, kPwRows) | PgType<T>::idesc;
+            constexpr uint32_t idesc_pv = umma_idesc_f16(128, kPwRows) | PgType<T>::idesc | (1u << 15);   // A (V^T) MN-major
             const uint64_t q_desc = umma_desc_sw128(smem_u32(q_rows));
             const uint64_t p_desc = umma_desc_sw128(smem_u32(p_rows));
             const uint64_t k_desc = umma_desc_sw128(smem_u32(ring));
@@ -241,7 +220,7 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 const int n = p.blocks, qb = pieces & 1;
                 ok = tc_wait(&sm.q_full[qb], (uint32_t)((pieces / 2) & 1), &sm.abort);
                 if (!ok) break;
-                const uint32_t tmem_s = tmem + (uint32_t)(qb * 3 * NR), tmem_o = tmem_s + 2 * NR;
+                const uint32_t tmem_s = tmem + (uint32_t)(qb * 3 * kPwRows), tmem_o = tmem_s + 2 * kPwRows;
                 int done_qk = qb ? qk[1] : qk[0], done_pv = done_qk;
                 auto issue_qk = [&](int j) -> bool {
                     if (!tc_wait(&sm.full[stage], phase, &sm.abort)) return false;
@@ -249,8 +228,8 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                     const uint64_t kd = k_desc + (uint64_t)(stage * (kTile >> 4)), qd = q_desc + (uint64_t)(qb * (Shape::kQ >> 4));
 #pragma unroll
                     for (int kk = 0; kk < D / 16; ++kk) {
-                        umma_f16(tmem_s + (uint32_t)((done_qk & 1) * NR), kd + (uint64_t)((kk >> 2) * (kHalf >> 4) + (kk & 3) * 2),
-                                 qd + (uint64_t)((kk >> 2) * (NR * 128 >> 4) + (kk & 3) * 2), idesc_qk, kk != 0);
+                        umma_f16(tmem_s + (uint32_t)((done_qk & 1) * kPwRows), kd + (uint64_t)((kk >> 2) * (kHalf >> 4) + (kk & 3) * 2),
+                                 qd + (uint64_t)((kk >> 2) * (kPwRows * 128 >> 4) + (kk & 3) * 2), idesc_qk, kk != 0);
                     }
                     umma_commit(&sm.s_full[qb][done_qk & 1]);
                     next_stage();
@@ -270,7 +249,7 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                                    pd = p_desc + (uint64_t)((2 * qb + (done_pv & 1)) * (Shape::kP >> 4));
 #pragma unroll
                     for (int kk = 0; kk < kPgKeys / 16; ++kk) {
-                        umma_f16(tmem_o, vd + (uint64_t)(kk * (2048 >> 4)), pd + (uint64_t)((kk >> 2) * (NR * 128 >> 4) + (kk & 3) * 2),
+                        umma_f16(tmem_o, vd + (uint64_t)(kk * (2048 >> 4)), pd + (uint64_t)((kk >> 2) * (kPwRows * 128 >> 4) + (kk & 3) * 2),
                                  idesc_pv, j != 0 || kk != 0);
                     }
                     umma_commit(&sm.pv_done[qb][done_pv & 1]);
@@ -289,13 +268,13 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         const int x = warp >> 2;                              // pieces go to the two groups in turn
         const int r = (warp & 3) * 32 + lane;                 // key of the block, and dim of O
         const uint32_t t_lane = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t tmem_s = tmem + t_lane + (uint32_t)(x * 3 * NR), tmem_o = tmem_s + 2 * NR;
+        const uint32_t tmem_s = tmem + t_lane + (uint32_t)(x * 3 * kPwRows), tmem_o = tmem_s + 2 * kPwRows;
         const float log2e = 1.4426950408889634f;
         const float to_log2 = a.scale * log2e;
         const int cap = (int)min((long long)a.max_pages << a.page_shift, 0x7fffffffLL);
-        PwRows<NR>& row = sm.rows[x];
+        PwRows& row = sm.rows[x];
         uint8_t* p_mine = p_rows + x * 2 * Shape::kP;
-        float* cross = reinterpret_cast<float*>(p_mine);      // [NR][128], for what crosses the threads while no product reads P
+        float* cross = reinterpret_cast<float*>(p_mine);      // [kPwRows][128], for what crosses the threads while no product reads P
         int stage = 0;                                        // of the loads, as the issuer counts them
         uint32_t phase = 0;
         int block = 0;                                        // blocks done
@@ -314,7 +293,7 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             const int rows = min(tile_tokens, p.s.tokens - token0) * group;
             const PgSpan span = pg_span(a, p.s, token0, token0 + tile_tokens);
             // (everybody has left the piece before: its last barrier stands behind the last use of these)
-            if (r < NR) {
+            if (r < kPwRows) {
                 const int pos = p.s.p0 + token0 + r / group;
                 row.pos[r] = pos;
                 row.low[r] = a.window > 0 ? (int)max((long long)p.s.first, (long long)pos - a.window + 1) : p.s.first;
@@ -326,35 +305,40 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             pw_any(x, false);
             // blocks all of whose keys every row sees
             const int all_low = row.low[rows - 1], all_high = row.high[0];
-            float l[NR];
+            float l[kPwRows];
 #pragma unroll
-            for (int n = 0; n < NR; ++n) l[n] = 0.f;
+            for (int n = 0; n < kPwRows; ++n) l[n] = 0.f;
             for (int j = 0; j < p.blocks; ++j, ++block) {
                 const int key0 = (p.top - j) * kPgKeys, key = key0 + r;
                 const int buf = block & 1;
                 ok = tc_wait_warp(&sm.s_full[x][buf], (uint32_t)((block >> 1) & 1), &sm.abort) && ok;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                float t[NR];
-                pw_tmem_ld<NR>(tmem_s + (uint32_t)(buf * NR), t);
+                float t[kPwRows];
+                {
+                    uint32_t u[kPwRows];
+                    tmem_ld16(tmem_s + (uint32_t)(buf * kPwRows), u);
+#pragma unroll
+                    for (int n = 0; n < kPwRows; ++n) t[n] = __uint_as_float(u[n]);
+                }
                 if (a.slopes != nullptr) {
 #pragma unroll
-                    for (int n = 0; n < NR; ++n) t[n] = fmaf(t[n], to_log2, row.slope[n] * (float)(key - row.pos[n]));
+                    for (int n = 0; n < kPwRows; ++n) t[n] = fmaf(t[n], to_log2, row.slope[n] * (float)(key - row.pos[n]));
                 }
                 else {
 #pragma unroll
-                    for (int n = 0; n < NR; ++n) t[n] *= to_log2;
+                    for (int n = 0; n < kPwRows; ++n) t[n] *= to_log2;
                 }
                 if (all_low <= key0 && all_high >= key0 + kPgKeys - 1) {
 #pragma unroll
-                    for (int n = 0; n < NR; ++n) t[n] = n < rows ? t[n] : -INFINITY;
+                    for (int n = 0; n < kPwRows; ++n) t[n] = n < rows ? t[n] : -INFINITY;
                 }
                 else {
 #pragma unroll
-                    for (int n = 0; n < NR; ++n) t[n] = key >= row.low[n] && key <= row.high[n] ? t[n] : -INFINITY;
+                    for (int n = 0; n < kPwRows; ++n) t[n] = key >= row.low[n] && key <= row.high[n] ? t[n] : -INFINITY;
                 }
                 bool over = j == 0;
 #pragma unroll
-                for (int n = 0; n < NR; ++n) over |= t[n] - row.ref[n] > 8.0f;
+                for (int n = 0; n < kPwRows; ++n) over |= t[n] - row.ref[n] > 8.0f;
                 // the buffer that the probabilities go to has been read by the product of two blocks before
                 if (block > 1) ok = tc_wait_warp(&sm.pv_done[x][buf], (uint32_t)(((block >> 1) - 1) & 1), &sm.abort) && ok;
                 if (pw_any(x, over || !ok)) {
@@ -362,13 +346,13 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                     if (j > 0) ok = tc_wait_warp(&sm.pv_done[x][buf ^ 1], (uint32_t)(((block - 1) >> 1) & 1), &sm.abort) && ok;
                     // (no product reads the probabilities now: their place holds the scores for a moment, row by row)
 #pragma unroll
-                    for (int n = 0; n < NR; ++n) cross[n * kPgKeys + r] = t[n];
+                    for (int n = 0; n < kPwRows; ++n) cross[n * kPgKeys + r] = t[n];
                     failed = pw_any(x, !ok);
                     if (failed) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     // (eight lanes a row: four rows of a warp at once)
-#pragma unroll 1
-                    for (int n = (warp & 3) * 4 + (lane >> 3); n < NR; n += 16) {
+                    {
+                        const int n = (warp & 3) * 4 + (lane >> 3);
                         const float4* v = reinterpret_cast<const float4*>(cross + n * kPgKeys) + (lane & 7);
                         float m = -INFINITY;
 #pragma unroll
@@ -383,10 +367,10 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                     }
                     pw_any(x, false);
 #pragma unroll
-                    for (int n = 0; n < NR; ++n) l[n] *= row.corr[n];
+                    for (int n = 0; n < kPwRows; ++n) l[n] *= row.corr[n];
                     if (j > 0) {
 #pragma unroll 1
-                        for (int c = 0; c < NR; c += 8) {
+                        for (int c = 0; c < kPwRows; c += 8) {
                             uint32_t o[8];
                             tmem_ld8(tmem_o + (uint32_t)c, o);
 #pragma unroll
@@ -397,10 +381,10 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                     }
                 }
                 // probabilities: row n of P holds 64 keys in 128 bytes, 16-byte pieces swizzled by n
-                uint8_t* dst = p_mine + buf * Shape::kP + (r >> 6) * (NR * 128) + (r & 7) * 2;
+                uint8_t* dst = p_mine + buf * Shape::kP + (r >> 6) * (kPwRows * 128) + (r & 7) * 2;
                 const int piece = (r & 63) >> 3;
 #pragma unroll
-                for (int n = 0; n < NR; ++n) {
+                for (int n = 0; n < kPwRows; ++n) {
                     const float e = ex2_approx(t[n] - row.ref[n]);
                     l[n] += e;
                     *reinterpret_cast<T*>(dst + n * 128 + ((piece ^ (n & 7)) << 4)) = (T)e;
@@ -436,13 +420,13 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             // ---- epilogue: the sums of the threads, then O, a dim a thread
             if (p.blocks > 0) ok = tc_wait_warp(&sm.pv_done[x][(block - 1) & 1], (uint32_t)(((block - 1) >> 1) & 1), &sm.abort) && ok;
 #pragma unroll
-            for (int n = 0; n < NR; ++n) cross[n * kPgKeys + r] = l[n];
+            for (int n = 0; n < kPwRows; ++n) cross[n * kPgKeys + r] = l[n];
             if (pw_any(x, !ok)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const bool complete = p.starts && p.ends;
-            const PgPartial part = pg_partial(ws, (int)gridDim.x, (int)blockIdx.x, p.starts ? 1 : 0, NR, D);
-#pragma unroll 1
-            for (int n = (warp & 3) * 4 + (lane >> 3); n < NR; n += 16) {
+            const PgPartial part = pg_partial(ws, (int)gridDim.x, (int)blockIdx.x, p.starts ? 1 : 0, kPwRows, D);
+            {
+                const int n = (warp & 3) * 4 + (lane >> 3);
                 const float4* v = reinterpret_cast<const float4*>(cross + n * kPgKeys) + (lane & 7);
                 float sum = 0.f;
 #pragma unroll
@@ -489,17 +473,17 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     }
 }
 
-template<typename T, int D, int NR>
+template<typename T, int D>
 int pg_launch_rows(const PagedMhaArgs& a, void* ws, int most, int whole, cudaStream_t stream)
 {
     CUtensorMap map_q, map_k, map_v;
-    if (int rc = pg_encode_maps<T, D>(a, NR / (a.heads / a.kv_heads), &map_q, &map_k, &map_v)) return rc;
-    auto kern = paged_mha_rows_kernel<T, D, NR>;
+    if (int rc = pg_encode_maps<T, D>(a, kPwRows / (a.heads / a.kv_heads), &map_q, &map_k, &map_v)) return rc;
+    auto kern = paged_mha_rows_kernel<T, D>;
     static bool attr_set[64] = {};
     int dev = 0;
     EET_CUDA(cudaGetDevice(&dev));
     dev &= 63;
-    constexpr int kSmem = PwShape<D, NR>::kSmem;
+    constexpr int kSmem = PwShape<D>::kSmem;
     if (!attr_set[dev]) {
         EET_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
         attr_set[dev] = true;

@@ -15,6 +15,8 @@ are read there, so a captured CUDA graph of these calls serves whatever they hol
 behind a sequence's last position are not read.  A page number outside the cache is not followed: the call completes and
 ``EET.check_device_status()`` reports it.
 
+`PagedMmha` is the attention block around them, beside `EET.LlamaMmha` and `EET.BaichuanMmha`.
+
 The reference serves one contiguous cache an op, all sequences at the same step (csrc/op/llama_mmha.cpp:94-112).
 """
 import math
@@ -23,9 +25,9 @@ import struct
 import torch
 
 from ._lib import check, lib
-from .EET import _current_device, _raw_stream
+from .EET import _current_device, _linear, _norm_head, _on, _pending, _pool, _raw_stream
 
-__all__ = ["rotary_frequencies", "apply_rotary", "paged_store", "paged_mha"]
+__all__ = ["rotary_frequencies", "apply_rotary", "paged_store", "paged_mha", "PagedMmha"]
 
 _DTYPES = (torch.float16, torch.bfloat16)
 _PAGE_SIZES = (16, 32, 64, 128, 256)
@@ -276,3 +278,72 @@ def paged_mha(q, k_cache, v_cache, pages, starts, lens, max_tokens=None, max_len
         args += _NO_SCRATCH
     _call(lib.eet_paged_mha, args, index)
     return out
+
+
+class PagedMmha:
+    """Attention block over a paged cache: RMSNorm, W8A16 (or fp16) QKV projection, rotary positions and append, attention, output
+    projection + residual - the flow of EET.LlamaMmha / EET.BaichuanMmha (csrc/op/llama_mmha.cpp:114-266) for sequences of
+    different ages, chunks and single tokens in one call, and kv heads that several query heads share.
+
+      QKV_weights     [hidden, (heads + 2 kv_heads) 128] (q, then k, then v), packed int8 or fp16 as MetaDesc.is_int8 says
+      Output_weights  [heads 128, hidden]
+      kv_head_num     MetaDesc.head_num by default
+      freqs           from rotary_frequencies; by default all 128 dims at base 10000, none with alibi_slopes
+      alibi_slopes    float32 [heads] instead of rotary positions (the op of Baichuan-13B)
+    The caches belong to the caller, a pair for each layer.  MetaDesc.batch_size * max_seq_len is the most tokens of a call.  The
+    output is a view of a buffer that the ops of a device share, as the other ops' outputs are."""
+
+    def __init__(self, desc, QKV_weights, QKV_scale, Output_weights, Output_scale, layernorm_weights, kv_head_num=None, freqs=None,
+                 interleaved=False, magnitude=1.0, alibi_slopes=None):
+        desc._require_half("PagedMmha")
+        if desc.tp is not None and desc.tp.size > 1:
+            raise RuntimeError("PagedMmha: tensor parallelism is not part of this op")
+        self.desc, self.heads = desc, desc.head_num
+        self.kv_heads = desc.head_num if kv_head_num is None else int(kv_head_num)
+        if self.kv_heads <= 0 or self.heads % self.kv_heads:
+            raise RuntimeError(f"PagedMmha: {self.heads} heads are not a multiple of {self.kv_heads} kv heads")
+        self.size_per_head = desc.hidden_units // desc.head_num if desc.d_kv == 0 else desc.d_kv
+        if self.size_per_head != 128:
+            raise RuntimeError("PagedMmha: only head size 128 is supported")
+        self.inner_dim, self.qkv_dim = 128 * self.heads, 128 * (self.heads + 2 * self.kv_heads)
+        for t, shape, what in ((QKV_weights, (desc.hidden_units, self.qkv_dim), "QKV_weights"),
+                               (Output_weights, (self.inner_dim, desc.hidden_units), "Output_weights")):
+            if tuple(t.shape) != shape or t.dtype != desc.weight_dtype or not t.is_cuda or not t.is_contiguous():
+                raise RuntimeError(f"PagedMmha: {what} must be a contiguous CUDA {desc.weight_dtype} tensor of shape {shape}, got "
+                                   f"{tuple(t.shape)} {t.dtype}")
+        self.qkv_w, self.qkv_s, self.out_w, self.out_s, self.ln_w = QKV_weights, QKV_scale, Output_weights, Output_scale, layernorm_weights
+        if alibi_slopes is not None and freqs is not None:
+            raise RuntimeError("PagedMmha: rotary positions and ALiBi exclude each other")
+        if alibi_slopes is None and freqs is None:
+            freqs, magnitude = rotary_frequencies(128, device=desc.device)
+        self.freqs, self.interleaved, self.magnitude, self.alibi_slopes = freqs, interleaved, magnitude, alibi_slopes
+
+    def forward(self, input, k_cache, v_cache, pages, starts, lens, max_tokens=None, max_len=None, window=0, first_key=None):
+        """input fp16 [tokens, hidden]: the new tokens of all sequences behind one another; the other arguments as in paged_mha."""
+        d = self.desc
+        if input.dtype != torch.float16 or not input.is_cuda or input.dim() != 2 or input.shape[1] != d.hidden_units or \
+                not input.is_contiguous():
+            raise RuntimeError("PagedMmha: input must be a contiguous CUDA fp16 tensor [tokens, hidden]")
+        n, cap = input.shape[0], d.batch_size * d.max_seq_len
+        if n > cap:
+            raise RuntimeError(f"PagedMmha: {n} tokens, MetaDesc allows {cap}")
+        with _on(d.device):
+            xn = _pool.rows("layernorm", n, d.hidden_units, cap * d.hidden_units, torch.float16, d.device)
+            qkv = _pool.rows("qkv_paged", n, self.qkv_dim, cap * self.qkv_dim, torch.float16, d.device)
+            ctx = _pool.rows("dst", n, self.inner_dim, cap * self.inner_dim, torch.float16, d.device).view(n, self.heads, 128)
+            out = _pool.rows("self_mask_attn_cache", n, d.hidden_units, cap * d.hidden_units, torch.float16, d.device)
+            if n == 0:
+                return out
+            _pending.pop(out.data_ptr(), None)   # whatever this buffer held before is gone
+            _norm_head(input, self.ln_w, d.layernorm_eps, xn)
+            _linear(xn, self.qkv_w, self.qkv_s, qkv)
+            q, k, v = qkv.view(n, -1, 128).split((self.heads, self.kv_heads, self.kv_heads), 1)
+            q = paged_store(k, v, k_cache, v_cache, pages, starts, lens, q=q, freqs=self.freqs, interleaved=self.interleaved,
+                            magnitude=self.magnitude, q_out=q)
+            # (rows that belong to no sequence go through the block like the others and mean nothing)
+            paged_mha(q, k_cache, v_cache, pages, starts, lens, max_tokens=max_tokens, max_len=max_len, window=window,
+                      first_key=first_key, alibi_slopes=self.alibi_slopes, out=ctx)
+            _linear(ctx.view(n, self.inner_dim), self.out_w, self.out_s, out, residual=input)
+        return out.view(n, d.hidden_units)
+
+    __call__ = forward

@@ -477,3 +477,143 @@ def test_store_and_attention_of_a_prompt_in_chunks_and_then_token_by_token():
         x = qkv[b][:done[b], H:H + K]
         _within(got, want, 2.0 ** -11 * want.abs() + rotate_tolerance(x, freqs.cpu(), False, FP16) + 2.0 ** -25)
     assert _status() == 0
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# the attention block
+# ---------------------------------------------------------------------------------------------------------------------
+def _block(heads, kv_heads, hidden, is_int8, seed=0, **kw):
+    """(PagedMmha, its weights as they were quantized)."""
+    from eet_b200 import EET
+    gen = torch.Generator().manual_seed(seed)
+    desc = EET.MetaDesc(FP16, 4, heads, hidden, 1, 128, 512, d_kv=128, is_int8=is_int8)
+    qkv = (torch.randn(hidden, 128 * (heads + 2 * kv_heads), generator=gen) * hidden ** -0.5).half()
+    out = (torch.randn(128 * heads, hidden, generator=gen) * (128 * heads) ** -0.5).half()
+    norm = (1 + 0.1 * torch.randn(hidden, generator=gen)).half().cuda()
+    if is_int8:
+        (qkv, qkv_s), (out, out_s) = (EET.quant_weights(w) for w in (qkv, out))
+        args = qkv.cuda(), qkv_s.cuda(), out.cuda(), out_s.cuda(), norm
+    else:
+        args = qkv.cuda(), None, out.cuda(), None, norm
+    return _paged().PagedMmha(desc, *args, kv_head_num=kv_heads, **kw), args
+
+
+@pytest.mark.parametrize("heads,kv_heads,is_int8,alibi", [(4, 2, True, False), (2, 2, False, False), (6, 1, True, True)])
+def test_block_is_the_calls_behind_one_another(heads, kv_heads, is_int8, alibi):
+    """At most 16 rows, where the projections add in one order: the same bits."""
+    from eet_b200 import EET
+    hidden = 256
+    slopes = torch.tensor(EET.alibi_slopes(heads), dtype=torch.float32).cuda() if alibi else None
+    block, (qkv_w, qkv_s, out_w, out_s, norm) = _block(heads, kv_heads, hidden, is_int8, alibi_slopes=slopes)
+    batch = Batch([3, 1, 6], [20, 300, 150], heads, kv_heads)
+    x = torch.randn(10, hidden, generator=torch.Generator().manual_seed(1)).half().cuda()
+    kc, vc, *table = _gpu(batch)
+    got = block(x, kc, vc, *table, max_tokens=6, window=100).clone()
+    kc2, vc2, *_ = _gpu(batch)
+    xn = EET.LayerNorm(block.desc, norm, torch.empty(0)).layer_norm(x.view(1, 10, hidden)).view(10, hidden)
+    qkv = EET.gemm_w8a16(xn, qkv_w, qkv_s) if is_int8 else xn @ qkv_w
+    qkv = qkv.view(10, -1, 128)
+    q, k, v = qkv[:, :heads], qkv[:, heads:heads + kv_heads], qkv[:, heads + kv_heads:]
+    freqs = None if alibi else _paged().rotary_frequencies(128)[0]
+    q = _paged().paged_store(k, v, kc2, vc2, *table, q=q, freqs=freqs)
+    ctx = _paged().paged_mha(q, kc2, vc2, *table, max_tokens=6, window=100, alibi_slopes=slopes).view(10, -1)
+    want = EET.gemm_w8a16(ctx, out_w, out_s, residual=x) if is_int8 else (ctx @ out_w) + x
+    assert torch.equal(got, want) and torch.equal(kc, kc2) and torch.equal(vc, vc2)
+
+
+def test_block_beside_llama_mmha():
+    """Two prompts of one length and three steps, the paged block against EET.LlamaMmha with its own caches.
+
+    Both round q, k, v and the context to fp16 once, so with |w| the weights: the outputs differ by at most the rounding of the
+    context and of the probabilities in both (4 half steps of the mean of |v|, times |w|), by that of q and k where their angles
+    differ in the last bit (2 half steps of each score's magnitude, as a relative error of the probabilities, twice), LlamaMmha's
+    scores in fp16 (one more half step of the score), and two roundings of the result and of the sum with the residual."""
+    from eet_b200 import EET
+    heads, hidden, S, B = 4, 256, 130, 2
+    block, (qkv_w, qkv_s, out_w, out_s, norm) = _block(heads, heads, hidden, True, seed=3)
+    desc = EET.MetaDesc(FP16, B, heads, hidden, 1, S, S + 4, d_kv=128, is_int8=True)
+    none = torch.empty(0)
+    llama = EET.LlamaMmha(desc, qkv_w, qkv_s, none, none, none, out_w, out_s, none, norm, none)
+    x = torch.randn(B, S + 3, hidden, generator=torch.Generator().manual_seed(2)).half().cuda()
+    kc, vc = (torch.full((20, heads, 16, 128), math.nan, dtype=FP16, device="cuda") for _ in range(2))
+    pages = torch.arange(20, dtype=torch.int32, device="cuda").view(2, 10)
+    weights = (EET.unpack_weights(out_w).double() * out_s.double()).abs()
+    u = 2.0 ** -11
+    for first, last in ((0, S), (S, S + 1), (S + 1, S + 2), (S + 2, S + 3)):
+        part = x[:, first:last].contiguous()
+        want = llama(part, none, none, True, True, first == 0).clone().view(-1, hidden)
+        n = last - first
+        starts = torch.tensor([0, n, 2 * n], dtype=torch.int32, device="cuda")
+        lens = torch.tensor([last, last], dtype=torch.int32, device="cuda")
+        got = block(part.view(-1, hidden), kc, vc, pages, starts, lens, max_tokens=n).clone()
+        k, v = (c[pages[:, :(last + 15) // 16].long()].transpose(2, 3).reshape(B, -1, heads, 128)[:, :last].abs().double().amax((1, 3))
+                for c in (kc, vc))                                                                 # [B][heads]
+        q = EET._pool.rows("qkv_paged", 2 * n, 3 * 512, 1, FP16, x.device).view(B, n, 3 * heads, 128)[:, :, :heads].abs().double()
+        score = q.sum(-1) * k[:, None] / math.sqrt(128)                                           # [B][n][heads], at least the largest
+        context = (4 * u + 2 * (4 + 1) * u * score) * v[:, None]
+        tol = context.repeat_interleave(128, -1).view(-1, 512) @ weights + 2 * u * (want.double().abs() + part.view(-1, hidden).double().abs()) + 1e-5
+        off = (got.double() - want.double()).abs()
+        assert (off <= tol).all() and off.max() < 0.02
+    assert _status() == 0
+
+
+def test_block_refuses():
+    from eet_b200 import EET
+    block, args = _block(4, 2, 256, True)
+    x = torch.zeros(3, 256, dtype=FP16, device="cuda")
+    batch = Batch([1, 2], [4, 5], 4, 2)
+    for bad in (x.float(), x[:, :128], x.cpu(), x.view(1, 3, 256), torch.zeros(513, 256, dtype=FP16, device="cuda")):
+        with pytest.raises(RuntimeError):
+            block(bad, *_gpu(batch))
+    assert block(x[:0], *_gpu(Batch([0], [3], 4, 2))).shape == (0, 256)
+    with pytest.raises(RuntimeError, match="kv heads"):
+        _paged().PagedMmha(block.desc, *args, kv_head_num=3)
+    with pytest.raises(RuntimeError, match="QKV_weights"):
+        _paged().PagedMmha(block.desc, *args, kv_head_num=4)
+    with pytest.raises(RuntimeError, match="exclude"):
+        _paged().PagedMmha(block.desc, *args, kv_head_num=2, freqs=_paged().rotary_frequencies(128)[0],
+                           alibi_slopes=torch.ones(4, device="cuda"))
+    wide = EET.MetaDesc(FP16, 4, 4, 256, 1, 128, 512, is_int8=True)
+    with pytest.raises(RuntimeError, match="head size 128"):
+        _paged().PagedMmha(wide, *args, kv_head_num=2)
+
+
+def test_a_layer_of_a_model_step_captured():
+    """Block and FFN op of one decoder layer in a captured step, replayed while lengths and pages change: as in eager calls."""
+    from eet_b200 import EET
+    hidden, heads, kv_heads = 256, 4, 2
+    block, _ = _block(heads, kv_heads, hidden, True, seed=5)
+    desc = EET.MetaDesc(FP16, 4, heads, hidden, 1, 128, 512, activation_fn="silu", d_kv=128, d_ff=512, is_int8=True)
+    gen = torch.Generator().manual_seed(8)
+    w = [EET.quant_weights((torch.randn(*s, generator=gen) * 0.05).half()) for s in ((hidden, 512), (hidden, 512), (512, hidden))]
+    none = torch.empty(0)
+    ffn = EET.GatedFeedForwardNetworkInt8(desc, w[0][0].cuda(), w[0][1].cuda(), none, w[1][0].cuda(), w[1][1].cuda(), none,
+                                          w[2][0].cuda(), w[2][1].cuda(), none, torch.ones(hidden, dtype=FP16, device="cuda"), none)
+    kc, vc = (torch.randn(12, kv_heads, 16, 128, generator=gen).half().cuda() for _ in range(2))
+    pages = torch.tensor([[0, 3, 6, 9], [1, 4, 7, 10], [2, 5, 8, 11]], dtype=torch.int32, device="cuda")
+    starts = torch.arange(4, dtype=torch.int32, device="cuda")
+    lens = torch.tensor([5, 17, 30], dtype=torch.int32, device="cuda")
+    x = torch.randn(3, hidden, generator=gen).half().cuda()
+
+    def step():
+        y = block(x, kc, vc, pages, starts, lens, max_tokens=1, max_len=64)
+        return ffn(y.view(1, 3, hidden)).view(3, hidden)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(6):
+        lens += 5
+        x.copy_(torch.randn(3, hidden, generator=gen).half())
+        before = kc.clone(), vc.clone()
+        graph.replay()
+        got = out.clone()
+        kc.copy_(before[0])
+        vc.copy_(before[1])
+        assert torch.equal(step(), got)
+    assert _status() == 0
