@@ -178,9 +178,11 @@ static PagedPlan paged_plan(const PagedMhaArgs& a)
     p.tiles = !p.rows;
     p.few = 0x7fffffff;
     if (p.tiles) {
-        // beside the longest: few tokens each?
+        // Few tokens each beside the longest, and much to read for them?  A launch more costs 12 us; one chunk and 31 or 23 single tokens
+        // take, on both kernels and on the second alone: 32 / 8 heads, up to 1000 positions (248 tiles of up to 9 blocks) 47 and 37 us;
+        // 40 heads, up to 2500 (920 of up to 20) 132 and 186.
         const long long others = a.seqs - 1, rest = a.tokens - a.max_tokens;
-        p.rows = others > 0 && is_few((rest + others - 1) / others);
+        p.rows = others > 0 && is_few((rest + others - 1) / others) && others * a.kv_heads * (a.max_len / kPgKeys + 1) >= 16384;
         p.few = p.rows ? kPwRows / group : 0;
     }
     // Cutting tiles evens out the shares and costs a second launch: 4 us behind the first kernel, 7 behind the second, whose blocks

@@ -183,14 +183,17 @@ __device__ __forceinline__ long long pg_seq_blocks(const PagedMhaArgs& a, const 
 }
 
 // Kernels this short spend much of their time on what runs once - the first fetch of every instruction among it - so what follows
-// is kept small: no 64-bit divisions, one pass over the sequences where the block has a thread for each.
-struct PgFound {
+// is kept small: no 64-bit divisions, no barrier where a warp has a lane for each sequence.
+struct PgFound {           // by the block together, where it takes more
     long long warp_sum[12];
-    long long total;       // blocks in all
-    long long begin;       // of the share
-    long long rest;        // from the sequence's first block of a head to it
+    long long rest, per_head;
     PgSeq s;
-    int seq, head, tile, at;
+    int seq;
+};
+
+// What the header of a share goes by: blocks in all, and where the share begins.
+struct PgPlace {
+    long long total, begin;
 };
 
 // CTA c's share of `total` blocks begins at q c + min(c, r), with total = q ctas + r.
@@ -212,80 +215,93 @@ struct PgCut {
     }
 };
 
-// The share of CTA `cta` of `ctas`, by all threads of the block.  Ends with a block-wide barrier; false: it has none.
+__device__ __forceinline__ int pg_div(long long x, long long d)
+{
+    return (x | d) >> 32 ? (int)(x / d) : (int)((uint32_t)x / (uint32_t)d);
+}
+
+// The share of CTA `cta` of `ctas`, found by every warp of the block; false: it has none.
 __device__ __forceinline__ bool pg_find_share(const PagedMhaArgs& a, const PgTiling& g, int cta, int ctas, bool whole, PgFound& f,
-                                              PgShare& share)
+                                              PgShare& share, PgPlace& place)
 {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5, threads = blockDim.x;
-    const bool once = a.seqs <= threads;
-    long long total = 0;
-    for (int pass = once; pass < 2; ++pass) {   // the first pass adds up, the second (or only) one looks for the share's begin
-        long long before = 0;                   // of the sequences of earlier rounds
-        for (int base = 0; base < a.seqs; base += threads) {
-            PgSeq s = {0, 0, 0, 0};
-            if (base + tid < a.seqs) s = pg_seq(a, g, base + tid);
-            const long long per_head = pg_seq_blocks(a, g, s), cost = a.kv_heads * per_head;
-            const long long upto = pg_warp_scan(cost);
-            if (lane == 31) f.warp_sum[warp] = upto;
-            __syncthreads();
-            long long end = before + upto;
-            for (int w = 0; w < warps; ++w) {
-                if (w < warp) end += f.warp_sum[w];
-                before += f.warp_sum[w];
-            }
-            if (once) total = before;
-            if (pass == 1) {
-                const long long begin = PgCut(total, ctas).begin(cta);
-                if (end - cost <= begin && begin < end) {
-                    long long rest = begin - (end - cost);
-                    int head = 0;
-                    if (rest >= per_head) {
-                        head = rest >> 32 ? (int)(rest / per_head) : (int)((uint32_t)rest / (uint32_t)per_head);
-                        rest -= head * per_head;
+    long long rest, per_head;    // from the begin of the share's first sequence to the share's; blocks of a kv head of that sequence
+    if (a.seqs <= 32) {
+        PgSeq s = {0, 0, 0, 0};
+        if (lane < a.seqs) s = pg_seq(a, g, lane);
+        per_head = pg_seq_blocks(a, g, s);
+        const long long cost = a.kv_heads * per_head, upto = pg_warp_scan(cost);
+        place.total = __shfl_sync(0xffffffffu, upto, 31);
+        const PgCut cut(place.total, ctas);
+        place.begin = cut.begin(cta);
+        share.left = cut.begin(cta + 1) - place.begin;
+        if (share.left == 0) return false;
+        share.seq = __ffs(__ballot_sync(0xffffffffu, upto - cost <= place.begin && place.begin < upto)) - 1;
+        rest = place.begin - __shfl_sync(0xffffffffu, upto - cost, share.seq);
+        per_head = __shfl_sync(0xffffffffu, per_head, share.seq);
+        share.s.row0 = __shfl_sync(0xffffffffu, s.row0, share.seq);
+        share.s.tokens = __shfl_sync(0xffffffffu, s.tokens, share.seq);
+        share.s.p0 = __shfl_sync(0xffffffffu, s.p0, share.seq);
+        share.s.first = __shfl_sync(0xffffffffu, s.first, share.seq);
+    }
+    else {
+        const bool once = a.seqs <= threads;
+        place.total = place.begin = 0;
+        for (int pass = once; pass < 2; ++pass) {   // the first pass adds up, the second (or only) one looks for the share's begin
+            long long before = 0;                   // of the sequences of earlier rounds
+            for (int base = 0; base < a.seqs; base += threads) {
+                PgSeq s = {0, 0, 0, 0};
+                if (base + tid < a.seqs) s = pg_seq(a, g, base + tid);
+                per_head = pg_seq_blocks(a, g, s);
+                const long long cost = a.kv_heads * per_head, upto = pg_warp_scan(cost);
+                if (lane == 31) f.warp_sum[warp] = upto;
+                __syncthreads();
+                long long end = before + upto;
+                for (int w = 0; w < warps; ++w) {
+                    if (w < warp) end += f.warp_sum[w];
+                    before += f.warp_sum[w];
+                }
+                if (once) place.total = before;
+                if (pass == 1) {
+                    place.begin = PgCut(place.total, ctas).begin(cta);
+                    if (end - cost <= place.begin && place.begin < end) {
+                        f.rest = place.begin - (end - cost);
+                        f.per_head = per_head;
+                        f.s = s;
+                        f.seq = base + tid;
                     }
-                    f.begin = begin;
-                    f.seq = base + tid;
-                    f.s = s;
-                    f.head = head;
-                    f.tile = 0;
-                    f.at = (int)rest;
-                    f.rest = rest;
                 }
+                __syncthreads();
             }
-            __syncthreads();
+            place.total = before;
         }
-        total = before;
+        share.left = PgCut(place.total, ctas).begin(cta + 1) - place.begin;
+        if (share.left == 0) return false;
+        rest = f.rest;
+        per_head = f.per_head;
+        share.s = f.s;
+        share.seq = f.seq;
     }
-    const PgCut cut(total, ctas);
-    share.left = cut.begin(cta + 1) - cut.begin(cta);
-    if (share.left == 0) return false;
-    share.s = f.s;
-    if (g.tiles(share.s) > 1) {
-        if (warp == 0) {
-            // the tile within the sequence
-            long long rest = f.rest;
-            const int tiles = g.tiles(share.s);
-            for (int t0 = 0; t0 < tiles; t0 += 32) {
-                const int t = t0 + lane;
-                const long long cost = t < tiles ? pg_span(a, share.s, t * g.tokens, (t + 1) * g.tokens).blocks() + g.extra : 0;
-                const long long upto = pg_warp_scan(cost);
-                if (upto - cost <= rest && rest < upto) {
-                    f.tile = t;
-                    f.at = (int)(rest - (upto - cost));
-                }
-                const long long all = __shfl_sync(0xffffffffu, upto, 31);
-                if (rest < all) break;
-                rest -= all;
-            }
-        }
-        __syncthreads();
-    }
-    share.seq = f.seq;
-    share.head = f.head;
-    share.tile = f.tile;
-    share.at = f.at;
     share.whole = whole;
-    f.total = total;   // (the same from every thread)
+    share.head = pg_div(rest, per_head);
+    rest -= share.head * per_head;
+    share.tile = 0;
+    const int tiles = g.tiles(share.s);
+    if (tiles > 1) {
+        for (int t0 = 0;; t0 += 32) {
+            const int t = t0 + lane;
+            const long long cost = t < tiles ? pg_span(a, share.s, t * g.tokens, (t + 1) * g.tokens).blocks() + g.extra : 0;
+            const long long upto = pg_warp_scan(cost), all = __shfl_sync(0xffffffffu, upto, 31);
+            if (rest < all || t0 + 32 >= tiles) {
+                const int src = __ffs(__ballot_sync(0xffffffffu, upto - cost <= rest && rest < upto)) - 1;
+                share.tile = t0 + src;
+                rest -= __shfl_sync(0xffffffffu, upto - cost, src);
+                break;
+            }
+            rest -= all;
+        }
+    }
+    share.at = (int)rest;
     return true;
 }
 
@@ -324,13 +340,13 @@ __device__ __forceinline__ PgPartial pg_partial(void* ws, int ctas, int cta, int
 
 // The header of a CTA's share (as pg_find_share left it), written by one thread that has time for the divisions.
 __device__ __forceinline__ void pg_write_header(const PagedMhaArgs& a, const PgTiling& g, void* ws, int cta, bool work, const PgShare& share,
-                                             const PgFound& found)
+                                                const PgPlace& place)
 {
     PgHeader h = {};
     if (work && share.at > g.extra) {
         const PgSpan span = pg_span(a, share.s, share.tile * g.tokens, (share.tile + 1) * g.tokens);
         h.kind = share.at + share.left >= span.blocks() + g.extra ? 1 : 2;
-        h.from = PgCut(found.total, (int)gridDim.x).of(found.begin - share.at + g.extra);   // where its first block is
+        h.from = PgCut(place.total, (int)gridDim.x).of(place.begin - share.at + g.extra);   // where its first block is
         h.head = share.head;
         h.row0 = share.s.row0 + share.tile * g.tokens;
         h.tokens = min(g.tokens, share.s.tokens - share.tile * g.tokens);

@@ -133,12 +133,13 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     PgShare share;
-    const bool work = pg_find_share(a, tiling, (int)blockIdx.x, (int)gridDim.x, whole != 0, sm.found, share);
+    PgPlace place;
+    const bool work = pg_find_share(a, tiling, (int)blockIdx.x, (int)gridDim.x, whole != 0, sm.found, share, place);
     const uint32_t tmem = sm.tmem_base;
     PgPiece p;
 
     if (!work) {
-        if (!whole && threadIdx.x == 0) pg_write_header(a, tiling, ws, (int)blockIdx.x, false, share, sm.found);
+        if (!whole && threadIdx.x == 0) pg_write_header(a, tiling, ws, (int)blockIdx.x, false, share, place);
     }
     else if (warp == 8) {
         // ------------------------------------------------------------------ producer
@@ -183,7 +184,7 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 page = next;
             }
         }
-        if (!whole && lane == 0) pg_write_header(a, tiling, ws, (int)blockIdx.x, true, all, sm.found);
+        if (!whole && lane == 0) pg_write_header(a, tiling, ws, (int)blockIdx.x, true, all, place);
         if (sm.abort) {
             // nothing of this CTA may still be on its way when it ends
             for (int e = max(0, issued - kPgStages); e < issued; ++e) {
