@@ -13,7 +13,7 @@
 //              of the one before (2.7 us a piece when there was one group): a thread per key = TMEM lane.  The powers are taken under a reference per row that all threads share; it
 //              moves only when a score has outgrown it by 2^8 (one vote of the 128 threads a block tells), so that no maximum
 //              crosses the threads in the usual block.  Sums stay with the threads until the end.
-//   warp 8     producer: Q, then K and V blocks of 128 keys through a ring of 32 KiB stages
+//   warp 8     producer: Q, then K and V blocks of 128 keys through two rings of 32 KiB stages
 //   warp 9     one thread issues the products; scores and probabilities have two buffers, so that S of the next block is there when
 //              the softmax of this one ends
 // Keys that no row sees may be anything, even NaN: masked by selection, their rows of V set to zero before the product.
@@ -32,10 +32,10 @@ template<int D>
 struct PwShape {
     static constexpr int kHalves = D / 64;
     static constexpr int kTile = kHalves * kPgKeys * 128;                    // a K or V block
-    static constexpr int kStages = D == 64 ? 8 : 6;
+    static constexpr int kStages = D == 64 ? 4 : 3;                          // blocks in flight, K and V each
     static constexpr int kQ = kHalves * kPwRows * 128;                            // rows of Q; two of them
     static constexpr int kP = 2 * kPwRows * 128;                                  // probabilities [2 x 64 keys][kPwRows]; two of them a group
-    static constexpr int kSmem = kStages * kTile + 2 * kQ + 4 * kP;
+    static constexpr int kSmem = 2 * kStages * kTile + 2 * kQ + 4 * kP;
     static constexpr uint32_t kTmemCols = 128;                               // two S, one O of either group: 96
 };
 
@@ -51,7 +51,7 @@ struct PwRows {
 
 struct PwSmem {
     uint64_t q_full[2], q_empty[2];
-    uint64_t full[8], empty[8];
+    uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];   // block i of the CTA is in stage i % kStages
     uint64_t s_full[2][2];      // [group][buffer]: S^T of a block has been computed
     uint64_t p_ready[2][2];     // its probabilities are there (four warps)
     uint64_t pv_done[2][2];     // its V^T.P^T has completed
@@ -99,8 +99,9 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         g_device_status = 2;
         return;
     }
-    uint8_t* ring = pw_dyn;
-    uint8_t* q_rows = ring + kStages * kTile;
+    uint8_t* k_ring = pw_dyn;
+    uint8_t* v_ring = k_ring + kStages * kTile;
+    uint8_t* q_rows = v_ring + kStages * kTile;
     uint8_t* p_rows = q_rows + 2 * Shape::kQ;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int group = a.heads / a.kv_heads;
@@ -119,8 +120,10 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             mbar_init(&sm.o_free[i], 4);
         }
         for (int i = 0; i < kStages; ++i) {
-            mbar_init(&sm.full[i], 1);
-            mbar_init(&sm.empty[i], 1);
+            mbar_init(&sm.k_full[i], 1);
+            mbar_init(&sm.k_empty[i], 1);
+            mbar_init(&sm.v_full[i], 1);
+            mbar_init(&sm.v_empty[i], 1);
         }
         sm.abort = 0;
         mbar_fence_init();
@@ -148,15 +151,25 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     else if (warp == 8) {
         // ------------------------------------------------------------------ producer
         const long long cap = (long long)a.max_pages << a.page_shift;
-        int stage = 0, issued = 0, pieces = 0;
-        uint32_t phase = 1;                                       // of `empty`: the first round finds the stages free
+        int k_loads = 0, v_loads = 0, pieces = 0;
         bool ok = true;
+        // K of a block goes out before V of the one in front, in the order of their use.
+        const int* v_row = nullptr;
+        int v_head = 0, v_key0 = 0, v_page = 0;
+        PgSpan v_span = {0, 0};
+        auto load_v = [&]() -> bool {
+            const int stage = v_loads % kStages;
+            if (!tc_wait_warp(&sm.v_empty[stage], (uint32_t)((v_loads / kStages + 1) & 1), &sm.abort)) return false;
+            PgLoader<D>{a, v_row, v_head, v_span}.load(&map_v, v_key0, v_page, v_ring + stage * kTile, &sm.v_full[stage]);
+            ++v_loads;
+            return true;
+        };
         const PgShare all = share;
         while (ok && share.next(a, tiling, p)) {
             if (p.blocks == 0) continue;
             const PgSpan span = pg_span(a, p.s, p.tile * tile_tokens, (p.tile + 1) * tile_tokens);
             const PgLoader<D> loader = {a, a.pages + p.seq * a.pages_stride, p.head, span};
-            int page = loader.page(p.top * kPgKeys), before = 0;
+            int page = loader.page(p.top * kPgKeys);
             const int qb = pieces & 1;
             if (pieces > 1 && !tc_wait_warp(&sm.q_empty[qb], (uint32_t)((pieces / 2 - 1) & 1), &sm.abort)) break;
             ++pieces;
@@ -167,29 +180,31 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                             &sm.q_full[qb]);
             }
             if (p.s.p0 + p.s.tokens > cap && lane == 0) g_device_status = 6;
-            auto put = [&](const CUtensorMap* map, int j, int page) -> bool {
-                if (!tc_wait_warp(&sm.empty[stage], phase, &sm.abort)) return false;
-                loader.load(map, (p.top - j) * kPgKeys, page, ring + stage * kTile, &sm.full[stage]);
-                ++issued;
-                if (++stage == kStages) {
-                    stage = 0;
-                    phase ^= 1;
-                }
-                return true;
-            };
-            for (int j = 0; j <= p.blocks && ok; ++j) {
-                const int next = j + 1 < p.blocks ? loader.page((p.top - j - 1) * kPgKeys) : 0;
-                if (j < p.blocks) ok = put(&map_k, j, page);
-                if (j > 0 && ok) ok = put(&map_v, j - 1, before);
-                before = page;
+            for (int j = 0; j < p.blocks && ok; ++j) {
+                const int key0 = (p.top - j) * kPgKeys;
+                const int next = j + 1 < p.blocks ? loader.page(key0 - kPgKeys) : 0;
+                const int stage = k_loads % kStages;
+                ok = tc_wait_warp(&sm.k_empty[stage], (uint32_t)((k_loads / kStages + 1) & 1), &sm.abort);
+                if (!ok) break;
+                loader.load(&map_k, key0, page, k_ring + stage * kTile, &sm.k_full[stage]);
+                if (k_loads++ > 0) ok = load_v();
+                v_row = loader.row;
+                v_head = p.head;
+                v_span = span;
+                v_key0 = key0;
+                v_page = page;
                 page = next;
             }
         }
+        if (ok && k_loads > 0) load_v();
         if (!whole && lane == 0) pg_write_header(a, tiling, ws, (int)blockIdx.x, true, all, place);
         if (sm.abort) {
             // nothing of this CTA may still be on its way when it ends
-            for (int e = max(0, issued - kStages); e < issued; ++e) {
-                mbar_wait_bounded(&sm.full[e % kStages], (uint32_t)((e / kStages) & 1));
+            for (int i = max(0, k_loads - kStages); i < k_loads; ++i) {
+                mbar_wait_bounded(&sm.k_full[i % kStages], (uint32_t)((i / kStages) & 1));
+            }
+            for (int i = max(0, v_loads - kStages); i < v_loads; ++i) {
+                mbar_wait_bounded(&sm.v_full[i % kStages], (uint32_t)((i / kStages) & 1));
             }
             for (int i = max(0, pieces - 2); i < pieces; ++i) mbar_wait_bounded(&sm.q_full[i & 1], (uint32_t)((i / 2) & 1));
         }
@@ -201,66 +216,76 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             constexpr uint32_t idesc_pv = umma_idesc_f16(128, kPwRows) | PgType<T>::idesc | (1u << 15);   // A (V^T) MN-major
             const uint64_t q_desc = umma_desc_sw128(smem_u32(q_rows));
             const uint64_t p_desc = umma_desc_sw128(smem_u32(p_rows));
-            const uint64_t k_desc = umma_desc_sw128(smem_u32(ring));
+            const uint64_t k_desc = umma_desc_sw128(smem_u32(k_ring));
             // (heads of 64: the tile's upper 64 rows read the same dims once more, nobody reads their sums)
-            const uint64_t v_desc = umma_desc_mn_sw128(smem_u32(ring), D == 128 ? (uint32_t)kHalf : 0u);
-            int pieces = 0;
-            int stage = 0;                  // loads are used in the order they are made
-            uint32_t phase = 0;
-            int qk[2] = {0, 0};             // blocks of either group whose products have been issued
-            bool ok = true;
-            auto next_stage = [&]() {
-                umma_commit(&sm.empty[stage]);
-                if (++stage == kStages) {
-                    stage = 0;
-                    phase ^= 1;
-                }
-            };
-            while (ok && share.next(a, tiling, p)) {
-                if (p.blocks == 0) continue;
-                const int n = p.blocks, qb = pieces & 1;
-                ok = tc_wait(&sm.q_full[qb], (uint32_t)((pieces / 2) & 1), &sm.abort);
-                if (!ok) break;
-                const uint32_t tmem_s = tmem + (uint32_t)(qb * 3 * kPwRows), tmem_o = tmem_s + 2 * kPwRows;
-                int done_qk = qb ? qk[1] : qk[0], done_pv = done_qk;
-                auto issue_qk = [&](int j) -> bool {
-                    if (!tc_wait(&sm.full[stage], phase, &sm.abort)) return false;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint64_t kd = k_desc + (uint64_t)(stage * (kTile >> 4)), qd = q_desc + (uint64_t)(qb * (Shape::kQ >> 4));
+            const uint64_t v_desc = umma_desc_mn_sw128(smem_u32(v_ring), D == 128 ? (uint32_t)kHalf : 0u);
+            int k_stage = 0, v_stage = 0;
+            uint32_t k_phase = 0, v_phase = 0;
+            int done[2] = {0, 0};           // blocks of either group whose scores have been asked for
+            // S^T of block j of piece number i (of n blocks), which is the next that has been loaded
+            auto issue_qk = [&](int i, int j, int n) -> bool {
+                const int x = i & 1;
+                if (j == 0 && !tc_wait(&sm.q_full[x], (uint32_t)((i / 2) & 1), &sm.abort)) return false;
+                if (!tc_wait(&sm.k_full[k_stage], k_phase, &sm.abort)) return false;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const int buf = (x ? done[1] : done[0]) & 1;
+                const uint64_t kd = k_desc + (uint64_t)(k_stage * (kTile >> 4)), qd = q_desc + (uint64_t)(x * (Shape::kQ >> 4));
 #pragma unroll
-                    for (int kk = 0; kk < D / 16; ++kk) {
-                        umma_f16(tmem_s + (uint32_t)((done_qk & 1) * kPwRows), kd + (uint64_t)((kk >> 2) * (kHalf >> 4) + (kk & 3) * 2),
-                                 qd + (uint64_t)((kk >> 2) * (kPwRows * 128 >> 4) + (kk & 3) * 2), idesc_qk, kk != 0);
-                    }
-                    umma_commit(&sm.s_full[qb][done_qk & 1]);
-                    next_stage();
-                    if (j == n - 1) umma_commit(&sm.q_empty[qb]);
-                    ++done_qk;
-                    return true;
-                };
-                // S of block j + 2 goes where that of block j was, which has been read when its probabilities are there
-                ok = issue_qk(0) && (n == 1 || issue_qk(1));
-                if (ok && pieces > 1) ok = tc_wait(&sm.o_free[qb], (uint32_t)((pieces / 2 - 1) & 1), &sm.abort);
-                for (int j = 0; j < n && ok; ++j) {
-                    ok = tc_wait(&sm.full[stage], phase, &sm.abort) &&
-                         tc_wait(&sm.p_ready[qb][done_pv & 1], (uint32_t)((done_pv >> 1) & 1), &sm.abort);
+                for (int kk = 0; kk < D / 16; ++kk) {
+                    umma_f16(tmem + (uint32_t)(x * 3 * kPwRows + buf * kPwRows), kd + (uint64_t)((kk >> 2) * (kHalf >> 4) + (kk & 3) * 2),
+                             qd + (uint64_t)((kk >> 2) * (kPwRows * 128 >> 4) + (kk & 3) * 2), idesc_qk, kk != 0);
+                }
+                umma_commit(&sm.s_full[x][buf]);
+                umma_commit(&sm.k_empty[k_stage]);
+                if (j == n - 1) umma_commit(&sm.q_empty[x]);
+                if (x) ++done[1];
+                else ++done[0];
+                if (++k_stage == kStages) {
+                    k_stage = 0;
+                    k_phase ^= 1;
+                }
+                return true;
+            };
+            auto next_piece = [&](int& n) -> bool {   // that has keys to read
+                while (share.next(a, tiling, p)) {
+                    n = p.blocks;
+                    if (n > 0) return true;
+                }
+                return false;
+            };
+            // Scores are asked for one block ahead of the probabilities, across the pieces: those of a piece's first block are there
+            // when the other group begins it.  They go where those of two blocks before were, which have been read then.
+            int n = 0, next_n = 0;
+            bool ok = next_piece(n) && issue_qk(0, 0, n);
+            for (int i = 0; ok; ++i) {
+                const int x = i & 1;
+                const uint32_t tmem_o = tmem + (uint32_t)(x * 3 * kPwRows + 2 * kPwRows);
+                int block = (x ? done[1] : done[0]) - 1;      // of this group
+                bool more = true;
+                for (int j = 0; j < n && ok; ++j, ++block) {
+                    if (j + 1 < n) ok = issue_qk(i, j + 1, n);
+                    else if ((more = next_piece(next_n))) ok = issue_qk(i + 1, 0, next_n);
+                    if (ok && j == 0 && i > 1) ok = tc_wait(&sm.o_free[x], (uint32_t)((i / 2 - 1) & 1), &sm.abort);
+                    ok = ok && tc_wait(&sm.v_full[v_stage], v_phase, &sm.abort) &&
+                         tc_wait(&sm.p_ready[x][block & 1], (uint32_t)((block >> 1) & 1), &sm.abort);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint64_t vd = v_desc + (uint64_t)(stage * (kTile >> 4)),
-                                   pd = p_desc + (uint64_t)((2 * qb + (done_pv & 1)) * (Shape::kP >> 4));
+                    const uint64_t vd = v_desc + (uint64_t)(v_stage * (kTile >> 4)),
+                                   pd = p_desc + (uint64_t)((2 * x + (block & 1)) * (Shape::kP >> 4));
 #pragma unroll
                     for (int kk = 0; kk < kPgKeys / 16; ++kk) {
                         umma_f16(tmem_o, vd + (uint64_t)(kk * (2048 >> 4)), pd + (uint64_t)((kk >> 2) * (kPwRows * 128 >> 4) + (kk & 3) * 2),
                                  idesc_pv, j != 0 || kk != 0);
                     }
-                    umma_commit(&sm.pv_done[qb][done_pv & 1]);
-                    next_stage();
-                    ++done_pv;
-                    if (j + 2 < n) ok = issue_qk(j + 2);
+                    umma_commit(&sm.pv_done[x][block & 1]);
+                    umma_commit(&sm.v_empty[v_stage]);
+                    if (++v_stage == kStages) {
+                        v_stage = 0;
+                        v_phase ^= 1;
+                    }
                 }
-                if (qb) qk[1] = done_qk;
-                else qk[0] = done_qk;
-                ++pieces;
+                if (!more) break;
+                n = next_n;
             }
         }
     }
@@ -276,20 +301,16 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         PwRows& row = sm.rows[x];
         uint8_t* p_mine = p_rows + x * 2 * Shape::kP;
         float* cross = reinterpret_cast<float*>(p_mine);      // [kPwRows][128], for what crosses the threads while no product reads P
-        int stage = 0;                                        // of the loads, as the issuer counts them
-        uint32_t phase = 0;
-        int block = 0;                                        // blocks done
+        int before = 0;                                       // blocks of the share in front of the piece
+        int block = 0;                                        // blocks that this group has done
         int pieces = 0;
         bool ok = true, failed = false;                       // this thread's waits; what the group has agreed on: all leave together
         while (share.next(a, tiling, p)) {
             const bool mine = p.blocks > 0 ? (pieces & 1) == x : x == 0;
             pieces += p.blocks > 0;
-            if (!mine) {
-                stage += 2 * p.blocks;
-                phase ^= (uint32_t)((stage / kStages) & 1);
-                stage %= kStages;
-                continue;
-            }
+            const int first_block = before;
+            before += p.blocks;
+            if (!mine) continue;
             const int token0 = p.tile * tile_tokens;
             const int rows = min(tile_tokens, p.s.tokens - token0) * group;
             const PgSpan span = pg_span(a, p.s, token0, token0 + tile_tokens);
@@ -392,15 +413,10 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 }
                 if (key0 < span.lo || key0 + kPgKeys > span.hi) {
                     // rows of V that nobody sees (late: V lands behind K, and this is the first block of most pieces)
-                    int v_stage = stage + pg_v_entry(j, p.blocks);
-                    uint32_t v_phase = phase;
-                    while (v_stage >= kStages) {
-                        v_stage -= kStages;
-                        v_phase ^= 1;
-                    }
-                    ok = tc_wait_warp(&sm.full[v_stage], v_phase, &sm.abort) && ok;   // (told at the next barrier)
+                    const int v_stage = (first_block + j) % kStages;
+                    ok = tc_wait_warp(&sm.v_full[v_stage], (uint32_t)(((first_block + j) / kStages) & 1), &sm.abort) && ok;   // (told at the next barrier)
                     if (key < span.lo || key >= span.hi) {
-                        uint4* zero = reinterpret_cast<uint4*>(ring + v_stage * kTile + r * 128);
+                        uint4* zero = reinterpret_cast<uint4*>(v_ring + v_stage * kTile + r * 128);
 #pragma unroll
                         for (int h = 0; h < kHalves; ++h) {
 #pragma unroll
@@ -414,9 +430,6 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 if (lane == 0) mbar_arrive(&sm.p_ready[x][buf]);
             }
             if (failed) break;
-            stage += 2 * p.blocks;
-            phase ^= (uint32_t)((stage / kStages) & 1);
-            stage %= kStages;
 
             // ---- epilogue: the sums of the threads, then O, a dim a thread
             if (p.blocks > 0) ok = tc_wait_warp(&sm.pv_done[x][(block - 1) & 1], (uint32_t)(((block - 1) >> 1) & 1), &sm.abort) && ok;
