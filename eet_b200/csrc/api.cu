@@ -616,7 +616,7 @@ static int check_paged(const char* who, int64_t tokens, int64_t seqs, int64_t he
     EET_CHECK(page_size >= 16 && page_size <= 256 && (page_size & (page_size - 1)) == 0,
               "%s: page size %lld, only 16, 32, 64, 128 and 256 are supported", who, (long long)page_size);
     EET_CHECK(num_pages >= 0 && num_pages <= INT32_MAX, "%s: bad number of pages", who);
-    EET_CHECK(max_pages >= 0 && max_pages <= INT32_MAX / page_size, "%s: sequences are limited to 2^31 - 1 positions", who);
+    EET_CHECK(max_pages >= 0 && max_pages <= (INT32_MAX - 255) / page_size, "%s: sequences are limited to 2^31 - 256 positions", who);
     EET_CHECK(pages_stride >= max_pages || seqs <= 1, "%s: rows of the page table overlap", who);
     return 0;
 }
@@ -703,7 +703,7 @@ static int paged_mha_args(const eet_paged_mha_args* p, PagedMhaArgs& a)
     a.q_tok = p->q_tok, a.q_head = p->q_head, a.o_tok = p->o_tok, a.o_head = p->o_head;
     a.kc_page = p->kc_page, a.kc_head = p->kc_head, a.kc_slot = p->kc_slot;
     a.vc_page = p->vc_page, a.vc_head = p->vc_head, a.vc_slot = p->vc_slot;
-    a.window = p->window;
+    a.window = p->window < ((int64_t)1 << 40) ? p->window : (int64_t)1 << 40;
     const auto clamp = [](int64_t v, int64_t top) { return (int)(v < 1 || v > top ? top : v); };
     a.max_tokens = clamp(p->max_tokens, p->tokens);
     a.max_len = clamp(p->max_len, p->max_pages * p->page_size);

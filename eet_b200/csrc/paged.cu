@@ -39,6 +39,7 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryArgs a)
 {
     using P2 = Pair2<T>;
     using V2 = typename P2::type;
+    constexpr int kAhead = 3;   // items a thread has in flight
     __shared__ __align__(16) float2 cs[kRotMaxPairs];
     const int token = blockIdx.x;
     const int tid = threadIdx.x;
@@ -46,6 +47,33 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryArgs a)
     long long pos = 0;
     T* kdst = nullptr;
     T* vdst = nullptr;
+    pdl_launch_dependents();
+    pdl_wait();
+
+    const int per_row = a.head_dim >> 4;
+    const int at_once = kRotThreads / per_row;
+    const int rows = a.heads + a.kv_heads + (kStore ? a.kv_heads : 0);
+    const int step = (int)gridDim.y * at_once;
+    const int c = tid % per_row;
+    const bool turned = c < (a.rotary_dim >> 4);
+    const int d0 = (turned && !a.interleaved) ? 8 * c : 16 * c;
+    const int d1 = (turned && !a.interleaved) ? 8 * c + pairs : 16 * c + 8;
+    const int row0 = tid / per_row < at_once ? (int)blockIdx.y * at_once + tid / per_row : rows;
+    uint4 x[kAhead], y[kAhead];
+    auto load = [&](int row, uint4& u, uint4& w) {
+        const T* src;
+        if (row < a.heads) src = (const T*)a.q + (size_t)token * a.q_tok + (size_t)row * a.q_head;
+        else if (row < a.heads + a.kv_heads) src = (const T*)a.k + (size_t)token * a.k_tok + (size_t)(row - a.heads) * a.k_head;
+        else src = (const T*)a.v + (size_t)token * a.v_tok + (size_t)(row - a.heads - a.kv_heads) * a.v_head;
+        u = *reinterpret_cast<const uint4*>(src + d0);
+        w = *reinterpret_cast<const uint4*>(src + d1);
+    };
+    // (on their way while the angles are computed)
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+        if (row0 + i * step < rows) load(row0 + i * step, x[i], y[i]);
+    }
+
     if (kStore) {
         // the sequence of the token: how many of them end at or before it
         int seq = 0;
@@ -70,67 +98,61 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryArgs a)
     if (a.positions != nullptr) pos = a.positions[token];
     for (int i = tid; i < pairs; i += kRotThreads) {
         const double turns = (double)pos * (a.freqs[i] * 0.15915494309189533577);   // 1 / (2 pi)
-        float s, c;
-        sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
-        cs[i] = make_float2(c * a.magnitude, s * a.magnitude);
+        float s, co;
+        sincospif((float)(2.0 * (turns - rint(turns))), &s, &co);
+        cs[i] = make_float2(co * a.magnitude, s * a.magnitude);
     }
     __syncthreads();
 
-    const int per_row = a.head_dim >> 4;
-    const int rows = a.heads + a.kv_heads + (kStore ? a.kv_heads : 0);
-    const int step = (int)gridDim.y * (kRotThreads / per_row);
-    const int c = tid % per_row;
-    if (tid >= kRotThreads / per_row * per_row) return;
-    const bool turned = c < (a.rotary_dim >> 4);
-    const int d0 = (turned && !a.interleaved) ? 8 * c : 16 * c;
-    const int d1 = (turned && !a.interleaved) ? 8 * c + pairs : 16 * c + 8;
-    for (int row = (int)blockIdx.y * (kRotThreads / per_row) + tid / per_row; row < rows; row += step) {
-        const T* src;
+    auto store = [&](int row, uint4 u, uint4 w) {
         T* dst;
-        bool rot = turned;
         if (row < a.heads) {
-            src = (const T*)a.q + (size_t)token * a.q_tok + (size_t)row * a.q_head;
             dst = (T*)a.q_out + (size_t)token * a.qo_tok + (size_t)row * a.qo_head;
         }
         else if (row < a.heads + a.kv_heads) {
-            const int h = row - a.heads;
-            src = (const T*)a.k + (size_t)token * a.k_tok + (size_t)h * a.k_head;
             dst = kStore ? kdst : (T*)a.k_out + (size_t)token * a.ko_tok;
-            if (dst != nullptr) dst += (size_t)h * (kStore ? a.kc_head : a.ko_head);
+            if (dst != nullptr) dst += (size_t)(row - a.heads) * (kStore ? a.kc_head : a.ko_head);
         }
         else {
-            const int h = row - a.heads - a.kv_heads;
-            src = (const T*)a.v + (size_t)token * a.v_tok + (size_t)h * a.v_head;
             dst = vdst;
-            if (dst != nullptr) dst += (size_t)h * a.vc_head;
-            rot = false;
+            if (dst != nullptr) dst += (size_t)(row - a.heads - a.kv_heads) * a.vc_head;
         }
-        if (dst == nullptr) continue;
-        uint4 x = *reinterpret_cast<const uint4*>(src + d0), y = *reinterpret_cast<const uint4*>(src + d1);
-        if (rot) {
-            V2* xh = reinterpret_cast<V2*>(&x);
-            V2* yh = reinterpret_cast<V2*>(&y);
+        if (dst == nullptr) return;
+        if (turned && row < a.heads + a.kv_heads) {
+            V2* xh = reinterpret_cast<V2*>(&u);
+            V2* yh = reinterpret_cast<V2*>(&w);
             if (a.interleaved) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float2 t0 = cs[8 * c + e], t1 = cs[8 * c + 4 + e];
-                    const float2 u = P2::up(xh[e]), w = P2::up(yh[e]);
-                    xh[e] = P2::down(u.x * t0.x - u.y * t0.y, u.y * t0.x + u.x * t0.y);
-                    yh[e] = P2::down(w.x * t1.x - w.y * t1.y, w.y * t1.x + w.x * t1.y);
+                    const float2 f = P2::up(xh[e]), g = P2::up(yh[e]);
+                    xh[e] = P2::down(f.x * t0.x - f.y * t0.y, f.y * t0.x + f.x * t0.y);
+                    yh[e] = P2::down(g.x * t1.x - g.y * t1.y, g.y * t1.x + g.x * t1.y);
                 }
             }
             else {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float2 t0 = cs[8 * c + 2 * e], t1 = cs[8 * c + 2 * e + 1];
-                    const float2 u = P2::up(xh[e]), w = P2::up(yh[e]);
-                    xh[e] = P2::down(u.x * t0.x - w.x * t0.y, u.y * t1.x - w.y * t1.y);
-                    yh[e] = P2::down(w.x * t0.x + u.x * t0.y, w.y * t1.x + u.y * t1.y);
+                    const float2 f = P2::up(xh[e]), g = P2::up(yh[e]);
+                    xh[e] = P2::down(f.x * t0.x - g.x * t0.y, f.y * t1.x - g.y * t1.y);
+                    yh[e] = P2::down(g.x * t0.x + f.x * t0.y, g.y * t1.x + f.y * t1.y);
                 }
             }
         }
-        *reinterpret_cast<uint4*>(dst + d0) = x;
-        *reinterpret_cast<uint4*>(dst + d1) = y;
+        *reinterpret_cast<uint4*>(dst + d0) = u;
+        *reinterpret_cast<uint4*>(dst + d1) = w;
+    };
+    for (int row = row0; row < rows; row += kAhead * step) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            if (row + i * step < rows) store(row + i * step, x[i], y[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int next = row + (kAhead + i) * step;
+            if (next < rows) load(next, x[i], y[i]);
+        }
     }
 }
 
@@ -146,8 +168,7 @@ static int launch_rotary_t(const RotaryArgs& a, cudaStream_t stream)
     const int wanted = (4 * sm_count() + a.tokens - 1) / a.tokens;
     if (shares > wanted) shares = wanted;
     if (shares < 1) shares = 1;
-    rotary_kernel<T, kStore><<<dim3((unsigned)a.tokens, (unsigned)shares), kRotThreads, 0, stream>>>(a);
-    EET_LAUNCH_CHECK();
+    EET_CUDA(launch_pdl(rotary_kernel<T, kStore>, dim3((unsigned)a.tokens, (unsigned)shares), dim3(kRotThreads), 0, stream, a));
     return 0;
 }
 

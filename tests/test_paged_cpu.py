@@ -102,7 +102,7 @@ def _mha(**kw):
     ({"heads": 7}, b"7 heads"), ({"heads": 0}, b"0 heads"), ({"heads": 512}, b"512 heads"), ({"kv_heads": 0}, b"number of heads"),
     ({"window": -1}, b"window"), ({"q_tok": 1028}, b"multiples of 8"), ({"vc_slot": 132}, b"multiples of 8"),
     ({"tokens": -1}, b"tokens"), ({"seqs": -1}, b"sequences"), ({"pages_stride": 3}, b"overlap"),
-    ({"max_pages": 1 << 28, "pages_stride": 1 << 28}, b"2^31"), ({"num_pages": -1}, b"pages")])
+    ({"max_pages": 1 << 28, "pages_stride": 1 << 28}, b"2^31"), ({"max_pages": (1 << 27) - 1, "pages_stride": 1 << 28}, b"2^31"), ({"num_pages": -1}, b"pages")])
 def test_mha_refuses(change, message):
     assert lib.eet_paged_mha(_mha(**change), None) != 0
     assert message in lib.eet_last_error()

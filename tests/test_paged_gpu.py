@@ -479,6 +479,69 @@ def test_store_and_attention_of_a_prompt_in_chunks_and_then_token_by_token():
     assert _status() == 0
 
 
+@pytest.mark.parametrize("new", [[1, 1], [5, 3], [150, 40], [700, 1]])
+def test_mha_out_in_the_place_of_q(new):
+    """A tile's rows are written by who has read them, or by the second launch."""
+    batch = Batch(new, [3000, 710 if new[0] < 700 else 900], 8, 2)
+    kc, vc, *table = _gpu(batch)
+    want = _paged().paged_mha(batch.q.cuda(), kc, vc, *table)
+    q = batch.q.cuda()
+    assert _paged().paged_mha(q, kc, vc, *table, out=q) is q
+    assert torch.equal(q, want)
+
+
+def test_pages_far_behind_the_2_to_the_31st_value():
+    """Caches of 2.6e9 values each: the pages at their end and the same rows at their beginning."""
+    pages, K, P, D = 20000, 8, 128, 128
+    kc, vc = (torch.zeros(pages, K, P, D, dtype=FP16, device="cuda") for _ in range(2))
+    assert kc.numel() > 2 ** 31
+    gen = torch.Generator().manual_seed(1)
+    lens = torch.tensor([200, 131], dtype=torch.int32).cuda()
+    for new in ([200, 131], [3, 1]):
+        n = sum(new)
+        k, v = (torch.randn(n, K, D, generator=gen).half().cuda() for _ in range(2))
+        q = torch.randn(n, 16, D, generator=gen).half().cuda()
+        starts = torch.tensor([0, new[0], n], dtype=torch.int32).cuda()
+        got = []
+        for table in ([[0, 1], [2, 3]], [[pages - 1, pages - 7], [16384 + 1, pages - 2]]):
+            table = torch.tensor(table, dtype=torch.int32).cuda()
+            _paged().paged_store(k, v, kc, vc, table, starts, lens)
+            got.append(_paged().paged_mha(q, kc, vc, table, starts, lens))
+        assert torch.equal(*got)
+        for a, b, t in ((0, pages - 1, 128), (1, pages - 7, 72), (2, 16385, 128), (3, pages - 2, 3)):
+            assert torch.equal(kc[a, :, :t], kc[b, :, :t]) and torch.equal(vc[a, :, :t], vc[b, :, :t])
+    assert _status() == 0
+
+
+def test_calls_on_streams_of_their_own_in_turn():
+    """Work of one call behind another's on two streams that wait for each other; each call takes scratch of its own."""
+    batch = Batch([1, 1, 1], [4000, 50, 900], 8, 2)
+    args = (batch.q.cuda(), *_gpu(batch))
+    want = _paged().paged_mha(*args)
+    chunk = Batch([300, 2], [2000, 900], 8, 2, seed=3)
+    chunk_args = (chunk.q.cuda(), *_gpu(chunk))
+    chunk_want = _paged().paged_mha(*chunk_args)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    outs = []
+    for i in range(30):
+        with torch.cuda.stream(streams[i % 3]):
+            outs.append((_paged().paged_mha(*args), want) if i % 2 else (_paged().paged_mha(*chunk_args), chunk_want))
+    torch.cuda.synchronize()
+    assert all(torch.equal(got, ref) for got, ref in outs)
+    assert _status() == 0
+
+
+def test_mha_both_kernels_in_one_call():
+    """One chunk beside so many single tokens that they get the kernel of their own."""
+    new, lens = [200] + [1] * 40, [1100] + [3000 + 37 * i for i in range(40)]
+    assert 40 * 32 * (max(lens) // 128 + 1) >= 16384
+    for dtype in (FP16, BF16):
+        batch = Batch(new, lens, 32, 32, 64, 64, dtype, behind=2)
+        _check(batch)
+    some = Batch([1, 300, 0] + [1] * 30, [0, 300, 5] + [4000] * 30, 64, 32, 64, 32, seed=2)
+    _check(some, window=700, first_key=torch.tensor([0, 10, 0] + [3700 + i for i in range(30)], dtype=torch.int32))
+
 # ---------------------------------------------------------------------------------------------------------------------
 # the attention block
 # ---------------------------------------------------------------------------------------------------------------------
