@@ -1,6 +1,7 @@
 """eet_b200 - the int8 weight-only (W8A16) inference path of NetEase-FuXi/EET, rebuilt for NVIDIA B200.
 
 * ``eet_b200.EET``      - drop-in for the reference's pybind11 module ``EET`` on this path
+* ``eet_b200.paged``    - rotary positions, append and attention over a paged cache
 * ``eet_b200.modeling`` - LLaMA / Baichuan model wrappers with the reference's schema and signatures
 * ``eet_b200.tp``       - tensor parallelism over torch.distributed (NCCL)
 * ``libeet_b200.so``    - the CUDA kernels behind a C ABI (include/eet_b200.h), built by ``eet_b200.build``

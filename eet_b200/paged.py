@@ -251,8 +251,9 @@ def paged_mha(q, k_cache, v_cache, pages, starts, lens, max_tokens=None, max_len
       window                0: no window
       first_key             int32 [sequences]: positions before it are padding
       alibi_slopes          float32 [heads]: slope * (key position - p) is added to the scores
-    Rows of out that belong to no sequence are left as they are, uninitialised where this call allocated out.
-    K and V of every position that a token of the same tile sees must be finite."""
+    out may be q.  Rows of out that belong to no sequence are left as they are, uninitialised where this call allocated out.
+    Slots that no new token sees may hold anything.  What some new token of a sequence sees must be finite: a NaN or infinity in v reaches
+    other new tokens of that sequence, too, also those before it."""
     who = "paged_mha"
     shape = tokens, heads, head_dim = _first(who, "q", q)
     dtype, device, index = q.dtype, q.device, q.get_device()
