@@ -10,12 +10,16 @@
 //
 // One CTA per SM, its share of the work as paged_share.cuh says:
 //   warps 0-3, 4-7  softmax, two groups that take the pieces of the share in turn, so that the beginning of one runs beside the end
-//              of the one before (2.7 us a piece when there was one group): a thread per key = TMEM lane.  The powers are taken under a reference per row that all threads share; it
-//              moves only when a score has outgrown it by 2^8 (one vote of the 128 threads a block tells), so that no maximum
-//              crosses the threads in the usual block.  Sums stay with the threads until the end.
+//              of the one before (2.7 us a piece when there was one group): a thread per key = TMEM lane.  The powers are taken
+//              under a reference per row that all threads share; it moves only when a score has outgrown it by 2^8 (one vote of the
+//              128 threads a block tells), so that no maximum crosses the threads in the usual block.  Sums stay with the threads
+//              until the end.
 //   warp 8     producer: Q, then K and V blocks of 128 keys through two rings of 32 KiB stages
-//   warp 9     one thread issues the products; scores and probabilities have two buffers, so that S of the next block is there when
-//              the softmax of this one ends
+//   warp 9     one thread issues the products; scores and probabilities have two buffers, so that S of the next block - of the next
+//              piece, too - is there when the softmax of this one ends
+//
+// Measured: 64 sequences of 200 to 8000 tokens, 32 / 8 heads, bf16 93 us = 5.6 TB/s with everything around it; two of 60000 to 100000, 64 / 8
+// heads 117 us, 2760 cycles a block and SM in the loop = 6.5 TB/s.
 // Keys that no row sees may be anything, even NaN: masked by selection, their rows of V set to zero before the product.
 #include "paged_share.cuh"
 
@@ -33,8 +37,8 @@ struct PwShape {
     static constexpr int kHalves = D / 64;
     static constexpr int kTile = kHalves * kPgKeys * 128;                    // a K or V block
     static constexpr int kStages = D == 64 ? 4 : 3;                          // blocks in flight, K and V each
-    static constexpr int kQ = kHalves * kPwRows * 128;                            // rows of Q; two of them
-    static constexpr int kP = 2 * kPwRows * 128;                                  // probabilities [2 x 64 keys][kPwRows]; two of them a group
+    static constexpr int kQ = kHalves * kPwRows * 128;                       // rows of Q; two of them
+    static constexpr int kP = 2 * kPwRows * 128;                             // probabilities [2 x 64 keys][16]; two of them a group
     static constexpr int kSmem = 2 * kStages * kTile + 2 * kQ + 4 * kP;
     static constexpr uint32_t kTmemCols = 128;                               // two S, one O of either group: 96
 };
