@@ -199,11 +199,11 @@ static PagedPlan paged_plan(const PagedMhaArgs& a)
     p.tiles = !p.rows;
     p.few = 0x7fffffff;
     if (p.tiles) {
-        // Few tokens each beside the longest, and much to read for them?  A launch more costs 12 us; one chunk and 31 or 23 single tokens
-        // take, on both kernels and on the second alone: 32 / 8 heads, up to 1000 positions (248 tiles of up to 9 blocks) 47 and 37 us;
-        // 40 heads, up to 2500 (920 of up to 20) 132 and 186.
+        // Few tokens each beside the longest, and something to read for them?  One chunk of 200 and 31 single tokens behind up to 1000
+        // positions take, with both kinds of CTAs and with tiles alone: 32 heads 67 and 82 us, 32 / 8 heads 32 and 36; with 7 single
+        // tokens 34 and 41, 28 and 26.
         const long long others = a.seqs - 1, rest = a.tokens - a.max_tokens;
-        p.rows = others > 0 && is_few((rest + others - 1) / others) && others * a.kv_heads * (a.max_len / kPgKeys + 1) >= 16384;
+        p.rows = others > 0 && is_few((rest + others - 1) / others) && others * a.kv_heads * (a.max_len / kPgKeys + 1) >= 1024;
         p.few = p.rows ? kPwRows / group : 0;
     }
     // Cutting tiles evens out the shares and costs a second launch: 4 us behind the first kernel, 7 behind the second, whose blocks
@@ -233,16 +233,14 @@ template<typename T, int D>
 static int launch_paged_mha_t(const PagedMhaArgs& a, const PagedPlan& p, cudaStream_t stream)
 {
     void* ws[2] = {a.ws, (char*)a.ws + p.bytes[0]};
-    int rc = 0;
-    if (p.rows) rc = pg_launch_rows<T, D>(a, ws[0], p.few, p.whole[0], stream);
+    // (the tiles without a bias take the maximum of the scores before the scale, which a negative one would turn round)
+    const bool bias = a.slopes != nullptr || !(a.scale > 0.f);
+    int rc;
+    if (!p.tiles) rc = pg_launch_rows<T, D>(a, ws[0], p.whole[0], stream);
+    else if (!p.rows) rc = bias ? pg_launch_tc<T, D, true>(a, ws[1], p.whole[1], stream) : pg_launch_tc<T, D, false>(a, ws[1], p.whole[1], stream);
+    else if (bias) rc = pg_launch_both<T, D, true>(a, ws[0], ws[1], p.few, p.whole[0], p.whole[1], stream);
+    else rc = pg_launch_both<T, D, false>(a, ws[0], ws[1], p.few, p.whole[0], p.whole[1], stream);
     if (rc) return rc;
-    if (p.tiles) {
-        const int least = p.few + 1;
-        // (the kernel without a bias takes the maximum of the scores before the scale, which a negative one would turn round)
-        rc = a.slopes != nullptr || !(a.scale > 0.f) ? pg_launch_tc<T, D, true>(a, ws[1], least, p.whole[1], stream)
-                                                     : pg_launch_tc<T, D, false>(a, ws[1], least, p.whole[1], stream);
-        if (rc) return rc;
-    }
     PgScratch s[2] = {};
     int n = 0;
     if (p.bytes[0]) s[n++] = {ws[0], kPwRows, 0};

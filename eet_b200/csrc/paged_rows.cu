@@ -90,20 +90,14 @@ __device__ __forceinline__ void tmem_st8_async(uint32_t taddr, const uint32_t (&
                  : "memory");
 }
 
+// The work of CTA `cta` of `ctas`; the scratch is laid out for `region` of them.
 template<typename T, int D>
-__global__ void __launch_bounds__(kPwThreads, 1)
-paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                      const __grid_constant__ CUtensorMap map_v, const __grid_constant__ PagedMhaArgs a, void* ws, int most, int whole)
+__device__ __forceinline__ void pw_rows(const CUtensorMap* map_q, const CUtensorMap* map_k, const CUtensorMap* map_v, const PagedMhaArgs& a,
+                                        void* ws, int most, int whole, int cta, int ctas, int region, PwSmem& sm, uint8_t* dyn)
 {
     using Shape = PwShape<D>;
     constexpr int kHalves = Shape::kHalves, kTile = Shape::kTile, kStages = Shape::kStages, kHalf = kPgKeys * 128;
-    extern __shared__ __align__(1024) uint8_t pw_dyn[];
-    __shared__ PwSmem sm;
-    if (smem_u32(pw_dyn) & 1023) {   // the swizzle goes by addresses; the alignment above is there, so this does not happen
-        g_device_status = 2;
-        return;
-    }
-    uint8_t* k_ring = pw_dyn;
+    uint8_t* k_ring = dyn;
     uint8_t* v_ring = k_ring + kStages * kTile;
     uint8_t* q_rows = v_ring + kStages * kTile;
     uint8_t* p_rows = q_rows + 2 * Shape::kQ;
@@ -145,12 +139,12 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     PgShare share;
     PgPlace place;
-    const bool work = pg_find_share(a, tiling, (int)blockIdx.x, (int)gridDim.x, whole != 0, sm.found, share, place);
+    const bool work = pg_find_share(a, tiling, cta, ctas, whole != 0, sm.found, share, place);
     const uint32_t tmem = sm.tmem_base;
     PgPiece p;
 
     if (!work) {
-        if (!whole && threadIdx.x == 0) pg_write_header(a, tiling, ws, (int)blockIdx.x, false, share, place);
+        if (!whole && threadIdx.x == 0) pg_write_header(a, tiling, ws, cta, ctas, false, share, place);
     }
     else if (warp == 8) {
         // ------------------------------------------------------------------ producer
@@ -164,7 +158,7 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         auto load_v = [&]() -> bool {
             const int stage = v_loads % kStages;
             if (!tc_wait_warp(&sm.v_empty[stage], (uint32_t)((v_loads / kStages + 1) & 1), &sm.abort)) return false;
-            PgLoader<D>{a, v_row, v_head, v_span}.load(&map_v, v_key0, v_page, v_ring + stage * kTile, &sm.v_full[stage]);
+            PgLoader<D>{a, v_row, v_head, v_span}.load(map_v, v_key0, v_page, v_ring + stage * kTile, &sm.v_full[stage]);
             ++v_loads;
             return true;
         };
@@ -180,7 +174,7 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             if (lane == 0) mbar_arrive_expect_tx(&sm.q_full[qb], (uint32_t)(tile_tokens * group * 128 * kHalves));
             __syncwarp();
             if (lane < kHalves) {
-                tma_load_3d(q_rows + qb * Shape::kQ + lane * kPwRows * 128, &map_q, 64 * lane, p.head * group, p.s.row0 + p.tile * tile_tokens,
+                tma_load_3d(q_rows + qb * Shape::kQ + lane * kPwRows * 128, map_q, 64 * lane, p.head * group, p.s.row0 + p.tile * tile_tokens,
                             &sm.q_full[qb]);
             }
             if (p.s.p0 + p.s.tokens > cap && lane == 0) g_device_status = 6;
@@ -190,7 +184,7 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 const int stage = k_loads % kStages;
                 ok = tc_wait_warp(&sm.k_empty[stage], (uint32_t)((k_loads / kStages + 1) & 1), &sm.abort);
                 if (!ok) break;
-                loader.load(&map_k, key0, page, k_ring + stage * kTile, &sm.k_full[stage]);
+                loader.load(map_k, key0, page, k_ring + stage * kTile, &sm.k_full[stage]);
                 if (k_loads++ > 0) ok = load_v();
                 v_row = loader.row;
                 v_head = p.head;
@@ -201,7 +195,7 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             }
         }
         if (ok && k_loads > 0) load_v();
-        if (!whole && lane == 0) pg_write_header(a, tiling, ws, (int)blockIdx.x, true, all, place);
+        if (!whole && lane == 0) pg_write_header(a, tiling, ws, cta, ctas, true, all, place);
         if (sm.abort) {
             // nothing of this CTA may still be on its way when it ends
             for (int i = max(0, k_loads - kStages); i < k_loads; ++i) {
@@ -442,7 +436,7 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             if (pw_any(x, !ok)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const bool complete = p.starts && p.ends;
-            const PgPartial part = pg_partial(ws, (int)gridDim.x, (int)blockIdx.x, p.starts ? 1 : 0, kPwRows, D);
+            const PgPartial part = pg_partial(ws, region, cta, p.starts ? 1 : 0, kPwRows, D);
             {
                 const int n = (warp & 3) * 4 + (lane >> 3);
                 const float4* v = reinterpret_cast<const float4*>(cross + n * kPgKeys) + (lane & 7);
@@ -492,7 +486,74 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
 }
 
 template<typename T, int D>
-int pg_launch_rows(const PagedMhaArgs& a, void* ws, int most, int whole, cudaStream_t stream)
+__global__ void __launch_bounds__(kPwThreads, 1)
+paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                      const __grid_constant__ CUtensorMap map_v, const __grid_constant__ PagedMhaArgs a, void* ws, int whole)
+{
+    extern __shared__ __align__(1024) uint8_t pw_dyn[];
+    __shared__ PwSmem sm;
+    if (smem_u32(pw_dyn) & 1023) {   // the swizzle goes by addresses; the alignment above is there, so this does not happen
+        g_device_status = 2;
+        return;
+    }
+    pw_rows<T, D>(&map_q, &map_k, &map_v, a, ws, 0x7fffffff, whole, (int)blockIdx.x, (int)gridDim.x, (int)gridDim.x, sm, pw_dyn);
+}
+
+// Both kinds of work in one launch: sequences of up to `few` new tokens for the first CTAs, the others for the rest, as many as their blocks
+// take of the time.  Measured, a block on one CTA (heads of 128): few rows 1.46 us with pages of 16 (32 copies of 2 KB), 0.85 with pages of 64
+// and more; tiles 1.9 us, with a bias 3 to 3.5.  All CTAs together get a block of the first kind every 0.0106 us from HBM: more of them than use that up
+// are better spent on the tiles.
+// (As two launches one chunk of 777 tokens beside 23 single ones, 40 heads, took 65 + 49 us, with HBM idle in the second.)
+template<int D>
+__device__ __forceinline__ int pg_divide(int ctas, float in_rows, float in_tiles, int page_shift, bool bias)
+{
+    if (!(in_rows > 0.f)) return 0;
+    if (!(in_tiles > 0.f)) return ctas;
+    const float per_row = (page_shift == 4 ? 1.46f : page_shift == 5 ? 1.1f : 0.85f) * (D == 64 ? 0.7f : 1.0f);
+    const float per_tile = (bias ? 3.5f : 1.9f) * (D == 64 ? 0.7f : 1.0f);
+    const float all_of_hbm = per_row / (D == 64 ? 0.0053f : 0.0106f);
+    const float n = fminf((float)ctas * in_rows * per_row / (in_rows * per_row + in_tiles * per_tile), all_of_hbm);
+    // An even number: two neighbouring CTAs share more of an instruction cache than they should with different code (as the two at an
+    // odd border they took 126 and 131 us where the others had ended after 110).
+    const int even = 2 * (int)(0.5f * n + 0.5f);
+    return min(max(even, min(2, ctas - 1)), ctas - 1);
+}
+
+template<typename T, int D, bool kBias>
+__global__ void __launch_bounds__(kPwThreads, 1)
+paged_mha_both_kernel(const __grid_constant__ CUtensorMap map_q_rows, const __grid_constant__ CUtensorMap map_q,
+                      const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                      const __grid_constant__ PagedMhaArgs a, void* ws_rows, void* ws, int few, int whole_rows, int whole)
+{
+    static_assert(kPwThreads == kPgThreads, "one launch serves both");
+    extern __shared__ __align__(1024) uint8_t pb_dyn[];
+    __shared__ __align__(16) uint8_t sm[sizeof(PgSmem) > sizeof(PwSmem) ? sizeof(PgSmem) : sizeof(PwSmem)];
+    if (smem_u32(pb_dyn) & 1023) {
+        g_device_status = 2;
+        return;
+    }
+    pdl_launch_dependents();
+    pdl_wait();
+    const int group = a.heads / a.kv_heads, n = gridDim.x, cta = blockIdx.x;
+    const PgTiling few_rows = {kPwRows / group, 1, few, kPwExtra}, tiles = {2 * (kPgRows / group), few + 1, 0x7fffffff, kPgExtra};
+    const int n_rows = pg_divide<D>(n, (float)pg_total(a, few_rows), (float)pg_total(a, tiles), a.page_shift, kBias);
+    // every header is written: those behind the CTAs of one kind by those of the other
+    if (threadIdx.x == 0) {
+        const PgHeader none = {};
+        if (cta < n_rows && !whole) reinterpret_cast<PgHeader*>(ws)[n - n_rows + cta] = none;
+        if (cta >= n_rows && !whole_rows) reinterpret_cast<PgHeader*>(ws_rows)[cta] = none;
+    }
+    if (cta < n_rows) {
+        pw_rows<T, D>(&map_q_rows, &map_k, &map_v, a, ws_rows, few, whole_rows, cta, n_rows, n, *reinterpret_cast<PwSmem*>(sm), pb_dyn);
+    }
+    else {
+        pg_tiles<T, D, kBias>(&map_q, &map_k, &map_v, a, ws, few + 1, whole, cta - n_rows, n - n_rows, n, *reinterpret_cast<PgSmem*>(sm),
+                              pb_dyn);
+    }
+}
+
+template<typename T, int D>
+int pg_launch_rows(const PagedMhaArgs& a, void* ws, int whole, cudaStream_t stream)
 {
     CUtensorMap map_q, map_k, map_v;
     if (int rc = pg_encode_maps<T, D>(a, kPwRows / (a.heads / a.kv_heads), &map_q, &map_k, &map_v)) return rc;
@@ -506,7 +567,29 @@ int pg_launch_rows(const PagedMhaArgs& a, void* ws, int most, int whole, cudaStr
         EET_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
         attr_set[dev] = true;
     }
-    EET_CUDA(launch_pdl(kern, dim3(sm_count()), dim3(kPwThreads), kSmem, stream, map_q, map_k, map_v, a, ws, most, whole));
+    EET_CUDA(launch_pdl(kern, dim3(sm_count()), dim3(kPwThreads), kSmem, stream, map_q, map_k, map_v, a, ws, whole));
+    return 0;
+}
+
+template<typename T, int D, bool kBias>
+int pg_launch_both(const PagedMhaArgs& a, void* ws_rows, void* ws, int few, int whole_rows, int whole, cudaStream_t stream)
+{
+    const int group = a.heads / a.kv_heads;
+    CUtensorMap map_q_rows, map_q, map_k, map_v;
+    if (int rc = pg_encode_maps<T, D>(a, kPwRows / group, &map_q_rows, &map_k, &map_v)) return rc;
+    if (int rc = pg_encode_maps<T, D>(a, kPgRows / group, &map_q, &map_k, &map_v)) return rc;
+    auto kern = paged_mha_both_kernel<T, D, kBias>;
+    static bool attr_set[64] = {};
+    int dev = 0;
+    EET_CUDA(cudaGetDevice(&dev));
+    dev &= 63;
+    constexpr int kSmem = pg_tiles_smem(D) > PwShape<D>::kSmem ? pg_tiles_smem(D) : PwShape<D>::kSmem;
+    if (!attr_set[dev]) {
+        EET_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+        attr_set[dev] = true;
+    }
+    EET_CUDA(launch_pdl(kern, dim3(sm_count()), dim3(kPwThreads), kSmem, stream, map_q_rows, map_q, map_k, map_v, a, ws_rows, ws, few, whole_rows,
+                        whole));
     return 0;
 }
 

@@ -215,6 +215,21 @@ struct PgCut {
     }
 };
 
+// Blocks in all, by every warp.
+__device__ __forceinline__ long long pg_total(const PagedMhaArgs& a, const PgTiling& g)
+{
+    const int lane = threadIdx.x & 31;
+    long long sum = 0;
+    for (int base = 0; base < a.seqs; base += 32) {
+        PgSeq s = {0, 0, 0, 0};
+        if (base + lane < a.seqs) s = pg_seq(a, g, base + lane);
+        sum += pg_seq_blocks(a, g, s);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    return a.kv_heads * sum;
+}
+
 __device__ __forceinline__ int pg_div(long long x, long long d)
 {
     return (x | d) >> 32 ? (int)(x / d) : (int)((uint32_t)x / (uint32_t)d);
@@ -339,14 +354,14 @@ __device__ __forceinline__ PgPartial pg_partial(void* ws, int ctas, int cta, int
 }
 
 // The header of a CTA's share (as pg_find_share left it), written by one thread that has time for the divisions.
-__device__ __forceinline__ void pg_write_header(const PagedMhaArgs& a, const PgTiling& g, void* ws, int cta, bool work, const PgShare& share,
+__device__ __forceinline__ void pg_write_header(const PagedMhaArgs& a, const PgTiling& g, void* ws, int cta, int ctas, bool work, const PgShare& share,
                                                 const PgPlace& place)
 {
     PgHeader h = {};
     if (work && share.at > g.extra) {
         const PgSpan span = pg_span(a, share.s, share.tile * g.tokens, (share.tile + 1) * g.tokens);
         h.kind = share.at + share.left >= span.blocks() + g.extra ? 1 : 2;
-        h.from = PgCut(place.total, (int)gridDim.x).of(place.begin - share.at + g.extra);   // where its first block is
+        h.from = PgCut(place.total, ctas).of(place.begin - share.at + g.extra);   // where its first block is
         h.head = share.head;
         h.row0 = share.s.row0 + share.tile * g.tokens;
         h.tokens = min(g.tokens, share.s.tokens - share.tile * g.tokens);

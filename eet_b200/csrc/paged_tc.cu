@@ -88,21 +88,15 @@ __device__ __forceinline__ PgTurns pg_turns(const PagedMhaArgs& a, const PgPiece
     return r;
 }
 
+// The work of CTA `cta` of `ctas`; the scratch is laid out for `region` of them.
 template<typename T, int D, bool kBias>
-__global__ void __launch_bounds__(kPgThreads, 1)
-paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                    const __grid_constant__ CUtensorMap map_v, const __grid_constant__ PagedMhaArgs a, void* ws, int least, int whole)
+__device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtensorMap* map_k, const CUtensorMap* map_v, const PagedMhaArgs& a,
+                                         void* ws, int least, int whole, int cta, int ctas, int region, PgSmem& sm, uint8_t* dyn)
 {
     constexpr int kHalves = D / 64;
     constexpr int kHalf = kPgRows * 128;         // bytes of [128 rows][64 values], swizzled
     constexpr int kTile = kHalves * kHalf;       // a Q tile, a K or a V block
-    extern __shared__ __align__(1024) uint8_t pg_dyn[];
-    __shared__ PgSmem sm;
-    if (smem_u32(pg_dyn) & 1023) {   // the swizzle goes by addresses; the alignment above is there, so this does not happen
-        g_device_status = 2;
-        return;
-    }
-    uint8_t* q_tiles = pg_dyn;
+    uint8_t* q_tiles = dyn;
     uint8_t* ring = q_tiles + 2 * kTile;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int group = a.heads / a.kv_heads;
@@ -140,12 +134,12 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     PgShare share;
     PgPlace place;
-    const bool work = pg_find_share(a, tiling, (int)blockIdx.x, (int)gridDim.x, whole != 0, sm.found, share, place);
+    const bool work = pg_find_share(a, tiling, cta, ctas, whole != 0, sm.found, share, place);
     const uint32_t tmem = sm.tmem_base;
     PgPiece p;
 
     if (!work) {
-        if (!whole && threadIdx.x == 0) pg_write_header(a, tiling, ws, (int)blockIdx.x, false, share, place);
+        if (!whole && threadIdx.x == 0) pg_write_header(a, tiling, ws, cta, ctas, false, share, place);
     }
     else if (warp == 8) {
         // ------------------------------------------------------------------ producer
@@ -166,7 +160,7 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             __syncwarp();
             if (lane < (pair ? 2 : 1) * kHalves) {
                 const int x = lane / kHalves, h = lane % kHalves;
-                tma_load_3d(q_tiles + x * kTile + h * kHalf, &map_q, 64 * h, p.head * group, p.s.row0 + token0 + x * tile_tokens,
+                tma_load_3d(q_tiles + x * kTile + h * kHalf, map_q, 64 * h, p.head * group, p.s.row0 + token0 + x * tile_tokens,
                             &sm.q_full);
             }
             if (p.s.p0 + p.s.tokens > cap && lane == 0) g_device_status = 6;
@@ -184,13 +178,13 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             int page = loader.page(p.top * kPgKeys), before = 0;
             for (int j = 0; j <= p.blocks && ok; ++j) {
                 const int next = j + 1 < p.blocks ? loader.page((p.top - j - 1) * kPgKeys) : 0;
-                if (j < p.blocks) ok = put(&map_k, j, page);
-                if (j > 0 && ok) ok = put(&map_v, j - 1, before);
+                if (j < p.blocks) ok = put(map_k, j, page);
+                if (j > 0 && ok) ok = put(map_v, j - 1, before);
                 before = page;
                 page = next;
             }
         }
-        if (!whole && lane == 0) pg_write_header(a, tiling, ws, (int)blockIdx.x, true, all, place);
+        if (!whole && lane == 0) pg_write_header(a, tiling, ws, cta, ctas, true, all, place);
         if (sm.abort) {
             // nothing of this CTA may still be on its way when it ends
             for (int e = max(0, issued - kPgStages); e < issued; ++e) {
@@ -520,7 +514,7 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 l_run = l_run * scale_a + sm.b_sum[r] * scale_b;
             }
             const bool complete = p.starts && p.ends;
-            const PgPartial part = pg_partial(ws, (int)gridDim.x, (int)blockIdx.x, p.starts ? 1 : 0, 2 * kPgRows, D);
+            const PgPartial part = pg_partial(ws, region, cta, p.starts ? 1 : 0, 2 * kPgRows, D);
             if (complete) {
                 const float inv = l_run > 0.f ? 1.0f / l_run : 0.f;
                 scale_a *= inv;
@@ -586,10 +580,29 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     }
 }
 
-template<typename T, int D, bool kBias>
-int pg_launch_tc(const PagedMhaArgs& a, void* ws, int least, int whole, cudaStream_t stream)
+constexpr int pg_tiles_smem(int head_dim)
 {
-    constexpr int kSmem = (2 + kPgStages) * (D / 64) * kPgRows * 128;
+    return (2 + kPgStages) * (head_dim / 64) * kPgRows * 128;
+}
+
+template<typename T, int D, bool kBias>
+__global__ void __launch_bounds__(kPgThreads, 1)
+paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                    const __grid_constant__ CUtensorMap map_v, const __grid_constant__ PagedMhaArgs a, void* ws, int whole)
+{
+    extern __shared__ __align__(1024) uint8_t pg_dyn[];
+    __shared__ PgSmem sm;
+    if (smem_u32(pg_dyn) & 1023) {   // the swizzle goes by addresses; the alignment above is there, so this does not happen
+        g_device_status = 2;
+        return;
+    }
+    pg_tiles<T, D, kBias>(&map_q, &map_k, &map_v, a, ws, 1, whole, (int)blockIdx.x, (int)gridDim.x, (int)gridDim.x, sm, pg_dyn);
+}
+
+template<typename T, int D, bool kBias>
+int pg_launch_tc(const PagedMhaArgs& a, void* ws, int whole, cudaStream_t stream)
+{
+    constexpr int kSmem = pg_tiles_smem(D);
     CUtensorMap map_q, map_k, map_v;
     if (int rc = pg_encode_maps<T, D>(a, kPgRows / (a.heads / a.kv_heads), &map_q, &map_k, &map_v)) return rc;
     auto kern = paged_mha_tc_kernel<T, D, kBias>;
@@ -601,7 +614,7 @@ int pg_launch_tc(const PagedMhaArgs& a, void* ws, int least, int whole, cudaStre
         EET_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
         attr_set[dev] = true;
     }
-    EET_CUDA(launch_pdl(kern, dim3(sm_count()), dim3(kPgThreads), kSmem, stream, map_q, map_k, map_v, a, ws, least, whole));
+    EET_CUDA(launch_pdl(kern, dim3(sm_count()), dim3(kPgThreads), kSmem, stream, map_q, map_k, map_v, a, ws, whole));
     return 0;
 }
 
