@@ -60,9 +60,9 @@ __device__ __forceinline__ PgSeq pg_seq(const PagedMhaArgs& a, const PgTiling& g
 {
     PgSeq s;
     s.row0 = a.starts[b];
-    const int end = min(a.starts[b + 1], a.tokens);
-    s.tokens = s.row0 >= 0 ? max(0, end - s.row0) : 0;
-    s.p0 = a.lens[b] - s.tokens;
+    const int end = a.starts[b + 1];
+    s.tokens = s.row0 >= 0 ? max(0, min(end, a.tokens) - s.row0) : 0;
+    s.p0 = max(a.lens[b], 0) - (s.tokens > 0 ? end - s.row0 : 0);
     if (s.tokens < g.least || s.tokens > g.most) s.tokens = 0;
     s.first = a.first_key != nullptr ? max(0, a.first_key[b]) : 0;
     return s;

@@ -198,7 +198,7 @@ LENGTHS = [
     ([1], [1]), ([1], [129]), ([1, 1, 1], [16, 127, 300]), ([1, 0, 1], [64, 5, 1000]), ([5, 3, 1, 2], [5, 70, 128, 131]),
     ([17], [17]), ([40, 1], [640, 33]), ([130, 1, 129], [130, 900, 700]), ([300], [333]),
 ]
-HEADS = [(1, 1), (4, 4), (8, 2), (5, 1), (12, 2), (16, 1), (28, 4), (32, 1)]
+HEADS = [(1, 1), (4, 4), (8, 2), (5, 1), (12, 2), (16, 1), (17, 1), (28, 4), (32, 1), (100, 1), (128, 1)]
 
 
 @pytest.mark.parametrize("new,lens", LENGTHS)
@@ -327,6 +327,43 @@ def test_mha_does_not_follow_bad_pages(new):
     a, b = new[0], new[0] + new[1]
     _within(got[:a], ref[:a], tol[:a])
     _within(got[b:], ref[b:], tol[b:])
+
+
+def test_a_bad_page_is_named():
+    from eet_b200 import EET
+    batch = Batch([1], [20], 4, 2)
+    batch.pages[0, 0] = 1 << 30
+    _mha(batch)
+    with pytest.raises(EET.EETError, match="paged cache"):
+        EET.check_device_status()
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [4, 2, 3], [100, 40, 200]])
+def test_mha_of_starts_and_lengths_that_go_too_far(new):
+    """Fewer rows than starts say, lengths behind the table and below zero: nothing out of range, the others are served."""
+    n = sum(new)
+    batch = Batch(new, [260, 300, 280], 8, 2)
+    ref, tol = attend64(batch)
+    kc, vc, pages, starts, lens = _gpu(batch)
+    q = batch.q.cuda()
+    cut = n - 1 if new[2] == 1 else n - 2       # the last sequence loses its last rows, the rows that are there keep their positions
+    got = _paged().paged_mha(q[:cut], kc, vc, pages, starts, lens)
+    _within(got, ref[:cut], tol[:cut])
+    assert _status() == 0
+    for bad in (2 ** 31 - 1, 10 ** 6, -1, -2 ** 31):
+        lens[1] = bad
+        got = _paged().paged_mha(q, kc, vc, pages, starts, lens)
+        a, b = new[0], new[0] + new[1]
+        _within(got[:a], ref[:a], tol[:a])
+        _within(got[b:], ref[b:], tol[b:])
+        assert _status() == (6 if bad > 0 else 0)
+        if bad < 0:
+            assert (got[a:b] == 0).all()
+    lens[1] = 300
+    for bad in ([0, n + 5, new[0] + new[1], n], [-3, -1, 2 ** 31 - 1, n], [5, 3, 1, 0], [0, -2 ** 31, n, 2 ** 31 - 1]):
+        _paged().paged_mha(q, kc, vc, pages, torch.tensor(bad, dtype=torch.int32).cuda(), lens)
+        _paged().paged_store(batch.k.cuda(), batch.v.cuda(), kc, vc, pages, torch.tensor(bad, dtype=torch.int32).cuda(), lens, q=q)
+        _status()
 
 
 def test_mha_of_nothing():
