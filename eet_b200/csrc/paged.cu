@@ -194,7 +194,7 @@ static PagedPlan paged_plan(const PagedMhaArgs& a)
 {
     PagedPlan p = {};
     const int group = a.heads / a.kv_heads;
-    auto is_few = [&](long long tokens) { return tokens * group <= kPwRows; };
+    auto is_few = [&](long long tokens) { return (tokens > 0 ? tokens : 1) * group <= kPwRows; };
     p.rows = is_few(a.max_tokens);
     p.tiles = !p.rows;
     p.few = 0x7fffffff;
@@ -237,7 +237,8 @@ static int launch_paged_mha_t(const PagedMhaArgs& a, const PagedPlan& p, cudaStr
     const bool bias = a.slopes != nullptr || !(a.scale > 0.f);
     int rc;
     if (!p.tiles) rc = pg_launch_rows<T, D>(a, ws[0], p.whole[0], stream);
-    else if (!p.rows) rc = bias ? pg_launch_tc<T, D, true>(a, ws[1], p.whole[1], stream) : pg_launch_tc<T, D, false>(a, ws[1], p.whole[1], stream);
+    else if (!p.rows && bias) rc = pg_launch_tc<T, D, true>(a, ws[1], p.whole[1], stream);
+    else if (!p.rows) rc = pg_launch_tc<T, D, false>(a, ws[1], p.whole[1], stream);
     else if (bias) rc = pg_launch_both<T, D, true>(a, ws[0], ws[1], p.few, p.whole[0], p.whole[1], stream);
     else rc = pg_launch_both<T, D, false>(a, ws[0], ws[1], p.few, p.whole[0], p.whole[1], stream);
     if (rc) return rc;

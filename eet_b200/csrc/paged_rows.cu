@@ -412,7 +412,8 @@ __device__ __forceinline__ void pw_rows(const CUtensorMap* map_q, const CUtensor
                 if (key0 < span.lo || key0 + kPgKeys > span.hi) {
                     // rows of V that nobody sees (late: V lands behind K, and this is the first block of most pieces)
                     const int v_stage = (first_block + j) % kStages;
-                    ok = tc_wait_warp(&sm.v_full[v_stage], (uint32_t)(((first_block + j) / kStages) & 1), &sm.abort) && ok;   // (told at the next barrier)
+                    const uint32_t parity = (uint32_t)(((first_block + j) / kStages) & 1);
+                    ok = tc_wait_warp(&sm.v_full[v_stage], parity, &sm.abort) && ok;   // (told at the next barrier)
                     if (key < span.lo || key >= span.hi) {
                         uint4* zero = reinterpret_cast<uint4*>(v_ring + v_stage * kTile + r * 128);
 #pragma unroll
@@ -500,9 +501,9 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
 }
 
 // Both kinds of work in one launch: sequences of up to `few` new tokens for the first CTAs, the others for the rest, as many as their blocks
-// take of the time.  Measured, a block on one CTA (heads of 128): few rows 1.46 us with pages of 16 (32 copies of 2 KB), 0.85 with pages of 64
-// and more; tiles 1.9 us, with a bias 3 to 3.5.  All CTAs together get a block of the first kind every 0.0106 us from HBM: more of them than use that up
-// are better spent on the tiles.
+// take of the time.  Measured, a block on one CTA (heads of 128): few rows 1.46 us with pages of 16 (32 copies of 2 KB), 0.85 with pages of
+// 64 and more; tiles 1.9 us, with a bias 3 to 3.5.  All CTAs together get a block of the first kind every 0.0106 us from HBM: more of them
+// than use that up are better spent on the tiles.
 // (As two launches one chunk of 777 tokens beside 23 single ones, 40 heads, took 65 + 49 us, with HBM idle in the second.)
 template<int D>
 __device__ __forceinline__ int pg_divide(int ctas, float in_rows, float in_tiles, int page_shift, bool bias)
@@ -588,8 +589,8 @@ int pg_launch_both(const PagedMhaArgs& a, void* ws_rows, void* ws, int few, int 
         EET_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
         attr_set[dev] = true;
     }
-    EET_CUDA(launch_pdl(kern, dim3(sm_count()), dim3(kPwThreads), kSmem, stream, map_q_rows, map_q, map_k, map_v, a, ws_rows, ws, few, whole_rows,
-                        whole));
+    EET_CUDA(launch_pdl(kern, dim3(sm_count()), dim3(kPwThreads), kSmem, stream, map_q_rows, map_q, map_k, map_v, a, ws_rows, ws,
+                        few, whole_rows, whole));
     return 0;
 }
 

@@ -354,8 +354,8 @@ __device__ __forceinline__ PgPartial pg_partial(void* ws, int ctas, int cta, int
 }
 
 // The header of a CTA's share (as pg_find_share left it), written by one thread that has time for the divisions.
-__device__ __forceinline__ void pg_write_header(const PagedMhaArgs& a, const PgTiling& g, void* ws, int cta, int ctas, bool work, const PgShare& share,
-                                                const PgPlace& place)
+__device__ __forceinline__ void pg_write_header(const PagedMhaArgs& a, const PgTiling& g, void* ws, int cta, int ctas, bool work,
+                                                const PgShare& share, const PgPlace& place)
 {
     PgHeader h = {};
     if (work && share.at > g.extra) {

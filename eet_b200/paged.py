@@ -99,8 +99,8 @@ def _heads(who, name, t, shape, dtype, index):
     """Token and head strides of a tensor that must have this shape."""
     strides = t.stride()
     if t.shape != shape or t.dtype != dtype or t.get_device() != index or strides[2] != 1:
-        raise RuntimeError(f"{who}: {name} must be a {dtype} tensor of shape {tuple(shape)} with a contiguous last dimension on cuda:{index}, "
-                           f"got {tuple(t.shape)} {t.dtype} with strides {strides} on {t.device}")
+        raise RuntimeError(f"{who}: {name} must be a {dtype} tensor of shape {tuple(shape)} with a contiguous last dimension on "
+                           f"cuda:{index}, got {tuple(t.shape)} {t.dtype} with strides {strides} on {t.device}")
     return strides[:2]
 
 

@@ -102,7 +102,8 @@ def _mha(**kw):
     ({"heads": 7}, b"7 heads"), ({"heads": 0}, b"0 heads"), ({"heads": 512}, b"512 heads"), ({"kv_heads": 0}, b"number of heads"),
     ({"window": -1}, b"window"), ({"q_tok": 1028}, b"multiples of 8"), ({"vc_slot": 132}, b"multiples of 8"),
     ({"tokens": -1}, b"tokens"), ({"seqs": -1}, b"sequences"), ({"pages_stride": 3}, b"overlap"),
-    ({"max_pages": 1 << 28, "pages_stride": 1 << 28}, b"2^31"), ({"max_pages": (1 << 27) - 1, "pages_stride": 1 << 28}, b"2^31"), ({"num_pages": -1}, b"pages")])
+    ({"max_pages": 1 << 28, "pages_stride": 1 << 28}, b"2^31"),
+    ({"max_pages": (1 << 27) - 1, "pages_stride": 1 << 28}, b"2^31"), ({"num_pages": -1}, b"pages")])
 def test_mha_refuses(change, message):
     assert lib.eet_paged_mha(_mha(**change), None) != 0
     assert message in lib.eet_last_error()
@@ -113,6 +114,21 @@ def test_nothing_to_do_is_no_error():
     assert lib.eet_paged_mha(_mha(seqs=0), None) == 0
     assert lib.eet_paged_mha_workspace_bytes(_mha(tokens=0)) == 0
     assert lib.eet_paged_mha(None, None) != 0 and b"NULL" in lib.eet_last_error()
+
+
+@pytest.mark.parametrize("group", [1, 3, 16, 17, 32, 128])
+def test_scratch_is_bounded_whatever_the_sizes(group):
+    """Any mix of chunks, single tokens and sequences that ask nothing; the work is planned before anything is launched."""
+    most = 148 * 2 * (256 + 16) * (128 + 2) * 4 + (1 << 16)     # two parts a CTA, of both kinds of tiles
+    for tokens in (1, 2, 5, 64, 65, 777, 10 ** 6):
+        for seqs in (1, 2, 33, 64, 3000):
+            for max_tokens in (0, 1, 2, 17, tokens):
+                for pages, max_len in ((0, 0), (1, 0), (4, 1), (4096, 0), (1 << 26, 0)):
+                    for window in (0, 1, 1000):
+                        need = lib.eet_paged_mha_workspace_bytes(_mha(
+                            heads=4 * group, kv_heads=4, tokens=tokens, seqs=seqs, max_tokens=max_tokens, max_pages=pages,
+                            pages_stride=pages, max_len=max_len, window=window))
+                        assert 0 <= need <= most
 
 
 def _store(**kw):

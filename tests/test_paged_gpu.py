@@ -366,6 +366,20 @@ def test_mha_of_starts_and_lengths_that_go_too_far(new):
         _status()
 
 
+@pytest.mark.parametrize("heads, kv_heads", [(32, 1), (34, 2), (128, 1), (16, 1), (8, 4)])
+@pytest.mark.parametrize("new", [[5] + [0] * 63, [0] * 40 + [7], [2] + [1] * 3 + [0] * 60])
+def test_mha_one_chunk_beside_sequences_without_tokens(heads, kv_heads, new):
+    """Long histories of sequences that ask nothing, with any number of query heads to a kv head."""
+    batch = Batch(new, [max(n, 40 + 3 * i % 70) for i, n in enumerate(new)], heads, kv_heads)
+    ref, tol = attend64(batch)
+    kc, vc, pages, starts, lens = _gpu(batch)
+    for kw in ({}, {"max_len": 10 ** 6}, {"max_tokens": 1}, {"max_tokens": 1, "max_len": 1}):
+        wide = torch.zeros(len(new), 4096, dtype=torch.int32, device="cuda")
+        wide[:, :pages.shape[1]] = pages
+        _within(_paged().paged_mha(batch.q.cuda(), kc, vc, wide, starts, lens, **kw), ref, tol)
+    assert _status() == 0
+
+
 def test_mha_of_nothing():
     batch = Batch([0, 0], [5, 0], 4, 2)
     assert _mha(batch).shape == (0, 4, 128)
@@ -651,7 +665,8 @@ def test_block_beside_llama_mmha():
         q = EET._pool.rows("qkv_paged", 2 * n, 3 * 512, 1, FP16, x.device).view(B, n, 3 * heads, 128)[:, :, :heads].abs().double()
         score = q.sum(-1) * k[:, None] / math.sqrt(128)                                           # [B][n][heads], at least the largest
         context = (4 * u + 2 * (4 + 1) * u * score) * v[:, None]
-        tol = context.repeat_interleave(128, -1).view(-1, 512) @ weights + 2 * u * (want.double().abs() + part.view(-1, hidden).double().abs()) + 1e-5
+        tol = context.repeat_interleave(128, -1).view(-1, 512) @ weights + 1e-5
+        tol += 2 * u * (want.double().abs() + part.view(-1, hidden).double().abs())
         off = (got.double() - want.double()).abs()
         assert (off <= tol).all() and off.max() < 0.02
     assert _status() == 0
