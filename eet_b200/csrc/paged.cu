@@ -206,9 +206,10 @@ static PagedPlan paged_plan(const PagedMhaArgs& a)
         p.rows = others > 0 && is_few((rest + others - 1) / others) && others * a.kv_heads * (a.max_len / kPgKeys + 1) >= 1024;
         p.few = p.rows ? kPwRows / group : 0;
     }
-    // Cutting tiles evens out the shares and costs a second launch: 4 us behind the first kernel, 7 behind the second, whose blocks
-    // take 0.8 us and 1.4 (heads of 64) or 1.9 us.  Not where whole tiles make the longest share no more than that longer, taking
-    // tiles to be three quarters as long as the longest on average.
+    // Cutting tiles evens out the shares and costs a second launch and parts to write, 4 to 6 us; a block takes 0.8 us in the first kernel
+    // and 1.4 (heads of 64) or 1.9 us in the second.  Not where whole tiles make the longest share no more than that longer, taking tiles
+    // to be three quarters as long as the longest on average.  (One block less for either, or two: 180 calls of the smaller kind 1.5 % and
+    // 2.3 % slower.)
     auto whole = [&](long long tokens, int most) {
         const long long sms = sm_count();
         const long long keys = a.window > 0 && a.window + tokens < a.max_len ? a.window + tokens : a.max_len;
@@ -247,8 +248,9 @@ static int launch_paged_mha_t(const PagedMhaArgs& a, const PagedPlan& p, cudaStr
     if (p.bytes[0]) s[n++] = {ws[0], kPwRows, 0};
     if (p.bytes[1]) s[n++] = {ws[1], 2 * kPgRows, 1};
     if (n > 0) {
-        const int y = ((p.bytes[1] ? 2 * kPgRows : kPwRows) * D / 16 + 255) / 256;   // 16 dims a thread
-        EET_CUDA(launch_pdl(paged_mha_join_kernel<T, D>, dim3(sm_count(), y, n), dim3(256), 0, stream, a, s[0], s[1]));
+        const long long rows = (long long)a.max_tokens * (a.heads / a.kv_heads), most = p.bytes[1] ? 2 * kPgRows : kPwRows;
+        const int y = (int)((rows < most ? rows : most) * (D / 8) + kPgJoinThreads - 1) / kPgJoinThreads;   // 8 dims a thread
+        EET_CUDA(launch_pdl(paged_mha_join_kernel<T, D>, dim3(sm_count(), y, n), dim3(kPgJoinThreads), 0, stream, a, s[0], s[1]));
     }
     return 0;
 }

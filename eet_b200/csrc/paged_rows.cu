@@ -447,7 +447,7 @@ __device__ __forceinline__ void pw_rows(const CUtensorMap* map_q, const CUtensor
 #pragma unroll
                 for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
                 if ((lane & 7) == 0) {
-                    row.corr[n] = sum > 0.f ? 1.0f / sum : 0.f;
+                    row.corr[n] = sum == 0.f ? 0.f : 1.0f / sum;
                     if (!complete) {
                         part.max2[n] = row.ref[n];
                         part.sum[n] = sum;
@@ -465,7 +465,7 @@ __device__ __forceinline__ void pw_rows(const CUtensorMap* map_q, const CUtensor
                         if (c + i < rows) {
                             const float v = __uint_as_float(o[i]), inv = row.corr[c + i];
                             if (!complete) reinterpret_cast<float*>(part.o)[(c + i) * D + r] = v;
-                            else ((T*)a.out)[row.out_at[c + i] + r] = (T)(inv > 0.f ? v * inv : 0.f);
+                            else ((T*)a.out)[row.out_at[c + i] + r] = (T)(inv == 0.f ? 0.f : v * inv);
                         }
                     }
                 }

@@ -375,11 +375,17 @@ struct PgScratch {
     int by_dim;            // O is [D / 4][rows], and a tile of 128 rows holds whole tokens only
 };
 
-// Adds up the partial results of the tiles that end in CTA blockIdx.x of one of the kernels (blockIdx.z), 16 dims of a row a
-// thread and turn.
+// Adds up the partial results of the tiles that end in CTA blockIdx.x of one of the kernels (blockIdx.z), 8 dims of a row a
+// thread and turn.  Bound: latency.  Two trips to L2, four parts on their way at once, and CTAs small enough (128 threads of 80
+// registers) to be resident beside the first kernel's, so that they wait for its end in place.  With CTAs of 256 threads of 64 registers,
+// which the 53760 of the 128-row kernel left no room for, and two passes over the parts: 16 x 5 tokens 39 us and not 36, the window
+// 24.7 and not 22.4, 64 single tokens 93.7 and not 91.6.
+constexpr int kPgJoinThreads = 128;
+
 template<typename T, int D>
-__global__ void __launch_bounds__(256) paged_mha_join_kernel(const __grid_constant__ PagedMhaArgs a, PgScratch s0, PgScratch s1)
+__global__ void __launch_bounds__(kPgJoinThreads, 6) paged_mha_join_kernel(const __grid_constant__ PagedMhaArgs a, PgScratch s0, PgScratch s1)
 {
+    constexpr int kAhead = 4;   // parts on their way
     pdl_wait();
     const PgScratch s = blockIdx.z ? s1 : s0;
     const PgHeader h = reinterpret_cast<const PgHeader*>(s.ws)[blockIdx.x];
@@ -388,51 +394,55 @@ __global__ void __launch_bounds__(256) paged_mha_join_kernel(const __grid_consta
     const int group = a.heads / a.kv_heads;
     const int rows = h.tokens * group;
     const int per_tile = s.by_dim ? kPgRows / group * group : s.rows;   // rows of a tile in use
-    for (int i = (int)(blockIdx.y * blockDim.x + threadIdx.x); i < rows * (D / 16); i += (int)(gridDim.y * blockDim.x)) {
-        const int row = s.by_dim ? i % rows : i / (D / 16), d16 = s.by_dim ? i / rows : i % (D / 16);
+    for (int i = (int)(blockIdx.y * blockDim.x + threadIdx.x); i < rows * (D / 8); i += (int)(gridDim.y * blockDim.x)) {
+        const int row = s.by_dim ? i % rows : i / (D / 8), d8 = s.by_dim ? i / rows : i % (D / 8);
         const int at = s.by_dim ? row / per_tile * kPgRows + row % per_tile : row;
-        const size_t o_at = s.by_dim ? (size_t)(4 * d16) * s.rows + at : (size_t)at * (D / 4) + 4 * d16;
+        const size_t o_at = s.by_dim ? (size_t)(2 * d8) * s.rows + at : (size_t)at * (D / 4) + 2 * d8;
         const int o_step = s.by_dim ? s.rows : 1;
         float top = -INFINITY, sum = 0.f;
-#pragma unroll 8
-        for (int c = h.from; c <= cta; ++c) {
-            const PgPartial p = pg_partial(s.ws, ctas, c, c == h.from ? 1 : 0, s.rows, D);
-            const float l = p.sum[at], m = p.max2[at];
-            if (l > 0.f) top = fmaxf(top, m);
-        }
-        float4 acc[4];
+        float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+        for (int c0 = h.from; c0 <= cta; c0 += kAhead) {
+            float l[kAhead], m[kAhead], next = top;
+            float4 o[kAhead][2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int c = h.from; c <= cta; ++c) {
-            const PgPartial p = pg_partial(s.ws, ctas, c, c == h.from ? 1 : 0, s.rows, D);
-            const float l = p.sum[at], m = p.max2[at];
-            float4 o[4];
+            for (int k = 0; k < kAhead; ++k) {
+                l[k] = 0.f;
+                if (c0 + k > cta) continue;
+                const PgPartial p = pg_partial(s.ws, ctas, c0 + k, c0 + k == h.from ? 1 : 0, s.rows, D);
+                l[k] = p.sum[at], m[k] = p.max2[at];
+                o[k][0] = p.o[o_at], o[k][1] = p.o[o_at + o_step];
+            }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = p.o[o_at + e * o_step];
-            if (l > 0.f) {   // (a piece that sees nothing has left no O)
-                const float w = ex2_approx(m - top);
-                sum += l * w;
+            for (int k = 0; k < kAhead; ++k) {
+                if (l[k] != 0.f) next = fmaxf(next, m[k]);
+            }
+            const float keep = sum != 0.f ? ex2_approx(top - next) : 0.f;
+            top = next;
+            sum *= keep;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    acc[e].x += o[e].x * w;
-                    acc[e].y += o[e].y * w;
-                    acc[e].z += o[e].z * w;
-                    acc[e].w += o[e].w * w;
+            for (int e = 0; e < 2; ++e) acc[e] = make_float4(acc[e].x * keep, acc[e].y * keep, acc[e].z * keep, acc[e].w * keep);
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                if (l[k] == 0.f) continue;   // (a piece that sees nothing has left no O)
+                const float w = ex2_approx(m[k] - top);
+                sum += l[k] * w;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    acc[e].x += o[k][e].x * w;
+                    acc[e].y += o[k][e].y * w;
+                    acc[e].z += o[k][e].z * w;
+                    acc[e].w += o[k][e].w * w;
                 }
             }
         }
-        const float inv = sum > 0.f ? 1.f / sum : 0.f;
-        T* dst = (T*)a.out + (size_t)(h.row0 + row / group) * a.o_tok + (size_t)(h.head * group + row % group) * a.o_head + 16 * d16;
-#pragma unroll
-        for (int e = 0; e < 4; e += 2) {
-            uint4 w;
-            w.x = PgType<T>::pack(acc[e].x * inv, acc[e].y * inv);
-            w.y = PgType<T>::pack(acc[e].z * inv, acc[e].w * inv);
-            w.z = PgType<T>::pack(acc[e + 1].x * inv, acc[e + 1].y * inv);
-            w.w = PgType<T>::pack(acc[e + 1].z * inv, acc[e + 1].w * inv);
-            *reinterpret_cast<uint4*>(dst + 4 * e) = w;
-        }
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        T* dst = (T*)a.out + (size_t)(h.row0 + row / group) * a.o_tok + (size_t)(h.head * group + row % group) * a.o_head + 8 * d8;
+        uint4 w;
+        w.x = PgType<T>::pack(acc[0].x * inv, acc[0].y * inv);
+        w.y = PgType<T>::pack(acc[0].z * inv, acc[0].w * inv);
+        w.z = PgType<T>::pack(acc[1].x * inv, acc[1].y * inv);
+        w.w = PgType<T>::pack(acc[1].z * inv, acc[1].w * inv);
+        *reinterpret_cast<uint4*>(dst) = w;
     }
 }
 

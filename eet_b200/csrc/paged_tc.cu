@@ -516,11 +516,11 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
             const bool complete = p.starts && p.ends;
             const PgPartial part = pg_partial(ws, region, cta, p.starts ? 1 : 0, 2 * kPgRows, D);
             if (complete) {
-                const float inv = l_run > 0.f ? 1.0f / l_run : 0.f;
+                const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;
                 scale_a *= inv;
                 scale_b *= inv;
             }
-            else {
+            else if (valid) {
                 part.max2[x * kPgRows + r] = max2;
                 part.sum[x * kPgRows + r] = l_run;
             }
@@ -530,9 +530,10 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
                 for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(dst + c) = make_uint4(0u, 0u, 0u, 0u);
             }
             if (mine) {
-                const bool nothing = complete && !(l_run > 0.f);
+                const bool nothing = complete && l_run == 0.f;
+                const int dims = __any_sync(0xffffffffu, valid) ? D : 0;   // (few rows: some warps have none)
 #pragma unroll 1
-                for (int c0 = 0; c0 < D; c0 += 32) {
+                for (int c0 = 0; c0 < dims; c0 += 32) {
                     uint32_t o[32];
                     tmem_ld32(t_o + (uint32_t)c0, o);
 #pragma unroll

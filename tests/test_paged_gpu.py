@@ -380,6 +380,21 @@ def test_mha_one_chunk_beside_sequences_without_tokens(heads, kv_heads, new):
     assert _status() == 0
 
 
+@pytest.mark.parametrize("new", [[1] * 40, [5, 7, 1], [70, 3, 200], [300]])
+@pytest.mark.parametrize("length", [400, 5000])
+def test_a_nan_in_q_stays_a_nan(new, length):
+    """Whole and cut tiles of both kinds: the token whose q holds it, no other."""
+    batch = Batch(new, [length + i for i in range(len(new))], 8, 2)
+    ref, tol = attend64(batch)
+    kc, vc, pages, starts, lens = _gpu(batch)
+    q, bad = batch.q.cuda(), sum(new) // 2
+    q[bad, 3, 17] = float("nan")
+    got = _paged().paged_mha(q, kc, vc, pages, starts, lens, max_tokens=max(new))
+    assert got[bad, 3].isnan().all()
+    got[bad, 3] = ref[bad, 3].to(got)
+    _within(got, ref, tol)
+
+
 def test_mha_of_nothing():
     batch = Batch([0, 0], [5, 0], 4, 2)
     assert _mha(batch).shape == (0, 4, 128)
