@@ -108,13 +108,26 @@ struct PgShare {
         tile = 0;
         if (++head < a.kv_heads) return;
         head = 0;
-        do {
+        for (;;) {
             if (++seq >= a.seqs) {
                 left = 0;
                 return;
             }
             s = pg_seq(a, g, seq);
-        } while (s.tokens == 0);
+            if (s.tokens > 0) return;
+            // Not one for this kernel; there may be many of them (slots without a sequence, single tokens around a chunk), so eight
+            // are looked at with one trip to memory (single tokens in the first and last of 300 slots: 31 us one by one, 21 so).
+            bool none = true;
+            while (none && seq + 1 < a.seqs) {
+                int found = 8;
+#pragma unroll
+                for (int i = 7; i >= 0; --i) {
+                    if (pg_seq(a, g, min(seq + 1 + i, a.seqs - 1)).tokens > 0) found = i;
+                }
+                none = found == 8;
+                seq += found;
+            }
+        }
     }
     __device__ __forceinline__ bool next(const PagedMhaArgs& a, const PgTiling& g, PgPiece& p)
     {
@@ -138,7 +151,7 @@ struct PgShare {
             p.ends = at + take == cost;
             left -= take;
             at += take;
-            if (p.ends) step(a, g);
+            if (p.ends && left > 0) step(a, g);
             if (p.blocks > 0 || n == 0 && p.ends) return true;
         }
         return false;

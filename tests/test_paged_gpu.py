@@ -380,6 +380,15 @@ def test_mha_one_chunk_beside_sequences_without_tokens(heads, kv_heads, new):
     assert _status() == 0
 
 
+@pytest.mark.parametrize("tokens", [1, 30])
+def test_mha_slots_without_a_sequence(tokens):
+    """Gaps of every length up to 19 between the sequences that ask something, many of them in one CTA's share."""
+    new = []
+    for gap in range(20):
+        new += [0] * gap + [tokens]
+    _check(Batch(new + [0] * 9, [tokens + 20 * i % 90 if n else 7 * i % 30 for i, n in enumerate(new + [0] * 9)], 2, 1, 64))
+
+
 @pytest.mark.parametrize("new", [[1] * 40, [5, 7, 1], [70, 3, 200], [300]])
 @pytest.mark.parametrize("length", [400, 5000])
 def test_a_nan_in_q_stays_a_nan(new, length):
