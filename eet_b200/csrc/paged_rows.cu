@@ -18,8 +18,8 @@
 //   warp 9     one thread issues the products; scores and probabilities have two buffers, so that S of the next block - of the next
 //              piece, too - is there when the softmax of this one ends
 //
-// Measured: 64 sequences of 200 to 8000 tokens, 32 / 8 heads, bf16 93 us = 5.6 TB/s with everything around it; two of 60000 to 100000, 64 / 8
-// heads 117 us, 2760 cycles a block and SM in the loop = 6.5 TB/s.
+// Measured: 64 sequences of 200 to 8000 tokens, 32 / 8 heads, bf16 92 us = 5.7 TB/s with everything around it; two of 60000 to 100000, 64 / 8
+// heads 114 us, 2760 cycles a block and SM in the loop = 6.5 TB/s.
 // Keys that no row sees may be anything, even NaN: masked by selection, their rows of V set to zero before the product.
 #include "paged_share.cuh"
 
