@@ -405,9 +405,10 @@ __device__ __forceinline__ void pw_rows(const CUtensorMap* map_q, const CUtensor
                 const int piece = (r & 63) >> 3;
 #pragma unroll
                 for (int n = 0; n < kPwRows; ++n) {
-                    const float e = ex2_approx(t[n] - row.ref[n]);
-                    l[n] += e;
-                    *reinterpret_cast<T*>(dst + n * 128 + ((piece ^ (n & 7)) << 4)) = (T)e;
+                    // (the sum is of the rounded ones: where one key has most of the weight, its rounding then cancels)
+                    const T e = (T)ex2_approx(t[n] - row.ref[n]);
+                    l[n] += (float)e;
+                    *reinterpret_cast<T*>(dst + n * 128 + ((piece ^ (n & 7)) << 4)) = e;
                 }
                 if (key0 < span.lo || key0 + kPgKeys > span.hi) {
                     // rows of V that nobody sees (late: V lands behind K, and this is the first block of most pieces)
