@@ -380,6 +380,33 @@ def test_mha_one_chunk_beside_sequences_without_tokens(heads, kv_heads, new):
     assert _status() == 0
 
 
+@pytest.mark.parametrize("tokens,heads", [(1, 4), (5, 1), (5, 4), (1, 1)])
+@pytest.mark.parametrize("view", ["plain", "fused", "heads first", "expanded heads", "expanded tokens", "wide rows"])
+def test_results_are_contiguous_whatever_the_strides(tokens, heads, view):
+    batch = Batch([tokens], [tokens + 40], heads, 1)
+    q = batch.q[:tokens].cuda()
+    if view == "fused":
+        q = torch.cat((q, q, q), 1)[:, heads:2 * heads]
+    elif view == "heads first":
+        q = q.transpose(0, 1).contiguous().transpose(0, 1)
+    elif view == "expanded heads":
+        q = q[:, :1].expand(tokens, heads, 128)
+    elif view == "expanded tokens":
+        q = q[:1].expand(tokens, heads, 128)
+    elif view == "wide rows":
+        q = torch.cat((q, q), 2)[..., :128]
+    kc, vc, pages, starts, lens = _gpu(batch)
+    freqs, at = _paged().rotary_frequencies(128, device="cuda")[0], torch.arange(tokens, device="cuda")
+    same = q.contiguous()
+    for get in (lambda x: _paged().paged_mha(x, kc, vc, pages, starts, lens),
+                lambda x: _paged().apply_rotary(x, None, at, freqs)[0],
+                lambda x: _paged().apply_rotary(None, x, at, freqs)[1],
+                lambda x: _paged().paged_store(batch.k.cuda()[:tokens], batch.v.cuda()[:tokens], kc, vc, pages, starts, lens, q=x,
+                                               freqs=freqs)):
+        got, want = get(q), get(same)
+        assert got.is_contiguous() and got.shape == q.shape and torch.equal(got, want)
+
+
 @pytest.mark.parametrize("tokens", [1, 30])
 def test_mha_slots_without_a_sequence(tokens):
     """Gaps of every length up to 19 between the sequences that ask something, many of them in one CTA's share."""
