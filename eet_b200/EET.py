@@ -334,9 +334,14 @@ def _gemm_row(x, w, scale, out, M, w2=None, scale2=None, residual=None, norm=Non
 def _linear(x, w, scale, out, residual=None):
     """One projection of an op: W8A16 when w is int8 (packed), else the fp16 twin - w fp16 [K, N] row-major
     through cuBLAS, as the reference's is_int8 == false branches do (cublasGemmEx in
-    csrc/op/llama_mmha.cpp:288-310, csrc/op/gated_ffn.cpp), then the residual with this library's kernel."""
+    csrc/op/llama_mmha.cpp:288-310, csrc/op/gated_ffn.cpp), then the residual with this library's kernel.  The residual may
+    lie in the place of out: an op's input is, when the op before it keeps its output in the same buffer."""
     if w.dtype == torch.int8:
         return gemm_w8a16(x, w, scale, out=out, residual=residual)
+    if residual is not None and residual.data_ptr() == out.data_ptr():
+        product = torch.matmul(x, w)
+        check(lib.eet_add_residual(out.data_ptr(), product.data_ptr(), out.numel(), _stream()))
+        return out
     torch.matmul(x, w, out=out)
     if residual is not None:
         check(lib.eet_add_residual(out.data_ptr(), residual.data_ptr(), out.numel(), _stream()))

@@ -783,3 +783,26 @@ def test_a_layer_of_a_model_step_captured():
         vc.copy_(before[1])
         assert torch.equal(step(), got)
     assert _status() == 0
+
+
+@pytest.mark.parametrize("rows,is_int8", [(3, False), (20, False), (70, False), (3, True), (16, True)])
+def test_block_and_llama_mmha_behind_one_another(rows, is_int8):
+    """The output of an attention op handed to the next: input and output of that one are the same buffer."""
+    from eet_b200 import EET
+    hidden, none = 256, torch.empty(0)
+    block, (qkv_w, qkv_s, out_w, out_s, norm) = _block(2, 2, hidden, is_int8, seed=7)
+    llama = EET.LlamaMmha(EET.MetaDesc(FP16, 4, 2, hidden, 1, 128, 512, d_kv=128, is_int8=is_int8), qkv_w, qkv_s, none, none, none, out_w,
+                          out_s, none, norm, none)
+    x = torch.randn(rows, hidden, generator=torch.Generator().manual_seed(rows)).half().cuda()
+    batch = Batch([rows], [rows], 2, 2)
+
+    def paged(y):
+        return block(y.view(rows, hidden), *_gpu(batch))
+
+    def own(y):
+        return llama(y.view(1, rows, hidden), none, none, True, True, True).view(rows, hidden)
+
+    for first in (paged, own):
+        for second in (paged, own):
+            want = second(first(x).clone()).clone()
+            assert torch.equal(second(first(x)), want)
