@@ -342,8 +342,8 @@ class PagedMmha:
             out = _pool.rows("self_mask_attn_cache", n, d.hidden_units, cap * d.hidden_units, torch.float16, d.device)
             if n == 0:
                 return out
-            _pending.pop(out.data_ptr(), None)   # whatever this buffer held before is gone
             _norm_head(input, self.ln_w, d.layernorm_eps, xn)
+            _pending.pop(out.data_ptr(), None)   # whatever this buffer held before is gone (behind the norm: it may be the input)
             _linear(xn, self.qkv_w, self.qkv_s, qkv)
             q, k, v = qkv.view(n, -1, 128).split((self.heads, self.kv_heads, self.kv_heads), 1)
             q = paged_store(k, v, k_cache, v_cache, pages, starts, lens, q=q, freqs=self.freqs, interleaved=self.interleaved,

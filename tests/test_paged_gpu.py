@@ -806,3 +806,57 @@ def test_block_and_llama_mmha_behind_one_another(rows, is_int8):
         for second in (paged, own):
             want = second(first(x).clone()).clone()
             assert torch.equal(second(first(x)), want)
+
+
+def _deferred_chain(rows, seed=11):
+    """A decode step of LlamaMmha (its input, behind a prompt of two), and a PagedMmha of fp16 weights that shows what it was given: its
+    queries, keys and values are channels of the norm, the output projection is zero, so that its output is its input."""
+    from eet_b200 import EET
+    hidden, none = 256, torch.empty(0)
+    gen = torch.Generator().manual_seed(seed)
+    desc = EET.MetaDesc(FP16, rows, 2, hidden, 1, 2, 4, d_kv=128, is_int8=True)
+    (qkv, qkv_s), (out, out_s) = (EET.quant_weights((torch.randn(hidden, n, generator=gen) / 16).half()) for n in (3 * hidden, hidden))
+    norm = (1 + 0.1 * torch.randn(hidden, generator=gen)).half().cuda()
+    llama = EET.LlamaMmha(desc, qkv.cuda(), qkv_s.cuda(), none, none, none, out.cuda(), out_s.cuda(), none, norm, none)
+    plain = EET.MetaDesc(FP16, rows, 2, hidden, 1, 2, 4, d_kv=128, is_int8=False)
+    eye = torch.eye(hidden, dtype=FP16)
+    block = _paged().PagedMmha(plain, torch.cat((eye, eye), 1).cuda(), None, torch.zeros(hidden, hidden, dtype=FP16).cuda(), None, norm,
+                               kv_head_num=1, alibi_slopes=torch.zeros(2, device="cuda"))
+    llama(torch.randn(rows, 2, hidden, generator=gen).half().cuda(), none, none, True, True, True)
+    x = torch.randn(rows, 1, hidden, generator=gen).half().cuda()
+
+    def step():
+        llama.step_ = 2
+        return llama(x, none, none, True, True, False).view(rows, hidden)
+
+    return step, block, norm
+
+
+@pytest.mark.parametrize("n", [17, 20, 64])
+def test_block_behind_an_attention_op_that_left_its_output_unfinished(n):
+    """17 to 64 rows inside deferred_epilogue(): the block finishes its input, which lies in the buffer that its own output takes.
+
+    Input and output are y, LlamaMmha's result, rounded to fp16 from sums that may be added in another order than outside: two roundings
+    of half a step u and 512 additions of terms that make at most 16 in magnitude (2^-24 each).  The keys and values are rounded norms of
+    it: two more roundings, and the factor of the norm, which moves by no more than its rows do."""
+    from eet_b200 import EET
+    step, block, norm = _deferred_chain(n)
+    want = step().clone()
+    batch = Batch([n], [n], 2, 1)
+    _, _, *table = _gpu(batch)
+    u, order = 2.0 ** -11, 512 * 16 * 2.0 ** -24
+    for _ in range(2):     # twice: the first leaves nothing behind
+        kc, vc = (torch.zeros(batch.k_cache.shape, dtype=FP16, device="cuda") for _ in range(2))
+        step().fill_(7.0)                 # what the buffer holds before
+        with EET.deferred_epilogue():
+            got = block(step(), kc, vc, *table).clone()
+        ref = want.double().cpu()
+        _within(got, ref, 2 * u * ref.abs() + order)
+        xn = ref * torch.rsqrt(ref.square().mean(-1, keepdim=True) + 1e-6) * norm.double().cpu()
+        tol = 6 * u * xn.abs() + 4 * order
+        for cache, part in ((kc, slice(0, 128)), (vc, slice(128, 256))):
+            _within(batch.history(cache.cpu(), 0)[:, 0], xn[:, part], tol[:, part])
+    with EET.deferred_epilogue():
+        again = step()
+    _within(again, want.double().cpu(), 2 * u * want.double().cpu().abs() + order)
+    assert _status() == 0
