@@ -486,6 +486,14 @@ def flush_pending():
     _pending.clear()
 
 
+def _forget(out):
+    """Before an op writes to `out`: whatever that buffer held is gone.  Sums that were to finish it, and that no op has read, become zero
+    again, as the next projection into them expects."""
+    p = _pending.pop(out.data_ptr(), None)
+    if isinstance(p, _Pending):
+        p.sums.zero_()
+
+
 def _norm_head(x2d, gamma, eps, xn):
     """RMSNorm at the head of a block; completes x first when it is a deferred output of the previous block."""
     M, n = x2d.shape
@@ -615,7 +623,7 @@ class _MmhaBase:
         out = _pool.rows("self_mask_attn_cache", B * S, d.hidden_units, d.batch_size * d.max_seq_len * d.hidden_units,
                          torch.float16, d.device)
         inp2d = inp.view(B * S, d.hidden_units)
-        _pending.pop(out.data_ptr(), None)   # whatever this buffer held before is gone
+        _forget(out)
         if _row_chain(B * S, d):
             _project_row(ctx2d, self.out_w, self.out_s, out, inp2d, B * S, d, "self_mask_attn_cache")
         elif _defer_ok(B * S, d):
@@ -862,7 +870,7 @@ class GatedFeedForwardNetworkInt8:
             act = _pool.rows("ffn_inner_act", M, self.d_ff, cap * self.d_ff, torch.float16, d.device)
             out = _pool.rows(self.cache_name, M, h, cap * h, torch.float16, d.device)
             inp2d = x2d
-            _pending.pop(out.data_ptr(), None)   # whatever this buffer held before is gone
+            _forget(out)
             deferred = _defer_ok(M, d)
             if deferred:
                 # gate and up in one launch, their epilogues inside the SwiGLU kernel

@@ -25,7 +25,7 @@ import struct
 import torch
 
 from ._lib import check, lib
-from .EET import _current_device, _linear, _norm_head, _on, _pending, _pool, _raw_stream
+from .EET import _current_device, _forget, _linear, _norm_head, _on, _pool, _raw_stream
 
 __all__ = ["rotary_frequencies", "apply_rotary", "paged_store", "paged_mha", "PagedMmha"]
 
@@ -343,7 +343,7 @@ class PagedMmha:
             if n == 0:
                 return out
             _norm_head(input, self.ln_w, d.layernorm_eps, xn)
-            _pending.pop(out.data_ptr(), None)   # whatever this buffer held before is gone (behind the norm: it may be the input)
+            _forget(out)   # (behind the norm: it may be the input)
             _linear(xn, self.qkv_w, self.qkv_s, qkv)
             q, k, v = qkv.view(n, -1, 128).split((self.heads, self.kv_heads, self.kv_heads), 1)
             q = paged_store(k, v, k_cache, v_cache, pages, starts, lens, q=q, freqs=self.freqs, interleaved=self.interleaved,

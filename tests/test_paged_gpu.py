@@ -860,3 +860,20 @@ def test_block_behind_an_attention_op_that_left_its_output_unfinished(n):
         again = step()
     _within(again, want.double().cpu(), 2 * u * want.double().cpu().abs() + order)
     assert _status() == 0
+
+
+def test_an_unfinished_output_that_nobody_reads_leaves_nothing_behind():
+    """Inside deferred_epilogue(): the sums of a projection whose output is overwritten, by this block or by an op of the same kind, are
+    zero for the next one.  The tolerance is that of the test above."""
+    from eet_b200 import EET
+    step, block, _ = _deferred_chain(20)
+    want = step().clone().double().cpu()
+    tol = 2 * 2.0 ** -11 * want.abs() + 512 * 16 * 2.0 ** -24
+    batch = Batch([20], [20], 2, 1)
+    other = torch.randn(20, 256, generator=torch.Generator().manual_seed(1)).half().cuda()
+    for write in (lambda: block(other, *_gpu(batch)), step):
+        with EET.deferred_epilogue():
+            step()
+            write()
+            got = step()
+        _within(got, want, tol)
