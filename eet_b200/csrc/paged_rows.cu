@@ -60,7 +60,6 @@ struct PwSmem {
     uint64_t p_ready[2][2];     // its probabilities are there (four warps)
     uint64_t pv_done[2][2];     // its V^T.P^T has completed
     uint64_t o_free[2];         // O of a piece has been read (four warps)
-    uint32_t tmem_base;
     volatile int abort;
     PwRows rows[2];
     PgFound found;
@@ -90,10 +89,35 @@ __device__ __forceinline__ void tmem_st8_async(uint32_t taddr, const uint32_t (&
                  : "memory");
 }
 
+// By one thread, in front of a barrier.
+template<int D>
+__device__ __forceinline__ void pw_init(PwSmem& sm)
+{
+    for (int i = 0; i < 2; ++i) {
+        mbar_init(&sm.q_full[i], 1);
+        mbar_init(&sm.q_empty[i], 1);
+        for (int buf = 0; buf < 2; ++buf) {
+            mbar_init(&sm.s_full[i][buf], 1);
+            mbar_init(&sm.p_ready[i][buf], 4);
+            mbar_init(&sm.pv_done[i][buf], 1);
+        }
+        mbar_init(&sm.o_free[i], 4);
+    }
+    for (int i = 0; i < PwShape<D>::kStages; ++i) {
+        mbar_init(&sm.k_full[i], 1);
+        mbar_init(&sm.k_empty[i], 1);
+        mbar_init(&sm.v_full[i], 1);
+        mbar_init(&sm.v_empty[i], 1);
+    }
+    sm.abort = 0;
+    mbar_fence_init();
+}
+
 // The work of CTA `cta` of `ctas`; the scratch is laid out for `region` of them.
 template<typename T, int D>
 __device__ __forceinline__ void pw_rows(const CUtensorMap* map_q, const CUtensorMap* map_k, const CUtensorMap* map_v, const PagedMhaArgs& a,
-                                        void* ws, int most, int whole, int cta, int ctas, int region, PwSmem& sm, uint8_t* dyn)
+                                        void* ws, int most, int whole, int cta, int ctas, int region, PwSmem& sm, const uint32_t& tmem_base,
+                                        uint8_t* dyn)
 {
     using Shape = PwShape<D>;
     constexpr int kHalves = Shape::kHalves, kTile = Shape::kTile, kStages = Shape::kStages, kHalf = kPgKeys * 128;
@@ -106,41 +130,10 @@ __device__ __forceinline__ void pw_rows(const CUtensorMap* map_q, const CUtensor
     const int tile_tokens = kPwRows / group;
     const PgTiling tiling = {tile_tokens, 1, most, kPwExtra};
 
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(&sm.q_full[i], 1);
-            mbar_init(&sm.q_empty[i], 1);
-            for (int buf = 0; buf < 2; ++buf) {
-                mbar_init(&sm.s_full[i][buf], 1);
-                mbar_init(&sm.p_ready[i][buf], 4);
-                mbar_init(&sm.pv_done[i][buf], 1);
-            }
-            mbar_init(&sm.o_free[i], 4);
-        }
-        for (int i = 0; i < kStages; ++i) {
-            mbar_init(&sm.k_full[i], 1);
-            mbar_init(&sm.k_empty[i], 1);
-            mbar_init(&sm.v_full[i], 1);
-            mbar_init(&sm.v_empty[i], 1);
-        }
-        sm.abort = 0;
-        mbar_fence_init();
-    }
-    if (warp == 9) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)),
-                     "r"(Shape::kTmemCols)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    pdl_launch_dependents();
-    pdl_wait();
-    __syncthreads();
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     PgShare share;
     PgPlace place;
     const bool work = pg_find_share(a, tiling, cta, ctas, whole != 0, sm.found, share, place);
-    const uint32_t tmem = sm.tmem_base;
+    const uint32_t tmem = tmem_base;
     PgPiece p;
 
     if (!work) {
@@ -479,12 +472,6 @@ __device__ __forceinline__ void pw_rows(const CUtensorMap* map_q, const CUtensor
             pw_any(x, false);   // the row's values have been read
         }
     }
-
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    __syncthreads();
-    if (warp == 9) {
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Shape::kTmemCols) : "memory");
-    }
 }
 
 template<typename T, int D>
@@ -494,11 +481,15 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
 {
     extern __shared__ __align__(1024) uint8_t pw_dyn[];
     __shared__ PwSmem sm;
+    __shared__ uint32_t tmem_base;
     if (smem_u32(pw_dyn) & 1023) {   // the swizzle goes by addresses; the alignment above is there, so this does not happen
         g_device_status = 2;
         return;
     }
-    pw_rows<T, D>(&map_q, &map_k, &map_v, a, ws, 0x7fffffff, whole, (int)blockIdx.x, (int)gridDim.x, (int)gridDim.x, sm, pw_dyn);
+    if (threadIdx.x == 0) pw_init<D>(sm);
+    pg_begin(&tmem_base, PwShape<D>::kTmemCols);
+    pw_rows<T, D>(&map_q, &map_k, &map_v, a, ws, 0x7fffffff, whole, (int)blockIdx.x, (int)gridDim.x, (int)gridDim.x, sm, tmem_base, pw_dyn);
+    pg_end(&tmem_base, PwShape<D>::kTmemCols);
 }
 
 // Both kinds of work in one launch: sequences of up to `few` new tokens for the first CTAs, the others for the rest, as many as their blocks
@@ -530,12 +521,12 @@ paged_mha_both_kernel(const __grid_constant__ CUtensorMap map_q_rows, const __gr
     static_assert(kPwThreads == kPgThreads, "one launch serves both");
     extern __shared__ __align__(1024) uint8_t pb_dyn[];
     __shared__ __align__(16) uint8_t sm[sizeof(PgSmem) > sizeof(PwSmem) ? sizeof(PgSmem) : sizeof(PwSmem)];
+    __shared__ uint32_t tmem_base;
     if (smem_u32(pb_dyn) & 1023) {
         g_device_status = 2;
         return;
     }
-    pdl_launch_dependents();
-    pdl_wait();
+    pg_begin(&tmem_base, kPgTmemCols);   // for either kind: which one follows from what the kernel in front leaves
     const int group = a.heads / a.kv_heads, n = gridDim.x, cta = blockIdx.x;
     const PgTiling few_rows = {kPwRows / group, 1, few, kPwExtra}, tiles = {2 * (kPgRows / group), few + 1, 0x7fffffff, kPgExtra};
     const int n_rows = pg_divide<D>(n, (float)pg_total(a, few_rows), (float)pg_total(a, tiles), a.page_shift, kBias);
@@ -545,13 +536,20 @@ paged_mha_both_kernel(const __grid_constant__ CUtensorMap map_q_rows, const __gr
         if (cta < n_rows && !whole) reinterpret_cast<PgHeader*>(ws)[n - n_rows + cta] = none;
         if (cta >= n_rows && !whole_rows) reinterpret_cast<PgHeader*>(ws_rows)[cta] = none;
     }
+    if (threadIdx.x == 0) {
+        if (cta < n_rows) pw_init<D>(*reinterpret_cast<PwSmem*>(sm));
+        else pg_init(*reinterpret_cast<PgSmem*>(sm));
+    }
+    __syncthreads();
     if (cta < n_rows) {
-        pw_rows<T, D>(&map_q_rows, &map_k, &map_v, a, ws_rows, few, whole_rows, cta, n_rows, n, *reinterpret_cast<PwSmem*>(sm), pb_dyn);
+        pw_rows<T, D>(&map_q_rows, &map_k, &map_v, a, ws_rows, few, whole_rows, cta, n_rows, n, *reinterpret_cast<PwSmem*>(sm), tmem_base,
+                      pb_dyn);
     }
     else {
         pg_tiles<T, D, kBias>(&map_q, &map_k, &map_v, a, ws, few + 1, whole, cta - n_rows, n - n_rows, n, *reinterpret_cast<PgSmem*>(sm),
-                              pb_dyn);
+                              tmem_base, pb_dyn);
     }
+    pg_end(&tmem_base, kPgTmemCols);
 }
 
 template<typename T, int D>

@@ -459,6 +459,33 @@ __global__ void __launch_bounds__(kPgJoinThreads, 6) paged_mha_join_kernel(const
     }
 }
 
+// ------------------------------------------------------------------------------------------------ tensor memory
+
+// Takes `columns` of tensor memory, by warp 9, and waits for the kernel in front.  The columns are taken, by all CTAs, before a dependent may
+// begin: the kernels that allocate before they wait (the projections do) rest on that no CTA of an earlier kernel waits for a later one, and
+// a dependent beside a CTA of this one could otherwise hold the columns that this one is still to take while it waits for its end.
+__device__ __forceinline__ void pg_begin(uint32_t* tmem_base, uint32_t columns)
+{
+    if ((threadIdx.x >> 5) == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_base)), "r"(columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    pdl_launch_dependents();
+    pdl_wait();
+}
+
+__device__ __forceinline__ void pg_end(const uint32_t* tmem_base, uint32_t columns)
+{
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if ((threadIdx.x >> 5) == 9) {
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*tmem_base), "r"(columns) : "memory");
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ keys and values
 
 __device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar)

@@ -45,7 +45,6 @@ struct PgSmem {
     uint64_t o_full[2];      // the last P.V of a piece has completed
     uint64_t o_free[2];      // O has been read (four warps)
     uint64_t b_ready;        // split: b's maximum and sum are in b_max, b_sum, its O is complete (four warps)
-    uint32_t tmem_base;
     volatile int abort;
     float b_max[kPgRows], b_sum[kPgRows];
     // what a softmax warp needs between its pieces, out of its registers while it works on one
@@ -88,10 +87,32 @@ __device__ __forceinline__ PgTurns pg_turns(const PagedMhaArgs& a, const PgPiece
     return r;
 }
 
+// By one thread, in front of a barrier.
+__device__ __forceinline__ void pg_init(PgSmem& sm)
+{
+    mbar_init(&sm.q_full, 1);
+    mbar_init(&sm.q_empty, 1);
+    for (int i = 0; i < kPgStages; ++i) {
+        mbar_init(&sm.full[i], 1);
+        mbar_init(&sm.empty[i], 1);
+    }
+    for (int x = 0; x < 2; ++x) {
+        mbar_init(&sm.s_full[x], 1);
+        mbar_init(&sm.p_half[x], 4);
+        mbar_init(&sm.p_ready[x], 4);
+        mbar_init(&sm.o_full[x], 1);
+        mbar_init(&sm.o_free[x], 4);
+    }
+    mbar_init(&sm.b_ready, 4);
+    sm.abort = 0;
+    mbar_fence_init();
+}
+
 // The work of CTA `cta` of `ctas`; the scratch is laid out for `region` of them.
 template<typename T, int D, bool kBias>
 __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtensorMap* map_k, const CUtensorMap* map_v, const PagedMhaArgs& a,
-                                         void* ws, int least, int whole, int cta, int ctas, int region, PgSmem& sm, uint8_t* dyn)
+                                         void* ws, int least, int whole, int cta, int ctas, int region, PgSmem& sm,
+                                         const uint32_t& tmem_base, uint8_t* dyn)
 {
     constexpr int kHalves = D / 64;
     constexpr int kHalf = kPgRows * 128;         // bytes of [128 rows][64 values], swizzled
@@ -103,39 +124,10 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
     const int tile_tokens = kPgRows / group, pair_tokens = 2 * tile_tokens;
     const PgTiling tiling = {pair_tokens, least, 0x7fffffff, kPgExtra};
 
-    if (threadIdx.x == 0) {
-        mbar_init(&sm.q_full, 1);
-        mbar_init(&sm.q_empty, 1);
-        for (int i = 0; i < kPgStages; ++i) {
-            mbar_init(&sm.full[i], 1);
-            mbar_init(&sm.empty[i], 1);
-        }
-        for (int x = 0; x < 2; ++x) {
-            mbar_init(&sm.s_full[x], 1);
-            mbar_init(&sm.p_half[x], 4);
-            mbar_init(&sm.p_ready[x], 4);
-            mbar_init(&sm.o_full[x], 1);
-            mbar_init(&sm.o_free[x], 4);
-        }
-        mbar_init(&sm.b_ready, 4);
-        sm.abort = 0;
-        mbar_fence_init();
-    }
-    if (warp == 9) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)),
-                     "r"(kPgTmemCols)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    pdl_launch_dependents();
-    pdl_wait();
-    __syncthreads();
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     PgShare share;
     PgPlace place;
     const bool work = pg_find_share(a, tiling, cta, ctas, whole != 0, sm.found, share, place);
-    const uint32_t tmem = sm.tmem_base;
+    const uint32_t tmem = tmem_base;
     PgPiece p;
 
     if (!work) {
@@ -573,12 +565,6 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
             }
         }
     }
-
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    __syncthreads();
-    if (warp == 9) {
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kPgTmemCols) : "memory");
-    }
 }
 
 constexpr int pg_tiles_smem(int head_dim)
@@ -593,11 +579,15 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 {
     extern __shared__ __align__(1024) uint8_t pg_dyn[];
     __shared__ PgSmem sm;
+    __shared__ uint32_t tmem_base;
     if (smem_u32(pg_dyn) & 1023) {   // the swizzle goes by addresses; the alignment above is there, so this does not happen
         g_device_status = 2;
         return;
     }
-    pg_tiles<T, D, kBias>(&map_q, &map_k, &map_v, a, ws, 1, whole, (int)blockIdx.x, (int)gridDim.x, (int)gridDim.x, sm, pg_dyn);
+    if (threadIdx.x == 0) pg_init(sm);
+    pg_begin(&tmem_base, kPgTmemCols);
+    pg_tiles<T, D, kBias>(&map_q, &map_k, &map_v, a, ws, 1, whole, (int)blockIdx.x, (int)gridDim.x, (int)gridDim.x, sm, tmem_base, pg_dyn);
+    pg_end(&tmem_base, kPgTmemCols);
 }
 
 template<typename T, int D, bool kBias>

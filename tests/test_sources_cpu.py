@@ -88,3 +88,19 @@ def test_exchange_arrives_at_the_cluster_barrier_once_behind_its_last_store():
     kernel = _body(text, "gemm_ts_kernel(")
     assert "summed = ok && tc_wait_warp(&sm.accum" in kernel
     assert re.search(r"if \([^)]*\bsummed\b.*\) mbar_arrive_cluster\(cluster_addr\(&sm.peers_done", kernel)
+
+
+def test_paged_attention_takes_its_tensor_memory_before_a_dependent_may_begin():
+    """The projections allocate tensor memory before they wait for the kernel in front, on the promise that no CTA of an earlier kernel
+    waits for a later one.  So a kernel that they may follow allocates, has a barrier behind that, and only then lets them begin; all
+    three kernels do it in one place, before they wait for anything themselves."""
+    share, rows, tiles = (_source(n) for n in ("paged_share.cuh", "paged_rows.cu", "paged_tc.cu"))
+    begin = _body(share, "void pg_begin(")
+    order = [begin.index(s) for s in ("tcgen05.alloc", "__syncthreads();", "pdl_launch_dependents();", "pdl_wait();")]
+    assert order == sorted(order)
+    for text in (rows, tiles, share.replace(begin, "")):
+        assert "tcgen05.alloc" not in text and "pdl_launch_dependents" not in text
+    for text, kernel in ((rows, "paged_mha_rows_kernel("), (rows, "paged_mha_both_kernel("), (tiles, "paged_mha_tc_kernel(")):
+        body = _body(text, kernel)
+        assert body.count("pg_begin(") == 1 and body.count("pg_end(") == 1
+        assert "wait" not in body[:body.index("pg_begin(")]
