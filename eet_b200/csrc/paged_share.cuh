@@ -56,12 +56,19 @@ struct PgTiling {
     __device__ __forceinline__ int tiles(const PgSeq& s) const { return (s.tokens + tokens - 1) / tokens; }
 };
 
+// Rows [row0, end) of q as far as they exist (`tokens` of them do), whatever starts holds: no difference is taken that could overflow.
+constexpr __host__ __device__ int pg_rows_of(int row0, int end, int tokens)
+{
+    const int to = end < tokens ? end : tokens;
+    return row0 >= 0 && to > row0 ? to - row0 : 0;
+}
+
 __device__ __forceinline__ PgSeq pg_seq(const PagedMhaArgs& a, const PgTiling& g, int b)
 {
     PgSeq s;
     s.row0 = a.starts[b];
     const int end = a.starts[b + 1];
-    s.tokens = s.row0 >= 0 ? max(0, min(end, a.tokens) - s.row0) : 0;
+    s.tokens = pg_rows_of(s.row0, end, a.tokens);
     s.p0 = max(a.lens[b], 0) - (s.tokens > 0 ? end - s.row0 : 0);
     if (s.tokens < g.least || s.tokens > g.most) s.tokens = 0;
     s.first = a.first_key != nullptr ? max(0, a.first_key[b]) : 0;

@@ -178,3 +178,39 @@ def test_structures_have_the_sizes_that_python_packs():
         fields = [f for decl in body.split(";") if decl.strip() for f in decl.split(",")]
         assert 8 * len(fields) == len(pack)
     assert ctypes.sizeof(ctypes.c_void_p) == 8
+
+
+def test_rows_of_a_sequence_whatever_starts_holds(tmp_path):
+    """How many rows of q a sequence has, by the kernels' own expression compiled for the host: never one outside q, also where the
+    difference of two bad starts would not fit 32 bits (which the compiler's check for that turns into an abort)."""
+    import os
+    import re
+    import subprocess
+    share = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "eet_b200", "csrc", "paged_share.cuh")
+    text = open(share).read()
+    seq = re.search(r"PgSeq pg_seq\([^)]*\)\s*\{(.*?)\n\}", text, re.S).group(1)
+    tokens = re.search(r"s\.tokens = (.*?);", seq).group(1).replace("s.row0", "row0").replace("a.tokens", "tokens")
+    helper = re.search(r"constexpr __host__ __device__ int pg_rows_of\(.*?\n\}", text, re.S)
+    source = (helper.group(0).replace("__host__ __device__", "") if helper else "") + """
+        #include <algorithm>
+        #include <cstdio>
+        #include <cstdlib>
+        using std::max;
+        using std::min;
+        int main(int, char** v)
+        {
+            const int row0 = (int)std::atoll(v[1]), end = (int)std::atoll(v[2]), tokens = (int)std::atoll(v[3]);
+            std::printf("%%d", %s);
+        }
+        """ % tokens
+    source = source.replace("max(", "max<int>(").replace("min(", "min<int>(")
+    (tmp_path / "rows.cc").write_text(source)
+    program = str(tmp_path / "rows")
+    subprocess.run(["g++", "-std=c++17", "-fsanitize=signed-integer-overflow", "-fsanitize-undefined-trap-on-error", "-o", program,
+                    str(tmp_path / "rows.cc")], check=True)
+    low, high = -2 ** 31, 2 ** 31 - 1
+    for tokens in (1, 100, high):
+        for row0 in (low, -1, 0, 1, 50, 100, high):
+            for end in (low, low + 1, -1, 0, 1, 50, 51, 100, high):
+                got = subprocess.run([program, str(row0), str(end), str(tokens)], check=True, capture_output=True, text=True).stdout
+                assert int(got) == (max(0, min(end, tokens) - row0) if row0 >= 0 else 0), (row0, end, tokens)

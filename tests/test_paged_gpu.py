@@ -877,3 +877,17 @@ def test_an_unfinished_output_that_nobody_reads_leaves_nothing_behind():
             write()
             got = step()
         _within(got, want, tol)
+
+
+@pytest.mark.parametrize("new", [[3, 1, 1], [3, 40, 200]])
+def test_mha_of_starts_that_end_far_below_their_beginning(new):
+    """The sequence whose rows would end at -2^31 has none; the rows of the others, and what lies behind q's, stay as they are to be."""
+    n = sum(new)
+    batch = Batch(new, [260, 300, 280], 8, 2)
+    ref, tol = attend64(batch)
+    kc, vc, pages, starts, lens = _gpu(batch)
+    starts[2] = -2 ** 31
+    out = torch.full((n + 400, 8, 128), 7.0, dtype=FP16, device="cuda")
+    _paged().paged_mha(batch.q.cuda(), kc, vc, pages, starts, lens, out=out[:n])
+    _within(out[:3], ref[:3], tol[:3])
+    assert (out[3:] == 7.0).all() and _status() == 0
