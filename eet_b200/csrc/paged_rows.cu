@@ -49,7 +49,7 @@ struct PwRows {
     float slope[kPwRows];         // of the bias, to the power of two
     int pos[kPwRows];             // its position
     long long out_at[kPwRows];    // where its result goes
-    float ref[kPwRows];           // the reference of its powers, as a power of two
+    float ref[kPwRows];           // the reference of its powers, as a power of two, less kUp
     float corr[kPwRows];          // what a moved reference takes from the sums so far; at the end 1 / sum
 };
 
@@ -286,6 +286,7 @@ __device__ __forceinline__ void pw_rows(const CUtensorMap* map_q, const CUtensor
         const int r = (warp & 3) * 32 + lane;                 // key of the block, and dim of O
         const uint32_t t_lane = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t tmem_s = tmem + t_lane + (uint32_t)(x * 3 * kPwRows), tmem_o = tmem_s + 2 * kPwRows;
+        constexpr float kUp = PgType<T>::kUp;
         const float log2e = 1.4426950408889634f;
         const float to_log2 = a.scale * log2e;
         const int cap = (int)min((long long)a.max_pages << a.page_shift, 0x7fffffffLL);
@@ -351,7 +352,7 @@ __device__ __forceinline__ void pw_rows(const CUtensorMap* map_q, const CUtensor
                 }
                 bool over = j == 0;
 #pragma unroll
-                for (int n = 0; n < kPwRows; ++n) over |= t[n] - row.ref[n] > 8.0f;
+                for (int n = 0; n < kPwRows; ++n) over |= t[n] - row.ref[n] > kPgLag + kUp;
                 // the buffer that the probabilities go to has been read by the product of two blocks before
                 if (block > 1) ok = tc_wait_warp(&sm.pv_done[x][buf], (uint32_t)(((block >> 1) - 1) & 1), &sm.abort) && ok;
                 if (pw_any(x, over || !ok)) {
@@ -374,8 +375,9 @@ __device__ __forceinline__ void pw_rows(const CUtensorMap* map_q, const CUtensor
                         for (int o = 4; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
                         if ((lane & 7) == 0) {
                             const float old = row.ref[n];
-                            row.corr[n] = m - old > 8.0f ? ex2_approx(old - m) : 1.0f;
-                            row.ref[n] = m - old > 8.0f ? m : old;
+                            const bool moves = m - old > kPgLag + kUp;
+                            row.corr[n] = moves ? ex2_approx(old - (m - kUp)) : 1.0f;
+                            row.ref[n] = moves ? m - kUp : old;
                         }
                     }
                     pw_any(x, false);

@@ -17,10 +17,17 @@ namespace {
 constexpr int kPgRows = 128;            // rows of a tile (paged_tc.cu)
 constexpr int kPgKeys = 128;            // keys of a block
 
+// Powers are taken under a reference that may stay behind a row's maximum by kPgLag (in powers of two).  The probabilities enter the product
+// as T: in fp16 they are held 2^kUp higher, so that they end at 2^15 and what lies down to 2^-21 of the largest is a normal value, to 2^-32
+// counts at all (without it 2^-14 and 2^-25: 20000 keys at 2^-26 of one other were lost, 3e-4 of the result).  The sums are of the same
+// powers, so nothing else knows.
+constexpr float kPgLag = 8.0f;
+
 template<typename T>
 struct PgType;
 template<>
 struct PgType<__half> {
+    static constexpr float kUp = 7.0f;
     static constexpr uint32_t idesc = 0;
     static constexpr CUtensorMapDataType tma = CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     static __device__ __forceinline__ uint32_t pack(float a, float b)
@@ -31,6 +38,7 @@ struct PgType<__half> {
 };
 template<>
 struct PgType<__nv_bfloat16> {
+    static constexpr float kUp = 0.0f;
     static constexpr uint32_t idesc = (1u << 7) | (1u << 10);
     static constexpr CUtensorMapDataType tma = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     static __device__ __forceinline__ uint32_t pack(float a, float b)

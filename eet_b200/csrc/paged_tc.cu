@@ -391,7 +391,7 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
                 m_run = fmaxf(m_run, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
                 float corr = 1.0f;
                 const bool first = j == turns.first;
-                const bool moves = (m_run - m_ref) * to_log2 > 8.0f;
+                const bool moves = (m_run - m_ref) * to_log2 > kPgLag;
                 if (moves) {
                     corr = ex2_approx((m_ref - m_run) * to_log2);
                     m_ref = m_run;
@@ -407,7 +407,8 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
                         tmem_st16_async(t_o + (uint32_t)c0, o);
                     }
                 }
-                const uint64_t scale2 = pair2(to_log2, to_log2), off2 = pair2(-m_ref * to_log2, -m_ref * to_log2);
+                const float off = PgType<T>::kUp - m_ref * to_log2;
+                const uint64_t scale2 = pair2(to_log2, to_log2), off2 = pair2(off, off);
                 uint64_t psum[2] = {0ull, 0ull};
                 auto exponents = [&](const uint32_t* v, uint32_t* pk) {
 #pragma unroll

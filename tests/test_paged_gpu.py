@@ -891,3 +891,27 @@ def test_mha_of_starts_that_end_far_below_their_beginning(new):
     _paged().paged_mha(batch.q.cuda(), kc, vc, pages, starts, lens, out=out[:n])
     _within(out[:3], ref[:3], tol[:3])
     assert (out[3:] == 7.0).all() and _status() == 0
+
+
+@pytest.mark.parametrize("new", [1, 20])
+def test_mha_fp16_counts_keys_far_below_the_largest(new):
+    """One key holds nearly all of the weight and 20000 others e^-18 = 2^-26 of it each: 3.0e-4 of the result, half a step of fp16 being
+    2.4e-4.  148 sequences that share one history, so that a CTA walks the whole of it under one reference.
+
+    The largest probability enters the product as 2^7 or more, so what is below the type's normal values is off by at most 2^-25 / 2^7 of it,
+    20000 times; the others and the result by half a step; the scores are exact."""
+    H, page, n = 1, 128, 20000
+    total = n + new
+    pages = -(-total // page)
+    kc, vc = torch.zeros(pages, H, page, 64, dtype=FP16), torch.ones(pages, H, page, 64, dtype=FP16)
+    kc[(n - 1) // page, 0, (n - 1) % page, 0] = 18.0
+    vc[(n - 1) // page, 0, (n - 1) % page] = 0.0
+    q = torch.zeros(148 * new, H, 64, dtype=FP16)
+    q[:, :, 0] = 1.0
+    table = torch.arange(pages, dtype=torch.int32).expand(148, pages).contiguous()
+    starts, lens = torch.arange(149, dtype=torch.int32) * new, torch.full((148,), total, dtype=torch.int32)
+    got = _paged().paged_mha(*(t.cuda() for t in (q, kc, vc, table, starts, lens)), scale=1.0, max_tokens=new).double().cpu()
+    w = math.exp(-18.0)
+    others = n - 1 + 1.0 + torch.arange(new, dtype=torch.float64).repeat(148)[:, None, None]     # the token itself and those before it
+    exact = others * w / (1.0 + others * w)
+    _within(got, exact.expand_as(got), (20100 * 2.0 ** -32 + 2 * 2.0 ** -11 * exact + 2.0 ** -25).expand_as(got))
