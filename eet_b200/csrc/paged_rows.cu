@@ -30,7 +30,6 @@ namespace {
 constexpr int kPwRows = 16;          // rows of a tile: the fewest columns that a product with 128 rows has
 constexpr int kPwThreads = 320;
 constexpr int kPwExtra = 2;         // a piece's beginning and end cost as much as two blocks
-constexpr float kPwNone = -1e20f;   // reference of a row that has seen nothing
 
 template<int D>
 struct PwShape {
@@ -314,7 +313,7 @@ __device__ __forceinline__ void pw_rows(const CUtensorMap* map_q, const CUtensor
                 row.high[r] = r < rows ? min(pos, cap - 1) : -1;
                 row.slope[r] = a.slopes != nullptr && r < rows ? a.slopes[p.head * group + r % group] * log2e : 0.f;
                 row.out_at[r] = (long long)(p.s.row0 + token0 + r / group) * a.o_tok + (long long)(p.head * group + r % group) * a.o_head;
-                row.ref[r] = kPwNone;
+                row.ref[r] = kPgNone;
             }
             pw_any(x, false);
             // blocks all of whose keys every row sees

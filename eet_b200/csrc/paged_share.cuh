@@ -22,6 +22,7 @@ constexpr int kPgKeys = 128;            // keys of a block
 // counts at all (without it 2^-14 and 2^-25: 20000 keys at 2^-26 of one other were lost, 3e-4 of the result).  The sums are of the same
 // powers, so nothing else knows.
 constexpr float kPgLag = 8.0f;
+constexpr float kPgNone = -3.402823466e38f;   // maximum and reference of a row that has seen nothing: no finite score lies below
 
 template<typename T>
 struct PgType;

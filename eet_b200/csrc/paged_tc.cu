@@ -32,7 +32,6 @@ constexpr int kPgThreads = 320;
 constexpr int kPgStages = 5;
 constexpr int kPgExtra = 3;             // a tile's beginning and end cost as much as three blocks
 constexpr uint32_t kPgTmemCols = 512;   // S of a, S of b (their probabilities over them), O of a, O of b: 128 each
-constexpr float kPgNone = -1e20f;       // running maximum of a row that has seen nothing
 
 // ------------------------------------------------------------------------------------------------ the kernel
 
@@ -61,6 +60,29 @@ __device__ __forceinline__ void tmem_st16_async(uint32_t taddr, const uint32_t (
         "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
         "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
         : "memory");
+}
+
+// The reference of a row: the power of a score s is 2^(s factor + off).  factor is log2(e) (and the scale, where scores are taken before it)
+// and off the reference times that, rounded to 24 bits: what of it is lost is a factor of all of the row's powers, and would be 2^512 at
+// scores of 10^10.  So from 2^24 on, where a unit in the last place of a score is a factor of 4 and more and a sum of products does not
+// hold so much, factor is the power of two below and off exact: equal scores weigh the same, a larger one hides the others.  (Subtracting
+// the reference from the scores first takes 2.5 % of a chunk, 4.5 with a bias.)
+struct PgReference {
+    float factor, off;
+    // what the sums under it are to be multiplied with, as a power of two
+    __device__ __forceinline__ float log2_of(float to_log2) const
+    {
+        const float inverse = __uint_as_float(0x7f000000u - __float_as_uint(factor));   // where it is a power of two
+        return factor == to_log2 ? -off : -off * inverse * to_log2;
+    }
+};
+
+template<typename T>
+__device__ __forceinline__ PgReference pg_reference(float maximum, float to_log2)
+{
+    if (!(fabsf(maximum * to_log2) >= 16777216.0f)) return {to_log2, fmaf(-maximum, to_log2, PgType<T>::kUp)};
+    const float below = __uint_as_float(__float_as_uint(to_log2) & 0xff800000u);
+    return {below, -maximum * below};
 }
 
 // The blocks of a piece that tile x (0: a, 1: b) works on: first, first + stride, ... below end (block numbers of the piece).
@@ -327,7 +349,8 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
                 if (kBias && valid && a.slopes != nullptr) slope = a.slopes[p.head * group + g];
             }
             const uint64_t rise[2] = {pair2(0.f, slope), pair2(2.f * slope, 3.f * slope)};   // of the bias over four keys
-            float m_run = kPgNone, m_ref = kPgNone, l_run = 0.f;
+            float m_run = kPgNone, l_run = 0.f;
+            PgReference ref = {1.0f, -kPgNone};   // (-inf stays -inf, and any score moves it)
             for (int j = turns.first; j < turns.end && ok; j += turns.stride) {
                 const int key0 = (top - j) * kPgKeys;
                 if (!tc_wait_warp(&sm.s_full[x], (uint32_t)(used & 1), &sm.abort)) {
@@ -391,10 +414,11 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
                 m_run = fmaxf(m_run, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
                 float corr = 1.0f;
                 const bool first = j == turns.first;
-                const bool moves = (m_run - m_ref) * to_log2 > kPgLag;
+                const bool moves = fmaf(m_run, ref.factor, ref.off) > kPgLag + PgType<T>::kUp;
                 if (moves) {
-                    corr = ex2_approx((m_ref - m_run) * to_log2);
-                    m_ref = m_run;
+                    const float old = ref.log2_of(to_log2);
+                    ref = pg_reference<T>(m_run, to_log2);
+                    corr = ex2_approx(old - ref.log2_of(to_log2));
                 }
                 // O under the new reference.  The P.V of the block before has completed: s_full was committed behind it.
                 if (!first && __any_sync(0xffffffffu, moves)) {
@@ -407,8 +431,7 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
                         tmem_st16_async(t_o + (uint32_t)c0, o);
                     }
                 }
-                const float off = PgType<T>::kUp - m_ref * to_log2;
-                const uint64_t scale2 = pair2(to_log2, to_log2), off2 = pair2(off, off);
+                const uint64_t scale2 = pair2(ref.factor, ref.factor), off2 = pair2(ref.off, ref.off);
                 uint64_t psum[2] = {0ull, 0ull};
                 auto exponents = [&](const uint32_t* v, uint32_t* pk) {
 #pragma unroll
@@ -479,7 +502,7 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
                 ++outs;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             }
-            float max2 = m_ref * to_log2;
+            float max2 = fmaxf(ref.log2_of(to_log2), kPgNone);
             float scale_a = 1.f, scale_b = 0.f;
             bool other = false;              // b's sums are to be added
             if (split && x == 1) {

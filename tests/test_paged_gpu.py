@@ -915,3 +915,69 @@ def test_mha_fp16_counts_keys_far_below_the_largest(new):
     others = n - 1 + 1.0 + torch.arange(new, dtype=torch.float64).repeat(148)[:, None, None]     # the token itself and those before it
     exact = others * w / (1.0 + others * w)
     _within(got, exact.expand_as(got), (20100 * 2.0 ** -32 + 2 * 2.0 ** -11 * exact + 2.0 ** -25).expand_as(got))
+
+
+@pytest.mark.parametrize("slopes,sign", [(False, 1), (True, 1), (False, -1)])
+@pytest.mark.parametrize("new,length", [(1, 300), (1, 6000), (5, 300), (200, 300), (200, 6000), (20, 300)])
+def test_mha_scores_far_below_zero(new, length, slopes, sign):
+    """All scores at -8e25, far within fp32: the mean of the values that a token sees.  All weights are the same number, so the result is
+    off by half a step of the probabilities and of its own, and by fp32 sums (2^-19)."""
+    batch = Batch([new], [length], 2, 1, 64, dtype=BF16)
+    batch.q[:] = 1e13
+    batch.k_cache[:] = -1e12 * sign
+    batch.poison()
+    got = _mha(batch, scale=sign / 8.0, alibi_slopes=torch.zeros(2) if slopes else None).double().cpu()
+    v = batch.history(batch.v_cache, 0).double()[:, 0]
+    seen = torch.arange(length - new, length)[:, None, None] + 1.0
+    mean, size = (x.cumsum(0)[length - new:, None] / seen for x in (v, v.abs()))
+    _within(got, mean.expand_as(got), (2 * 2.0 ** -8 * size + 2.0 ** -8 * mean.abs() + 2.0 ** -19).expand_as(got))
+    assert _status() == 0
+
+
+@pytest.mark.parametrize("slopes", [False, True])
+@pytest.mark.parametrize("new,length", [(1, 300), (5, 6000), (200, 300), (200, 6000), (20, 300)])
+@pytest.mark.parametrize("dtype,large", [(FP16, 20000.0), (BF16, 20000.0), (BF16, 1e8)])
+def test_mha_scores_far_above_zero(new, length, slopes, dtype, large):
+    """All scores 64 large^2 / 8, where one unit in the last place of fp32 is 2^8 and more: the mean of the values, as above."""
+    batch = Batch([new], [length], 2, 1, 64, dtype=dtype)
+    batch.q[:] = large
+    batch.k_cache[:] = large
+    batch.poison()
+    got = _mha(batch, alibi_slopes=torch.zeros(2) if slopes else None).double().cpu()
+    u, v = HALF_STEP[dtype], batch.history(batch.v_cache, 0).double()[:, 0]
+    seen = torch.arange(length - new, length)[:, None, None] + 1.0
+    mean, size = (x.cumsum(0)[length - new:, None] / seen for x in (v, v.abs()))
+    _within(got, mean.expand_as(got), (2 * u * size + u * mean.abs() + 2.0 ** -19).expand_as(got))
+    assert _status() == 0
+
+
+@pytest.mark.parametrize("new,length,slopes", [([1], 400, False), ([5], 5000, False), ([200], 1000, False), ([200], 1000, True),
+                                               ([30, 300], 3000, False)])
+@pytest.mark.parametrize("dtype,size", [(FP16, 100.0), (FP16, 3000.0), (BF16, 1e6), (BF16, 1e15)])
+def test_mha_of_large_scores_takes_the_largest(new, length, slopes, dtype, size):
+    """Scores of 10^4 to 10^30, both signs, some references near and some far: where the largest leads by more than what fp32 can lose of
+    both (D + 8 half steps of their sums of magnitudes each) and 40 units, its value alone is the result, to two roundings."""
+    heads = 4
+    batch = Batch(new, [length] * len(new), heads, 2, 64, dtype=dtype, q_scale=size)
+    batch.k_cache = (batch.k_cache * size).clamp(-6e4, 6e4) if dtype == FP16 else batch.k_cache * size
+    batch.q = batch.q.clamp(-6e4, 6e4) if dtype == FP16 else batch.q
+    batch.poison()
+    bias = torch.tensor([0.5, 0.25, 0.125, 0.0625]) if slopes else None
+    got = _mha(batch, alibi_slopes=bias).double().cpu()
+    at, rows = 0, 0
+    for b, t in enumerate(new):
+        k, v = (batch.history(c, b).double().repeat_interleave(2, 1).transpose(0, 1) for c in (batch.k_cache, batch.v_cache))
+        q = batch.q[at:at + t].double().transpose(0, 1)
+        s, lost = q @ k.transpose(1, 2) / 8.0, q.abs() @ k.abs().transpose(1, 2) / 8.0 * (64 + 8) * 2.0 ** -24
+        p, j = torch.arange(length - t, length)[:, None], torch.arange(length)[None, :]
+        if slopes:
+            s, lost = s + bias.double()[:, None, None] * (j - p), lost + bias.double()[:, None, None] * (p - j) * 2.0 ** -22
+        s, lost = s.masked_fill(j > p, -math.inf), lost.masked_fill(j > p, 0.0)
+        two = s.topk(2, -1).values
+        clear = two[..., 0] - two[..., 1] > 40 + 2 * lost.amax(-1)
+        want = torch.gather(v, 1, s.argmax(-1, keepdim=True).expand(-1, -1, 64))
+        off = (got[at:at + t].transpose(0, 1) - want).abs() - 2 * HALF_STEP[dtype] * want.abs() - 1e-7
+        assert not got[at:at + t].isnan().any() and (off[clear] <= 0).all()
+        rows += int(clear.sum())
+        at += t
+    assert rows >= 0.9 * sum(new) * heads and _status() == 0
