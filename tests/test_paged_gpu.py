@@ -981,3 +981,50 @@ def test_mha_of_large_scores_takes_the_largest(new, length, slopes, dtype, size)
         rows += int(clear.sum())
         at += t
     assert rows >= 0.9 * sum(new) * heads and _status() == 0
+
+
+def _scratch(batch, max_tokens, max_len, window=0):
+    """What the host plans: the scratch of the call, in bytes."""
+    from eet_b200._lib import lib
+    from test_paged_cpu import _mha as args
+    H, D = batch.q.shape[1:]
+    K, P = batch.k_cache.shape[1:3]
+    return lib.eet_paged_mha_workspace_bytes(args(
+        heads=H, kv_heads=K, head_dim=D, tokens=batch.q.shape[0], seqs=len(batch.new), page_size=P, max_pages=batch.pages.shape[1],
+        pages_stride=batch.pages.shape[1], num_pages=batch.k_cache.shape[0], max_tokens=max_tokens, max_len=max_len, window=window))
+
+
+def _scratch_of_both(head_dim):
+    """Two parts of 16 and of 256 rows - a maximum, a sum and head_dim values each - and a header, twice for every CTA."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    return sum(sms * (32 + 2 * 4 * rows * (2 + head_dim)) for rows in (16, 256))
+
+
+@pytest.mark.parametrize("page", [16, 32, 64])
+@pytest.mark.parametrize("dtype,head_dim", [(FP16, 64), (FP16, 128), (BF16, 64), (BF16, 128)])
+@pytest.mark.parametrize("kind", ["plain", "slopes", "negative scale", "whole"])
+def test_mha_both_kernels_with_every_kind_of_scores(kind, dtype, head_dim, page):
+    """A chunk and an empty sequence among 40 single tokens behind histories of up to 900, where the plan has few-row CTAs and tiles in one
+    launch: tiles of both kinds cut, or ("whole", behind a window) neither, then without a second launch."""
+    from eet_b200.EET import alibi_slopes
+    new = [1] * 15 + [200, 0] + [1] * 25
+    lens = [800 + 5 * i % 100 if n else 77 for i, n in enumerate(new)]
+    heads, kv_heads = ((12, 6), (8, 8))[page % 3 % 2]
+    batch = Batch(new, lens, heads, kv_heads, head_dim, page, dtype, seed=page, behind=2)
+    slopes = torch.tensor(alibi_slopes(heads), dtype=torch.float32)
+    kw = {"plain": {}, "slopes": dict(alibi_slopes=slopes, first_key=torch.arange(42, dtype=torch.int32) * 7),
+          "negative scale": dict(scale=-0.1), "whole": dict(alibi_slopes=slopes, window=100)}[kind]
+    both = _scratch_of_both(head_dim)
+    assert _scratch(batch, 200, max(lens), kw.get("window", 0)) == (0 if kind == "whole" else both)
+    if kind == "whole":   # beside a plan that cuts, for the same sizes: both kinds are there
+        assert _scratch(batch, 200, max(lens)) == both
+    _check(batch, **kw)
+
+
+def test_mha_both_kernels_where_there_is_work_for_one_only():
+    """The plan goes by the hints; what the sequences turn out to be may leave either kind without work."""
+    for new in ([1] * 41, [0] * 10 + [3] + [0] * 30, [30] * 3 + [0] * 38, [0] * 40 + [200], [0] * 41):
+        batch = Batch(new, [900 - i for i in range(41)], 8, 8, 128, 32, behind=40)
+        assert _scratch(batch, 200, 900) == _scratch_of_both(128)
+        for kw in ({}, {"alibi_slopes": torch.full((8,), 0.1)}):
+            _check(batch, hints=False, max_tokens=200, max_len=900, **kw)
