@@ -1028,3 +1028,42 @@ def test_mha_both_kernels_where_there_is_work_for_one_only():
         assert _scratch(batch, 200, 900) == _scratch_of_both(128)
         for kw in ({}, {"alibi_slopes": torch.full((8,), 0.1)}):
             _check(batch, hints=False, max_tokens=200, max_len=900, **kw)
+
+
+@pytest.mark.parametrize("new", [[200] + [1] * 40, [24] + [1] * 40, [1] * 40])
+@pytest.mark.parametrize("window", [0, 100])
+def test_block_over_both_kernels_and_projections_without_a_pause(new, window):
+    """The projections take tensor memory while the attention in front of them runs, and the other way round: thirty blocks behind one
+    another against one call at a time.
+
+    Rotation, append and attention give the same bits, as does the projection in front of them.  That behind adds 1024 products in any
+    order (2^-24 of their magnitudes each time, on either side) and rounds the sum and its sum with the residual (half a step each)."""
+    heads, kv_heads, hidden = 8, 8, 256
+    from eet_b200 import EET
+    gen = torch.Generator().manual_seed(0)
+    desc = EET.MetaDesc(FP16, 4, heads, hidden, 1, 128, 512, d_kv=128, is_int8=True)
+    qkv, out = (EET.quant_weights((torch.randn(*s, generator=gen) / 16).half()) for s in ((hidden, 3 * 1024), (1024, hidden)))
+    norm = torch.ones(hidden, dtype=FP16).cuda()
+    block = _paged().PagedMmha(desc, qkv[0].cuda(), qkv[1].cuda(), out[0].cuda(), out[1].cuda(), norm)
+    batch = Batch(new, [900 - i for i in range(len(new))], heads, kv_heads)
+    kc, vc, *table = _gpu(batch)
+    x = torch.randn(sum(new), hidden, generator=gen).half().cuda()
+    kw = dict(max_tokens=max(new), max_len=900, window=window)
+    xn = EET.LayerNorm(desc, norm, torch.empty(0)).layer_norm(x.view(1, -1, hidden)).view(-1, hidden).clone()
+    rows = EET.gemm_w8a16(xn, qkv[0].cuda(), qkv[1].cuda()).view(-1, 3 * heads, 128).clone()
+    torch.cuda.synchronize()
+    q = _paged().paged_store(rows[:, 8:16], rows[:, 16:], kc, vc, *table, q=rows[:, :8], freqs=block.freqs)
+    torch.cuda.synchronize()
+    ctx = _paged().paged_mha(q, kc, vc, *table, **kw)
+    torch.cuda.synchronize()
+    want = EET.gemm_w8a16(ctx.view(-1, 1024), out[0].cuda(), out[1].cuda(), residual=x).clone()
+    torch.cuda.synchronize()
+    weights = EET.unpack_weights(out[0]).double().cuda() * out[1].double().cuda()
+    ctx, want = ctx.view(-1, 1024).double(), want.double()
+    tol = 2 * 1024 * 2.0 ** -24 * (ctx.abs() @ weights.abs()) + 2 * 2.0 ** -11 * ((ctx @ weights).abs() + want.abs())
+    stored = kc.clone(), vc.clone()
+    got = [block(x, kc, vc, *table, **kw).clone() for _ in range(30)]
+    for y in got:
+        _within(y, want.cpu(), tol.cpu())
+    assert torch.equal(kc, stored[0]) and torch.equal(vc, stored[1])
+    assert _status() == 0
