@@ -495,8 +495,12 @@ paged_mha_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
 
 // Both kinds of work in one launch: sequences of up to `few` new tokens for the first CTAs, the others for the rest, as many as their blocks
 // take of the time.  Measured, a block on one CTA (heads of 128): few rows 1.46 us with pages of 16 (32 copies of 2 KB), 0.85 with pages of
-// 64 and more; tiles 1.9 us, with a bias 3 to 3.5.  All CTAs together get a block of the first kind every 0.0106 us from HBM: more of them
-// than use that up are better spent on the tiles.
+// 64 and more; tiles 1.9 us, with a bias and masks 3 to 3.5.  All CTAs together get a block of the first kind every 0.0106 us from HBM: more
+// of them than use that up are better spent on the tiles.  The other constants below are estimates, and close: measured afterwards, 148
+// histories in the same pages (so from L2), us a block and CTA
+//   few rows, pages of 16 / 32 / 64 and more   heads of 128: 1.50 / 1.01 / 0.86     heads of 64: 1.00 / 0.83 / 0.84
+//   tiles that need no masks, without / with a bias   heads of 128: 1.76 / 2.44     heads of 64: 1.68 / 2.43
+// and with pages of their own, from HBM, 1.43 for heads of 128 (one every 0.0097 us) and 0.84, not bound by HBM, for heads of 64.
 // (As two launches one chunk of 777 tokens beside 23 single ones, 40 heads, took 65 + 49 us, with HBM idle in the second.)
 template<int D>
 __device__ __forceinline__ int pg_divide(int ctas, float in_rows, float in_tiles, int page_shift, bool bias)

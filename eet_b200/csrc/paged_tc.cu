@@ -13,8 +13,8 @@
 // Bound: the softmax.  A block of both tiles takes 3200 cycles where the tensor core and the exponential unit need 2048 each: P lies over S
 // and tensor memory is full, so the next Q.K^T follows P.V, and a warp waits 1300 cycles for it after 1900 of its own.  P.V begins with the
 // first half of P, the reference under which O is accumulated moves in steps of 2^8 only, and code that runs with few registers beat
-// everything that did not (1024 tokens behind 24000, 64 / 8 heads, bf16: 775 us = 1.06 PF/s among other calls at the power cap, 711 alone;
-// 512 behind 8192, 32 / 8 heads: 87 us).
+// everything that did not (1024 tokens behind 24000, 64 / 8 heads, bf16: 788 us = 1.04 PF/s among other calls at the power cap, 711 alone;
+// 512 behind 8192, 32 / 8 heads: 87 us).  168 registers; 8 bytes of spills with a bias, in the kernel of both kinds of CTAs 8 without and 24 with it.
 //
 //   warps 0-3, 4-7  softmax of tile a / b: one thread per row = TMEM lane
 //   warp 8          producer: Q, then K and V blocks through a ring of five 32 KiB stages (order K0 K1 V0 K2 V1 ...), a lane

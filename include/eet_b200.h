@@ -336,7 +336,8 @@ int eet_gather_rows(const void* table, const int64_t* ids, void* out, int rows, 
  * head_dim.  Sequence b holds lens[b] positions; position p of it is slot p % page_size of page pages[b][p / page_size].
  * The new tokens of all sequences are rows behind one another, those of sequence b the rows [starts[b], starts[b + 1]), and
  * they are the last positions of their sequence: row starts[b] + i is position lens[b] - (starts[b + 1] - starts[b]) + i.
- * Rows that belong to no sequence and positions below zero are left alone (paged_mha: zeros for positions below zero).
+ * Rows that belong to no sequence are left alone.  A row at a position below zero (more new tokens than positions) is appended to no
+ * page, its q is rotated by that position, and paged_mha gives it zeros.
  * starts, lens and pages are read on the device, so that a captured graph serves other lengths when it is replayed; a page
  * outside the cache is not touched and recorded as status 6 (paged_mha: its keys count as zeros).
  * The reference has contiguous caches [batch][head][time][dim] with all sequences at the same step (csrc/op/llama_mmha.cpp:
