@@ -319,6 +319,17 @@ class PagedMmha:
             if tuple(t.shape) != shape or t.dtype != desc.weight_dtype or not t.is_cuda or not t.is_contiguous():
                 raise RuntimeError(f"PagedMmha: {what} must be a contiguous CUDA {desc.weight_dtype} tensor of shape {shape}, got "
                                    f"{tuple(t.shape)} {t.dtype}")
+        vectors = [(layernorm_weights, desc.hidden_units, "layernorm_weights")]
+        if desc.is_int8:
+            vectors += [(QKV_scale, self.qkv_dim, "QKV_scale"), (Output_scale, desc.hidden_units, "Output_scale")]
+        self.index = QKV_weights.get_device()
+        for t, numel, what in vectors:
+            if not torch.is_tensor(t) or t.numel() != numel or t.dtype != torch.float16 or t.get_device() != self.index or \
+                    not t.is_contiguous():
+                raise RuntimeError(f"PagedMmha: {what} must be a contiguous fp16 tensor of {numel} values on cuda:{self.index}, got " +
+                                   (f"{tuple(t.shape)} {t.dtype} on {t.device}" if torch.is_tensor(t) else repr(t)))
+        if Output_weights.get_device() != self.index:
+            raise RuntimeError("PagedMmha: QKV_weights and Output_weights are on different devices")
         self.qkv_w, self.qkv_s, self.out_w, self.out_s, self.ln_w = QKV_weights, QKV_scale, Output_weights, Output_scale, layernorm_weights
         if alibi_slopes is not None and freqs is not None:
             raise RuntimeError("PagedMmha: rotary positions and ALiBi exclude each other")
@@ -329,9 +340,9 @@ class PagedMmha:
     def forward(self, input, k_cache, v_cache, pages, starts, lens, max_tokens=None, max_len=None, window=0, first_key=None):
         """input fp16 [tokens, hidden]: the new tokens of all sequences behind one another; the other arguments as in paged_mha."""
         d = self.desc
-        if input.dtype != torch.float16 or not input.is_cuda or input.dim() != 2 or input.shape[1] != d.hidden_units or \
+        if input.dtype != torch.float16 or input.get_device() != self.index or input.dim() != 2 or input.shape[1] != d.hidden_units or \
                 not input.is_contiguous():
-            raise RuntimeError("PagedMmha: input must be a contiguous CUDA fp16 tensor [tokens, hidden]")
+            raise RuntimeError(f"PagedMmha: input must be a contiguous fp16 tensor [tokens, hidden] on cuda:{self.index}")
         n, cap = input.shape[0], d.batch_size * d.max_seq_len
         if n > cap:
             raise RuntimeError(f"PagedMmha: {n} tokens, MetaDesc allows {cap}")

@@ -1067,3 +1067,13 @@ def test_block_over_both_kernels_and_projections_without_a_pause(new, window):
         _within(y, want.cpu(), tol.cpu())
     assert torch.equal(kc, stored[0]) and torch.equal(vc, stored[1])
     assert _status() == 0
+
+
+@pytest.mark.parametrize("which", ["QKV_scale", "Output_scale", "layernorm_weights"])
+def test_block_refuses_scales_and_norms_that_the_kernels_would_read_past(which):
+    block, args = _block(4, 2, 256, True)
+    at = {"QKV_scale": 1, "Output_scale": 3, "layernorm_weights": 4}[which]
+    good = args[at]
+    for bad in (good[:-1].contiguous(), good[::2], good.float(), good.cpu(), None, torch.empty(0)):
+        with pytest.raises(RuntimeError, match=which):
+            _paged().PagedMmha(block.desc, *args[:at], bad, *args[at + 1:], kv_head_num=2)
