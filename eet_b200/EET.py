@@ -348,6 +348,11 @@ def _linear(x, w, scale, out, residual=None):
     return out
 
 
+def _apart(residual, out):
+    """The residual where writing to `out` leaves it as it is: an op's input may lie in its output's buffer."""
+    return residual.clone() if residual.data_ptr() == out.data_ptr() else residual
+
+
 def gemm_w8a16_accum(x, packed_w, sums, packed_w2=None, sums2=None):
     """sums[M, N] += x[M, K] @ q (unscaled int8 values); optionally the same for a second weight in the same
     launch.  The decode-regime half of gemm_w8a16: whoever reads `sums` applies scale / residual."""
@@ -641,6 +646,7 @@ class _MmhaBase:
         elif d.tp is None or d.tp.size == 1:
             _linear(ctx2d, self.out_w, self.out_s, out, residual=inp2d)
         else:
+            inp2d = _apart(inp2d, out)
             _linear(ctx2d, self.out_w, self.out_s, out)
             d.tp.all_reduce(out)
             check(lib.eet_add_residual(out.data_ptr(), inp2d.data_ptr(), out.numel(), _stream()))
@@ -905,6 +911,7 @@ class GatedFeedForwardNetworkInt8:
             elif d.tp is None or d.tp.size == 1:
                 _linear(act, self.w_out, self.s_out, out, residual=inp2d if add_residual else None)
             else:
+                inp2d = _apart(inp2d, out)
                 _linear(act, self.w_out, self.s_out, out)
                 d.tp.all_reduce(out)
                 if add_residual:

@@ -142,3 +142,35 @@ def test_two_gpu_fused_exchange_above_16_rows():
     """Batch 32 (the Baichuan-13B decode batch): the fused exchange with more than 16 rows per inbox, fed by the
     stream-K tensor-core GEMM instead of the skinny one, and the sharded lm_head's greedy kernel with 32 rows."""
     _run(2, small=False, batch=32)
+
+
+@pytest.mark.parametrize("rows,is_int8", [(3, True), (100, True), (3, False), (100, False)])
+def test_an_op_whose_input_lies_in_the_buffer_of_its_output(rows, is_int8):
+    """Two ops of one kind behind one another, as the first of two ranks whose other's partial sums are zero: the residual is what the
+    input was when the op began, not its own partial sums.  From the same input both ways: the projections may add in another order, so
+    the rounded partial sums (below 4 here) and their sums with the residual may each be one half step apart."""
+    import types
+    from eet_b200 import EET
+    hidden, none = 256, torch.empty(0)
+    gen = torch.Generator().manual_seed(rows)
+    tp = types.SimpleNamespace(size=2, rank=0, all_reduce=lambda t: t)
+    desc = EET.MetaDesc(torch.float16, 1, 2, hidden, 1, 128, 256, "silu", 128, 512, is_int8=is_int8, tp=tp)
+
+    def weight(K, N):
+        w = (torch.randn(K, N, generator=gen) * K ** -0.5).half()
+        return [t.cuda() for t in EET.quant_weights(w)] if is_int8 else [w.cuda(), None]
+    norm = torch.ones(hidden, dtype=torch.float16, device="cuda")
+    att = EET.LlamaMmha(desc, *weight(hidden, 3 * hidden), none, none, none, *weight(hidden, hidden), none, norm, none)
+    w0, w1, w2 = weight(hidden, 512), weight(hidden, 512), weight(512, hidden)
+    if is_int8:
+        ffn = EET.GatedFeedForwardNetworkInt8(desc, *w0, none, *w1, none, *w2, none, norm, none)
+    else:
+        ffn = EET.GatedFeedForwardNetwork(desc, w0[0], none, w1[0], none, w2[0], none, norm, none)
+    x = torch.randn(1, rows, hidden, generator=gen).half().cuda()
+    for op in (lambda y: att(y, none, none, True, True, True), lambda y: ffn(y, True, True)):
+        y = op(x).clone()
+        want = op(y).clone()
+        place = op(x)
+        got = op(place.copy_(y))
+        assert got.data_ptr() == place.data_ptr()
+        assert torch.allclose(got, want, rtol=2.0 ** -9, atol=2.0 ** -8)
