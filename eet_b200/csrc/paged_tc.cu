@@ -14,7 +14,8 @@
 // and tensor memory is full, so the next Q.K^T follows P.V, and a warp waits 1300 cycles for it after 1900 of its own.  P.V begins with the
 // first half of P, the reference under which O is accumulated moves in steps of 2^8 only, and code that runs with few registers beat
 // everything that did not (1024 tokens behind 24000, 64 / 8 heads, bf16: 788 us = 1.04 PF/s among other calls at the power cap, 711 alone;
-// 512 behind 8192, 32 / 8 heads: 87 us).  168 registers; 8 bytes of spills with a bias, in the kernel of both kinds of CTAs 8 without and 24 with it.
+// 512 behind 8192, 32 / 8 heads: 87 us).  168 registers; 8 bytes of spills with a bias, in the kernel of both kinds of CTAs 8 without and 24
+// with it.
 //
 //   warps 0-3, 4-7  softmax of tile a / b: one thread per row = TMEM lane
 //   warp 8          producer: Q, then K and V blocks through a ring of five 32 KiB stages (order K0 K1 V0 K2 V1 ...), a lane
@@ -65,8 +66,8 @@ __device__ __forceinline__ void tmem_st16_async(uint32_t taddr, const uint32_t (
 // The reference of a row: the power of a score s is 2^(s factor + off).  factor is log2(e) (and the scale, where scores are taken before it)
 // and off the reference times that, rounded to 24 bits: what of it is lost is a factor of all of the row's powers, and would be 2^512 at
 // scores of 10^10.  So from 2^24 on, where a unit in the last place of a score is a factor of 4 and more and a sum of products does not
-// hold so much, factor is the power of two below and off exact: equal scores weigh the same, a larger one hides the others.  (Subtracting
-// the reference from the scores first takes 2.5 % of a chunk, 4.5 with a bias.)
+// hold so much, factor is the power of two below and off exact: equal scores weigh the same, one that leads by more than that hides the
+// others.  (Subtracting the reference from the scores first takes 2.5 % of a chunk, 4.5 with a bias.)
 struct PgReference {
     float factor, off;
     // what the sums under it are to be multiplied with, as a power of two

@@ -213,8 +213,8 @@ def paged_store(k, v, k_cache, v_cache, pages, starts, lens, q=None, freqs=None,
     [tokens, heads, head_dim] rotated the same way (in q_out; a new tensor unless given, q_out=q works in place; None without q).
 
     The positions of the rotation are those in the sequence, or positions int64 [tokens].  Rows of k, v and q that belong to no
-    sequence are not touched; of rows in front of a sequence's first position only q is.  Two sequences must not append to the same slot (one that they share must lie before both's new
-    tokens)."""
+    sequence are not touched; of rows in front of a sequence's first position only q is.  Two sequences must not append to the same
+    slot (one that they share must lie before both's new tokens)."""
     who = "paged_store"
     shape, dtype, index, k_str = _first(who, "k", k)
     tokens, kv_heads, head_dim = shape
