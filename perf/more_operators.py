@@ -180,7 +180,7 @@ def _prepare_sample(case, gen):
     # what a language model says: most tokens far below a handful of likely ones, some rows surer than others
     x = 2.0 * torch.randn(rows, vocab, generator=gen, device="cuda")
     sure = 0.7 + torch.rand(rows, 1, generator=gen, device="cuda")
-    place = torch.randint(0, vocab, (rows, 60), generator=gen, device="cuda")
+    place = (torch.randint(0, vocab, (rows, 1), generator=gen, device="cuda") + 7 * torch.arange(60, device="cuda")) % vocab
     likely = 6.0 + 2.5 * torch.empty(rows, 60, device="cuda").exponential_(generator=gen)
     x = x.scatter(1, place, likely) * sure
     if case["banned"]:
@@ -258,8 +258,8 @@ def _rotated(x, positions, freqs, interleaved):
 def _plain_quantize(y, codes):
     dtype, most = CODES[codes]
     top = y.abs().amax(-1)
-    scale = torch.where(top > 0, top / most, torch.ones_like(top))
     # (in 64 bits: 16-bit values over a scale made from one of them often lie on the border of two codes, or next to it)
+    scale = torch.where(top > 0, top.double() / most, torch.ones_like(top)).float()
     z = (y.double() / scale[..., None].double()).clamp(-most, most)
     # the distance of two codes: 1, in e4m3 of three bits behind the leading one, down to 2^-6
     step = 1.0 if codes == "int8" else torch.ldexp(torch.ones_like(z), (torch.frexp(z).exponent - 4).clamp(min=-9))
