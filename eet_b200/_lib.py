@@ -51,6 +51,10 @@ SIGNATURES = {
     "eet_paged_store": (_i, [_vp, _vp]),
     "eet_paged_mha_workspace_bytes": (_sz, [_vp]),
     "eet_paged_mha": (_i, [_vp, _vp]),
+    "eet_paged_store_codes": (_i, [_vp, _vp]),
+    "eet_paged_load": (_i, [_vp, _vp]),
+    "eet_paged_mha_codes_workspace_bytes": (_sz, [_vp]),
+    "eet_paged_mha_codes": (_i, [_vp, _vp]),
     "eet_gather_rows": (_i, [_vp, _vp, _vp, _i, _i, _c.c_int64, _vp]),
 }
 

@@ -58,6 +58,7 @@ static inline bool aligned16(const void* p)
 #include "paged_tc.cu"
 #include "paged_rows.cu"
 #include "paged.cu"
+#include "paged_codes.cu"
 #include "quantize.cu"
 
 using namespace eet;
@@ -654,7 +655,7 @@ int eet_rotary(const eet_rotary_args* p, void* stream)
     return launch_rotary(a, false, (cudaStream_t)stream);
 }
 
-int eet_paged_store(const eet_paged_store_args* p, void* stream)
+static int paged_store_args(const eet_paged_store_args* p, RotaryArgs& a)
 {
     EET_CHECK(p != nullptr, "eet_paged_store: args is NULL");
     if (int rc = check_paged("eet_paged_store", p->tokens, p->seqs, p->heads, p->kv_heads, p->head_dim, p->num_pages, p->page_size,
@@ -669,7 +670,6 @@ int eet_paged_store(const eet_paged_store_args* p, void* stream)
     EET_CHECK(multiples_of_8({p->q_tok, p->q_head, p->k_tok, p->k_head, p->v_tok, p->v_head, p->qo_tok, p->qo_head, p->kc_page, p->kc_head,
                               p->kc_slot, p->vc_page, p->vc_head, p->vc_slot}),
               "eet_paged_store: strides must be multiples of 8 elements");
-    RotaryArgs a = {};
     a.q = p->q, a.k = p->k, a.v = p->v, a.q_out = p->q_out, a.k_cache = p->k_cache, a.v_cache = p->v_cache;
     a.pages = p->pages, a.starts = p->starts, a.lens = p->lens, a.positions = p->positions, a.freqs = p->freqs;
     a.tokens = (int)p->tokens, a.seqs = (int)p->seqs, a.heads = (int)p->heads, a.kv_heads = (int)p->kv_heads;
@@ -681,7 +681,67 @@ int eet_paged_store(const eet_paged_store_args* p, void* stream)
     a.kc_page = p->kc_page, a.kc_head = p->kc_head, a.kc_slot = p->kc_slot;
     a.vc_page = p->vc_page, a.vc_head = p->vc_head, a.vc_slot = p->vc_slot;
     a.magnitude = (float)p->magnitude;
+    return 0;
+}
+
+int eet_paged_store(const eet_paged_store_args* p, void* stream)
+{
+    RotaryArgs a = {};
+    if (int rc = paged_store_args(p, a)) return rc;
     return launch_rotary(a, true, (cudaStream_t)stream);
+}
+
+// The codes of a cache and their scales, for a call that is not empty.
+static int check_codes(const char* who, int64_t codes, const void* k_scale, const void* v_scale, std::initializer_list<int64_t> code_strides)
+{
+    EET_CHECK(codes == kCodesInt8 || codes == kCodesE4M3, "%s: unknown kind of codes %lld", who, (long long)codes);
+    EET_CHECK(k_scale && v_scale, "%s: NULL scales", who);
+    EET_CHECK(((uintptr_t)k_scale & 3) == 0 && ((uintptr_t)v_scale & 3) == 0, "%s: scales must be 4-byte aligned", who);
+    for (int64_t s : code_strides) EET_CHECK(s % 16 == 0, "%s: strides of codes must be multiples of 16", who);
+    return 0;
+}
+
+int eet_paged_store_codes(const eet_paged_store_codes_args* p, void* stream)
+{
+    RotaryArgs a = {};
+    EET_CHECK(p != nullptr, "eet_paged_store_codes: args is NULL");
+    if (int rc = paged_store_args(&p->store, a)) return rc;
+    if (a.tokens == 0 || a.seqs == 0) return 0;
+    if (int rc = check_codes("eet_paged_store_codes", p->codes, p->k_scale, p->v_scale,
+                             {a.kc_page, a.kc_head, a.kc_slot, a.vc_page, a.vc_head, a.vc_slot})) return rc;
+    a.codes = (int)p->codes, a.k_scale = p->k_scale, a.v_scale = p->v_scale;
+    a.ks_page = p->ks_page, a.ks_head = p->ks_head, a.vs_page = p->vs_page, a.vs_head = p->vs_head;
+    return launch_rotary(a, true, (cudaStream_t)stream);
+}
+
+int eet_paged_load(const eet_paged_load_args* p, void* stream)
+{
+    EET_CHECK(p != nullptr, "eet_paged_load: args is NULL");
+    if (int rc = check_paged("eet_paged_load", p->tokens, p->seqs, 0, p->kv_heads, p->head_dim, p->num_pages, p->page_size,
+                             p->max_pages, p->pages_stride)) return rc;
+    EET_CHECK(p->codes >= 0 && p->codes <= kCodesE4M3, "eet_paged_load: unknown kind of codes %lld", (long long)p->codes);
+    if (p->tokens == 0 || p->seqs == 0) return 0;
+    EET_CHECK(p->k_cache && p->v_cache && p->k_out && p->v_out && p->pages && p->starts && p->lens, "eet_paged_load: NULL argument");
+    EET_CHECK(all_aligned16({p->k_cache, p->v_cache, p->k_out, p->v_out}), "eet_paged_load: pointers must be 16-byte aligned");
+    EET_CHECK(multiples_of_8({p->ko_tok, p->ko_head, p->vo_tok, p->vo_head, p->kc_page, p->kc_head, p->kc_slot, p->vc_page, p->vc_head,
+                              p->vc_slot}),
+              "eet_paged_load: strides must be multiples of 8 elements");
+    if (p->codes != 0) {
+        if (int rc = check_codes("eet_paged_load", p->codes, p->k_scale, p->v_scale,
+                                 {p->kc_page, p->kc_head, p->kc_slot, p->vc_page, p->vc_head, p->vc_slot})) return rc;
+    }
+    PagedLoadArgs a = {};
+    a.k_cache = p->k_cache, a.v_cache = p->v_cache, a.k_scale = p->k_scale, a.v_scale = p->v_scale, a.k_out = p->k_out, a.v_out = p->v_out;
+    a.pages = p->pages, a.starts = p->starts, a.lens = p->lens;
+    a.tokens = (int)p->tokens, a.seqs = (int)p->seqs, a.kv_heads = (int)p->kv_heads, a.head_dim = (int)p->head_dim;
+    a.codes = (int)p->codes, a.bf16 = p->bf16 != 0;
+    a.num_pages = (int)p->num_pages, a.page_shift = page_shift(p->page_size), a.max_pages = (int)p->max_pages;
+    a.pages_stride = p->pages_stride;
+    a.ko_tok = p->ko_tok, a.ko_head = p->ko_head, a.vo_tok = p->vo_tok, a.vo_head = p->vo_head;
+    a.kc_page = p->kc_page, a.kc_head = p->kc_head, a.kc_slot = p->kc_slot;
+    a.vc_page = p->vc_page, a.vc_head = p->vc_head, a.vc_slot = p->vc_slot;
+    a.ks_page = p->ks_page, a.ks_head = p->ks_head, a.vs_page = p->vs_page, a.vs_head = p->vs_head;
+    return launch_paged_load(a, (cudaStream_t)stream);
 }
 
 static int paged_mha_args(const eet_paged_mha_args* p, PagedMhaArgs& a)
@@ -730,6 +790,40 @@ int eet_paged_mha(const eet_paged_mha_args* p, void* stream)
     EET_CHECK(a.ws_bytes >= paged_mha_workspace_bytes(a) && (a.ws != nullptr || paged_mha_workspace_bytes(a) == 0),
               "eet_paged_mha: workspace too small");
     return launch_paged_mha(a, (cudaStream_t)stream);
+}
+
+static int paged_mha_codes_args(const eet_paged_mha_codes_args* p, PagedMhaArgs& a)
+{
+    EET_CHECK(p != nullptr, "eet_paged_mha_codes: args is NULL");
+    if (int rc = paged_mha_args(&p->mha, a)) return rc;
+    EET_CHECK(p->codes == kCodesInt8 || p->codes == kCodesE4M3, "eet_paged_mha_codes: unknown kind of codes %lld", (long long)p->codes);
+    a.codes = (int)p->codes, a.k_scale = p->k_scale, a.v_scale = p->v_scale;
+    a.ks_page = p->ks_page, a.ks_head = p->ks_head, a.vs_page = p->vs_page, a.vs_head = p->vs_head;
+    return 0;
+}
+
+size_t eet_paged_mha_codes_workspace_bytes(const eet_paged_mha_codes_args* args)
+{
+    PagedMhaArgs a = {};
+    if (paged_mha_codes_args(args, a) || a.tokens == 0 || a.seqs == 0) return 0;
+    return paged_mha_codes_workspace_bytes(a);
+}
+
+int eet_paged_mha_codes(const eet_paged_mha_codes_args* p, void* stream)
+{
+    PagedMhaArgs a = {};
+    if (int rc = paged_mha_codes_args(p, a)) return rc;
+    if (a.tokens == 0 || a.seqs == 0) return 0;
+    const eet_paged_mha_args& m = p->mha;
+    EET_CHECK(m.q && m.k_cache && m.v_cache && m.out && m.pages && m.starts && m.lens, "eet_paged_mha_codes: NULL argument");
+    EET_CHECK(all_aligned16({m.q, m.k_cache, m.v_cache, m.out, m.ws}), "eet_paged_mha_codes: pointers must be 16-byte aligned");
+    if (int rc = check_codes("eet_paged_mha_codes", p->codes, p->k_scale, p->v_scale,
+                             {m.kc_page, m.kc_head, m.kc_slot, m.vc_page, m.vc_head, m.vc_slot})) return rc;
+    a.ws = m.ws;
+    a.ws_bytes = m.ws_bytes > 0 ? (size_t)m.ws_bytes : 0;
+    EET_CHECK(a.ws_bytes >= paged_mha_codes_workspace_bytes(a) && (a.ws != nullptr || paged_mha_codes_workspace_bytes(a) == 0),
+              "eet_paged_mha_codes: workspace too small");
+    return launch_paged_mha_codes(a, (cudaStream_t)stream);
 }
 
 }  // extern "C"

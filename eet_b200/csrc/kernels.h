@@ -159,8 +159,26 @@ struct RotaryArgs {
     long long q_tok, q_head, k_tok, k_head, v_tok, v_head, qo_tok, qo_head, ko_tok, ko_head;
     long long kc_page, kc_head, kc_slot, vc_page, vc_head, vc_slot;
     float magnitude;
+    // caches of 8-bit codes
+    int codes;                                   // PagedCodes
+    float *k_scale, *v_scale;
+    long long ks_page, ks_head, vs_page, vs_head;
 };
+enum PagedCodes { kCodesNone = 0, kCodesInt8 = 1, kCodesE4M3 = 2 };
 int launch_rotary(const RotaryArgs& a, bool store, cudaStream_t stream);
+struct PagedLoadArgs {
+    const void *k_cache, *v_cache;
+    const float *k_scale, *v_scale;
+    void *k_out, *v_out;
+    const int *pages, *starts, *lens;
+    int tokens, seqs, kv_heads, head_dim, codes, bf16;
+    int num_pages, page_shift, max_pages;
+    long long pages_stride;
+    long long ko_tok, ko_head, vo_tok, vo_head;
+    long long kc_page, kc_head, kc_slot, vc_page, vc_head, vc_slot;
+    long long ks_page, ks_head, vs_page, vs_head;
+};
+int launch_paged_load(const PagedLoadArgs& a, cudaStream_t stream);
 struct PagedMhaArgs {
     const void *q, *k_cache, *v_cache;
     void* out;
@@ -176,8 +194,14 @@ struct PagedMhaArgs {
     float scale;
     void* ws;
     size_t ws_bytes;
+    // caches of 8-bit codes
+    int codes;                                   // PagedCodes
+    const float *k_scale, *v_scale;
+    long long ks_page, ks_head, vs_page, vs_head;
 };
 size_t paged_mha_workspace_bytes(const PagedMhaArgs& a);
 int launch_paged_mha(const PagedMhaArgs& a, cudaStream_t stream);
+size_t paged_mha_codes_workspace_bytes(const PagedMhaArgs& a);
+int launch_paged_mha_codes(const PagedMhaArgs& a, cudaStream_t stream);
 
 }  // namespace eet

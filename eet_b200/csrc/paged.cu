@@ -5,7 +5,12 @@
 // there and only then rounded to 32 bits: at position 10^6 a 32-bit product would be off by 0.06 radians.  sincospif of the
 // rest is good to 2 ulp.
 //
+// Into a cache of 8-bit codes a row of k or v goes as code = y / s, rounded to int8 or e4m3, with the scale s = max |y| / 127 or / 448
+// beside it; y is what the 16-bit cache would be rounded from, so that k is rounded once.  The lanes that hold a row's 16-dim items are
+// neighbours, its maximum takes two or three shuffles.
+//
 // Bound: HBM for prompts, launch latency for decode steps.
+#include "codes.cuh"
 #include "common.cuh"
 #include "kernels.h"
 
@@ -32,9 +37,10 @@ struct Pair2<__nv_bfloat16> {
 };
 
 // kStore: the keys go to their pages and the values with them, the position follows from the lengths unless it is given.
+// kCodes: the pages hold 8-bit codes.
 // An item is 16 dims of a head: with the half layout dims 8c .. 8c+7 and the partners half the rotated part further, with the
 // interleaved layout and in the part that is not rotated dims 16c .. 16c+15.
-template<typename T, bool kStore>
+template<typename T, bool kStore, int kCodes>
 __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryArgs a)
 {
     using P2 = Pair2<T>;
@@ -45,8 +51,10 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryArgs a)
     const int tid = threadIdx.x;
     const int pairs = a.rotary_dim >> 1;
     long long pos = 0;
-    T* kdst = nullptr;
-    T* vdst = nullptr;
+    using C = typename PagedCode<T, kCodes>::type;   // what the pages hold
+    C* kdst = nullptr;
+    C* vdst = nullptr;
+    float *kscale = nullptr, *vscale = nullptr;
     pdl_launch_dependents();
     pdl_wait();
 
@@ -87,8 +95,12 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryArgs a)
             const int page = column < a.max_pages ? a.pages[seq * a.pages_stride + column] : -1;
             if (page >= 0 && page < a.num_pages) {
                 const long long slot = pos & ((1 << a.page_shift) - 1);
-                kdst = (T*)a.k_cache + page * a.kc_page + slot * a.kc_slot;
-                vdst = (T*)a.v_cache + page * a.vc_page + slot * a.vc_slot;
+                kdst = (C*)a.k_cache + page * a.kc_page + slot * a.kc_slot;
+                vdst = (C*)a.v_cache + page * a.vc_page + slot * a.vc_slot;
+                if (kCodes) {
+                    kscale = a.k_scale + page * a.ks_page + slot;
+                    vscale = a.v_scale + page * a.vs_page + slot;
+                }
             }
             else if (tid == 0) {
                 g_device_status = 6;
@@ -104,17 +116,62 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryArgs a)
     }
     __syncthreads();
 
+    // a row of k or v as codes: this thread's 16 dims of it
+    auto store_codes = [&](int row, uint4 u, uint4 w) {
+        const bool is_k = row < a.heads + a.kv_heads;
+        const int head = row - a.heads - (is_k ? 0 : a.kv_heads);
+        if ((is_k ? kdst : vdst) == nullptr) return;   // (of the whole token)
+        float y[16];
+        const V2* xh = reinterpret_cast<const V2*>(&u);
+        const V2* yh = reinterpret_cast<const V2*>(&w);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float2 f = P2::up(xh[e]), g = P2::up(yh[e]);
+            y[2 * e] = f.x, y[2 * e + 1] = f.y, y[8 + 2 * e] = g.x, y[9 + 2 * e] = g.y;
+        }
+        auto turn = [&](float& f, float& g, float2 t) {
+            const float x = f * t.x - g * t.y;
+            g = g * t.x + f * t.y;
+            f = x;
+        };
+        if (turned && is_k) {
+            if (a.interleaved) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) turn(y[2 * e], y[2 * e + 1], cs[8 * c + e]);
+            }
+            else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) turn(y[e], y[8 + e], cs[8 * c + e]);
+            }
+        }
+        uint32_t top = 0;   // (as whole numbers: a NaN counts as more than an infinity)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = max(top, __float_as_uint(fabsf(y[e])));
+        const uint32_t lanes = ((1u << per_row) - 1) << ((tid & 31) & ~(per_row - 1));
+        for (int o = per_row >> 1; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(lanes, top, o));
+        const float scale = code_scale<kCodes ? kCodes : kCodesInt8>(top);
+        uint32_t codes[4];
+        quantize16<kCodes ? kCodes : kCodesInt8>(y, scale, codes);
+        C* dst = is_k ? kdst + head * a.kc_head : vdst + head * a.vc_head;
+        *reinterpret_cast<uint2*>(dst + d0) = make_uint2(codes[0], codes[1]);
+        *reinterpret_cast<uint2*>(dst + d1) = make_uint2(codes[2], codes[3]);
+        if (c == 0) *(is_k ? kscale + head * a.ks_head : vscale + head * a.vs_head) = scale;
+    };
     auto store = [&](int row, uint4 u, uint4 w) {
+        if (kCodes && row >= a.heads) {
+            store_codes(row, u, w);
+            return;
+        }
         T* dst;
         if (row < a.heads) {
             dst = (T*)a.q_out + (size_t)token * a.qo_tok + (size_t)row * a.qo_head;
         }
         else if (row < a.heads + a.kv_heads) {
-            dst = kStore ? kdst : (T*)a.k_out + (size_t)token * a.ko_tok;
+            dst = kStore ? (T*)kdst : (T*)a.k_out + (size_t)token * a.ko_tok;
             if (dst != nullptr) dst += (size_t)(row - a.heads) * (kStore ? a.kc_head : a.ko_head);
         }
         else {
-            dst = vdst;
+            dst = (T*)vdst;
             if (dst != nullptr) dst += (size_t)(row - a.heads - a.kv_heads) * a.vc_head;
         }
         if (dst == nullptr) return;
@@ -158,7 +215,7 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryArgs a)
 
 }  // namespace
 
-template<typename T, bool kStore>
+template<typename T, bool kStore, int kCodes>
 static int launch_rotary_t(const RotaryArgs& a, cudaStream_t stream)
 {
     // few tokens: their heads are shared out, so that some 600 CTAs exist
@@ -168,15 +225,136 @@ static int launch_rotary_t(const RotaryArgs& a, cudaStream_t stream)
     const int wanted = (4 * sm_count() + a.tokens - 1) / a.tokens;
     if (shares > wanted) shares = wanted;
     if (shares < 1) shares = 1;
-    EET_CUDA(launch_pdl(rotary_kernel<T, kStore>, dim3((unsigned)a.tokens, (unsigned)shares), dim3(kRotThreads), 0, stream, a));
+    EET_CUDA(launch_pdl(rotary_kernel<T, kStore, kCodes>, dim3((unsigned)a.tokens, (unsigned)shares), dim3(kRotThreads), 0, stream, a));
     return 0;
 }
 
 int launch_rotary(const RotaryArgs& a, bool store, cudaStream_t stream)
 {
     if (a.tokens == 0 || (store && a.seqs == 0)) return 0;
-    if (a.bf16) return store ? launch_rotary_t<__nv_bfloat16, true>(a, stream) : launch_rotary_t<__nv_bfloat16, false>(a, stream);
-    return store ? launch_rotary_t<__half, true>(a, stream) : launch_rotary_t<__half, false>(a, stream);
+    if (store && a.codes == kCodesInt8) {
+        return a.bf16 ? launch_rotary_t<__nv_bfloat16, true, kCodesInt8>(a, stream) : launch_rotary_t<__half, true, kCodesInt8>(a, stream);
+    }
+    if (store && a.codes == kCodesE4M3) {
+        return a.bf16 ? launch_rotary_t<__nv_bfloat16, true, kCodesE4M3>(a, stream) : launch_rotary_t<__half, true, kCodesE4M3>(a, stream);
+    }
+    if (a.bf16) return store ? launch_rotary_t<__nv_bfloat16, true, 0>(a, stream) : launch_rotary_t<__nv_bfloat16, false, 0>(a, stream);
+    return store ? launch_rotary_t<__half, true, 0>(a, stream) : launch_rotary_t<__half, false, 0>(a, stream);
+}
+
+namespace {
+
+// Rows of the pages back as 16-bit values: the mirror of the append, with its rows.  A CTA takes kLoadTokens of them, finds their
+// pages, and then has all of its reads on their way at once.
+//
+// Bound: HBM.
+constexpr int kLoadThreads = 256;
+constexpr int kLoadTokens = 16;
+
+template<typename T, int kCodes>
+__global__ void __launch_bounds__(kLoadThreads) paged_load_kernel(const PagedLoadArgs a)
+{
+    using C = typename PagedCode<T, kCodes>::type;
+    constexpr int kItem = kCodes ? 16 : 8;      // dims a thread and turn: 16 bytes of the cache
+    constexpr int kAhead = 4;                   // turns on their way
+    __shared__ long long at[kLoadTokens];       // page * 256 + slot; -1: zeros, -2: not this call's business
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int token0 = blockIdx.x * kLoadTokens;
+    pdl_launch_dependents();
+    pdl_wait();
+    for (int t = warp; t < kLoadTokens; t += kLoadThreads / 32) {
+        const int token = token0 + t;
+        int seq = 0;   // how many sequences end at or before it
+        for (int i = 0; i < a.seqs; i += 32) seq += __popc(__ballot_sync(0xffffffffu, i + lane < a.seqs && a.starts[i + lane + 1] <= token));
+        if (lane != 0) continue;
+        long long place = -2;
+        if (token < a.tokens && seq < a.seqs && a.starts[seq] <= token) {
+            const long long pos = (long long)a.lens[seq] - a.starts[seq + 1] + token, column = pos >> a.page_shift;
+            if (pos >= 0) {
+                const int page = column < a.max_pages ? a.pages[seq * a.pages_stride + column] : -1;
+                if (page >= 0 && page < a.num_pages) {
+                    place = ((long long)page << 8) + (pos & ((1 << a.page_shift) - 1));
+                }
+                else {
+                    g_device_status = 6;
+                    place = -1;
+                }
+            }
+        }
+        at[t] = place;
+    }
+    __syncthreads();
+    const int per_row = a.head_dim / kItem, rows = 2 * a.kv_heads, items = kLoadTokens * rows * per_row;
+    for (int i0 = blockIdx.y * kLoadThreads + tid; i0 < items; i0 += kAhead * kLoadThreads * gridDim.y) {
+        uint4 x[kAhead];
+        float scale[kAhead];
+        T* dst[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const int i = i0 + j * kLoadThreads * gridDim.y;
+            dst[j] = nullptr;
+            x[j] = make_uint4(0u, 0u, 0u, 0u);
+            scale[j] = 0.f;
+            if (i >= items) continue;
+            const int c = i % per_row, r = i / per_row, row = r % rows, t = r / rows;
+            const long long place = at[t];
+            if (place == -2) continue;
+            const bool is_k = row < a.kv_heads;
+            const int head = is_k ? row : row - a.kv_heads;
+            dst[j] = (is_k ? (T*)a.k_out + (size_t)(token0 + t) * a.ko_tok + (size_t)head * a.ko_head
+                           : (T*)a.v_out + (size_t)(token0 + t) * a.vo_tok + (size_t)head * a.vo_head) + c * kItem;
+            if (place < 0) continue;
+            const long long page = place >> 8, slot = place & 255;
+            const C* src = is_k ? (const C*)a.k_cache + page * a.kc_page + head * a.kc_head + slot * a.kc_slot
+                                : (const C*)a.v_cache + page * a.vc_page + head * a.vc_head + slot * a.vc_slot;
+            x[j] = *reinterpret_cast<const uint4*>(src + c * kItem);
+            if (kCodes) scale[j] = is_k ? a.k_scale[page * a.ks_page + head * a.ks_head + slot] : a.v_scale[page * a.vs_page + head * a.vs_head + slot];
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            if (dst[j] == nullptr) continue;
+            uint4* out = reinterpret_cast<uint4*>(dst[j]);
+            if (!kCodes) {
+                out[0] = x[j];
+                continue;
+            }
+            float y[16];
+            dequantize16<kCodes ? kCodes : kCodesInt8>(x[j], scale[j], y);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint4 w;
+                uint32_t* p = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const auto v = Pair2<T>::down(y[8 * h + 2 * e], y[8 * h + 2 * e + 1]);
+                    p[e] = *reinterpret_cast<const uint32_t*>(&v);
+                }
+                out[h] = w;
+            }
+        }
+    }
+}
+
+}  // namespace
+
+template<typename T, int kCodes>
+static int launch_paged_load_t(const PagedLoadArgs& a, cudaStream_t stream)
+{
+    const int tiles = (a.tokens + kLoadTokens - 1) / kLoadTokens;
+    const int items = kLoadTokens * 2 * a.kv_heads * (a.head_dim / (kCodes ? 16 : 8));
+    // few tokens: their rows are shared out, so that some 600 CTAs exist
+    int shares = (items + kLoadThreads - 1) / kLoadThreads;
+    const int wanted = (4 * sm_count() + tiles - 1) / tiles;
+    if (shares > wanted) shares = wanted;
+    EET_CUDA(launch_pdl(paged_load_kernel<T, kCodes>, dim3((unsigned)tiles, (unsigned)shares), dim3(kLoadThreads), 0, stream, a));
+    return 0;
+}
+
+int launch_paged_load(const PagedLoadArgs& a, cudaStream_t stream)
+{
+    if (a.codes == kCodesInt8) return a.bf16 ? launch_paged_load_t<__nv_bfloat16, kCodesInt8>(a, stream) : launch_paged_load_t<__half, kCodesInt8>(a, stream);
+    if (a.codes == kCodesE4M3) return a.bf16 ? launch_paged_load_t<__nv_bfloat16, kCodesE4M3>(a, stream) : launch_paged_load_t<__half, kCodesE4M3>(a, stream);
+    return a.bf16 ? launch_paged_load_t<__nv_bfloat16, 0>(a, stream) : launch_paged_load_t<__half, 0>(a, stream);
 }
 
 // Which kernels serve a call.  Sequences whose new tokens make at most 16 rows with the heads that share a kv head are for the kernel

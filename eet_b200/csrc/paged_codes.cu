@@ -1,0 +1,564 @@
+// Attention of few new tokens over a paged cache of 8-bit codes: up to kRows (8 or 16) rows a kv head, a row being a (token, query
+// head) pair that shares it.
+//
+//   out = sum_j w_j c^v_j / sum_j w_j / s^v_j,   w_j = s^v_j 2^(s^k_j (q . c^k_j) scale log2(e) + slope (j - p) log2(e) - ref)
+//
+// The codes enter the products as fp16, where they are exact, and the scales stay outside: that of a key on its score, that of its
+// value on its weight, before that is rounded to fp16.  So that the weights fit fp16 whatever the scales are, the reference ref of a row
+// follows the largest score + log2(s^v), not the largest score.  q of bf16 is multiplied by a power of two that brings its largest
+// value to 2^14 and enters as fp16 too: eight bits of every value down to 2^-28 of the largest are kept.
+//
+// Bound: HBM, the codes and scales of every sequence once.  A block of 128 keys is half the bytes of a 16-bit one, and everything on
+// the way has to keep up: pages of 16 slots are eight copies of 2 KiB a block, which the copy engine takes 85 cycles each for, so the
+// warps copy themselves (cp.async), each into a ring of its own that nobody else waits for; and a code becomes a value in registers, in
+// the layout in which mma.sync takes its 16-row operand, so that nothing is written back to shared memory:
+//   S^T [16 keys][8] = K.Q^T       lane (g, t) = (lane / 4, lane % 4) holds dims 32 t .. 32 t + 31 of keys g and g + 8: which dims stand
+//                                  for which index of the sum is free as long as Q's do the same
+//   O^T [16 dims][8] += V^T.P^T    lane (g, t) holds dims 16 g .. 16 g + 15 of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9; two keys' bytes are
+//                                  interleaved to pairs, dims 16 g + 2 i and 16 g + 2 i + 1 are rows g and g + 8 of tile i
+// P^T leaves S^T's layout by a transposition of 8 x 8 in the warp (movmatrix).  (Tensor memory and tcgen05 would need the values in shared
+// memory: 64 KiB written and read again for every 32 KiB that arrive.)
+//
+// A CTA is four warps, 32 keys of a block each; two CTAs share an SM, so that the beginning and the end of a piece of one run beside the
+// other's blocks.  The warps' sums meet in shared memory at the end of a piece.  The work is cut up as paged_share.cuh says.
+#include "codes.cuh"
+#include "paged_share.cuh"
+
+namespace eet {
+
+namespace {
+
+constexpr int kPcWarps = 4;
+constexpr int kPcThreads = 32 * kPcWarps;
+constexpr int kPcKeys = kPgKeys / kPcWarps;     // of a block, for a warp
+constexpr int kPcStages = 3;
+constexpr int kPcPerSm = 2;                     // CTAs
+constexpr int kPcExtra = 2;                     // a piece's beginning and end cost as much as two blocks
+static_assert(kPcKeys == 32, "a lane a scale, two runs of 16 keys");
+
+template<int D>
+struct PcShape {
+    static constexpr int kTile = kPcKeys * D;                           // bytes: a warp's codes of K or V of a block
+    static constexpr int kStage = 2 * kTile + 2 * kPcKeys * 4;          // and the scales
+    static constexpr int kSmem = kPcWarps * kPcStages * kStage;
+};
+
+struct PcSmem {
+    float ref[kPcWarps][16], sum[kPcWarps][16];
+    PgFound found;
+};
+
+__device__ __forceinline__ void copy16_async(uint32_t dst, const void* src, uint32_t bytes)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+__device__ __forceinline__ void copy4_async(uint32_t dst, const void* src, uint32_t bytes)
+{
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x)
+{
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t at)
+{
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+    return v;
+}
+
+__device__ __forceinline__ uint2 lds64(uint32_t at)
+{
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
+    return v;
+}
+
+// Where 16 bytes of a row lie in a tile: swizzled, so that neither of the two ways of reading meets a bank twice.
+template<int D>
+__device__ __forceinline__ uint32_t pc_place(int row, int chunk)
+{
+    if (D == 128) return (uint32_t)(row * 128 + ((chunk ^ (row & 7)) << 4));
+    return (uint32_t)((row >> 1) * 128 + ((((row & 1) * 4 + chunk) ^ (row & 6)) << 4));
+}
+
+// What a warp copies: its 32 keys of a block of a piece.
+template<int D>
+struct PcCopies {
+    const PagedMhaArgs& a;
+    uint32_t ring;                // of this warp
+    int offset;                   // of its keys in a block
+
+    // the page of the run of 16 keys that this half of the warp looks after; -1: it has none of the keys that the tile sees
+    __device__ __forceinline__ int page(const PgPiece& p, const PgSpan& span, int key0) const
+    {
+        const int key = key0 + offset + (int)(threadIdx.x & 16);
+        if (key >= span.hi || key + 16 <= span.lo) return -1;
+        const int page = (a.pages + p.seq * a.pages_stride)[key >> a.page_shift];
+        if (page < 0 || page >= a.num_pages) {
+            g_device_status = 6;
+            return -2;            // zeros
+        }
+        return page;
+    }
+    __device__ __forceinline__ void issue(const PgPiece& p, int key0, int page, int stage) const
+    {
+        constexpr int kChunks = D / 16, kRowsAtOnce = 32 / kChunks, kTimes = 16 / kRowsAtOnce;
+        const int lane = threadIdx.x & 31, key = key0 + offset, slot = key & ((1 << a.page_shift) - 1);
+        const uint32_t at = ring + (uint32_t)(stage * PcShape<D>::kStage);
+#pragma unroll
+        for (int run = 0; run < 2; ++run) {
+            const int n = __shfl_sync(0xffffffffu, page, 16 * run);
+            if (n == -1) continue;
+            const uint32_t bytes = n >= 0 ? 16 : 0;
+            const int s = (slot + 16 * run) & ((1 << a.page_shift) - 1), row0 = lane / kChunks, c = lane % kChunks;
+            const uint8_t *k = (const uint8_t*)a.k_cache, *v = (const uint8_t*)a.v_cache;
+            if (n >= 0) {
+                k += n * a.kc_page + p.head * a.kc_head + (s + row0) * a.kc_slot + 16 * c;
+                v += n * a.vc_page + p.head * a.vc_head + (s + row0) * a.vc_slot + 16 * c;
+            }
+            const long long k_step = n >= 0 ? kRowsAtOnce * a.kc_slot : 0, v_step = n >= 0 ? kRowsAtOnce * a.vc_slot : 0;
+#pragma unroll
+            for (int i = 0; i < kTimes; ++i) {
+                const uint32_t to = at + pc_place<D>(16 * run + row0 + kRowsAtOnce * i, c);
+                copy16_async(to, k + i * k_step, bytes);
+                copy16_async(to + PcShape<D>::kTile, v + i * v_step, bytes);
+            }
+            // a half of the warp for the scales of either
+            const float* scale = lane < 16 ? a.k_scale : a.v_scale;
+            if (n >= 0) scale += (lane < 16 ? n * a.ks_page + p.head * a.ks_head : n * a.vs_page + p.head * a.vs_head) + s + (lane & 15);
+            copy4_async(at + 2 * PcShape<D>::kTile + (uint32_t)(((lane < 16 ? 0 : kPcKeys) + 16 * run + (lane & 15)) * 4), scale, bytes / 4);
+        }
+    }
+};
+
+template<int kCodes, int D, int kRows>
+__global__ void __launch_bounds__(kPcThreads, kPcPerSm)
+paged_mha_codes_kernel(const __grid_constant__ PagedMhaArgs a, void* ws, int most, int whole)
+{
+    using Shape = PcShape<D>;
+    constexpr int kN = kRows / 8;                // tiles of 8 rows
+    constexpr int kSteps = D / 16;               // of the sum over dims; tiles of 16 dims
+    constexpr float kUp = PgType<__half>::kUp;
+    constexpr float kLog2e = 1.4426950408889634f;
+    extern __shared__ __align__(1024) uint8_t pc_dyn[];
+    __shared__ PcSmem sm;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int group = a.heads / a.kv_heads, tile_tokens = kRows / group;
+    const int cta = blockIdx.x, ctas = gridDim.x;
+    const PgTiling tiling = {tile_tokens, 1, most, kPcExtra};
+    pdl_launch_dependents();
+    pdl_wait();
+
+    PgShare share;
+    PgPlace place;
+    const bool work = pg_find_share(a, tiling, cta, ctas, whole != 0, sm.found, share, place);
+    if (!whole && threadIdx.x == 0) pg_write_header(a, tiling, ws, cta, ctas, work, share, place);
+    if (!work) return;
+
+    const long long cap = (long long)a.max_pages << a.page_shift;
+    const int last = (int)min(cap, 0x7fffffffLL) - 1;      // position that has a place in the table
+    auto span_of = [&](const PgPiece& p) { return pg_span(a, p.s, p.tile * tile_tokens, (p.tile + 1) * tile_tokens); };
+    const PcCopies<D> copies = {a, smem_u32(pc_dyn) + (uint32_t)(warp * kPcStages * Shape::kStage), warp * kPcKeys};
+
+    // The piece at work and the one behind it; the copies run kPcStages - 1 blocks ahead, into the latter but not beyond.
+    PgPiece p, next;
+    bool more = share.next(a, tiling, p);
+    bool have_next = more && share.next(a, tiling, next);
+    PgSpan span = {0, 0}, next_span = {0, 0};
+    if (more) span = span_of(p);
+    if (have_next) next_span = span_of(next);
+    int ahead = 0, into = 0;       // next block to copy, of p or from p.blocks on of next; its stage
+    int stage = 0;                 // of the next block to work on
+    int page = -1;                 // of the block to copy
+    auto look = [&]() {
+        if (ahead < p.blocks) page = copies.page(p, span, (p.top - ahead) * kPgKeys);
+        else if (have_next && ahead < p.blocks + next.blocks) page = copies.page(next, next_span, (next.top - (ahead - p.blocks)) * kPgKeys);
+    };
+    auto fetch = [&]() -> bool {   // a block, in a group of its own
+        if (ahead < p.blocks) copies.issue(p, (p.top - ahead) * kPgKeys, page, into);
+        else if (have_next && ahead < p.blocks + next.blocks) copies.issue(next, (next.top - (ahead - p.blocks)) * kPgKeys, page, into);
+        else return false;
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        ++ahead;
+        into = into == kPcStages - 1 ? 0 : into + 1;
+        look();
+        return true;
+    };
+    if (more) {
+        look();
+        while (ahead < kPcStages - 1 && fetch()) {}
+    }
+
+    while (more) {
+        const int token0 = p.tile * tile_tokens;
+        const int rows = min(tile_tokens, p.s.tokens - token0) * group;
+        if (p.s.p0 + p.s.tokens > cap && threadIdx.x == 0) g_device_status = 6;
+        // Q: lane (g, t) holds dims D / 4 t .. of rows g, and what of rows 2 t and 2 t + 1 the scores need
+        uint32_t q[kN][kSteps][2];
+        float factor[kN][2], slope[kN][2], ref[kN][2], l[kN][2];
+        int low[kN][2], high[kN][2], pos[kN][2];
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+            const int r = 8 * n + g;
+            uint32_t* w = &q[n][0][0];
+#pragma unroll
+            for (int i = 0; i < 2 * kSteps; ++i) w[i] = 0u;
+            if (r < rows) {
+                const uint16_t* src = (const uint16_t*)a.q + (size_t)(p.s.row0 + token0 + r / group) * a.q_tok +
+                                      (size_t)(p.head * group + r % group) * a.q_head + t * (D / 4);
+#pragma unroll
+                for (int i = 0; i < kSteps / 2; ++i) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(src + 8 * i);
+                    w[4 * i] = x.x, w[4 * i + 1] = x.y, w[4 * i + 2] = x.z, w[4 * i + 3] = x.w;
+                }
+            }
+            int e = 0;             // what the row was multiplied with, as a power of two
+            if (a.bf16) {
+                uint32_t top = 0;
+#pragma unroll
+                for (int i = 0; i < 2 * kSteps; ++i) top = max(top, max(w[i] << 16 & 0x7fffffffu, w[i] & 0x7fff0000u));
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                // (in two factors, since 2^(14 - exponent) may lie outside fp32's range)
+                e = top >= 0x00800000u ? 141 - (int)(top >> 23) : 140;
+                const float f0 = __uint_as_float((uint32_t)(127 + e / 2) << 23), f1 = __uint_as_float((uint32_t)(127 + e - e / 2) << 23);
+#pragma unroll
+                for (int i = 0; i < 2 * kSteps; ++i) {
+                    const __half2 h = __floats2half2_rn(__uint_as_float(w[i] << 16) * f0 * f1, __uint_as_float(w[i] & 0xffff0000u) * f0 * f1);
+                    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int row = 8 * n + 2 * t + i;
+                const int down = __shfl_sync(0xffffffffu, e, 4 * (2 * t + i));
+                // (again in two: scale / kCodeUnit and the power of the row)
+                factor[n][i] = a.scale * kLog2e / kCodeUnit<kCodes> * __uint_as_float((uint32_t)(127 - down / 2) << 23) *
+                               __uint_as_float((uint32_t)(127 - (down - down / 2)) << 23);
+                const bool valid = row < rows;
+                pos[n][i] = p.s.p0 + token0 + row / group;
+                low[n][i] = valid ? p.s.first : 0;
+                if (valid && a.window > 0) low[n][i] = (int)max((long long)low[n][i], (long long)pos[n][i] - a.window + 1);
+                high[n][i] = valid ? min(pos[n][i], last) : 0x7fffffff;   // (a row that stands for no token takes what comes)
+                slope[n][i] = a.slopes != nullptr && valid ? a.slopes[p.head * group + row % group] * kLog2e : 0.f;
+                ref[n][i] = kPgNone;
+                l[n][i] = 0.f;
+            }
+        }
+        float o[kN][kSteps][4];
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[n][i][e] = 0.f;
+            }
+        }
+        int used = stage;          // stage of the piece's last block
+        for (int j = 0; j < p.blocks; ++j) {
+            if (ahead - j > kPcStages - 2) asm volatile("cp.async.wait_group %0;" ::"n"(kPcStages - 2) : "memory");
+            else asm volatile("cp.async.wait_group 0;" ::: "memory");
+            __syncwarp();
+            used = stage;
+            fetch();               // (to the stage of the block before, which all lanes have read before the barrier above)
+            const uint32_t at = copies.ring + (uint32_t)(stage * Shape::kStage);
+            stage = stage == kPcStages - 1 ? 0 : stage + 1;
+            const int key0 = (p.top - j) * kPgKeys + copies.offset;
+            if (key0 >= span.hi || key0 + kPcKeys <= span.lo) continue;
+            // ---- scores
+            float s[2][kN][4];
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+#pragma unroll
+                for (int n = 0; n < kN; ++n) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[m][n][e] = 0.f;
+                }
+#pragma unroll
+                for (int h = 0; h < D / 64; ++h) {
+                    const int c = D / 64 * t + h;
+                    const uint4 x = lds128(at + pc_place<D>(16 * m + g, c)), y = lds128(at + pc_place<D>(16 * m + 8 + g, c));
+                    const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t a0, a1, a2, a3;
+                        codes_to_half<kCodes>(xs[i], a0, a2);
+                        codes_to_half<kCodes>(ys[i], a1, a3);
+#pragma unroll
+                        for (int n = 0; n < kN; ++n) mma_m16n8k16(s[m][n], a0, a1, a2, a3, q[n][4 * h + i][0], q[n][4 * h + i][1]);
+                    }
+                }
+            }
+            // ---- weights
+            float vs[2][2], lvs[2][2];
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t place = at + 2 * Shape::kTile + (uint32_t)((16 * m + 8 * i + g) * 4);
+                    float ks;
+                    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(ks) : "r"(place));
+                    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(vs[m][i]) : "r"(place + kPcKeys * 4));
+                    lvs[m][i] = __log2f(fmaxf(vs[m][i], 8.67361738e-19f));   // (2^-60 at least: a scale of zero weighs nothing)
+                    const int key = key0 + 16 * m + 8 * i + g;
+#pragma unroll
+                    for (int n = 0; n < kN; ++n) {
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            float& x = s[m][n][2 * i + r];
+                            x *= ks * factor[n][r];
+                            if (a.slopes != nullptr) x = fmaf(slope[n][r], (float)(key - pos[n][r]), x);
+                            x = key >= low[n][r] && key <= high[n][r] ? x : -INFINITY;
+                        }
+                    }
+                }
+            }
+            bool over = false;
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+#pragma unroll
+                for (int n = 0; n < kN; ++n) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) over |= s[m][n][e] + lvs[m][e >> 1] - ref[n][e & 1] > kPgLag + kUp;
+                }
+            }
+            if (__any_sync(0xffffffffu, over)) {
+                // some row's reference moves
+#pragma unroll
+                for (int n = 0; n < kN; ++n) {
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        float m = -INFINITY;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) m = fmaxf(m, s[k >> 1][n][2 * (k & 1) + r] + lvs[k >> 1][k & 1]);
+#pragma unroll
+                        for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+                        const bool moves = m - ref[n][r] > kPgLag + kUp;
+                        const float to = moves ? m - kUp : ref[n][r], corr = moves ? ex2_approx(ref[n][r] - to) : 1.0f;
+                        ref[n][r] = to;
+                        l[n][r] *= corr;
+#pragma unroll
+                        for (int i = 0; i < kSteps; ++i) {
+                            o[n][i][r] *= corr;
+                            o[n][i][2 + r] *= corr;
+                        }
+                    }
+                }
+            }
+            uint32_t w[2][kN][2];
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float scale = vs[m][i], inverse = __fdividef(1.0f, scale);
+#pragma unroll
+                    for (int n = 0; n < kN; ++n) {
+                        float e[2];
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            const float x = s[m][n][2 * i + r];
+                            const float power = ex2_approx(x - ref[n][r]);
+                            // (a scale in a place that nobody sees may be anything; beyond 2^24 a score may not know of log2 s^v)
+                            asm("min.NaN.f32 %0, %1, %2;" : "=f"(e[r]) : "f"(x == -INFINITY ? 0.f : power * scale), "f"(65504.0f));
+                            s[m][n][2 * i + r] = power;
+                        }
+                        const __half2 h = __floats2half2_rn(e[0], e[1]);
+                        const float2 f = __half22float2(h);
+                        // (The sum is of the rounded weights: where one key has most of the weight, its rounding then cancels.  Below
+                        // the smallest normal value, a scale of zero among it, what rounding leaves says nothing of the power.)
+                        l[n][0] += f.x >= 6.103515625e-5f ? f.x * inverse : s[m][n][2 * i];
+                        l[n][1] += f.y >= 6.103515625e-5f ? f.y * inverse : s[m][n][2 * i + 1];
+                        w[m][n][i] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h));
+                    }
+                }
+            }
+            // ---- sums
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                constexpr int kWords = D / 32;     // of the D / 8 bytes of a key that a lane has
+                uint32_t v[4][kWords];             // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int row = 16 * m + 2 * t + (k & 1) + 8 * (k >> 1);
+                    if (D == 128) {
+                        const uint4 x = lds128(at + Shape::kTile + pc_place<D>(row, g));
+                        v[k][0] = x.x, v[k][1] = x.y, v[k][2 % kWords] = x.z, v[k][3 % kWords] = x.w;
+                    }
+                    else {
+                        const uint2 x = lds64(at + Shape::kTile + pc_place<D>(row, g >> 1) + (uint32_t)((g & 1) * 8));
+                        v[k][0] = x.x, v[k][1] = x.y;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < kWords; ++i) {
+                    // dims 4 i .. 4 i + 3 of the lane's, pairs of keys
+                    uint32_t lo[4], hi[4];
+                    codes_to_half<kCodes>(__byte_perm(v[0][i], v[1][i], 0x5140), lo[0], lo[1]);
+                    codes_to_half<kCodes>(__byte_perm(v[0][i], v[1][i], 0x7362), lo[2], lo[3]);
+                    codes_to_half<kCodes>(__byte_perm(v[2][i], v[3][i], 0x5140), hi[0], hi[1]);
+                    codes_to_half<kCodes>(__byte_perm(v[2][i], v[3][i], 0x7362), hi[2], hi[3]);
+#pragma unroll
+                    for (int n = 0; n < kN; ++n) {
+                        mma_m16n8k16(o[n][2 * i], lo[0], lo[1], hi[0], hi[1], w[m][n][0], w[m][n][1]);
+                        mma_m16n8k16(o[n][2 * i + 1], lo[2], lo[3], hi[2], hi[3], w[m][n][0], w[m][n][1]);
+                    }
+                }
+            }
+        }
+
+        // ---- the end of a piece: the sums of the lanes, then of the warps
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) l[n][r] += __shfl_xor_sync(0xffffffffu, l[n][r], x);
+                if (g == 0) {
+                    sm.ref[warp][8 * n + 2 * t + r] = ref[n][r];
+                    sm.sum[warp][8 * n + 2 * t + r] = l[n][r];
+                }
+            }
+        }
+        // O goes where the codes of the piece's last block were, [row][dim], rows D floats apart and rotated against the banks.  (Nothing
+        // is on its way there: the copies that follow go to that stage with the next block.)
+        float* mine = reinterpret_cast<float*>(pc_dyn + (warp * kPcStages + used) * Shape::kStage);
+        __syncwarp();
+        if (p.blocks > 0) {
+#pragma unroll
+            for (int n = 0; n < kN; ++n) {
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int row = 8 * n + 2 * t + (e & 1), d = D / 8 * g + 2 * i + (e >> 1);
+                        mine[row * D + ((d + 8 * row) & (D - 1))] = o[n][i][e];
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        const bool complete = p.starts && p.ends;
+        const PgPartial part = pg_partial(ws, ctas, cta, p.starts ? 1 : 0, kRows, D);
+        for (int i = threadIdx.x; i < rows * (D / 4); i += kPcThreads) {
+            const int row = i / (D / 4), d = i % (D / 4) * 4;
+            float top = kPgNone, sum = 0.f;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < kPcWarps; ++w) {
+                if (sm.sum[w][row] != 0.f) top = fmaxf(top, sm.ref[w][row]);
+            }
+#pragma unroll
+            for (int w = 0; w < kPcWarps; ++w) {
+                const float part_sum = sm.sum[w][row];
+                if (part_sum == 0.f) continue;      // (it has seen nothing)
+                const float f = ex2_approx(sm.ref[w][row] - top);
+                sum += part_sum * f;
+                const float4 x = *reinterpret_cast<const float4*>(
+                    reinterpret_cast<const float*>(pc_dyn + (w * kPcStages + used) * Shape::kStage) + row * D + ((d + 8 * row) & (D - 1)));
+                v.x += x.x * f, v.y += x.y * f, v.z += x.z * f, v.w += x.w * f;
+            }
+            const float f = (complete ? (sum == 0.f ? 0.f : 1.0f / sum) : 1.0f) / kCodeUnit<kCodes>;
+            v = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
+            if (!complete) {
+                part.o[row * (D / 4) + d / 4] = v;
+                if (d == 0) {
+                    part.max2[row] = top;
+                    part.sum[row] = sum;
+                }
+            }
+            else {
+                uint16_t* dst = (uint16_t*)a.out + (size_t)(p.s.row0 + token0 + row / group) * a.o_tok +
+                                (size_t)(p.head * group + row % group) * a.o_head + d;
+                uint2 w;
+                if (a.bf16) w = make_uint2(PgType<__nv_bfloat16>::pack(v.x, v.y), PgType<__nv_bfloat16>::pack(v.z, v.w));
+                else w = make_uint2(PgType<__half>::pack(v.x, v.y), PgType<__half>::pack(v.z, v.w));
+                *reinterpret_cast<uint2*>(dst) = w;
+            }
+        }
+        __syncthreads();   // the stage is free again
+        more = have_next;
+        ahead -= p.blocks;
+        p = next;
+        span = next_span;
+        if (more) {
+            const bool waiting = ahead == p.blocks;   // the copies, for the piece behind
+            have_next = share.next(a, tiling, next);
+            if (have_next) next_span = span_of(next);
+            if (waiting) look();
+            while (ahead < kPcStages - 1 && fetch()) {}
+        }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+template<int kCodes, int D, int kRows>
+int pc_launch(const PagedMhaArgs& a, void* ws, int most, int whole, cudaStream_t stream)
+{
+    auto kern = paged_mha_codes_kernel<kCodes, D, kRows>;
+    constexpr int kSmem = PcShape<D>::kSmem;
+    static bool attr_set[64] = {};
+    int dev = 0;
+    EET_CUDA(cudaGetDevice(&dev));
+    dev &= 63;
+    if (!attr_set[dev]) {
+        EET_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+        attr_set[dev] = true;
+    }
+    EET_CUDA(launch_pdl(kern, dim3(kPcPerSm * sm_count()), dim3(kPcThreads), kSmem, stream, a, ws, most, whole));
+    return 0;
+}
+
+}  // namespace
+
+struct PagedCodesPlan {
+    int rows;            // of a tile: 8 or 16
+    bool whole;
+    size_t bytes;
+};
+
+static PagedCodesPlan paged_codes_plan(const PagedMhaArgs& a)
+{
+    PagedCodesPlan p = {};
+    const int group = a.heads / a.kv_heads;
+    p.rows = (long long)a.max_tokens * group <= 8 ? 8 : 16;
+    p.whole = false;
+    p.bytes = pg_scratch_bytes(kPcPerSm * sm_count(), p.rows, a.head_dim);
+    return p;
+}
+
+size_t paged_mha_codes_workspace_bytes(const PagedMhaArgs& a)
+{
+    return paged_codes_plan(a).bytes;
+}
+
+template<int kCodes, int D>
+static int launch_paged_mha_codes_t(const PagedMhaArgs& a, const PagedCodesPlan& p, cudaStream_t stream)
+{
+    const int rc = p.rows == 8 ? pc_launch<kCodes, D, 8>(a, a.ws, 0x7fffffff, p.whole, stream)
+                               : pc_launch<kCodes, D, 16>(a, a.ws, 0x7fffffff, p.whole, stream);
+    if (rc || p.whole) return rc;
+    const PgScratch s = {a.ws, p.rows, 0}, none = {};
+    const int y = (p.rows * (D / 8) + kPgJoinThreads - 1) / kPgJoinThreads;
+    const dim3 grid(kPcPerSm * sm_count(), y, 1);
+    if (a.bf16) EET_CUDA(launch_pdl(paged_mha_join_kernel<__nv_bfloat16, D>, grid, dim3(kPgJoinThreads), 0, stream, a, s, none));
+    else EET_CUDA(launch_pdl(paged_mha_join_kernel<__half, D>, grid, dim3(kPgJoinThreads), 0, stream, a, s, none));
+    return 0;
+}
+
+int launch_paged_mha_codes(const PagedMhaArgs& a, cudaStream_t stream)
+{
+    const PagedCodesPlan p = paged_codes_plan(a);
+    EET_CHECK(a.heads / a.kv_heads <= 16, "eet_paged_mha_codes: more than 16 query heads to a kv head");
+    if (a.codes == kCodesInt8) {
+        return a.head_dim == 128 ? launch_paged_mha_codes_t<kCodesInt8, 128>(a, p, stream) : launch_paged_mha_codes_t<kCodesInt8, 64>(a, p, stream);
+    }
+    return a.head_dim == 128 ? launch_paged_mha_codes_t<kCodesE4M3, 128>(a, p, stream) : launch_paged_mha_codes_t<kCodesE4M3, 64>(a, p, stream);
+}
+
+}  // namespace eet

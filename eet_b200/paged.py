@@ -15,6 +15,10 @@ are read there, so a captured CUDA graph of these calls serves whatever they hol
 behind a sequence's last position are not read.  A page number outside the cache is not followed: the call completes and
 ``EET.check_device_status()`` reports it.
 
+A cache may also hold 8-bit codes: k_cache and v_cache int8 or float8_e4m3fn, beside k_scale and v_scale float32 [pages, kv_heads,
+page_size] - half the memory, and half of what a decode step reads.  A row of head_dim values is kept as code * scale with scale = max |y| /
+127 or / 448; paged_store writes both, paged_mha and paged_load take both, as k_scale= and v_scale=.  `paged_load` reads rows back.
+
 `PagedMmha` is the attention block around them, beside `EET.LlamaMmha` and `EET.BaichuanMmha`.
 
 The reference serves one contiguous cache an op, all sequences at the same step (csrc/op/llama_mmha.cpp:94-112).
@@ -27,7 +31,7 @@ import torch
 from ._lib import check, lib
 from .EET import _current_device, _forget, _linear, _norm_head, _on, _pool, _raw_stream
 
-__all__ = ["rotary_frequencies", "apply_rotary", "paged_store", "paged_mha", "PagedMmha"]
+__all__ = ["rotary_frequencies", "apply_rotary", "paged_store", "paged_load", "paged_mha", "PagedMmha"]
 
 _DTYPES = (torch.float16, torch.bfloat16)
 _PAGE_SIZES = (16, 32, 64, 128, 256)
@@ -36,6 +40,9 @@ _pack_store = struct.Struct("11P26qd").pack
 _pack_mha = struct.Struct("9P23qd").pack
 _pack_scratch = struct.Struct("Pq").pack
 _NO_SCRATCH = _pack_scratch(0, 0)
+_CODES = {torch.int8: 1, torch.float8_e4m3fn: 2}
+_pack_codes = struct.Struct("2P5q").pack
+_pack_load = struct.Struct("9P20q").pack
 
 
 def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, device="cuda:0"):
@@ -127,11 +134,11 @@ def _call(function, args, index):
             check(function(args, _raw_stream(index)))
 
 
-def _workspace_bytes(args, index):
+def _workspace_bytes(function, args, index):
     if index == _current_device():
-        return lib.eet_paged_mha_workspace_bytes(args + _NO_SCRATCH)
+        return function(args)
     with torch.cuda.device(index):
-        return lib.eet_paged_mha_workspace_bytes(args + _NO_SCRATCH)
+        return function(args)
 
 
 def _array(who, name, t, dtype, numel, index):
@@ -143,7 +150,7 @@ def _array(who, name, t, dtype, numel, index):
 
 
 def _cache(who, k_cache, v_cache, dtype, index):
-    """(pages, kv_heads, page_size, head_dim) and the strides of a cache."""
+    """(pages, kv_heads, page_size, head_dim) and the strides of a cache of this type, a 16-bit one or that of codes."""
     shape = k_cache.shape
     if len(shape) != 4 or v_cache.shape != shape:
         raise RuntimeError(f"{who}: k_cache and v_cache must both be [pages, kv_heads, page_size, head_dim], got {tuple(shape)} and "
@@ -156,6 +163,26 @@ def _cache(who, k_cache, v_cache, dtype, index):
     if shape[2] not in _PAGE_SIZES:
         raise RuntimeError(f"{who}: page size {shape[2]}, only 16, 32, 64, 128 and 256 are supported")
     return shape, ks[:3] + vs[:3]
+
+
+def _scales(who, k_cache, k_scale, v_scale, shape, index):
+    """What the entry points for codes take behind the arguments of the others."""
+    if k_scale is None or v_scale is None:
+        raise RuntimeError(f"{who}: a cache of codes has both k_scale and v_scale")
+    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+        if t.shape != shape[:3] or t.dtype != torch.float32 or t.get_device() != index or t.stride(2) != 1:
+            raise RuntimeError(f"{who}: {name} must be a float32 tensor {tuple(shape[:3])} with contiguous slots on cuda:{index}, got "
+                               f"{tuple(t.shape)} {t.dtype} with strides {t.stride()} on {t.device}")
+    return _pack_codes(k_scale.data_ptr(), v_scale.data_ptr(), _CODES[k_cache.dtype], *k_scale.stride()[:2], *v_scale.stride()[:2])
+
+
+def _kept_type(who, k_cache, dtype, k_scale, v_scale):
+    """The type that both caches must have: q's, or with scales that of codes."""
+    if k_scale is None and v_scale is None:
+        return dtype
+    if k_cache.dtype not in _CODES:
+        raise RuntimeError(f"{who}: scales belong to a cache of codes, int8 or float8_e4m3fn, not to {k_cache.dtype}")
+    return k_cache.dtype
 
 
 def _table(who, pages, starts, lens, index):
@@ -208,9 +235,12 @@ def apply_rotary(q, k, positions, freqs, interleaved=False, magnitude=1.0, q_out
 
 
 def paged_store(k, v, k_cache, v_cache, pages, starts, lens, q=None, freqs=None, interleaved=False, magnitude=1.0, positions=None,
-                q_out=None):
+                q_out=None, k_scale=None, v_scale=None):
     """Appends k and v [tokens, kv_heads, head_dim] of new tokens to their pages, k rotated when freqs is given, and returns q
     [tokens, heads, head_dim] rotated the same way (in q_out; a new tensor unless given, q_out=q works in place; None without q).
+
+    With caches of codes k_scale and v_scale are written beside them: k behind its rotation, in fp32, and v are divided by their scale and
+    rounded once, to nearest; a row of zeros has the scale 1, one with a NaN or an infinity NaN.
 
     The positions of the rotation are those in the sequence, or positions int64 [tokens].  Rows of k, v and q that belong to no
     sequence are not touched; of rows in front of a sequence's first position only q is.  Two sequences must not append to the same
@@ -219,7 +249,7 @@ def paged_store(k, v, k_cache, v_cache, pages, starts, lens, q=None, freqs=None,
     shape, dtype, index, k_str = _first(who, "k", k)
     tokens, kv_heads, head_dim = shape
     v_str = _heads(who, "v", v, shape, dtype, index)
-    cache_shape, cache_strides = _cache(who, k_cache, v_cache, dtype, index)
+    cache_shape, cache_strides = _cache(who, k_cache, v_cache, _kept_type(who, k_cache, dtype, k_scale, v_scale), index)
     if cache_shape[1] != kv_heads or cache_shape[3] != head_dim:
         raise RuntimeError(f"paged_store: caches of {cache_shape[1]} heads of {cache_shape[3]} beside {kv_heads} heads of {head_dim}")
     seqs, columns, pages_stride, table = _table(who, pages, starts, lens, index)
@@ -242,12 +272,59 @@ def paged_store(k, v, k_cache, v_cache, pages, starts, lens, q=None, freqs=None,
     args = _pack_store(q_at, k.data_ptr(), v.data_ptr(), qo_at, k_cache.data_ptr(), v_cache.data_ptr(), *table, where, turns, tokens, seqs,
                        heads, kv_heads, head_dim, 2 * half, bool(interleaved), dtype == torch.bfloat16, cache_shape[0], cache_shape[2],
                        columns, pages_stride, *q_str, *k_str, *v_str, *qo_str, *cache_strides, magnitude)
-    _call(lib.eet_paged_store, args, index)
+    if k_scale is None and v_scale is None:
+        _call(lib.eet_paged_store, args, index)
+    else:
+        _call(lib.eet_paged_store_codes, args + _scales(who, k_cache, k_scale, v_scale, cache_shape, index), index)
     return q_out
 
 
+def paged_load(k_cache, v_cache, pages, starts, lens, tokens=None, dtype=None, k_scale=None, v_scale=None, k_out=None, v_out=None):
+    """Reads rows back from their pages, the mirror of paged_store: returns (k, v) [tokens, kv_heads, head_dim], rows starts[b] to
+    starts[b + 1] being the last positions of sequence b (whole histories: starts = 0, lens[0], lens[0] + lens[1], ...).
+
+      tokens         the number of rows, that of k_out by default
+      dtype          fp16 or bf16 for a cache of codes, whose values code * scale are rounded to it; a 16-bit cache comes back as it is
+      k_out, v_out   new tensors unless given
+    Rows that belong to no sequence, or lie in front of its first position, are left as they are, uninitialised in new tensors."""
+    who = "paged_load"
+    index, kept = k_cache.get_device(), k_cache.dtype
+    if index < 0 or (kept not in _DTYPES and kept not in _CODES):
+        raise RuntimeError(f"{who}: k_cache must be a CUDA tensor of fp16, bf16, int8 or float8_e4m3fn, got {kept} on {k_cache.device}")
+    shape, strides = _cache(who, k_cache, v_cache, kept, index)
+    codes = _CODES.get(kept, 0)
+    if codes:
+        scales = _scales(who, k_cache, k_scale, v_scale, shape, index)
+    elif k_scale is not None or v_scale is not None:
+        raise RuntimeError(f"{who}: scales belong to a cache of codes, int8 or float8_e4m3fn, not to {kept}")
+    else:
+        scales = _pack_codes(0, 0, 0, 0, 0, 0, 0)
+    if dtype is None:
+        dtype = next((t.dtype for t in (k_out, v_out) if t is not None), torch.float16 if codes else kept)
+    if dtype not in _DTYPES or (not codes and dtype != kept):
+        raise RuntimeError(f"{who}: a cache of {kept} is not read back as {dtype}")
+    if tokens is None:
+        given = next((t for t in (k_out, v_out) if t is not None), None)
+        if given is None:
+            raise RuntimeError(f"{who}: neither tokens nor k_out is given")
+        tokens = given.shape[0]
+    rows = torch.Size((tokens, shape[1], shape[3]))
+    outs, out_strides = [], ()
+    for name, t in (("k_out", k_out), ("v_out", v_out)):
+        if t is None:
+            t = torch.empty(rows, dtype=dtype, device=k_cache.device)
+        out_strides += _heads(who, name, t, rows, dtype, index)
+        outs.append(t)
+    seqs, columns, pages_stride, table = _table(who, pages, starts, lens, index)
+    args = _pack_load(k_cache.data_ptr(), v_cache.data_ptr(), 0 if not codes else k_scale.data_ptr(), 0 if not codes else v_scale.data_ptr(),
+                      outs[0].data_ptr(), outs[1].data_ptr(), *table, tokens, seqs, shape[1], shape[3], codes, dtype == torch.bfloat16,
+                      shape[0], shape[2], columns, pages_stride, *out_strides, *strides) + scales[24:]
+    _call(lib.eet_paged_load, args, index)
+    return outs[0], outs[1]
+
+
 def paged_mha(q, k_cache, v_cache, pages, starts, lens, max_tokens=None, max_len=None, scale=None, window=0, first_key=None,
-              alibi_slopes=None, out=None):
+              alibi_slopes=None, out=None, k_scale=None, v_scale=None):
     """Attention of new tokens q [tokens, heads, head_dim] over the pages, which hold the new tokens' own keys and values already
     (paged_store).  Returns out, the shape of q.
 
@@ -259,13 +336,14 @@ def paged_mha(q, k_cache, v_cache, pages, starts, lens, max_tokens=None, max_len
       window                0: no window
       first_key             int32 [sequences]: positions before it are padding
       alibi_slopes          float32 [heads]: slope * (key position - p) is added to the scores
+      k_scale, v_scale      of caches of codes
     out may be q.  Rows of out that belong to no sequence are left as they are, uninitialised where this call allocated out.
     Slots that no new token sees may hold anything.  What some new token of a sequence sees must be finite: a NaN or infinity in v reaches
     other new tokens of that sequence, too, also those before it."""
     who = "paged_mha"
     shape, dtype, index, q_str = _first(who, "q", q)
     tokens, heads, head_dim = shape
-    cache_shape, cache_strides = _cache(who, k_cache, v_cache, dtype, index)
+    cache_shape, cache_strides = _cache(who, k_cache, v_cache, _kept_type(who, k_cache, dtype, k_scale, v_scale), index)
     if cache_shape[3] != head_dim:
         raise RuntimeError(f"paged_mha: caches of head size {cache_shape[3]} beside a q of {head_dim}")
     seqs, columns, pages_stride, table = _table(who, pages, starts, lens, index)
@@ -278,13 +356,18 @@ def paged_mha(q, k_cache, v_cache, pages, starts, lens, max_tokens=None, max_len
                      cache_shape[1], head_dim, dtype == torch.bfloat16, cache_shape[0], cache_shape[2], columns, pages_stride, *q_str,
                      *o_str, *cache_strides, window, max_tokens, max_len or 0, 1.0 / math.sqrt(head_dim) if scale is None else scale)
     # (how the call is planned, and with it the scratch, goes by sizes and by the device's number of SMs)
-    ws_bytes = _workspace_bytes(args, index)
+    if k_scale is None and v_scale is None:
+        call, size, scales = lib.eet_paged_mha, lib.eet_paged_mha_workspace_bytes, b""
+    else:
+        call, size = lib.eet_paged_mha_codes, lib.eet_paged_mha_codes_workspace_bytes
+        scales = _scales(who, k_cache, k_scale, v_scale, cache_shape, index)
+    ws_bytes = _workspace_bytes(size, args + _NO_SCRATCH + scales, index)
     if ws_bytes:
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
         args += _pack_scratch(ws.data_ptr(), ws_bytes)
     else:
         args += _NO_SCRATCH
-    _call(lib.eet_paged_mha, args, index)
+    _call(call, args + scales, index)
     return out
 
 
@@ -337,7 +420,8 @@ class PagedMmha:
             freqs, magnitude = rotary_frequencies(128, device=desc.device)
         self.freqs, self.interleaved, self.magnitude, self.alibi_slopes = freqs, interleaved, magnitude, alibi_slopes
 
-    def forward(self, input, k_cache, v_cache, pages, starts, lens, max_tokens=None, max_len=None, window=0, first_key=None):
+    def forward(self, input, k_cache, v_cache, pages, starts, lens, max_tokens=None, max_len=None, window=0, first_key=None,
+                k_scale=None, v_scale=None):
         """input fp16 [tokens, hidden]: the new tokens of all sequences behind one another; the other arguments as in paged_mha."""
         d = self.desc
         if input.dtype != torch.float16 or input.get_device() != self.index or input.dim() != 2 or input.shape[1] != d.hidden_units or \
@@ -358,10 +442,10 @@ class PagedMmha:
             _linear(xn, self.qkv_w, self.qkv_s, qkv)
             q, k, v = qkv.view(n, -1, 128).split((self.heads, self.kv_heads, self.kv_heads), 1)
             q = paged_store(k, v, k_cache, v_cache, pages, starts, lens, q=q, freqs=self.freqs, interleaved=self.interleaved,
-                            magnitude=self.magnitude, q_out=q)
+                            magnitude=self.magnitude, q_out=q, k_scale=k_scale, v_scale=v_scale)
             # (rows that belong to no sequence go through the block like the others and mean nothing)
             paged_mha(q, k_cache, v_cache, pages, starts, lens, max_tokens=max_tokens, max_len=max_len, window=window,
-                      first_key=first_key, alibi_slopes=self.alibi_slopes, out=ctx)
+                      first_key=first_key, alibi_slopes=self.alibi_slopes, out=ctx, k_scale=k_scale, v_scale=v_scale)
             _linear(ctx.view(n, self.inner_dim), self.out_w, self.out_s, out, residual=input)
         return out.view(n, d.hidden_units)
 

@@ -383,6 +383,38 @@ typedef struct {
  * Stands beside: eet_qkv_split_store, which does this for contiguous caches and prompts from position 0. */
 int eet_paged_store(const eet_paged_store_args* args, void* stream);
 
+/* Caches of 8-bit codes: k and v are codes of one byte, [pages][kv_heads][page_size][head_dim] as above, and a value is its code times
+ * the scale of its row of head_dim, float [pages][kv_heads][page_size] with consecutive slots behind one another.
+ *   codes 1   int8, -127 .. 127, scale = max |y| / 127
+ *   codes 2   e4m3 (1 sign, 4 exponent, 3 mantissa bits), up to 448, scale = max |y| / 448
+ * Strides of codes are in bytes and multiples of 16, those of scales in elements.  Scales are positive; of a row with a NaN or an infinity it is
+ * NaN. */
+typedef struct {
+    eet_paged_store_args store;             /* k_cache and v_cache are the codes */
+    float *k_scale, *v_scale;
+    int64_t codes;
+    int64_t ks_page, ks_head, vs_page, vs_head;
+} eet_paged_store_codes_args;
+
+/* eet_paged_store into such a cache: k behind its rotation in fp32 and v are divided by their scale and rounded once, to nearest, ties to even. */
+int eet_paged_store_codes(const eet_paged_store_codes_args* args, void* stream);
+
+typedef struct {
+    const void *k_cache, *v_cache;
+    const float *k_scale, *v_scale;         /* not read with codes = 0 */
+    void *k_out, *v_out;                    /* [tokens][kv_heads][head_dim], fp16 or bf16 */
+    const int32_t *pages, *starts, *lens;   /* as above: rows [starts[b], starts[b + 1]) are the last positions of sequence b */
+    int64_t tokens, seqs, kv_heads, head_dim, codes, bf16;   /* codes 0: the cache holds values of k_out's type */
+    int64_t num_pages, page_size, max_pages, pages_stride;
+    int64_t ko_tok, ko_head, vo_tok, vo_head;
+    int64_t kc_page, kc_head, kc_slot, vc_page, vc_head, vc_slot;
+    int64_t ks_page, ks_head, vs_page, vs_head;
+} eet_paged_load_args;
+
+/* Reads rows back from a cache, the mirror of the two calls above: starts = 0, lens[0], lens[0] + lens[1], ... gives whole histories.
+ * Rows that belong to no sequence or lie in front of its first position are left alone; those of a page outside the cache are zeros (status 6). */
+int eet_paged_load(const eet_paged_load_args* args, void* stream);
+
 typedef struct {
     const void *q, *k_cache, *v_cache;      /* q [tokens][heads][head_dim] */
     void* out;                              /* [tokens][heads][head_dim] */
@@ -412,6 +444,19 @@ size_t eet_paged_mha_workspace_bytes(const eet_paged_mha_args* args);
  * Stands beside: eet_prefill_mha and eet_decode_mha (csrc/op/llama_mmha.cpp:354-426, csrc/core/attention_dispatch.cu:140-324).
  */
 int eet_paged_mha(const eet_paged_mha_args* args, void* stream);
+
+typedef struct {
+    eet_paged_mha_args mha;                 /* k_cache and v_cache are the codes */
+    const float *k_scale, *v_scale;
+    int64_t codes;
+    int64_t ks_page, ks_head, vs_page, vs_head;
+} eet_paged_mha_codes_args;
+
+size_t eet_paged_mha_codes_workspace_bytes(const eet_paged_mha_codes_args* args);
+
+/* eet_paged_mha over a cache of 8-bit codes.  The codes enter the products exactly, as fp16, for q of either type; the weights p_j s^v_j are
+ * rounded to fp16. */
+int eet_paged_mha_codes(const eet_paged_mha_codes_args* args, void* stream);
 
 #ifdef __cplusplus
 }

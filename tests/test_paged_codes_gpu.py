@@ -1,0 +1,241 @@
+"""A paged cache of 8-bit codes against a plain restatement in 64 bits (codes_util), through the Python calls."""
+import itertools
+import math
+
+import pytest
+import torch
+
+from codes_util import CODES, MOST, CodesBatch, attend_codes64, half_step, quantize64
+from paged_util import HALF_STEP, Batch, rotate64, rotate_tolerance
+
+pytestmark = pytest.mark.gpu
+
+FP16, BF16, INT8, E4M3 = torch.float16, torch.bfloat16, torch.int8, torch.float8_e4m3fn
+
+
+def _paged():
+    from eet_b200 import paged
+    return paged
+
+
+def _status():
+    from eet_b200 import _lib
+    return _lib.device_status()
+
+
+def _within(got, ref, tol, what=""):
+    off = (got.double().cpu() - ref).abs() - tol
+    assert not torch.isnan(off).any(), what
+    assert (off <= 0).all(), f"{what} {off.max().item():.3g} beyond the tolerance at {int(off.argmax())}"
+
+
+def _slots(batch, b, t):
+    p = torch.arange(batch.lens_list[b] - t, batch.lens_list[b])
+    return batch.pages[b].long()[p // batch.page], p % batch.page
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# append
+# ---------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("new,lens,page", [
+    ([1], [1], 16), ([1, 1, 1], [5, 16, 17], 16), ([3, 0, 20, 1], [3, 40, 33, 64], 32), ([130], [257], 64), ([0, 0], [3, 0], 16),
+    ([5, 2], [300, 2], 256), ([1] * 300, [1 + i % 50 for i in range(300)], 16)])
+@pytest.mark.parametrize("dtype,head_dim,interleaved,rotary_dim", [(FP16, 128, False, 128), (BF16, 64, True, 32), (BF16, 128, False, 64),
+                                                                   (FP16, 64, False, 0)])
+@pytest.mark.parametrize("kind", CODES)
+def test_store(new, lens, page, dtype, head_dim, interleaved, rotary_dim, kind):
+    batch = CodesBatch(new, lens, 6, 2, head_dim, page, dtype, kind, behind=2)
+    kc, vc, pages, starts, n = batch.gpu()
+    scales = batch.scales()
+    freqs = _paged().rotary_frequencies(rotary_dim, device="cpu")[0] if rotary_dim else None
+    out = torch.full_like(batch.q, 7.0).cuda()
+    got = _paged().paged_store(batch.k.cuda(), batch.v.cuda(), kc, vc, pages, starts, n, q=batch.q.cuda(), interleaved=interleaved,
+                               freqs=None if freqs is None else freqs.cuda(), q_out=out, **scales)
+    assert got is out
+    total, positions = sum(new), batch.positions()
+    k64, k_off = batch.k[:total].double(), torch.zeros(total, 2, head_dim, dtype=torch.float64)
+    q64, q_off = batch.q[:total].double(), torch.zeros_like(batch.q[:total], dtype=torch.float64)
+    if rotary_dim:
+        q64, k64 = (rotate64(x[:total], positions, freqs, interleaved) for x in (batch.q, batch.k))
+        q_off, k_off = (rotate_tolerance(x[:total], freqs, interleaved, dtype) for x in (batch.q, batch.k))
+        q_off += HALF_STEP[dtype] * q64.abs() + 2.0 ** -25
+    _within(out[:total], q64, q_off)
+    assert (out[total:] == 7.0).all(), "rows behind the last sequence"
+    kc, vc, ks, vs = kc.cpu(), vc.cpu(), scales["k_scale"].cpu(), scales["v_scale"].cpu()
+    v_codes, v_scale = quantize64(batch.v[:total], kind)
+    at = 0
+    for b, t in enumerate(new):
+        page_of, slot = _slots(batch, b, t)
+        rows = slice(at, at + t)
+        # v goes in as it is: its scale and codes are known to the bit
+        assert torch.equal(vs[page_of, :, slot], v_scale[rows])
+        assert torch.equal(vc.view(torch.uint8)[page_of, :, slot], v_codes[rows].view(torch.uint8))
+        # k: the scale is that of the rotated values, which are off by k_off; the codes stand for them to half a step of the scale used
+        scale = ks[page_of, :, slot]
+        if t:
+            top = k64[rows].abs().amax(-1)
+            assert ((scale.double() * MOST[kind] - top).abs() <= k_off[rows].amax(-1) + 2.0 ** -23 * top).all()
+        value = kc.float()[page_of, :, slot].double() * scale.double()[..., None]
+        _within(value, k64[rows], half_step(k64[rows], scale, kind) * (1 + 2.0 ** -20) + 2 * k_off[rows])
+        for held, was in ((kc, batch.k_cache), (vc, batch.v_cache), (ks, batch.k_scale), (vs, batch.v_scale)):
+            held.view(torch.uint8 if held.dtype in CODES else held.dtype)[page_of, :, slot] = \
+                was.view(torch.uint8 if was.dtype in CODES else was.dtype)[page_of, :, slot]
+        at += t
+    # every other slot holds what it held
+    assert torch.equal(kc.view(torch.uint8), batch.k_cache.view(torch.uint8)) and torch.equal(ks, batch.k_scale)
+    assert torch.equal(vc.view(torch.uint8), batch.v_cache.view(torch.uint8)) and torch.equal(vs, batch.v_scale)
+    assert _status() == 0
+
+
+@pytest.mark.parametrize("kind", CODES)
+@pytest.mark.parametrize("dtype", [FP16, BF16])
+def test_store_of_rows_on_the_border_of_two_codes(kind, dtype):
+    """Small whole numbers under a scale made from one of them: many quotients lie on a border, and must go to the even code, many beside it."""
+    gen = torch.Generator().manual_seed(3)
+    batch = CodesBatch([400], [400], 2, 2, 128, 16, dtype, kind)
+    v = torch.randint(-254, 255, (400, 2, 128), generator=gen).float()
+    v[:, :, 5] = 254.0 if kind == INT8 else 448.0
+    v[:100] *= 2.0 ** -12
+    v[100:150, 1] = 0.0
+    v[150:200] = torch.randint(-3, 4, (50, 2, 128), generator=gen).float() * 2.0 ** -24
+    batch.v = v.to(dtype)
+    kc, vc, *table = batch.gpu()
+    scales = batch.scales()
+    _paged().paged_store(batch.v.cuda(), batch.v.cuda(), kc, vc, *table, **scales)
+    codes, scale = quantize64(batch.v, kind)
+    page_of, slot = _slots(batch, 0, 400)
+    for cache, s in ((kc, scales["k_scale"]), (vc, scales["v_scale"])):
+        assert torch.equal(s.cpu()[page_of, :, slot], scale)
+        assert torch.equal(cache.cpu().view(torch.uint8)[page_of, :, slot] & 127, codes.view(torch.uint8) & 127)
+        assert torch.equal(cache.cpu().float()[page_of, :, slot], codes.float())
+
+
+@pytest.mark.parametrize("kind", CODES)
+def test_store_of_what_has_no_codes(kind):
+    """A row with a NaN or an infinity reads back as NaN, its neighbours are kept; the largest and smallest values are, too."""
+    batch = CodesBatch([7], [7], 2, 2, 128, 16, BF16, kind)
+    v = batch.v.clone()
+    v[0, 0, 3], v[1, 1, 127], v[2, 0, 0] = math.nan, math.inf, -math.inf
+    v[3], v[4] = 3.3e38, 1e-38
+    v[5, 0, 1:] = 0.0
+    kc, vc, *table = batch.gpu()
+    scales = batch.scales()
+    _paged().paged_store(v.cuda(), v.cuda(), kc, vc, *table, **scales)
+    k, back = _paged().paged_load(kc, vc, *table, 7, dtype=BF16, **scales)
+    assert torch.equal(k.isnan(), back.isnan())
+    lost = torch.zeros(7, 2, dtype=torch.bool)
+    lost[0, 0] = lost[1, 1] = lost[2, 0] = True
+    assert back.isnan().cpu().all(-1).equal(lost) and back.isnan().cpu().any(-1).equal(lost)
+    ok = ~lost
+    scale = scales["v_scale"].cpu()[_slots(batch, 0, 7)[0], :, _slots(batch, 0, 7)[1]]
+    tol = half_step(v, scale, kind) + 2.0 ** -8 * v.double().abs()
+    _within(back.cpu()[ok], v.double()[ok], tol[ok] * (1 + 2.0 ** -20))
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# reading back
+# ---------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("new,lens,page", [
+    ([1], [1], 16), ([300], [300], 16), ([3, 0, 20, 1], [3, 40, 33, 64], 32), ([7, 600, 0, 1], [7, 601, 5, 900], 64), ([0, 0], [3, 0], 16),
+    ([255, 2], [700, 2], 256), ([2] * 100, [2 + i % 50 for i in range(100)], 128)])
+@pytest.mark.parametrize("kind", CODES + (None,))
+@pytest.mark.parametrize("dtype,head_dim,kv_heads", [(FP16, 128, 2), (BF16, 64, 3)])
+def test_load(new, lens, page, kind, dtype, head_dim, kv_heads):
+    batch = Batch(new, lens, kv_heads, kv_heads, head_dim, page, dtype) if kind is None else \
+        CodesBatch(new, lens, kv_heads, kv_heads, head_dim, page, dtype, kind)
+    total = sum(new)
+    cache = [t.cuda() for t in (batch.k_cache, batch.v_cache, batch.pages, batch.starts, batch.lens)]
+    scales = {} if kind is None else batch.scales()
+    outs = [torch.full((total + 2, kv_heads, head_dim), 7.0, dtype=dtype, device="cuda") for _ in range(2)]
+    got = _paged().paged_load(*cache, k_out=outs[0], v_out=outs[1], **scales)
+    assert got[0] is outs[0] and got[1] is outs[1]
+    for w, y in zip("kv", outs):
+        at = 0
+        for b, t in enumerate(new):
+            if kind is None:
+                want = batch.history(getattr(batch, w + "_cache"), b)[lens[b] - t:]
+                assert torch.equal(y[at:at + t].cpu(), want)
+            else:
+                want = batch.values(w, b)[lens[b] - t:]
+                # (code times scale in fp32 and one rounding)
+                _within(y[at:at + t], want, (HALF_STEP[dtype] + 2.0 ** -23) * want.abs() + 2.0 ** -25)
+            at += t
+        assert (y[total:] == 7.0).all(), "rows behind the last sequence"
+    fresh = _paged().paged_load(*cache, total, dtype=dtype, **scales)
+    assert all(torch.equal(x, y[:total]) for x, y in zip(fresh, outs))
+    assert _status() == 0
+
+
+def test_load_of_missing_pages_and_positions():
+    batch = CodesBatch([4, 6], [40, 3], 2, 2)
+    batch.pages[0, 2] = 10 ** 6
+    cache, scales = batch.gpu(), batch.scales()
+    out = [torch.full((10, 2, 128), 7.0, dtype=FP16, device="cuda") for _ in range(2)]
+    _paged().paged_load(*cache, k_out=out[0], v_out=out[1], **scales)
+    assert _status() == 6
+    for w, y in zip("kv", out):
+        assert (y[:4] == 0).all(), "a page outside the cache"
+        assert (y[4:7] == 7.0).all(), "in front of the first position"
+        _within(y[7:], batch.values(w, 1), 2.0 ** -11 * batch.values(w, 1).abs() * 1.01 + 2.0 ** -25)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------------------------------------------------
+def _check(batch, what="", **options):
+    given = {w: (x.cuda() if torch.is_tensor(x) else x) for w, x in options.items()}
+    total = sum(batch.new)
+    out = torch.full_like(batch.q, 7.0).cuda()
+    got = _paged().paged_mha(batch.q.cuda(), *batch.gpu(), out=out, **batch.scales(), **given)
+    assert got is out
+    plain = {w: x for w, x in options.items() if w in ("scale", "window", "first_key", "alibi_slopes")}
+    ref, tol = attend_codes64(batch, **plain)
+    _within(out[:total], ref, tol, what)
+    assert (out[total:] == 7.0).all(), "rows behind the last sequence"
+    assert _status() == 0
+
+
+ROWS = [([1], [1]), ([1], [300]), ([1, 1, 1], [5, 128, 129]), ([1] * 40, [1 + 37 * i % 400 for i in range(40)]), ([2, 0, 1], [2, 50, 1000]),
+        ([1], [5000]), ([4, 3], [700, 1300])]
+
+
+@pytest.mark.parametrize("new,lens", ROWS)
+@pytest.mark.parametrize("heads,kv_heads,head_dim,page", [(4, 4, 128, 16), (8, 2, 128, 64), (8, 1, 64, 16), (16, 1, 128, 32), (6, 2, 64, 256)])
+@pytest.mark.parametrize("kind,dtype", itertools.product(CODES, (FP16, BF16)))
+def test_mha_few_rows(new, lens, heads, kv_heads, head_dim, page, kind, dtype):
+    batch = CodesBatch(new, lens, heads, kv_heads, head_dim, page, dtype, kind, behind=1)
+    batch.poison()
+    _check(batch, max_tokens=max(new))
+
+
+@pytest.mark.parametrize("kind", CODES)
+@pytest.mark.parametrize("options", [dict(window=1), dict(window=100), dict(first=True), dict(alibi=True), dict(window=33, first=True, alibi=True),
+                                     dict(scale=0.3), dict(scale=-0.1), dict(scale=0.0)])
+def test_mha_few_rows_options(kind, options):
+    lens = [3, 200, 517, 1]
+    batch = CodesBatch([1, 2, 1, 1], lens, 8, 4, 128, 16, FP16, kind)
+    batch.poison()
+    options = dict(options)
+    if options.pop("first", False):
+        options["first_key"] = torch.tensor([3, 150, 0, 1], dtype=torch.int32)      # the first and last sequences see nothing
+    if options.pop("alibi", False):
+        options["alibi_slopes"] = torch.tensor([2.0 ** -i for i in range(1, 9)])
+    _check(batch, max_tokens=2, **options)
+
+
+@pytest.mark.parametrize("kind", CODES)
+@pytest.mark.parametrize("spread", [0.0, 6.0, 13.0])
+def test_mha_scales_of_very_different_sizes(kind, spread):
+    """Rows of the cache that differ by up to 2^26 in size; q so small that all keys count."""
+    batch = CodesBatch([1, 1], [900, 40], 4, 4, 128, 16, BF16, kind, spread=spread, q_scale=0.01)
+    _check(batch, max_tokens=1)
+
+
+def test_mha_is_the_same_whatever_the_hints():
+    batch = CodesBatch([1, 3, 1], [700, 1500, 90], 8, 4, 128, 32)
+    runs = [_paged().paged_mha(batch.q.cuda(), *batch.gpu(), **batch.scales(), **hint)
+            for hint in (dict(max_tokens=3, max_len=1500), dict(max_tokens=3, max_len=1500), dict(), dict(max_tokens=1, max_len=1))]
+    assert torch.equal(runs[0], runs[1])
+    ref, tol = attend_codes64(batch)
+    for r in runs:
+        _within(r, ref, tol)
