@@ -18,6 +18,7 @@ CUDA graph (eet_b200.modeling).
 import ctypes
 import functools
 import math
+import struct
 
 import torch
 
@@ -373,6 +374,56 @@ def argmax_rows(logits2d):
     check(lib.eet_argmax_rows(logits2d.data_ptr(), out.data_ptr(), rows, n, logits2d.stride(0) if rows > 1 else n,
                               _stream()))
     return out
+
+
+_pack_sample = struct.Struct("8P5q3d").pack
+_LOGIT_TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+
+
+def _sample_setting(name, value, dtype, rows, index, low, high):
+    """(address of one a row, or 0; the number for all rows) of a setting of sample_rows."""
+    if not torch.is_tensor(value):
+        if not low <= value <= high or (dtype == torch.int32 and value != int(value)):
+            raise RuntimeError(f"sample_rows: {name} {value!r} is not {'a whole number ' if dtype == torch.int32 else ''}within {low} .. {high}")
+        return 0, value
+    if value.dtype != dtype or value.get_device() != index or value.shape != (rows,) or not value.is_contiguous():
+        raise RuntimeError(f"sample_rows: {name} must be a number or a contiguous {dtype} tensor [{rows}] on cuda:{index}, got "
+                           f"{tuple(value.shape)} {value.dtype} on {value.device}")
+    return value.data_ptr(), 0
+
+
+def sample_rows(logits2d, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """Draws the next token of each row of a CUDA fp16, bf16 or fp32 matrix of logits (rows may be strided): returns (tokens int64
+    [rows], logprobs float32 [rows]), logprobs being ln of the probability with which the token was drawn.
+
+      uniform       float32 [rows] in [0, 1), from the caller's generator: the same numbers give the same tokens
+      temperature   of exp(logit / temperature); 0: the largest logit, the smallest index on ties, as argmax_rows
+      top_k         the so many largest logits stay, the smallest index first on ties; 0: all
+      top_p         of those, the most probable ones in front of which stands a probability below top_p; 1: all
+      min_p         of those, the ones with at least min_p times the largest probability; 0: all
+    Each setting is a number, or a tensor of one a row on the device (float32, top_k int32), which a captured call reads again when it is
+    replayed.  The largest logit always stays.  Of what stays, laid out in the order of the indices, the token is drawn in which the
+    share `uniform` of the sum of probabilities lies.  NaN counts as -inf; a row without a logit above -inf gives -1 and -inf."""
+    if logits2d.dim() != 2 or logits2d.dtype not in _LOGIT_TYPES or not logits2d.is_cuda or logits2d.stride(1) != 1:
+        raise RuntimeError(f"sample_rows: a CUDA fp16, bf16 or fp32 matrix with contiguous rows is required, got {tuple(logits2d.shape)} "
+                           f"{logits2d.dtype} on {logits2d.device}")
+    rows, n = logits2d.shape
+    index = logits2d.get_device()
+    if uniform.dtype != torch.float32 or uniform.get_device() != index or uniform.shape != (rows,) or not uniform.is_contiguous():
+        raise RuntimeError(f"sample_rows: uniform must be a contiguous float32 tensor [{rows}] on cuda:{index}, got {tuple(uniform.shape)} "
+                           f"{uniform.dtype} on {uniform.device}")
+    inf = float("inf")
+    t, temperature = _sample_setting("temperature", temperature, torch.float32, rows, index, 0.0, inf)
+    k, top_k = _sample_setting("top_k", top_k, torch.int32, rows, index, 0, 2 ** 31 - 1)
+    p, top_p = _sample_setting("top_p", top_p, torch.float32, rows, index, 0.0, 1.0)
+    m, min_p = _sample_setting("min_p", min_p, torch.float32, rows, index, 0.0, 1.0)
+    tokens = torch.empty(rows, dtype=torch.int64, device=logits2d.device)
+    logprobs = torch.empty(rows, dtype=torch.float32, device=logits2d.device)
+    args = _pack_sample(logits2d.data_ptr(), uniform.data_ptr(), t, p, m, k, tokens.data_ptr(), logprobs.data_ptr(), rows, n,
+                        _LOGIT_TYPES[logits2d.dtype], logits2d.stride(0) if rows > 1 else n, int(top_k), temperature, top_p, min_p)
+    with _on(logits2d.device):
+        check(lib.eet_sample_rows(args, _stream()))
+    return tokens, logprobs
 
 
 def gather_rows(table, ids, out=None):

@@ -60,6 +60,7 @@ static inline bool aligned16(const void* p)
 #include "paged.cu"
 #include "paged_codes.cu"
 #include "quantize.cu"
+#include "sample.cu"
 
 using namespace eet;
 
@@ -587,6 +588,25 @@ int eet_gather_rows(const void* table, const int64_t* ids, void* out, int rows, 
     EET_CHECK(rows >= 0 && n > 0 && rows_in_table > 0 && (rows == 0 || (table && ids && out)), "eet_gather_rows: bad arguments");
     EET_CHECK(aligned16(table) && aligned16(out), "eet_gather_rows: pointers must be 16-byte aligned");
     return launch_gather_rows((const __half*)table, ids, (__half*)out, rows, n, rows_in_table, (cudaStream_t)stream);
+}
+
+int eet_sample_rows(const eet_sample_rows_args* p, void* stream)
+{
+    EET_CHECK(p != nullptr, "eet_sample_rows: args is NULL");
+    EET_CHECK(p->rows >= 0 && p->rows <= INT32_MAX / kSaMaxCluster, "eet_sample_rows: bad number of rows");
+    EET_CHECK(p->vocab > 0 && p->vocab <= kSaMaxVocab, "eet_sample_rows: %lld tokens, only 1 to %d are supported", (long long)p->vocab, kSaMaxVocab);
+    EET_CHECK(p->type >= 0 && p->type <= 2, "eet_sample_rows: unknown type %lld", (long long)p->type);
+    EET_CHECK(p->row_stride >= p->vocab || p->rows <= 1, "eet_sample_rows: rows overlap");
+    EET_CHECK(p->top_k >= 0 && p->top_k <= INT32_MAX, "eet_sample_rows: top_k must not be negative");
+    if (p->rows == 0) return 0;
+    EET_CHECK(p->logits && p->uniform && p->tokens && p->logprobs, "eet_sample_rows: NULL argument");
+    EET_CHECK(((uintptr_t)p->logits & (p->type == 2 ? 3 : 1)) == 0, "eet_sample_rows: logits are not aligned to their type");
+    SampleArgs a = {};
+    a.logits = p->logits, a.uniform = p->uniform, a.temperatures = p->temperatures, a.top_ps = p->top_ps, a.min_ps = p->min_ps;
+    a.top_ks = p->top_ks, a.tokens = (long long*)p->tokens, a.logprobs = p->logprobs;
+    a.rows = (int)p->rows, a.vocab = (int)p->vocab, a.type = (int)p->type, a.row_stride = p->row_stride;
+    a.temperature = (float)p->temperature, a.top_p = (float)p->top_p, a.min_p = (float)p->min_p, a.top_k = (int)p->top_k;
+    return launch_sample(a, (cudaStream_t)stream);
 }
 
 // ---- serving from a paged cache -----------------------------------------------------------------------------------------

@@ -204,4 +204,18 @@ int launch_paged_mha(const PagedMhaArgs& a, cudaStream_t stream);
 size_t paged_mha_codes_workspace_bytes(const PagedMhaArgs& a);
 int launch_paged_mha_codes(const PagedMhaArgs& a, cudaStream_t stream);
 
+// sample.cu
+struct SampleArgs {
+    const void* logits;
+    const float *uniform, *temperatures, *top_ps, *min_ps;
+    const int* top_ks;
+    long long* tokens;
+    float* logprobs;
+    int rows, vocab, type;                       // type 0 fp16, 1 bf16, 2 fp32
+    long long row_stride;
+    float temperature, top_p, min_p;             // where there are none a row
+    int top_k;
+};
+int launch_sample(const SampleArgs& a, cudaStream_t stream);
+
 }  // namespace eet

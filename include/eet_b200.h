@@ -324,6 +324,29 @@ int eet_argmax_rows(const void* logits, int64_t* out, int rows, int n, size_t ro
 int eet_lm_head_argmax(float* sums, const void* scale, int M, int n_local, int64_t col_offset, void* const* peer_inbox,
                        int world, int rank, int* epochs, int64_t* out_ids, void* logits_out, void* stream);
 
+typedef struct {
+    const void* logits;                     /* [rows][vocab], rows row_stride elements apart */
+    const float* uniform;                   /* [rows], in [0, 1) */
+    const float *temperatures, *top_ps, *min_ps;   /* [rows], or NULL: the same for all, below */
+    const int32_t* top_ks;
+    int64_t* tokens;                        /* [rows] */
+    float* logprobs;                        /* [rows] */
+    int64_t rows, vocab, type, row_stride;  /* type 0 fp16, 1 bf16, 2 fp32; vocab up to 2^18 */
+    int64_t top_k;                          /* 0, or as many as there are tokens: all */
+    double temperature, top_p, min_p;       /* temperature 0: the largest; top_p 1 and min_p 0: all */
+} eet_sample_rows_args;
+
+/*
+ * Draws a token for each row.  With w_i = exp((x_i - max x) / temperature), and tokens in the order of x from the largest, the lowest index
+ * first among equals: top_k leaves the first top_k; top_p of those the ones in front of which stands a sum of w below top_p of the sum of the top_k;
+ * min_p those with w >= min_p; the first always stays.  Among what is left, in the order of the indices, the first token whose running
+ * sum of w exceeds uniform times the sum of all is drawn, and logprobs is ln of its share of that sum.
+ * NaN counts as -inf; a row without a token above -inf gives -1 and -inf.  A temperature that is not above 0 gives the first token and 0; per
+ * row, a top_k below 1, a top_p not below 1 and a min_p not above 0 leave all.  No scratch; the same answer whatever else runs.
+ * Stands beside: eet_argmax_rows.
+ */
+int eet_sample_rows(const eet_sample_rows_args* args, void* stream);
+
 /* out[r][0..n) = table[ids[r]][0..n), fp16, n a multiple of 8, ids device int64 (an id outside
  * [0, rows_in_table) reads row 0): the token-embedding lookup, torch.nn.Embedding in the reference
  * (python/eet/transformers/modeling_llama.py:281-283). */
