@@ -21,6 +21,8 @@
 //
 // A CTA is four warps, 32 keys of a block each; two CTAs share an SM, so that the beginning and the end of a piece of one run beside the
 // other's blocks.  The warps' sums meet in shared memory at the end of a piece.  The work is cut up as paged_share.cuh says.
+#include <type_traits>
+
 #include "codes.cuh"
 #include "paged_share.cuh"
 
@@ -516,49 +518,83 @@ int pc_launch(const PagedMhaArgs& a, void* ws, int most, int whole, cudaStream_t
 
 }  // namespace
 
+// Which kernels serve a call, as in paged_plan: sequences of up to `few` tokens go to the tiles of 8 or 16 rows, the others to those of 128.
 struct PagedCodesPlan {
-    int rows;            // of a tile: 8 or 16
-    bool whole;
-    size_t bytes;
+    int rows;            // of a tile of the first kind: 8 or 16; 0: none
+    bool tiles;
+    int few;
+    size_t bytes[2];     // scratch
 };
 
 static PagedCodesPlan paged_codes_plan(const PagedMhaArgs& a)
 {
     PagedCodesPlan p = {};
     const int group = a.heads / a.kv_heads;
-    p.rows = (long long)a.max_tokens * group <= 8 ? 8 : 16;
-    p.whole = false;
-    p.bytes = pg_scratch_bytes(kPcPerSm * sm_count(), p.rows, a.head_dim);
+    auto is_few = [&](long long tokens) { return (tokens > 0 ? tokens : 1) * group <= 16; };
+    p.tiles = !is_few(a.max_tokens);
+    p.few = 0x7fffffff;
+    if (!p.tiles) {
+        p.rows = (long long)a.max_tokens * group <= 8 ? 8 : 16;
+    }
+    else if (group <= 16) {
+        // few tokens each beside the longest, and something to read for them?
+        const long long others = a.seqs - 1, rest = a.tokens - a.max_tokens;
+        if (others > 0 && is_few((rest + others - 1) / others) && others * a.kv_heads * (a.max_len / kPgKeys + 1) >= 1024) {
+            p.rows = (rest + others - 1) / others * group <= 8 ? 8 : 16;
+            p.few = p.rows / group;
+        }
+    }
+    if (p.rows) p.bytes[0] = pg_scratch_bytes(kPcPerSm * sm_count(), p.rows, a.head_dim);
+    if (p.tiles) p.bytes[1] = pg_scratch_bytes(sm_count(), 2 * kPgRows, a.head_dim);
     return p;
 }
 
 size_t paged_mha_codes_workspace_bytes(const PagedMhaArgs& a)
 {
-    return paged_codes_plan(a).bytes;
+    const PagedCodesPlan p = paged_codes_plan(a);
+    return p.bytes[0] + p.bytes[1];
 }
 
-template<int kCodes, int D>
+template<typename T, int D, int kCodes>
 static int launch_paged_mha_codes_t(const PagedMhaArgs& a, const PagedCodesPlan& p, cudaStream_t stream)
 {
-    const int rc = p.rows == 8 ? pc_launch<kCodes, D, 8>(a, a.ws, 0x7fffffff, p.whole, stream)
-                               : pc_launch<kCodes, D, 16>(a, a.ws, 0x7fffffff, p.whole, stream);
-    if (rc || p.whole) return rc;
-    const PgScratch s = {a.ws, p.rows, 0}, none = {};
-    const int y = (p.rows * (D / 8) + kPgJoinThreads - 1) / kPgJoinThreads;
-    const dim3 grid(kPcPerSm * sm_count(), y, 1);
-    if (a.bf16) EET_CUDA(launch_pdl(paged_mha_join_kernel<__nv_bfloat16, D>, grid, dim3(kPgJoinThreads), 0, stream, a, s, none));
-    else EET_CUDA(launch_pdl(paged_mha_join_kernel<__half, D>, grid, dim3(kPgJoinThreads), 0, stream, a, s, none));
+    void* ws[2] = {a.ws, (char*)a.ws + p.bytes[0]};
+    auto join = [&](const PgScratch& s, int ctas) -> int {
+        const PgScratch none = {};
+        const long long rows = (long long)a.max_tokens * (a.heads / a.kv_heads);
+        const int y = (int)((rows < s.rows ? rows : s.rows) * (D / 8) + kPgJoinThreads - 1) / kPgJoinThreads;   // 8 dims a thread
+        EET_CUDA(launch_pdl(paged_mha_join_kernel<T, D>, dim3(ctas, y, 1), dim3(kPgJoinThreads), 0, stream, a, s, none));
+        return 0;
+    };
+    if (p.rows) {
+        const int most = p.tiles ? p.few : 0x7fffffff;
+        if (int rc = p.rows == 8 ? pc_launch<kCodes, D, 8>(a, ws[0], most, 0, stream) : pc_launch<kCodes, D, 16>(a, ws[0], most, 0, stream)) return rc;
+        if (int rc = join({ws[0], p.rows, 0}, kPcPerSm * sm_count())) return rc;
+    }
+    if (p.tiles) {
+        // (the tiles without a bias take the maximum of the scores before the scale, which a negative one would turn round)
+        const bool bias = a.slopes != nullptr || !(a.scale > 0.f);
+        const int least = p.rows ? p.few + 1 : 1;
+        if (int rc = bias ? pg_launch_tc_codes<T, D, true, kCodes>(a, ws[1], least, 0, stream)
+                          : pg_launch_tc_codes<T, D, false, kCodes>(a, ws[1], least, 0, stream)) return rc;
+        if (int rc = join({ws[1], 2 * kPgRows, 1}, sm_count())) return rc;
+    }
     return 0;
 }
 
 int launch_paged_mha_codes(const PagedMhaArgs& a, cudaStream_t stream)
 {
     const PagedCodesPlan p = paged_codes_plan(a);
-    EET_CHECK(a.heads / a.kv_heads <= 16, "eet_paged_mha_codes: more than 16 query heads to a kv head");
-    if (a.codes == kCodesInt8) {
-        return a.head_dim == 128 ? launch_paged_mha_codes_t<kCodesInt8, 128>(a, p, stream) : launch_paged_mha_codes_t<kCodesInt8, 64>(a, p, stream);
-    }
-    return a.head_dim == 128 ? launch_paged_mha_codes_t<kCodesE4M3, 128>(a, p, stream) : launch_paged_mha_codes_t<kCodesE4M3, 64>(a, p, stream);
+    auto launch = [&](auto codes) -> int {
+        constexpr int kCodes = decltype(codes)::value;
+        if (a.bf16) {
+            return a.head_dim == 128 ? launch_paged_mha_codes_t<__nv_bfloat16, 128, kCodes>(a, p, stream)
+                                     : launch_paged_mha_codes_t<__nv_bfloat16, 64, kCodes>(a, p, stream);
+        }
+        return a.head_dim == 128 ? launch_paged_mha_codes_t<__half, 128, kCodes>(a, p, stream)
+                                 : launch_paged_mha_codes_t<__half, 64, kCodes>(a, p, stream);
+    };
+    return a.codes == kCodesInt8 ? launch(std::integral_constant<int, kCodesInt8>()) : launch(std::integral_constant<int, kCodesE4M3>());
 }
 
 }  // namespace eet

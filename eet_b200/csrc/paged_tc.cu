@@ -23,6 +23,13 @@
 //   warp 9          one thread issues S = Q.K^T and O += P.V (P from tensor memory, V as MN-major operand)
 // Keys outside of what any row of the pair sees may be anything, even NaN (slots behind the end of a sequence): their scores are
 // masked by selection and their rows of V are set to zero in shared memory before the product reads them.
+//
+// Over a cache of 8-bit codes four more warps (12-15, a warpgroup of their own) put K and V into the ring: each reads its 32 keys of an entry
+// into registers, one entry ahead, multiplies the codes with the scale of their row in fp32, rounds once to q's type and writes that
+// where the copy engine would have put it; the rest of the kernel does not know.  (The scales could stay outside the products as in
+// paged_codes.cu, two multiplications and two reads of shared memory more for every score: the softmax is the bound here, and these warps
+// have time.)  512 threads of 128 registers are launched, of which the softmax takes 144 and the others 112.
+#include "codes.cuh"
 #include "paged_share.cuh"
 
 namespace eet {
@@ -30,6 +37,7 @@ namespace eet {
 namespace {
 
 constexpr int kPgThreads = 320;
+constexpr int kPgCodesThreads = 512;    // with the warps that convert codes
 constexpr int kPgStages = 5;
 constexpr int kPgExtra = 3;             // a tile's beginning and end cost as much as three blocks
 constexpr uint32_t kPgTmemCols = 512;   // S of a, S of b (their probabilities over them), O of a, O of b: 128 each
@@ -110,13 +118,13 @@ __device__ __forceinline__ PgTurns pg_turns(const PagedMhaArgs& a, const PgPiece
     return r;
 }
 
-// By one thread, in front of a barrier.
-__device__ __forceinline__ void pg_init(PgSmem& sm)
+// By one thread, in front of a barrier.  `writers`: arrivals that fill a stage.
+__device__ __forceinline__ void pg_init(PgSmem& sm, uint32_t writers = 1)
 {
     mbar_init(&sm.q_full, 1);
     mbar_init(&sm.q_empty, 1);
     for (int i = 0; i < kPgStages; ++i) {
-        mbar_init(&sm.full[i], 1);
+        mbar_init(&sm.full[i], writers);
         mbar_init(&sm.empty[i], 1);
     }
     for (int x = 0; x < 2; ++x) {
@@ -131,8 +139,85 @@ __device__ __forceinline__ void pg_init(PgSmem& sm)
     mbar_fence_init();
 }
 
-// The work of CTA `cta` of `ctas`; the scratch is laid out for `region` of them.
-template<typename T, int D, bool kBias>
+// Sixteen codes times their scale as 16-bit values, two to a word.
+template<typename T, int kCodes>
+__device__ __forceinline__ void pg_values16(const uint4& x, float scale, uint32_t (&out)[8])
+{
+    float y[16];
+    dequantize16<kCodes>(x, scale, y);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) out[i] = PgType<T>::pack(y[2 * i], y[2 * i + 1]);
+}
+
+// A warp that converts: its 32 keys of every entry of the ring, in the entries' order.  Lane (r, c) = (lane / 4, lane % 4) has 16 codes of keys
+// r, r + 8, r + 16 and r + 24 in either half of a row (odd keys the halves in the other order: eight lanes then meet no bank twice).
+template<typename T, int D, int kCodes>
+struct PgConverter {
+    static constexpr int kHalves = D / 64, kHalf = kPgRows * 128;
+    const PagedMhaArgs& a;
+    int warp;                          // 0 .. 3
+    uint4 x[4 * kHalves];              // of the entry on its way
+    float scale[4];
+
+    // the pages of the two runs of 16 keys of a block at key0; -1: nobody sees them, -2: zeros
+    __device__ __forceinline__ int2 pages(const int* row, const PgSpan& span, int key0) const
+    {
+        int n[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int key = key0 + 32 * warp + 16 * i;
+            n[i] = -1;
+            if (key < span.hi && key + 16 > span.lo) {
+                n[i] = row[key >> a.page_shift];
+                if (n[i] < 0 || n[i] >= a.num_pages) {
+                    g_device_status = 6;
+                    n[i] = -2;
+                }
+            }
+        }
+        return make_int2(n[0], n[1]);
+    }
+    __device__ __forceinline__ void load(bool v, int head, const PgSpan& span, int key0, int2 page)
+    {
+        const int lane = threadIdx.x & 31;
+        const uint8_t* cache = (const uint8_t*)(v ? a.v_cache : a.k_cache) + head * (v ? a.vc_head : a.kc_head);
+        const float* scales = (v ? a.v_scale : a.k_scale) + head * (v ? a.vs_head : a.ks_head);
+        const long long page_step = v ? a.vc_page : a.kc_page, slot_step = v ? a.vc_slot : a.kc_slot, scale_step = v ? a.vs_page : a.ks_page;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int key = key0 + 32 * warp + 8 * i + (lane >> 2), n = i < 2 ? page.x : page.y;
+            scale[i] = 0.f;
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h) x[i * kHalves + h] = make_uint4(0u, 0u, 0u, 0u);
+            if (n < 0 || key < span.lo || key >= span.hi) continue;
+            const int slot = key & ((1 << a.page_shift) - 1);
+            const uint8_t* src = cache + n * page_step + slot * slot_step + 16 * (lane & 3);
+            scale[i] = scales[n * scale_step + slot];
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h) x[i * kHalves + h] = *reinterpret_cast<const uint4*>(src + 64 * (kHalves == 2 ? h ^ ((lane >> 2) & 1) : 0));
+        }
+    }
+    __device__ __forceinline__ void store(uint8_t* stage) const
+    {
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int key = 32 * warp + 8 * i + (lane >> 2);
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h) {
+                uint32_t y[8];
+                pg_values16<T, kCodes>(x[i * kHalves + h], scale[i], y);
+                uint8_t* dst = stage + (kHalves == 2 ? h ^ (key & 1) : 0) * kHalf + key * 128;
+                const int c = 2 * (lane & 3);
+                *reinterpret_cast<uint4*>(dst + ((c ^ (key & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
+                *reinterpret_cast<uint4*>(dst + (((c + 1) ^ (key & 7)) << 4)) = make_uint4(y[4], y[5], y[6], y[7]);
+            }
+        }
+    }
+};
+
+// The work of CTA `cta` of `ctas`; the scratch is laid out for `region` of them.  kCodes: the cache holds codes, and warps 12-15 convert them.
+template<typename T, int D, bool kBias, int kCodes = 0>
 __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtensorMap* map_k, const CUtensorMap* map_v, const PagedMhaArgs& a,
                                          void* ws, int least, int whole, int cta, int ctas, int region, PgSmem& sm,
                                          const uint32_t& tmem_base, uint8_t* dyn)
@@ -179,6 +264,7 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
                             &sm.q_full);
             }
             if (p.s.p0 + p.s.tokens > cap && lane == 0) g_device_status = 6;
+            if (kCodes) continue;
             const PgLoader<D> loader = {a, a.pages + p.seq * a.pages_stride, p.head, span};
             auto put = [&](const CUtensorMap* map, int j, int page) -> bool {
                 if (!tc_wait_warp(&sm.empty[stage], phase, &sm.abort)) return false;
@@ -306,7 +392,50 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
             }
         }
     }
-    else {
+    else if (kCodes && warp >= 12) {
+        // ------------------------------------------------------------------ codes into the ring
+        // An entry is read while the one before is converted; pages are known a block ahead of that.
+        PgConverter<T, D, kCodes ? kCodes : kCodesInt8> conv = {a, warp - 12};
+        int stage = 0;
+        uint32_t phase = 1;                                       // of `empty`: the first round finds the stages free
+        bool ok = true, loaded = false;
+        auto put = [&]() -> bool {                                // what was read last
+            if (!tc_wait_warp(&sm.empty[stage], phase, &sm.abort)) return false;
+            conv.store(ring + stage * kTile);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.full[stage]);
+            if (++stage == kPgStages) {
+                stage = 0;
+                phase ^= 1;
+            }
+            return true;
+        };
+        while (ok && share.next(a, tiling, p)) {
+            if (p.blocks == 0) continue;
+            const PgSpan span = pg_span(a, p.s, p.tile * pair_tokens, (p.tile + 1) * pair_tokens);
+            const int* row = a.pages + p.seq * a.pages_stride;
+            int2 page = conv.pages(row, span, p.top * kPgKeys), before = page;
+            for (int j = 0; j <= p.blocks && ok; ++j) {
+                const int key0 = (p.top - j) * kPgKeys;
+                int2 next = page;
+                if (j + 1 < p.blocks) next = conv.pages(row, span, key0 - kPgKeys);
+                if (j < p.blocks) {
+                    if (loaded) ok = put();
+                    if (ok) conv.load(false, p.head, span, key0, page);
+                    loaded = true;
+                }
+                if (j > 0 && ok) {
+                    ok = put();
+                    if (ok) conv.load(true, p.head, span, key0 + kPgKeys, before);
+                }
+                before = page;
+                page = next;
+            }
+        }
+        if (ok && loaded) put();
+    }
+    else if (warp < 8) {
         // ------------------------------------------------------------------ softmax, epilogue
         const int x = warp >> 2;
         const int r = (warp & 3) * 32 + lane;                 // row of the tile = lane of tensor memory
@@ -450,8 +579,8 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
                 tmem_st16_async(t_s + 16, pk);
                 tmem_ld32_async(t_s + 64, v);
                 tmem_ld32_async(t_s + 96, v + 32);
-                if (key0 < span.lo || key0 + kPgKeys > span.hi) {
-                    // rows of V that nobody sees
+                if (!kCodes && (key0 < span.lo || key0 + kPgKeys > span.hi)) {
+                    // rows of V that nobody sees (of codes: zeros already)
                     const int entry = entry0 + pg_v_entry(j, blocks), stage = entry % kPgStages;
                     if (!tc_wait_warp(&sm.full[stage], (uint32_t)((entry / kPgStages) & 1), &sm.abort)) {
                         ok = false;
@@ -613,6 +742,63 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     pg_begin(&tmem_base, kPgTmemCols);
     pg_tiles<T, D, kBias>(&map_q, &map_k, &map_v, a, ws, 1, whole, (int)blockIdx.x, (int)gridDim.x, (int)gridDim.x, sm, tmem_base, pg_dyn);
     pg_end(&tmem_base, kPgTmemCols);
+}
+
+// Moves registers between the warpgroups; by all warps of a warpgroup.
+template<int kRegisters>
+__device__ __forceinline__ void pg_more_registers()
+{
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegisters));
+}
+template<int kRegisters>
+__device__ __forceinline__ void pg_fewer_registers()
+{
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegisters));
+}
+
+// Sequences of `least` new tokens and more, over a cache of codes.
+template<typename T, int D, bool kBias, int kCodes>
+__global__ void __launch_bounds__(kPgCodesThreads, 1)
+paged_mha_tc_codes_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ PagedMhaArgs a, void* ws, int least, int whole)
+{
+    static_assert(2 * 144 + 112 + 112 <= 4 * 128, "of what the CTA was launched with");
+    extern __shared__ __align__(1024) uint8_t pg_dyn[];
+    __shared__ PgSmem sm;
+    __shared__ uint32_t tmem_base;
+    if (smem_u32(pg_dyn) & 1023) {   // the swizzle goes by addresses; the alignment above is there, so this does not happen
+        g_device_status = 2;
+        return;
+    }
+    if (threadIdx.x == 0) pg_init(sm, 4);
+    pg_begin(&tmem_base, kPgTmemCols);
+    const int group = threadIdx.x >> 7;
+    if (group < 2) pg_more_registers<144>();
+    else if (group == 2) pg_fewer_registers<112>();
+    else pg_fewer_registers<112>();
+    pg_tiles<T, D, kBias, kCodes>(&map_q, nullptr, nullptr, a, ws, least, whole, (int)blockIdx.x, (int)gridDim.x, (int)gridDim.x, sm, tmem_base,
+                                  pg_dyn);
+    pg_end(&tmem_base, kPgTmemCols);
+}
+
+template<typename T, int D, bool kBias, int kCodes>
+int pg_launch_tc_codes(const PagedMhaArgs& a, void* ws, int least, int whole, cudaStream_t stream)
+{
+    constexpr int kSmem = pg_tiles_smem(D);
+    CUtensorMap map_q;
+    const long long q_dims[3] = {D, a.heads, a.tokens}, q_str[3] = {1, a.q_head, a.q_tok};
+    const int group = a.heads / a.kv_heads, q_box[3] = {64, group, kPgRows / group};
+    if (int rc = pg_encode(&map_q, PgType<T>::tma, a.q, 3, q_dims, q_str, q_box)) return rc;
+    auto kern = paged_mha_tc_codes_kernel<T, D, kBias, kCodes>;
+    static bool attr_set[64] = {};
+    int dev = 0;
+    EET_CUDA(cudaGetDevice(&dev));
+    dev &= 63;
+    if (!attr_set[dev]) {
+        EET_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+        attr_set[dev] = true;
+    }
+    EET_CUDA(launch_pdl(kern, dim3(sm_count()), dim3(kPgCodesThreads), kSmem, stream, map_q, a, ws, least, whole));
+    return 0;
 }
 
 template<typename T, int D, bool kBias>

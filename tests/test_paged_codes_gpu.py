@@ -1,5 +1,4 @@
 """A paged cache of 8-bit codes against a plain restatement in 64 bits (codes_util), through the Python calls."""
-import itertools
 import math
 
 import pytest
@@ -182,14 +181,14 @@ def test_load_of_missing_pages_and_positions():
 # ---------------------------------------------------------------------------------------------------------------------
 # attention
 # ---------------------------------------------------------------------------------------------------------------------
-def _check(batch, what="", **options):
+def _check(batch, what="", read_back=False, **options):
     given = {w: (x.cuda() if torch.is_tensor(x) else x) for w, x in options.items()}
     total = sum(batch.new)
     out = torch.full_like(batch.q, 7.0).cuda()
     got = _paged().paged_mha(batch.q.cuda(), *batch.gpu(), out=out, **batch.scales(), **given)
     assert got is out
     plain = {w: x for w, x in options.items() if w in ("scale", "window", "first_key", "alibi_slopes")}
-    ref, tol = attend_codes64(batch, **plain)
+    ref, tol = attend_codes64(batch, read_back=read_back, **plain)
     _within(out[:total], ref, tol, what)
     assert (out[total:] == 7.0).all(), "rows behind the last sequence"
     assert _status() == 0
@@ -201,11 +200,11 @@ ROWS = [([1], [1]), ([1], [300]), ([1, 1, 1], [5, 128, 129]), ([1] * 40, [1 + 37
 
 @pytest.mark.parametrize("new,lens", ROWS)
 @pytest.mark.parametrize("heads,kv_heads,head_dim,page", [(4, 4, 128, 16), (8, 2, 128, 64), (8, 1, 64, 16), (16, 1, 128, 32), (6, 2, 64, 256)])
-@pytest.mark.parametrize("kind,dtype", itertools.product(CODES, (FP16, BF16)))
+@pytest.mark.parametrize("kind,dtype", [(INT8, FP16), (INT8, BF16), (E4M3, FP16), (E4M3, BF16)])
 def test_mha_few_rows(new, lens, heads, kv_heads, head_dim, page, kind, dtype):
     batch = CodesBatch(new, lens, heads, kv_heads, head_dim, page, dtype, kind, behind=1)
     batch.poison()
-    _check(batch, max_tokens=max(new))
+    _check(batch, max_tokens=max(new), read_back=max(new) * heads // kv_heads > 16)
 
 
 @pytest.mark.parametrize("kind", CODES)
@@ -221,6 +220,47 @@ def test_mha_few_rows_options(kind, options):
     if options.pop("alibi", False):
         options["alibi_slopes"] = torch.tensor([2.0 ** -i for i in range(1, 9)])
     _check(batch, max_tokens=2, **options)
+
+
+TILES = [([17], [17]), ([200], [300]), ([129], [2000]), ([300, 260], [300, 700]), ([40, 0, 70], [40, 5, 1000]), ([513], [1300])]
+
+
+@pytest.mark.parametrize("new,lens", TILES)
+@pytest.mark.parametrize("heads,kv_heads,head_dim,page", [(4, 4, 128, 16), (8, 2, 128, 64), (8, 1, 64, 16), (32, 1, 128, 32), (6, 2, 64, 256),
+                                                          (7, 1, 128, 128)])
+@pytest.mark.parametrize("kind,dtype", [(INT8, FP16), (INT8, BF16), (E4M3, FP16), (E4M3, BF16)])
+def test_mha_tiles(new, lens, heads, kv_heads, head_dim, page, kind, dtype):
+    batch = CodesBatch(new, lens, heads, kv_heads, head_dim, page, dtype, kind, behind=1)
+    batch.poison()
+    _check(batch, max_tokens=max(new), read_back=True)
+
+
+@pytest.mark.parametrize("kind", CODES)
+@pytest.mark.parametrize("heads,kv_heads", [(8, 2), (64, 1), (128, 1)])
+@pytest.mark.parametrize("options", [dict(window=1), dict(window=100), dict(first=True), dict(alibi=True), dict(window=33, first=True, alibi=True),
+                                     dict(scale=0.3), dict(scale=-0.1), dict(scale=0.0)])
+def test_mha_tiles_options(kind, heads, kv_heads, options):
+    lens = [30, 200, 617, 50]
+    batch = CodesBatch([30, 120, 200, 1], lens, heads, kv_heads, 128, 16, FP16, kind)
+    batch.poison()
+    options = dict(options)
+    if options.pop("first", False):
+        options["first_key"] = torch.tensor([30, 150, 0, 49], dtype=torch.int32)     # the first sequence sees nothing
+    if options.pop("alibi", False):
+        options["alibi_slopes"] = torch.tensor([2.0 ** -(i % 8 + 1) for i in range(heads)])
+    _check(batch, max_tokens=200, read_back=True, **options)
+
+
+@pytest.mark.parametrize("kind", CODES)
+@pytest.mark.parametrize("dtype,heads,kv_heads,head_dim,page", [(FP16, 8, 8, 128, 16), (BF16, 8, 2, 64, 64), (FP16, 32, 4, 128, 32)])
+@pytest.mark.parametrize("alibi", [False, True])
+def test_mha_a_chunk_beside_single_tokens(kind, dtype, heads, kv_heads, head_dim, page, alibi):
+    """Both kinds of tiles in one call."""
+    new, lens = [1] * 20 + [150] + [2] + [1] * 10, [100 + 41 * i for i in range(20)] + [700, 900] + [1 + 300 * i for i in range(10)]
+    batch = CodesBatch(new, lens, heads, kv_heads, head_dim, page, dtype, kind, behind=3)
+    batch.poison()
+    more = dict(alibi_slopes=torch.tensor([2.0 ** -(i % 8 + 1) for i in range(heads)])) if alibi else {}
+    _check(batch, max_tokens=150, max_len=3000, read_back=True, **more)
 
 
 @pytest.mark.parametrize("kind", CODES)
