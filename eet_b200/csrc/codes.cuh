@@ -67,13 +67,10 @@ __device__ __forceinline__ void quantize16(const float (&y)[16], float scale, ui
     }
 }
 
-// Four codes as fp16 pairs {c0, c1}, {c2, c3}, times kCodeUnit.
+// Four codes as fp16 pairs {c0, c1}, {c2, c3}, exactly.
 //   int8   under the exponent pattern 0x64 a byte b reads as 1024 + b; b is the code + 128
-//   e4m3   the seven bits below the sign, moved to the top of fp16's exponent and mantissa, read as the code times 2^-8 (the biases
-//          are 7 and 15), those below the smallest normal code as fp16's own; no pattern is an infinity or NaN
-template<int kCodes>
-constexpr float kCodeUnit = kCodes == kCodesInt8 ? 1.0f : 1.0f / 256;
-
+//   e4m3   an instruction for two (with shifts and masks instead, eight instructions for four codes, two sequences of 60000 to 100000
+//          positions took 104 us)
 template<int kCodes>
 __device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t& lo, uint32_t& hi)
 {
@@ -81,9 +78,14 @@ __device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t& lo, uint32_t
         cvt_u8x4_to_f16x4(w ^ 0x80808080u, lo, hi);
     }
     else {
-        const uint32_t a = __byte_perm(w, 0u, 0x1404), b = __byte_perm(w, 0u, 0x3424);   // a byte each under eight zeros
-        lo = (a & 0x80008000u) | ((a >> 1) & 0x3f803f80u);
-        hi = (b & 0x80008000u) | ((b >> 1) & 0x3f803f80u);
+        asm("{\n"
+            ".reg .b16 a, b;\n"
+            "mov.b32 {a, b}, %2;\n"
+            "cvt.rn.f16x2.e4m3x2 %0, a;\n"
+            "cvt.rn.f16x2.e4m3x2 %1, b;\n"
+            "}\n"
+            : "=r"(lo), "=r"(hi)
+            : "r"(w));
     }
 }
 
@@ -91,8 +93,6 @@ template<int kCodes>
 __device__ __forceinline__ void dequantize16(const uint4& x, float scale, float (&y)[16])
 {
     const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-    // (the unit is a power of two, and goes to the codes: times the scale it could overflow)
-    constexpr float up = 1.0f / kCodeUnit<kCodes>;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         uint32_t h[2];
@@ -100,8 +100,8 @@ __device__ __forceinline__ void dequantize16(const uint4& x, float scale, float 
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[e]));
-            y[4 * i + 2 * e] = f.x * up * scale;
-            y[4 * i + 2 * e + 1] = f.y * up * scale;
+            y[4 * i + 2 * e] = f.x * scale;
+            y[4 * i + 2 * e + 1] = f.y * scale;
         }
     }
 }

@@ -96,7 +96,7 @@ struct PcCopies {
     uint32_t ring;                // of this warp
     int offset;                   // of its keys in a block
 
-    // the page of the run of 16 keys that this half of the warp looks after; -1: it has none of the keys that the tile sees
+    // the page of the run of 16 keys that this half of the warp looks after; -1: nothing to be read
     __device__ __forceinline__ int page(const PgPiece& p, const PgSpan& span, int key0) const
     {
         const int key = key0 + offset + (int)(threadIdx.x & 16);
@@ -104,37 +104,51 @@ struct PcCopies {
         const int page = (a.pages + p.seq * a.pages_stride)[key >> a.page_shift];
         if (page < 0 || page >= a.num_pages) {
             g_device_status = 6;
-            return -2;            // zeros
+            return -1;
         }
         return page;
     }
-    __device__ __forceinline__ void issue(const PgPiece& p, int key0, int page, int stage) const
+    // Keys that the tile does not see, and pages outside the cache, become zeros: codes and scales there may be anything.
+    __device__ __forceinline__ void issue(const PgPiece& p, const PgSpan& span, int key0, int page, int stage) const
     {
         constexpr int kChunks = D / 16, kRowsAtOnce = 32 / kChunks, kTimes = 16 / kRowsAtOnce;
-        const int lane = threadIdx.x & 31, key = key0 + offset, slot = key & ((1 << a.page_shift) - 1);
+        const int lane = threadIdx.x & 31, key = key0 + offset, row0 = lane / kChunks, c = lane % kChunks;
         const uint32_t at = ring + (uint32_t)(stage * PcShape<D>::kStage);
+        const bool whole = key >= span.lo && key + kPcKeys <= span.hi;
+        const long long k_step = kRowsAtOnce * a.kc_slot, v_step = kRowsAtOnce * a.vc_slot;
 #pragma unroll
         for (int run = 0; run < 2; ++run) {
-            const int n = __shfl_sync(0xffffffffu, page, 16 * run);
-            if (n == -1) continue;
-            const uint32_t bytes = n >= 0 ? 16 : 0;
-            const int s = (slot + 16 * run) & ((1 << a.page_shift) - 1), row0 = lane / kChunks, c = lane % kChunks;
-            const uint8_t *k = (const uint8_t*)a.k_cache, *v = (const uint8_t*)a.v_cache;
-            if (n >= 0) {
-                k += n * a.kc_page + p.head * a.kc_head + (s + row0) * a.kc_slot + 16 * c;
-                v += n * a.vc_page + p.head * a.vc_head + (s + row0) * a.vc_slot + 16 * c;
+            const int n = __shfl_sync(0xffffffffu, page, 16 * run), slot = (key + 16 * run) & ((1 << a.page_shift) - 1);
+            const long long page_at = max(n, 0);
+            const uint8_t* k = (const uint8_t*)a.k_cache + page_at * a.kc_page + p.head * a.kc_head + (slot + row0) * a.kc_slot + 16 * c;
+            const uint8_t* v = (const uint8_t*)a.v_cache + page_at * a.vc_page + p.head * a.vc_head + (slot + row0) * a.vc_slot + 16 * c;
+            // a half of the warp for the scales of either
+            const float* scale = (lane < 16 ? a.k_scale + page_at * a.ks_page + p.head * a.ks_head
+                                            : a.v_scale + page_at * a.vs_page + p.head * a.vs_head) + slot + (lane & 15);
+            const uint32_t scale_to = at + 2 * PcShape<D>::kTile + (uint32_t)(((lane < 16 ? 0 : kPcKeys) + 16 * run + (lane & 15)) * 4);
+            const uint32_t to = at + pc_place<D>(16 * run + row0, c);
+            if (whole && n >= 0) {
+#pragma unroll
+                for (int i = 0; i < kTimes; ++i) {
+                    const uint32_t to_i = D == 128 ? to ^ (uint32_t)((kRowsAtOnce * i & 7) << 4) : to;   // (a row's swizzle)
+                    copy16_async(to_i + kRowsAtOnce * i * D, k + i * k_step, 16);
+                    copy16_async(to_i + kRowsAtOnce * i * D + PcShape<D>::kTile, v + i * v_step, 16);
+                }
+                copy4_async(scale_to, scale, 4);
+                continue;
             }
-            const long long k_step = n >= 0 ? kRowsAtOnce * a.kc_slot : 0, v_step = n >= 0 ? kRowsAtOnce * a.vc_slot : 0;
+            // (nothing is read where a size is zero; the addresses stay inside the cache)
 #pragma unroll
             for (int i = 0; i < kTimes; ++i) {
-                const uint32_t to = at + pc_place<D>(16 * run + row0 + kRowsAtOnce * i, c);
-                copy16_async(to, k + i * k_step, bytes);
-                copy16_async(to + PcShape<D>::kTile, v + i * v_step, bytes);
+                const int at_key = key + 16 * run + row0 + kRowsAtOnce * i;
+                const uint32_t bytes = n >= 0 && at_key >= span.lo && at_key < span.hi ? 16 : 0;
+                const uint32_t to_i = D == 128 ? to ^ (uint32_t)((kRowsAtOnce * i & 7) << 4) : to;
+                copy16_async(to_i + kRowsAtOnce * i * D, bytes ? k + i * k_step : (const uint8_t*)a.k_cache, bytes);
+                copy16_async(to_i + kRowsAtOnce * i * D + PcShape<D>::kTile, bytes ? v + i * v_step : (const uint8_t*)a.v_cache, bytes);
             }
-            // a half of the warp for the scales of either
-            const float* scale = lane < 16 ? a.k_scale : a.v_scale;
-            if (n >= 0) scale += (lane < 16 ? n * a.ks_page + p.head * a.ks_head : n * a.vs_page + p.head * a.vs_head) + s + (lane & 15);
-            copy4_async(at + 2 * PcShape<D>::kTile + (uint32_t)(((lane < 16 ? 0 : kPcKeys) + 16 * run + (lane & 15)) * 4), scale, bytes / 4);
+            const int at_key = key + 16 * run + (lane & 15);
+            const uint32_t bytes = n >= 0 && at_key >= span.lo && at_key < span.hi ? 4 : 0;
+            copy4_async(scale_to, bytes ? scale : a.k_scale, bytes);
         }
     }
 };
@@ -183,8 +197,8 @@ paged_mha_codes_kernel(const __grid_constant__ PagedMhaArgs a, void* ws, int mos
         else if (have_next && ahead < p.blocks + next.blocks) page = copies.page(next, next_span, (next.top - (ahead - p.blocks)) * kPgKeys);
     };
     auto fetch = [&]() -> bool {   // a block, in a group of its own
-        if (ahead < p.blocks) copies.issue(p, (p.top - ahead) * kPgKeys, page, into);
-        else if (have_next && ahead < p.blocks + next.blocks) copies.issue(next, (next.top - (ahead - p.blocks)) * kPgKeys, page, into);
+        if (ahead < p.blocks) copies.issue(p, span, (p.top - ahead) * kPgKeys, page, into);
+        else if (have_next && ahead < p.blocks + next.blocks) copies.issue(next, next_span, (next.top - (ahead - p.blocks)) * kPgKeys, page, into);
         else return false;
         asm volatile("cp.async.commit_group;" ::: "memory");
         ++ahead;
@@ -240,8 +254,7 @@ paged_mha_codes_kernel(const __grid_constant__ PagedMhaArgs a, void* ws, int mos
             for (int i = 0; i < 2; ++i) {
                 const int row = 8 * n + 2 * t + i;
                 const int down = __shfl_sync(0xffffffffu, e, 4 * (2 * t + i));
-                // (again in two: scale / kCodeUnit and the power of the row)
-                factor[n][i] = a.scale * kLog2e / kCodeUnit<kCodes> * __uint_as_float((uint32_t)(127 - down / 2) << 23) *
+                factor[n][i] = a.scale * kLog2e * __uint_as_float((uint32_t)(127 - down / 2) << 23) *
                                __uint_as_float((uint32_t)(127 - (down - down / 2)) << 23);
                 const bool valid = row < rows;
                 pos[n][i] = p.s.p0 + token0 + row / group;
@@ -262,6 +275,10 @@ paged_mha_codes_kernel(const __grid_constant__ PagedMhaArgs a, void* ws, int mos
                 for (int e = 0; e < 4; ++e) o[n][i][e] = 0.f;
             }
         }
+        // blocks all of whose keys every row sees
+        const int pos0 = p.s.p0 + token0, pos1 = pos0 + (rows - 1) / group;
+        const int all_high = min(pos0, last), all_low = a.window > 0 ? (int)max((long long)p.s.first, (long long)pos1 - a.window + 1) : p.s.first;
+        bool huge = false;
         int used = stage;          // stage of the piece's last block
         for (int j = 0; j < p.blocks; ++j) {
             if (ahead - j > kPcStages - 2) asm volatile("cp.async.wait_group %0;" ::"n"(kPcStages - 2) : "memory");
@@ -298,7 +315,7 @@ paged_mha_codes_kernel(const __grid_constant__ PagedMhaArgs a, void* ws, int mos
                 }
             }
             // ---- weights
-            float vs[2][2], lvs[2][2];
+            float vs[2][2], top_scale = 8.67361738e-19f;   // (2^-60: a scale of zero weighs nothing)
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
 #pragma unroll
@@ -307,27 +324,45 @@ paged_mha_codes_kernel(const __grid_constant__ PagedMhaArgs a, void* ws, int mos
                     float ks;
                     asm volatile("ld.shared.f32 %0, [%1];" : "=f"(ks) : "r"(place));
                     asm volatile("ld.shared.f32 %0, [%1];" : "=f"(vs[m][i]) : "r"(place + kPcKeys * 4));
-                    lvs[m][i] = __log2f(fmaxf(vs[m][i], 8.67361738e-19f));   // (2^-60 at least: a scale of zero weighs nothing)
-                    const int key = key0 + 16 * m + 8 * i + g;
+                    top_scale = fmaxf(top_scale, vs[m][i]);
 #pragma unroll
                     for (int n = 0; n < kN; ++n) {
 #pragma unroll
-                        for (int r = 0; r < 2; ++r) {
-                            float& x = s[m][n][2 * i + r];
-                            x *= ks * factor[n][r];
-                            if (a.slopes != nullptr) x = fmaf(slope[n][r], (float)(key - pos[n][r]), x);
-                            x = key >= low[n][r] && key <= high[n][r] ? x : -INFINITY;
-                        }
+                        for (int r = 0; r < 2; ++r) s[m][n][2 * i + r] *= ks * factor[n][r];
                     }
                 }
             }
-            bool over = false;
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
+            if (a.slopes != nullptr) {
 #pragma unroll
                 for (int n = 0; n < kN; ++n) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) over |= s[m][n][e] + lvs[m][e >> 1] - ref[n][e & 1] > kPgLag + kUp;
+                    for (int k = 0; k < 8; ++k) {
+                        const int i = k >> 1 & 1, r = k & 1;
+                        float& x = s[k >> 2][n][2 * i + r];
+                        x = fmaf(slope[n][r], (float)(key0 + 16 * (k >> 2) + 8 * i + g - pos[n][r]), x);
+                    }
+                }
+            }
+            if (key0 < all_low || key0 + kPcKeys - 1 > all_high) {
+#pragma unroll
+                for (int n = 0; n < kN; ++n) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int i = k >> 1 & 1, r = k & 1, key = key0 + 16 * (k >> 2) + 8 * i + g;
+                        float& x = s[k >> 2][n][2 * i + r];
+                        x = key >= low[n][r] && key <= high[n][r] ? x : -INFINITY;
+                    }
+                }
+            }
+            // (with the largest scale of the lane's keys: never too small, and looked at closely where it says so)
+            bool over = false;
+            const float most = __log2f(top_scale) - kPgLag - kUp;
+#pragma unroll
+            for (int n = 0; n < kN; ++n) {
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const float m = fmaxf(fmaxf(s[0][n][r], s[0][n][2 + r]), fmaxf(s[1][n][r], s[1][n][2 + r]));
+                    over |= m + most > ref[n][r];
                 }
             }
             if (__any_sync(0xffffffffu, over)) {
@@ -338,12 +373,15 @@ paged_mha_codes_kernel(const __grid_constant__ PagedMhaArgs a, void* ws, int mos
                     for (int r = 0; r < 2; ++r) {
                         float m = -INFINITY;
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) m = fmaxf(m, s[k >> 1][n][2 * (k & 1) + r] + lvs[k >> 1][k & 1]);
+                        for (int k = 0; k < 4; ++k) {
+                            m = fmaxf(m, s[k >> 1][n][2 * (k & 1) + r] + __log2f(fmaxf(vs[k >> 1][k & 1], 8.67361738e-19f)));
+                        }
 #pragma unroll
                         for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
                         const bool moves = m - ref[n][r] > kPgLag + kUp;
                         const float to = moves ? m - kUp : ref[n][r], corr = moves ? ex2_approx(ref[n][r] - to) : 1.0f;
                         ref[n][r] = to;
+                        huge |= fabsf(to) >= 1048576.0f && moves;
                         l[n][r] *= corr;
 #pragma unroll
                         for (int i = 0; i < kSteps; ++i) {
@@ -358,24 +396,20 @@ paged_mha_codes_kernel(const __grid_constant__ PagedMhaArgs a, void* ws, int mos
             for (int m = 0; m < 2; ++m) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const float scale = vs[m][i], inverse = __fdividef(1.0f, scale);
 #pragma unroll
                     for (int n = 0; n < kN; ++n) {
                         float e[2];
 #pragma unroll
                         for (int r = 0; r < 2; ++r) {
-                            const float x = s[m][n][2 * i + r];
-                            const float power = ex2_approx(x - ref[n][r]);
-                            // (a scale in a place that nobody sees may be anything; beyond 2^24 a score may not know of log2 s^v)
-                            asm("min.NaN.f32 %0, %1, %2;" : "=f"(e[r]) : "f"(x == -INFINITY ? 0.f : power * scale), "f"(65504.0f));
-                            s[m][n][2 * i + r] = power;
+                            const float power = ex2_approx(s[m][n][2 * i + r] - ref[n][r]);
+                            l[n][r] += power;
+                            e[r] = power * vs[m][i];
+                        }
+                        if (huge) {   // (beyond 2^20 a score knows little of log2 s^v, and a weight could leave fp16)
+#pragma unroll
+                            for (int r = 0; r < 2; ++r) asm("min.NaN.f32 %0, %0, %1;" : "+f"(e[r]) : "f"(65504.0f));
                         }
                         const __half2 h = __floats2half2_rn(e[0], e[1]);
-                        const float2 f = __half22float2(h);
-                        // (The sum is of the rounded weights: where one key has most of the weight, its rounding then cancels.  Below
-                        // the smallest normal value, a scale of zero among it, what rounding leaves says nothing of the power.)
-                        l[n][0] += f.x >= 6.103515625e-5f ? f.x * inverse : s[m][n][2 * i];
-                        l[n][1] += f.y >= 6.103515625e-5f ? f.y * inverse : s[m][n][2 * i + 1];
                         w[m][n][i] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h));
                     }
                 }
@@ -465,7 +499,7 @@ paged_mha_codes_kernel(const __grid_constant__ PagedMhaArgs a, void* ws, int mos
                     reinterpret_cast<const float*>(pc_dyn + (w * kPcStages + used) * Shape::kStage) + row * D + ((d + 8 * row) & (D - 1)));
                 v.x += x.x * f, v.y += x.y * f, v.z += x.z * f, v.w += x.w * f;
             }
-            const float f = (complete ? (sum == 0.f ? 0.f : 1.0f / sum) : 1.0f) / kCodeUnit<kCodes>;
+            const float f = complete ? (sum == 0.f ? 0.f : 1.0f / sum) : 1.0f;
             v = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
             if (!complete) {
                 part.o[row * (D / 4) + d / 4] = v;
