@@ -30,23 +30,35 @@ namespace eet {
 
 namespace {
 
-constexpr int kPcWarps = 4;
-constexpr int kPcThreads = 32 * kPcWarps;
-constexpr int kPcKeys = kPgKeys / kPcWarps;     // of a block, for a warp
-constexpr int kPcStages = 3;
-constexpr int kPcPerSm = 2;                     // CTAs
 constexpr int kPcExtra = 2;                     // a piece's beginning and end cost as much as two blocks
-static_assert(kPcKeys == 32, "a lane a scale, two runs of 16 keys");
 
-template<int D>
+template<int D, int kRows>
 struct PcShape {
-    static constexpr int kTile = kPcKeys * D;                           // bytes: a warp's codes of K or V of a block
-    static constexpr int kStage = 2 * kTile + 2 * kPcKeys * 4;          // and the scales
-    static constexpr int kSmem = kPcWarps * kPcStages * kStage;
+    static constexpr int kWarps = 4;
+    static constexpr int kKeys = kPgKeys / kWarps;                      // of a block, for a warp: one or two runs of 16
+    static constexpr int kAtOnce = kRows == 8 ? 2 : 1;// runs that are worked on together
+    static constexpr int kPerSm = kRows == 8 ? 3 : 2;// CTAs
+    static constexpr int kStages = kRows == 8 && D == 128 ? 2 : 3;
+    static constexpr int kTile = kKeys * D;                             // bytes: a warp's codes of K or V of a block
+    static constexpr int kStage = 2 * kTile + 2 * kKeys * 4;            // and the scales
+    static constexpr int kSmem = kWarps * kStages * kStage;
+    static_assert(kStage >= kRows * D * 4, "the sums of a warp fit where its codes were");
+};
+
+constexpr int pc_per_sm(int rows) { return rows == 8 ? PcShape<128, 8>::kPerSm : PcShape<128, 16>::kPerSm; }
+
+// What a warp knows of the rows of its piece, out of its registers: few blocks ask for it.
+struct PcRows {
+    int low[16], high[16];        // keys that a row sees
+    int pos[16];
+    float slope[16];              // of the bias, to the power of two
 };
 
 struct PcSmem {
-    float ref[kPcWarps][16], sum[kPcWarps][16];
+    PcRows rows[8];
+    PgShare share[8];
+    PgPiece piece[8][2];          // of a warp: the one at work and the one behind it
+    float ref[8][16], sum[8][16];
     PgFound found;
 };
 
@@ -89,75 +101,68 @@ __device__ __forceinline__ uint32_t pc_place(int row, int chunk)
     return (uint32_t)((row >> 1) * 128 + ((((row & 1) * 4 + chunk) ^ (row & 6)) << 4));
 }
 
-// What a warp copies: its 32 keys of a block of a piece.
-template<int D>
+// What a warp copies: its keys of a block of a piece.
+template<int D, int kRows>
 struct PcCopies {
+    using Shape = PcShape<D, kRows>;
+    static constexpr int kRuns = Shape::kKeys / 16;
     const PagedMhaArgs& a;
     uint32_t ring;                // of this warp
     int offset;                   // of its keys in a block
 
-    // the page of the run of 16 keys that this half of the warp looks after; -1: nothing to be read
-    __device__ __forceinline__ int page(const PgPiece& p, const PgSpan& span, int key0) const
+    // The pages of its runs of 16 keys, of the block at key0, in the lanes 0 .. 15 and 16 .. 31, as the table has them; -1: nobody sees them.
+    // (Nothing looks at them before the copies: a trip to L2 that they would wait for with every block.)
+    __device__ __forceinline__ int page(const int* row, int lo, int hi, int key0) const
     {
-        const int key = key0 + offset + (int)(threadIdx.x & 16);
-        if (key >= span.hi || key + 16 <= span.lo) return -1;
-        const int page = (a.pages + p.seq * a.pages_stride)[key >> a.page_shift];
-        if (page < 0 || page >= a.num_pages) {
-            g_device_status = 6;
-            return -1;
-        }
-        return page;
+        const int key = key0 + offset + (kRuns == 2 ? (int)(threadIdx.x & 16) : 0);
+        return key < hi && key + 16 > lo ? row[key >> a.page_shift] : -1;
     }
     // Keys that the tile does not see, and pages outside the cache, become zeros: codes and scales there may be anything.
-    __device__ __forceinline__ void issue(const PgPiece& p, const PgSpan& span, int key0, int page, int stage) const
+    __device__ __forceinline__ void issue(int head, int lo, int hi, int key0, int page, int stage) const
     {
         constexpr int kChunks = D / 16, kRowsAtOnce = 32 / kChunks, kTimes = 16 / kRowsAtOnce;
-        const int lane = threadIdx.x & 31, key = key0 + offset, row0 = lane / kChunks, c = lane % kChunks;
-        const uint32_t at = ring + (uint32_t)(stage * PcShape<D>::kStage);
-        const bool whole = key >= span.lo && key + kPcKeys <= span.hi;
-        const long long k_step = kRowsAtOnce * a.kc_slot, v_step = kRowsAtOnce * a.vc_slot;
-#pragma unroll
-        for (int run = 0; run < 2; ++run) {
-            const int n = __shfl_sync(0xffffffffu, page, 16 * run), slot = (key + 16 * run) & ((1 << a.page_shift) - 1);
-            const long long page_at = max(n, 0);
-            const uint8_t* k = (const uint8_t*)a.k_cache + page_at * a.kc_page + p.head * a.kc_head + (slot + row0) * a.kc_slot + 16 * c;
-            const uint8_t* v = (const uint8_t*)a.v_cache + page_at * a.vc_page + p.head * a.vc_head + (slot + row0) * a.vc_slot + 16 * c;
-            // a half of the warp for the scales of either
-            const float* scale = (lane < 16 ? a.k_scale + page_at * a.ks_page + p.head * a.ks_head
-                                            : a.v_scale + page_at * a.vs_page + p.head * a.vs_head) + slot + (lane & 15);
-            const uint32_t scale_to = at + 2 * PcShape<D>::kTile + (uint32_t)(((lane < 16 ? 0 : kPcKeys) + 16 * run + (lane & 15)) * 4);
-            const uint32_t to = at + pc_place<D>(16 * run + row0, c);
-            if (whole && n >= 0) {
-#pragma unroll
-                for (int i = 0; i < kTimes; ++i) {
-                    const uint32_t to_i = D == 128 ? to ^ (uint32_t)((kRowsAtOnce * i & 7) << 4) : to;   // (a row's swizzle)
-                    copy16_async(to_i + kRowsAtOnce * i * D, k + i * k_step, 16);
-                    copy16_async(to_i + kRowsAtOnce * i * D + PcShape<D>::kTile, v + i * v_step, 16);
-                }
-                copy4_async(scale_to, scale, 4);
-                continue;
+        const int lane = threadIdx.x & 31, row0 = lane / kChunks, c = lane % kChunks;
+        const uint32_t at = ring + (uint32_t)(stage * Shape::kStage);
+#pragma unroll 1
+        for (int run = 0; run < kRuns; ++run) {
+            int n = kRuns == 2 ? __shfl_sync(0xffffffffu, page, 16 * run) : page;
+            const int key = key0 + offset + 16 * run, slot = key & ((1 << a.page_shift) - 1);
+            if (n < 0 || n >= a.num_pages) {
+                if (key < hi && key + 16 > lo) g_device_status = 6;
+                n = -1;
             }
+            const long long page_at = max(n, 0);
+            const uint8_t* k = (const uint8_t*)a.k_cache + page_at * a.kc_page + head * a.kc_head + (slot + row0) * a.kc_slot + 16 * c;
+            const uint8_t* v = (const uint8_t*)a.v_cache + page_at * a.vc_page + head * a.vc_head + (slot + row0) * a.vc_slot + 16 * c;
+            // a half of the warp for the scales of either
+            const float* scale = (lane < 16 ? a.k_scale + page_at * a.ks_page + head * a.ks_head
+                                            : a.v_scale + page_at * a.vs_page + head * a.vs_head) + slot + (lane & 15);
+            const uint32_t to = at + (uint32_t)(16 * run * D) + pc_place<D>(row0, c);
             // (nothing is read where a size is zero; the addresses stay inside the cache)
+            const int from = n < 0 ? 16 : lo - key, upto = hi - key;
+            const long long k_step = kRowsAtOnce * a.kc_slot, v_step = kRowsAtOnce * a.vc_slot;
 #pragma unroll
             for (int i = 0; i < kTimes; ++i) {
-                const int at_key = key + 16 * run + row0 + kRowsAtOnce * i;
-                const uint32_t bytes = n >= 0 && at_key >= span.lo && at_key < span.hi ? 16 : 0;
-                const uint32_t to_i = D == 128 ? to ^ (uint32_t)((kRowsAtOnce * i & 7) << 4) : to;
-                copy16_async(to_i + kRowsAtOnce * i * D, bytes ? k + i * k_step : (const uint8_t*)a.k_cache, bytes);
-                copy16_async(to_i + kRowsAtOnce * i * D + PcShape<D>::kTile, bytes ? v + i * v_step : (const uint8_t*)a.v_cache, bytes);
+                const int r = row0 + kRowsAtOnce * i;
+                const uint32_t bytes = r >= from && r < upto ? 16 : 0;
+                const uint32_t to_i = (D == 128 ? to ^ (uint32_t)((kRowsAtOnce * i & 7) << 4) : to) + kRowsAtOnce * i * D;   // (a row's swizzle)
+                copy16_async(to_i, k, bytes);
+                copy16_async(to_i + Shape::kTile, v, bytes);
+                k += k_step;
+                v += v_step;
             }
-            const int at_key = key + 16 * run + (lane & 15);
-            const uint32_t bytes = n >= 0 && at_key >= span.lo && at_key < span.hi ? 4 : 0;
-            copy4_async(scale_to, bytes ? scale : a.k_scale, bytes);
+            const int r = lane & 15;
+            copy4_async(at + 2 * Shape::kTile + (uint32_t)(((lane < 16 ? 0 : Shape::kKeys) + 16 * run + r) * 4), scale,
+                        r >= from && r < upto ? 4 : 0);
         }
     }
 };
 
 template<int kCodes, int D, int kRows>
-__global__ void __launch_bounds__(kPcThreads, kPcPerSm)
+__global__ void __launch_bounds__(32 * PcShape<D, kRows>::kWarps, PcShape<D, kRows>::kPerSm)
 paged_mha_codes_kernel(const __grid_constant__ PagedMhaArgs a, void* ws, int most, int whole)
 {
-    using Shape = PcShape<D>;
+    using Shape = PcShape<D, kRows>;
     constexpr int kN = kRows / 8;                // tiles of 8 rows
     constexpr int kSteps = D / 16;               // of the sum over dims; tiles of 16 dims
     constexpr float kUp = PgType<__half>::kUp;
@@ -170,55 +175,80 @@ paged_mha_codes_kernel(const __grid_constant__ PagedMhaArgs a, void* ws, int mos
     const PgTiling tiling = {tile_tokens, 1, most, kPcExtra};
     pdl_launch_dependents();
     pdl_wait();
-
-    PgShare share;
-    PgPlace place;
-    const bool work = pg_find_share(a, tiling, cta, ctas, whole != 0, sm.found, share, place);
-    if (!whole && threadIdx.x == 0) pg_write_header(a, tiling, ws, cta, ctas, work, share, place);
-    if (!work) return;
-
-    const long long cap = (long long)a.max_pages << a.page_shift;
-    const int last = (int)min(cap, 0x7fffffffLL) - 1;      // position that has a place in the table
+    {
+        PgShare share;
+        PgPlace place;
+        const bool work = pg_find_share(a, tiling, cta, ctas, whole != 0, sm.found, share, place);
+        if (!whole && threadIdx.x == 0) pg_write_header(a, tiling, ws, cta, ctas, work, share, place);
+        if (!work) return;
+        if (lane == 0) sm.share[warp] = share;
+        __syncwarp();
+    }
+    PcRows& row_of = sm.rows[warp];
     auto span_of = [&](const PgPiece& p) { return pg_span(a, p.s, p.tile * tile_tokens, (p.tile + 1) * tile_tokens); };
-    const PcCopies<D> copies = {a, smem_u32(pc_dyn) + (uint32_t)(warp * kPcStages * Shape::kStage), warp * kPcKeys};
+    // walks on: the piece into place `which`; false: there is none
+    auto walk = [&](int which) -> bool {
+        PgShare share = sm.share[warp];
+        PgPiece p;
+        const bool any = share.next(a, tiling, p);
+        __syncwarp();
+        if (lane == 0) {
+            sm.share[warp] = share;
+            if (any) sm.piece[warp][which] = p;
+        }
+        __syncwarp();
+        return any;
+    };
+    const PcCopies<D, kRows> copies = {a, smem_u32(pc_dyn) + (uint32_t)(warp * Shape::kStages * Shape::kStage), warp * Shape::kKeys};
 
-    // The piece at work and the one behind it; the copies run kPcStages - 1 blocks ahead, into the latter but not beyond.
-    PgPiece p, next;
-    bool more = share.next(a, tiling, p);
-    bool have_next = more && share.next(a, tiling, next);
-    PgSpan span = {0, 0}, next_span = {0, 0};
-    if (more) span = span_of(p);
-    if (have_next) next_span = span_of(next);
-    int ahead = 0, into = 0;       // next block to copy, of p or from p.blocks on of next; its stage
+    // The copies run some blocks ahead of the work, into the piece behind the one at work but not beyond.
+    int now = 0;                   // place of the piece at work
+    bool have_next = false;
+    int copy_key0 = 0, copy_left = 0, copy_lo = 0, copy_hi = 0, copy_head = 0, page = -1;   // what is copied next; copy_left blocks of it
+    const int* copy_row = nullptr;
+    bool copy_next = false;        // it is the piece behind
+    int ahead = 0, into = 0;       // blocks copied and not worked on; the next one's stage
     int stage = 0;                 // of the next block to work on
-    int page = -1;                 // of the block to copy
-    auto look = [&]() {
-        if (ahead < p.blocks) page = copies.page(p, span, (p.top - ahead) * kPgKeys);
-        else if (have_next && ahead < p.blocks + next.blocks) page = copies.page(next, next_span, (next.top - (ahead - p.blocks)) * kPgKeys);
+    auto copy_from = [&](int which) {
+        const PgPiece& p = sm.piece[warp][which];
+        const PgSpan span = span_of(p);
+        copy_key0 = p.top * kPgKeys, copy_left = p.blocks, copy_lo = span.lo, copy_hi = span.hi, copy_head = p.head;
+        copy_row = a.pages + p.seq * a.pages_stride;
+        copy_next = which != now;
+        if (copy_left > 0) page = copies.page(copy_row, copy_lo, copy_hi, copy_key0);
     };
-    auto fetch = [&]() -> bool {   // a block, in a group of its own
-        if (ahead < p.blocks) copies.issue(p, span, (p.top - ahead) * kPgKeys, page, into);
-        else if (have_next && ahead < p.blocks + next.blocks) copies.issue(next, next_span, (next.top - (ahead - p.blocks)) * kPgKeys, page, into);
-        else return false;
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        ++ahead;
-        into = into == kPcStages - 1 ? 0 : into + 1;
-        look();
-        return true;
-    };
+    bool more = walk(0);
     if (more) {
-        look();
-        while (ahead < kPcStages - 1 && fetch()) {}
+        have_next = walk(1);
+        copy_from(0);
+        if (copy_left == 0 && have_next) copy_from(1);
     }
 
     while (more) {
-        const int token0 = p.tile * tile_tokens;
+        const PgPiece& p = sm.piece[warp][now];
+        const int token0 = p.tile * tile_tokens, blocks = p.blocks;
         const int rows = min(tile_tokens, p.s.tokens - token0) * group;
-        if (p.s.p0 + p.s.tokens > cap && threadIdx.x == 0) g_device_status = 6;
+        const PgSpan span = span_of(p);
+        int all_low, all_high;     // keys that every row sees
+        {
+            const long long cap = (long long)a.max_pages << a.page_shift;
+            const int last = (int)min(cap, 0x7fffffffLL) - 1;      // position that has a place in the table
+            if (p.s.p0 + p.s.tokens > cap && threadIdx.x == 0) g_device_status = 6;
+            __syncwarp();
+            if (lane < kRows) {
+                const bool valid = lane < rows;
+                const int pos = p.s.p0 + token0 + lane / group;
+                row_of.pos[lane] = pos;
+                row_of.low[lane] = !valid ? 0 : a.window > 0 ? (int)max((long long)p.s.first, (long long)pos - a.window + 1) : p.s.first;
+                row_of.high[lane] = valid ? min(pos, last) : 0x7fffffff;   // (a row that stands for no token takes what comes)
+                row_of.slope[lane] = a.slopes != nullptr && valid ? a.slopes[p.head * group + lane % group] * kLog2e : 0.f;
+            }
+            __syncwarp();
+            all_low = row_of.low[rows - 1], all_high = row_of.high[0];
+        }
         // Q: lane (g, t) holds dims D / 4 t .. of rows g, and what of rows 2 t and 2 t + 1 the scores need
         uint32_t q[kN][kSteps][2];
-        float factor[kN][2], slope[kN][2], ref[kN][2], l[kN][2];
-        int low[kN][2], high[kN][2], pos[kN][2];
+        float factor[kN][2], ref[kN][2], l[kN][2];
 #pragma unroll
         for (int n = 0; n < kN; ++n) {
             const int r = 8 * n + g;
@@ -252,16 +282,9 @@ paged_mha_codes_kernel(const __grid_constant__ PagedMhaArgs a, void* ws, int mos
             }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const int row = 8 * n + 2 * t + i;
                 const int down = __shfl_sync(0xffffffffu, e, 4 * (2 * t + i));
                 factor[n][i] = a.scale * kLog2e * __uint_as_float((uint32_t)(127 - down / 2) << 23) *
                                __uint_as_float((uint32_t)(127 - (down - down / 2)) << 23);
-                const bool valid = row < rows;
-                pos[n][i] = p.s.p0 + token0 + row / group;
-                low[n][i] = valid ? p.s.first : 0;
-                if (valid && a.window > 0) low[n][i] = (int)max((long long)low[n][i], (long long)pos[n][i] - a.window + 1);
-                high[n][i] = valid ? min(pos[n][i], last) : 0x7fffffff;   // (a row that stands for no token takes what comes)
-                slope[n][i] = a.slopes != nullptr && valid ? a.slopes[p.head * group + row % group] * kLog2e : 0.f;
                 ref[n][i] = kPgNone;
                 l[n][i] = 0.f;
             }
@@ -275,174 +298,197 @@ paged_mha_codes_kernel(const __grid_constant__ PagedMhaArgs a, void* ws, int mos
                 for (int e = 0; e < 4; ++e) o[n][i][e] = 0.f;
             }
         }
-        // blocks all of whose keys every row sees
-        const int pos0 = p.s.p0 + token0, pos1 = pos0 + (rows - 1) / group;
-        const int all_high = min(pos0, last), all_low = a.window > 0 ? (int)max((long long)p.s.first, (long long)pos1 - a.window + 1) : p.s.first;
         bool huge = false;
         int used = stage;          // stage of the piece's last block
-        for (int j = 0; j < p.blocks; ++j) {
-            if (ahead - j > kPcStages - 2) asm volatile("cp.async.wait_group %0;" ::"n"(kPcStages - 2) : "memory");
+        int key0 = p.top * kPgKeys + copies.offset;
+        for (int j = 0; j < blocks; ++j, key0 -= kPgKeys) {
+            __syncwarp();          // all lanes have read the block before, whose stage is the next to be copied to
+            while (ahead < Shape::kStages && copy_left > 0) {
+                copies.issue(copy_head, copy_lo, copy_hi, copy_key0, page, into);
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                ++ahead;
+                into = into == Shape::kStages - 1 ? 0 : into + 1;
+                copy_key0 -= kPgKeys;
+                if (--copy_left > 0) page = copies.page(copy_row, copy_lo, copy_hi, copy_key0);
+                else if (!copy_next && have_next) copy_from(now ^ 1);
+            }
+            if (ahead >= Shape::kStages) asm volatile("cp.async.wait_group %0;" ::"n"(Shape::kStages - 1) : "memory");
+            else if (ahead == Shape::kStages - 1) asm volatile("cp.async.wait_group %0;" ::"n"(Shape::kStages - 2) : "memory");
             else asm volatile("cp.async.wait_group 0;" ::: "memory");
             __syncwarp();
+            --ahead;
             used = stage;
-            fetch();               // (to the stage of the block before, which all lanes have read before the barrier above)
             const uint32_t at = copies.ring + (uint32_t)(stage * Shape::kStage);
-            stage = stage == kPcStages - 1 ? 0 : stage + 1;
-            const int key0 = (p.top - j) * kPgKeys + copies.offset;
-            if (key0 >= span.hi || key0 + kPcKeys <= span.lo) continue;
-            // ---- scores
-            float s[2][kN][4];
+            stage = stage == Shape::kStages - 1 ? 0 : stage + 1;
+            if (key0 >= span.hi || key0 + Shape::kKeys <= span.lo) continue;
+            const bool masked = key0 < all_low || key0 + Shape::kKeys - 1 > all_high;
+#pragma unroll 1
+            for (int m0 = 0; m0 < Shape::kKeys / 16; m0 += Shape::kAtOnce) {
+                constexpr int kM = Shape::kAtOnce;
+                const uint32_t at_m = at + (uint32_t)(m0 * 16 * D);
+                const int key_m = key0 + 16 * m0 + g;
+                // ---- scores
+                float s[kM][kN][4];
 #pragma unroll
-            for (int m = 0; m < 2; ++m) {
-#pragma unroll
-                for (int n = 0; n < kN; ++n) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) s[m][n][e] = 0.f;
-                }
-#pragma unroll
-                for (int h = 0; h < D / 64; ++h) {
-                    const int c = D / 64 * t + h;
-                    const uint4 x = lds128(at + pc_place<D>(16 * m + g, c)), y = lds128(at + pc_place<D>(16 * m + 8 + g, c));
-                    const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint32_t a0, a1, a2, a3;
-                        codes_to_half<kCodes>(xs[i], a0, a2);
-                        codes_to_half<kCodes>(ys[i], a1, a3);
-#pragma unroll
-                        for (int n = 0; n < kN; ++n) mma_m16n8k16(s[m][n], a0, a1, a2, a3, q[n][4 * h + i][0], q[n][4 * h + i][1]);
-                    }
-                }
-            }
-            // ---- weights
-            float vs[2][2], top_scale = 8.67361738e-19f;   // (2^-60: a scale of zero weighs nothing)
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const uint32_t place = at + 2 * Shape::kTile + (uint32_t)((16 * m + 8 * i + g) * 4);
-                    float ks;
-                    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(ks) : "r"(place));
-                    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(vs[m][i]) : "r"(place + kPcKeys * 4));
-                    top_scale = fmaxf(top_scale, vs[m][i]);
+                for (int m = 0; m < kM; ++m) {
 #pragma unroll
                     for (int n = 0; n < kN; ++n) {
 #pragma unroll
-                        for (int r = 0; r < 2; ++r) s[m][n][2 * i + r] *= ks * factor[n][r];
+                        for (int e = 0; e < 4; ++e) s[m][n][e] = 0.f;
+                    }
+#pragma unroll
+                    for (int h = 0; h < D / 64; ++h) {
+                        const int c = D / 64 * t + h;
+                        const uint4 x = lds128(at_m + 16 * m * D + pc_place<D>(g, c)), y = lds128(at_m + 16 * m * D + pc_place<D>(8 + g, c));
+                        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            uint32_t a0, a1, a2, a3;
+                            codes_to_half<kCodes>(xs[i], a0, a2);
+                            codes_to_half<kCodes>(ys[i], a1, a3);
+#pragma unroll
+                            for (int n = 0; n < kN; ++n) mma_m16n8k16(s[m][n], a0, a1, a2, a3, q[n][4 * h + i][0], q[n][4 * h + i][1]);
+                        }
                     }
                 }
-            }
-            if (a.slopes != nullptr) {
+                // ---- weights
+                float vs[kM][2], top_scale = 8.67361738e-19f;   // (2^-60: a scale of zero weighs nothing)
 #pragma unroll
-                for (int n = 0; n < kN; ++n) {
+                for (int m = 0; m < kM; ++m) {
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const int i = k >> 1 & 1, r = k & 1;
-                        float& x = s[k >> 2][n][2 * i + r];
-                        x = fmaf(slope[n][r], (float)(key0 + 16 * (k >> 2) + 8 * i + g - pos[n][r]), x);
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t place = at + 2 * Shape::kTile + (uint32_t)((16 * (m0 + m) + 8 * i + g) * 4);
+                        float ks;
+                        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(ks) : "r"(place));
+                        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(vs[m][i]) : "r"(place + Shape::kKeys * 4));
+                        top_scale = fmaxf(top_scale, vs[m][i]);
+#pragma unroll
+                        for (int n = 0; n < kN; ++n) {
+#pragma unroll
+                            for (int r = 0; r < 2; ++r) s[m][n][2 * i + r] *= ks * factor[n][r];
+                        }
                     }
                 }
-            }
-            if (key0 < all_low || key0 + kPcKeys - 1 > all_high) {
+                if (a.slopes != nullptr) {
 #pragma unroll
-                for (int n = 0; n < kN; ++n) {
+                    for (int n = 0; n < kN; ++n) {
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const int i = k >> 1 & 1, r = k & 1, key = key0 + 16 * (k >> 2) + 8 * i + g;
-                        float& x = s[k >> 2][n][2 * i + r];
-                        x = key >= low[n][r] && key <= high[n][r] ? x : -INFINITY;
+                        for (int r = 0; r < 2; ++r) {
+                            const int row = 8 * n + 2 * t + r;
+                            const float slope = row_of.slope[row], from = (float)(key_m - row_of.pos[row]);
+#pragma unroll
+                            for (int k = 0; k < 2 * kM; ++k) {
+                                float& x = s[k >> 1][n][2 * (k & 1) + r];
+                                x = fmaf(slope, from + 8.0f * k, x);
+                            }
+                        }
                     }
                 }
-            }
-            // (with the largest scale of the lane's keys: never too small, and looked at closely where it says so)
-            bool over = false;
-            const float most = __log2f(top_scale) - kPgLag - kUp;
+                if (masked) {
 #pragma unroll
-            for (int n = 0; n < kN; ++n) {
+                    for (int n = 0; n < kN; ++n) {
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const float m = fmaxf(fmaxf(s[0][n][r], s[0][n][2 + r]), fmaxf(s[1][n][r], s[1][n][2 + r]));
-                    over |= m + most > ref[n][r];
+                        for (int r = 0; r < 2; ++r) {
+                            const int row = 8 * n + 2 * t + r, low = row_of.low[row] - key_m, high = row_of.high[row] - key_m;
+#pragma unroll
+                            for (int k = 0; k < 2 * kM; ++k) {
+                                if (8 * k < low || 8 * k > high) s[k >> 1][n][2 * (k & 1) + r] = -INFINITY;
+                            }
+                        }
+                    }
                 }
-            }
-            if (__any_sync(0xffffffffu, over)) {
-                // some row's reference moves
+                // (with the largest scale of the lane's keys: never too small, and looked at closely where it says so)
+                bool over = false;
+                const float most = __log2f(top_scale) - kPgLag - kUp;
 #pragma unroll
                 for (int n = 0; n < kN; ++n) {
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-                        float m = -INFINITY;
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            m = fmaxf(m, s[k >> 1][n][2 * (k & 1) + r] + __log2f(fmaxf(vs[k >> 1][k & 1], 8.67361738e-19f)));
-                        }
-#pragma unroll
-                        for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-                        const bool moves = m - ref[n][r] > kPgLag + kUp;
-                        const float to = moves ? m - kUp : ref[n][r], corr = moves ? ex2_approx(ref[n][r] - to) : 1.0f;
-                        ref[n][r] = to;
-                        huge |= fabsf(to) >= 1048576.0f && moves;
-                        l[n][r] *= corr;
-#pragma unroll
-                        for (int i = 0; i < kSteps; ++i) {
-                            o[n][i][r] *= corr;
-                            o[n][i][2 + r] *= corr;
-                        }
+                        float top = fmaxf(s[0][n][r], s[0][n][2 + r]);
+                        if (kM == 2) top = fmaxf(top, fmaxf(s[kM - 1][n][r], s[kM - 1][n][2 + r]));
+                        over |= top + most > ref[n][r];
                     }
                 }
-            }
-            uint32_t w[2][kN][2];
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
+                if (__any_sync(0xffffffffu, over)) {
+                    // some row's reference moves
 #pragma unroll
                     for (int n = 0; n < kN; ++n) {
-                        float e[2];
 #pragma unroll
                         for (int r = 0; r < 2; ++r) {
-                            const float power = ex2_approx(s[m][n][2 * i + r] - ref[n][r]);
-                            l[n][r] += power;
-                            e[r] = power * vs[m][i];
-                        }
-                        if (huge) {   // (beyond 2^20 a score knows little of log2 s^v, and a weight could leave fp16)
+                            float top = -INFINITY;
 #pragma unroll
-                            for (int r = 0; r < 2; ++r) asm("min.NaN.f32 %0, %0, %1;" : "+f"(e[r]) : "f"(65504.0f));
+                            for (int k = 0; k < 2 * kM; ++k) {
+                                top = fmaxf(top, s[k >> 1][n][2 * (k & 1) + r] + __log2f(fmaxf(vs[k >> 1][k & 1], 8.67361738e-19f)));
+                            }
+#pragma unroll
+                            for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+                            const bool moves = top - ref[n][r] > kPgLag + kUp;
+                            const float to = moves ? top - kUp : ref[n][r], corr = moves ? ex2_approx(ref[n][r] - to) : 1.0f;
+                            ref[n][r] = to;
+                            huge |= fabsf(to) >= 1048576.0f && moves;
+                            l[n][r] *= corr;
+#pragma unroll
+                            for (int i = 0; i < kSteps; ++i) {
+                                o[n][i][r] *= corr;
+                                o[n][i][2 + r] *= corr;
+                            }
                         }
-                        const __half2 h = __floats2half2_rn(e[0], e[1]);
-                        w[m][n][i] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h));
                     }
                 }
-            }
-            // ---- sums
+                uint32_t w[kM][kN][2];
 #pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                constexpr int kWords = D / 32;     // of the D / 8 bytes of a key that a lane has
-                uint32_t v[4][kWords];             // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int row = 16 * m + 2 * t + (k & 1) + 8 * (k >> 1);
-                    if (D == 128) {
-                        const uint4 x = lds128(at + Shape::kTile + pc_place<D>(row, g));
-                        v[k][0] = x.x, v[k][1] = x.y, v[k][2 % kWords] = x.z, v[k][3 % kWords] = x.w;
-                    }
-                    else {
-                        const uint2 x = lds64(at + Shape::kTile + pc_place<D>(row, g >> 1) + (uint32_t)((g & 1) * 8));
-                        v[k][0] = x.x, v[k][1] = x.y;
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < kWords; ++i) {
-                    // dims 4 i .. 4 i + 3 of the lane's, pairs of keys
-                    uint32_t lo[4], hi[4];
-                    codes_to_half<kCodes>(__byte_perm(v[0][i], v[1][i], 0x5140), lo[0], lo[1]);
-                    codes_to_half<kCodes>(__byte_perm(v[0][i], v[1][i], 0x7362), lo[2], lo[3]);
-                    codes_to_half<kCodes>(__byte_perm(v[2][i], v[3][i], 0x5140), hi[0], hi[1]);
-                    codes_to_half<kCodes>(__byte_perm(v[2][i], v[3][i], 0x7362), hi[2], hi[3]);
+                for (int m = 0; m < kM; ++m) {
 #pragma unroll
                     for (int n = 0; n < kN; ++n) {
-                        mma_m16n8k16(o[n][2 * i], lo[0], lo[1], hi[0], hi[1], w[m][n][0], w[m][n][1]);
-                        mma_m16n8k16(o[n][2 * i + 1], lo[2], lo[3], hi[2], hi[3], w[m][n][0], w[m][n][1]);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            float e[2];
+#pragma unroll
+                            for (int r = 0; r < 2; ++r) {
+                                const float power = ex2_approx(s[m][n][2 * i + r] - ref[n][r]);
+                                l[n][r] += power;
+                                e[r] = power * vs[m][i];
+                            }
+                            if (huge) {   // (beyond 2^20 a score knows little of log2 s^v, and a weight could leave fp16)
+#pragma unroll
+                                for (int r = 0; r < 2; ++r) asm("min.NaN.f32 %0, %0, %1;" : "+f"(e[r]) : "f"(65504.0f));
+                            }
+                            const __half2 h = __floats2half2_rn(e[0], e[1]);
+                            w[m][n][i] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h));
+                        }
+                    }
+                }
+                // ---- sums
+#pragma unroll
+                for (int m = 0; m < kM; ++m) {
+                    constexpr int kWords = D / 32;     // of the D / 8 bytes of a key that a lane has
+                    uint32_t v[4][kWords];             // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t tile = at_m + 16 * m * D + Shape::kTile;
+                        const int row = 2 * t + (k & 1) + 8 * (k >> 1);
+                        if (D == 128) {
+                            const uint4 x = lds128(tile + pc_place<D>(row, g));
+                            v[k][0] = x.x, v[k][1] = x.y, v[k][2 % kWords] = x.z, v[k][3 % kWords] = x.w;
+                        }
+                        else {
+                            const uint2 x = lds64(tile + pc_place<D>(row, g >> 1) + (uint32_t)((g & 1) * 8));
+                            v[k][0] = x.x, v[k][1] = x.y;
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < kWords; ++i) {
+                        // dims 4 i .. 4 i + 3 of the lane's, pairs of keys
+                        uint32_t lo[4], hi[4];
+                        codes_to_half<kCodes>(__byte_perm(v[0][i], v[1][i], 0x5140), lo[0], lo[1]);
+                        codes_to_half<kCodes>(__byte_perm(v[0][i], v[1][i], 0x7362), lo[2], lo[3]);
+                        codes_to_half<kCodes>(__byte_perm(v[2][i], v[3][i], 0x5140), hi[0], hi[1]);
+                        codes_to_half<kCodes>(__byte_perm(v[2][i], v[3][i], 0x7362), hi[2], hi[3]);
+#pragma unroll
+                        for (int n = 0; n < kN; ++n) {
+                            mma_m16n8k16(o[n][2 * i], lo[0], lo[1], hi[0], hi[1], w[m][n][0], w[m][n][1]);
+                            mma_m16n8k16(o[n][2 * i + 1], lo[2], lo[3], hi[2], hi[3], w[m][n][0], w[m][n][1]);
+                        }
                     }
                 }
             }
@@ -463,9 +509,9 @@ paged_mha_codes_kernel(const __grid_constant__ PagedMhaArgs a, void* ws, int mos
         }
         // O goes where the codes of the piece's last block were, [row][dim], rows D floats apart and rotated against the banks.  (Nothing
         // is on its way there: the copies that follow go to that stage with the next block.)
-        float* mine = reinterpret_cast<float*>(pc_dyn + (warp * kPcStages + used) * Shape::kStage);
+        float* mine = reinterpret_cast<float*>(pc_dyn + (warp * Shape::kStages + used) * Shape::kStage);
         __syncwarp();
-        if (p.blocks > 0) {
+        if (blocks > 0) {
 #pragma unroll
             for (int n = 0; n < kN; ++n) {
 #pragma unroll
@@ -481,22 +527,22 @@ paged_mha_codes_kernel(const __grid_constant__ PagedMhaArgs a, void* ws, int mos
         __syncthreads();
         const bool complete = p.starts && p.ends;
         const PgPartial part = pg_partial(ws, ctas, cta, p.starts ? 1 : 0, kRows, D);
-        for (int i = threadIdx.x; i < rows * (D / 4); i += kPcThreads) {
+        for (int i = threadIdx.x; i < rows * (D / 4); i += 32 * Shape::kWarps) {
             const int row = i / (D / 4), d = i % (D / 4) * 4;
             float top = kPgNone, sum = 0.f;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int w = 0; w < kPcWarps; ++w) {
+            for (int w = 0; w < Shape::kWarps; ++w) {
                 if (sm.sum[w][row] != 0.f) top = fmaxf(top, sm.ref[w][row]);
             }
 #pragma unroll
-            for (int w = 0; w < kPcWarps; ++w) {
+            for (int w = 0; w < Shape::kWarps; ++w) {
                 const float part_sum = sm.sum[w][row];
                 if (part_sum == 0.f) continue;      // (it has seen nothing)
                 const float f = ex2_approx(sm.ref[w][row] - top);
                 sum += part_sum * f;
                 const float4 x = *reinterpret_cast<const float4*>(
-                    reinterpret_cast<const float*>(pc_dyn + (w * kPcStages + used) * Shape::kStage) + row * D + ((d + 8 * row) & (D - 1)));
+                    reinterpret_cast<const float*>(pc_dyn + (w * Shape::kStages + used) * Shape::kStage) + row * D + ((d + 8 * row) & (D - 1)));
                 v.x += x.x * f, v.y += x.y * f, v.z += x.z * f, v.w += x.w * f;
             }
             const float f = complete ? (sum == 0.f ? 0.f : 1.0f / sum) : 1.0f;
@@ -519,16 +565,11 @@ paged_mha_codes_kernel(const __grid_constant__ PagedMhaArgs a, void* ws, int mos
         }
         __syncthreads();   // the stage is free again
         more = have_next;
-        ahead -= p.blocks;
-        p = next;
-        span = next_span;
-        if (more) {
-            const bool waiting = ahead == p.blocks;   // the copies, for the piece behind
-            have_next = share.next(a, tiling, next);
-            if (have_next) next_span = span_of(next);
-            if (waiting) look();
-            while (ahead < kPcStages - 1 && fetch()) {}
-        }
+        if (!more) break;
+        have_next = walk(now);
+        now ^= 1;
+        if (copy_next && copy_left > 0) copy_next = false;   // in the piece at work now
+        else if (have_next) copy_from(now ^ 1);              // that one is copied, or has nothing to copy
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
@@ -537,7 +578,7 @@ template<int kCodes, int D, int kRows>
 int pc_launch(const PagedMhaArgs& a, void* ws, int most, int whole, cudaStream_t stream)
 {
     auto kern = paged_mha_codes_kernel<kCodes, D, kRows>;
-    constexpr int kSmem = PcShape<D>::kSmem;
+    constexpr int kSmem = PcShape<D, kRows>::kSmem;
     static bool attr_set[64] = {};
     int dev = 0;
     EET_CUDA(cudaGetDevice(&dev));
@@ -546,7 +587,7 @@ int pc_launch(const PagedMhaArgs& a, void* ws, int most, int whole, cudaStream_t
         EET_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
         attr_set[dev] = true;
     }
-    EET_CUDA(launch_pdl(kern, dim3(kPcPerSm * sm_count()), dim3(kPcThreads), kSmem, stream, a, ws, most, whole));
+    EET_CUDA(launch_pdl(kern, dim3(PcShape<D, kRows>::kPerSm * sm_count()), dim3(32 * PcShape<D, kRows>::kWarps), kSmem, stream, a, ws, most, whole));
     return 0;
 }
 
@@ -578,7 +619,7 @@ static PagedCodesPlan paged_codes_plan(const PagedMhaArgs& a)
             p.few = p.rows / group;
         }
     }
-    if (p.rows) p.bytes[0] = pg_scratch_bytes(kPcPerSm * sm_count(), p.rows, a.head_dim);
+    if (p.rows) p.bytes[0] = pg_scratch_bytes(pc_per_sm(p.rows) * sm_count(), p.rows, a.head_dim);
     if (p.tiles) p.bytes[1] = pg_scratch_bytes(sm_count(), 2 * kPgRows, a.head_dim);
     return p;
 }
@@ -603,7 +644,7 @@ static int launch_paged_mha_codes_t(const PagedMhaArgs& a, const PagedCodesPlan&
     if (p.rows) {
         const int most = p.tiles ? p.few : 0x7fffffff;
         if (int rc = p.rows == 8 ? pc_launch<kCodes, D, 8>(a, ws[0], most, 0, stream) : pc_launch<kCodes, D, 16>(a, ws[0], most, 0, stream)) return rc;
-        if (int rc = join({ws[0], p.rows, 0}, kPcPerSm * sm_count())) return rc;
+        if (int rc = join({ws[0], p.rows, 0}, pc_per_sm(p.rows) * sm_count())) return rc;
     }
     if (p.tiles) {
         // (the tiles without a bias take the maximum of the scores before the scale, which a negative one would turn round)
