@@ -12,12 +12,13 @@
 //   4  those values, sorted, with exact sums in front of each: the cut.  (Where one bin of the second histogram holds more than the list can,
 //      as with very many equal values: bisection on x.)
 //   5  what is left, summed by threads in the order of the indices; the thread whose part of the sum the random number falls into draws
-// Sums are of w as whole multiples of 2^-44, from exp in 64 bits: whatever the number of CTAs and their order, they are the same, and a cut or
-// a draw lies where the definition puts it but for one chance in about 2^-44 times the vocabulary.  (In 32 bits a draw from 64000 tokens would
+// Sums are of w as whole multiples of 2^-44, from powers in 64 bits: whatever the number of CTAs and their order, they are the same, and a cut
+// or a draw lies where the definition puts it but for one chance in about 2^-44 times the vocabulary.  (In 32 bits a draw from 64000 tokens would
 // miss the border of some token once in some hundred rows.)
 //
 // A row is worked on by a cluster of 1 to 8 CTAs, which hold it in shared memory and exchange counts and candidates there.  Bound: latency,
-// seven barriers of the cluster and as many trips through a slice of the row.
+// six barriers of the cluster and four trips through a slice of the row; with many rows the issue of instructions, the powers of all
+// tokens first (11 instructions in 64 bits each, with a table of 128; exp() took three times as long).
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -37,9 +38,13 @@ constexpr float kSaBinsPerE = 64.0f;
 constexpr int kSaList = 4096;
 constexpr int kSaMaxCluster = 8;
 constexpr int kSaMaxVocab = 1 << 18;         // their sum of w stays below 2^62
-constexpr int kSaMaxSlice = 160 * 1024;      // bytes of a row in a CTA
+constexpr int kSaMaxSlice = 128 * 1024;      // bytes of a row in a CTA at the most,
+constexpr int kSaSlice = 68 * 1024;          // and where there are CTAs for more of them: two share an SM
 constexpr double kSaUnit = 17592186044416.0; // 2^44
 constexpr uint32_t kSaNothing = 0x007fffffu; // the key of -inf
+
+constexpr int kSaTable = 128;                // powers of 2^(1 / 128)
+constexpr int kSaCounted = 256;              // lists up to here are sorted by counting
 
 typedef unsigned long long u64;
 
@@ -55,6 +60,7 @@ struct SaBracket {
 };
 
 struct SaSmem {
+    double table[kSaTable];
     uint32_t hist[kSaBins], fine[kSaBins];
     uint32_t list[kSaList];
     uint32_t listed;
@@ -67,11 +73,10 @@ struct SaSmem {
     SaCut cut;
     // of this CTA
     u64 warp_sum[kSaWarps];
-    double warp_low[kSaWarps], warp_high[kSaWarps];
     uint32_t warp_count[kSaWarps];
+    double warp_low[kSaWarps], warp_high[kSaWarps];
     float warp_max[kSaWarps];
-    uint32_t total;
-    u64 mass;
+    uint32_t front, upto;
 };
 
 // Values in an order of whole numbers; -0 has become 0 and NaN -inf before.
@@ -91,71 +96,92 @@ __device__ __forceinline__ float sa_clean(float x)
     return x == x ? x + 0.0f : -INFINITY;
 }
 
-__device__ __forceinline__ float sa_float(float x) { return x; }
-__device__ __forceinline__ float sa_float(__half x) { return __half2float(x); }
-__device__ __forceinline__ float sa_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+// The words of a row in shared memory: one or two values each.
+template<typename T>
+struct SaWord;
+template<>
+struct SaWord<float> {
+    static constexpr int kValues = 1;
+    static constexpr uint32_t kNothing = 0xff800000u;
+    static __device__ __forceinline__ float get(uint32_t w, int) { return __uint_as_float(w); }
+};
+template<>
+struct SaWord<__half> {
+    static constexpr int kValues = 2;
+    static constexpr uint32_t kNothing = 0xfc00fc00u;
+    static __device__ __forceinline__ float get(uint32_t w, int i) { return __half2float(__ushort_as_half((unsigned short)(i ? w >> 16 : w & 0xffffu))); }
+};
+template<>
+struct SaWord<__nv_bfloat16> {
+    static constexpr int kValues = 2;
+    static constexpr uint32_t kNothing = 0xff80ff80u;
+    static __device__ __forceinline__ float get(uint32_t w, int i) { return __uint_as_float(i ? w & 0xffff0000u : w << 16); }
+};
 
 struct SaRow {
     float top;
-    double over_t;       // 1 / T
-    float scale;         // bins a unit of x
-    // (max - x) / T, negative
+    float scale;          // bins a unit of x
+    double over_t;        // 1 / T
+    double fine;          // kSaTable log2(e) / T
+    const double* table;
+
+    // (x - max) / T
     __device__ __forceinline__ double power(float x) const { return x == top ? 0.0 : ((double)x - (double)top) * over_t; }
+    // w in multiples of 2^-44.  2^(t / 128) is 2^(k >> 7) times the table's entry k & 127 times a polynomial in what is left of t, at most half a
+    // step: the fourth power's rest is below 2^-49.
     __device__ __forceinline__ u64 weight(float x) const
     {
-        if (x == -INFINITY) return 0;
-        const double e = exp(power(x));
-        const u64 w = __double2ull_rn(e * kSaUnit);
-        return w == 0 && e > 0.0 ? 1 : w;   // (what can be drawn stays so)
+        if (x == top) return 1ull << 44;
+        const double t = ((double)x - (double)top) * fine;
+        if (!(t > -5568.0)) return t > -137600.0 ? 1 : 0;   // below half a unit: what can be drawn stays so (down to exp(-745), a number's end)
+        constexpr double kShift = 6755399441055744.0;        // 1.5 2^52: whole numbers in the low bits
+        const double shifted = t + kShift;
+        const int k = __double2loint(shifted);
+        const double f = t - (shifted - kShift);
+        double p = 3.583032305400251e-11;                            // (ln 2 / 128)^4 / 24
+        p = fma(p, f, 2.6466421444330967e-8);                         // ^3 / 6
+        p = fma(p, f, 1.4662262387640423e-5);                         // ^2 / 2
+        p = fma(p, f, 5.4152123481245725e-3);                // ln 2 / 128
+        p = fma(p, f, 1.0);
+        const double e = table[k & (kSaTable - 1)] * p;
+        // times 2^(44 + (k >> 7)), then rounded by adding 2^52
+        const double w = __hiloint2double(__double2hiint(e) + ((44 + (k >> 7)) << 20), __double2loint(e)) + 4503599627370496.0;
+        const u64 units = (u64)__double_as_longlong(w) & 0xfffffffffffffull;
+        return units == 0 ? 1 : units;
     }
     __device__ __forceinline__ float place(float x) const { return (top - x) * scale; }
     __device__ __forceinline__ int bin(float x) const { return min(kSaBins - 1, (int)place(x)); }
     // bins of the second histogram: those of [b0, b1] cut into kSaBins
-    __device__ __forceinline__ int fine(float x, int b0, float per_bin) const
+    __device__ __forceinline__ int sub_bin(float x, int b0, float per_bin) const
     {
         return max(0, min(kSaBins - 1, (int)((place(x) - (float)b0) * per_bin)));
     }
 };
 
-// Sums over the threads in front of this one, and over all (to be read behind the barrier it ends with).
-template<typename V>
-__device__ __forceinline__ V sa_scan(V v, V* per_warp, V& all)
-{
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    V s = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const V u = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= o) s += u;
-    }
-    __syncthreads();   // per_warp may still be read
-    if (lane == 31) per_warp[warp] = s;
-    __syncthreads();
-    V before = 0;
-    all = 0;
-#pragma unroll
-    for (int w = 0; w < kSaWarps; ++w) {
-        if (w < warp) before += per_warp[w];
-        all += per_warp[w];
-    }
-    return before + s - v;
-}
-
 template<typename T>
 struct SaKernel {
+    using Word = SaWord<T>;
     SaSmem& sm;
-    const T* x;            // the slice, in shared memory
-    int n, run;            // its values; those of a thread, consecutive and an odd number
+    const uint32_t* x;     // the slice's words, in shared memory
+    int begin, end;        // this thread's: consecutive, an odd number to a thread, so that a warp's reads meet no bank twice
     int ranks, rank;
     SaRow row;
     int turn = 0;          // buffer of the next exchange
 
-    __device__ __forceinline__ float at(int i) const { return sa_clean(sa_float(x[i])); }
+    // f(value) for this thread's values, in the order of the indices; -inf among them
     template<typename F>
     __device__ __forceinline__ void each(F f) const
     {
-        const int begin = (int)threadIdx.x * run, end = min(n, begin + run);
-        for (int i = begin; i < end; ++i) f(at(i));
+        for (int i0 = begin; i0 < end; i0 += 4) {
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[k] = i0 + k < end ? x[i0 + k] : Word::kNothing;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+#pragma unroll
+                for (int h = 0; h < Word::kValues; ++h) f(sa_clean(Word::get(w[k], h)));
+            }
+        }
     }
     __device__ __forceinline__ void barrier() const
     {
@@ -168,199 +194,253 @@ struct SaKernel {
         return ranks > 1 ? cg::this_cluster().map_shared_rank(p, r) : p;
     }
 
-    // Sum and count of all CTAs' threads, to all; `before`, where asked for, those of the threads in front of this one.
-    __device__ __forceinline__ void exchange(u64 sum, uint32_t count, u64& all_sum, uint32_t& all_count, u64* sum_before = nullptr,
-                                             uint32_t* count_before = nullptr)
+    // Sums over the threads of the CTA in front of this one, and over all of them.
+    struct Sums {
+        u64 sum, sum_before;
+        uint32_t count, count_before;
+    };
+    __device__ __forceinline__ Sums scan(u64 sum, uint32_t count) const
     {
-        u64 cta_sum;
-        uint32_t cta_count;
-        u64 s = sa_scan(sum, sm.warp_sum, cta_sum);
-        uint32_t c = sa_scan(count, sm.warp_count, cta_count);
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        u64 s = sum;
+        uint32_t c = count;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const u64 u = __shfl_up_sync(0xffffffffu, s, o);
+            const uint32_t d = __shfl_up_sync(0xffffffffu, c, o);
+            if (lane >= o) s += u, c += d;
+        }
+        __syncthreads();   // the last scan's may still be read
+        if (lane == 31) sm.warp_sum[warp] = s, sm.warp_count[warp] = c;
+        __syncthreads();
+        Sums r = {0, s - sum, 0, c - count};
+#pragma unroll
+        for (int w = 0; w < kSaWarps; ++w) {
+            const u64 u = sm.warp_sum[w];
+            const uint32_t d = sm.warp_count[w];
+            if (w < warp) r.sum_before += u, r.count_before += d;
+            r.sum += u, r.count += d;
+        }
+        return r;
+    }
+    // Leaves a CTA's sums with all of the cluster, to be read with collect() behind a barrier.  (Whoever writes a buffer again has passed the
+    // barrier of the other one, behind everybody's reads.)
+    __device__ __forceinline__ void publish(const Sums& s)
+    {
         if ((int)threadIdx.x < ranks) {
-            *of(&sm.sums[turn][rank], threadIdx.x) = cta_sum;
-            *of(&sm.counts[turn][rank], threadIdx.x) = cta_count;
+            *of(&sm.sums[turn][rank], threadIdx.x) = s.sum;
+            *of(&sm.counts[turn][rank], threadIdx.x) = s.count;
         }
-        barrier();
-        all_sum = 0;
-        all_count = 0;
+    }
+    __device__ __forceinline__ Sums collect(Sums s)
+    {
+        s.sum = 0, s.count = 0;
         for (int r = 0; r < ranks; ++r) {
-            if (r < rank) {
-                s += sm.sums[turn][r];
-                c += sm.counts[turn][r];
-            }
-            all_sum += sm.sums[turn][r];
-            all_count += sm.counts[turn][r];
+            const u64 u = sm.sums[turn][r];
+            const uint32_t d = sm.counts[turn][r];
+            if (r < rank) s.sum_before += u, s.count_before += d;
+            s.sum += u, s.count += d;
         }
-        if (sum_before != nullptr) *sum_before = s;
-        if (count_before != nullptr) *count_before = c;
-        turn ^= 1;         // (whoever writes this buffer again has passed the barrier of the other one, behind everybody's reads)
+        turn ^= 1;
+        return s;
+    }
+    __device__ __forceinline__ Sums exchange(u64 sum, uint32_t count)
+    {
+        const Sums s = scan(sum, count);
+        publish(s);
+        barrier();
+        return collect(s);
     }
 
-    // Counts into `bins` of the first CTA; `f` is handed a value and answers its bin, or -1.
-    template<typename F>
-    __device__ __forceinline__ void histogram(uint32_t* bins, F f)
+    // This CTA's counts to those of the first.  (Its own are complete behind the barriers of a scan.)
+    __device__ __forceinline__ void merge(uint32_t* bins) const
     {
-        for (int i = threadIdx.x; i < kSaBins; i += kSaThreads) bins[i] = 0;
-        barrier();         // (the first CTA's are empty, too)
-        each([&](float v) {
-            const int b = f(v);
-            if (b >= 0) atomicAdd(&bins[b], 1u);
-        });
-        if (rank > 0) {
-            __syncthreads();
-            uint32_t* first = of(bins, 0);
-            for (int i = threadIdx.x; i < kSaBins; i += kSaThreads) {
-                if (bins[i] != 0) atomicAdd(&first[i], bins[i]);
-            }
+        if (rank == 0) return;
+        uint32_t* first = of(bins, 0);
+        for (int i = threadIdx.x; i < kSaBins; i += kSaThreads) {
+            if (bins[i] != 0) atomicAdd(&first[i], bins[i]);
         }
-        barrier();
     }
 
     // The bins of the first CTA's histogram that hold the cut, by that CTA; to all.
     //   by count   the one in which the count passes `k`, `counted` values standing in front of all of them
     //   by mass    those in which the sum of w may pass `goal`, `mass` standing in front; bin b's are between e^(-low(b + 1)) and e^(-low(b))
+    // `total` values are in the bins; what they do not say is in the last one.  open_end: it holds all that lie behind.
     template<typename F>
-    __device__ __forceinline__ SaBracket narrow(const uint32_t* bins, bool by_mass, uint32_t k, uint32_t counted, double goal, double mass,
-                                                F low, bool open_end)
+    __device__ __forceinline__ SaBracket narrow(const uint32_t* bins, uint32_t total, bool by_mass, uint32_t k, uint32_t counted, double goal,
+                                                double mass, F low, bool open_end)
     {
         if (rank == 0) {
-            uint32_t c[kSaPerThread], sum = 0, all;
+            const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, first = threadIdx.x * kSaPerThread;
+            uint32_t c[kSaPerThread], count = 0;
+            double lo[kSaPerThread], hi[kSaPerThread], low_sum = 0, high_sum = 0;
 #pragma unroll
             for (int i = 0; i < kSaPerThread; ++i) {
-                c[i] = bins[threadIdx.x * kSaPerThread + i];
-                sum += c[i];
-            }
-            if (threadIdx.x == 0) sm.bracket = {kSaBins - 1, kSaBins - 1, 0, 0};   // (there behind the barriers of the sum)
-            const uint32_t before = sa_scan(sum, sm.warp_count, all);
-            if (by_mass) {
-                double lo[kSaPerThread], hi[kSaPerThread], lo_sum = 0, hi_sum = 0, rest;
-#pragma unroll
-                for (int i = 0; i < kSaPerThread; ++i) {
-                    const int b = threadIdx.x * kSaPerThread + i;
+                const int b = first + i;
+                c[i] = bins[b];
+                count += c[i];
+                lo[i] = hi[i] = 0;
+                if (by_mass && c[i] > 0) {
                     // (2e-5: what single precision may do to a value's place, and expf)
                     hi[i] = c[i] * kSaUnit * (double)(expf(-low(b)) * 1.00002f);
                     lo[i] = open_end && b == kSaBins - 1 ? 0.0 : c[i] * kSaUnit * (double)(expf(-low(b + 1)) * 0.99998f);
-                    lo_sum += lo[i];
-                    hi_sum += hi[i];
                 }
-                double lo_before = mass + sa_scan(lo_sum, sm.warp_low, rest), hi_before = mass + sa_scan(hi_sum, sm.warp_high, rest);
-#pragma unroll
-                for (int i = 0; i < kSaPerThread; ++i) {
-                    const int b = threadIdx.x * kSaPerThread + i;
-                    if (hi_before < goal && hi_before + hi[i] >= goal) sm.bracket.b0 = b;
-                    if (lo_before < goal && lo_before + lo[i] >= goal) sm.bracket.b1 = b;
-                    hi_before += hi[i];
-                    lo_before += lo[i];
-                }
+                low_sum += lo[i];
+                high_sum += hi[i];
             }
-            else {
-                uint32_t at = counted + before;
+            if (threadIdx.x == 0) {
+                sm.bracket.b0 = sm.bracket.b1 = kSaBins - 1;
+                sm.front = sm.upto = 0xffffffffu;
+            }
+            uint32_t cs = count;
+            double ls = low_sum, hs = high_sum;
 #pragma unroll
-                for (int i = 0; i < kSaPerThread; ++i) {
-                    if (at < k && at + c[i] >= k) sm.bracket.b0 = sm.bracket.b1 = threadIdx.x * kSaPerThread + i;
-                    at += c[i];
-                }
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t cu = __shfl_up_sync(0xffffffffu, cs, o);
+                const double lu = __shfl_up_sync(0xffffffffu, ls, o), hu = __shfl_up_sync(0xffffffffu, hs, o);
+                if (lane >= o) cs += cu, ls += lu, hs += hu;
             }
             __syncthreads();
-            const int b0 = sm.bracket.b0, b1 = sm.bracket.b1;
-            uint32_t in = 0, front = 0;
+            if (lane == 31) sm.warp_count[warp] = cs, sm.warp_low[warp] = ls, sm.warp_high[warp] = hs;
+            __syncthreads();
+            uint32_t at = cs - count, all = 0;
+            double low_at = mass + (ls - low_sum), high_at = mass + (hs - high_sum);
+#pragma unroll
+            for (int w = 0; w < kSaWarps; ++w) {
+                if (w < warp) at += sm.warp_count[w], low_at += sm.warp_low[w], high_at += sm.warp_high[w];
+                all += sm.warp_count[w];
+            }
+            if (threadIdx.x == kSaThreads - 1) {
+                c[kSaPerThread - 1] += total - all;
+                if (by_mass) hi[kSaPerThread - 1] = c[kSaPerThread - 1] * kSaUnit * (double)(expf(-low(kSaBins - 1)) * 1.00002f);
+            }
 #pragma unroll
             for (int i = 0; i < kSaPerThread; ++i) {
-                const int b = threadIdx.x * kSaPerThread + i;
-                front += b < b0 ? c[i] : 0;
-                in += b >= b0 && b <= b1 ? c[i] : 0;
+                if (by_mass) {
+                    if (high_at < goal && high_at + hi[i] >= goal) sm.bracket.b0 = first + i, sm.front = at;
+                    if (low_at < goal && low_at + lo[i] >= goal) sm.bracket.b1 = first + i, sm.upto = at + c[i];
+                    high_at += hi[i];
+                    low_at += lo[i];
+                }
+                else if (counted + at < k && counted + at + c[i] >= k) {
+                    sm.bracket.b0 = sm.bracket.b1 = first + i;
+                    sm.front = at;
+                    sm.upto = at + c[i];
+                }
+                at += c[i];
             }
-            uint32_t all_in, all_front;
-            sa_scan(in, sm.warp_count, all_in);
-            sa_scan(front, sm.warp_count, all_front);
-            if ((int)threadIdx.x < ranks) *of(&sm.bracket, threadIdx.x) = {b0, b1, all_in, counted + all_front};
+            __syncthreads();
+            // (sums of doubles over the warps are rounded: a border between two threads may be nobody's, and then all bins are looked at)
+            const bool none = sm.front == 0xffffffffu;
+            const uint32_t upto = sm.upto == 0xffffffffu ? total : sm.upto, front = none ? 0 : min(sm.front, upto);
+            const SaBracket found = {none ? 0 : min(sm.bracket.b0, sm.bracket.b1), sm.bracket.b1, upto - front, counted + front};
+            __syncthreads();
+            if ((int)threadIdx.x < ranks) *of(&sm.bracket, threadIdx.x) = found;
         }
         barrier();
         return sm.bracket;
     }
 
-    // The list of values between the cut's bins into the first CTA, sorted from the largest; returns the sum of w of those in front.
-    // f(v): 0 in front, 1 in the bins, 2 behind.
+    // The values between the cut's bins into the first CTA's list, and the sum of w of those in front.  f(v): 0 in front, 1 in the bins, 2 behind.
     template<typename F>
-    __device__ __forceinline__ u64 gather(uint32_t count, bool sums, F f)
+    __device__ __forceinline__ u64 gather(bool sums, F f)
     {
-        if (rank == 0 && threadIdx.x == 0) sm.listed = 0;
-        barrier();
         u64 front = 0;
         uint32_t* listed = of(&sm.listed, 0);
         uint32_t* list = of(sm.list, 0);
         each([&](float v) {
-            const int where = f(v);
+            const int where = v == -INFINITY ? 2 : f(v);
             if (where == 0 && sums) front += row.weight(v);
             if (where == 1) {
                 const uint32_t i = atomicAdd(listed, 1u);
                 if (i < kSaList) list[i] = sa_key(v);
             }
         });
-        u64 all_front;
-        uint32_t none;
-        exchange(front, 0, all_front, none);
-        if (rank == 0) {
-            int size = 32;
-            while (size < (int)count) size <<= 1;
-            for (int i = count + threadIdx.x; i < size; i += kSaThreads) sm.list[i] = 0;
-            __syncthreads();
-            for (int k = 2; k <= size; k <<= 1) {
-                for (int j = k >> 1; j > 0; j >>= 1) {
-                    for (int i = threadIdx.x; i < size / 2; i += kSaThreads) {
-                        const int a = 2 * i - (i & (j - 1)), b = a + j;
-                        const uint32_t u = sm.list[a], v = sm.list[b];
-                        if ((u < v) == ((a & k) == 0)) {
-                            sm.list[a] = v;
-                            sm.list[b] = u;
-                        }
-                    }
-                    __syncthreads();
-                }
-            }
-        }
-        return all_front;
+        return exchange(front, 0).sum;
     }
 
-    // By the first CTA, the cut in the sorted list: of `count` values, in front of which stand `before` with the sum `front`.  Leaves the first
-    // `k` (none of them at all: the list is not cut by count), of those the ones in front of which stands less than `goal`, or with part > 0
-    // less than that part of the sum of the k.
-    __device__ __forceinline__ void cut_list(uint32_t count, uint32_t before, u64 front, uint32_t k, double goal, float part)
+    // By the first CTA: the list, from the largest.
+    __device__ __forceinline__ const uint32_t* sorted(int count)
     {
-        constexpr int kEach = kSaList / kSaThreads;
-        uint32_t keep = count;
-        if (k > 0) keep = min(count, k - before);
-        if (part > 0.f || goal > 0.0) {
-            u64 w[kEach], sum = 0, all;
-            const int per = ((int)count + kSaThreads - 1) / kSaThreads, at = threadIdx.x * per;
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) {
-                w[i] = i < per && at + i < (int)keep ? row.weight(sa_value(sm.list[at + i])) : 0;
-                sum += w[i];
+        if (count <= kSaCounted) {
+            // (a value's place is the number of those in front of it)
+            if ((int)threadIdx.x < count) {
+                const uint32_t mine = sm.list[threadIdx.x];
+                int place = 0;
+#pragma unroll 8
+                for (int i = 0; i < count; ++i) {
+                    const uint32_t other = sm.list[i];
+                    place += other > mine || (other == mine && i < (int)threadIdx.x);
+                }
+                sm.fine[place] = mine;
             }
-            u64 run_sum = front + sa_scan(sum, sm.warp_sum, all);
-            if (part > 0.f) goal = fmax((double)part * (double)(front + all), 0.5);
-            uint32_t stay = 0;
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) {
-                if (i < per && at + i < (int)keep && (double)run_sum < goal) ++stay;
-                run_sum += w[i];
-            }
-            sa_scan(stay, sm.warp_count, keep);
-            keep = max(keep, 1u);
+            __syncthreads();
+            return sm.fine;
         }
-        const uint32_t key = sm.list[keep - 1];
-        uint32_t equals = 0, all_equals;
-        for (int i = threadIdx.x; i < (int)keep; i += kSaThreads) equals += sm.list[i] == key;
-        sa_scan(equals, sm.warp_count, all_equals);
-        if ((int)threadIdx.x < ranks) *of(&sm.cut, threadIdx.x) = {key, all_equals};
+        int size = 2 * kSaCounted;
+        while (size < count) size <<= 1;
+        for (int i = count + threadIdx.x; i < size; i += kSaThreads) sm.list[i] = 0;
+        __syncthreads();
+        for (int k = 2; k <= size; k <<= 1) {
+            for (int j = k >> 1; j > 0; j >>= 1) {
+                for (int i = threadIdx.x; i < size / 2; i += kSaThreads) {
+                    const int a = 2 * i - (i & (j - 1)), b = a + j;
+                    const uint32_t u = sm.list[a], v = sm.list[b];
+                    if ((u < v) == ((a & k) == 0)) {
+                        sm.list[a] = v;
+                        sm.list[b] = u;
+                    }
+                }
+                __syncthreads();
+            }
+        }
+        return sm.list;
+    }
+
+    // By the first CTA, the cut in the list of `count` values, in front of which stand `before` with the sum `front`; to all, behind a barrier.  The
+    // first `k` stay (0: it is not cut by count), of those the ones in front of which stands less than `goal`, or with part > 0 less
+    // than that part of the sum of the k.
+    __device__ __forceinline__ SaCut cut_list(uint32_t count, uint32_t before, u64 front, uint32_t k, double goal, float part)
+    {
+        if (rank == 0) {
+            constexpr int kEach = kSaList / kSaThreads;
+            const uint32_t* list = sorted((int)count);
+            uint32_t keep = k > 0 ? min(count, k - before) : count;
+            if (part > 0.f || goal > 0.0) {
+                u64 w[kEach], sum = 0;
+                const int per = ((int)count + kSaThreads - 1) / kSaThreads, at = threadIdx.x * per;
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) {
+                    w[i] = i < per && at + i < (int)keep ? row.weight(sa_value(list[at + i])) : 0;
+                    sum += w[i];
+                }
+                const Sums s = scan(sum, 0);
+                u64 run = front + s.sum_before;
+                if (part > 0.f) goal = fmax((double)part * (double)(front + s.sum), 0.5);
+                uint32_t stay = 0;
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) {
+                    if (i < per && at + i < (int)keep && (double)run < goal) ++stay;
+                    run += w[i];
+                }
+                keep = max(scan(0, stay).count, 1u);
+            }
+            const uint32_t key = list[keep - 1];
+            uint32_t equals = 0;
+            for (int i = threadIdx.x; i < (int)keep; i += kSaThreads) equals += list[i] == key;
+            const SaCut cut = {key, scan(0, equals).count};
+            if ((int)threadIdx.x < ranks) *of(&sm.cut, threadIdx.x) = cut;
+            if (threadIdx.x == 0) sm.listed = 0;   // (for the next list)
+        }
+        barrier();
+        return sm.cut;
     }
 
     // The cut by bisection: the largest key with `k` values, or a sum of w of `goal`, from it on.
     __device__ __forceinline__ SaCut bisect(bool by_mass, uint32_t k, double goal)
     {
         uint32_t lo = kSaNothing + 1, hi = sa_key(row.top);
-        auto from = [&](uint32_t key, u64& mass, uint32_t& count) {
+        auto from = [&](uint32_t key) {
             u64 m = 0;
             uint32_t c = 0;
             each([&](float v) {
@@ -368,38 +448,33 @@ struct SaKernel {
                 ++c;
                 if (by_mass) m += row.weight(v);
             });
-            exchange(m, c, mass, count);
+            return exchange(m, c);
         };
-        u64 mass;
-        uint32_t count;
         while (lo < hi) {
             const uint32_t mid = lo + (hi - lo + 1) / 2;
-            from(mid, mass, count);
-            if (by_mass ? (double)mass >= goal : count >= k) lo = mid;
+            const Sums s = from(mid);
+            if (by_mass ? (double)s.sum >= goal : s.count >= k) lo = mid;
             else hi = mid - 1;
         }
-        mass = 0, count = 0;
-        if (lo < 0xffffffffu) from(lo + 1, mass, count);
-        uint32_t equals = by_mass ? 0 : k - count;
-        if (by_mass) {
-            // the first sum of equals that reaches the goal
-            const u64 w = row.weight(sa_value(lo));
-            uint32_t a = 1, b = kSaMaxVocab;
-            while (a < b) {
-                const uint32_t m = a + (b - a) / 2;
-                if ((double)(mass + (u64)m * w) >= goal) b = m;
-                else a = m + 1;
-            }
-            equals = a;
+        Sums above = {};
+        if (lo < 0xffffffffu) above = from(lo + 1);
+        if (!by_mass) return {lo, k - above.count};
+        // the first sum of equals that reaches the goal
+        const u64 w = row.weight(sa_value(lo));
+        uint32_t a = 1, b = kSaMaxVocab;
+        while (a < b) {
+            const uint32_t m = a + (b - a) / 2;
+            if ((double)(above.sum + (u64)m * w) >= goal) b = m;
+            else a = m + 1;
         }
-        return {lo, equals};
+        return {lo, a};
     }
 
-    // The cut by count, or by mass; with part > 0 both where one list does (`both` says so).  The first histogram is there.
-    __device__ __forceinline__ SaCut find(bool by_mass, uint32_t k, double goal, float part, bool& both, u64& front)
+    // The cut by count, or by mass; with part > 0 both where one list does (`both` says so).  The first histogram, of `total` values, is there.
+    __device__ __forceinline__ SaCut find(uint32_t total, bool by_mass, uint32_t k, double goal, float part, bool& both)
     {
         const float per_e = 1.0f / kSaBinsPerE;
-        SaBracket br = narrow(sm.hist, by_mass, k, 0, goal, 0.0, [&](int b) { return b * per_e; }, true);
+        SaBracket br = narrow(sm.hist, total, by_mass, k, 0, goal, 0.0, [&](int b) { return b * per_e; }, true);
         both = false;
         if (!by_mass && part > 0.f && br.before + br.count <= kSaList) {
             both = true;       // everything up to the cut
@@ -407,44 +482,39 @@ struct SaKernel {
         }
         if (br.count <= kSaList) {
             const SaBracket b = br;
-            front = gather(b.count, by_mass, [&](float v) {
-                if (v == -INFINITY) return 2;
+            const u64 front = gather(by_mass, [&](float v) {
                 const int i = row.bin(v);
                 return i < b.b0 ? 0 : i <= b.b1 ? 1 : 2;
             });
-            if (rank == 0) cut_list(b.count, b.before, front, by_mass ? 0 : k, by_mass ? goal : 0.0, both ? part : 0.f);
-            barrier();
-            return sm.cut;
+            return cut_list(b.count, b.before, front, by_mass ? 0 : k, by_mass ? goal : 0.0, both ? part : 0.f);
         }
         // the second histogram, and what stands in front of it
         const int c0 = br.b0, c1 = br.b1;
         const float per_bin = (float)kSaBins / (float)(c1 - c0 + 1);
+        for (int i = threadIdx.x; i < kSaBins; i += kSaThreads) sm.fine[i] = 0;
+        barrier();
         u64 ahead = 0;
-        histogram(sm.fine, [&](float v) {
-            if (v == -INFINITY) return -1;
+        each([&](float v) {
+            if (v == -INFINITY) return;
             const int i = row.bin(v);
             if (i < c0 && by_mass) ahead += row.weight(v);
-            return i < c0 || i > c1 ? -1 : row.fine(v, c0, per_bin);
+            if (i >= c0 && i <= c1) atomicAdd(&sm.fine[row.sub_bin(v, c0, per_bin)], 1u);
         });
-        u64 mass;
-        uint32_t none;
-        exchange(ahead, 0, mass, none);
-        br = narrow(sm.fine, by_mass, k, br.before, goal, (double)mass, [&](int b) { return (c0 + b / per_bin) * per_e; }, c1 == kSaBins - 1);
-        if (br.count <= kSaList) {
-            const SaBracket b = br;
-            front = gather(b.count, by_mass, [&](float v) {
-                if (v == -INFINITY) return 2;
-                const int i = row.bin(v);
-                if (i < c0 || i > c1) return i < c0 ? 0 : 2;
-                const int j = row.fine(v, c0, per_bin);
-                return j < b.b0 ? 0 : j <= b.b1 ? 1 : 2;
-            });
-            if (rank == 0) cut_list(b.count, b.before, front, by_mass ? 0 : k, by_mass ? goal : 0.0, 0.f);
-            barrier();
-            return sm.cut;
-        }
-        front = 0;
-        return bisect(by_mass, k, goal);
+        const Sums s = scan(ahead, 0);
+        publish(s);
+        merge(sm.fine);
+        barrier();
+        const u64 mass = collect(s).sum;
+        br = narrow(sm.fine, br.count, by_mass, k, br.before, goal, (double)mass, [&](int b) { return (c0 + b / per_bin) * per_e; }, c1 == kSaBins - 1);
+        if (br.count > kSaList) return bisect(by_mass, k, goal);
+        const SaBracket b = br;
+        const u64 front = gather(by_mass, [&](float v) {
+            const int i = row.bin(v);
+            if (i < c0 || i > c1) return i < c0 ? 0 : 2;
+            const int j = row.sub_bin(v, c0, per_bin);
+            return j < b.b0 ? 0 : j <= b.b1 ? 1 : 2;
+        });
+        return cut_list(b.count, b.before, front, by_mass ? 0 : k, by_mass ? goal : 0.0, 0.f);
     }
 };
 
@@ -456,29 +526,32 @@ __global__ void __launch_bounds__(kSaThreads) sample_rows_kernel(const SampleArg
     const int tid = threadIdx.x;
     const int rank = ranks > 1 ? (int)cg::this_cluster().block_rank() : 0;
     const long long r = blockIdx.x / ranks;
+    if (ranks > 1) cluster_arrive();             // waited for before the first remote access
+    for (int i = tid; i < kSaBins; i += kSaThreads) sm.hist[i] = 0;
+    if (tid < kSaTable) sm.table[tid] = exp2(tid * (1.0 / kSaTable));
+    if (tid == 0) sm.listed = 0;
     pdl_launch_dependents();
     pdl_wait();
     const T* src = (const T*)a.logits + r * a.row_stride + (long long)rank * slice;
     const int n = max(0, min(slice, a.vocab - rank * slice));
-    // ---- 1  the slice, whole 16 bytes at a time; it begins in shared memory where its first byte lies in 16 of global memory
+    // ---- 1  the slice, whole 16 bytes at a time, as it lies in global memory: what is not of it at its ends becomes -inf
     constexpr int kPer = 16 / sizeof(T);
     const int skew = (int)((reinterpret_cast<uintptr_t>(src) & 15) / sizeof(T));
-    T* x = reinterpret_cast<T*>(sa_dyn) + skew;
+    const int loads = n > 0 ? (skew + n + kPer - 1) / kPer : 0;
     float top = -INFINITY;
     {
         const uint4* from = reinterpret_cast<const uint4*>(src - skew);
-        const int words = (skew + n + kPer - 1) / kPer;
         constexpr int kAhead = 4;
-        for (int i0 = tid; i0 < words; i0 += kAhead * kSaThreads) {
+        for (int i0 = tid; i0 < loads; i0 += kAhead * kSaThreads) {
             uint4 v[kAhead];
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) {
                 const int i = i0 + k * kSaThreads;
-                if (i >= words) continue;
+                if (i >= loads) continue;
                 if (i * kPer >= skew && (i + 1) * kPer <= skew + n) {
                     v[k] = from[i];
                 }
-                else {             // the ends
+                else {
                     T* e = reinterpret_cast<T*>(&v[k]);
 #pragma unroll
                     for (int j = 0; j < kPer; ++j) {
@@ -490,18 +563,24 @@ __global__ void __launch_bounds__(kSaThreads) sample_rows_kernel(const SampleArg
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) {
                 const int i = i0 + k * kSaThreads;
-                if (i >= words) continue;
+                if (i >= loads) continue;
                 reinterpret_cast<uint4*>(sa_dyn)[i] = v[k];
-                const T* e = reinterpret_cast<const T*>(&v[k]);
+                const uint32_t w[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
 #pragma unroll
-                for (int j = 0; j < kPer; ++j) top = fmaxf(top, sa_clean(sa_float(e[j])));
+                for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                    for (int h = 0; h < SaWord<T>::kValues; ++h) top = fmaxf(top, SaWord<T>::get(w[j], h));   // (a NaN loses)
+                }
             }
         }
     }
-    SaKernel<T> s = {sm, x, n, ((n + kSaThreads - 1) / kSaThreads) | 1, ranks, rank, {}};
+    const int words = 4 * loads, run = ((words + kSaThreads - 1) / kSaThreads) | 1, begin = min(words, tid * run);
+    SaKernel<T> s = {sm, reinterpret_cast<const uint32_t*>(sa_dyn), begin, min(words, begin + run), ranks, rank, {}};
     top = warp_max(top);
     if ((tid & 31) == 0) sm.warp_max[tid >> 5] = top;
-    s.barrier();                   // (every CTA of the cluster has begun)
+    __syncthreads();
+    if (ranks > 1) cluster_wait();
+#pragma unroll
     for (int w = 0; w < kSaWarps; ++w) top = fmaxf(top, sm.warp_max[w]);
     if (tid < ranks) *s.of(&sm.maxima[rank], tid) = top;
     s.barrier();
@@ -513,13 +592,14 @@ __global__ void __launch_bounds__(kSaThreads) sample_rows_kernel(const SampleArg
         }
         return;                    // (all of the cluster, and the last word to another CTA lies in front of a barrier)
     }
+    top = sa_clean(top);           // (-0)
     float temperature = a.temperatures != nullptr ? a.temperatures[r] : a.temperature;
     const float part = a.top_ps != nullptr ? a.top_ps[r] : a.top_p;
     const float least = a.min_ps != nullptr ? a.min_ps[r] : a.min_p;
     const int wanted = a.top_ks != nullptr ? a.top_ks[r] : a.top_k;
     const bool greedy = !(temperature > 0.f);
     if (greedy) temperature = 1.0f;
-    s.row = {top, 1.0 / (double)temperature, kSaBinsPerE / temperature};
+    s.row = {top, kSaBinsPerE / temperature, 1.0 / (double)temperature, kSaTable * 1.4426950408889634 / (double)temperature, sm.table};
 
     SaCut cut = {kSaNothing, 0u};   // everything above -inf
     float floor = -INFINITY;        // of min-p
@@ -530,70 +610,70 @@ __global__ void __launch_bounds__(kSaThreads) sample_rows_kernel(const SampleArg
         if (least > 0.f) floor = __double2float_ru((double)top + (double)temperature * log(fmin((double)least, 1.0)));
         const bool by_count = wanted > 0 && wanted < a.vocab, by_mass = part < 1.0f;
         if (by_count || by_mass) {
-            // ---- 2
+            // ---- 2  (the last bin, which may hold most of the row, is not counted but follows from the others)
             u64 sum = 0;
             uint32_t count = 0;
-            s.histogram(sm.hist, [&](float v) {
-                if (v == -INFINITY) return -1;
+            s.each([&](float v) {
+                if (v == -INFINITY) return;
                 ++count;
                 if (!by_count) sum += s.row.weight(v);
-                return s.row.bin(v);
+                const int b = s.row.bin(v);
+                if (b < kSaBins - 1) atomicAdd(&sm.hist[b], 1u);
             });
-            s.exchange(sum, count, sum, count);
+            const auto mine = s.scan(sum, count);
+            s.publish(mine);
+            s.merge(sm.hist);
+            s.barrier();
+            const auto all = s.collect(mine);
             // ---- 3, 4
+            sum = all.sum;
             bool both = false;
-            u64 front = 0;
-            const bool cut_count = by_count && (uint32_t)wanted < count;
-            if (cut_count) cut = s.find(false, wanted, 0.0, by_mass ? fmaxf(part, 1e-30f) : 0.f, both, front);
+            const bool cut_count = by_count && (uint32_t)wanted < all.count;
+            if (cut_count) cut = s.find(all.count, false, wanted, 0.0, by_mass ? fmaxf(part, 1e-30f) : 0.f, both);
             if (by_mass && !both) {
                 if (by_count) {    // the sum of what top-k leaves
                     u64 w = 0;
                     s.each([&](float v) {
                         if (sa_key(v) > cut.key) w += s.row.weight(v);
                     });
-                    uint32_t none;
-                    s.exchange(w, 0, sum, none);
-                    sum += cut.equals * s.row.weight(sa_value(cut.key));
+                    sum = s.exchange(w, 0).sum + (cut.equals > 0 ? cut.equals * s.row.weight(sa_value(cut.key)) : 0);
                 }
                 const SaCut by_k = cut;
-                cut = s.find(true, 0, fmax((double)part * (double)sum, 0.5), 0.f, both, front);
+                cut = s.find(all.count, true, 0, fmax((double)part * (double)sum, 0.5), 0.f, both);
                 if (cut.key == by_k.key) cut.equals = min(cut.equals, by_k.equals);
             }
         }
     }
-    // ---- 5
-    u64 mine = 0, all, before;
-    uint32_t equals = 0, all_equals, equals_before;
-    const int begin = tid * s.run, end = min(n, begin + s.run);
+    // ---- 5  sums of what lies above the cut, and its equals, in the order of the indices: how many of a thread's equals stay follows from those
+    // in front
     const float edge = sa_value(cut.key);
     const bool some = cut.equals > 0 && edge >= floor;
-    for (int i = begin; i < end; ++i) {
-        const float v = s.at(i);
+    u64 mine = 0;
+    uint32_t equals = 0;
+    s.each([&](float v) {
         if (v > edge && v >= floor) mine += s.row.weight(v);
-        equals += v == edge;
-    }
-    // (equals first: how many of this thread's stay follows from those in front)
-    u64 none;
-    s.exchange(0, some ? equals : 0, none, all_equals, nullptr, &equals_before);
+        equals += some && v == edge;
+    });
+    const auto at = s.exchange(mine, equals);
     const u64 edge_weight = some ? s.row.weight(edge) : 0;
-    const uint32_t stay = some && equals_before < cut.equals ? min(equals, cut.equals - equals_before) : 0;
+    const uint32_t stay = at.count_before < cut.equals ? min(equals, cut.equals - at.count_before) : 0;
+    const u64 before = at.sum_before + min(at.count_before, cut.equals) * edge_weight, all = at.sum + min(at.count, cut.equals) * edge_weight;
     mine += stay * edge_weight;
-    uint32_t one;
-    s.exchange(mine, 0, all, one, &before, nullptr);
     double goal = (double)a.uniform[r] * (double)all;
     if (!(goal >= 0.0)) goal = 0.0;
     if (goal >= (double)all) goal = __longlong_as_double(__double_as_longlong((double)all) - 1);   // (the number below)
     if ((double)before <= goal && (double)(before + mine) > goal && mine > 0) {
         uint32_t seen = 0;
-        u64 sum = before;
-        for (int i = begin; i < end; ++i) {
-            const float v = s.at(i);
+        u64 run_sum = before;
+        constexpr int kValues = SaWord<T>::kValues;
+        for (int i = s.begin * kValues; i < s.end * kValues; ++i) {
+            const float v = sa_clean(SaWord<T>::get(s.x[i / kValues], i % kValues));
             u64 w = 0;
             if (v > edge && v >= floor) w = s.row.weight(v);
-            else if (v == edge && seen < stay) w = edge_weight, ++seen;
-            sum += w;
-            if (w > 0 && (double)sum > goal) {
-                a.tokens[r] = (long long)rank * slice + i;
+            else if (some && v == edge && seen < stay) w = edge_weight, ++seen;
+            run_sum += w;
+            if (w > 0 && (double)run_sum > goal) {
+                a.tokens[r] = (long long)rank * slice + i - skew;
                 a.logprobs[r] = (float)(s.row.power(v) - log((double)all / kSaUnit));
                 break;
             }
@@ -641,7 +721,7 @@ int launch_sample(const SampleArgs& a, cudaStream_t stream)
     const int bytes = a.type == 2 ? 4 : 2;
     // As many CTAs a row as its slices need, and as fit the GPU at once; a slice of some thousand values at least.
     int ranks = 1;
-    while (ranks < kSaMaxCluster && (long long)a.vocab * bytes > (long long)ranks * (kSaMaxSlice - 64)) ranks *= 2;
+    while (ranks < kSaMaxCluster && (long long)a.vocab * bytes > (long long)ranks * kSaSlice) ranks *= 2;
     while (ranks < kSaMaxCluster && (long long)a.rows * 2 * ranks <= sm_count() && a.vocab / ranks >= 4096) ranks *= 2;
     if (a.type == 0) return launch_sample_t<__half>(a, ranks, stream);
     if (a.type == 1) return launch_sample_t<__nv_bfloat16>(a, ranks, stream);
