@@ -7,7 +7,7 @@
 // All of these leave a beginning of one order, so they come down to a cut: a value x*, and how many of its equals stay.  Nothing is sorted but
 // a few candidates around it.
 //   1  the row into shared memory, its maximum
-//   2  a histogram over (max - x) / T, 64 bins to a factor of e in w: counts in front of a bin are exact, sums of w known to 1.6 %, and mostly to
+//   2  a histogram over (max - x) / T, 64 bins to a factor of e in w (fewer where top-k may reach further down than 32 such factors): counts in front of a bin are exact, sums of w known to 1.6 %, and mostly to
 //      1e-4
 //   3  the bins in which the cut must lie - by mass first those where it very likely lies, which the sums in step 4 confirm or not; where they
 //      hold too many values for a list, a second histogram over them alone
@@ -69,7 +69,7 @@ struct SaSmem {
     uint32_t list[kSaList];
     uint32_t listed;
     // from every CTA of the cluster, two buffers each
-    float maxima[kSaMaxCluster];
+    float maxima[kSaMaxCluster], minima[kSaMaxCluster];
     u64 sums[2][kSaMaxCluster], fronts[2][kSaMaxCluster];
     uint32_t counts[2][kSaMaxCluster];
     // from the first CTA
@@ -79,7 +79,7 @@ struct SaSmem {
     u64 warp_sum[kSaWarps], warp_front[kSaWarps];
     uint32_t warp_count[kSaWarps];
     double warp_low[kSaWarps], warp_high[kSaWarps];
-    float warp_max[kSaWarps];
+    float warp_max[kSaWarps], warp_min[kSaWarps];
     uint32_t front, upto;
 };
 
@@ -137,7 +137,8 @@ struct SaWord<__nv_bfloat16> {
 
 struct SaRow {
     float top;            // finite
-    float scale;          // bins a unit of x
+    float scale;          // bins a unit of x,
+    float per_bin;        // and units of (max - x) / T a bin
     float least;          // below it exp(-745) is passed, where a number in 64 bits ends: w is 0
     double over_t;        // 1 / T
     double step;          // kSaTable log2(e) / T
@@ -536,7 +537,7 @@ struct SaKernel {
     // where one list does (`both` says so).  The first histogram, of `total` values, is there.  mine: as in gather().
     __device__ __forceinline__ SaCut find(uint32_t total, bool by_mass, uint32_t k, double goal, float part, bool& both, u64& mine)
     {
-        const float per_e = 1.0f / kSaBinsPerE;
+        const float per_e = row.per_bin;
         const auto low = [&](int b) { return fmaxf(b - 0.5f, 0.f) * per_e; };
         both = false;
         const auto goal_of = [&](const Sums& s) { return goal > 0.0 || !by_mass ? goal : fmax((double)part * (double)s.sum, 0.5); };
@@ -621,7 +622,14 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_rows_kernel(const Sample
     constexpr int kPer = 16 / sizeof(T);
     const int skew = (int)((reinterpret_cast<uintptr_t>(src) & 15) / sizeof(T));
     const int loads = n > 0 ? (skew + n + kPer - 1) / kPer : 0;
-    float top = -INFINITY;
+    float temperature = a.temperatures != nullptr ? a.temperatures[r] : a.temperature;
+    const float part = a.top_ps != nullptr ? a.top_ps[r] : a.top_p;
+    const float least = a.min_ps != nullptr ? a.min_ps[r] : a.min_p;
+    const int wanted = a.top_ks != nullptr ? a.top_ks[r] : a.top_k;
+    const bool greedy = !(temperature > 0.f);
+    if (greedy) temperature = 1.0f;
+    const bool by_count = wanted > 0 && wanted < a.vocab, by_mass = part < 1.0f;
+    float top = -INFINITY, bottom = INFINITY;   // of the finite and infinite values above -inf
     {
         const uint4* from = reinterpret_cast<const uint4*>(src - skew);
         constexpr int kAhead = 4;
@@ -652,7 +660,11 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_rows_kernel(const Sample
                 for (int j = 0; j < 4; ++j) {
                     w[j] = SaWord<T>::clean(w[j]);
 #pragma unroll
-                    for (int h = 0; h < SaWord<T>::kValues; ++h) top = fmaxf(top, SaWord<T>::get(w[j], h));
+                    for (int h = 0; h < SaWord<T>::kValues; ++h) {
+                        const float value = SaWord<T>::get(w[j], h);
+                        top = fmaxf(top, value);
+                        if (by_count && value > -INFINITY) bottom = fminf(bottom, value);
+                    }
                 }
                 reinterpret_cast<uint4*>(sa_dyn)[i] = make_uint4(w[0], w[1], w[2], w[3]);
             }
@@ -661,14 +673,15 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_rows_kernel(const Sample
     const int words = 4 * loads, run = ((words + kSaThreads - 1) / kSaThreads) | 1, begin = min(words, tid * run);
     SaKernel<T> s = {sm, reinterpret_cast<const uint32_t*>(sa_dyn), begin, min(words, begin + run), ranks, rank, {}};
     top = warp_max(top);
-    if ((tid & 31) == 0) sm.warp_max[tid >> 5] = top;
+    bottom = -warp_max(-bottom);
+    if ((tid & 31) == 0) sm.warp_max[tid >> 5] = top, sm.warp_min[tid >> 5] = bottom;
     __syncthreads();
     if (ranks > 1) cluster_wait();
 #pragma unroll
-    for (int w = 0; w < kSaWarps; ++w) top = fmaxf(top, sm.warp_max[w]);
-    if (tid < ranks) *s.of(&sm.maxima[rank], tid) = top;
+    for (int w = 0; w < kSaWarps; ++w) top = fmaxf(top, sm.warp_max[w]), bottom = fminf(bottom, sm.warp_min[w]);
+    if (tid < ranks) *s.of(&sm.maxima[rank], tid) = top, *s.of(&sm.minima[rank], tid) = bottom;
     s.barrier();
-    for (int i = 0; i < ranks; ++i) top = fmaxf(top, sm.maxima[i]);
+    for (int i = 0; i < ranks; ++i) top = fmaxf(top, sm.maxima[i]), bottom = fminf(bottom, sm.minima[i]);
     if (top == -INFINITY) {        // nothing can be drawn
         if (rank == 0 && tid == 0) {
             a.tokens[r] = -1;
@@ -676,15 +689,10 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_rows_kernel(const Sample
         }
         return;                    // (all of the cluster, and the last word to another CTA lies in front of a barrier)
     }
-    float temperature = a.temperatures != nullptr ? a.temperatures[r] : a.temperature;
-    const float part = a.top_ps != nullptr ? a.top_ps[r] : a.top_p;
-    const float least = a.min_ps != nullptr ? a.min_ps[r] : a.min_p;
-    const int wanted = a.top_ks != nullptr ? a.top_ks[r] : a.top_k;
-    const bool greedy = !(temperature > 0.f);
-    if (greedy) temperature = 1.0f;
-    const bool by_count = wanted > 0 && wanted < a.vocab, by_mass = part < 1.0f;
     // (a finite scale: nothing times infinity is no place)
-    s.row = {top, fminf(kSaBinsPerE / temperature, 1e30f), (float)((double)top - 745.0 * (double)temperature), 1.0 / (double)temperature,
+    float scale = fminf(kSaBinsPerE / temperature, 1e30f);
+    if (by_count && (top - bottom) * scale > kSaBins - 2) scale = fmaxf((kSaBins - 2) / (top - bottom), scale / 32);
+    s.row = {top, scale, 1.0f / (scale * temperature), (float)((double)top - 745.0 * (double)temperature), 1.0 / (double)temperature,
              kSaTable * 1.4426950408889634 / (double)temperature, sm.table};
 
     SaCut cut = {kSaNothing, 0u, kSaUnlisted};   // everything above -inf

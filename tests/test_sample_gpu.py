@@ -110,6 +110,17 @@ def test_sample_where_no_list_holds_the_candidates(settings, kind, dtype):
     _check(x, torch.tensor([0.25, 0.8], device="cuda"), **settings)
 
 
+@pytest.mark.parametrize("settings", [dict(top_k=50, top_p=0.95, temperature=0.3), dict(top_k=20000, temperature=0.05), dict(top_k=1000), dict(top_k=7)])
+@pytest.mark.parametrize("spread", [4.0, 60.0, 3000.0])
+def test_sample_of_the_most_from_a_row_that_reaches_far_down(settings, spread):
+    """Nearly all tokens lie more than 32 factors of e below the largest, some of them masked with the lowest number."""
+    logits, uniform = _logits(3, 32000, FP32, 11, spread, peaks=10)
+    logits[:, 0] = 10 * spread
+    _check(logits, uniform, **settings)
+    logits[:, 1000:9000] = torch.finfo(FP32).min
+    _check(logits, uniform, **settings)
+
+
 @pytest.mark.parametrize("settings", [dict(), dict(top_k=3), dict(top_p=0.6), dict(min_p=0.4), dict(top_k=2, top_p=0.5)])
 def test_sample_among_ties(settings):
     """Equal logits: the lower index stays, also where they lie in different threads and CTAs."""
