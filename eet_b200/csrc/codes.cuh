@@ -106,6 +106,25 @@ __device__ __forceinline__ void dequantize16(const uint4& x, float scale, float 
     }
 }
 
+// ------------------------------------------------------------------------------------------------ shared memory
+// (of a size of zero nothing is read, and zeros are written)
+__device__ __forceinline__ void copy16_async(uint32_t dst, const void* src, uint32_t bytes)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+__device__ __forceinline__ void copy4_async(uint32_t dst, const void* src, uint32_t bytes)
+{
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t at)
+{
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+    return v;
+}
+
 }  // namespace
 
 }  // namespace eet

@@ -62,28 +62,11 @@ struct PcSmem {
     PgFound found;
 };
 
-__device__ __forceinline__ void copy16_async(uint32_t dst, const void* src, uint32_t bytes)
-{
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-
-__device__ __forceinline__ void copy4_async(uint32_t dst, const void* src, uint32_t bytes)
-{
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x)
 {
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
-}
-
-__device__ __forceinline__ uint4 lds128(uint32_t at)
-{
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
-    return v;
 }
 
 __device__ __forceinline__ uint2 lds64(uint32_t at)

@@ -24,11 +24,13 @@
 // Keys outside of what any row of the pair sees may be anything, even NaN (slots behind the end of a sequence): their scores are
 // masked by selection and their rows of V are set to zero in shared memory before the product reads them.
 //
-// Over a cache of 8-bit codes four more warps (12-15, a warpgroup of their own) put K and V into the ring: each reads its 32 keys of an entry
-// into registers, one entry ahead, multiplies the codes with the scale of their row in fp32, rounds once to q's type and writes that
-// where the copy engine would have put it; the rest of the kernel does not know.  (The scales could stay outside the products as in
+// Over a cache of 8-bit codes four more warps (12-15, a warpgroup of their own) put K and V into the ring: each copies its 32 keys of an entry
+// two entries ahead, multiplies the codes with the scale of their row in fp32, rounds once to q's type and writes that where the copy
+// engine would have put it; the rest of the kernel does not know.  (The scales could stay outside the products as in
 // paged_codes.cu, two multiplications and two reads of shared memory more for every score: the softmax is the bound here, and these warps
 // have time.)  512 threads of 128 registers are launched, of which the softmax takes 144 and the others 112.
+#include <type_traits>
+
 #include "codes.cuh"
 #include "paged_share.cuh"
 
@@ -39,6 +41,7 @@ namespace {
 constexpr int kPgThreads = 320;
 constexpr int kPgCodesThreads = 512;    // with the warps that convert codes
 constexpr int kPgStages = 5;
+constexpr __host__ __device__ int pg_ring(int head_dim, int codes) { return codes && head_dim == 128 ? 4 : kPgStages; }   // (with codes their own ring takes room)
 constexpr int kPgExtra = 3;             // a tile's beginning and end cost as much as three blocks
 constexpr uint32_t kPgTmemCols = 512;   // S of a, S of b (their probabilities over them), O of a, O of b: 128 each
 
@@ -149,65 +152,73 @@ __device__ __forceinline__ void pg_values16(const uint4& x, float scale, uint32_
     for (int i = 0; i < 8; ++i) out[i] = PgType<T>::pack(y[2 * i], y[2 * i + 1]);
 }
 
-// A warp that converts: its 32 keys of every entry of the ring, in the entries' order.  Lane (r, c) = (lane / 4, lane % 4) has 16 codes of keys
-// r, r + 8, r + 16 and r + 24 in either half of a row (odd keys the halves in the other order: eight lanes then meet no bank twice).
+// A warp that converts: its 32 keys of every entry of the ring, in the entries' order.  Their codes come through two places of the warp's own in
+// shared memory (cp.async), an entry ahead, their scales into a register of either place.
 template<typename T, int D, int kCodes>
 struct PgConverter {
     static constexpr int kHalves = D / 64, kHalf = kPgRows * 128;
+    static constexpr int kEntry = 32 * D;                  // bytes
     const PagedMhaArgs& a;
     int warp;                          // 0 .. 3
-    uint4 x[4 * kHalves];              // of the entry on its way
-    float scale[4];
+    uint32_t staged;                   // the places
+    float scales[2];                   // a lane a key
 
-    // the pages of the two runs of 16 keys of a block at key0; -1: nobody sees them, -2: zeros
-    __device__ __forceinline__ int2 pages(const int* row, const PgSpan& span, int key0) const
+    // The pages of the two runs of 16 keys of a block at key0, in the lanes 0 .. 15 and 16 .. 31, as the table has them; -1: nobody sees them.
+    __device__ __forceinline__ int page(const int* row, const PgSpan& span, int key0) const
     {
-        int n[2];
+        const int key = key0 + 32 * warp + (int)(threadIdx.x & 16);
+        return key < span.hi && key + 16 > span.lo ? row[key >> a.page_shift] : -1;
+    }
+    // Keys that the tile does not see, and pages outside the cache, become zeros.
+    template<int kSlot>
+    __device__ __forceinline__ void copy(bool v, int head, const PgSpan& span, int key0, int page)
+    {
+        constexpr int kChunks = D / 16, kRowsAtOnce = 32 / kChunks;
+        const int lane = threadIdx.x & 31, key = key0 + 32 * warp, row0 = lane / kChunks, c = lane % kChunks;
+        const uint32_t at = staged + (uint32_t)(kSlot * kEntry);
+        const uint8_t* cache = (const uint8_t*)(v ? a.v_cache : a.k_cache) + head * (v ? a.vc_head : a.kc_head) + 16 * c;
+        const long long page_step = v ? a.vc_page : a.kc_page, slot_step = v ? a.vc_slot : a.kc_slot;
+        const int mask = (1 << a.page_shift) - 1;
+        const bool known = page >= 0 && page < a.num_pages;
+        if (!known && key + (lane & 16) < span.hi && key + (lane & 16) + 16 > span.lo) g_device_status = 6;
+        const int n = known ? page : -1;
+#pragma unroll 1
+        for (int run = 0; run < 32; run += 16) {
+            const int m = __shfl_sync(0xffffffffu, n, run);
+            const uint8_t* src = cache + max(m, 0) * page_step + (((key + run) & mask) + row0) * slot_step;
+            const int from = m < 0 ? 32 : span.lo - key - run, upto = span.hi - key - run;
+            const uint32_t to = at + (uint32_t)((run + row0) * D + 16 * c);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int key = key0 + 32 * warp + 16 * i;
-            n[i] = -1;
-            if (key < span.hi && key + 16 > span.lo) {
-                n[i] = row[key >> a.page_shift];
-                if (n[i] < 0 || n[i] >= a.num_pages) {
-                    g_device_status = 6;
-                    n[i] = -2;
-                }
+            for (int i = 0; i < 16 / kRowsAtOnce; ++i) {
+                const int r = row0 + kRowsAtOnce * i;
+                copy16_async(to + kRowsAtOnce * i * D, src, r >= from && r < upto ? 16 : 0);
+                src += kRowsAtOnce * slot_step;
             }
         }
-        return make_int2(n[0], n[1]);
+        const bool seen = n >= 0 && key + lane >= span.lo && key + lane < span.hi;
+        const float* scale = (v ? a.v_scale + head * a.vs_head + max(n, 0) * a.vs_page : a.k_scale + head * a.ks_head + max(n, 0) * a.ks_page) +
+                             ((key + lane) & mask);
+        scales[kSlot] = 0.f;
+        if (seen) scales[kSlot] = *scale;
+        asm volatile("cp.async.commit_group;" ::: "memory");
     }
-    __device__ __forceinline__ void load(bool v, int head, const PgSpan& span, int key0, int2 page)
-    {
-        const int lane = threadIdx.x & 31;
-        const uint8_t* cache = (const uint8_t*)(v ? a.v_cache : a.k_cache) + head * (v ? a.vc_head : a.kc_head);
-        const float* scales = (v ? a.v_scale : a.k_scale) + head * (v ? a.vs_head : a.ks_head);
-        const long long page_step = v ? a.vc_page : a.kc_page, slot_step = v ? a.vc_slot : a.kc_slot, scale_step = v ? a.vs_page : a.ks_page;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int key = key0 + 32 * warp + 8 * i + (lane >> 2), n = i < 2 ? page.x : page.y;
-            scale[i] = 0.f;
-#pragma unroll
-            for (int h = 0; h < kHalves; ++h) x[i * kHalves + h] = make_uint4(0u, 0u, 0u, 0u);
-            if (n < 0 || key < span.lo || key >= span.hi) continue;
-            const int slot = key & ((1 << a.page_shift) - 1);
-            const uint8_t* src = cache + n * page_step + slot * slot_step + 16 * (lane & 3);
-            scale[i] = scales[n * scale_step + slot];
-#pragma unroll
-            for (int h = 0; h < kHalves; ++h) x[i * kHalves + h] = *reinterpret_cast<const uint4*>(src + 64 * (kHalves == 2 ? h ^ ((lane >> 2) & 1) : 0));
-        }
-    }
+    // Lane (r, c) = (lane / 4, lane % 4) has 16 codes of keys r, r + 8, r + 16 and r + 24 in either half of a row, odd keys the halves in the other
+    // order: eight lanes then meet no bank twice, reading or writing.
+    template<int kSlot>
     __device__ __forceinline__ void store(uint8_t* stage) const
     {
         const int lane = threadIdx.x & 31;
-#pragma unroll
+        const uint32_t at = staged + (uint32_t)(kSlot * kEntry);
+#pragma unroll 1
         for (int i = 0; i < 4; ++i) {
-            const int key = 32 * warp + 8 * i + (lane >> 2);
+            const int r = 8 * i + (lane >> 2), key = 32 * warp + r;
+            const float scale = __shfl_sync(0xffffffffu, scales[kSlot], r);
 #pragma unroll
             for (int h = 0; h < kHalves; ++h) {
+                const int half = kHalves == 2 ? h ^ (r & 1) : 0;
                 uint32_t y[8];
-                pg_values16<T, kCodes>(x[i * kHalves + h], scale[i], y);
-                uint8_t* dst = stage + (kHalves == 2 ? h ^ (key & 1) : 0) * kHalf + key * 128;
+                pg_values16<T, kCodes>(lds128(at + (uint32_t)(r * D + 64 * half + 16 * (lane & 3))), scale, y);
+                uint8_t* dst = stage + half * kHalf + key * 128;
                 const int c = 2 * (lane & 3);
                 *reinterpret_cast<uint4*>(dst + ((c ^ (key & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
                 *reinterpret_cast<uint4*>(dst + (((c + 1) ^ (key & 7)) << 4)) = make_uint4(y[4], y[5], y[6], y[7]);
@@ -225,6 +236,7 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
     constexpr int kHalves = D / 64;
     constexpr int kHalf = kPgRows * 128;         // bytes of [128 rows][64 values], swizzled
     constexpr int kTile = kHalves * kHalf;       // a Q tile, a K or a V block
+    constexpr int kRing = pg_ring(D, kCodes);
     uint8_t* q_tiles = dyn;
     uint8_t* ring = q_tiles + 2 * kTile;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -270,7 +282,7 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
                 if (!tc_wait_warp(&sm.empty[stage], phase, &sm.abort)) return false;
                 loader.load(map, (p.top - j) * kPgKeys, page, ring + stage * kTile, &sm.full[stage]);
                 ++issued;
-                if (++stage == kPgStages) {
+                if (++stage == kRing) {
                     stage = 0;
                     phase ^= 1;
                 }
@@ -288,8 +300,8 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
         if (!whole && lane == 0) pg_write_header(a, tiling, ws, cta, ctas, true, all, place);
         if (sm.abort) {
             // nothing of this CTA may still be on its way when it ends
-            for (int e = max(0, issued - kPgStages); e < issued; ++e) {
-                mbar_wait_bounded(&sm.full[e % kPgStages], (uint32_t)((e / kPgStages) & 1));
+            for (int e = max(0, issued - kRing); e < issued; ++e) {
+                mbar_wait_bounded(&sm.full[e % kRing], (uint32_t)((e / kRing) & 1));
             }
             if (pieces > 0) mbar_wait_bounded(&sm.q_full, (uint32_t)((pieces - 1) & 1));
         }
@@ -309,7 +321,7 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
             bool ok = true;
             auto landed = [&](int entry) -> bool {
                 // (entries are waited for in any order within the ring's length)
-                return tc_wait(&sm.full[entry % kPgStages], (uint32_t)((entry / kPgStages) & 1), &sm.abort);
+                return tc_wait(&sm.full[entry % kRing], (uint32_t)((entry / kRing) & 1), &sm.abort);
             };
             while (ok && share.next(a, tiling, p)) {
                 if (p.blocks == 0) continue;
@@ -326,7 +338,7 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
                     if (!landed(k_entry(j))) return false;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint64_t qd = q_desc + (uint64_t)((split ? 0 : x) * (kTile >> 4));
-                    const uint64_t kd = k_desc + (uint64_t)((k_entry(j) % kPgStages) * (kTile >> 4));
+                    const uint64_t kd = k_desc + (uint64_t)((k_entry(j) % kRing) * (kTile >> 4));
 #pragma unroll
                     for (int kk = 0; kk < D / 16; ++kk) {
                         const uint64_t off = (uint64_t)((kk >> 2) * (kHalf >> 4) + (kk & 3) * 2);
@@ -339,7 +351,7 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
                     const bool first = j == turns[x].first;
                     if (first && outs[x] > 0 && !tc_wait(&sm.o_free[x], (uint32_t)((outs[x] - 1) & 1), &sm.abort)) return false;
                     if (!landed(v_entry(j))) return false;
-                    const uint64_t vd = v_desc + (uint64_t)((v_entry(j) % kPgStages) * (kTile >> 4));
+                    const uint64_t vd = v_desc + (uint64_t)((v_entry(j) % kRing) * (kTile >> 4));
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         if (!tc_wait(half ? &sm.p_ready[x] : &sm.p_half[x], (uint32_t)(used[x] & 1), &sm.abort)) return false;
@@ -364,7 +376,7 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
                     if (active(x, j) && !issue_qk(x, j)) return false;
                     if (split || x == 1) {
                         if (!split && !active(0, j) && !active(1, j) && !landed(k_entry(j))) return false;
-                        umma_commit(&sm.empty[k_entry(j) % kPgStages]);
+                        umma_commit(&sm.empty[k_entry(j) % kRing]);
                         if (j == last_qk) umma_commit(&sm.q_empty);
                     }
                     return true;
@@ -376,7 +388,7 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
                     if (act && !issue_pv(x, j)) return false;
                     if (split || x == 1) {
                         if (!split && !active(0, j) && !active(1, j) && !landed(v_entry(j))) return false;
-                        umma_commit(&sm.empty[v_entry(j) % kPgStages]);
+                        umma_commit(&sm.empty[v_entry(j) % kRing]);
                     }
                     if (act && j + turns[x].stride >= turns[x].end) {
                         ++outs[x];
@@ -394,46 +406,63 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
     }
     else if (kCodes && warp >= 12) {
         // ------------------------------------------------------------------ codes into the ring
-        // An entry is read while the one before is converted; pages are known a block ahead of that.
-        PgConverter<T, D, kCodes ? kCodes : kCodesInt8> conv = {a, warp - 12};
+        using Converter = PgConverter<T, D, kCodes ? kCodes : kCodesInt8>;
+        Converter conv = {a, warp - 12, smem_u32(ring + kRing * kTile) + (uint32_t)((warp - 12) * 2 * Converter::kEntry), {}};
         int stage = 0;
         uint32_t phase = 1;                                       // of `empty`: the first round finds the stages free
-        bool ok = true, loaded = false;
-        auto put = [&]() -> bool {                                // what was read last
+        bool ok = true, held = false;                             // both places hold an entry
+        auto put = [&](auto slot, bool last) -> bool {            // what a place holds; last: nothing has been copied behind it
+            if (last) asm volatile("cp.async.wait_group 0;" ::: "memory");
+            else asm volatile("cp.async.wait_group 1;" ::: "memory");
+            __syncwarp();
             if (!tc_wait_warp(&sm.empty[stage], phase, &sm.abort)) return false;
-            conv.store(ring + stage * kTile);
+            conv.template store<decltype(slot)::value>(ring + stage * kTile);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(&sm.full[stage]);
-            if (++stage == kPgStages) {
+            if (++stage == kRing) {
                 stage = 0;
                 phase ^= 1;
             }
             return true;
         };
+        const std::integral_constant<int, 0> first;
+        const std::integral_constant<int, 1> second;
         while (ok && share.next(a, tiling, p)) {
             if (p.blocks == 0) continue;
             const PgSpan span = pg_span(a, p.s, p.tile * pair_tokens, (p.tile + 1) * pair_tokens);
             const int* row = a.pages + p.seq * a.pages_stride;
-            int2 page = conv.pages(row, span, p.top * kPgKeys), before = page;
-            for (int j = 0; j <= p.blocks && ok; ++j) {
-                const int key0 = (p.top - j) * kPgKeys;
-                int2 next = page;
-                if (j + 1 < p.blocks) next = conv.pages(row, span, key0 - kPgKeys);
-                if (j < p.blocks) {
-                    if (loaded) ok = put();
-                    if (ok) conv.load(false, p.head, span, key0, page);
-                    loaded = true;
+            const int n = p.blocks;
+            // K0 K1, V0 K2, V1 K3, .., V(n-2) V(n-1): a pair a turn.  The pages of the next K, of the last one and of that before
+            int key0 = p.top * kPgKeys, next = conv.page(row, span, key0), last = -1, older = -1;
+#pragma unroll 1
+            for (int i = 0; i < n && ok; ++i) {
+                if (held) ok = put(first, false);
+                if (!ok) break;
+                if (i == 0) {
+                    conv.template copy<0>(false, p.head, span, key0, next);
+                    last = next;
+                    if (n > 1) next = conv.page(row, span, key0 - kPgKeys);
                 }
-                if (j > 0 && ok) {
-                    ok = put();
-                    if (ok) conv.load(true, p.head, span, key0 + kPgKeys, before);
+                else {
+                    conv.template copy<0>(true, p.head, span, key0 - (i - 1) * kPgKeys, older);
                 }
-                before = page;
-                page = next;
+                if (held) ok = put(second, false);
+                if (!ok) break;
+                if (i + 1 < n) {                                   // K(i + 1)
+                    conv.template copy<1>(false, p.head, span, key0 - (i + 1) * kPgKeys, next);
+                    older = last;
+                    last = next;
+                    if (i + 2 < n) next = conv.page(row, span, key0 - (i + 2) * kPgKeys);
+                }
+                else {                                             // V(n - 1)
+                    conv.template copy<1>(true, p.head, span, key0 - i * kPgKeys, last);
+                }
+                held = true;
             }
         }
-        if (ok && loaded) put();
+        if (held && ok) ok = put(first, false) && put(second, true);
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
     else if (warp < 8) {
         // ------------------------------------------------------------------ softmax, epilogue
@@ -581,8 +610,8 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
                 tmem_ld32_async(t_s + 96, v + 32);
                 if (!kCodes && (key0 < span.lo || key0 + kPgKeys > span.hi)) {
                     // rows of V that nobody sees (of codes: zeros already)
-                    const int entry = entry0 + pg_v_entry(j, blocks), stage = entry % kPgStages;
-                    if (!tc_wait_warp(&sm.full[stage], (uint32_t)((entry / kPgStages) & 1), &sm.abort)) {
+                    const int entry = entry0 + pg_v_entry(j, blocks), stage = entry % kRing;
+                    if (!tc_wait_warp(&sm.full[stage], (uint32_t)((entry / kRing) & 1), &sm.abort)) {
                         ok = false;
                         break;
                     }
@@ -721,9 +750,9 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
     }
 }
 
-constexpr int pg_tiles_smem(int head_dim)
+constexpr int pg_tiles_smem(int head_dim, int codes = 0)
 {
-    return (2 + kPgStages) * (head_dim / 64) * kPgRows * 128;
+    return (2 + pg_ring(head_dim, codes)) * (head_dim / 64) * kPgRows * 128 + (codes ? 4 * 2 * 32 * head_dim : 0);
 }
 
 template<typename T, int D, bool kBias>
@@ -783,7 +812,7 @@ paged_mha_tc_codes_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
 template<typename T, int D, bool kBias, int kCodes>
 int pg_launch_tc_codes(const PagedMhaArgs& a, void* ws, int least, int whole, cudaStream_t stream)
 {
-    constexpr int kSmem = pg_tiles_smem(D);
+    constexpr int kSmem = pg_tiles_smem(D, kCodes);
     CUtensorMap map_q;
     const long long q_dims[3] = {D, a.heads, a.tokens}, q_str[3] = {1, a.q_head, a.q_tok};
     const int group = a.heads / a.kv_heads, q_box[3] = {64, group, kPgRows / group};
