@@ -142,14 +142,47 @@ __device__ __forceinline__ void pg_init(PgSmem& sm, uint32_t writers = 1)
     mbar_fence_init();
 }
 
-// Sixteen codes times their scale as 16-bit values, two to a word.
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b)
+{
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+// Sixteen codes times their scale as 16-bit values, two to a word, by pairs.  A byte under the exponent of 2^23 is a number in fp32 at once, without
+// a trip through fp16 (60 instructions that way and 44 this way).
 template<typename T, int kCodes>
 __device__ __forceinline__ void pg_values16(const uint4& x, float scale, uint32_t (&out)[8])
 {
-    float y[16];
-    dequantize16<kCodes>(x, scale, y);
+    const uint32_t words[4] = {x.x, x.y, x.z, x.w};
+    const uint64_t scale2 = pair2(scale, scale);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) out[i] = PgType<T>::pack(y[2 * i], y[2 * i + 1]);
+    for (int i = 0; i < 4; ++i) {
+        uint64_t y[2];
+        if (kCodes == kCodesInt8) {
+            const uint32_t w = words[i] ^ 0x80808080u;
+            const uint64_t less = pair2(-8388736.0f, -8388736.0f);   // 2^23 + 128
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                y[e] = add2(pair2(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7540 | (2 * e))),
+                                  __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7540 | (2 * e + 1)))), less);
+            }
+        }
+        else {
+            uint32_t h[2];
+            codes_to_half<kCodes>(words[i], h[0], h[1]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[e]));
+                y[e] = pair2(f.x, f.y);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const float2 f = split2(mul2(y[e], scale2));
+            out[2 * i + e] = PgType<T>::pack(f.x, f.y);
+        }
+    }
 }
 
 // A warp that converts: its 32 keys of every entry of the ring, in the entries' order.  Their codes come through two places of the warp's own in
