@@ -525,7 +525,7 @@ paged_mha_both_kernel(const __grid_constant__ CUtensorMap map_q_rows, const __gr
 {
     static_assert(kPwThreads == kPgThreads, "one launch serves both");
     extern __shared__ __align__(1024) uint8_t pb_dyn[];
-    __shared__ __align__(16) uint8_t sm[sizeof(PgSmem) > sizeof(PwSmem) ? sizeof(PgSmem) : sizeof(PwSmem)];
+    __shared__ __align__(16) uint8_t sm[sizeof(PgSmemFound) > sizeof(PwSmem) ? sizeof(PgSmemFound) : sizeof(PwSmem)];
     __shared__ uint32_t tmem_base;
     if (smem_u32(pb_dyn) & 1023) {
         g_device_status = 2;
@@ -543,7 +543,7 @@ paged_mha_both_kernel(const __grid_constant__ CUtensorMap map_q_rows, const __gr
     }
     if (threadIdx.x == 0) {
         if (cta < n_rows) pw_init<D>(*reinterpret_cast<PwSmem*>(sm));
-        else pg_init(*reinterpret_cast<PgSmem*>(sm));
+        else pg_init(*reinterpret_cast<PgSmemFound*>(sm));
     }
     __syncthreads();
     if (cta < n_rows) {
@@ -551,8 +551,9 @@ paged_mha_both_kernel(const __grid_constant__ CUtensorMap map_q_rows, const __gr
                       pb_dyn);
     }
     else {
-        pg_tiles<T, D, kBias>(&map_q, &map_k, &map_v, a, ws, few + 1, whole, cta - n_rows, n - n_rows, n, *reinterpret_cast<PgSmem*>(sm),
-                              tmem_base, pb_dyn);
+        PgSmemFound& tiles_sm = *reinterpret_cast<PgSmemFound*>(sm);
+        pg_tiles<T, D, kBias>(&map_q, &map_k, &map_v, a, ws, few + 1, whole, cta - n_rows, n - n_rows, n, tiles_sm, tiles_sm.found, tmem_base,
+                              pb_dyn);
     }
     pg_end(&tmem_base, kPgTmemCols);
 }

@@ -24,11 +24,13 @@
 // Keys outside of what any row of the pair sees may be anything, even NaN (slots behind the end of a sequence): their scores are
 // masked by selection and their rows of V are set to zero in shared memory before the product reads them.
 //
-// Over a cache of 8-bit codes four more warps (12-15, a warpgroup of their own) put K and V into the ring: each copies its 32 keys of an entry
-// two entries ahead, multiplies the codes with the scale of their row in fp32, rounds once to q's type and writes that where the copy
-// engine would have put it; the rest of the kernel does not know.  (The scales could stay outside the products as in
-// paged_codes.cu, two multiplications and two reads of shared memory more for every score: the softmax is the bound here, and these warps
-// have time.)  512 threads of 128 registers are launched, of which the softmax takes 144 and the others 112.
+// Over a cache of 8-bit codes warp 8 brings codes and scales to two places in shared memory, an entry each, and four more warps (12-15, a
+// warpgroup of their own) put K and V into the ring from there: 32 keys of an entry each, codes times the scale of their row in fp32, rounded
+// once to q's type, written where the copy engine would have put it; the rest of the kernel does not know.  (The scales could stay outside
+// the products as in paged_codes.cu, two multiplications and two reads of shared memory more for every score: the softmax is the bound
+// here.)  What these warps do has to be little code as well as few instructions: five kinds of warps share an instruction cache (512 behind 8192,
+// 32 / 8 heads, bf16: unrolled 187 us, in a loop of 32 codes 130; with the copies among their duties 126).  512 threads of 128 registers are launched, of
+// which the softmax takes 144 and the others 112.
 #include <type_traits>
 
 #include "codes.cuh"
@@ -56,11 +58,15 @@ struct PgSmem {
     uint64_t o_full[2];      // the last P.V of a piece has completed
     uint64_t o_free[2];      // O has been read (four warps)
     uint64_t b_ready;        // split: b's maximum and sum are in b_max, b_sum, its O is complete (four warps)
+    uint64_t staged_full[2], staged_empty[2];   // codes: the two places they come to (33 arrivals and the bytes; four warps)
     volatile int abort;
-    float b_max[kPgRows], b_sum[kPgRows];
+    __align__(8) float b_max[kPgRows], b_sum[kPgRows];
     // what a softmax warp needs between its pieces, out of its registers while it works on one
     PgShare share[8];
     PgPiece piece[8];
+};
+
+struct PgSmemFound : PgSmem {
     PgFound found;
 };
 
@@ -138,6 +144,10 @@ __device__ __forceinline__ void pg_init(PgSmem& sm, uint32_t writers = 1)
         mbar_init(&sm.o_free[x], 4);
     }
     mbar_init(&sm.b_ready, 4);
+    for (int i = 0; i < 2; ++i) {
+        mbar_init(&sm.staged_full[i], 33);
+        mbar_init(&sm.staged_empty[i], 4);
+    }
     sm.abort = 0;
     mbar_fence_init();
 }
@@ -185,86 +195,85 @@ __device__ __forceinline__ void pg_values16(const uint4& x, float scale, uint32_
     }
 }
 
-// A warp that converts: its 32 keys of every entry of the ring, in the entries' order.  Their codes come through two places of the warp's own in
-// shared memory (cp.async), an entry ahead, their scales into a register of either place.
-template<typename T, int D, int kCodes>
-struct PgConverter {
-    static constexpr int kHalves = D / 64, kHalf = kPgRows * 128;
-    static constexpr int kEntry = 32 * D;                  // bytes
+// An entry of 128 keys' codes and scales on its way to its place, by a whole warp: a lane per page for the codes, a lane per key for the scales.
+// Scales of keys that the tile does not see, and of pages outside the cache, become zero, and with them the values.
+template<int D>
+struct PgCodesLoader {
+    static constexpr int kCodeBytes = kPgKeys * D, kEntry = kCodeBytes + kPgKeys * 4;
     const PagedMhaArgs& a;
-    int warp;                          // 0 .. 3
-    uint32_t staged;                   // the places
-    float scales[2];                   // a lane a key
+    const int* row;      // the sequence's row of the page table
+    int head;
+    PgSpan span;
 
-    // The pages of the two runs of 16 keys of a block at key0, in the lanes 0 .. 15 and 16 .. 31, as the table has them; -1: nobody sees them.
-    __device__ __forceinline__ int page(const int* row, const PgSpan& span, int key0) const
+    __device__ __forceinline__ int rows() const { return min(1 << a.page_shift, kPgKeys); }
+    // the page of keys rows() lane .. of the block at key0, in the lanes that have one; -1: nobody sees them
+    __device__ __forceinline__ int page(int key0) const
     {
-        const int key = key0 + 32 * warp + (int)(threadIdx.x & 16);
-        return key < span.hi && key + 16 > span.lo ? row[key >> a.page_shift] : -1;
+        const int key = key0 + (int)(threadIdx.x & 31) * rows();
+        return key < key0 + kPgKeys && key < span.hi && key + rows() > span.lo ? row[key >> a.page_shift] : -1;
     }
-    // Keys that the tile does not see, and pages outside the cache, become zeros.
-    template<int kSlot>
-    __device__ __forceinline__ void copy(bool v, int head, const PgSpan& span, int key0, int page)
+    __device__ __forceinline__ void load(const CUtensorMap* map, const float* scales, long long scale_page, long long scale_head, int key0,
+                                         int page, uint8_t* place, uint64_t* full) const
     {
-        constexpr int kChunks = D / 16, kRowsAtOnce = 32 / kChunks;
-        const int lane = threadIdx.x & 31, key = key0 + 32 * warp, row0 = lane / kChunks, c = lane % kChunks;
-        const uint32_t at = staged + (uint32_t)(kSlot * kEntry);
-        const uint8_t* cache = (const uint8_t*)(v ? a.v_cache : a.k_cache) + head * (v ? a.vc_head : a.kc_head) + 16 * c;
-        const long long page_step = v ? a.vc_page : a.kc_page, slot_step = v ? a.vc_slot : a.kc_slot;
-        const int mask = (1 << a.page_shift) - 1;
-        const bool known = page >= 0 && page < a.num_pages;
-        if (!known && key + (lane & 16) < span.hi && key + (lane & 16) + 16 > span.lo) g_device_status = 6;
-        const int n = known ? page : -1;
-#pragma unroll 1
-        for (int run = 0; run < 32; run += 16) {
-            const int m = __shfl_sync(0xffffffffu, n, run);
-            const uint8_t* src = cache + max(m, 0) * page_step + (((key + run) & mask) + row0) * slot_step;
-            const int from = m < 0 ? 32 : span.lo - key - run, upto = span.hi - key - run;
-            const uint32_t to = at + (uint32_t)((run + row0) * D + 16 * c);
-#pragma unroll
-            for (int i = 0; i < 16 / kRowsAtOnce; ++i) {
-                const int r = row0 + kRowsAtOnce * i;
-                copy16_async(to + kRowsAtOnce * i * D, src, r >= from && r < upto ? 16 : 0);
-                src += kRowsAtOnce * slot_step;
-            }
+        static_assert(kPgKeys == 128, "a shift below");
+        const int lane = threadIdx.x & 31, n = rows(), key = key0 + lane * n;
+        const bool mine = key < key0 + kPgKeys && key < span.hi && key + n > span.lo;
+        const int count = __popc(__ballot_sync(0xffffffffu, mine));
+        if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)(count * n * D));
+        __syncwarp();
+        if (mine && (page < 0 || page >= a.num_pages)) {
+            g_device_status = 6;
+            page = a.num_pages;   // behind the last: reads as zeros
         }
-        const bool seen = n >= 0 && key + lane >= span.lo && key + lane < span.hi;
-        const float* scale = (v ? a.v_scale + head * a.vs_head + max(n, 0) * a.vs_page : a.k_scale + head * a.ks_head + max(n, 0) * a.ks_page) +
-                             ((key + lane) & mask);
-        scales[kSlot] = 0.f;
-        if (seen) scales[kSlot] = *scale;
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    }
-    // Lane (r, c) = (lane / 4, lane % 4) has 16 codes of keys r, r + 8, r + 16 and r + 24 in either half of a row, odd keys the halves in the other
-    // order: eight lanes then meet no bank twice, reading or writing.
-    template<int kSlot>
-    __device__ __forceinline__ void store(uint8_t* stage) const
-    {
-        const int lane = threadIdx.x & 31;
-        const uint32_t at = staged + (uint32_t)(kSlot * kEntry);
-#pragma unroll 1
-        for (int i = 0; i < 4; ++i) {
-            const int r = 8 * i + (lane >> 2), key = 32 * warp + r;
-            const float scale = __shfl_sync(0xffffffffu, scales[kSlot], r);
+        if (mine) tma_load_4d(place + lane * n * D, map, 0, key & ((1 << a.page_shift) - 1), head, page, full);
+        const uint32_t to = smem_u32(place + kCodeBytes) + 4 * lane;
+        const float* from = scales + head * scale_head;
 #pragma unroll
-            for (int h = 0; h < kHalves; ++h) {
-                const int half = kHalves == 2 ? h ^ (r & 1) : 0;
-                uint32_t y[8];
-                pg_values16<T, kCodes>(lds128(at + (uint32_t)(r * D + 64 * half + 16 * (lane & 3))), scale, y);
-                uint8_t* dst = stage + half * kHalf + key * 128;
-                const int c = 2 * (lane & 3);
-                *reinterpret_cast<uint4*>(dst + ((c ^ (key & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
-                *reinterpret_cast<uint4*>(dst + (((c + 1) ^ (key & 7)) << 4)) = make_uint4(y[4], y[5], y[6], y[7]);
-            }
+        for (int i = 0; i < kPgKeys / 32; ++i) {
+            const int k = 32 * i + lane, of = __shfl_sync(0xffffffffu, page, k >> min(a.page_shift, 7)), at = key0 + k;
+            const bool seen = at >= span.lo && at < span.hi && of < a.num_pages;
+            copy4_async(to + 128 * i, from + (seen ? of : 0) * scale_page + (at & ((1 << a.page_shift) - 1)), seen ? 4 : 0);
         }
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(full)) : "memory");
     }
 };
 
-// The work of CTA `cta` of `ctas`; the scratch is laid out for `region` of them.  kCodes: the cache holds codes, and warps 12-15 convert them.
+// 32 keys of an entry into the ring.  Lane (r, c) = (lane / 4, lane % 4) has 16 codes of keys r, r + 8, r + 16 and r + 24 in either half of a row, odd
+// keys the halves in the other order: eight lanes then meet no bank twice, reading or writing.
+template<typename T, int D, int kCodes>
+__device__ __forceinline__ void pg_convert(const uint8_t* place, int key0, uint8_t* stage)
+{
+    constexpr int kHalves = D / 64, kHalf = kPgRows * 128;
+    const int lane = threadIdx.x & 31, c = 2 * (lane & 3);
+    const uint32_t codes = smem_u32(place) + 16 * (lane & 3), scales = smem_u32(place) + kPgKeys * D;
+#pragma unroll 1
+    for (int key = key0 + (lane >> 2); key < key0 + 32; key += 8) {
+        float scale;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(scale) : "r"(scales + 4 * key));
+        uint4 x[kHalves];
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h) x[h] = lds128(codes + (uint32_t)(key * D + 64 * (kHalves == 2 ? h ^ (key & 1) : 0)));
+        if (kCodes == kCodesE4M3 && __any_sync(0xffffffffu, scale == 0.f)) {   // (what nobody sees may be NaN, and nothing times that is NaN)
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h) x[h] = scale == 0.f ? make_uint4(0u, 0u, 0u, 0u) : x[h];
+        }
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h) {
+            uint32_t y[8];
+            pg_values16<T, kCodes>(x[h], scale, y);
+            uint8_t* dst = stage + (kHalves == 2 ? h ^ (key & 1) : 0) * kHalf + key * 128;
+            *reinterpret_cast<uint4*>(dst + ((c ^ (key & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
+            *reinterpret_cast<uint4*>(dst + (((c + 1) ^ (key & 7)) << 4)) = make_uint4(y[4], y[5], y[6], y[7]);
+        }
+    }
+}
+
+// The work of CTA `cta` of `ctas`; the scratch is laid out for `region` of them.  kCodes: the cache holds codes, which warps 12-15
+// convert, and map_k and map_v are of those.
 template<typename T, int D, bool kBias, int kCodes = 0>
 __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtensorMap* map_k, const CUtensorMap* map_v, const PagedMhaArgs& a,
                                          void* ws, int least, int whole, int cta, int ctas, int region, PgSmem& sm,
-                                         const uint32_t& tmem_base, uint8_t* dyn)
+                                         PgFound& found, const uint32_t& tmem_base, uint8_t* dyn)
 {
     constexpr int kHalves = D / 64;
     constexpr int kHalf = kPgRows * 128;         // bytes of [128 rows][64 values], swizzled
@@ -279,7 +288,8 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
 
     PgShare share;
     PgPlace place;
-    const bool work = pg_find_share(a, tiling, cta, ctas, whole != 0, sm.found, share, place);
+    const bool work = pg_find_share(a, tiling, cta, ctas, whole != 0, found, share, place);
+    if (kCodes) __syncthreads();   // (what it was found with lies in b_max, b_sum)
     const uint32_t tmem = tmem_base;
     PgPiece p;
 
@@ -309,7 +319,28 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
                             &sm.q_full);
             }
             if (p.s.p0 + p.s.tokens > cap && lane == 0) g_device_status = 6;
-            if (kCodes) continue;
+            if (kCodes) {
+                using Loader = PgCodesLoader<D>;
+                const Loader loader = {a, a.pages + p.seq * a.pages_stride, p.head, span};
+                uint8_t* places = ring + kRing * kTile;
+                const int n = p.blocks, key_top = p.top * kPgKeys;
+                int next = loader.page(key_top), last = -1, older = -1;   // pages of the next K, of the last one and of that before
+                for (int e = 0; e < 2 * n && ok; ++e) {                   // K0 K1 V0 K2 V1 ..
+                    const bool end = e == 2 * n - 1, v = end || (e > 0 && e % 2 == 0);
+                    const int j = end ? n - 1 : v ? e / 2 - 1 : (e + 1) / 2, x = issued & 1;
+                    ok = tc_wait_warp(&sm.staged_empty[x], (uint32_t)(((issued >> 1) + 1) & 1), &sm.abort);
+                    if (!ok) break;
+                    loader.load(v ? map_v : map_k, v ? a.v_scale : a.k_scale, v ? a.vs_page : a.ks_page, v ? a.vs_head : a.ks_head,
+                                key_top - j * kPgKeys, !v ? next : end ? last : older, places + x * Loader::kEntry, &sm.staged_full[x]);
+                    ++issued;
+                    if (!v) {
+                        older = last;
+                        last = next;
+                        if (j + 1 < n) next = loader.page(key_top - (j + 1) * kPgKeys);
+                    }
+                }
+                continue;
+            }
             const PgLoader<D> loader = {a, a.pages + p.seq * a.pages_stride, p.head, span};
             auto put = [&](const CUtensorMap* map, int j, int page) -> bool {
                 if (!tc_wait_warp(&sm.empty[stage], phase, &sm.abort)) return false;
@@ -331,7 +362,15 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
             }
         }
         if (!whole && lane == 0) pg_write_header(a, tiling, ws, cta, ctas, true, all, place);
-        if (sm.abort) {
+        if (kCodes) {
+            // (nor may copies by this warp's threads be on their way)
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            if (sm.abort) {
+                for (int e = max(0, issued - 2); e < issued; ++e) mbar_wait_bounded(&sm.staged_full[e & 1], (uint32_t)((e >> 1) & 1));
+                if (pieces > 0) mbar_wait_bounded(&sm.q_full, (uint32_t)((pieces - 1) & 1));
+            }
+        }
+        else if (sm.abort) {
             // nothing of this CTA may still be on its way when it ends
             for (int e = max(0, issued - kRing); e < issued; ++e) {
                 mbar_wait_bounded(&sm.full[e % kRing], (uint32_t)((e / kRing) & 1));
@@ -439,63 +478,29 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
     }
     else if (kCodes && warp >= 12) {
         // ------------------------------------------------------------------ codes into the ring
-        using Converter = PgConverter<T, D, kCodes ? kCodes : kCodesInt8>;
-        Converter conv = {a, warp - 12, smem_u32(ring + kRing * kTile) + (uint32_t)((warp - 12) * 2 * Converter::kEntry), {}};
-        int stage = 0;
+        using Loader = PgCodesLoader<D>;
+        const uint8_t* places = ring + kRing * kTile;
+        int stage = 0, done = 0;
         uint32_t phase = 1;                                       // of `empty`: the first round finds the stages free
-        bool ok = true, held = false;                             // both places hold an entry
-        auto put = [&](auto slot, bool last) -> bool {            // what a place holds; last: nothing has been copied behind it
-            if (last) asm volatile("cp.async.wait_group 0;" ::: "memory");
-            else asm volatile("cp.async.wait_group 1;" ::: "memory");
-            __syncwarp();
-            if (!tc_wait_warp(&sm.empty[stage], phase, &sm.abort)) return false;
-            conv.template store<decltype(slot)::value>(ring + stage * kTile);
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sm.full[stage]);
-            if (++stage == kRing) {
-                stage = 0;
-                phase ^= 1;
-            }
-            return true;
-        };
-        const std::integral_constant<int, 0> first;
-        const std::integral_constant<int, 1> second;
+        bool ok = true;
         while (ok && share.next(a, tiling, p)) {
-            if (p.blocks == 0) continue;
-            const PgSpan span = pg_span(a, p.s, p.tile * pair_tokens, (p.tile + 1) * pair_tokens);
-            const int* row = a.pages + p.seq * a.pages_stride;
-            const int n = p.blocks;
-            // K0 K1, V0 K2, V1 K3, .., V(n-2) V(n-1): a pair a turn.  The pages of the next K, of the last one and of that before
-            int key0 = p.top * kPgKeys, next = conv.page(row, span, key0), last = -1, older = -1;
-#pragma unroll 1
-            for (int i = 0; i < n && ok; ++i) {
-                if (held) ok = put(first, false);
+            for (int e = 0; e < 2 * p.blocks; ++e, ++done) {
+                const int x = done & 1;
+                ok = tc_wait_warp(&sm.staged_full[x], (uint32_t)((done >> 1) & 1), &sm.abort) && tc_wait_warp(&sm.empty[stage], phase, &sm.abort);
                 if (!ok) break;
-                if (i == 0) {
-                    conv.template copy<0>(false, p.head, span, key0, next);
-                    last = next;
-                    if (n > 1) next = conv.page(row, span, key0 - kPgKeys);
+                pg_convert<T, D, kCodes ? kCodes : kCodesInt8>(places + x * Loader::kEntry, 32 * (warp - 12), ring + stage * kTile);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&sm.full[stage]);
+                    mbar_arrive(&sm.staged_empty[x]);
                 }
-                else {
-                    conv.template copy<0>(true, p.head, span, key0 - (i - 1) * kPgKeys, older);
+                if (++stage == kRing) {
+                    stage = 0;
+                    phase ^= 1;
                 }
-                if (held) ok = put(second, false);
-                if (!ok) break;
-                if (i + 1 < n) {                                   // K(i + 1)
-                    conv.template copy<1>(false, p.head, span, key0 - (i + 1) * kPgKeys, next);
-                    older = last;
-                    last = next;
-                    if (i + 2 < n) next = conv.page(row, span, key0 - (i + 2) * kPgKeys);
-                }
-                else {                                             // V(n - 1)
-                    conv.template copy<1>(true, p.head, span, key0 - i * kPgKeys, last);
-                }
-                held = true;
             }
         }
-        if (held && ok) ok = put(first, false) && put(second, true);
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
     else if (warp < 8) {
         // ------------------------------------------------------------------ softmax, epilogue
@@ -785,7 +790,7 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
 
 constexpr int pg_tiles_smem(int head_dim, int codes = 0)
 {
-    return (2 + pg_ring(head_dim, codes)) * (head_dim / 64) * kPgRows * 128 + (codes ? 4 * 2 * 32 * head_dim : 0);
+    return (2 + pg_ring(head_dim, codes)) * (head_dim / 64) * kPgRows * 128 + (codes ? 2 * (kPgKeys * head_dim + kPgKeys * 4) : 0);
 }
 
 template<typename T, int D, bool kBias>
@@ -794,7 +799,7 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     const __grid_constant__ CUtensorMap map_v, const __grid_constant__ PagedMhaArgs a, void* ws, int whole)
 {
     extern __shared__ __align__(1024) uint8_t pg_dyn[];
-    __shared__ PgSmem sm;
+    __shared__ PgSmemFound sm;
     __shared__ uint32_t tmem_base;
     if (smem_u32(pg_dyn) & 1023) {   // the swizzle goes by addresses; the alignment above is there, so this does not happen
         g_device_status = 2;
@@ -802,7 +807,8 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     }
     if (threadIdx.x == 0) pg_init(sm);
     pg_begin(&tmem_base, kPgTmemCols);
-    pg_tiles<T, D, kBias>(&map_q, &map_k, &map_v, a, ws, 1, whole, (int)blockIdx.x, (int)gridDim.x, (int)gridDim.x, sm, tmem_base, pg_dyn);
+    pg_tiles<T, D, kBias>(&map_q, &map_k, &map_v, a, ws, 1, whole, (int)blockIdx.x, (int)gridDim.x, (int)gridDim.x, sm, sm.found, tmem_base,
+                          pg_dyn);
     pg_end(&tmem_base, kPgTmemCols);
 }
 
@@ -821,7 +827,8 @@ __device__ __forceinline__ void pg_fewer_registers()
 // Sequences of `least` new tokens and more, over a cache of codes.
 template<typename T, int D, bool kBias, int kCodes>
 __global__ void __launch_bounds__(kPgCodesThreads, 1)
-paged_mha_tc_codes_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ PagedMhaArgs a, void* ws, int least, int whole)
+paged_mha_tc_codes_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                          const __grid_constant__ CUtensorMap map_v, const __grid_constant__ PagedMhaArgs a, void* ws, int least, int whole)
 {
     static_assert(2 * 144 + 112 + 112 <= 4 * 128, "of what the CTA was launched with");
     extern __shared__ __align__(1024) uint8_t pg_dyn[];
@@ -837,19 +844,39 @@ paged_mha_tc_codes_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     if (group < 2) pg_more_registers<144>();
     else if (group == 2) pg_fewer_registers<112>();
     else pg_fewer_registers<112>();
-    pg_tiles<T, D, kBias, kCodes>(&map_q, nullptr, nullptr, a, ws, least, whole, (int)blockIdx.x, (int)gridDim.x, (int)gridDim.x, sm, tmem_base,
-                                  pg_dyn);
+    static_assert(sizeof(PgFound) <= sizeof(sm.b_max) + sizeof(sm.b_sum) && alignof(PgFound) <= 8, "lies there for a while");
+    pg_tiles<T, D, kBias, kCodes>(&map_q, &map_k, &map_v, a, ws, least, whole, (int)blockIdx.x, (int)gridDim.x, (int)gridDim.x, sm,
+                                  *reinterpret_cast<PgFound*>(sm.b_max), tmem_base, pg_dyn);
     pg_end(&tmem_base, kPgTmemCols);
+}
+
+// Codes as [page][head][slot][dim] bytes, boxes of a page (of 128 slots of a larger one) and a head.
+template<int D>
+int pg_encode_codes(CUtensorMap* map, const void* base, const PagedMhaArgs& a, long long page_step, long long head_step, long long slot_step)
+{
+    EncodeTiledFn encode = encode_tiled_fn();
+    EET_CHECK(encode != nullptr, "paged attention: cuTensorMapEncodeTiled is not available from the driver");
+    const int page = 1 << a.page_shift;
+    const cuuint64_t dims[4] = {D, (cuuint64_t)page, (cuuint64_t)a.kv_heads, (cuuint64_t)a.num_pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)slot_step, (cuuint64_t)head_step, (cuuint64_t)page_step};
+    const cuuint32_t box[4] = {D, (cuuint32_t)(page < kPgKeys ? page : kPgKeys), 1, 1}, elem[4] = {1, 1, 1, 1};
+    const CUresult rc = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, box, elem,
+                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    EET_CHECK(rc == CUDA_SUCCESS, "paged attention: cuTensorMapEncodeTiled failed with code %d (strides too large or negative)", (int)rc);
+    return 0;
 }
 
 template<typename T, int D, bool kBias, int kCodes>
 int pg_launch_tc_codes(const PagedMhaArgs& a, void* ws, int least, int whole, cudaStream_t stream)
 {
     constexpr int kSmem = pg_tiles_smem(D, kCodes);
-    CUtensorMap map_q;
+    CUtensorMap map_q, map_k, map_v;
     const long long q_dims[3] = {D, a.heads, a.tokens}, q_str[3] = {1, a.q_head, a.q_tok};
     const int group = a.heads / a.kv_heads, q_box[3] = {64, group, kPgRows / group};
     if (int rc = pg_encode(&map_q, PgType<T>::tma, a.q, 3, q_dims, q_str, q_box)) return rc;
+    if (int rc = pg_encode_codes<D>(&map_k, a.k_cache, a, a.kc_page, a.kc_head, a.kc_slot)) return rc;
+    if (int rc = pg_encode_codes<D>(&map_v, a.v_cache, a, a.vc_page, a.vc_head, a.vc_slot)) return rc;
     auto kern = paged_mha_tc_codes_kernel<T, D, kBias, kCodes>;
     static bool attr_set[64] = {};
     int dev = 0;
@@ -859,7 +886,7 @@ int pg_launch_tc_codes(const PagedMhaArgs& a, void* ws, int least, int whole, cu
         EET_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
         attr_set[dev] = true;
     }
-    EET_CUDA(launch_pdl(kern, dim3(sm_count()), dim3(kPgCodesThreads), kSmem, stream, map_q, a, ws, least, whole));
+    EET_CUDA(launch_pdl(kern, dim3(sm_count()), dim3(kPgCodesThreads), kSmem, stream, map_q, map_k, map_v, a, ws, least, whole));
     return 0;
 }
 
