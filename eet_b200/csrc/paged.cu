@@ -423,8 +423,8 @@ static int launch_paged_mha_t(const PagedMhaArgs& a, const PagedPlan& p, cudaStr
     if (rc) return rc;
     PgScratch s[2] = {};
     int n = 0;
-    if (p.bytes[0]) s[n++] = {ws[0], kPwRows, 0};
-    if (p.bytes[1]) s[n++] = {ws[1], 2 * kPgRows, 1};
+    if (p.bytes[0]) s[n++] = {ws[0], kPwRows, 0, sm_count()};
+    if (p.bytes[1]) s[n++] = {ws[1], 2 * kPgRows, 1, sm_count()};
     if (n > 0) {
         const long long rows = (long long)a.max_tokens * (a.heads / a.kv_heads), most = p.bytes[1] ? 2 * kPgRows : kPwRows;
         const int y = (int)((rows < most ? rows : most) * (D / 8) + kPgJoinThreads - 1) / kPgJoinThreads;   // 8 dims a thread

@@ -141,9 +141,28 @@ struct PcCopies {
     }
 };
 
+// Both kinds of work at once: sequences of up to `few` new tokens for the kernel of few rows, the others for tiles of 128, each on a part of the
+// SMs that goes by what their blocks take (measured with heads of 128: 1.0 us a block with an SM's three CTAs, 2.7 as a pair of tiles, 3.5
+// with a bias).  The kernel of tiles is launched first: a CTA of it fills an SM, those without work leave theirs, and the three of the
+// other kernel go where there is room - which they find by themselves, since that one does not wait for this one before its end.  So
+// this one lets it begin only when the kernels in front have ended for sure.
+struct PcSplit {
+    int sms_rows, sms_tiles;
+};
+
+__device__ __forceinline__ PcSplit pc_split(const PagedMhaArgs& a, int rows_tokens, int few, int sms, bool bias)
+{
+    const PgTiling rows = {rows_tokens, 1, few, kPcExtra}, tiles = {2 * (kPgRows / (a.heads / a.kv_heads)), few + 1, 0x7fffffff, kPgExtra};
+    const float in_rows = (float)pg_total(a, rows), in_tiles = (float)pg_total(a, tiles) * (bias ? 3.5f : 2.7f);
+    if (!(in_rows > 0.f)) return {0, sms};
+    if (!(in_tiles > 0.f)) return {sms, 0};
+    const int n = min(max((int)(sms * in_rows / (in_rows + in_tiles) + 0.5f), 1), sms - 1);
+    return {n, sms - n};
+}
+
 template<int kCodes, int D, int kRows>
 __global__ void __launch_bounds__(32 * PcShape<D, kRows>::kWarps, PcShape<D, kRows>::kPerSm)
-paged_mha_codes_kernel(const __grid_constant__ PagedMhaArgs a, void* ws, int most, int whole)
+paged_mha_codes_kernel(const __grid_constant__ PagedMhaArgs a, void* ws, int few, int beside)
 {
     using Shape = PcShape<D, kRows>;
     constexpr int kN = kRows / 8;                // tiles of 8 rows
@@ -154,16 +173,26 @@ paged_mha_codes_kernel(const __grid_constant__ PagedMhaArgs a, void* ws, int mos
     __shared__ PcSmem sm;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int group = a.heads / a.kv_heads, tile_tokens = kRows / group;
-    const int cta = blockIdx.x, ctas = gridDim.x;
-    const PgTiling tiling = {tile_tokens, 1, most, kPcExtra};
+    const int cta = blockIdx.x, region = gridDim.x;
+    const PgTiling tiling = {tile_tokens, 1, few, kPcExtra};
     pdl_launch_dependents();
-    pdl_wait();
+    // (beside the kernel of tiles: that one has waited already, and its end is waited for at the end)
+    if (!beside) pdl_wait();
+    const int ctas = beside ? Shape::kPerSm * pc_split(a, tile_tokens, few, region / Shape::kPerSm, beside > 1).sms_rows : region;
+    if (cta >= ctas) {
+        if (threadIdx.x == 0) reinterpret_cast<PgHeader*>(ws)[cta] = {};
+        pdl_wait();
+        return;
+    }
     {
         PgShare share;
         PgPlace place;
-        const bool work = pg_find_share(a, tiling, cta, ctas, whole != 0, sm.found, share, place);
-        if (!whole && threadIdx.x == 0) pg_write_header(a, tiling, ws, cta, ctas, work, share, place);
-        if (!work) return;
+        const bool work = pg_find_share(a, tiling, cta, ctas, false, sm.found, share, place);
+        if (threadIdx.x == 0) pg_write_header(a, tiling, ws, cta, ctas, work, share, place);
+        if (!work) {
+            pdl_wait();
+            return;
+        }
         if (lane == 0) sm.share[warp] = share;
         __syncwarp();
     }
@@ -509,7 +538,7 @@ paged_mha_codes_kernel(const __grid_constant__ PagedMhaArgs a, void* ws, int mos
         }
         __syncthreads();
         const bool complete = p.starts && p.ends;
-        const PgPartial part = pg_partial(ws, ctas, cta, p.starts ? 1 : 0, kRows, D);
+        const PgPartial part = pg_partial(ws, region, cta, p.starts ? 1 : 0, kRows, D);
         for (int i = threadIdx.x; i < rows * (D / 4); i += 32 * Shape::kWarps) {
             const int row = i / (D / 4), d = i % (D / 4) * 4;
             float top = kPgNone, sum = 0.f;
@@ -555,10 +584,109 @@ paged_mha_codes_kernel(const __grid_constant__ PagedMhaArgs a, void* ws, int mos
         else if (have_next) copy_from(now ^ 1);              // that one is copied, or has nothing to copy
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
+    pdl_wait();
+}
+
+// Moves registers between the warpgroups; by all warps of a warpgroup.
+template<int kRegisters>
+__device__ __forceinline__ void pg_more_registers()
+{
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegisters));
+}
+template<int kRegisters>
+__device__ __forceinline__ void pg_fewer_registers()
+{
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegisters));
+}
+
+// As pg_begin, but a dependent may begin only when the kernels in front have ended.
+__device__ __forceinline__ void pc_begin(uint32_t* tmem_base, uint32_t columns)
+{
+    if ((threadIdx.x >> 5) == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_base)), "r"(columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    pdl_wait();
+    pdl_launch_dependents();
+}
+
+// Sequences of more than `few` new tokens; rows_tokens: those of a tile of the other kernel, where that one runs beside this (else 0).
+template<typename T, int D, bool kBias, int kCodes>
+__global__ void __launch_bounds__(kPgCodesThreads, 1)
+paged_mha_tc_codes_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                          const __grid_constant__ CUtensorMap map_v, const __grid_constant__ PagedMhaArgs a, void* ws, int few, int rows_tokens)
+{
+    static_assert(2 * 144 + 112 + 112 <= 4 * 128, "of what the CTA was launched with");
+    extern __shared__ __align__(1024) uint8_t pg_dyn[];
+    __shared__ PgSmem sm;
+    __shared__ uint32_t tmem_base;
+    if (smem_u32(pg_dyn) & 1023) {   // the swizzle goes by addresses; the alignment above is there, so this does not happen
+        g_device_status = 2;
+        return;
+    }
+    if (threadIdx.x == 0) pg_init(sm, 4);
+    pc_begin(&tmem_base, kPgTmemCols);
+    const int n = gridDim.x, cta = blockIdx.x, ctas = rows_tokens ? pc_split(a, rows_tokens, few, n, kBias).sms_tiles : n;
+    const int group = threadIdx.x >> 7;
+    if (group < 2) pg_more_registers<144>();
+    else if (group == 2) pg_fewer_registers<112>();
+    else pg_fewer_registers<112>();
+    static_assert(sizeof(PgFound) <= sizeof(sm.b_max) + sizeof(sm.b_sum) && alignof(PgFound) <= 8, "lies there for a while");
+    if (cta < ctas) {
+        pg_tiles<T, D, kBias, kCodes>(&map_q, &map_k, &map_v, a, ws, few + 1, 0, cta, ctas, n, sm, *reinterpret_cast<PgFound*>(sm.b_max), tmem_base,
+                                      pg_dyn);
+    }
+    else if (threadIdx.x == 0) {
+        reinterpret_cast<PgHeader*>(ws)[cta] = {};
+    }
+    pg_end(&tmem_base, kPgTmemCols);
+}
+
+// Codes as [page][head][slot][dim] bytes, boxes of a page (of 128 slots of a larger one) and a head.
+template<int D>
+int pg_encode_codes(CUtensorMap* map, const void* base, const PagedMhaArgs& a, long long page_step, long long head_step, long long slot_step)
+{
+    EncodeTiledFn encode = encode_tiled_fn();
+    EET_CHECK(encode != nullptr, "paged attention: cuTensorMapEncodeTiled is not available from the driver");
+    const int page = 1 << a.page_shift;
+    const cuuint64_t dims[4] = {D, (cuuint64_t)page, (cuuint64_t)a.kv_heads, (cuuint64_t)a.num_pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)slot_step, (cuuint64_t)head_step, (cuuint64_t)page_step};
+    const cuuint32_t box[4] = {D, (cuuint32_t)(page < kPgKeys ? page : kPgKeys), 1, 1}, elem[4] = {1, 1, 1, 1};
+    const CUresult rc = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, box, elem,
+                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    EET_CHECK(rc == CUDA_SUCCESS, "paged attention: cuTensorMapEncodeTiled failed with code %d (strides too large or negative)", (int)rc);
+    return 0;
+}
+
+template<typename T, int D, bool kBias, int kCodes>
+int pc_launch_tiles(const PagedMhaArgs& a, void* ws, int few, int rows_tokens, cudaStream_t stream)
+{
+    constexpr int kSmem = pg_tiles_smem(D, kCodes);
+    CUtensorMap map_q, map_k, map_v;
+    const long long q_dims[3] = {D, a.heads, a.tokens}, q_str[3] = {1, a.q_head, a.q_tok};
+    const int group = a.heads / a.kv_heads, q_box[3] = {64, group, kPgRows / group};
+    if (int rc = pg_encode(&map_q, PgType<T>::tma, a.q, 3, q_dims, q_str, q_box)) return rc;
+    if (int rc = pg_encode_codes<D>(&map_k, a.k_cache, a, a.kc_page, a.kc_head, a.kc_slot)) return rc;
+    if (int rc = pg_encode_codes<D>(&map_v, a.v_cache, a, a.vc_page, a.vc_head, a.vc_slot)) return rc;
+    auto kern = paged_mha_tc_codes_kernel<T, D, kBias, kCodes>;
+    static bool attr_set[64] = {};
+    int dev = 0;
+    EET_CUDA(cudaGetDevice(&dev));
+    dev &= 63;
+    if (!attr_set[dev]) {
+        EET_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+        attr_set[dev] = true;
+    }
+    EET_CUDA(launch_pdl(kern, dim3(sm_count()), dim3(kPgCodesThreads), kSmem, stream, map_q, map_k, map_v, a, ws, few, rows_tokens));
+    return 0;
 }
 
 template<int kCodes, int D, int kRows>
-int pc_launch(const PagedMhaArgs& a, void* ws, int most, int whole, cudaStream_t stream)
+int pc_launch(const PagedMhaArgs& a, void* ws, int few, int beside, cudaStream_t stream)
 {
     auto kern = paged_mha_codes_kernel<kCodes, D, kRows>;
     constexpr int kSmem = PcShape<D, kRows>::kSmem;
@@ -570,7 +698,7 @@ int pc_launch(const PagedMhaArgs& a, void* ws, int most, int whole, cudaStream_t
         EET_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
         attr_set[dev] = true;
     }
-    EET_CUDA(launch_pdl(kern, dim3(PcShape<D, kRows>::kPerSm * sm_count()), dim3(32 * PcShape<D, kRows>::kWarps), kSmem, stream, a, ws, most, whole));
+    EET_CUDA(launch_pdl(kern, dim3(PcShape<D, kRows>::kPerSm * sm_count()), dim3(32 * PcShape<D, kRows>::kWarps), kSmem, stream, a, ws, few, beside));
     return 0;
 }
 
@@ -617,26 +745,27 @@ template<typename T, int D, int kCodes>
 static int launch_paged_mha_codes_t(const PagedMhaArgs& a, const PagedCodesPlan& p, cudaStream_t stream)
 {
     void* ws[2] = {a.ws, (char*)a.ws + p.bytes[0]};
-    auto join = [&](const PgScratch& s, int ctas) -> int {
-        const PgScratch none = {};
-        const long long rows = (long long)a.max_tokens * (a.heads / a.kv_heads);
-        const int y = (int)((rows < s.rows ? rows : s.rows) * (D / 8) + kPgJoinThreads - 1) / kPgJoinThreads;   // 8 dims a thread
-        EET_CUDA(launch_pdl(paged_mha_join_kernel<T, D>, dim3(ctas, y, 1), dim3(kPgJoinThreads), 0, stream, a, s, none));
-        return 0;
-    };
-    if (p.rows) {
-        const int most = p.tiles ? p.few : 0x7fffffff;
-        if (int rc = p.rows == 8 ? pc_launch<kCodes, D, 8>(a, ws[0], most, 0, stream) : pc_launch<kCodes, D, 16>(a, ws[0], most, 0, stream)) return rc;
-        if (int rc = join({ws[0], p.rows, 0}, pc_per_sm(p.rows) * sm_count())) return rc;
-    }
+    const bool both = p.rows && p.tiles;
+    // (the tiles without a bias take the maximum of the scores before the scale, which a negative one would turn round)
+    const bool bias = a.slopes != nullptr || !(a.scale > 0.f);
     if (p.tiles) {
-        // (the tiles without a bias take the maximum of the scores before the scale, which a negative one would turn round)
-        const bool bias = a.slopes != nullptr || !(a.scale > 0.f);
-        const int least = p.rows ? p.few + 1 : 1;
-        if (int rc = bias ? pg_launch_tc_codes<T, D, true, kCodes>(a, ws[1], least, 0, stream)
-                          : pg_launch_tc_codes<T, D, false, kCodes>(a, ws[1], least, 0, stream)) return rc;
-        if (int rc = join({ws[1], 2 * kPgRows, 1}, sm_count())) return rc;
+        const int few = both ? p.few : 0, rows_tokens = both ? p.few : 0;
+        if (int rc = bias ? pc_launch_tiles<T, D, true, kCodes>(a, ws[1], few, rows_tokens, stream)
+                          : pc_launch_tiles<T, D, false, kCodes>(a, ws[1], few, rows_tokens, stream)) return rc;
     }
+    if (p.rows) {
+        const int few = both ? p.few : 0x7fffffff, beside = !both ? 0 : bias ? 2 : 1;
+        if (int rc = p.rows == 8 ? pc_launch<kCodes, D, 8>(a, ws[0], few, beside, stream) : pc_launch<kCodes, D, 16>(a, ws[0], few, beside, stream)) return rc;
+    }
+    // One launch adds up the parts of either kind.  (Its grid is that of the larger number of CTAs; the scratch of each kind knows its own.)
+    PgScratch s[2] = {};
+    int n = 0;
+    if (p.rows) s[n++] = {ws[0], p.rows, 0, pc_per_sm(p.rows) * sm_count()};
+    if (p.tiles) s[n++] = {ws[1], 2 * kPgRows, 1, sm_count()};
+    const long long rows = (long long)a.max_tokens * (a.heads / a.kv_heads), most = p.tiles ? 2 * kPgRows : p.rows;
+    const int y = (int)((rows < most ? rows : most) * (D / 8) + kPgJoinThreads - 1) / kPgJoinThreads;   // 8 dims a thread
+    const int ctas = s[0].ctas > s[1].ctas ? s[0].ctas : s[1].ctas;
+    EET_CUDA(launch_pdl(paged_mha_join_kernel<T, D>, dim3(ctas, y, n), dim3(kPgJoinThreads), 0, stream, a, s[0], s[1]));
     return 0;
 }
 

@@ -402,6 +402,7 @@ struct PgScratch {
     void* ws;
     int rows;              // of a partial result; 0: none
     int by_dim;            // O is [D / 4][rows], and a tile of 128 rows holds whole tokens only
+    int ctas;              // that it is laid out for
 };
 
 // Adds up the partial results of the tiles that end in CTA blockIdx.x of one of the kernels (blockIdx.z), 8 dims of a row a
@@ -417,9 +418,10 @@ __global__ void __launch_bounds__(kPgJoinThreads, 6) paged_mha_join_kernel(const
     constexpr int kAhead = 4;   // parts on their way
     pdl_wait();
     const PgScratch s = blockIdx.z ? s1 : s0;
+    if ((int)blockIdx.x >= s.ctas) return;
     const PgHeader h = reinterpret_cast<const PgHeader*>(s.ws)[blockIdx.x];
     if (h.kind != 1) return;
-    const int cta = blockIdx.x, ctas = gridDim.x;
+    const int cta = blockIdx.x, ctas = s.ctas;
     const int group = a.heads / a.kv_heads;
     const int rows = h.tokens * group;
     const int per_tile = s.by_dim ? kPgRows / group * group : s.rows;   // rows of a tile in use

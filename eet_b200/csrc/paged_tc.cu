@@ -812,84 +812,6 @@ paged_mha_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     pg_end(&tmem_base, kPgTmemCols);
 }
 
-// Moves registers between the warpgroups; by all warps of a warpgroup.
-template<int kRegisters>
-__device__ __forceinline__ void pg_more_registers()
-{
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegisters));
-}
-template<int kRegisters>
-__device__ __forceinline__ void pg_fewer_registers()
-{
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegisters));
-}
-
-// Sequences of `least` new tokens and more, over a cache of codes.
-template<typename T, int D, bool kBias, int kCodes>
-__global__ void __launch_bounds__(kPgCodesThreads, 1)
-paged_mha_tc_codes_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                          const __grid_constant__ CUtensorMap map_v, const __grid_constant__ PagedMhaArgs a, void* ws, int least, int whole)
-{
-    static_assert(2 * 144 + 112 + 112 <= 4 * 128, "of what the CTA was launched with");
-    extern __shared__ __align__(1024) uint8_t pg_dyn[];
-    __shared__ PgSmem sm;
-    __shared__ uint32_t tmem_base;
-    if (smem_u32(pg_dyn) & 1023) {   // the swizzle goes by addresses; the alignment above is there, so this does not happen
-        g_device_status = 2;
-        return;
-    }
-    if (threadIdx.x == 0) pg_init(sm, 4);
-    pg_begin(&tmem_base, kPgTmemCols);
-    const int group = threadIdx.x >> 7;
-    if (group < 2) pg_more_registers<144>();
-    else if (group == 2) pg_fewer_registers<112>();
-    else pg_fewer_registers<112>();
-    static_assert(sizeof(PgFound) <= sizeof(sm.b_max) + sizeof(sm.b_sum) && alignof(PgFound) <= 8, "lies there for a while");
-    pg_tiles<T, D, kBias, kCodes>(&map_q, &map_k, &map_v, a, ws, least, whole, (int)blockIdx.x, (int)gridDim.x, (int)gridDim.x, sm,
-                                  *reinterpret_cast<PgFound*>(sm.b_max), tmem_base, pg_dyn);
-    pg_end(&tmem_base, kPgTmemCols);
-}
-
-// Codes as [page][head][slot][dim] bytes, boxes of a page (of 128 slots of a larger one) and a head.
-template<int D>
-int pg_encode_codes(CUtensorMap* map, const void* base, const PagedMhaArgs& a, long long page_step, long long head_step, long long slot_step)
-{
-    EncodeTiledFn encode = encode_tiled_fn();
-    EET_CHECK(encode != nullptr, "paged attention: cuTensorMapEncodeTiled is not available from the driver");
-    const int page = 1 << a.page_shift;
-    const cuuint64_t dims[4] = {D, (cuuint64_t)page, (cuuint64_t)a.kv_heads, (cuuint64_t)a.num_pages};
-    const cuuint64_t strides[3] = {(cuuint64_t)slot_step, (cuuint64_t)head_step, (cuuint64_t)page_step};
-    const cuuint32_t box[4] = {D, (cuuint32_t)(page < kPgKeys ? page : kPgKeys), 1, 1}, elem[4] = {1, 1, 1, 1};
-    const CUresult rc = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, box, elem,
-                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    EET_CHECK(rc == CUDA_SUCCESS, "paged attention: cuTensorMapEncodeTiled failed with code %d (strides too large or negative)", (int)rc);
-    return 0;
-}
-
-template<typename T, int D, bool kBias, int kCodes>
-int pg_launch_tc_codes(const PagedMhaArgs& a, void* ws, int least, int whole, cudaStream_t stream)
-{
-    constexpr int kSmem = pg_tiles_smem(D, kCodes);
-    CUtensorMap map_q, map_k, map_v;
-    const long long q_dims[3] = {D, a.heads, a.tokens}, q_str[3] = {1, a.q_head, a.q_tok};
-    const int group = a.heads / a.kv_heads, q_box[3] = {64, group, kPgRows / group};
-    if (int rc = pg_encode(&map_q, PgType<T>::tma, a.q, 3, q_dims, q_str, q_box)) return rc;
-    if (int rc = pg_encode_codes<D>(&map_k, a.k_cache, a, a.kc_page, a.kc_head, a.kc_slot)) return rc;
-    if (int rc = pg_encode_codes<D>(&map_v, a.v_cache, a, a.vc_page, a.vc_head, a.vc_slot)) return rc;
-    auto kern = paged_mha_tc_codes_kernel<T, D, kBias, kCodes>;
-    static bool attr_set[64] = {};
-    int dev = 0;
-    EET_CUDA(cudaGetDevice(&dev));
-    dev &= 63;
-    if (!attr_set[dev]) {
-        EET_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
-        attr_set[dev] = true;
-    }
-    EET_CUDA(launch_pdl(kern, dim3(sm_count()), dim3(kPgCodesThreads), kSmem, stream, map_q, map_k, map_v, a, ws, least, whole));
-    return 0;
-}
-
 template<typename T, int D, bool kBias>
 int pg_launch_tc(const PagedMhaArgs& a, void* ws, int whole, cudaStream_t stream)
 {
