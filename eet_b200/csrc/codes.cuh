@@ -56,7 +56,11 @@ __device__ __forceinline__ void quantize16(const float (&y)[16], float scale, ui
         if (kCodes == kCodesInt8) {
             codes[w] = 0;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) codes[w] |= ((uint32_t)__float2int_rn(z[4 * w + e]) & 0xffu) << (8 * e);
+            for (int e = 0; e < 4; e += 2) {
+                // (whole numbers, in two's complement, as the low bits of a sum with 1.5 2^23)
+                const uint32_t lo = __float_as_uint(z[4 * w + e] + 12582912.0f), hi = __float_as_uint(z[4 * w + e + 1] + 12582912.0f);
+                codes[w] = e == 0 ? __byte_perm(lo, hi, 0x0040) : __byte_perm(codes[w], __byte_perm(lo, hi, 0x0040), 0x5410);
+            }
         }
         else {
             uint16_t lo, hi;

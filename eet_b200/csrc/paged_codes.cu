@@ -162,7 +162,7 @@ __device__ __forceinline__ PcSplit pc_split(const PagedMhaArgs& a, int rows_toke
 
 template<int kCodes, int D, int kRows>
 __global__ void __launch_bounds__(32 * PcShape<D, kRows>::kWarps, PcShape<D, kRows>::kPerSm)
-paged_mha_codes_kernel(const __grid_constant__ PagedMhaArgs a, void* ws, int few, int beside)
+paged_mha_codes_kernel(const __grid_constant__ PagedMhaArgs a, void* ws, int few, int beside, int whole)
 {
     using Shape = PcShape<D, kRows>;
     constexpr int kN = kRows / 8;                // tiles of 8 rows
@@ -180,15 +180,15 @@ paged_mha_codes_kernel(const __grid_constant__ PagedMhaArgs a, void* ws, int few
     if (!beside) pdl_wait();
     const int ctas = beside ? Shape::kPerSm * pc_split(a, tile_tokens, few, region / Shape::kPerSm, beside > 1).sms_rows : region;
     if (cta >= ctas) {
-        if (threadIdx.x == 0) reinterpret_cast<PgHeader*>(ws)[cta] = {};
+        if (!whole && threadIdx.x == 0) reinterpret_cast<PgHeader*>(ws)[cta] = {};
         pdl_wait();
         return;
     }
     {
         PgShare share;
         PgPlace place;
-        const bool work = pg_find_share(a, tiling, cta, ctas, false, sm.found, share, place);
-        if (threadIdx.x == 0) pg_write_header(a, tiling, ws, cta, ctas, work, share, place);
+        const bool work = pg_find_share(a, tiling, cta, ctas, whole != 0, sm.found, share, place);
+        if (!whole && threadIdx.x == 0) pg_write_header(a, tiling, ws, cta, ctas, work, share, place);
         if (!work) {
             pdl_wait();
             return;
@@ -617,7 +617,8 @@ __device__ __forceinline__ void pc_begin(uint32_t* tmem_base, uint32_t columns)
 template<typename T, int D, bool kBias, int kCodes>
 __global__ void __launch_bounds__(kPgCodesThreads, 1)
 paged_mha_tc_codes_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                          const __grid_constant__ CUtensorMap map_v, const __grid_constant__ PagedMhaArgs a, void* ws, int few, int rows_tokens)
+                          const __grid_constant__ CUtensorMap map_v, const __grid_constant__ PagedMhaArgs a, void* ws, int few, int rows_tokens,
+                          int whole)
 {
     static_assert(2 * 144 + 112 + 112 <= 4 * 128, "of what the CTA was launched with");
     extern __shared__ __align__(1024) uint8_t pg_dyn[];
@@ -636,10 +637,10 @@ paged_mha_tc_codes_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     else pg_fewer_registers<112>();
     static_assert(sizeof(PgFound) <= sizeof(sm.b_max) + sizeof(sm.b_sum) && alignof(PgFound) <= 8, "lies there for a while");
     if (cta < ctas) {
-        pg_tiles<T, D, kBias, kCodes>(&map_q, &map_k, &map_v, a, ws, few + 1, 0, cta, ctas, n, sm, *reinterpret_cast<PgFound*>(sm.b_max), tmem_base,
+        pg_tiles<T, D, kBias, kCodes>(&map_q, &map_k, &map_v, a, ws, few + 1, whole, cta, ctas, n, sm, *reinterpret_cast<PgFound*>(sm.b_max), tmem_base,
                                       pg_dyn);
     }
-    else if (threadIdx.x == 0) {
+    else if (!whole && threadIdx.x == 0) {
         reinterpret_cast<PgHeader*>(ws)[cta] = {};
     }
     pg_end(&tmem_base, kPgTmemCols);
@@ -663,7 +664,7 @@ int pg_encode_codes(CUtensorMap* map, const void* base, const PagedMhaArgs& a, l
 }
 
 template<typename T, int D, bool kBias, int kCodes>
-int pc_launch_tiles(const PagedMhaArgs& a, void* ws, int few, int rows_tokens, cudaStream_t stream)
+int pc_launch_tiles(const PagedMhaArgs& a, void* ws, int few, int rows_tokens, int whole, cudaStream_t stream)
 {
     constexpr int kSmem = pg_tiles_smem(D, kCodes);
     CUtensorMap map_q, map_k, map_v;
@@ -681,12 +682,12 @@ int pc_launch_tiles(const PagedMhaArgs& a, void* ws, int few, int rows_tokens, c
         EET_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
         attr_set[dev] = true;
     }
-    EET_CUDA(launch_pdl(kern, dim3(sm_count()), dim3(kPgCodesThreads), kSmem, stream, map_q, map_k, map_v, a, ws, few, rows_tokens));
+    EET_CUDA(launch_pdl(kern, dim3(sm_count()), dim3(kPgCodesThreads), kSmem, stream, map_q, map_k, map_v, a, ws, few, rows_tokens, whole));
     return 0;
 }
 
 template<int kCodes, int D, int kRows>
-int pc_launch(const PagedMhaArgs& a, void* ws, int few, int beside, cudaStream_t stream)
+int pc_launch(const PagedMhaArgs& a, void* ws, int few, int beside, int whole, cudaStream_t stream)
 {
     auto kern = paged_mha_codes_kernel<kCodes, D, kRows>;
     constexpr int kSmem = PcShape<D, kRows>::kSmem;
@@ -698,7 +699,7 @@ int pc_launch(const PagedMhaArgs& a, void* ws, int few, int beside, cudaStream_t
         EET_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
         attr_set[dev] = true;
     }
-    EET_CUDA(launch_pdl(kern, dim3(PcShape<D, kRows>::kPerSm * sm_count()), dim3(32 * PcShape<D, kRows>::kWarps), kSmem, stream, a, ws, few, beside));
+    EET_CUDA(launch_pdl(kern, dim3(PcShape<D, kRows>::kPerSm * sm_count()), dim3(32 * PcShape<D, kRows>::kWarps), kSmem, stream, a, ws, few, beside, whole));
     return 0;
 }
 
@@ -709,6 +710,7 @@ struct PagedCodesPlan {
     int rows;            // of a tile of the first kind: 8 or 16; 0: none
     bool tiles;
     int few;
+    bool whole[2];       // their tiles are not cut (no scratch, no second launch)
     size_t bytes[2];     // scratch
 };
 
@@ -730,8 +732,19 @@ static PagedCodesPlan paged_codes_plan(const PagedMhaArgs& a)
             p.few = p.rows / group;
         }
     }
-    if (p.rows) p.bytes[0] = pg_scratch_bytes(pc_per_sm(p.rows) * sm_count(), p.rows, a.head_dim);
-    if (p.tiles) p.bytes[1] = pg_scratch_bytes(sm_count(), 2 * kPgRows, a.head_dim);
+    // Cutting tiles evens out the shares and costs a second launch and parts to write, 4 to 10 us.  Not where the longest share of whole tiles is
+    // a few blocks longer, taking tiles to be three quarters as long as the longest on average, as in paged_plan; a block takes 0.7 us with few
+    // rows and an SM for itself, 1.5 us as a tile.
+    auto whole = [&](long long tokens, long long ctas, int most) {
+        const long long keys = a.window > 0 && a.window + tokens < a.max_len ? a.window + tokens : a.max_len;
+        const long long blocks = keys / kPgKeys + 1;
+        const long long tiles = (a.seqs + (a.max_tokens > tokens ? a.tokens / tokens : 0)) * a.kv_heads;
+        return blocks - (tiles < ctas ? 3 * blocks * tiles / (4 * ctas) : 0) <= most;
+    };
+    if (p.rows) p.whole[0] = whole(p.rows / group, pc_per_sm(p.rows) * sm_count(), 5);
+    if (p.tiles) p.whole[1] = whole(2 * (kPgRows / group), sm_count(), 4);
+    if (p.rows && !p.whole[0]) p.bytes[0] = pg_scratch_bytes(pc_per_sm(p.rows) * sm_count(), p.rows, a.head_dim);
+    if (p.tiles && !p.whole[1]) p.bytes[1] = pg_scratch_bytes(sm_count(), 2 * kPgRows, a.head_dim);
     return p;
 }
 
@@ -750,19 +763,21 @@ static int launch_paged_mha_codes_t(const PagedMhaArgs& a, const PagedCodesPlan&
     const bool bias = a.slopes != nullptr || !(a.scale > 0.f);
     if (p.tiles) {
         const int few = both ? p.few : 0, rows_tokens = both ? p.few : 0;
-        if (int rc = bias ? pc_launch_tiles<T, D, true, kCodes>(a, ws[1], few, rows_tokens, stream)
-                          : pc_launch_tiles<T, D, false, kCodes>(a, ws[1], few, rows_tokens, stream)) return rc;
+        if (int rc = bias ? pc_launch_tiles<T, D, true, kCodes>(a, ws[1], few, rows_tokens, p.whole[1], stream)
+                          : pc_launch_tiles<T, D, false, kCodes>(a, ws[1], few, rows_tokens, p.whole[1], stream)) return rc;
     }
     if (p.rows) {
         const int few = both ? p.few : 0x7fffffff, beside = !both ? 0 : bias ? 2 : 1;
-        if (int rc = p.rows == 8 ? pc_launch<kCodes, D, 8>(a, ws[0], few, beside, stream) : pc_launch<kCodes, D, 16>(a, ws[0], few, beside, stream)) return rc;
+        if (int rc = p.rows == 8 ? pc_launch<kCodes, D, 8>(a, ws[0], few, beside, p.whole[0], stream)
+                                 : pc_launch<kCodes, D, 16>(a, ws[0], few, beside, p.whole[0], stream)) return rc;
     }
     // One launch adds up the parts of either kind.  (Its grid is that of the larger number of CTAs; the scratch of each kind knows its own.)
     PgScratch s[2] = {};
     int n = 0;
-    if (p.rows) s[n++] = {ws[0], p.rows, 0, pc_per_sm(p.rows) * sm_count()};
-    if (p.tiles) s[n++] = {ws[1], 2 * kPgRows, 1, sm_count()};
-    const long long rows = (long long)a.max_tokens * (a.heads / a.kv_heads), most = p.tiles ? 2 * kPgRows : p.rows;
+    if (p.bytes[0]) s[n++] = {ws[0], p.rows, 0, pc_per_sm(p.rows) * sm_count()};
+    if (p.bytes[1]) s[n++] = {ws[1], 2 * kPgRows, 1, sm_count()};
+    if (n == 0) return 0;
+    const long long rows = (long long)a.max_tokens * (a.heads / a.kv_heads), most = p.bytes[1] ? 2 * kPgRows : p.rows;
     const int y = (int)((rows < most ? rows : most) * (D / 8) + kPgJoinThreads - 1) / kPgJoinThreads;   // 8 dims a thread
     const int ctas = s[0].ctas > s[1].ctas ? s[0].ctas : s[1].ctas;
     EET_CUDA(launch_pdl(paged_mha_join_kernel<T, D>, dim3(ctas, y, n), dim3(kPgJoinThreads), 0, stream, a, s[0], s[1]));

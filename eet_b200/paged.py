@@ -169,11 +169,13 @@ def _scales(who, k_cache, k_scale, v_scale, shape, index):
     """What the entry points for codes take behind the arguments of the others."""
     if k_scale is None or v_scale is None:
         raise RuntimeError(f"{who}: a cache of codes has both k_scale and v_scale")
-    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-        if t.shape != shape[:3] or t.dtype != torch.float32 or t.get_device() != index or t.stride(2) != 1:
-            raise RuntimeError(f"{who}: {name} must be a float32 tensor {tuple(shape[:3])} with contiguous slots on cuda:{index}, got "
-                               f"{tuple(t.shape)} {t.dtype} with strides {t.stride()} on {t.device}")
-    return _pack_codes(k_scale.data_ptr(), v_scale.data_ptr(), _CODES[k_cache.dtype], *k_scale.stride()[:2], *v_scale.stride()[:2])
+    rows = shape[:3]
+    ks, vs = k_scale.stride(), v_scale.stride()
+    for name, t, strides in (("k_scale", k_scale, ks), ("v_scale", v_scale, vs)):
+        if t.shape != rows or t.dtype != torch.float32 or t.get_device() != index or strides[2] != 1:
+            raise RuntimeError(f"{who}: {name} must be a float32 tensor {tuple(rows)} with contiguous slots on cuda:{index}, got "
+                               f"{tuple(t.shape)} {t.dtype} with strides {strides} on {t.device}")
+    return _pack_codes(k_scale.data_ptr(), v_scale.data_ptr(), _CODES[k_cache.dtype], ks[0], ks[1], vs[0], vs[1])
 
 
 def _kept_type(who, k_cache, dtype, k_scale, v_scale):
@@ -299,28 +301,32 @@ def paged_load(k_cache, v_cache, pages, starts, lens, tokens=None, dtype=None, k
         raise RuntimeError(f"{who}: scales belong to a cache of codes, int8 or float8_e4m3fn, not to {kept}")
     else:
         scales = _pack_codes(0, 0, 0, 0, 0, 0, 0)
+    given = v_out if k_out is None else k_out
     if dtype is None:
-        dtype = next((t.dtype for t in (k_out, v_out) if t is not None), torch.float16 if codes else kept)
+        dtype = given.dtype if given is not None else torch.float16 if codes else kept
     if dtype not in _DTYPES or (not codes and dtype != kept):
         raise RuntimeError(f"{who}: a cache of {kept} is not read back as {dtype}")
     if tokens is None:
-        given = next((t for t in (k_out, v_out) if t is not None), None)
         if given is None:
             raise RuntimeError(f"{who}: neither tokens nor k_out is given")
         tokens = given.shape[0]
-    rows = torch.Size((tokens, shape[1], shape[3]))
-    outs, out_strides = [], ()
-    for name, t in (("k_out", k_out), ("v_out", v_out)):
-        if t is None:
-            t = torch.empty(rows, dtype=dtype, device=k_cache.device)
-        out_strides += _heads(who, name, t, rows, dtype, index)
-        outs.append(t)
+    kv_heads, head_dim = shape[1], shape[3]
+    dense = (kv_heads * head_dim, head_dim)
+    rows = None if given is None else torch.Size((tokens, kv_heads, head_dim))
+    if k_out is None:
+        k_out, k_str = torch.empty((tokens, kv_heads, head_dim), dtype=dtype, device=k_cache.device), dense
+    else:
+        k_str = _heads(who, "k_out", k_out, rows, dtype, index)
+    if v_out is None:
+        v_out, v_str = torch.empty_like(k_out) if k_str == dense else torch.empty((tokens, kv_heads, head_dim), dtype=dtype, device=k_cache.device), dense
+    else:
+        v_str = _heads(who, "v_out", v_out, rows, dtype, index)
     seqs, columns, pages_stride, table = _table(who, pages, starts, lens, index)
-    args = _pack_load(k_cache.data_ptr(), v_cache.data_ptr(), 0 if not codes else k_scale.data_ptr(), 0 if not codes else v_scale.data_ptr(),
-                      outs[0].data_ptr(), outs[1].data_ptr(), *table, tokens, seqs, shape[1], shape[3], codes, dtype == torch.bfloat16,
-                      shape[0], shape[2], columns, pages_stride, *out_strides, *strides) + scales[24:]
+    args = _pack_load(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr() if codes else 0, v_scale.data_ptr() if codes else 0,
+                      k_out.data_ptr(), v_out.data_ptr(), *table, tokens, seqs, kv_heads, head_dim, codes, dtype == torch.bfloat16, shape[0],
+                      shape[2], columns, pages_stride, *k_str, *v_str, *strides) + scales[24:]
     _call(lib.eet_paged_load, args, index)
-    return outs[0], outs[1]
+    return k_out, v_out
 
 
 def paged_mha(q, k_cache, v_cache, pages, starts, lens, max_tokens=None, max_len=None, scale=None, window=0, first_key=None,
