@@ -12,8 +12,8 @@ modeling_baichuan.py import for ``data_type=torch.int8``.  The fp16/fp32 ops of 
 (GatedFeedForwardNetwork, Embedding, the BERT/GPT-2/T5 ops) are not part of this path.
 
 Additions that the reference does not have, all optional: `tp` (a tensor-parallel handle, see
-eet_b200.tp) on MetaDesc, and device-resident step counters so that a decode step can be replayed as a
-CUDA graph (eet_b200.modeling).
+eet_b200.tp) on MetaDesc, device-resident step counters so that a decode step can be replayed as a
+CUDA graph (eet_b200.modeling), and `sample_rows`, the choice of the next token as one kernel.
 """
 import ctypes
 import functools
@@ -27,7 +27,7 @@ from ._lib import EETError, check, lib
 
 __all__ = ["MetaDesc", "LlamaMmha", "BaichuanMmha", "GatedFeedForwardNetworkInt8", "LayerNorm", "quant_weights",
            "preprocess_weights", "unpack_weights", "repack_reference_weights", "gemm_w8a16", "gemm_w8a16_accum",
-           "deferred_epilogue", "check_device_status", "EETError"]
+           "sample_rows", "deferred_epilogue", "check_device_status", "EETError"]
 
 
 # The raw handle of the current device's current stream, without building a Stream object around it (0.2 us instead of

@@ -726,9 +726,9 @@ static PagedCodesPlan paged_codes_plan(const PagedMhaArgs& a)
     }
     else if (group <= 16) {
         // few tokens each beside the longest, and something to read for them?
-        const long long others = a.seqs - 1, rest = a.tokens - a.max_tokens;
-        if (others > 0 && is_few((rest + others - 1) / others) && others * a.kv_heads * (a.max_len / kPgKeys + 1) >= 1024) {
-            p.rows = (rest + others - 1) / others * group <= 8 ? 8 : 16;
+        const long long others = a.seqs - 1, rest = a.tokens - a.max_tokens, each = others > 0 && rest > others ? (rest + others - 1) / others : 1;
+        if (others > 0 && is_few(each) && others * a.kv_heads * (a.max_len / kPgKeys + 1) >= 1024) {
+            p.rows = each * group <= 8 ? 8 : 16;
             p.few = p.rows / group;
         }
     }

@@ -383,6 +383,11 @@ class _LmHead:
             local = torch.cat([p[:, : hi - lo] for p, (lo, hi) in zip(parts, ranges)], 1)
         return local.view(*hidden.shape[:-1], self.vocab)
 
+    def sample(self, hidden2d, uniform, **settings):
+        """Next token ids [B, 1] (int64) for hidden2d [B, hidden], drawn from the logits with the given random numbers [B]
+        and EET.sample_rows's temperature, top_k, top_p and min_p."""
+        return EET.sample_rows(self(hidden2d.contiguous()), uniform, **settings)[0].view(-1, 1)
+
     def greedy(self, hidden2d):
         """Next token ids [B, 1] (int64) for hidden2d [B, hidden]: argmax of the fp16 logits, the smallest index on
         ties, identical on every rank."""
@@ -417,6 +422,7 @@ class _CausalLMBase:
         self.main_input_name = "input_ids"
         self.use_cuda_graph = False
         self._graph = None
+        self._sampling = None      # how tokens are drawn, while generate() does so: EET.sample_rows's arguments behind the logits
 
     @classmethod
     def from_eet(cls, model_dict, config, max_batch, max_prompt_seq_len, max_full_seq_len, data_type=torch.int8,
@@ -473,7 +479,11 @@ class _CausalLMBase:
         # inside the kernel that consumes it
         with EET.deferred_epilogue():
             hidden = self.model(input_ids=ids, first_pass=False)
-        return self.lm_head.greedy(hidden[:, -1, :])
+        return self._choose(hidden[:, -1, :])
+
+    def _choose(self, hidden2d):
+        """Next token ids [B, 1], the largest logits' or drawn."""
+        return self.lm_head.greedy(hidden2d) if self._sampling is None else self.lm_head.sample(hidden2d, **self._sampling)
 
     def decode_logits(self, ids):
         """Logits [B, 1, vocab] of one decode step for ids [B, 1], computed by the same chain of kernels that
@@ -543,22 +553,45 @@ class _CausalLMBase:
         self._warmed = False
 
     @torch.no_grad()
-    def generate(self, input_ids, max_new_tokens, attention_mask=None):
+    def generate(self, input_ids, max_new_tokens, attention_mask=None, do_sample=False, temperature=1.0, top_k=0, top_p=1.0,
+                 min_p=0.0, generator=None):
         """Greedy search in the shape of GenerationMixin_EET.greedy_search
         (python/eet/pipelines/generation.py:1080-1243): one first_pass=True call over the prompt, then one
-        token per call; no EOS stop.  Returns [B, prompt + max_new_tokens] ids."""
+        token per call; no EOS stop.  Returns [B, prompt + max_new_tokens] ids.
+
+        do_sample: tokens are drawn instead, under the settings of EET.sample_rows (numbers, or a tensor of one for each
+        sequence on the device), with random numbers from `generator`, a torch.Generator of the model's device, or that
+        device's own.  Without tensor parallelism."""
+        if not do_sample:
+            return self._generate(input_ids, max_new_tokens, attention_mask, None)
+        tp = self.model.desc.tp
+        if tp is not None and tp.size > 1:
+            raise RuntimeError("generate: drawing tokens is not supported with tensor parallelism")
+        B, dev = input_ids.shape[0], self.model.desc.device
+        uniform = torch.rand((max(1, max_new_tokens), B), generator=generator, dtype=torch.float32, device=dev)
+        # (a captured step reads its numbers from one place; settings of the caller's own stay where they are)
+        self._sampling = dict(uniform=uniform[0].clone(), temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        try:
+            return self._generate(input_ids, max_new_tokens, attention_mask, uniform)
+        finally:
+            self._sampling = None
+            self.end_graph()       # a captured step draws: the next call's may not
+
+    def _generate(self, input_ids, max_new_tokens, attention_mask, uniform):
         self.end_graph()
         if attention_mask is not None and self.use_cuda_graph:
             self.model.pre_padding_len = torch.sum(1 - attention_mask, 1, True).to(self.model.desc.device).long()
         # only the last position's logits are needed to choose the first new token: the lm_head runs on that
         # row alone (the reference computes and discards the logits of every prompt position, modeling_llama.py:471)
         hidden = self.model(input_ids=input_ids, first_pass=True, attention_mask=attention_mask)
-        nxt = self.lm_head.greedy(hidden[:, -1, :].contiguous()).clone()
+        nxt = self._choose(hidden[:, -1, :].contiguous()).clone()
         toks = [input_ids, nxt]
-        for _ in range(max_new_tokens - 1):
+        for t in range(1, max_new_tokens):
+            if uniform is not None:
+                self._sampling["uniform"].copy_(uniform[t])
             if attention_mask is not None and not self.use_cuda_graph:
                 hidden = self.model(input_ids=nxt, first_pass=False, attention_mask=attention_mask)
-                nxt = self.lm_head.greedy(hidden[:, -1, :]).clone()
+                nxt = self._choose(hidden[:, -1, :]).clone()
             else:
                 nxt = self.decode_step(nxt).clone()
             toks.append(nxt)

@@ -279,3 +279,244 @@ def test_mha_is_the_same_whatever_the_hints():
     ref, tol = attend_codes64(batch)
     for r in runs:
         _within(r, ref, tol)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# refusals, pages outside the cache, streams, graphs
+# ---------------------------------------------------------------------------------------------------------------------
+def test_refuses():
+    paged = _paged()
+    batch = CodesBatch([1, 2], [20, 40], 4, 2)
+    kc, vc, *table = batch.gpu()
+    scales = batch.scales()
+    q, k, v = batch.q.cuda(), batch.k.cuda(), batch.v.cuda()
+    ks, vs = scales["k_scale"], scales["v_scale"]
+    for bad in (dict(k_scale=ks), dict(v_scale=vs), dict(k_scale=ks.half(), v_scale=vs), dict(k_scale=ks[1:], v_scale=vs),
+                dict(k_scale=ks.cpu(), v_scale=vs), dict(k_scale=ks, v_scale=vs.transpose(1, 2).contiguous().transpose(1, 2)),
+                dict(k_scale=ks[..., 0], v_scale=vs[..., 0])):
+        with pytest.raises(RuntimeError):
+            paged.paged_mha(q, kc, vc, *table, **bad)
+        with pytest.raises(RuntimeError):
+            paged.paged_store(k, v, kc, vc, *table, **bad)
+        with pytest.raises(RuntimeError):
+            paged.paged_load(kc, vc, *table, 3, **bad)
+    for call in (lambda **s: paged.paged_mha(q, kc, vc, *table, **s), lambda **s: paged.paged_store(k, v, kc, vc, *table, **s),
+                 lambda **s: paged.paged_load(kc, vc, *table, 3, **s)):
+        with pytest.raises(RuntimeError):
+            call()                                                              # codes without scales
+    with pytest.raises(RuntimeError, match="scales belong"):
+        paged.paged_mha(q, kc.half(), vc.half(), *table, **scales)             # scales without codes
+    with pytest.raises(RuntimeError, match="scales belong"):
+        paged.paged_load(kc.half(), vc.half(), *table, 3, **scales)
+    with pytest.raises(RuntimeError):
+        paged.paged_mha(q, kc, vc.view(E4M3), *table, **scales)                # two kinds of codes
+    with pytest.raises(RuntimeError):
+        paged.paged_load(kc, vc, *table, **scales)                             # how many rows?
+    with pytest.raises(RuntimeError, match="read back as"):
+        paged.paged_load(kc, vc, *table, 3, dtype=torch.float32, **scales)
+    with pytest.raises(RuntimeError):
+        paged.paged_load(kc, vc, *table, k_out=k, v_out=v[1:], **scales)
+    wide = torch.zeros(kc.shape[0], 2, 16, 136, dtype=INT8, device="cuda")[..., :128]   # rows 136 bytes apart
+    with pytest.raises(RuntimeError, match="multiples of 16"):
+        paged.paged_mha(q, wide, wide, *table, **scales)
+
+
+@pytest.mark.parametrize("new,most", [([1, 2], 2), ([30, 1], 30)])
+@pytest.mark.parametrize("kind", CODES)
+def test_mha_over_missing_pages(new, most, kind):
+    """Keys of a page outside the cache count as zeros, and the status says so."""
+    batch = CodesBatch(new, [70, 45], 4, 2, 128, 16, FP16, kind)
+    batch.pages[0, 1] = 10 ** 6
+    batch.pages[1, 0] = -7
+    got = _paged().paged_mha(batch.q.cuda(), *batch.gpu(), max_tokens=most, **batch.scales())
+    assert _status() == 6
+    spare = batch.unused[0]
+    for cache, scale in ((batch.k_cache, batch.k_scale), (batch.v_cache, batch.v_scale)):
+        cache.view(torch.uint8)[spare] = 0
+        scale[spare] = 1.0
+    batch.pages[0, 1] = batch.pages[1, 0] = spare
+    ref, tol = attend_codes64(batch, read_back=most > 8)
+    _within(got, ref, tol)
+
+
+def test_mha_of_strided_caches():
+    """[page][slot][head][dim] codes and scales that are views of larger tensors."""
+    batch = CodesBatch([1, 20, 1], [300, 50, 77], 8, 4, 64, 32, BF16, INT8)
+    total = batch.k_cache.shape[0]
+    kc, vc = (c.transpose(1, 2).contiguous().cuda().transpose(1, 2) for c in (batch.k_cache, batch.v_cache))
+    both = torch.stack((batch.k_scale, batch.v_scale), 1).cuda()               # [page][k, v][head][slot]
+    for most in (1, 20):
+        got = _paged().paged_mha(batch.q.cuda(), kc, vc, *(t.cuda() for t in (batch.pages, batch.starts, batch.lens)), max_tokens=most,
+                                 k_scale=both[:, 0], v_scale=both[:, 1])
+        ref, tol = attend_codes64(batch, read_back=True)
+        _within(got, ref, tol)
+    k, v = _paged().paged_load(kc, vc, *(t.cuda() for t in (batch.pages, batch.starts, batch.lens)), 22, dtype=BF16, k_scale=both[:, 0],
+                               v_scale=both[:, 1])
+    assert total and torch.equal(k, _paged().paged_load(*batch.gpu(), 22, dtype=BF16, **batch.scales())[0])
+
+
+def test_empty_calls():
+    batch = CodesBatch([1], [20], 4, 2)
+    kc, vc, pages, starts, lens = batch.gpu()
+    scales = batch.scales()
+    none = torch.zeros(1, dtype=torch.int32, device="cuda")
+    assert _paged().paged_mha(batch.q[:0].cuda(), kc, vc, pages[:0], none, lens[:0], **scales).shape == (0, 4, 128)
+    assert _paged().paged_load(kc, vc, pages[:0], none, lens[:0], 0, **scales)[0].shape == (0, 2, 128)
+    zero = CodesBatch([0, 0], [0, 5], 4, 2)
+    for most in (1, 40):
+        out = torch.full((3, 4, 128), 7.0, dtype=FP16, device="cuda")
+        _paged().paged_mha(out, *zero.gpu(), out=out, max_tokens=most, **zero.scales())
+        assert (out == 7.0).all()
+
+
+@pytest.mark.parametrize("kind", CODES)
+@pytest.mark.parametrize("new,most", [([1] * 6, 1), ([3, 1, 2, 1, 1, 2], 3), ([90, 1, 1, 1, 1, 1], 90)])
+def test_a_captured_call_serves_other_lengths(kind, new, most):
+    lens = [200, 7, 3000, 90, 1, 1000]
+    batch = CodesBatch(new, [max(a, b) for a, b in zip(lens, new)], 8, 2, 128, 16, FP16, kind)
+    cache, scales, q = batch.gpu(), batch.scales(), batch.q.cuda()
+    run = lambda: _paged().paged_mha(q, *cache, max_tokens=most, max_len=3000, **scales)  # noqa: E731
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for other in (batch.lens_list, [max(n, x // 2) for n, x in zip(new, batch.lens_list)], list(new)):
+        batch.lens_list = list(other)
+        cache[4].copy_(torch.tensor(other, dtype=torch.int32))
+        out.fill_(9.0)
+        graph.replay()
+        ref, tol = attend_codes64(batch, read_back=True)
+        _within(out, ref, tol, str(other))
+    assert _status() == 0
+
+
+def test_calls_behind_one_another_without_a_pause():
+    """Append and attention in turn, in place, many times over and captured: what one writes the next one reads, and the programmatic launches
+    may overlap only as far as that allows."""
+    paged = _paged()
+    for new, most in (([1] * 5, 1), ([100, 1, 1, 1, 1], 100), ([2, 3, 1, 0, 4], 4)):
+        batch = CodesBatch(new, [700 + 3 * n for n in new], 8, 2, 128, 16, FP16, INT8)
+        freqs = paged.rotary_frequencies(128)[0]
+        q, k, v = (t.cuda() for t in (batch.q, batch.k, batch.v))
+
+        def steps(cache, scales, pause):
+            out, x = [], q
+            for i in range(12):
+                turned = paged.paged_store((k * (1 + i)).half(), (v - i).half(), *cache, q=x, freqs=freqs, **scales)
+                if pause:
+                    torch.cuda.synchronize()
+                x = paged.paged_mha(turned, *cache, max_tokens=most, **scales) * 3
+                if pause:
+                    torch.cuda.synchronize()
+                out.append(x)
+            return torch.stack(out)
+
+        want = steps(batch.gpu(), batch.scales(), True)
+        cache, scales = batch.gpu(), batch.scales()
+        assert torch.equal(steps(cache, scales, False), want)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = steps(cache, scales, False)
+        for t, s in zip(cache, batch.gpu()):
+            t.copy_(s)
+        for _ in range(3):
+            graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+    assert _status() == 0
+
+
+def test_two_streams_at_once():
+    batches = [CodesBatch(new, lens, 8, 2, seed=i) for i, (new, lens) in enumerate((([1] * 9, [900] * 9), ([120, 1], [500, 3000])))]
+    inputs = [(b.q.cuda(), b.gpu(), b.scales()) for b in batches]
+    most = [1, 120]
+    want = [_paged().paged_mha(q, *c, max_tokens=m, **s) for (q, c, s), m in zip(inputs, most)]
+    streams = [torch.cuda.Stream() for _ in batches]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                q, c, s = inputs[i]
+                got[i].append(_paged().paged_mha(q, *c, max_tokens=most[i], **s))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, want[i]) for x in got[i])
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# serving: prompt and decode steps of the block, to the next token
+# ---------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind", CODES)
+@pytest.mark.parametrize("kv_heads", [2, 1])
+def test_serving_to_the_next_token(kind, kv_heads):
+    """PagedMmha over a cache of codes is its parts called by hand, for a prompt of chunks and steps of single tokens behind it; a captured step
+    draws the tokens that the calls by hand draw."""
+    from eet_b200 import EET
+    paged, heads, hidden, page = _paged(), 2, 256, 16
+    gen = torch.Generator().manual_seed(3)
+    desc = EET.MetaDesc(FP16, 4, heads, hidden, 1, 64, 128, "silu", 128, 512, "cuda:0", False, 1e-6, True)
+    make = lambda k, n: EET.quant_weights((torch.randn(k, n, generator=gen) * 0.05).half().cuda(), torch.int8, False)  # noqa: E731
+    qkv_w, qkv_s = make(hidden, 128 * (heads + 2 * kv_heads))[-2:]
+    out_w, out_s = make(128 * heads, hidden)[-2:]
+    qkv_s, out_s = qkv_s.half(), out_s.half()
+    norm = torch.ones(hidden, dtype=FP16, device="cuda")
+    head = (torch.randn(hidden, 1000, generator=gen) * 0.3).half().cuda()
+    block = paged.PagedMmha(desc, qkv_w, qkv_s, out_w, out_s, norm, kv_head_num=kv_heads)
+    freqs, _ = paged.rotary_frequencies(128)
+
+    def cache():
+        codes = [torch.zeros(24, kv_heads, page, 128, dtype=kind, device="cuda") for _ in "kv"]
+        return codes, dict(k_scale=torch.zeros(24, kv_heads, page, device="cuda"), v_scale=torch.zeros(24, kv_heads, page, device="cuda"))
+
+    def by_hand(x, codes, scales, table, most):
+        xn = torch.empty_like(x)
+        EET.check(EET.lib.eet_rmsnorm(x.data_ptr(), norm.data_ptr(), xn.data_ptr(), x.shape[0], hidden, 1e-6, EET._stream()))
+        qkv = EET.gemm_w8a16(xn, qkv_w, qkv_s).view(x.shape[0], -1, 128)
+        q, k, v = qkv.split((heads, kv_heads, kv_heads), 1)
+        q = paged.paged_store(k, v, *codes, *table, q=q, freqs=freqs, **scales)
+        ctx = paged.paged_mha(q, *codes, *table, max_tokens=most, **scales)
+        return EET.gemm_w8a16(ctx.view(x.shape[0], -1), out_w, out_s, residual=x)
+
+    pages = torch.randperm(24, generator=gen)[:16].view(2, 8).int().cuda()
+    lens = torch.tensor([20, 33], dtype=torch.int32, device="cuda")
+    starts = torch.tensor([0, 20, 53], dtype=torch.int32, device="cuda")
+    x = torch.randn(53, hidden, generator=gen).half().cuda()
+    mine, other = cache(), cache()
+    got, want = block(x, *mine[0], pages, starts, lens, max_tokens=33, **mine[1]).clone(), by_hand(x, *other, (pages, starts, lens), 33)
+    # (the two go through the same kernels, the projections maybe with sums in another order: fp16 values of a few units)
+    assert torch.allclose(got.float(), want.float(), atol=2e-2, rtol=1e-2)
+    embed = torch.randn(1000, hidden, generator=gen).half().cuda()
+    step = torch.arange(3, dtype=torch.int32, device="cuda")
+    uniform = torch.rand(2, generator=gen).cuda()
+    token = torch.tensor([5, 7], device="cuda")
+
+    def one(token, attend):
+        hidden_states = attend(embed[token])
+        return EET.sample_rows((hidden_states @ head).float(), uniform, temperature=0.8, top_k=100, top_p=0.95)[0]
+
+    def captured(token):
+        return one(token, lambda y: block(y, *mine[0], pages, step, lens, max_tokens=1, max_len=128, **mine[1]))
+
+    def hand(token):
+        return one(token, lambda y: by_hand(y, *other, (pages, step, lens), 1))
+
+    # the same cache for both from here on
+    for a, b in zip((*mine[0], *mine[1].values()), (*other[0], *other[1].values())):
+        b.copy_(a)
+    held = token.clone()
+    lens += 1
+    captured(held)                      # (sizes the pooled buffers; the same rows are appended again below)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        drawn = captured(held)
+    for t in range(6):
+        if t:
+            lens += 1
+        graph.replay()
+        by = hand(held)
+        assert torch.equal(drawn, by), f"step {t}"
+        uniform.copy_((uniform + 0.37) % 1.0)
+        held.copy_(drawn)
+    EET.check_device_status()
