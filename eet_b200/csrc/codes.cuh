@@ -66,7 +66,8 @@ __device__ __forceinline__ void quantize16(const float (&y)[16], float scale, ui
             uint16_t lo, hi;
             asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(z[4 * w + 1]), "f"(z[4 * w]));
             asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(z[4 * w + 3]), "f"(z[4 * w + 2]));
-            codes[w] = (uint32_t)lo | ((uint32_t)hi << 16);
+            // (zeros beside a scale of NaN: a code of NaN would reach rows of a tile that do not see it)
+            codes[w] = scale == scale ? (uint32_t)lo | ((uint32_t)hi << 16) : 0u;
         }
     }
 }

@@ -465,6 +465,10 @@ paged_mha_codes_kernel(const __grid_constant__ PagedMhaArgs a, void* ws, int few
 #pragma unroll
                                 for (int r = 0; r < 2; ++r) asm("min.NaN.f32 %0, %0, %1;" : "+f"(e[r]) : "f"(65504.0f));
                             }
+                            if (masked) {   // (a scale that is not finite, of a value that the row does not see)
+#pragma unroll
+                                for (int r = 0; r < 2; ++r) e[r] = s[m][n][2 * i + r] == -INFINITY ? 0.f : e[r];
+                            }
                             const __half2 h = __floats2half2_rn(e[0], e[1]);
                             w[m][n][i] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h));
                         }
@@ -620,7 +624,7 @@ paged_mha_tc_codes_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
                           const __grid_constant__ CUtensorMap map_v, const __grid_constant__ PagedMhaArgs a, void* ws, int few, int rows_tokens,
                           int whole)
 {
-    static_assert(2 * 144 + 112 + 112 <= 4 * 128, "of what the CTA was launched with");
+    static_assert(2 * 136 + 120 + 120 <= 4 * 128, "of what the CTA was launched with");
     extern __shared__ __align__(1024) uint8_t pg_dyn[];
     __shared__ PgSmem sm;
     __shared__ uint32_t tmem_base;
@@ -632,9 +636,8 @@ paged_mha_tc_codes_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     pc_begin(&tmem_base, kPgTmemCols);
     const int n = gridDim.x, cta = blockIdx.x, ctas = rows_tokens ? pc_split(a, rows_tokens, few, n, kBias).sms_tiles : n;
     const int group = threadIdx.x >> 7;
-    if (group < 2) pg_more_registers<144>();
-    else if (group == 2) pg_fewer_registers<112>();
-    else pg_fewer_registers<112>();
+    if (group < 2) pg_more_registers<136>();
+    else pg_fewer_registers<120>();
     static_assert(sizeof(PgFound) <= sizeof(sm.b_max) + sizeof(sm.b_sum) && alignof(PgFound) <= 8, "lies there for a while");
     if (cta < ctas) {
         pg_tiles<T, D, kBias, kCodes>(&map_q, &map_k, &map_v, a, ws, few + 1, whole, cta, ctas, n, sm, *reinterpret_cast<PgFound*>(sm.b_max), tmem_base,
@@ -646,7 +649,7 @@ paged_mha_tc_codes_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     pg_end(&tmem_base, kPgTmemCols);
 }
 
-// Codes as [page][head][slot][dim] bytes, boxes of a page (of 128 slots of a larger one) and a head.
+// Codes as [page][head][slot][dim] bytes, boxes of a page (of 64 slots of a larger one) and a head.
 template<int D>
 int pg_encode_codes(CUtensorMap* map, const void* base, const PagedMhaArgs& a, long long page_step, long long head_step, long long slot_step)
 {
@@ -655,7 +658,7 @@ int pg_encode_codes(CUtensorMap* map, const void* base, const PagedMhaArgs& a, l
     const int page = 1 << a.page_shift;
     const cuuint64_t dims[4] = {D, (cuuint64_t)page, (cuuint64_t)a.kv_heads, (cuuint64_t)a.num_pages};
     const cuuint64_t strides[3] = {(cuuint64_t)slot_step, (cuuint64_t)head_step, (cuuint64_t)page_step};
-    const cuuint32_t box[4] = {D, (cuuint32_t)(page < kPgKeys ? page : kPgKeys), 1, 1}, elem[4] = {1, 1, 1, 1};
+    const cuuint32_t box[4] = {D, (cuuint32_t)(page < kPgKeys / 2 ? page : kPgKeys / 2), 1, 1}, elem[4] = {1, 1, 1, 1};
     const CUresult rc = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, box, elem,
                                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);

@@ -24,13 +24,14 @@
 // Keys outside of what any row of the pair sees may be anything, even NaN (slots behind the end of a sequence): their scores are
 // masked by selection and their rows of V are set to zero in shared memory before the product reads them.
 //
-// Over a cache of 8-bit codes warp 8 brings codes and scales to two places in shared memory, an entry each, and four more warps (12-15, a
-// warpgroup of their own) put K and V into the ring from there: 32 keys of an entry each, codes times the scale of their row in fp32, rounded
-// once to q's type, written where the copy engine would have put it; the rest of the kernel does not know.  (The scales could stay outside
-// the products as in paged_codes.cu, two multiplications and two reads of shared memory more for every score: the softmax is the bound
-// here.)  What these warps do has to be little code as well as few instructions: five kinds of warps share an instruction cache (512 behind 8192,
-// 32 / 8 heads, bf16: unrolled 187 us, in a loop of 32 codes 130; with the copies among their duties 126).  512 threads of 128 registers are launched, of
-// which the softmax takes 144 and the others 112.
+// Over a cache of 8-bit codes the products take the codes, which are exact in q's type, and the scales stay outside: that of a key on its scores, that
+// of a value on its weight, before that is rounded.  (With code times scale rounded to 16 bits in front of the products the result was off by up to
+// 4.5 times as much as the rounded exact one: scores are sums of 128 rounded keys.)  In fp16 the weights are held under a power of two that
+// follows the largest scale of the values so far.  Warp 8 brings codes to three places in shared memory, half an entry each, and the scales of a
+// block to a ring of six; four more warps (12-15, a warpgroup of their own) turn the codes into 16-bit values where the copy engine would have put
+// K and V.  What these warps do has to be little code as well as few instructions: five kinds of warps share an instruction cache (512 behind
+// 8192, 32 / 8 heads, bf16: unrolled 187 us, in a loop of 32 codes 130; with the copies among their duties 126, without 101).  512 threads of 128
+// registers are launched, of which the softmax takes 136 and the others 120.
 #include <type_traits>
 
 #include "codes.cuh"
@@ -58,7 +59,9 @@ struct PgSmem {
     uint64_t o_full[2];      // the last P.V of a piece has completed
     uint64_t o_free[2];      // O has been read (four warps)
     uint64_t b_ready;        // split: b's maximum and sum are in b_max, b_sum, its O is complete (four warps)
-    uint64_t staged_full[2], staged_empty[2];   // codes: the two places they come to (33 arrivals and the bytes; four warps)
+    uint64_t staged_full[3], staged_empty[3];   // codes: the places they come to (the bytes; four warps)
+    uint64_t scales_full[6];                    // the scales of a block (32 threads' copies)
+    float b_unit;            // split: what b's O is to be multiplied with
     volatile int abort;
     __align__(8) float b_max[kPgRows], b_sum[kPgRows];
     // what a softmax warp needs between its pieces, out of its registers while it works on one
@@ -144,10 +147,11 @@ __device__ __forceinline__ void pg_init(PgSmem& sm, uint32_t writers = 1)
         mbar_init(&sm.o_free[x], 4);
     }
     mbar_init(&sm.b_ready, 4);
-    for (int i = 0; i < 2; ++i) {
-        mbar_init(&sm.staged_full[i], 33);
+    for (int i = 0; i < 3; ++i) {
+        mbar_init(&sm.staged_full[i], 1);
         mbar_init(&sm.staged_empty[i], 4);
     }
+    for (int i = 0; i < 6; ++i) mbar_init(&sm.scales_full[i], 32);
     sm.abort = 0;
     mbar_fence_init();
 }
@@ -159,111 +163,130 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b)
     return d;
 }
 
-// Sixteen codes times their scale as 16-bit values, two to a word, by pairs.  A byte under the exponent of 2^23 is a number in fp32 at once, without
-// a trip through fp16 (60 instructions that way and 44 this way).
+// Four codes as two words of T.  int8 as bf16: a byte under the exponent of 128, where the low seven bits are units, less 128, or 256 where its top bit
+// says that it is negative.
 template<typename T, int kCodes>
-__device__ __forceinline__ void pg_values16(const uint4& x, float scale, uint32_t (&out)[8])
+__device__ __forceinline__ void pg_values4(uint32_t w, uint32_t& lo, uint32_t& hi)
 {
-    const uint32_t words[4] = {x.x, x.y, x.z, x.w};
-    const uint64_t scale2 = pair2(scale, scale);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        uint64_t y[2];
-        if (kCodes == kCodesInt8) {
-            const uint32_t w = words[i] ^ 0x80808080u;
-            const uint64_t less = pair2(-8388736.0f, -8388736.0f);   // 2^23 + 128
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                y[e] = add2(pair2(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7540 | (2 * e))),
-                                  __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7540 | (2 * e + 1)))), less);
-            }
-        }
-        else {
-            uint32_t h[2];
-            codes_to_half<kCodes>(words[i], h[0], h[1]);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[e]));
-                y[e] = pair2(f.x, f.y);
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const float2 f = split2(mul2(y[e], scale2));
-            out[2 * i + e] = PgType<T>::pack(f.x, f.y);
-        }
+    if (std::is_same<T, __half>::value) {
+        codes_to_half<kCodes>(w, lo, hi);
+    }
+    else if (kCodes == kCodesInt8) {
+        const uint32_t a = __byte_perm(w, 0x43434343u, 0x4140), b = __byte_perm(w, 0x43434343u, 0x4342);
+        const uint32_t more[2] = {a & 0xff7fff7fu, b & 0xff7fff7fu}, less[2] = {a & 0xff80ff80u, b & 0xff80ff80u};
+        asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(lo) : "r"(more[0]), "r"(less[0]));
+        asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(hi) : "r"(more[1]), "r"(less[1]));
+    }
+    else {
+        uint32_t h[2];
+        codes_to_half<kCodes>(w, h[0], h[1]);
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[0])), g = __half22float2(*reinterpret_cast<const __half2*>(&h[1]));
+        lo = PgType<T>::pack(f.x, f.y);
+        hi = PgType<T>::pack(g.x, g.y);
     }
 }
 
-// An entry of 128 keys' codes and scales on its way to its place, by a whole warp: a lane per page for the codes, a lane per key for the scales.
-// Scales of keys that the tile does not see, and of pages outside the cache, become zero, and with them the values.
+__device__ __forceinline__ void tmem_ld_wait32(uint32_t* v)
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int c = 0; c < 32; ++c) asm volatile("" : "+r"(v[c]));
+}
+__device__ __forceinline__ void tmem_st32_async(uint32_t taddr, uint32_t* v)
+{
+    tmem_st16_async(taddr, *reinterpret_cast<uint32_t(*)[16]>(v));
+    tmem_st16_async(taddr + 16, *reinterpret_cast<uint32_t(*)[16]>(v + 16));
+}
+
+// Codes and scales on their way to their places, by a whole warp.  Scales of keys that the tile does not see, and of pages outside the cache, become
+// zero.
 template<int D>
 struct PgCodesLoader {
-    static constexpr int kCodeBytes = kPgKeys * D, kEntry = kCodeBytes + kPgKeys * 4;
+    static constexpr int kPlaces = 3, kScales = 6;
+    static constexpr int kPlace = kPgKeys / 2 * D;                         // bytes: half an entry
+    static constexpr int kBytes = kPlaces * kPlace + kScales * 2 * kPgKeys * 4;
     const PagedMhaArgs& a;
     const int* row;      // the sequence's row of the page table
     int head;
     PgSpan span;
 
-    __device__ __forceinline__ int rows() const { return min(1 << a.page_shift, kPgKeys); }
-    // the page of keys rows() lane .. of the block at key0, in the lanes that have one; -1: nobody sees them
+    // the page of the run of 16 keys lane .. of the block at key0, in the first eight lanes, as the table has it; -1: nobody sees them
     __device__ __forceinline__ int page(int key0) const
     {
-        const int key = key0 + (int)(threadIdx.x & 31) * rows();
-        return key < key0 + kPgKeys && key < span.hi && key + rows() > span.lo ? row[key >> a.page_shift] : -1;
+        const int lane = threadIdx.x & 31, key = key0 + 16 * lane;
+        return lane < kPgKeys / 16 && key < span.hi && key + 16 > span.lo ? row[key >> a.page_shift] : -1;
     }
-    __device__ __forceinline__ void load(const CUtensorMap* map, const float* scales, long long scale_page, long long scale_head, int key0,
-                                         int page, uint8_t* place, uint64_t* full) const
+    // half `half` of an entry: a lane a page
+    __device__ __forceinline__ void load(const CUtensorMap* map, int key0, int half, int page, uint8_t* place, uint64_t* full) const
     {
-        static_assert(kPgKeys == 128, "a shift below");
-        const int lane = threadIdx.x & 31, n = rows(), key = key0 + lane * n;
-        const bool mine = key < key0 + kPgKeys && key < span.hi && key + n > span.lo;
+        constexpr int kKeys = kPgKeys / 2;
+        const int lane = threadIdx.x & 31, n = min(1 << a.page_shift, kKeys), at = lane * n, key = key0 + half * kKeys + at;
+        // (the first run of a page may be one that nobody sees: any of its runs knows the page)
+        int of = -1;
+#pragma unroll
+        for (int i = 0; i < kKeys / 16; ++i) {
+            const int other = __shfl_sync(0xffffffffu, page, half * (kKeys / 16) + min(at / 16 + i, kKeys / 16 - 1));
+            if (16 * i < n) of = max(of, other);
+        }
+        const bool mine = at < kKeys && key < span.hi && key + n > span.lo;
         const int count = __popc(__ballot_sync(0xffffffffu, mine));
         if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)(count * n * D));
         __syncwarp();
-        if (mine && (page < 0 || page >= a.num_pages)) {
-            g_device_status = 6;
-            page = a.num_pages;   // behind the last: reads as zeros
+        if (mine) {
+            if (of < 0 || of >= a.num_pages) {
+                g_device_status = 6;
+                of = a.num_pages;   // behind the last: reads as zeros
+            }
+            tma_load_4d(place + at * D, map, 0, key & ((1 << a.page_shift) - 1), head, of, full);
         }
-        if (mine) tma_load_4d(place + lane * n * D, map, 0, key & ((1 << a.page_shift) - 1), head, page, full);
-        const uint32_t to = smem_u32(place + kCodeBytes) + 4 * lane;
-        const float* from = scales + head * scale_head;
+    }
+    // the scales of a block: four keys a lane, k in front of v
+    __device__ __forceinline__ void load_scales(int key0, int page, float* place, uint64_t* full) const
+    {
+        const int lane = threadIdx.x & 31;
+        const float *k = a.k_scale + head * a.ks_head, *v = a.v_scale + head * a.vs_head;
+        const uint32_t to = smem_u32(place + lane);
 #pragma unroll
         for (int i = 0; i < kPgKeys / 32; ++i) {
-            const int k = 32 * i + lane, of = __shfl_sync(0xffffffffu, page, k >> min(a.page_shift, 7)), at = key0 + k;
-            const bool seen = at >= span.lo && at < span.hi && of < a.num_pages;
-            copy4_async(to + 128 * i, from + (seen ? of : 0) * scale_page + (at & ((1 << a.page_shift) - 1)), seen ? 4 : 0);
+            const int of = __shfl_sync(0xffffffffu, page, 2 * i + (lane >> 4)), key = key0 + 32 * i + lane, slot = key & ((1 << a.page_shift) - 1);
+            const uint32_t bytes = key >= span.lo && key < span.hi && of >= 0 && of < a.num_pages ? 4 : 0;
+            copy4_async(to + 128 * i, k + (bytes ? of : 0) * a.ks_page + slot, bytes);
+            copy4_async(to + 128 * i + kPgKeys * 4, v + (bytes ? of : 0) * a.vs_page + slot, bytes);
         }
         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(full)) : "memory");
     }
 };
 
-// 32 keys of an entry into the ring.  Lane (r, c) = (lane / 4, lane % 4) has 16 codes of keys r, r + 8, r + 16 and r + 24 in either half of a row, odd
-// keys the halves in the other order: eight lanes then meet no bank twice, reading or writing.
+// 16 keys of half an entry into the ring, from key0 of it.  Lane (r, c) = (lane / 4, lane % 4) has 16 codes of keys r and r + 8 in either half of a row, odd
+// keys the halves in the other order: eight lanes then meet no bank twice, reading or writing.  scales: of the block's values, where rows
+// are to be zero that nobody sees, and those whose scale is not finite: what is there may be NaN, and nothing times that is NaN.
 template<typename T, int D, int kCodes>
-__device__ __forceinline__ void pg_convert(const uint8_t* place, int key0, uint8_t* stage)
+__device__ __forceinline__ void pg_convert(const uint8_t* place, int key0, const float* scales, uint8_t* stage, int stage_key)
 {
     constexpr int kHalves = D / 64, kHalf = kPgRows * 128;
     const int lane = threadIdx.x & 31, c = 2 * (lane & 3);
-    const uint32_t codes = smem_u32(place) + 16 * (lane & 3), scales = smem_u32(place) + kPgKeys * D;
+    const uint32_t codes = smem_u32(place) + 16 * (lane & 3);
 #pragma unroll 1
-    for (int key = key0 + (lane >> 2); key < key0 + 32; key += 8) {
-        float scale;
-        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(scale) : "r"(scales + 4 * key));
+    for (int i = 0; i < 16; i += 8) {
+        const int from = key0 + i + (lane >> 2), key = stage_key + i + (lane >> 2);
         uint4 x[kHalves];
 #pragma unroll
-        for (int h = 0; h < kHalves; ++h) x[h] = lds128(codes + (uint32_t)(key * D + 64 * (kHalves == 2 ? h ^ (key & 1) : 0)));
-        if (kCodes == kCodesE4M3 && __any_sync(0xffffffffu, scale == 0.f)) {   // (what nobody sees may be NaN, and nothing times that is NaN)
+        for (int h = 0; h < kHalves; ++h) x[h] = lds128(codes + (uint32_t)(from * D + 64 * (kHalves == 2 ? h ^ (key & 1) : 0)));
+        if (kCodes == kCodesE4M3 && scales != nullptr) {
+            const bool none = (__float_as_uint(scales[key]) & 0x7fffffffu) - 1u >= 0x7f7fffffu;
 #pragma unroll
-            for (int h = 0; h < kHalves; ++h) x[h] = scale == 0.f ? make_uint4(0u, 0u, 0u, 0u) : x[h];
+            for (int h = 0; h < kHalves; ++h) x[h] = none ? make_uint4(0u, 0u, 0u, 0u) : x[h];
         }
 #pragma unroll
         for (int h = 0; h < kHalves; ++h) {
-            uint32_t y[8];
-            pg_values16<T, kCodes>(x[h], scale, y);
+            uint4 y[2];
+            pg_values4<T, kCodes>(x[h].x, y[0].x, y[0].y);
+            pg_values4<T, kCodes>(x[h].y, y[0].z, y[0].w);
+            pg_values4<T, kCodes>(x[h].z, y[1].x, y[1].y);
+            pg_values4<T, kCodes>(x[h].w, y[1].z, y[1].w);
             uint8_t* dst = stage + (kHalves == 2 ? h ^ (key & 1) : 0) * kHalf + key * 128;
-            *reinterpret_cast<uint4*>(dst + ((c ^ (key & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
-            *reinterpret_cast<uint4*>(dst + (((c + 1) ^ (key & 7)) << 4)) = make_uint4(y[4], y[5], y[6], y[7]);
+            *reinterpret_cast<uint4*>(dst + ((c ^ (key & 7)) << 4)) = y[0];
+            *reinterpret_cast<uint4*>(dst + (((c + 1) ^ (key & 7)) << 4)) = y[1];
         }
     }
 }
@@ -299,7 +322,7 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
     else if (warp == 8) {
         // ------------------------------------------------------------------ producer
         const long long cap = (long long)a.max_pages << a.page_shift;
-        int stage = 0, issued = 0, pieces = 0;
+        int stage = 0, issued = 0, pieces = 0, scaled = 0;
         uint32_t phase = 1;                                       // of `empty`: the first round finds the stages free
         bool ok = true;
         const PgShare all = share;
@@ -323,16 +346,25 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
                 using Loader = PgCodesLoader<D>;
                 const Loader loader = {a, a.pages + p.seq * a.pages_stride, p.head, span};
                 uint8_t* places = ring + kRing * kTile;
+                float* scales = reinterpret_cast<float*>(places + Loader::kPlaces * Loader::kPlace);
                 const int n = p.blocks, key_top = p.top * kPgKeys;
                 int next = loader.page(key_top), last = -1, older = -1;   // pages of the next K, of the last one and of that before
                 for (int e = 0; e < 2 * n && ok; ++e) {                   // K0 K1 V0 K2 V1 ..
                     const bool end = e == 2 * n - 1, v = end || (e > 0 && e % 2 == 0);
-                    const int j = end ? n - 1 : v ? e / 2 - 1 : (e + 1) / 2, x = issued & 1;
-                    ok = tc_wait_warp(&sm.staged_empty[x], (uint32_t)(((issued >> 1) + 1) & 1), &sm.abort);
-                    if (!ok) break;
-                    loader.load(v ? map_v : map_k, v ? a.v_scale : a.k_scale, v ? a.vs_page : a.ks_page, v ? a.vs_head : a.ks_head,
-                                key_top - j * kPgKeys, !v ? next : end ? last : older, places + x * Loader::kEntry, &sm.staged_full[x]);
-                    ++issued;
+                    const int j = end ? n - 1 : v ? e / 2 - 1 : (e + 1) / 2, page = !v ? next : end ? last : older;
+                    for (int half = 0; half < 2 && ok; ++half) {
+                        const int x = issued % Loader::kPlaces;
+                        ok = tc_wait_warp(&sm.staged_empty[x], (uint32_t)((issued / Loader::kPlaces + 1) & 1), &sm.abort);
+                        if (!ok) break;
+                        // (the softmax has done with the scales of six blocks before: their K has left the ring three blocks ago, behind
+                        // products that wait for its weights)
+                        if (!v && half == 0) {
+                            const int slot = scaled++ % Loader::kScales;
+                            loader.load_scales(key_top - j * kPgKeys, page, scales + slot * 2 * kPgKeys, &sm.scales_full[slot]);
+                        }
+                        loader.load(v ? map_v : map_k, key_top - j * kPgKeys, half, page, places + x * Loader::kPlace, &sm.staged_full[x]);
+                        ++issued;
+                    }
                     if (!v) {
                         older = last;
                         last = next;
@@ -366,7 +398,7 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
             // (nor may copies by this warp's threads be on their way)
             asm volatile("cp.async.wait_all;" ::: "memory");
             if (sm.abort) {
-                for (int e = max(0, issued - 2); e < issued; ++e) mbar_wait_bounded(&sm.staged_full[e & 1], (uint32_t)((e >> 1) & 1));
+                for (int e = max(0, issued - 3); e < issued; ++e) mbar_wait_bounded(&sm.staged_full[e % 3], (uint32_t)((e / 3) & 1));
                 if (pieces > 0) mbar_wait_bounded(&sm.q_full, (uint32_t)((pieces - 1) & 1));
             }
         }
@@ -480,26 +512,38 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
         // ------------------------------------------------------------------ codes into the ring
         using Loader = PgCodesLoader<D>;
         const uint8_t* places = ring + kRing * kTile;
-        int stage = 0, done = 0;
+        const float* scales = reinterpret_cast<const float*>(places + Loader::kPlaces * Loader::kPlace);
+        int stage = 0, done = 0, before = 0;                      // before: blocks of the pieces before
         uint32_t phase = 1;                                       // of `empty`: the first round finds the stages free
         bool ok = true;
         while (ok && share.next(a, tiling, p)) {
-            for (int e = 0; e < 2 * p.blocks; ++e, ++done) {
-                const int x = done & 1;
-                ok = tc_wait_warp(&sm.staged_full[x], (uint32_t)((done >> 1) & 1), &sm.abort) && tc_wait_warp(&sm.empty[stage], phase, &sm.abort);
+            const int n = p.blocks;
+            for (int e = 0; e < 2 * n && ok; ++e) {
+                ok = tc_wait_warp(&sm.empty[stage], phase, &sm.abort);
+                const bool end = e == 2 * n - 1, v = end || (e > 0 && e % 2 == 0);
+                const int block = before + (end ? n - 1 : e / 2 - 1);   // (of V)
+                // (rows that nobody sees: at the ends of what the tile reads, and of pages outside the cache; K's scores are masked)
+                const float* of = kCodes == kCodesE4M3 && v ? scales + (block % Loader::kScales * 2 + 1) * kPgKeys : nullptr;
+                if (of != nullptr && ok) ok = tc_wait_warp(&sm.scales_full[block % Loader::kScales], (uint32_t)((block / Loader::kScales) & 1), &sm.abort);
+#pragma unroll 1
+                for (int half = 0; half < 2 && ok; ++half, ++done) {
+                    const int x = done % Loader::kPlaces, at = 16 * (warp - 12);
+                    ok = tc_wait_warp(&sm.staged_full[x], (uint32_t)((done / Loader::kPlaces) & 1), &sm.abort);
+                    if (!ok) break;
+                    pg_convert<T, D, kCodes ? kCodes : kCodesInt8>(places + x * Loader::kPlace, at, of, ring + stage * kTile, kPgKeys / 2 * half + at);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sm.staged_empty[x]);
+                }
                 if (!ok) break;
-                pg_convert<T, D, kCodes ? kCodes : kCodesInt8>(places + x * Loader::kEntry, 32 * (warp - 12), ring + stage * kTile);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(&sm.full[stage]);
-                    mbar_arrive(&sm.staged_empty[x]);
-                }
+                if (lane == 0) mbar_arrive(&sm.full[stage]);
                 if (++stage == kRing) {
                     stage = 0;
                     phase ^= 1;
                 }
             }
+            before += n;
         }
     }
     else if (warp < 8) {
@@ -548,8 +592,32 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
             const uint64_t rise[2] = {pair2(0.f, slope), pair2(2.f * slope, 3.f * slope)};   // of the bias over four keys
             float m_run = kPgNone, l_run = 0.f;
             PgReference ref = {1.0f, -kPgNone};   // (-inf stays -inf, and any score moves it)
+            // Codes in fp16: O is held under 2^unit, no less than the largest scale of the values so far, so that weights times scales stay below 2^15.
+            constexpr bool kUnit = kCodes != 0 && std::is_same<T, __half>::value;
+            int unit = -126;
             for (int j = turns.first; j < turns.end && ok; j += turns.stride) {
                 const int key0 = (top - j) * kPgKeys;
+                const float *k_scales = nullptr, *v_scales = nullptr;
+                float less = 1.0f;             // a power of two: of O under the unit before
+                if (kCodes) {
+                    const int block = entry0 / 2 + j, slot = block % PgCodesLoader<D>::kScales;
+                    k_scales = reinterpret_cast<const float*>(ring + kRing * kTile + PgCodesLoader<D>::kPlaces * PgCodesLoader<D>::kPlace) + slot * 2 * kPgKeys;
+                    v_scales = k_scales + kPgKeys;
+                    if (!tc_wait_warp(&sm.scales_full[slot], (uint32_t)((block / PgCodesLoader<D>::kScales) & 1), &sm.abort)) {
+                        ok = false;
+                        break;
+                    }
+                    if (kUnit) {
+                        const float4 v = reinterpret_cast<const float4*>(v_scales)[lane];
+                        auto finite = [](float f) { return fabsf(f) < __uint_as_float(0x7f800000u) ? fabsf(f) : 0.f; };
+                        const uint32_t bits = __float_as_uint(warp_max(fmaxf(fmaxf(finite(v.x), finite(v.y)), fmaxf(finite(v.z), finite(v.w)))));
+                        const int needed = max(-126, min((int)(bits >> 23) - 126, 126));
+                        if (needed > unit) {
+                            less = unit == -126 ? 1.0f : ex2_approx((float)(unit - needed));
+                            unit = needed;
+                        }
+                    }
+                }
                 if (!tc_wait_warp(&sm.s_full[x], (uint32_t)(used & 1), &sm.abort)) {
                     ok = false;
                     break;
@@ -559,7 +627,16 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
                 // scores of keys c0 .. c0 + 31 of the block: bias, masks
                 float base0 = kBias ? slope * (float)(key0 - pos) : 0.f;
                 const bool masked = !__all_sync(0xffffffffu, low <= key0 && high >= key0 + kPgKeys - 1);
-                auto finish = [&](uint32_t* v, int c0) {
+                auto finish = [&](uint32_t* v, int c0, const float4* k) {
+                    if (kCodes) {
+#pragma unroll
+                        for (int c = 0; c < 32; c += 4) {
+                            const float4 f = k[c / 4];
+                            const float2 t = split2(mul2(pair2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), pair2(f.x, f.y)));
+                            const float2 u = split2(mul2(pair2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3])), pair2(f.z, f.w)));
+                            v[c] = __float_as_uint(t.x), v[c + 1] = __float_as_uint(t.y), v[c + 2] = __float_as_uint(u.x), v[c + 3] = __float_as_uint(u.y);
+                        }
+                    }
                     if (kBias) {
 #pragma unroll
                         for (int c = 0; c < 32; c += 4) {
@@ -594,20 +671,37 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
                 // its exponentials (all 128 at once did not fit the registers).  The probabilities go over the scores of keys
                 // 0 .. 63, so the lower half comes first.
                 uint32_t v[64];
-                tmem_ld32_async(t_s + 64, v);
-                tmem_ld32_async(t_s + 96, v + 32);
-                tmem_ld_wait(v);
-                finish(v, 64);
-                finish(v + 32, 96);
-                maxima(v);
-                maxima(v + 32);
-                tmem_ld32_async(t_s, v);
-                tmem_ld32_async(t_s + 32, v + 32);
-                tmem_ld_wait(v);
-                finish(v, 0);
-                finish(v + 32, 32);
-                maxima(v);
-                maxima(v + 32);
+                if (kCodes) {
+                    // In loops of 32 keys, with the scores back where they were as they are now, which is cheaper than scales, bias and masks a second
+                    // time.  (Without loops, and the upper half done twice: registers spilled, 512 behind 8192 took 143 us and not 118.)
+                    float4 k[8];
+#pragma unroll 1
+                    for (int c0 = 96; c0 >= 0; c0 -= 32) {
+                        tmem_ld32_async(t_s + c0, v);
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) k[c] = reinterpret_cast<const float4*>(k_scales + c0)[c];
+                        tmem_ld_wait32(v);
+                        finish(v, c0, k);
+                        maxima(v);
+                        if (c0) tmem_st32_async(t_s + c0, v);
+                    }
+                }
+                else {
+                    tmem_ld32_async(t_s + 64, v);
+                    tmem_ld32_async(t_s + 96, v + 32);
+                    tmem_ld_wait(v);
+                    finish(v, 64, nullptr);
+                    finish(v + 32, 96, nullptr);
+                    maxima(v);
+                    maxima(v + 32);
+                    tmem_ld32_async(t_s, v);
+                    tmem_ld32_async(t_s + 32, v + 32);
+                    tmem_ld_wait(v);
+                    finish(v, 0, nullptr);
+                    finish(v + 32, 32, nullptr);
+                    maxima(v);
+                    maxima(v + 32);
+                }
                 m_run = fmaxf(m_run, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
                 float corr = 1.0f;
                 const bool first = j == turns.first;
@@ -618,67 +712,107 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
                     corr = ex2_approx(old - ref.log2_of(to_log2));
                 }
                 // O under the new reference.  The P.V of the block before has completed: s_full was committed behind it.
-                if (!first && __any_sync(0xffffffffu, moves)) {
+                if (!first && __any_sync(0xffffffffu, moves || less != 1.0f)) {
+                    const float times = kUnit ? corr * less : corr;
 #pragma unroll 1
                     for (int c0 = 0; c0 < D; c0 += 16) {
                         uint32_t o[16];
                         tmem_ld16(t_o + (uint32_t)c0, o);
 #pragma unroll
-                        for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * corr);
+                        for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * times);
                         tmem_st16_async(t_o + (uint32_t)c0, o);
                     }
                 }
                 const uint64_t scale2 = pair2(ref.factor, ref.factor), off2 = pair2(ref.off, ref.off);
                 uint64_t psum[2] = {0ull, 0ull};
-                auto exponents = [&](const uint32_t* v, uint32_t* pk) {
+                const float per_unit = kUnit ? __uint_as_float((uint32_t)(127 - unit) << 23) : 1.0f;
+                const uint64_t per_unit2 = pair2(per_unit, per_unit);
+                auto exponents = [&](const uint32_t* v, uint32_t* pk, const float4* k) {
 #pragma unroll
                     for (int c = 0; c < 16; ++c) {
                         const float2 e = split2(fma2(pair2(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1])), scale2, off2));
                         const float p0 = ex2_approx(e.x), p1 = ex2_approx(e.y);
                         psum[c & 1] = add2(psum[c & 1], pair2(p0, p1));
-                        pk[c] = PgType<T>::pack(p0, p1);
+                        if (kCodes) {
+                            const float4 of = k[c / 2];
+                            uint64_t w = pair2(p0, p1);
+                            if (kUnit) w = mul2(w, per_unit2);
+                            const float2 q = split2(mul2(w, c % 2 ? pair2(of.z, of.w) : pair2(of.x, of.y)));
+                            pk[c] = PgType<T>::pack(q.x, q.y);
+                        }
+                        else {
+                            pk[c] = PgType<T>::pack(p0, p1);
+                        }
                     }
                 };
                 uint32_t pk[16];
-                exponents(v, pk);
-                tmem_st16_async(t_s, pk);
-                exponents(v + 32, pk);
-                tmem_st16_async(t_s + 16, pk);
-                tmem_ld32_async(t_s + 64, v);
-                tmem_ld32_async(t_s + 96, v + 32);
-                if (!kCodes && (key0 < span.lo || key0 + kPgKeys > span.hi)) {
-                    // rows of V that nobody sees (of codes: zeros already)
-                    const int entry = entry0 + pg_v_entry(j, blocks), stage = entry % kRing;
-                    if (!tc_wait_warp(&sm.full[stage], (uint32_t)((entry / kRing) & 1), &sm.abort)) {
-                        ok = false;
-                        break;
-                    }
-                    if (key0 + r < span.lo || key0 + r >= span.hi) {
-                        uint4* dst = reinterpret_cast<uint4*>(ring + stage * kTile + r * 128);
+                if (kCodes) {
+                    float4 k[8];
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+#pragma unroll 1
+                    for (int i = 0; i < 4; ++i) {
 #pragma unroll
-                        for (int h = 0; h < kHalves; ++h) {
+                        for (int c = 0; c < 8; ++c) k[c] = reinterpret_cast<const float4*>(v_scales + 32 * i)[c];
+                        if (i > 0) tmem_ld_wait32(v);
+                        exponents(v, pk, k);
+                        if (masked) {
+                            // (a scale that is not finite, of a value that this row does not see)
 #pragma unroll
-                            for (int c = 0; c < 8; ++c) dst[h * (kHalf / 16) + c] = make_uint4(0u, 0u, 0u, 0u);
+                            for (int c = 0; c < 16; ++c) {
+                                pk[c] &= (v[2 * c] == 0xff800000u ? 0u : 0xffffu) | (v[2 * c + 1] == 0xff800000u ? 0u : 0xffff0000u);
+                            }
+                        }
+                        tmem_st16_async(t_s + 16 * i, pk);
+                        if (i < 3) tmem_ld32_async(t_s + 32 * i + 32, v);
+                        if (i & 1) {
+                            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(i == 1 ? &sm.p_half[x] : &sm.p_ready[x]);
                         }
                     }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
-                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sm.p_half[x]);
-                tmem_ld_wait(v);
-                if (kBias) asm volatile("" : "+f"(base0), "+f"(slope));   // (or the bias would be kept from the first time, in 64 registers)
-                finish(v, 64);
-                finish(v + 32, 96);
-                exponents(v, pk);
-                tmem_st16_async(t_s + 32, pk);
-                exponents(v + 32, pk);
-                tmem_st16_async(t_s + 48, pk);
-                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sm.p_ready[x]);
+                else {
+                    exponents(v, pk, nullptr);
+                    tmem_st16_async(t_s, pk);
+                    exponents(v + 32, pk, nullptr);
+                    tmem_st16_async(t_s + 16, pk);
+                    tmem_ld32_async(t_s + 64, v);
+                    tmem_ld32_async(t_s + 96, v + 32);
+                    if (key0 < span.lo || key0 + kPgKeys > span.hi) {
+                        // rows of V that nobody sees
+                        const int entry = entry0 + pg_v_entry(j, blocks), stage = entry % kRing;
+                        if (!tc_wait_warp(&sm.full[stage], (uint32_t)((entry / kRing) & 1), &sm.abort)) {
+                            ok = false;
+                            break;
+                        }
+                        if (key0 + r < span.lo || key0 + r >= span.hi) {
+                            uint4* dst = reinterpret_cast<uint4*>(ring + stage * kTile + r * 128);
+#pragma unroll
+                            for (int h = 0; h < kHalves; ++h) {
+#pragma unroll
+                                for (int c = 0; c < 8; ++c) dst[h * (kHalf / 16) + c] = make_uint4(0u, 0u, 0u, 0u);
+                            }
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    }
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sm.p_half[x]);
+                    tmem_ld_wait(v);
+                    if (kBias) asm volatile("" : "+f"(base0), "+f"(slope));   // (or the bias would be kept from the first time, in 64 registers)
+                    finish(v, 64, nullptr);
+                    finish(v + 32, 96, nullptr);
+                    exponents(v, pk, nullptr);
+                    tmem_st16_async(t_s + 32, pk);
+                    exponents(v + 32, pk, nullptr);
+                    tmem_st16_async(t_s + 48, pk);
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sm.p_ready[x]);
+                }
                 const float2 ps = split2(add2(psum[0], psum[1]));
                 l_run = l_run * corr + (ps.x + ps.y);
             }
@@ -700,12 +834,13 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             }
             float max2 = fmaxf(ref.log2_of(to_log2), kPgNone);
-            float scale_a = 1.f, scale_b = 0.f;
+            float scale_a = kUnit ? __uint_as_float((uint32_t)(127 + unit) << 23) : 1.f, scale_b = 0.f;
             bool other = false;              // b's sums are to be added
             if (split && x == 1) {
                 if (mine) {
                     sm.b_max[r] = max2;
                     sm.b_sum[r] = l_run;
+                    if (kUnit) sm.b_unit = scale_a;   // (all threads the same)
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sm.b_ready);
@@ -721,10 +856,12 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 other = true;
                 const float bm = sm.b_max[r], top = fmaxf(max2, bm);
+                const float unit_a = scale_a;
                 scale_a = ex2_approx(max2 - top);
                 scale_b = ex2_approx(bm - top);
                 max2 = top;
                 l_run = l_run * scale_a + sm.b_sum[r] * scale_b;
+                if (kUnit) scale_a *= unit_a, scale_b *= sm.b_unit;
             }
             const bool complete = p.starts && p.ends;
             const PgPartial part = pg_partial(ws, region, cta, p.starts ? 1 : 0, 2 * kPgRows, D);
@@ -790,7 +927,7 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
 
 constexpr int pg_tiles_smem(int head_dim, int codes = 0)
 {
-    return (2 + pg_ring(head_dim, codes)) * (head_dim / 64) * kPgRows * 128 + (codes ? 2 * (kPgKeys * head_dim + kPgKeys * 4) : 0);
+    return (2 + pg_ring(head_dim, codes)) * (head_dim / 64) * kPgRows * 128 + (codes ? 3 * (kPgKeys / 2) * head_dim + 6 * 2 * kPgKeys * 4 : 0);
 }
 
 template<typename T, int D, bool kBias>

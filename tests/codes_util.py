@@ -63,7 +63,7 @@ class CodesBatch(Batch):
             scale.transpose(1, 2)[~held] = math.nan
 
 
-def attend_codes64(batch, scale=None, window=0, first_key=None, alibi_slopes=None, read_back=False):
+def attend_codes64(batch, scale=None, window=0, first_key=None, alibi_slopes=None, tiles=False):
     """(out, tolerance) [tokens of the sequences, heads, head_dim] in float64.
 
     The tolerance, first order.  A weight p_j s_j (s_j the scale of the value) is rounded to fp16, by u = 2^-11 of itself; the sum that
@@ -74,11 +74,12 @@ def attend_codes64(batch, scale=None, window=0, first_key=None, alibi_slopes=Non
     power of two with the largest value at 2^14 or more, off by 2^-25 at most: 2^-39 of the largest.  The result is rounded by half a
     step.
 
-    read_back: for tiles of 128 rows, which round code times scale to q's type first, by half a step of it, or in fp16 2^-25: every key, which
-    moves its score, and every value; and weights as 16-bit caches have them, in q's type, without the scale."""
+    tiles: for calls that take tiles of 128 rows, where the weight times the scale is rounded to q's type, and the sum that divides is of weights that
+    are not rounded; and for the sequences of few tokens among them as above.  In fp16 a weight is held under a power of two that is at most twice the largest scale among the values that the tile reads, so what
+    falls below the smallest normal value is off by 2^-25 of that power where the largest weight is 2^7 or more: 2^-31 of that scale, times the codes."""
     H, D = batch.q.shape[1:]
     K = batch.k_cache.shape[1]
-    u = HALF_STEP[batch.dtype] if read_back else 2.0 ** -11
+    u = HALF_STEP[batch.dtype] if tiles else 2.0 ** -11
     scale = 1 / math.sqrt(D) if scale is None else scale
     n = sum(batch.new)
     out, tol = torch.zeros(n, H, D, dtype=torch.float64), torch.zeros(n, H, D, dtype=torch.float64)
@@ -106,16 +107,12 @@ def attend_codes64(batch, scale=None, window=0, first_key=None, alibi_slopes=Non
         e = torch.exp(s - s.amax(-1, keepdim=True).clamp(min=-1e300))
         l = e.sum(-1, keepdim=True)
         w = torch.where(l > 0, e / l, 0.0)
-        least = 2.0 ** -25 if batch.dtype == torch.float16 else 0.0
         off = (2 * D + 8) * 2.0 ** -24 * size
-        if read_back:
-            off = off + u * size + least * abs(scale) * q.abs().sum(-1, keepdim=True)
         off = off.masked_fill(~seen, 0).amax(-1, keepdim=True)
         o, mag = w @ v, w @ v.abs()
         t_o = (2 * u + 2 * off + 2.0 ** -19) * mag + HALF_STEP[batch.dtype] * o.abs() + 2.0 ** -25
-        if read_back:
-            t_o += u * mag + least
-        t_o += 2.0 ** -32 * (w * vs).amax(-1, keepdim=True) * (seen.double() @ (v.abs() / vs.transpose(1, 2)))
+        codes = seen.double() @ (v.abs() / vs.transpose(1, 2))
+        t_o += (2.0 ** -31 * vs.amax() if tiles else 2.0 ** -32 * (w * vs).amax(-1, keepdim=True)) * codes
         out[at:at + t], tol[at:at + t] = o.transpose(0, 1), t_o.transpose(0, 1)
         at += t
     return out, tol

@@ -181,14 +181,14 @@ def test_load_of_missing_pages_and_positions():
 # ---------------------------------------------------------------------------------------------------------------------
 # attention
 # ---------------------------------------------------------------------------------------------------------------------
-def _check(batch, what="", read_back=False, **options):
+def _check(batch, what="", tiles=False, **options):
     given = {w: (x.cuda() if torch.is_tensor(x) else x) for w, x in options.items()}
     total = sum(batch.new)
     out = torch.full_like(batch.q, 7.0).cuda()
     got = _paged().paged_mha(batch.q.cuda(), *batch.gpu(), out=out, **batch.scales(), **given)
     assert got is out
     plain = {w: x for w, x in options.items() if w in ("scale", "window", "first_key", "alibi_slopes")}
-    ref, tol = attend_codes64(batch, read_back=read_back, **plain)
+    ref, tol = attend_codes64(batch, tiles=tiles, **plain)
     _within(out[:total], ref, tol, what)
     assert (out[total:] == 7.0).all(), "rows behind the last sequence"
     assert _status() == 0
@@ -204,7 +204,7 @@ ROWS = [([1], [1]), ([1], [300]), ([1, 1, 1], [5, 128, 129]), ([1] * 40, [1 + 37
 def test_mha_few_rows(new, lens, heads, kv_heads, head_dim, page, kind, dtype):
     batch = CodesBatch(new, lens, heads, kv_heads, head_dim, page, dtype, kind, behind=1)
     batch.poison()
-    _check(batch, max_tokens=max(new), read_back=max(new) * heads // kv_heads > 16)
+    _check(batch, max_tokens=max(new), tiles=max(new) * heads // kv_heads > 16)
 
 
 @pytest.mark.parametrize("kind", CODES)
@@ -232,7 +232,7 @@ TILES = [([17], [17]), ([200], [300]), ([129], [2000]), ([300, 260], [300, 700])
 def test_mha_tiles(new, lens, heads, kv_heads, head_dim, page, kind, dtype):
     batch = CodesBatch(new, lens, heads, kv_heads, head_dim, page, dtype, kind, behind=1)
     batch.poison()
-    _check(batch, max_tokens=max(new), read_back=True)
+    _check(batch, max_tokens=max(new), tiles=True)
 
 
 @pytest.mark.parametrize("kind", CODES)
@@ -248,7 +248,7 @@ def test_mha_tiles_options(kind, heads, kv_heads, options):
         options["first_key"] = torch.tensor([30, 150, 0, 49], dtype=torch.int32)     # the first sequence sees nothing
     if options.pop("alibi", False):
         options["alibi_slopes"] = torch.tensor([2.0 ** -(i % 8 + 1) for i in range(heads)])
-    _check(batch, max_tokens=200, read_back=True, **options)
+    _check(batch, max_tokens=200, tiles=True, **options)
 
 
 @pytest.mark.parametrize("kind", CODES)
@@ -260,7 +260,7 @@ def test_mha_a_chunk_beside_single_tokens(kind, dtype, heads, kv_heads, head_dim
     batch = CodesBatch(new, lens, heads, kv_heads, head_dim, page, dtype, kind, behind=3)
     batch.poison()
     more = dict(alibi_slopes=torch.tensor([2.0 ** -(i % 8 + 1) for i in range(heads)])) if alibi else {}
-    _check(batch, max_tokens=150, max_len=3000, read_back=True, **more)
+    _check(batch, max_tokens=150, max_len=3000, tiles=True, **more)
 
 
 @pytest.mark.parametrize("kind", CODES)
@@ -269,6 +269,30 @@ def test_mha_scales_of_very_different_sizes(kind, spread):
     """Rows of the cache that differ by up to 2^26 in size; q so small that all keys count."""
     batch = CodesBatch([1, 1], [900, 40], 4, 4, 128, 16, BF16, kind, spread=spread, q_scale=0.01)
     _check(batch, max_tokens=1)
+
+
+@pytest.mark.parametrize("kind", CODES)
+@pytest.mark.parametrize("dtype", [FP16, BF16])
+@pytest.mark.parametrize("spread", [6.0, 13.0])
+def test_mha_tiles_scales_of_very_different_sizes(kind, dtype, spread):
+    batch = CodesBatch([150, 40], [900, 40], 4, 2, 128, 16, dtype, kind, spread=spread, q_scale=0.01)
+    _check(batch, max_tokens=150, tiles=True)
+
+
+@pytest.mark.parametrize("kind", CODES)
+@pytest.mark.parametrize("new", [2, 3, 90])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_mha_scales_that_are_not_finite_reach_the_rows_that_see_them(kind, new, bad):
+    """(Such a scale stands for a row of k or v that was not finite.)"""
+    batch = CodesBatch([new], [300], 4, 2, 128, 16, FP16, kind)
+    clean = _paged().paged_mha(batch.q.cuda(), *batch.gpu(), **batch.scales(), max_tokens=new)
+    page, slot = int(batch.gpu()[2][0, 299 // 16]), 299 % 16
+    for which in ("k", "v"):
+        scales = {w: x.clone() for w, x in batch.scales().items()}
+        scales[which + "_scale"][page, :, slot] = bad
+        out = _paged().paged_mha(batch.q.cuda(), *batch.gpu(), **scales, max_tokens=new)
+        assert torch.equal(out[:-1], clean[:-1]), which
+        assert not torch.isfinite(out[-1]).any() or which == "k" or bad == math.inf
 
 
 def test_mha_is_the_same_whatever_the_hints():
@@ -335,7 +359,7 @@ def test_mha_over_missing_pages(new, most, kind):
         cache.view(torch.uint8)[spare] = 0
         scale[spare] = 1.0
     batch.pages[0, 1] = batch.pages[1, 0] = spare
-    ref, tol = attend_codes64(batch, read_back=most > 8)
+    ref, tol = attend_codes64(batch, tiles=most > 8)
     _within(got, ref, tol)
 
 
@@ -348,7 +372,7 @@ def test_mha_of_strided_caches():
     for most in (1, 20):
         got = _paged().paged_mha(batch.q.cuda(), kc, vc, *(t.cuda() for t in (batch.pages, batch.starts, batch.lens)), max_tokens=most,
                                  k_scale=both[:, 0], v_scale=both[:, 1])
-        ref, tol = attend_codes64(batch, read_back=True)
+        ref, tol = attend_codes64(batch, tiles=True)
         _within(got, ref, tol)
     k, v = _paged().paged_load(kc, vc, *(t.cuda() for t in (batch.pages, batch.starts, batch.lens)), 22, dtype=BF16, k_scale=both[:, 0],
                                v_scale=both[:, 1])
@@ -386,7 +410,7 @@ def test_a_captured_call_serves_other_lengths(kind, new, most):
         cache[4].copy_(torch.tensor(other, dtype=torch.int32))
         out.fill_(9.0)
         graph.replay()
-        ref, tol = attend_codes64(batch, read_back=True)
+        ref, tol = attend_codes64(batch, tiles=True)
         _within(out, ref, tol, str(other))
     assert _status() == 0
 
