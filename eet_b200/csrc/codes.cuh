@@ -1,8 +1,8 @@
 // 8-bit codes of a paged cache: a row of head_dim values y is kept as codes c and one fp32 scale s, and stands for c * s.
 //   int8   c in [-127, 127], s = max |y| / 127
 //   e4m3   1 sign, 4 exponent (bias 7), 3 mantissa bits, c in [-448, 448], s = max |y| / 448
-// s is 1 for a row of zeros, at least the smallest normal number otherwise, and NaN for a row with a NaN or an infinity, which has
-// no codes: whoever reads it gets NaN.
+// s is 1 for a row of zeros, at least the smallest normal number otherwise, and NaN for a row with a NaN or an infinity, whose
+// codes stand for nothing (of e4m3 they are zeros): whoever reads it gets NaN.
 #pragma once
 #include "common.cuh"
 #include "kernels.h"

@@ -19,8 +19,14 @@
 // P^T leaves S^T's layout by a transposition of 8 x 8 in the warp (movmatrix).  (Tensor memory and tcgen05 would need the values in shared
 // memory: 64 KiB written and read again for every 32 KiB that arrive.)
 //
-// A CTA is four warps, 32 keys of a block each; two CTAs share an SM, so that the beginning and the end of a piece of one run beside the
-// other's blocks.  The warps' sums meet in shared memory at the end of a piece.  The work is cut up as paged_share.cuh says.
+// A CTA is four warps, 32 keys of a block each; three CTAs share an SM, two where there are 16 rows, so that the beginning and the end of a
+// piece of one run beside the others' blocks.  The warps' sums meet in shared memory at the end of a piece.  The work is cut up as
+// paged_share.cuh says.  Measured: 64 sequences of 200 to 8000 tokens, 32 / 8 heads, bf16 over int8, 65 us (75 with two CTAs), which is 4.1 TB/s;
+// two of 60 and 100 thousand tokens, 64 / 8 heads, fp16 over e4m3, 70 us (4.6 TB/s).  What bounds it then is the issue of instructions: codes
+// take 8 conversions and bytes' selections for every 16 bytes, which issue every second cycle.
+//
+// Longer chunks go to tiles of 128 rows (paged_tc.cu has what a CTA does), in a kernel of their own behind the same plan.  Where a call has both kinds of
+// sequences, the kernels run side by side on parts of the SMs, divided by what a block takes on either, and one launch adds up the parts of both.
 #include <type_traits>
 
 #include "codes.cuh"
@@ -36,8 +42,8 @@ template<int D, int kRows>
 struct PcShape {
     static constexpr int kWarps = 4;
     static constexpr int kKeys = kPgKeys / kWarps;                      // of a block, for a warp: one or two runs of 16
-    static constexpr int kAtOnce = kRows == 8 ? 2 : 1;// runs that are worked on together
-    static constexpr int kPerSm = kRows == 8 ? 3 : 2;// CTAs
+    static constexpr int kAtOnce = kRows == 8 ? 2 : 1;                  // runs that are worked on together
+    static constexpr int kPerSm = kRows == 8 ? 3 : 2;                   // CTAs
     static constexpr int kStages = kRows == 8 && D == 128 ? 2 : 3;
     static constexpr int kTile = kKeys * D;                             // bytes: a warp's codes of K or V of a block
     static constexpr int kStage = 2 * kTile + 2 * kKeys * 4;            // and the scales

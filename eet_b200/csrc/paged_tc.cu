@@ -24,14 +24,17 @@
 // Keys outside of what any row of the pair sees may be anything, even NaN (slots behind the end of a sequence): their scores are
 // masked by selection and their rows of V are set to zero in shared memory before the product reads them.
 //
-// Over a cache of 8-bit codes the products take the codes, which are exact in q's type, and the scales stay outside: that of a key on its scores, that
-// of a value on its weight, before that is rounded.  (With code times scale rounded to 16 bits in front of the products the result was off by up to
-// 4.5 times as much as the rounded exact one: scores are sums of 128 rounded keys.)  In fp16 the weights are held under a power of two that
-// follows the largest scale of the values so far.  Warp 8 brings codes to three places in shared memory, half an entry each, and the scales of a
-// block to a ring of six; four more warps (12-15, a warpgroup of their own) turn the codes into 16-bit values where the copy engine would have put
-// K and V.  What these warps do has to be little code as well as few instructions: five kinds of warps share an instruction cache (512 behind
-// 8192, 32 / 8 heads, bf16: unrolled 187 us, in a loop of 32 codes 130; with the copies among their duties 126, without 101).  512 threads of 128
-// registers are launched, of which the softmax takes 136 and the others 120.
+// Over a cache of 8-bit codes the products take the codes, which are exact in q's type, and the scales stay outside: that of a key on its
+// scores, that of a value on its weight, before that is rounded.  (With code times scale rounded to 16 bits in front of the products
+// the result was off by 2.9 times as much as the exact one rounded once, and by 1.4 times so: scores are sums of 128 rounded keys.)
+// In fp16 O and the weights are held under a power of two that follows the largest scale of the values so far.  Warp 8 brings codes to three places in shared
+// memory, half an entry each, and the scales of a block to a ring of six; four more warps (12-15, a warpgroup of their own) turn the
+// codes into 16-bit values where the copy engine would have put K and V.  What these warps and the softmax do has to be little code as well
+// as few instructions: five kinds of warps share an instruction cache.  512 tokens behind 8192, 32 / 8 heads, bf16: conversions written
+// out 187 us, in a loop 130, with the copies taken from them 101; that was with rounded keys.  With exact codes, and the softmax written
+// out as it is for 16 bits, 143; its scores put back after their scales instead of scaled twice 129, in loops of 32 keys 120.  (The 16-bit cache: 87.)
+// 512 threads of 128 registers are launched, of which the softmax takes 136 and the others 120, without spills but for 12 bytes with a
+// bias (144 and 112: 124 us, with spills).
 #include <type_traits>
 
 #include "codes.cuh"
@@ -44,7 +47,8 @@ namespace {
 constexpr int kPgThreads = 320;
 constexpr int kPgCodesThreads = 512;    // with the warps that convert codes
 constexpr int kPgStages = 5;
-constexpr __host__ __device__ int pg_ring(int head_dim, int codes) { return codes && head_dim == 128 ? 4 : kPgStages; }   // (with codes their own ring takes room)
+// (the codes' own places take room)
+constexpr __host__ __device__ int pg_ring(int head_dim, int codes) { return codes && head_dim == 128 ? 4 : kPgStages; }
 constexpr int kPgExtra = 3;             // a tile's beginning and end cost as much as three blocks
 constexpr uint32_t kPgTmemCols = 512;   // S of a, S of b (their probabilities over them), O of a, O of b: 128 each
 
@@ -163,8 +167,8 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b)
     return d;
 }
 
-// Four codes as two words of T.  int8 as bf16: a byte under the exponent of 128, where the low seven bits are units, less 128, or 256 where its top bit
-// says that it is negative.
+// Four codes as two words of T.  int8 as bf16: a byte under the exponent of 128, where the low seven bits are units, less 128, or 256 where
+// its top bit says that it is negative.
 template<typename T, int kCodes>
 __device__ __forceinline__ void pg_values4(uint32_t w, uint32_t& lo, uint32_t& hi)
 {
@@ -257,9 +261,10 @@ struct PgCodesLoader {
     }
 };
 
-// 16 keys of half an entry into the ring, from key0 of it.  Lane (r, c) = (lane / 4, lane % 4) has 16 codes of keys r and r + 8 in either half of a row, odd
-// keys the halves in the other order: eight lanes then meet no bank twice, reading or writing.  scales: of the block's values, where rows
-// are to be zero that nobody sees, and those whose scale is not finite: what is there may be NaN, and nothing times that is NaN.
+// 16 keys of half an entry into the ring, from key0 of it, eight at a time.  Lane (r, c) = (lane / 4, lane % 4) has 16 codes of key r in
+// either half of a row, odd keys the halves in the other order: eight lanes then meet no bank twice, reading or writing.  scales: of the
+// block's values, where rows are to be zero that nobody sees, and those whose scale is not finite: what is there may be NaN, and nothing
+// times that is NaN.
 template<typename T, int D, int kCodes>
 __device__ __forceinline__ void pg_convert(const uint8_t* place, int key0, const float* scales, uint8_t* stage, int stage_key)
 {
@@ -524,13 +529,16 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
                 const int block = before + (end ? n - 1 : e / 2 - 1);   // (of V)
                 // (rows that nobody sees: at the ends of what the tile reads, and of pages outside the cache; K's scores are masked)
                 const float* of = kCodes == kCodesE4M3 && v ? scales + (block % Loader::kScales * 2 + 1) * kPgKeys : nullptr;
-                if (of != nullptr && ok) ok = tc_wait_warp(&sm.scales_full[block % Loader::kScales], (uint32_t)((block / Loader::kScales) & 1), &sm.abort);
+                if (of != nullptr && ok) {
+                    ok = tc_wait_warp(&sm.scales_full[block % Loader::kScales], (uint32_t)((block / Loader::kScales) & 1), &sm.abort);
+                }
 #pragma unroll 1
                 for (int half = 0; half < 2 && ok; ++half, ++done) {
                     const int x = done % Loader::kPlaces, at = 16 * (warp - 12);
                     ok = tc_wait_warp(&sm.staged_full[x], (uint32_t)((done / Loader::kPlaces) & 1), &sm.abort);
                     if (!ok) break;
-                    pg_convert<T, D, kCodes ? kCodes : kCodesInt8>(places + x * Loader::kPlace, at, of, ring + stage * kTile, kPgKeys / 2 * half + at);
+                    pg_convert<T, D, kCodes ? kCodes : kCodesInt8>(places + x * Loader::kPlace, at, of, ring + stage * kTile,
+                                                                   kPgKeys / 2 * half + at);
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sm.staged_empty[x]);
                 }
@@ -592,16 +600,17 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
             const uint64_t rise[2] = {pair2(0.f, slope), pair2(2.f * slope, 3.f * slope)};   // of the bias over four keys
             float m_run = kPgNone, l_run = 0.f;
             PgReference ref = {1.0f, -kPgNone};   // (-inf stays -inf, and any score moves it)
-            // Codes in fp16: O is held under 2^unit, no less than the largest scale of the values so far, so that weights times scales stay below 2^15.
+            // Codes in fp16: O is held under 2^unit, above the largest scale of the values so far, so that weights times scales stay below 2^15.
             constexpr bool kUnit = kCodes != 0 && std::is_same<T, __half>::value;
-            int unit = -126;
+            int unit = -127;   // (none yet)
             for (int j = turns.first; j < turns.end && ok; j += turns.stride) {
                 const int key0 = (top - j) * kPgKeys;
                 const float *k_scales = nullptr, *v_scales = nullptr;
                 float less = 1.0f;             // a power of two: of O under the unit before
                 if (kCodes) {
                     const int block = entry0 / 2 + j, slot = block % PgCodesLoader<D>::kScales;
-                    k_scales = reinterpret_cast<const float*>(ring + kRing * kTile + PgCodesLoader<D>::kPlaces * PgCodesLoader<D>::kPlace) + slot * 2 * kPgKeys;
+                    const uint8_t* ring_end = ring + kRing * kTile + PgCodesLoader<D>::kPlaces * PgCodesLoader<D>::kPlace;
+                    k_scales = reinterpret_cast<const float*>(ring_end) + slot * 2 * kPgKeys;
                     v_scales = k_scales + kPgKeys;
                     if (!tc_wait_warp(&sm.scales_full[slot], (uint32_t)((block / PgCodesLoader<D>::kScales) & 1), &sm.abort)) {
                         ok = false;
@@ -613,7 +622,7 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
                         const uint32_t bits = __float_as_uint(warp_max(fmaxf(fmaxf(finite(v.x), finite(v.y)), fmaxf(finite(v.z), finite(v.w)))));
                         const int needed = max(-126, min((int)(bits >> 23) - 126, 126));
                         if (needed > unit) {
-                            less = unit == -126 ? 1.0f : ex2_approx((float)(unit - needed));
+                            less = unit == -127 ? 1.0f : ex2_approx((float)(unit - needed));
                             unit = needed;
                         }
                     }
@@ -634,7 +643,8 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
                             const float4 f = k[c / 4];
                             const float2 t = split2(mul2(pair2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), pair2(f.x, f.y)));
                             const float2 u = split2(mul2(pair2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3])), pair2(f.z, f.w)));
-                            v[c] = __float_as_uint(t.x), v[c + 1] = __float_as_uint(t.y), v[c + 2] = __float_as_uint(u.x), v[c + 3] = __float_as_uint(u.y);
+                            v[c] = __float_as_uint(t.x), v[c + 1] = __float_as_uint(t.y);
+                            v[c + 2] = __float_as_uint(u.x), v[c + 3] = __float_as_uint(u.y);
                         }
                     }
                     if (kBias) {
@@ -672,8 +682,8 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
                 // 0 .. 63, so the lower half comes first.
                 uint32_t v[64];
                 if (kCodes) {
-                    // In loops of 32 keys, with the scores back where they were as they are now, which is cheaper than scales, bias and masks a second
-                    // time.  (Without loops, and the upper half done twice: registers spilled, 512 behind 8192 took 143 us and not 118.)
+                    // (in loops of 32 keys, with the scores back where they were as they are now: cheaper than scales, bias and masks a second
+                    // time, and without spills)
                     float4 k[8];
 #pragma unroll 1
                     for (int c0 = 96; c0 >= 0; c0 -= 32) {

@@ -7,8 +7,8 @@
 // All of these leave a beginning of one order, so they come down to a cut: a value x*, and how many of its equals stay.  Nothing is sorted but
 // a few candidates around it.
 //   1  the row into shared memory, its maximum
-//   2  a histogram over (max - x) / T, 64 bins to a factor of e in w (fewer where top-k may reach further down than 32 such factors): counts in front of a bin are exact, sums of w known to 1.6 %, and mostly to
-//      1e-4
+//   2  a histogram over (max - x) / T, 64 bins to a factor of e in w (fewer where top-k may reach further down than 32 such factors): counts in
+//      front of a bin are exact, sums of w known to 1.6 %, and mostly to 1e-4
 //   3  the bins in which the cut must lie - by mass first those where it very likely lies, which the sums in step 4 confirm or not; where they
 //      hold too many values for a list, a second histogram over them alone
 //   4  those values in a list, and the exact sums of w of all and of what stands in front of them; the list sorted: the cut.  (Where one bin
@@ -20,7 +20,8 @@
 //
 // A row is worked on by a cluster of 1 to 8 CTAs, which hold it in shared memory and exchange counts and candidates there.  Bound: latency,
 // six barriers of the cluster and four trips through a slice of the row; with many rows the issue of instructions, the powers of all
-// tokens first (11 instructions in 64 bits each, with a table of 128; exp() took three times as long).
+// tokens first (11 instructions in 64 bits each, with a table of 128; exp() took three times as long).  Measured: one row of 32000 fp32 logits
+// 18 us, 64 rows of 64000 fp16 42, 256 of 64000 bf16 145 (22, 119 and 287 with exp() and lists gathered by atomics on one counter).
 #include <cooperative_groups.h>
 
 #include "common.cuh"

@@ -477,8 +477,9 @@ typedef struct {
 
 size_t eet_paged_mha_codes_workspace_bytes(const eet_paged_mha_codes_args* args);
 
-/* eet_paged_mha over a cache of 8-bit codes.  The codes enter the products exactly, as fp16, for q of either type; the weights p_j s^v_j are
- * rounded to fp16. */
+/* eet_paged_mha over a cache of 8-bit codes.  The codes enter the products exactly; the weights p_j s^v_j are rounded, to fp16 where a kv head
+ * has up to 16 rows (new tokens x query heads) of a sequence, else to the type of q.  A row of the cache whose scale is NaN reaches the rows
+ * that see it, and no others. */
 int eet_paged_mha_codes(const eet_paged_mha_codes_args* args, void* stream);
 
 #ifdef __cplusplus
