@@ -602,7 +602,8 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
             PgReference ref = {1.0f, -kPgNone};   // (-inf stays -inf, and any score moves it)
             // Codes in fp16: O is held under 2^unit, above the largest scale of the values so far, so that weights times scales stay below 2^15.
             constexpr bool kUnit = kCodes != 0 && std::is_same<T, __half>::value;
-            int unit = -127;   // (none yet)
+            constexpr int kLeastUnit = -110;   // 2^15 over it is still a number
+            int unit = kLeastUnit - 1;         // (none yet)
             for (int j = turns.first; j < turns.end && ok; j += turns.stride) {
                 const int key0 = (top - j) * kPgKeys;
                 const float *k_scales = nullptr, *v_scales = nullptr;
@@ -620,9 +621,9 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
                         const float4 v = reinterpret_cast<const float4*>(v_scales)[lane];
                         auto finite = [](float f) { return fabsf(f) < __uint_as_float(0x7f800000u) ? fabsf(f) : 0.f; };
                         const uint32_t bits = __float_as_uint(warp_max(fmaxf(fmaxf(finite(v.x), finite(v.y)), fmaxf(finite(v.z), finite(v.w)))));
-                        const int needed = max(-126, min((int)(bits >> 23) - 126, 126));
+                        const int needed = max(kLeastUnit, min((int)(bits >> 23) - 126, 126));
                         if (needed > unit) {
-                            less = unit == -127 ? 1.0f : ex2_approx((float)(unit - needed));
+                            less = unit < kLeastUnit ? 1.0f : ex2_approx((float)(unit - needed));
                             unit = needed;
                         }
                     }

@@ -280,6 +280,23 @@ def test_mha_tiles_scales_of_very_different_sizes(kind, dtype, spread):
 
 
 @pytest.mark.parametrize("kind", CODES)
+@pytest.mark.parametrize("dtype", [FP16, BF16])
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("least", [1e-39, 1e-37, 1e-20, 0.0])
+def test_mha_scales_next_to_nothing_in_the_newest_blocks(kind, dtype, new, least):
+    """Positions 0 to 39 weigh, what is behind them hardly does or not at all."""
+    batch = CodesBatch([new], [300], 4, 2, 128, 16, dtype, kind)
+    batch.v_scale[:] = least
+    for position in range(40):
+        batch.v_scale[batch.pages[0, position // 16], :, position % 16] = 0.01
+    total = sum(batch.new)
+    out = _paged().paged_mha(batch.q.cuda(), *batch.gpu(), **batch.scales(), max_tokens=new)
+    batch.v_scale.clamp_(min=1e-30)       # (the tolerance divides by it; 1e-30 times 448 is nothing beside the step of the result)
+    ref, tol = attend_codes64(batch, tiles=new > 8)
+    _within(out[:total], ref, tol)
+
+
+@pytest.mark.parametrize("kind", CODES)
 @pytest.mark.parametrize("new", [2, 3, 90])
 @pytest.mark.parametrize("bad", [math.nan, math.inf])
 def test_mha_scales_that_are_not_finite_reach_the_rows_that_see_them(kind, new, bad):
