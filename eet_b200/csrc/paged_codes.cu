@@ -597,18 +597,6 @@ paged_mha_codes_kernel(const __grid_constant__ PagedMhaArgs a, void* ws, int few
     pdl_wait();
 }
 
-// Moves registers between the warpgroups; by all warps of a warpgroup.
-template<int kRegisters>
-__device__ __forceinline__ void pg_more_registers()
-{
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegisters));
-}
-template<int kRegisters>
-__device__ __forceinline__ void pg_fewer_registers()
-{
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegisters));
-}
-
 // As pg_begin, but a dependent may begin only when the kernels in front have ended.
 __device__ __forceinline__ void pc_begin(uint32_t* tmem_base, uint32_t columns)
 {
@@ -630,7 +618,6 @@ paged_mha_tc_codes_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
                           const __grid_constant__ CUtensorMap map_v, const __grid_constant__ PagedMhaArgs a, void* ws, int few, int rows_tokens,
                           int whole)
 {
-    static_assert(2 * 136 + 120 + 120 <= 4 * 128, "of what the CTA was launched with");
     extern __shared__ __align__(1024) uint8_t pg_dyn[];
     __shared__ PgSmem sm;
     __shared__ uint32_t tmem_base;
@@ -641,9 +628,6 @@ paged_mha_tc_codes_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     if (threadIdx.x == 0) pg_init(sm, 4);
     pc_begin(&tmem_base, kPgTmemCols);
     const int n = gridDim.x, cta = blockIdx.x, ctas = rows_tokens ? pc_split(a, rows_tokens, few, n, kBias).sms_tiles : n;
-    const int group = threadIdx.x >> 7;
-    if (group < 2) pg_more_registers<136>();
-    else pg_fewer_registers<120>();
     static_assert(sizeof(PgFound) <= sizeof(sm.b_max) + sizeof(sm.b_sum) && alignof(PgFound) <= 8, "lies there for a while");
     if (cta < ctas) {
         pg_tiles<T, D, kBias, kCodes>(&map_q, &map_k, &map_v, a, ws, few + 1, whole, cta, ctas, n, sm, *reinterpret_cast<PgFound*>(sm.b_max), tmem_base,

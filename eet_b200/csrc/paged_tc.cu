@@ -32,9 +32,9 @@
 // codes into 16-bit values where the copy engine would have put K and V.  What these warps and the softmax do has to be little code as well
 // as few instructions: five kinds of warps share an instruction cache.  512 tokens behind 8192, 32 / 8 heads, bf16: conversions written
 // out 187 us, in a loop 130, with the copies taken from them 101; that was with rounded keys.  With exact codes, and the softmax written
-// out as it is for 16 bits, 143; its scores put back after their scales instead of scaled twice 129, in loops of 32 keys 120.  (The 16-bit cache: 87.)
-// 512 threads of 128 registers are launched, of which the softmax takes 136 and the others 120, without spills but for 12 bytes with a
-// bias (144 and 112: 124 us, with spills).
+// out as it is for 16 bits, 143; its scores put back after their scales instead of scaled twice 129, in loops of 32 keys 123.  (The 16-bit cache: 87.)
+// 512 threads of 128 registers, 12 to 28 bytes of spills.  (Shares of 136 for the softmax and 120 for the others, by setmaxnreg: 24 to 48 bytes, the chunk
+// 122 us and not 123, 333 tokens with a bias beside 23 single ones 115 and not 113; 144 and 112: 124.5 and 113.)
 #include <type_traits>
 
 #include "codes.cuh"
