@@ -213,8 +213,10 @@ __device__ __forceinline__ long long pg_seq_blocks(const PagedMhaArgs& a, const 
 
 // Kernels this short spend much of their time on what runs once - the first fetch of every instruction among it - so what follows
 // is kept small: no 64-bit divisions, no barrier where a warp has a lane for each sequence.
+constexpr int kPgMostWarps = 16;   // of a block of any of the kernels
+
 struct PgFound {           // by the block together, where it takes more
-    long long warp_sum[12];
+    long long warp_sum[kPgMostWarps];
     long long rest, per_head;
     PgSeq s;
     int seq;

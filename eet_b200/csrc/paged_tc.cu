@@ -46,6 +46,7 @@ namespace {
 
 constexpr int kPgThreads = 320;
 constexpr int kPgCodesThreads = 512;    // with the warps that convert codes
+static_assert(kPgThreads <= 32 * kPgMostWarps && kPgCodesThreads <= 32 * kPgMostWarps, "a sum for each warp in PgFound");
 constexpr int kPgStages = 5;
 // (the codes' own places take room)
 constexpr __host__ __device__ int pg_ring(int head_dim, int codes) { return codes && head_dim == 128 ? 4 : kPgStages; }
