@@ -27,3 +27,72 @@ def test_every_warp_has_a_place_for_its_sum():
     bounds = set(re.findall(r"__launch_bounds__\((kP\w+Threads|32 \* PcShape[^,]*, kRows>::kWarps)", rows + tiles + codes))
     assert bounds == {"kPwThreads", "kPgThreads", "kPgCodesThreads", "32 * PcShape<D, kRows>::kWarps"}
     assert max(threads) <= 32 * places
+
+
+def _body(text, head):
+    """The braces behind `head`, and what they hold."""
+    start = text.index("{", text.index(head))
+    depth = 0
+    for i in range(start, len(text)):
+        depth += {"{": 1, "}": -1}.get(text[i], 0)
+        if depth == 0:
+            return text[start:i + 1]
+    raise AssertionError(head)
+
+
+def _passed_by_b(new, lens, heads, kv_heads, whole, ctas=148, extra=3, keys=128):
+    """For each first block that tile b of a pair has in a piece: how many blocks it has passed without a wait in front of that, since its
+    last turn.  The walk of PgShare: tiles of 2 (128 / group) tokens, each `extra` blocks more than it has, the shares equal."""
+    tokens = 2 * (128 // (heads // kv_heads))
+    tiles = []                                       # (blocks, blocks of which b has a turn)
+    for t, n in zip(new, lens):
+        for _ in range(kv_heads):
+            for at in range(0, t, tokens):
+                blocks = -(-(n - t + min(at + tokens, t)) // keys)
+                tiles.append((blocks, t - at <= tokens // 2))
+    total = sum(b + extra for b, _ in tiles)
+    pieces, place = [[] for _ in range(ctas)], 0
+    begin = [total // ctas * c + min(c, total % ctas) for c in range(ctas + 1)]
+    for blocks, split in tiles:
+        for c in range(ctas):
+            if whole:
+                n = blocks if begin[c] <= place < begin[c + 1] else 0
+            else:
+                low, high = (min(max(begin[c + i] - place - extra, 0), blocks) for i in (0, 1))
+                n = high - low
+            if n:
+                pieces[c].append((n, split))
+        place += blocks + extra
+    passed = []
+    for share in pieces:
+        ahead = 0
+        for n, split in share:
+            if split and n == 1:
+                ahead += 1
+                continue
+            passed.append(ahead)
+            ahead = 0
+    return passed
+
+
+def test_the_warps_of_tile_b_come_to_their_first_block_from_far_ahead():
+    """Ordinary loads of few new tokens: in some shares tile b has passed six blocks and more, a turn of the ring of scales, without a wait.
+    A wait by parity would then end before its data is there, so the softmax waits for the scores of a piece's first block first, in front
+    of everything that it reads of the scales."""
+    tiles = _source("paged_tc.cu")
+    ring = int(re.search(r"kPlaces = 3, kScales = (\d+);", tiles).group(1))
+    import random
+    rng = random.Random(1)
+    loads = [([5] * 256, [rng.randint(60, 260) for _ in range(256)], 32, 8),
+             ([17] * 64, [17 + rng.randint(20, 250) for _ in range(64)], 32, 32)]
+    for new, lens, heads, kv_heads in loads:
+        assert any(max(_passed_by_b(new, lens, heads, kv_heads, whole)) >= ring for whole in (False, True))
+    assert max(_passed_by_b([512], [8704], 32, 8, False)) < ring      # (a chunk's pieces are long)
+    # The loop over a piece's blocks: s_full, under `first`, is waited for in front of scales_full and of the first look at a scale.
+    softmax = tiles[tiles.index("pg_reference<T>(m_run") - 20000:]
+    loop = _body(softmax[softmax.index("PgReference ref = {1.0f, -kPgNone};"):], "for (int j = turns.first;")
+    assert re.search(r"const bool first = j == turns\.first;", loop)
+    guard = re.search(r"if \(first && !tc_wait_warp\(&sm\.s_full\[x\], \(uint32_t\)\(used & 1\), &sm\.abort\)\) \{\s*ok = false;\s*break;\s*\}", loop)
+    assert guard, "the scores of the first block"
+    assert guard.end() < loop.index("sm.scales_full[slot]") < loop.index("v_scales)[lane]")
+    assert "v_scales" not in loop[:guard.start()].replace("*v_scales = nullptr", "")
