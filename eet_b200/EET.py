@@ -397,7 +397,7 @@ def sample_rows(logits2d, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
     [rows], logprobs float32 [rows]), logprobs being ln of the probability with which the token was drawn.
 
       uniform       float32 [rows] in [0, 1), from the caller's generator: the same numbers give the same tokens
-      temperature   of exp(logit / temperature); 0: the largest logit, the smallest index on ties, as argmax_rows
+      temperature   of exp(logit / temperature); 0: the largest logit, the smallest index on ties, as argmax_rows; inf: all alike
       top_k         the so many largest logits stay, the smallest index first on ties; 0: all
       top_p         of those, the most probable ones in front of which stands a probability below top_p; 1: all
       min_p         of those, the ones with at least min_p times the largest probability; 0: all

@@ -3,6 +3,8 @@
 // so that the device-side status word and the inline helpers are shared without relocatable device code.
 #include "../../include/eet_b200.h"
 
+#include <cfloat>
+#include <cmath>
 #include <cstring>
 #include <initializer_list>
 #include <string>
@@ -605,7 +607,7 @@ int eet_sample_rows(const eet_sample_rows_args* p, void* stream)
     a.logits = p->logits, a.uniform = p->uniform, a.temperatures = p->temperatures, a.top_ps = p->top_ps, a.min_ps = p->min_ps;
     a.top_ks = p->top_ks, a.tokens = (long long*)p->tokens, a.logprobs = p->logprobs;
     a.rows = (int)p->rows, a.vocab = (int)p->vocab, a.type = (int)p->type, a.row_stride = p->row_stride;
-    a.temperature = (float)p->temperature, a.top_p = (float)p->top_p, a.min_p = (float)p->min_p, a.top_k = (int)p->top_k;
+    a.temperature = p->temperature > FLT_MAX ? INFINITY : (float)p->temperature, a.top_p = (float)p->top_p, a.min_p = (float)p->min_p, a.top_k = (int)p->top_k;
     return launch_sample(a, (cudaStream_t)stream);
 }
 

@@ -690,8 +690,9 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_rows_kernel(const Sample
         }
         return;                    // (all of the cluster, and the last word to another CTA lies in front of a barrier)
     }
-    // (a finite scale: nothing times infinity is no place)
-    float scale = fminf(kSaBinsPerE / temperature, 1e30f);
+    // (a finite scale: nothing times infinity is no place; and above zero, also where the temperature is infinite and all weigh the same: -inf would
+    // stand in the first bin)
+    float scale = fmaxf(fminf(kSaBinsPerE / temperature, 1e30f), 1e-37f);
     if (by_count && (top - bottom) * scale > kSaBins - 2) scale = fmaxf((kSaBins - 2) / (top - bottom), scale / 32);
     s.row = {top, scale, 1.0f / (scale * temperature), (float)((double)top - 745.0 * (double)temperature), 1.0 / (double)temperature,
              kSaTable * 1.4426950408889634 / (double)temperature, sm.table};
@@ -714,7 +715,8 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_rows_kernel(const Sample
         cut.equals = count;
     }
     else {
-        if (least > 0.f) floor = __double2float_ru((double)top + (double)temperature * log(fmin((double)least, 1.0)));
+        // (at an infinite temperature every w is 1, the largest min-p)
+        if (least > 0.f && s.row.over_t > 0.0) floor = __double2float_ru((double)top + (double)temperature * log(fmin((double)least, 1.0)));
         if (by_count || by_mass) {
             // ---- 2  (the last bin, which may hold most of the row, is not counted but follows from the others)
             uint32_t count = 0;

@@ -341,8 +341,9 @@ typedef struct {
  * first among equals: top_k leaves the first top_k; top_p of those the ones in front of which stands a sum of w below top_p of the sum of the top_k;
  * min_p those with w >= min_p; the first always stays.  Among what is left, in the order of the indices, the first token whose running
  * sum of w exceeds uniform times the sum of all is drawn, and logprobs is ln of its share of that sum.
- * NaN counts as -inf; a row without a token above -inf gives -1 and -inf.  A temperature that is not above 0 gives the first token and 0; per
- * row, a top_k below 1, a top_p not below 1 and a min_p not above 0 leave all.  No scratch; the same answer whatever else runs.
+ * NaN counts as -inf; a row without a token above -inf gives -1 and -inf.  A temperature that is not above 0 gives the first token and 0, one
+ * that is infinite in fp32 makes every w_i 1; per row, a top_k below 1, a top_p not below 1 and a min_p not above 0 leave all.  No scratch; the
+ * same answer whatever else runs.
  * Stands beside: eet_argmax_rows.
  */
 int eet_sample_rows(const eet_sample_rows_args* args, void* stream);
