@@ -553,6 +553,9 @@ struct SaKernel {
                 if (cut.listed != kSaMissed) return cut;
                 goal = goal_of(s);
             }
+            else {
+                barrier();     // all have read the bracket that narrow() writes again
+            }
         }
         SaBracket br = narrow(sm.hist, total, by_mass, k, 0, goal, part, 0.0, 0.f, low, true);
         if (!by_mass && part > 0.f && br.before + br.count <= kSaList) {
