@@ -392,6 +392,15 @@ def _sample_setting(name, value, dtype, rows, index, low, high):
     return value.data_ptr(), 0
 
 
+def _sample_settings(rows, index, temperature, top_k, top_p, min_p):
+    """The settings of sample_rows for `rows` rows on cuda:index, checked: address and number of each."""
+    inf = float("inf")
+    return (*_sample_setting("temperature", temperature, torch.float32, rows, index, 0.0, inf),
+            *_sample_setting("top_k", top_k, torch.int32, rows, index, 0, 2 ** 31 - 1),
+            *_sample_setting("top_p", top_p, torch.float32, rows, index, 0.0, 1.0),
+            *_sample_setting("min_p", min_p, torch.float32, rows, index, 0.0, 1.0))
+
+
 def sample_rows(logits2d, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """Draws the next token of each row of a CUDA fp16, bf16 or fp32 matrix of logits (rows may be strided): returns (tokens int64
     [rows], logprobs float32 [rows]), logprobs being ln of the probability with which the token was drawn.
@@ -412,11 +421,7 @@ def sample_rows(logits2d, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
     if uniform.dtype != torch.float32 or uniform.get_device() != index or uniform.shape != (rows,) or not uniform.is_contiguous():
         raise RuntimeError(f"sample_rows: uniform must be a contiguous float32 tensor [{rows}] on cuda:{index}, got {tuple(uniform.shape)} "
                            f"{uniform.dtype} on {uniform.device}")
-    inf = float("inf")
-    t, temperature = _sample_setting("temperature", temperature, torch.float32, rows, index, 0.0, inf)
-    k, top_k = _sample_setting("top_k", top_k, torch.int32, rows, index, 0, 2 ** 31 - 1)
-    p, top_p = _sample_setting("top_p", top_p, torch.float32, rows, index, 0.0, 1.0)
-    m, min_p = _sample_setting("min_p", min_p, torch.float32, rows, index, 0.0, 1.0)
+    t, temperature, k, top_k, p, top_p, m, min_p = _sample_settings(rows, index, temperature, top_k, top_p, min_p)
     tokens = torch.empty(rows, dtype=torch.int64, device=logits2d.device)
     logprobs = torch.empty(rows, dtype=torch.float32, device=logits2d.device)
     args = _pack_sample(logits2d.data_ptr(), uniform.data_ptr(), t, p, m, k, tokens.data_ptr(), logprobs.data_ptr(), rows, n,

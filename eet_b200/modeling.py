@@ -568,6 +568,8 @@ class _CausalLMBase:
         if tp is not None and tp.size > 1:
             raise RuntimeError("generate: drawing tokens is not supported with tensor parallelism")
         B, dev = input_ids.shape[0], self.model.desc.device
+        # (what sample_rows would refuse is refused in front of the prompt)
+        EET._sample_settings(B, torch.empty(0, device=dev).get_device(), temperature, top_k, top_p, min_p)
         uniform = torch.rand((max(1, max_new_tokens), B), generator=generator, dtype=torch.float32, device=dev)
         # (a captured step reads its numbers from one place; settings of the caller's own stay where they are)
         self._sampling = dict(uniform=uniform[0].clone(), temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
@@ -581,22 +583,24 @@ class _CausalLMBase:
         self.end_graph()
         if attention_mask is not None and self.use_cuda_graph:
             self.model.pre_padding_len = torch.sum(1 - attention_mask, 1, True).to(self.model.desc.device).long()
-        # only the last position's logits are needed to choose the first new token: the lm_head runs on that
-        # row alone (the reference computes and discards the logits of every prompt position, modeling_llama.py:471)
-        hidden = self.model(input_ids=input_ids, first_pass=True, attention_mask=attention_mask)
-        nxt = self._choose(hidden[:, -1, :].contiguous()).clone()
-        toks = [input_ids, nxt]
-        for t in range(1, max_new_tokens):
-            if uniform is not None:
-                self._sampling["uniform"].copy_(uniform[t])
-            if attention_mask is not None and not self.use_cuda_graph:
-                hidden = self.model(input_ids=nxt, first_pass=False, attention_mask=attention_mask)
-                nxt = self._choose(hidden[:, -1, :]).clone()
-            else:
-                nxt = self.decode_step(nxt).clone()
-            toks.append(nxt)
-        if attention_mask is not None:
-            self.model.pre_padding_len = torch.empty(0).long()
+        try:
+            # only the last position's logits are needed to choose the first new token: the lm_head runs on that
+            # row alone (the reference computes and discards the logits of every prompt position, modeling_llama.py:471)
+            hidden = self.model(input_ids=input_ids, first_pass=True, attention_mask=attention_mask)
+            nxt = self._choose(hidden[:, -1, :].contiguous()).clone()
+            toks = [input_ids, nxt]
+            for t in range(1, max_new_tokens):
+                if uniform is not None:
+                    self._sampling["uniform"].copy_(uniform[t])
+                if attention_mask is not None and not self.use_cuda_graph:
+                    hidden = self.model(input_ids=nxt, first_pass=False, attention_mask=attention_mask)
+                    nxt = self._choose(hidden[:, -1, :]).clone()
+                else:
+                    nxt = self.decode_step(nxt).clone()
+                toks.append(nxt)
+        finally:
+            if attention_mask is not None:   # (the next call's prompts are others, also where this one was refused)
+                self.model.pre_padding_len = torch.empty(0).long()
         out = torch.cat(toks, dim=1)
         EET.check_device_status(self.model.desc.tp)   # a kernel that gave up on a wait must not go unnoticed
         return out
