@@ -38,6 +38,11 @@ namespace {
 
 constexpr int kPcExtra = 2;                     // a piece's beginning and end cost as much as two blocks
 
+// Scales of values below 2^-90 count as that where a reference is chosen.  The powers, of which the sum that divides is, then end at 2^(90 + 15),
+// and 2^22 of them are still a number in fp32; weights are good to 11 bits down to scales of 2^-104, to fewer below that (bf16 values of 10^-29).
+// With 2^-60 bf16 values below 10^-16 came out as zeros.
+constexpr float kPcLeastScale = 8.07793567e-28f;
+
 template<int D, int kRows>
 struct PcShape {
     static constexpr int kWarps = 4;
@@ -370,7 +375,7 @@ paged_mha_codes_kernel(const __grid_constant__ PagedMhaArgs a, void* ws, int few
                     }
                 }
                 // ---- weights
-                float vs[kM][2], top_scale = 8.67361738e-19f;   // (2^-60: a scale of zero weighs nothing)
+                float vs[kM][2], top_scale = kPcLeastScale;   // (a scale of zero weighs nothing)
 #pragma unroll
                 for (int m = 0; m < kM; ++m) {
 #pragma unroll
@@ -436,7 +441,7 @@ paged_mha_codes_kernel(const __grid_constant__ PagedMhaArgs a, void* ws, int few
                             float top = -INFINITY;
 #pragma unroll
                             for (int k = 0; k < 2 * kM; ++k) {
-                                top = fmaxf(top, s[k >> 1][n][2 * (k & 1) + r] + __log2f(fmaxf(vs[k >> 1][k & 1], 8.67361738e-19f)));
+                                top = fmaxf(top, s[k >> 1][n][2 * (k & 1) + r] + __log2f(fmaxf(vs[k >> 1][k & 1], kPcLeastScale)));
                             }
 #pragma unroll
                             for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
