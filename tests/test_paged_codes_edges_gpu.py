@@ -37,3 +37,36 @@ def test_mha_of_small_values(kind, new, heads, kv_heads, down):
     ref, tol = attend_codes64(batch, tiles=max(new) > 8)
     batch.v_scale *= 2.0 ** -down
     _within(_mha(batch, max_tokens=max(new)).double() * 2.0 ** down, ref, tol)
+
+
+@pytest.mark.parametrize("new,length,at", [(2, 300, 299), (3, 300, 299), (90, 300, 299), (2, 300, 7), (90, 300, 7), (1, 9000, 4321), (3, 9000, 8999),
+                                           (90, 9000, 4321), (90, 9000, 8999)])
+@pytest.mark.parametrize("kind,dtype", [(INT8, FP16), (E4M3, FP16), (INT8, BF16), (E4M3, BF16)])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_mha_a_scale_of_nan_reaches_all_rows_that_see_it(which, kind, dtype, new, length, at):
+    """That of a key as that of a value, every dim, also where a tile is cut and its parts are added up; the rows in front do not change."""
+    batch = CodesBatch([new], [length], 4, 2, 128, 16, dtype, kind)
+    clean = _mha(batch, max_tokens=new, max_len=length)
+    getattr(batch, which + "_scale")[batch.pages[0, at // 16].long(), :, at % 16] = math.nan
+    out = _mha(batch, max_tokens=new, max_len=length)
+    blind = max(0, at - (length - new))                       # rows in front of that position
+    assert torch.equal(out[:blind], clean[:blind]) and not torch.isnan(clean).any()
+    assert torch.isnan(out[blind:]).all()
+
+
+@pytest.mark.parametrize("kind", CODES)
+@pytest.mark.parametrize("heads,kv_heads,head_dim", [(8, 2, 64), (8, 8, 128)])
+@pytest.mark.parametrize("max_len", [3000, 100])
+def test_mha_rows_beside_a_chunk_are_as_good_as_alone(kind, heads, kv_heads, head_dim, max_len):
+    """bf16, sequences of few tokens beside a chunk.  Where they are many and long enough (by max_len) they go to the kernel of few rows, whose
+    weights are fp16: the tolerance is that of a call of their own.  Otherwise they go to the chunk's tiles, and so is the tolerance."""
+    new, lens = [1] * 20 + [150] + [2] + [1] * 10, [100 + 41 * i for i in range(20)] + [700, 900] + [1 + 300 * i for i in range(10)]
+    batch = CodesBatch(new, lens, heads, kv_heads, head_dim, 32, BF16, kind)
+    batch.poison()
+    got = _mha(batch, max_tokens=150, max_len=max_len)
+    assert ((len(new) - 1) * kv_heads * (max_len // 128 + 1) >= 1024) == (max_len == 3000)
+    ref, tight = attend_codes64(batch)
+    wide = attend_codes64(batch, tiles=True)[1]
+    tol = tight.clone() if max_len == 3000 else wide
+    tol[20:170] = wide[20:170]
+    _within(got, ref, tol)
