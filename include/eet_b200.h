@@ -478,9 +478,12 @@ typedef struct {
 
 size_t eet_paged_mha_codes_workspace_bytes(const eet_paged_mha_codes_args* args);
 
-/* eet_paged_mha over a cache of 8-bit codes.  The codes enter the products exactly; the weights p_j s^v_j are rounded, to fp16 where a kv head
- * has up to 16 rows (new tokens x query heads) of a sequence, else to the type of q.  A row of the cache whose scale is NaN reaches the rows
- * that see it, and no others. */
+/* eet_paged_mha over a cache of 8-bit codes.  The codes enter the products exactly; the weights p_j s^v_j are rounded, by the kernel
+ * of few rows to fp16, by the tiles of 128 rows to the type of q, and the sum that divides is of the powers p_j as they are in fp32.  All of a call
+ * goes to the kernel of few rows where max_tokens x (heads / kv_heads) is at most 16; beside longer chunks the sequences of few tokens do (as many
+ * as make 8 rows where they have that few on average, else 16) where they are many and long enough by max_len, else they go to the tiles.
+ * Scales of values far below others count with fewer bits: by the kernel of few rows below 2^-111, by the tiles in fp16 below 2^-20 of the
+ * largest that a tile reads.  A row of the cache whose scale is NaN reaches the rows that see it, and no others. */
 int eet_paged_mha_codes(const eet_paged_mha_codes_args* args, void* stream);
 
 #ifdef __cplusplus
