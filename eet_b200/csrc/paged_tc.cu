@@ -605,20 +605,16 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
             constexpr bool kUnit = kCodes != 0 && std::is_same<T, __half>::value;
             constexpr int kLeastUnit = -110;   // 2^15 over it is still a number
             int unit = kLeastUnit - 1;         // (none yet)
+            // A wait for scales by parity is only good less than a turn of their ring ahead of the copies.  Tile b, which has no turn in a split
+            // piece of one block, comes from any number of those to its next first block: the parity would be that of the turn before, and the
+            // wait would end before the scales are there.  So the scores of a piece's first block are waited for in front of its scales: the
+            // copies of those were asked for in front of their keys'.
+            if (kCodes && turns.any()) ok = tc_wait_warp(&sm.s_full[x], (uint32_t)(used & 1), &sm.abort);
             for (int j = turns.first; j < turns.end && ok; j += turns.stride) {
                 const int key0 = (top - j) * kPgKeys;
                 const float *k_scales = nullptr, *v_scales = nullptr;
                 float less = 1.0f;             // a power of two: of O under the unit before
-                const bool first = j == turns.first;
                 if (kCodes) {
-                    // A wait for the scales by parity is only good less than a turn of their ring ahead of the copies.  Tile b, which has no
-                    // turn in a split piece of one block, comes from any number of those to its next first block: the parity would be that
-                    // of the turn before, and its wait would end before the scales are there.  So the scores come first, once a piece: the
-                    // copies of their scales were asked for in front of their keys'.
-                    if (first && !tc_wait_warp(&sm.s_full[x], (uint32_t)(used & 1), &sm.abort)) {
-                        ok = false;
-                        break;
-                    }
                     const int block = entry0 / 2 + j, slot = block % PgCodesLoader<D>::kScales;
                     const uint8_t* ring_end = ring + kRing * kTile + PgCodesLoader<D>::kPlaces * PgCodesLoader<D>::kPlace;
                     k_scales = reinterpret_cast<const float*>(ring_end) + slot * 2 * kPgKeys;
@@ -725,6 +721,7 @@ __device__ __forceinline__ void pg_tiles(const CUtensorMap* map_q, const CUtenso
                 }
                 m_run = fmaxf(m_run, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
                 float corr = 1.0f;
+                const bool first = j == turns.first;
                 const bool moves = fmaf(m_run, ref.factor, ref.off) > kPgLag + PgType<T>::kUp;
                 if (moves) {
                     const float old = ref.log2_of(to_log2);

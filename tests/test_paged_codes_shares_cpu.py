@@ -88,11 +88,11 @@ def test_the_warps_of_tile_b_come_to_their_first_block_from_far_ahead():
     for new, lens, heads, kv_heads in loads:
         assert any(max(_passed_by_b(new, lens, heads, kv_heads, whole)) >= ring for whole in (False, True))
     assert max(_passed_by_b([512], [8704], 32, 8, False)) < ring      # (a chunk's pieces are long)
-    # The loop over a piece's blocks: s_full, under `first`, is waited for in front of scales_full and of the first look at a scale.
-    softmax = tiles[tiles.index("pg_reference<T>(m_run") - 20000:]
-    loop = _body(softmax[softmax.index("PgReference ref = {1.0f, -kPgNone};"):], "for (int j = turns.first;")
-    assert re.search(r"const bool first = j == turns\.first;", loop)
-    guard = re.search(r"if \(first && !tc_wait_warp\(&sm\.s_full\[x\], \(uint32_t\)\(used & 1\), &sm\.abort\)\) \{\s*ok = false;\s*break;\s*\}", loop)
+    # s_full of a piece's first block is waited for in front of the loop over its blocks, which looks at the scales.
+    softmax = tiles[tiles.index("PgReference ref = {1.0f, -kPgNone};"):]
+    loop = _body(softmax, "for (int j = turns.first;")
+    front = softmax[:softmax.index(loop)]
+    guard = re.search(r"if \(kCodes && turns\.any\(\)\) ok = tc_wait_warp\(&sm\.s_full\[x\], \(uint32_t\)\(used & 1\), &sm\.abort\);\s*"
+                      r"for \(int j = turns\.first; j < turns\.end && ok; j \+= turns\.stride\) $", front)
     assert guard, "the scores of the first block"
-    assert guard.end() < loop.index("sm.scales_full[slot]") < loop.index("v_scales)[lane]")
-    assert "v_scales" not in loop[:guard.start()].replace("*v_scales = nullptr", "")
+    assert "scales_full" in loop and "scales" not in front
