@@ -629,10 +629,11 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_rows_kernel(const Sample
     const int loads = n > 0 ? (skew + n + kPer - 1) / kPer : 0;
     float temperature = a.temperatures != nullptr ? a.temperatures[r] : a.temperature;
     const float part = a.top_ps != nullptr ? a.top_ps[r] : a.top_p;
-    const float least = a.min_ps != nullptr ? a.min_ps[r] : a.min_p;
+    float least = a.min_ps != nullptr ? a.min_ps[r] : a.min_p;
     const int wanted = a.top_ks != nullptr ? a.top_ks[r] : a.top_k;
     const bool greedy = !(temperature > 0.f);
     if (greedy) temperature = 1.0f;
+    if (temperature == INFINITY) least = 0.f;   // every w is 1, the largest min-p
     const bool by_count = wanted > 0 && wanted < a.vocab, by_mass = part < 1.0f;
     float top = -INFINITY, bottom = INFINITY;   // of the finite and infinite values above -inf
     {
@@ -719,8 +720,7 @@ __global__ void __launch_bounds__(kSaThreads, 2) sample_rows_kernel(const Sample
         cut.equals = count;
     }
     else {
-        // (at an infinite temperature every w is 1, the largest min-p)
-        if (least > 0.f && s.row.over_t > 0.0) floor = __double2float_ru((double)top + (double)temperature * log(fmin((double)least, 1.0)));
+        if (least > 0.f) floor = __double2float_ru((double)top + (double)temperature * log(fmin((double)least, 1.0)));
         if (by_count || by_mass) {
             // ---- 2  (the last bin, which may hold most of the row, is not counted but follows from the others)
             uint32_t count = 0;
