@@ -4,9 +4,10 @@
 //   out = sum_j w_j c^v_j / sum_j w_j / s^v_j,   w_j = s^v_j 2^(s^k_j (q . c^k_j) scale log2(e) + slope (j - p) log2(e) - ref)
 //
 // The codes enter the products as fp16, where they are exact, and the scales stay outside: that of a key on its score, that of its
-// value on its weight, before that is rounded to fp16 (the sum that divides is of the powers, which are not).  So that the weights fit fp16 whatever the scales are, the reference ref of a row
-// follows the largest score + log2(s^v), not the largest score.  q of bf16 is multiplied by a power of two that brings its largest
-// value to 2^14 and enters as fp16 too: eight bits of every value down to 2^-28 of the largest are kept.
+// value on its weight, before that is rounded to fp16 (the sum that divides is of the powers, which are not).  So that the weights fit
+// fp16 whatever the scales are, the reference ref of a row follows the largest score + log2(s^v), not the largest score.  q of bf16 is
+// multiplied by a power of two that brings its largest value to 2^14 and enters as fp16 too: eight bits of every value down to 2^-28 of
+// the largest are kept.
 //
 // Bound: HBM, the codes and scales of every sequence once.  A block of 128 keys is half the bytes of a 16-bit one, and everything on
 // the way has to keep up: pages of 16 slots are eight copies of 2 KiB a block, which the copy engine takes 85 cycles each for, so the
@@ -21,11 +22,11 @@
 //
 // A CTA is four warps, 32 keys of a block each; three CTAs share an SM, two where there are 16 rows, so that the beginning and the end of a
 // piece of one run beside the others' blocks.  The warps' sums meet in shared memory at the end of a piece.  The work is cut up as
-// paged_share.cuh says.  Measured: 64 sequences of 200 to 8000 tokens, 32 / 8 heads, bf16 over int8, 65 us (75 with two CTAs), which is 4.1 TB/s;
-// two of 60 and 100 thousand tokens, 64 / 8 heads, fp16 over e4m3, 70 us (4.6 TB/s).  What bounds it then is how fast three warps a scheduler go through
-// their instructions: one in six cycles each (issue slots 46 % taken, 41 in the second case).  Of the six, 1.2 are fixed latencies, 1.1 instructions that
-// are not there yet, 0.6 another warp's turn, 0.6 shared memory, 0.5 the pipe of conversions' and bytes' selections, the fullest one at 40 %, and 0.4 the
-// copies (1.2 in the second case).
+// paged_share.cuh says.  Measured: 64 sequences of 200 to 8000 tokens, 32 / 8 heads, bf16 over int8, 66 us (75 with two CTAs), which is 4.1 TB/s;
+// two of 60 and 100 thousand tokens, 64 / 8 heads, fp16 over e4m3, 71 us (4.6 TB/s).  What bounds it then is how fast three warps a scheduler
+// go through their instructions: one in six cycles each (issue slots 46 % taken, 41 in the second case).  Of the six, 1.2 are fixed
+// latencies, 1.1 instructions that are not there yet, 0.6 another warp's turn, 0.6 shared memory, 0.5 the pipe of conversions' and bytes'
+// selections, the fullest one at 40 %, and 0.4 the copies (1.2 in the second case).
 //
 // Longer chunks go to tiles of 128 rows (paged_tc.cu has what a CTA does), in a kernel of their own behind the same plan.  Where a call has both kinds of
 // sequences, the kernels run side by side on parts of the SMs, divided by what a block takes on either, and one launch adds up the parts of both.

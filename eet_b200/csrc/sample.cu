@@ -20,9 +20,9 @@
 //
 // A row is worked on by a cluster of 1 to 8 CTAs, which hold it in shared memory and exchange counts and candidates there.  Bound: latency,
 // six barriers of the cluster and four trips through a slice of the row; with many rows the issue of instructions, the powers of all
-// tokens first (11 instructions in 64 bits each, with a table of 128; exp() took three times as long): 58 % of the slots taken, the pipe of whole numbers 46 % full, that
-// of 64 bits 12 %.  Measured: one row of 32000 fp32 logits 18 us, 64 rows of 64000 fp16 44, 256 of 64000 bf16 146 (22, 119 and 287 with
-// exp() and lists gathered by atomics on one counter).
+// tokens first (11 instructions in 64 bits each, with a table of 128; exp() took three times as long): 58 % of the slots taken, the pipe
+// of whole numbers 46 % full, that of 64 bits 12 %.  Measured: one row of 32000 fp32 logits 18 us, 64 rows of 64000 fp16 41, 256 of 64000
+// bf16 139 (22, 119 and 287 with exp() and lists gathered by atomics on one counter).
 #include <cooperative_groups.h>
 
 #include "common.cuh"
